@@ -30,6 +30,7 @@ FAMILY_LAST_TOKEN = 4
 
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
+DTYPE_U4 = 2
 
 KERNEL_CLASSES = 15
 
@@ -41,6 +42,34 @@ class ModelSpecStruct(ctypes.Structure):
                 ("hidden", ctypes.c_int32), ("weight_dtype", ctypes.c_int32),
                 ("kv_dtype", ctypes.c_int32), ("max_rows", ctypes.c_int32),
                 ("reserved", ctypes.c_int32 * 6)]
+
+
+class SequencesStruct(ctypes.Structure):
+    _fields_ = [("count", ctypes.c_int32), ("tokens", ctypes.c_int32),
+                ("rows", ctypes.c_void_p), ("starts", ctypes.c_void_p),
+                ("lengths", ctypes.c_void_p)]
+
+
+class KvCacheStruct(ctypes.Structure):
+    _fields_ = [("storage", ctypes.c_int32), ("rows", ctypes.c_int32),
+                ("kv_heads", ctypes.c_int32), ("slots", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("reserved", ctypes.c_int32 * 3),
+                ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p)]
+
+
+class AttentionSpecStruct(ctypes.Structure):
+    _fields_ = [("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("window", ctypes.c_int32), ("sinks", ctypes.c_int32),
+                ("scale", ctypes.c_float), ("reserved", ctypes.c_int32)]
+
+
+class SamplingStruct(ctypes.Structure):
+    _fields_ = [("temperature", ctypes.c_float), ("top_p", ctypes.c_float),
+                ("min_p", ctypes.c_float), ("top_k", ctypes.c_int32),
+                ("temperatures", ctypes.c_void_p), ("top_ps", ctypes.c_void_p),
+                ("min_ps", ctypes.c_void_p), ("top_ks", ctypes.c_void_p)]
 
 
 TOKEN_SINK = ctypes.CFUNCTYPE(ctypes.c_int32, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32,
@@ -124,6 +153,30 @@ SIGNATURES = {
     "bst_execute_queue": (ctypes.c_int32, [_u64, ctypes.c_void_p, ctypes.c_int32]),
     "bst_context_stats": (ctypes.c_int32, [_u64, _i64p]),
     "bst_context_clear_graph": (ctypes.c_int32, [_u64]),
+    "bst_kv_append": (ctypes.c_int32, [ctypes.c_int32, ctypes.c_void_p, _P(KvCacheStruct),
+                                       _P(SequencesStruct), ctypes.c_void_p, ctypes.c_int64,
+                                       ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32]),
+    "bst_kv_read": (ctypes.c_int32, [ctypes.c_int32, ctypes.c_void_p, _P(KvCacheStruct),
+                                     _P(SequencesStruct), ctypes.c_void_p, ctypes.c_int64,
+                                     ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32]),
+    "bst_attention_cached_workspace": (ctypes.c_int32, [_P(KvCacheStruct), _P(SequencesStruct),
+                                                        _P(AttentionSpecStruct), _i64p]),
+    "bst_attention_cached": (ctypes.c_int32, [ctypes.c_int32, ctypes.c_void_p, _P(KvCacheStruct),
+                                              _P(SequencesStruct), _P(AttentionSpecStruct),
+                                              ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
+                                              ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64]),
+    "bst_attention_packed_workspace": (ctypes.c_int32, [_P(SequencesStruct),
+                                                        _P(AttentionSpecStruct), _i64p]),
+    "bst_attention_packed": (ctypes.c_int32, [ctypes.c_int32, ctypes.c_void_p,
+                                              _P(SequencesStruct), _P(AttentionSpecStruct),
+                                              ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
+                                              ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64,
+                                              ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
+                                              ctypes.c_int64]),
+    "bst_sample_tokens": (ctypes.c_int32, [ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p,
+                                           ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
+                                           ctypes.c_int64, _P(SamplingStruct), ctypes.c_void_p,
+                                           ctypes.c_void_p]),
     "bst_last_error": (ctypes.c_int32, [_u64, ctypes.c_char_p, ctypes.c_int32]),
     "bst_write_synthetic_weights": (ctypes.c_int32, [_P(ModelSpecStruct), ctypes.c_char_p,
                                                      ctypes.c_int64, ctypes.c_double]),

@@ -50,6 +50,7 @@ extern "C" {
 
 #define BST_DTYPE_F32 0
 #define BST_DTYPE_BF16 1
+#define BST_DTYPE_U4 2 /* caches only: 4-bit codes, a bf16 step and low per 32 channels */
 
 typedef uint64_t bst_engine;
 
@@ -252,6 +253,119 @@ int32_t bst_execute_queue(bst_context context, const void* commands, int32_t cou
  * out[3] kernels launched. */
 int32_t bst_context_stats(bst_context context, int64_t out[4]);
 int32_t bst_context_clear_graph(bst_context context);
+
+/* ---- Serving operators on caller-owned device buffers ----
+ * The parts of a decode step that a host program schedules itself: a cache of keys and values (in
+ * 4 bits, bf16 or float32), attention over it, attention over packed prompts, and drawing tokens.
+ * No counterpart in the reference. All pointers inside the structs and arguments are device
+ * pointers on `device`; the structs themselves are host memory, read before the call returns.
+ *
+ * Every call queues its kernels on `stream` (a cudaStream_t; NULL is the legacy default stream) and
+ * returns without waiting for them: it allocates nothing, never synchronises, leaves the calling
+ * thread's current device as it was, and may be captured into a CUDA graph (call it once on the
+ * device before the first capture: that loads its kernels). Calls may run at the same time on
+ * several streams as long as they do not share a workspace or write the same memory. Errors are
+ * found from the host's arguments alone, before anything is queued; bst_last_error(0) has the
+ * message.
+ *
+ * A batch is a list of sequences. Sequence s owns cache row rows[s] (distinct rows; s itself when
+ * rows is NULL) and the packed tokens [starts[s], starts[s + 1]) of this call (token s alone when
+ * starts is NULL, and then tokens == count). lengths[s] counts the row's cached tokens with this
+ * call's tokens included: with n tokens, token i of the sequence has position (and cache slot)
+ * lengths[s] - n + i. starts must not decrease. The arrays are read on the device: tokens that no
+ * sequence owns are left alone (their outputs stay as they were), and tokens whose row or slot lies
+ * outside the cache are not stored, see no keys and read as zeros. */
+typedef struct bst_sequences {
+    int32_t count;
+    int32_t tokens;         /* packed tokens: the first dimension of k, v, q and out */
+    const int32_t* rows;    /* [count] or NULL */
+    const int32_t* starts;  /* [count + 1] or NULL */
+    const int32_t* lengths; /* [count] */
+} bst_sequences;
+
+/* k and v are [rows][kv_heads][slots][head_dim], head_dim 32, 64 or 128, 16-byte aligned. With
+ * BST_DTYPE_U4 a head's channels of one token take head_dim / 2 bytes and k_scale and v_scale are
+ * [rows][kv_heads][slots][head_dim / 32][2] bf16: (step, low) of every 32 channels. A code c stands
+ * for low + c * step. low is the 32 channels' minimum rounded down to bf16, step is
+ * (maximum - low) / 15 rounded up to bf16, and codes are (x - low) / step rounded to nearest even;
+ * 32 channels that hold a NaN, an infinity or a value below bf16's lowest read back as NaN. The codes of a token's head are [8][head_dim / 32][4] nibbles, low nibble first: channel
+ * 32 g + 4 h + j is nibble j of the 16 bits at [h][g]. */
+typedef struct bst_kv_cache {
+    int32_t storage; /* BST_DTYPE_F32, BST_DTYPE_BF16 or BST_DTYPE_U4 */
+    int32_t rows, kv_heads, slots, head_dim;
+    int32_t reserved[3]; /* must be zero */
+    void *k, *v;
+    void *k_scale, *v_scale; /* BST_DTYPE_U4 only */
+} bst_kv_cache;
+
+/* Stores the batch's keys and values in their slots. k and v: [tokens][kv_heads][head_dim] of
+ * `dtype`, tokens k_stride and v_stride elements apart (their heads contiguous). */
+int32_t bst_kv_append(int32_t device, void* stream, const bst_kv_cache* cache,
+                      const bst_sequences* sequences, const void* k, int64_t k_stride,
+                      const void* v, int64_t v_stride, int32_t dtype);
+/* The values that the batch's slots stand for, in the same layout. */
+int32_t bst_kv_read(int32_t device, void* stream, const bst_kv_cache* cache,
+                    const bst_sequences* sequences, void* k, int64_t k_stride, void* v,
+                    int64_t v_stride, int32_t dtype);
+
+/* heads must be a multiple of kv_heads: query head h reads key head h * kv_heads / heads. A query
+ * at position i sees key j when j <= i and (window == 0, or i - j < window, or j < sinks): the
+ * last `window` tokens and the first `sinks`. A query that sees nothing gives zeros. dtype is the
+ * type of q and out (and of packed k and v); scores, weights and sums are float32. */
+typedef struct bst_attention_spec {
+    int32_t heads, kv_heads, head_dim, dtype;
+    int32_t window, sinks;
+    float scale; /* of the scores, e.g. 1 / sqrt(head_dim) */
+    int32_t reserved; /* must be zero */
+} bst_attention_spec;
+
+/* out[t] = attention of the batch's queries over their rows of the cache, this call's own tokens
+ * included (append them first). q and out: [tokens][heads][head_dim], tokens q_stride and
+ * out_stride elements apart. A cache of float32 or bf16 takes one token per sequence (starts
+ * NULL); a 4-bit cache takes any number. workspace: at least the bytes that
+ * bst_attention_cached_workspace gives for the same arguments (16-byte aligned, may be NULL when
+ * that is 0), not shared with calls that run at the same time. */
+int32_t bst_attention_cached_workspace(const bst_kv_cache* cache, const bst_sequences* sequences,
+                                       const bst_attention_spec* spec, int64_t* bytes);
+int32_t bst_attention_cached(int32_t device, void* stream, const bst_kv_cache* cache,
+                             const bst_sequences* sequences, const bst_attention_spec* spec,
+                             const void* q, int64_t q_stride, void* out, int64_t out_stride,
+                             void* workspace, int64_t workspace_bytes);
+
+/* Causal attention of packed sequences over their own keys and values (prompts that need no cache
+ * yet): sequences->starts is required, rows and lengths must be NULL, positions count from 0.
+ * q and out [tokens][heads][head_dim], k and v [tokens][kv_heads][head_dim]. */
+int32_t bst_attention_packed_workspace(const bst_sequences* sequences,
+                                       const bst_attention_spec* spec, int64_t* bytes);
+int32_t bst_attention_packed(int32_t device, void* stream, const bst_sequences* sequences,
+                             const bst_attention_spec* spec, const void* q, int64_t q_stride,
+                             const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                             void* out, int64_t out_stride, void* workspace,
+                             int64_t workspace_bytes);
+
+/* How tokens are drawn; a per-row array, where given, replaces the scalar. In order:
+ *   temperature  weights w = exp((logit - largest logit) / temperature); at 0, below, or NaN the
+ *                row takes the first of its largest logits instead.
+ *                Weights below 2^-40 are never drawn.
+ *   top_k        keeps the k largest (<= 0: all), ties lowest index first.
+ *   top_p        keeps the fewest of the largest whose weights reach top_p of what is left (at
+ *                least one; >= 1 or NaN: all), ties lowest index first.
+ *   min_p        keeps weights of at least min_p times the largest (<= 0 or NaN: all).
+ * The token is the first, by index, at which the running sum of the kept weights exceeds
+ * uniform * their sum. NaN logits count as -infinity; rows with no logit above it give -1. */
+typedef struct bst_sampling {
+    float temperature, top_p, min_p;
+    int32_t top_k;
+    const float *temperatures, *top_ps, *min_ps; /* [rows] or NULL */
+    const int32_t* top_ks;                       /* [rows] or NULL */
+} bst_sampling;
+
+/* tokens[r] drawn from logits [rows][vocabulary] (`dtype`, rows row_stride elements apart) with
+ * uniforms[r] in [0, 1) (values outside are clamped). vocabulary <= 2^20. The draw is decided in
+ * 64-bit integers, so it does not depend on how rows are scheduled. */
+int32_t bst_sample_tokens(int32_t device, void* stream, const void* logits, int32_t dtype,
+                          int32_t rows, int32_t vocabulary, int64_t row_stride,
+                          const bst_sampling* sampling, const double* uniforms, int32_t* tokens);
 
 /* Message of the last failure on this engine (engine 0: on this thread). */
 int32_t bst_last_error(bst_engine engine, char* buffer, int32_t capacity);
