@@ -21,9 +21,9 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-I", str(INCLUDE),
           "-I", str(CSRC)]
 SOURCES = ["kernels.cu", "gemm_tc.cu", "decode_fused.cu", "ops.cu", "ops_static.cu", "tensors.cu",
-           "kv_cache.cu", "attention.cu", "sample.cu", "operators.cpp", "engine.cpp"]
+           "kv_cache.cu", "attention_cached.cu", "attention_packed.cu", "sample.cu", "operators.cpp", "engine.cpp"]
 HEADERS = ["kernels.h", "java_random.h", "epilogue.cuh", "device.cuh", "select.cuh",
-           "operators.h"]
+           "operators.h", "attention.cuh"]
 
 
 def nvcc() -> str:

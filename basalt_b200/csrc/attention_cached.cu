@@ -1,0 +1,746 @@
+// Attention of one or a few new tokens per sequence over a cache, split over the keys.
+//
+// Bound by memory: every visible key and value is read once (0.625 bytes a value in 4 bits) and
+// takes two multiply-adds per query head. With the 4-bit codes the reading is so short that the
+// arithmetic has to stay below four lane operations a value, which rules out scaling each value;
+// so the codes go to the tensor cores as they are and the scales are applied around the products:
+//
+//   s_ij    = sum_g step_jg (q_ig . c_jg) + low_jg sum(q_ig)         g: groups of 32 channels
+//   out_icg = sum_j (p_ij step_jg) c_jgc + sum_j p_ij low_jg
+//
+// A nibble becomes a bf16 number without a conversion: 0x4300 | c is 128 + c. bf16 queries keep
+// the 128 and take it out through low - 128 step, float32 ones subtract it (it would cost them four
+// bits). mma.sync m16n8k16 reads its B operand from registers, which is where unpacked codes are;
+// tcgen05 would need them written to shared memory at four times their size first, and a tile
+// of at most eight query rows would leave 120 of its 128 rows empty.
+//
+// The sixteen rows of the A operand hold eight queries (tokens x heads of one key head) twice: rows
+// 0-7 the leading bf16 part of the weights p step (and of float32 q), rows 8-15 what that rounding
+// left, so one product carries 16 bits; float32 adds a second product for the next eight. Weights,
+// sums and the running maximum are float32.
+//
+// A warp works on 16 keys at a time and alone: it copies its keys into its own ring in shared memory
+// with cp.async (keys that nobody sees are filled with zeros there, whatever their slots hold), and
+// warps meet only at the end. Lane (g, t) = (lane / 4, lane % 4) owns query row g, and its
+// fragments' key columns 2 t and 2 t + 1 of either half of the 16. Splits leave their maximum, sum
+// and output in the workspace and a second kernel joins them.
+
+#include <cuda_bf16.h>
+
+#include <algorithm>
+
+#include "attention.cuh"
+#include "device.cuh"
+#include "operators.h"
+
+namespace bst {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kBlock = 16;   // keys a warp takes at a time
+constexpr int kRows = 8;     // query rows of a tile
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <int STORAGE, int HD>
+struct Layout {
+    static constexpr int kGroups = HD / 32;
+    static constexpr bool kCodes = STORAGE == BST_DTYPE_U4;
+    static constexpr int kRowBytes = kCodes ? HD / 2 : (STORAGE == BST_DTYPE_F32 ? 4 : 2) * HD;
+    static constexpr int kChunks = kRowBytes / 16;
+    static constexpr int kScaleBytes = kCodes ? kBlock * kGroups * 4 : 0;
+    static constexpr int kStage = 2 * (kBlock * kRowBytes + kScaleBytes);
+    // Enough in flight to cover the memory's latency from every SM: 20 to 130 KB a CTA.
+    static constexpr int kStages = kStage <= 2560 ? 4 : (kStage <= 8192 ? 3 : 2);
+    static constexpr int kRing = kWarps * kStages * kStage;
+    static constexpr int kMerge = kWarps * kRows * (HD + 2) * 4;
+    static constexpr int kSmem = kRing > kMerge ? kRing : kMerge;
+};
+
+// Where 16-byte chunk `chunk` of key row `row` of a block lies in its row in shared memory, so that
+// the reads below meet no bank twice.
+template <int STORAGE, int HD>
+__device__ __forceinline__ int swizzled(int row, int chunk) {
+    if constexpr (STORAGE == BST_DTYPE_U4) {
+        return HD == 128 ? chunk ^ (row & 2) : chunk;
+    } else if constexpr (STORAGE == BST_DTYPE_BF16) {
+        return HD == 32 ? chunk ^ ((row >> 1) & 3) : chunk ^ (((row & 1) << 2) | ((row >> 1) & 3));
+    } else {
+        return chunk ^ (row & 7);
+    }
+}
+
+// The key row (0..7) behind column n of a fragment's eight key columns. For 4-bit rows, which are
+// shorter than the banks, an order in which neither the key nor the value reads collide.
+template <int STORAGE, int HD>
+__device__ __forceinline__ int row_of_column(int n) {
+    if constexpr (STORAGE == BST_DTYPE_U4) {
+        const int t = n >> 1;
+        return (n & 1) ? 4 + (t ^ (HD == 128 ? 1 : 2)) : t;
+    } else {
+        return n;
+    }
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+                 : "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src, int bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N),
+                 "r"(bytes)
+                 : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {  // lo in the low half
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float low_of(uint32_t p) { return __uint_as_float(p << 16); }
+__device__ __forceinline__ float high_of(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
+
+// (a, b) as bf16 pairs whose sum is (a, b) to 8 bits a term.
+template <int TERMS>
+__device__ __forceinline__ void terms_of(float a, float b, uint32_t* out) {
+    out[0] = pack2(a, b);
+#pragma unroll
+    for (int i = 1; i < TERMS; ++i) {
+        a -= low_of(out[i - 1]);
+        b -= high_of(out[i - 1]);
+        out[i] = pack2(a, b);
+    }
+}
+
+// Nibble i of both halves of x as bf16 numbers: c or, with OFFSET, 128 + c.
+template <bool OFFSET>
+__device__ __forceinline__ uint32_t nibbles(uint32_t x, int i) {
+    const uint32_t v = ((x >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+    if constexpr (OFFSET) return v;
+    uint32_t r;
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(0x43004300u));
+    return r;
+}
+
+template <int G>
+__device__ __forceinline__ void load_words(uint32_t addr, uint32_t (&w)[G]) {
+    if constexpr (G == 1) {
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(addr));
+    } else if constexpr (G == 2) {
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
+    } else {
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr));
+    }
+}
+
+// The keys that a tile of queries at positions p0..p1 sees: blocks of 16 that hold the sinks before
+// the window, then blocks from the window's first key (rounded down) to the last key.
+struct Visible {
+    int64_t first, end;   // the window
+    int64_t aligned;      // first, rounded down to a block
+    int sinks;            // keys below it are visible too
+    int sink_blocks, blocks;
+    __device__ Visible(int64_t p0, int64_t p1, int slots, int window, int sinks_) {
+        end = min(p1 + 1, static_cast<int64_t>(slots));
+        first = window ? max(static_cast<int64_t>(0), p0 - window + 1) : 0;
+        aligned = first & ~static_cast<int64_t>(kBlock - 1);
+        sinks = sinks_;
+        blocks = sink_blocks = 0;
+        if (end > 0 && first < end) {
+            sink_blocks = static_cast<int>((min(static_cast<int64_t>(sinks), aligned) + kBlock - 1) / kBlock);
+            blocks = sink_blocks + static_cast<int>((end - aligned + kBlock - 1) / kBlock);
+        }
+    }
+    __device__ int64_t key(int block) const {
+        return block < sink_blocks ? static_cast<int64_t>(block) * kBlock
+                                   : aligned + static_cast<int64_t>(block - sink_blocks) * kBlock;
+    }
+    __device__ bool holds(int64_t key) const { return key < end && (key >= first || key < sinks); }
+};
+
+// Splits that a tile of this many blocks is worth: at least 8 blocks a split, two a warp.
+__host__ __device__ __forceinline__ int useful_splits(int blocks, int splits) {
+    const int most = blocks / 8;
+    return most < 1 ? 1 : (most < splits ? most : splits);
+}
+
+// One tile of eight query rows of one key head.
+struct Tile {
+    int seq, first, n;   // the sequence, its first packed token and its tokens
+    int r0;              // the tile's first query row: row r is token r / group, head r % group
+};
+
+// Tile number `index` of a batch whose sequences have n group rows each, eight to a tile. Without
+// starts every sequence has the same number of tiles; with them the tiles before each sequence are
+// summed, 32 sequences at a time.
+__device__ __forceinline__ bool find_tile(const Batch& b, int group, int index, Tile* t) {
+    if (!b.starts) {
+        const int per = (group + kRows - 1) / kRows;
+        t->seq = index / per;
+        t->first = t->seq;
+        t->n = 1;
+        t->r0 = (index - t->seq * per) * kRows;
+        return t->seq < b.count;
+    }
+    const int lane = threadIdx.x & 31;
+    int before = 0;
+    for (int s0 = 0; s0 < b.count; s0 += 32) {
+        const int s = s0 + lane;
+        int from = 0, n = 0;
+        if (s < b.count) {
+            from = __ldg(b.starts + s);
+            n = max(0, min(__ldg(b.starts + s + 1), b.tokens) - from);
+        }
+        const int tiles = (n * group + kRows - 1) / kRows;
+        int run = tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(kFull, run, o);
+            if (lane >= o) run += v;
+        }
+        const unsigned hit = __ballot_sync(kFull, before + run > index);
+        if (hit) {
+            const int who = __ffs(hit) - 1;
+            t->seq = s0 + who;
+            t->first = __shfl_sync(kFull, from, who);
+            t->n = __shfl_sync(kFull, n, who);
+            t->r0 = (index - before - __shfl_sync(kFull, run - tiles, who)) * kRows;
+            return true;
+        }
+        before += __shfl_sync(kFull, run, 31);
+    }
+    return false;
+}
+
+template <typename T, int STORAGE, int HD>
+__global__ void __launch_bounds__(kThreads)
+k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride,
+         T* __restrict__ out, int64_t out_stride, int splits, float* __restrict__ part) {
+    using L = Layout<STORAGE, HD>;
+    constexpr int G = L::kGroups;
+    constexpr bool kExact = sizeof(T) == 4;      // float32: 24-bit operands
+    constexpr int kTerms = kExact ? 3 : 2;       // of the weights
+    constexpr int kQ = kExact ? 3 : 1;           // of the queries (a bf16 query is one)
+    constexpr int kK = STORAGE == BST_DTYPE_F32 ? (kExact ? 3 : 2) : 1;  // of keys and values
+    constexpr int kMma = HD / 16;
+    extern __shared__ __align__(16) unsigned char smem[];
+
+    const int group = a.heads / a.kv_heads;
+    const int kvh = blockIdx.y;
+    const int split = blockIdx.z;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    Tile tile;
+    if (!find_tile(b, group, blockIdx.x, &tile)) return;
+    const int row = b.rows ? __ldg(b.rows + tile.seq) : tile.seq;
+    const int64_t length = __ldg(b.lengths + tile.seq);
+    const int rows = min(kRows, tile.n * group - tile.r0);
+    // Positions of the tile's tokens; a row or slot outside the cache sees nothing.
+    const bool inside = row >= 0 && row < c.rows;
+    const int64_t p_first = length - tile.n + tile.r0 / group;
+    const int64_t p_last = length - tile.n + (tile.r0 + rows - 1) / group;
+    const Visible seen(p_first, inside ? p_last : -1, c.slots, a.window, a.sinks);
+    const int use = useful_splits(seen.blocks, splits);
+    if (split >= use) return;
+    const int b0 = static_cast<int>(static_cast<int64_t>(seen.blocks) * split / use);
+    const int b1 = static_cast<int>(static_cast<int64_t>(seen.blocks) * (split + 1) / use);
+
+    const int my_row = tile.r0 + g;
+    const bool live = g < rows;
+    int64_t position = length - tile.n + my_row / group;
+    if (!live || !inside || position >= c.slots) position = -1;
+    const float to_log2 = a.scale * kLog2e;
+
+    // This lane's part of the queries as A fragments: product m of group gr takes, for 4-bit
+    // keys, channels 8 t + {2 m, 2 m + 4} and {2 m + 1, 2 m + 5} (the order in which nibbles
+    // unpack), otherwise 8 t + 4 m + {0, 1} and {2, 3}.
+    uint32_t qa[kMma][2][kQ];
+    float qsum[G];
+    {
+        const int token = tile.first + my_row / group;
+        const T* src = q + token * q_stride + (kvh * group + my_row % group) * HD + 8 * t;
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) {
+            float x[8], sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[i] = live ? to_f(src[32 * gr + i]) : 0.0f;
+                if (kExact) x[i] *= to_log2;
+                sum += x[i];
+            }
+            sum += __shfl_xor_sync(kFull, sum, 1);
+            qsum[gr] = sum + __shfl_xor_sync(kFull, sum, 2);
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                if constexpr (L::kCodes) {
+                    terms_of<kQ>(x[2 * m], x[2 * m + 4], qa[2 * gr + m][0]);
+                    terms_of<kQ>(x[2 * m + 1], x[2 * m + 5], qa[2 * gr + m][1]);
+                } else {
+                    terms_of<kQ>(x[4 * m], x[4 * m + 1], qa[2 * gr + m][0]);
+                    terms_of<kQ>(x[4 * m + 2], x[4 * m + 3], qa[2 * gr + m][1]);
+                }
+            }
+        }
+    }
+
+    const int64_t at = (static_cast<int64_t>(inside ? row : 0) * c.kv_heads + kvh) * c.slots;
+    const char* kb = static_cast<const char*>(c.k) + at * L::kRowBytes;
+    const char* vb = static_cast<const char*>(c.v) + at * L::kRowBytes;
+    const char* ksb = static_cast<const char*>(c.k_scale) + at * (G * 4);
+    const char* vsb = static_cast<const char*>(c.v_scale) + at * (G * 4);
+    const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) +
+                          warp * L::kStages * L::kStage;
+    auto fetch = [&](int block, int stage) {
+        if (block < b1) {
+            const int64_t key0 = seen.key(block);
+            const uint32_t dst = ring + stage * L::kStage;
+#pragma unroll
+            for (int i = 0; i < L::kChunks; ++i) {
+                const int index = lane + 32 * i;
+                const int half = index / (kBlock * L::kChunks);
+                const int rest = index % (kBlock * L::kChunks);
+                const int r = rest / L::kChunks, chunk = rest % L::kChunks;
+                const bool ok = seen.holds(key0 + r);
+                const char* src = (half ? vb : kb) + (ok ? (key0 + r) * L::kRowBytes + chunk * 16 : 0);
+                cp_async16(dst + half * (kBlock * L::kRowBytes) + r * L::kRowBytes +
+                               swizzled<STORAGE, HD>(r, chunk) * 16,
+                           src, ok ? 16 : 0);
+            }
+            if constexpr (L::kCodes) {
+                const int half = lane >> 4, r = lane & 15;
+                const bool ok = seen.holds(key0 + r);
+                const char* src = (half ? vsb : ksb) + (ok ? (key0 + r) * (G * 4) : 0);
+                cp_async_small<G * 4>(dst + 2 * kBlock * L::kRowBytes + half * L::kScaleBytes +
+                                          r * (G * 4),
+                                      src, ok ? G * 4 : 0);
+            }
+        }
+        cp_commit();
+    };
+
+    float o[G * 4][4], low_sum[G], top = -INFINITY, total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < G * 4; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < G; ++i) low_sum[i] = 0.0f;
+
+    int next = b0 + warp;
+#pragma unroll
+    for (int i = 0; i < L::kStages - 1; ++i) {
+        fetch(next, i);
+        next += kWarps;
+    }
+    int stage = 0;
+    for (int block = b0 + warp; block < b1; block += kWarps) {
+        cp_wait<L::kStages - 2>();
+        __syncwarp();
+        const uint32_t ks = ring + stage * L::kStage;
+        const uint32_t vs = ks + kBlock * L::kRowBytes;
+        const uint32_t kss = ks + 2 * kBlock * L::kRowBytes, vss = kss + L::kScaleBytes;
+        const int64_t key0 = seen.key(block);
+
+        // Scores of keys key0 + 8 nb + row_of_column(2 t + e), this lane's query row.
+        float s[2][2];
+        int key_row[2];
+        key_row[0] = row_of_column<STORAGE, HD>(2 * t);
+        key_row[1] = row_of_column<STORAGE, HD>(2 * t + 1);
+#pragma unroll
+        for (int nb = 0; nb < 2; ++nb) {
+            const int r = 8 * nb + row_of_column<STORAGE, HD>(g);  // the key this lane loads
+            if constexpr (L::kCodes) {
+                // Bytes [t * 4 G, ...) of the row: half 2 t of every group, then half 2 t + 1.
+                uint32_t w[G];
+                {
+                    const int chunk = t * 4 * G / 16, rest = t * 4 * G % 16;
+                    load_words<G>(ks + r * L::kRowBytes + swizzled<STORAGE, HD>(r, chunk) * 16 + rest, w);
+                }
+                uint32_t sa[G], sb[G];  // (step, low) of the two keys this lane scores
+                load_words<G>(kss + (8 * nb + key_row[0]) * (G * 4), sa);
+                load_words<G>(kss + (8 * nb + key_row[1]) * (G * 4), sb);
+                s[nb][0] = s[nb][1] = 0.0f;
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr) {
+                    uint32_t x;
+                    if constexpr (G == 1) {
+                        x = w[0];
+                    } else {
+                        // 16-bit entries gr and G + gr of the lane's 2 G.
+                        x = __byte_perm(w[gr / 2], w[G / 2 + gr / 2], gr & 1 ? 0x7632 : 0x5410);
+                    }
+                    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int m = 0; m < 2; ++m) {
+                        const uint32_t k0 = nibbles<!kExact>(x, 2 * m);
+                        const uint32_t k1 = nibbles<!kExact>(x, 2 * m + 1);
+                        uint32_t(&A)[2][kQ] = qa[2 * gr + m];
+                        if constexpr (kExact) {
+                            mma_bf16(acc, A[0][0], A[0][1], A[1][0], A[1][1], k0, k1);
+                            mma_bf16(acc, A[0][2], 0u, A[1][2], 0u, k0, k1);
+                        } else {
+                            mma_bf16(acc, A[0][0], 0u, A[1][0], 0u, k0, k1);
+                        }
+                    }
+                    const float pa = kExact ? acc[0] + acc[2] : acc[0];
+                    const float pb = kExact ? acc[1] + acc[3] : acc[1];
+                    const float step_a = low_of(sa[gr]), step_b = low_of(sb[gr]);
+                    float low_a = high_of(sa[gr]), low_b = high_of(sb[gr]);
+                    if constexpr (!kExact) {
+                        low_a = fmaf(-128.0f, step_a, low_a);
+                        low_b = fmaf(-128.0f, step_b, low_b);
+                    }
+                    s[nb][0] = fmaf(step_a, pa, fmaf(low_a, qsum[gr], s[nb][0]));
+                    s[nb][1] = fmaf(step_b, pb, fmaf(low_b, qsum[gr], s[nb][1]));
+                }
+            } else {
+                float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr) {
+                    uint32_t kw[4][kK];  // channels 8 t .. 8 t + 7 of the group, in pairs
+                    if constexpr (STORAGE == BST_DTYPE_BF16) {
+                        uint32_t w[4];
+                        load_words<4>(ks + r * L::kRowBytes + swizzled<STORAGE, HD>(r, 4 * gr + t) * 16, w);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) kw[i][0] = w[i];
+                    } else {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            uint32_t w[4];
+                            load_words<4>(ks + r * L::kRowBytes +
+                                              swizzled<STORAGE, HD>(r, 8 * gr + 2 * t + h) * 16, w);
+                            terms_of<kK>(__uint_as_float(w[0]), __uint_as_float(w[1]), kw[2 * h]);
+                            terms_of<kK>(__uint_as_float(w[2]), __uint_as_float(w[3]), kw[2 * h + 1]);
+                        }
+                    }
+#pragma unroll
+                    for (int m = 0; m < 2; ++m) {
+                        uint32_t(&A)[2][kQ] = qa[2 * gr + m];
+#pragma unroll
+                        for (int i = 0; i < kK; ++i) {
+                            if constexpr (kExact) {
+                                mma_bf16(acc, A[0][0], A[0][1], A[1][0], A[1][1], kw[2 * m][i],
+                                         kw[2 * m + 1][i]);
+                            } else {
+                                mma_bf16(acc, A[0][0], 0u, A[1][0], 0u, kw[2 * m][i],
+                                         kw[2 * m + 1][i]);
+                            }
+                        }
+                        if constexpr (kExact) {
+                            mma_bf16(acc, A[0][2], 0u, A[1][2], 0u, kw[2 * m][0], kw[2 * m + 1][0]);
+                        }
+                    }
+                }
+                s[nb][0] = kExact ? acc[0] + acc[2] : acc[0];
+                s[nb][1] = kExact ? acc[1] + acc[3] : acc[1];
+            }
+        }
+        // Mask, running maximum.
+        bool ok[2][2];
+        float block_top = -INFINITY;
+#pragma unroll
+        for (int nb = 0; nb < 2; ++nb) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int64_t key = key0 + 8 * nb + key_row[e];
+                ok[nb][e] = key <= position &&
+                            (a.window == 0 || position - key < a.window || key < a.sinks);
+                if (!kExact) s[nb][e] *= to_log2;
+                s[nb][e] = ok[nb][e] ? s[nb][e] : -INFINITY;
+                block_top = fmaxf(block_top, s[nb][e]);
+            }
+        }
+        block_top = fmaxf(block_top, __shfl_xor_sync(kFull, block_top, 1));
+        block_top = fmaxf(block_top, __shfl_xor_sync(kFull, block_top, 2));
+        const bool grows = block_top > top;
+        if (__any_sync(kFull, grows)) {
+            const float keep = grows ? (top == -INFINITY ? 0.0f : exp2_fast(top - block_top)) : 1.0f;
+            top = grows ? block_top : top;
+            total *= keep;
+#pragma unroll
+            for (int i = 0; i < G; ++i) low_sum[i] *= keep;
+#pragma unroll
+            for (int i = 0; i < G * 4; ++i) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[i][j] *= keep;
+            }
+        }
+        const float base = top == -INFINITY ? 0.0f : top;
+        float p[2][2];
+#pragma unroll
+        for (int nb = 0; nb < 2; ++nb) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                p[nb][e] = exp2_fast(s[nb][e] - base);
+                total += p[nb][e];
+            }
+        }
+
+        // Weights times values.
+        if constexpr (L::kCodes) {
+            uint32_t sv[2][2][G];
+            uint32_t wv[2][2][(G + 1) / 2];
+#pragma unroll
+            for (int nb = 0; nb < 2; ++nb) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int r = 8 * nb + key_row[e];
+                    load_words<G>(vss + r * (G * 4), sv[nb][e]);
+                    // 16-bit entries [g][0 .. G): nibble j is channel 4 g + j of a group.
+                    if constexpr (G == 1) {
+                        uint16_t h;
+                        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(vs + r * L::kRowBytes + g * 2));
+                        wv[nb][e][0] = h;
+                    } else {
+                        const int chunk = g * 2 * G / 16, rest = g * 2 * G % 16;
+                        load_words<G / 2>(vs + r * L::kRowBytes + swizzled<STORAGE, HD>(r, chunk) * 16 + rest,
+                                          wv[nb][e]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr) {
+                uint32_t pa[2][kTerms], x[2];
+#pragma unroll
+                for (int nb = 0; nb < 2; ++nb) {
+                    const float step0 = low_of(sv[nb][0][gr]), step1 = low_of(sv[nb][1][gr]);
+                    float low0 = high_of(sv[nb][0][gr]), low1 = high_of(sv[nb][1][gr]);
+                    if constexpr (!kExact) {
+                        low0 = fmaf(-128.0f, step0, low0);
+                        low1 = fmaf(-128.0f, step1, low1);
+                    }
+                    // A key this query does not see may hold a NaN that another one does see.
+                    low_sum[gr] = fmaf(p[nb][0], ok[nb][0] ? low0 : 0.0f, low_sum[gr]);
+                    low_sum[gr] = fmaf(p[nb][1], ok[nb][1] ? low1 : 0.0f, low_sum[gr]);
+                    terms_of<kTerms>(p[nb][0] * step0, p[nb][1] * step1, pa[nb]);
+                    x[nb] = __byte_perm(wv[nb][0][gr / 2], wv[nb][1][gr / 2], gr & 1 ? 0x7632 : 0x5410);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t v0 = nibbles<!kExact>(x[0], j), v1 = nibbles<!kExact>(x[1], j);
+                    mma_bf16(o[4 * gr + j], pa[0][0], pa[0][1], pa[1][0], pa[1][1], v0, v1);
+                    if constexpr (kExact) mma_bf16(o[4 * gr + j], pa[0][2], 0u, pa[1][2], 0u, v0, v1);
+                }
+            }
+        } else {
+            uint32_t pa[2][kTerms];
+            terms_of<kTerms>(p[0][0], p[0][1], pa[0]);
+            terms_of<kTerms>(p[1][0], p[1][1], pa[1]);
+#pragma unroll
+            for (int j = 0; j < G * 4; ++j) {  // channels 8 j .. 8 j + 7, column n of them at lane n = g
+                uint32_t v0[kK], v1[kK];
+                if constexpr (STORAGE == BST_DTYPE_BF16) {
+                    // Lanes 0-15 name the rows; the transposed 8x8 pair is this lane's fragment.
+                    const int r = lane & 15;
+                    const uint32_t addr = vs + r * L::kRowBytes + swizzled<STORAGE, HD>(r, j) * 16;
+                    asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];"
+                                 : "=r"(v0[0]), "=r"(v1[0]) : "r"(addr));
+                } else {
+                    float v[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = 2 * t + (i & 1) + 8 * (i >> 1);
+                        const int chunk = 2 * j + (g >> 2);
+                        asm volatile("ld.shared.f32 %0, [%1];"
+                                     : "=f"(v[i])
+                                     : "r"(vs + r * L::kRowBytes + swizzled<STORAGE, HD>(r, chunk) * 16 +
+                                           (g & 3) * 4));
+                    }
+                    terms_of<kK>(v[0], v[1], v0);
+                    terms_of<kK>(v[2], v[3], v1);
+                }
+#pragma unroll
+                for (int i = 0; i < kK; ++i) {
+                    mma_bf16(o[j], pa[0][0], pa[0][1], pa[1][0], pa[1][1], v0[i], v1[i]);
+                }
+                if constexpr (kExact) mma_bf16(o[j], pa[0][2], 0u, pa[1][2], 0u, v0[0], v1[0]);
+            }
+        }
+        __syncwarp();
+        fetch(next, (stage + L::kStages - 1) % L::kStages);
+        next += kWarps;
+        stage = (stage + 1) % L::kStages;
+    }
+    cp_wait<0>();
+    __syncthreads();  // the rings become the merge buffer
+
+    // The warps' results: [warp][row][HD outputs, maximum, sum].
+    total += __shfl_xor_sync(kFull, total, 1);
+    total += __shfl_xor_sync(kFull, total, 2);
+    float* merge = reinterpret_cast<float*>(smem);
+    float* mine = merge + (warp * kRows + g) * (HD + 2);
+#pragma unroll
+    for (int gr = 0; gr < G; ++gr) {
+        float low = low_sum[gr];
+        if constexpr (L::kCodes) {
+            low += __shfl_xor_sync(kFull, low, 1);
+            low += __shfl_xor_sync(kFull, low, 2);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float(&x)[4] = o[4 * gr + j];
+            // Columns 2 t and 2 t + 1: channels 4 n + j of the group (codes) or 8 j + n.
+            const int c0 = L::kCodes ? 32 * gr + 8 * t + j : 32 * gr + 8 * j + 2 * t;
+            mine[c0] = x[0] + x[2] + low;
+            mine[c0 + (L::kCodes ? 4 : 1)] = x[1] + x[3] + low;
+        }
+    }
+    if (t == 0) {
+        mine[HD] = top;
+        mine[HD + 1] = total;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows * HD; i += kThreads) {
+        const int r = i / HD, ch = i % HD;
+        float m = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, merge[(w * kRows + r) * (HD + 2) + HD]);
+        float sum = 0.0f, value = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float* from = merge + (w * kRows + r) * (HD + 2);
+            const float f = from[HD] == -INFINITY ? 0.0f : exp2_fast(from[HD] - m);
+            sum = fmaf(from[HD + 1], f, sum);
+            // A warp that saw no key has nothing to add, not even zero times its output.
+            if (from[HD] != -INFINITY || from[HD + 1] != 0.0f) value = fmaf(from[ch], f, value);
+        }
+        const int query = tile.r0 + r;
+        const int64_t token = tile.first + query / group;
+        const int head = kvh * group + query % group;
+        if (splits == 1) {
+            put(out + token * out_stride + head * HD + ch, sum == 0.0f ? 0.0f : value / sum);
+        } else {
+            float* to = part + ((token * a.heads + head) * splits + split) * (HD + 2);
+            to[ch] = value;
+            if (ch == 0) {
+                to[HD] = m;
+                to[HD + 1] = sum;
+            }
+        }
+    }
+}
+
+// Joins the splits of a query, one warp each: the largest maximum, then the weighted sums.
+template <typename T, int HD>
+__global__ void __launch_bounds__(kThreads)
+k_cached_join(Cache c, Batch b, AttnSpec a, T* __restrict__ out, int64_t out_stride, int splits,
+              const float* __restrict__ part) {
+    constexpr int C = HD / 32;
+    const int64_t unit = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (unit >= static_cast<int64_t>(b.tokens) * a.heads) return;
+    const int token = static_cast<int>(unit / a.heads), head = static_cast<int>(unit % a.heads);
+    int seq, first, n;
+    if (!find_sequence(b, token, &seq, &first, &n)) return;
+    // How many splits the query's tile used, as k_cached found it.
+    n = min(n, b.tokens - first);
+    const int group = a.heads / a.kv_heads;
+    const int row = b.rows ? __ldg(b.rows + seq) : seq;
+    const int64_t length = __ldg(b.lengths + seq);
+    const int r0 = ((token - first) * group + head % group) / kRows * kRows;
+    const int rows = min(kRows, n * group - r0);
+    const int64_t p_last = row >= 0 && row < c.rows ? length - n + (r0 + rows - 1) / group : -1;
+    const Visible seen(length - n + r0 / group, p_last, c.slots, a.window, a.sinks);
+    const int use = useful_splits(seen.blocks, splits);
+    pdl_wait();
+    const float* from = part + unit * splits * (HD + 2);
+    float m = -INFINITY;
+    for (int s = lane; s < use; s += 32) m = fmaxf(m, from[s * (HD + 2) + HD]);
+    m = warp_max(m);
+    float sum = 0.0f, value[C] = {};
+    for (int s = 0; s < use; ++s) {
+        const float* x = from + s * (HD + 2);
+        const float top = x[HD];
+        const float f = top == -INFINITY ? 0.0f : exp2_fast(top - m);
+        sum = fmaf(x[HD + 1], f, sum);
+        if (top != -INFINITY || x[HD + 1] != 0.0f) {
+#pragma unroll
+            for (int i = 0; i < C; ++i) value[i] = fmaf(x[lane + 32 * i], f, value[i]);
+        }
+    }
+    T* to = out + token * out_stride + head * HD;
+#pragma unroll
+    for (int i = 0; i < C; ++i) put(to + lane + 32 * i, sum == 0.0f ? 0.0f : value[i] / sum);
+}
+
+// Tiles of eight query rows: exact without starts, at most one partial tile a sequence with them.
+int tile_bound(const Batch& b, const AttnSpec& a) {
+    const int64_t group = a.heads / a.kv_heads;
+    if (!b.starts) return static_cast<int>(b.count * ((group + kRows - 1) / kRows));
+    return static_cast<int>(std::min<int64_t>((b.tokens * group) / kRows + b.count, b.tokens * group));
+}
+
+// CTAs for about four on every SM, and splits of at most 2048 keys so that a few long sequences
+// among short ones are spread over the SMs too; never less than 128 keys a split. The lengths are
+// on the device, so the bound is what the cache and the window allow; tiles with fewer keys use
+// fewer splits (useful_splits).
+int split_count(const Cache& c, const Batch& b, const AttnSpec& a) {
+    int64_t keys = c.slots;
+    if (a.window) keys = std::min<int64_t>(keys, static_cast<int64_t>(a.window) + a.sinks + 2 * kBlock);
+    const int64_t units = static_cast<int64_t>(tile_bound(b, a)) * a.kv_heads;
+    const int64_t fill = (148 * 4 + units - 1) / std::max<int64_t>(units, 1);
+    const int64_t even = (keys + 2047) / 2048;
+    const int64_t most = std::max<int64_t>(1, keys / 128);
+    return static_cast<int>(std::min<int64_t>({std::max(fill, even), most, 512}));
+}
+
+}  // namespace
+
+size_t attention_cached_workspace(const Cache& c, const Batch& b, const AttnSpec& a) {
+    const int splits = split_count(c, b, a);
+    if (splits == 1) return 0;
+    return static_cast<size_t>(b.tokens) * a.heads * splits * (a.head_dim + 2) * sizeof(float);
+}
+
+cudaError_t launch_attention_cached(cudaStream_t s, const Cache& c, const Batch& b,
+                                    const AttnSpec& a, const void* q, int64_t q_stride, void* out,
+                                    int64_t out_stride, void* workspace) {
+    if (b.tokens < 1 || b.count < 1) return cudaSuccess;
+    return by_dtype(a.dtype, [&](auto type) {
+        using T = decltype(type);
+        return by_head_dim(a.head_dim, [&](auto hd) {
+            constexpr int HD = decltype(hd)::value;
+            return by_storage(c.storage, [&](auto st) {
+                constexpr int STORAGE = decltype(st)::value;
+                using L = Layout<STORAGE, HD>;
+                const int splits = split_count(c, b, a);
+                const dim3 grid(tile_bound(b, a), a.kv_heads, splits);
+                cudaError_t e = cudaFuncSetAttribute(k_cached<T, STORAGE, HD>,
+                                                     cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                     L::kSmem);
+                if (e) return e;
+                k_cached<T, STORAGE, HD><<<grid, kThreads, L::kSmem, s>>>(
+                    c, b, a, static_cast<const T*>(q), q_stride, static_cast<T*>(out), out_stride,
+                    splits, static_cast<float*>(workspace));
+                e = cudaGetLastError();
+                if (e || splits == 1) return e;
+                const int64_t units = static_cast<int64_t>(b.tokens) * a.heads;
+                return launch_pdl(k_cached_join<T, HD>,
+                                  dim3(static_cast<unsigned>((units + kWarps - 1) / kWarps)),
+                                  dim3(kThreads), 0, s, c, b, a, static_cast<T*>(out), out_stride,
+                                  splits, static_cast<const float*>(workspace));
+            });
+        });
+    });
+}
+
+}  // namespace bst
