@@ -8,9 +8,12 @@
 //   s_ij    = sum_g step_jg (q_ig . c_jg) + low_jg sum(q_ig)         g: groups of 32 channels
 //   out_icg = sum_j (p_ij step_jg) c_jgc + sum_j p_ij low_jg
 //
-// A nibble becomes a bf16 number without a conversion: 0x4300 | c is 128 + c. bf16 queries keep
-// the 128 and take it out through low - 128 step, float32 ones subtract it (it would cost them four
-// bits). mma.sync m16n8k16 reads its B operand from registers, which is where unpacked codes are;
+// A nibble becomes a bf16 number without a conversion. Keys: the bits themselves, c or 16 c in the
+// lowest mantissa bits, are c 2^-133 or 16 c 2^-133 (bf16's subnormals and its first binade have the
+// same spacing); the queries carry the 2^127 and 2^123 that bring them back, normalised by a power
+// of two per row so that nothing overflows. Values: 0x4300 | c is 128 + c; bf16 queries keep the 128
+// and take it out through low - 128 step, float32 ones subtract it (it would cost them four bits).
+// mma.sync m16n8k16 reads its B operand from registers, which is where unpacked codes are;
 // tcgen05 would need them written to shared memory at four times their size first, and a tile
 // of at most eight query rows would leave 120 of its 128 rows empty.
 //
@@ -28,6 +31,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <cfloat>
 
 #include "attention.cuh"
 #include "device.cuh"
@@ -133,10 +137,11 @@ __device__ __forceinline__ void terms_of(float a, float b, uint32_t* out) {
     }
 }
 
-// Nibble i of both halves of x as bf16 numbers: c or, with OFFSET, 128 + c.
+// Nibble i of both halves of x as bf16 numbers: c or, with OFFSET, 128 + c. The shifts are high
+// halves of products, which run beside the logic operations instead of among them.
 template <bool OFFSET>
 __device__ __forceinline__ uint32_t nibbles(uint32_t x, int i) {
-    const uint32_t v = ((x >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+    const uint32_t v = ((i ? __umulhi(x, 1u << (32 - 4 * i)) : x) & 0x000f000fu) | 0x43004300u;
     if constexpr (OFFSET) return v;
     uint32_t r;
     asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(0x43004300u));
@@ -158,26 +163,29 @@ __device__ __forceinline__ void load_words(uint32_t addr, uint32_t (&w)[G]) {
 // The keys that a tile of queries at positions p0..p1 sees: blocks of 16 that hold the sinks before
 // the window, then blocks from the window's first key (rounded down) to the last key.
 struct Visible {
-    int64_t first, end;   // the window
-    int64_t aligned;      // first, rounded down to a block
+    int first, end;       // the window
+    int aligned;          // first, rounded down to a block
     int sinks;            // keys below it are visible too
     int sink_blocks, blocks;
-    __device__ Visible(int64_t p0, int64_t p1, int slots, int window, int sinks_) {
-        end = min(p1 + 1, static_cast<int64_t>(slots));
-        first = window ? max(static_cast<int64_t>(0), p0 - window + 1) : 0;
-        aligned = first & ~static_cast<int64_t>(kBlock - 1);
+    __device__ Visible(int p0, int p1, int slots, int window, int sinks_) {
+        end = min(p1 + 1, slots);
+        first = window ? max(0, p0 - window + 1) : 0;
+        aligned = first & ~(kBlock - 1);
         sinks = sinks_;
         blocks = sink_blocks = 0;
-        if (end > 0 && first < end) {
-            sink_blocks = static_cast<int>((min(static_cast<int64_t>(sinks), aligned) + kBlock - 1) / kBlock);
-            blocks = sink_blocks + static_cast<int>((end - aligned + kBlock - 1) / kBlock);
+        if (first < end) {
+            sink_blocks = (min(sinks, aligned) + kBlock - 1) / kBlock;
+            blocks = sink_blocks + (end - aligned + kBlock - 1) / kBlock;
         }
     }
-    __device__ int64_t key(int block) const {
-        return block < sink_blocks ? static_cast<int64_t>(block) * kBlock
-                                   : aligned + static_cast<int64_t>(block - sink_blocks) * kBlock;
+    __device__ int key(int block) const {
+        return block < sink_blocks ? block * kBlock : aligned + (block - sink_blocks) * kBlock;
     }
-    __device__ bool holds(int64_t key) const { return key < end && (key >= first || key < sinks); }
+    __device__ bool holds(int key) const { return key < end && (key >= first || key < sinks); }
+    // Whether all keys of the block at key0 are held.
+    __device__ bool whole(int key0) const {
+        return key0 + kBlock <= end && (key0 >= first || key0 + kBlock <= sinks);
+    }
 };
 
 // Splits that a tile of this many blocks is worth: at least 8 blocks a split, two a warp.
@@ -254,12 +262,12 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
     Tile tile;
     if (!find_tile(b, group, blockIdx.x, &tile)) return;
     const int row = b.rows ? __ldg(b.rows + tile.seq) : tile.seq;
-    const int64_t length = __ldg(b.lengths + tile.seq);
+    const int length = max(0, __ldg(b.lengths + tile.seq));
     const int rows = min(kRows, tile.n * group - tile.r0);
     // Positions of the tile's tokens; a row or slot outside the cache sees nothing.
     const bool inside = row >= 0 && row < c.rows;
-    const int64_t p_first = length - tile.n + tile.r0 / group;
-    const int64_t p_last = length - tile.n + (tile.r0 + rows - 1) / group;
+    const int p_first = length - tile.n + tile.r0 / group;
+    const int p_last = length - tile.n + (tile.r0 + rows - 1) / group;
     const Visible seen(p_first, inside ? p_last : -1, c.slots, a.window, a.sinks);
     const int use = useful_splits(seen.blocks, splits);
     if (split >= use) return;
@@ -268,37 +276,60 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
 
     const int my_row = tile.r0 + g;
     const bool live = g < rows;
-    int64_t position = length - tile.n + my_row / group;
+    int position = length - tile.n + my_row / group;
     if (!live || !inside || position >= c.slots) position = -1;
     const float to_log2 = a.scale * kLog2e;
 
     // This lane's part of the queries as A fragments: product m of group gr takes, for 4-bit
     // keys, channels 8 t + {2 m, 2 m + 4} and {2 m + 1, 2 m + 5} (the order in which nibbles
-    // unpack), otherwise 8 t + 4 m + {0, 1} and {2, 3}.
+    // unpack, the second pair 16 times too large), otherwise 8 t + 4 m + {0, 1} and {2, 3}.
+    // to_score takes a product to the base-2 logarithm of its weight.
     uint32_t qa[kMma][2][kQ];
-    float qsum[G];
+    float qsum[G], to_score = a.scale * kLog2e;
     {
         const int token = tile.first + my_row / group;
         const T* src = q + token * q_stride + (kvh * group + my_row % group) * HD + 8 * t;
+        float x[G][8], largest = 0.0f;
 #pragma unroll
         for (int gr = 0; gr < G; ++gr) {
-            float x[8], sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                x[i] = live ? to_f(src[32 * gr + i]) : 0.0f;
-                if (kExact) x[i] *= to_log2;
-                sum += x[i];
+                x[gr][i] = live ? to_f(src[32 * gr + i]) : 0.0f;
+                largest = fmaxf(largest, fabsf(x[gr][i]));
             }
+        }
+        if constexpr (L::kCodes) {
+            // Normalised to |q| < 1; products come out 2^-6 too small (2^127 for 2^133).
+            largest = fmaxf(largest, __shfl_xor_sync(kFull, largest, 1));
+            largest = fmaxf(largest, __shfl_xor_sync(kFull, largest, 2));
+            const int e = max(min(ilogbf(fmaxf(largest, FLT_MIN)), 126) + 1, -100);
+            const float shrink = exp2f(static_cast<float>(-e));
+            to_score *= exp2f(static_cast<float>(e));
+            to_score *= 64.0f;
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[gr][i] *= shrink;
+            }
+        }
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum += x[gr][i];
             sum += __shfl_xor_sync(kFull, sum, 1);
-            qsum[gr] = sum + __shfl_xor_sync(kFull, sum, 2);
+            sum += __shfl_xor_sync(kFull, sum, 2);
+            qsum[gr] = sum * 0.015625f;
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
                 if constexpr (L::kCodes) {
-                    terms_of<kQ>(x[2 * m], x[2 * m + 4], qa[2 * gr + m][0]);
-                    terms_of<kQ>(x[2 * m + 1], x[2 * m + 5], qa[2 * gr + m][1]);
+                    terms_of<kQ>(x[gr][2 * m] * 0x1p127f, x[gr][2 * m + 4] * 0x1p127f,
+                                 qa[2 * gr + m][0]);
+                    terms_of<kQ>(x[gr][2 * m + 1] * 0x1p123f, x[gr][2 * m + 5] * 0x1p123f,
+                                 qa[2 * gr + m][1]);
                 } else {
-                    terms_of<kQ>(x[4 * m], x[4 * m + 1], qa[2 * gr + m][0]);
-                    terms_of<kQ>(x[4 * m + 2], x[4 * m + 3], qa[2 * gr + m][1]);
+                    terms_of<kQ>(x[gr][4 * m], x[gr][4 * m + 1], qa[2 * gr + m][0]);
+                    terms_of<kQ>(x[gr][4 * m + 2], x[gr][4 * m + 3], qa[2 * gr + m][1]);
                 }
             }
         }
@@ -311,29 +342,37 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
     const char* vsb = static_cast<const char*>(c.v_scale) + at * (G * 4);
     const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) +
                           warp * L::kStages * L::kStage;
+    // This lane's chunks of a block: row and byte offsets, in its source and in a stage.
+    int from_row[L::kChunks], from[L::kChunks], to[L::kChunks];
+#pragma unroll
+    for (int i = 0; i < L::kChunks; ++i) {
+        const int index = lane + 32 * i;
+        const int half = index / (kBlock * L::kChunks), rest = index % (kBlock * L::kChunks);
+        const int r = rest / L::kChunks, chunk = rest % L::kChunks;
+        from_row[i] = r;
+        from[i] = r * L::kRowBytes + chunk * 16;
+        to[i] = half * (kBlock * L::kRowBytes) + r * L::kRowBytes + swizzled<STORAGE, HD>(r, chunk) * 16;
+    }
+    // Chunk i lies in the keys or in the values: by the lane where a row is one chunk.
+    const char* const first_base = L::kChunks == 1 && lane >= 16 ? vb : kb;
+    const char* const scale_base = (lane >= 16 ? vsb : ksb) + (lane & 15) * (G * 4);
     auto fetch = [&](int block, int stage) {
         if (block < b1) {
-            const int64_t key0 = seen.key(block);
+            const int key0 = seen.key(block);
             const uint32_t dst = ring + stage * L::kStage;
+            const int64_t bytes = static_cast<int64_t>(key0) * L::kRowBytes;
+            const bool whole = seen.whole(key0);
 #pragma unroll
             for (int i = 0; i < L::kChunks; ++i) {
-                const int index = lane + 32 * i;
-                const int half = index / (kBlock * L::kChunks);
-                const int rest = index % (kBlock * L::kChunks);
-                const int r = rest / L::kChunks, chunk = rest % L::kChunks;
-                const bool ok = seen.holds(key0 + r);
-                const char* src = (half ? vb : kb) + (ok ? (key0 + r) * L::kRowBytes + chunk * 16 : 0);
-                cp_async16(dst + half * (kBlock * L::kRowBytes) + r * L::kRowBytes +
-                               swizzled<STORAGE, HD>(r, chunk) * 16,
-                           src, ok ? 16 : 0);
+                const char* src = (L::kChunks == 1 ? first_base : (i < L::kChunks / 2 ? kb : vb));
+                const bool ok = whole || seen.holds(key0 + from_row[i]);
+                cp_async16(dst + to[i], src + (ok ? bytes + from[i] : 0), ok ? 16 : 0);
             }
             if constexpr (L::kCodes) {
-                const int half = lane >> 4, r = lane & 15;
-                const bool ok = seen.holds(key0 + r);
-                const char* src = (half ? vsb : ksb) + (ok ? (key0 + r) * (G * 4) : 0);
-                cp_async_small<G * 4>(dst + 2 * kBlock * L::kRowBytes + half * L::kScaleBytes +
-                                          r * (G * 4),
-                                      src, ok ? G * 4 : 0);
+                const bool ok = whole || seen.holds(key0 + (lane & 15));
+                const char* src = ok ? scale_base + static_cast<int64_t>(key0) * (G * 4) : ksb;
+                cp_async_small<G * 4>(dst + 2 * kBlock * L::kRowBytes + lane * (G * 4), src,
+                                      ok ? G * 4 : 0);
             }
         }
         cp_commit();
@@ -358,7 +397,7 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
         const uint32_t ks = ring + stage * L::kStage;
         const uint32_t vs = ks + kBlock * L::kRowBytes;
         const uint32_t kss = ks + 2 * kBlock * L::kRowBytes, vss = kss + L::kScaleBytes;
-        const int64_t key0 = seen.key(block);
+        const int key0 = seen.key(block);
 
         // Scores of keys key0 + 8 nb + row_of_column(2 t + e), this lane's query row.
         float s[2][2];
@@ -391,8 +430,8 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
                     float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int m = 0; m < 2; ++m) {
-                        const uint32_t k0 = nibbles<!kExact>(x, 2 * m);
-                        const uint32_t k1 = nibbles<!kExact>(x, 2 * m + 1);
+                        const uint32_t y = m ? __umulhi(x, 1u << 24) : x;  // x >> 8
+                        const uint32_t k0 = y & 0x000f000fu, k1 = y & 0x00f000f0u;
                         uint32_t(&A)[2][kQ] = qa[2 * gr + m];
                         if constexpr (kExact) {
                             mma_bf16(acc, A[0][0], A[0][1], A[1][0], A[1][1], k0, k1);
@@ -404,11 +443,7 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
                     const float pa = kExact ? acc[0] + acc[2] : acc[0];
                     const float pb = kExact ? acc[1] + acc[3] : acc[1];
                     const float step_a = low_of(sa[gr]), step_b = low_of(sb[gr]);
-                    float low_a = high_of(sa[gr]), low_b = high_of(sb[gr]);
-                    if constexpr (!kExact) {
-                        low_a = fmaf(-128.0f, step_a, low_a);
-                        low_b = fmaf(-128.0f, step_b, low_b);
-                    }
+                    const float low_a = high_of(sa[gr]), low_b = high_of(sb[gr]);
                     s[nb][0] = fmaf(step_a, pa, fmaf(low_a, qsum[gr], s[nb][0]));
                     s[nb][1] = fmaf(step_b, pb, fmaf(low_b, qsum[gr], s[nb][1]));
                 }
@@ -454,18 +489,27 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
                 s[nb][1] = kExact ? acc[1] + acc[3] : acc[1];
             }
         }
-        // Mask, running maximum.
-        bool ok[2][2];
+        // Mask, running maximum. Every query of the tile sees all of a block in the middle.
+        const bool all = key0 + kBlock - 1 <= p_first && p_last < c.slots &&
+                         (a.window == 0 || p_last - key0 < a.window || key0 + kBlock <= a.sinks);
+        bool hidden[2][2] = {};
         float block_top = -INFINITY;
+        if (!all) {
+#pragma unroll
+            for (int nb = 0; nb < 2; ++nb) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int key = key0 + 8 * nb + key_row[e];
+                    hidden[nb][e] = key > position || (a.window != 0 && position - key >= a.window &&
+                                                       key >= a.sinks);
+                }
+            }
+        }
 #pragma unroll
         for (int nb = 0; nb < 2; ++nb) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const int64_t key = key0 + 8 * nb + key_row[e];
-                ok[nb][e] = key <= position &&
-                            (a.window == 0 || position - key < a.window || key < a.sinks);
-                if (!kExact) s[nb][e] *= to_log2;
-                s[nb][e] = ok[nb][e] ? s[nb][e] : -INFINITY;
+                s[nb][e] = hidden[nb][e] ? -INFINITY : s[nb][e] * to_score;
                 block_top = fmaxf(block_top, s[nb][e]);
             }
         }
@@ -505,6 +549,11 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
                 for (int e = 0; e < 2; ++e) {
                     const int r = 8 * nb + key_row[e];
                     load_words<G>(vss + r * (G * 4), sv[nb][e]);
+                    if (hidden[nb][e]) {
+                        // Its low may be a NaN that another query sees.
+#pragma unroll
+                        for (int gr = 0; gr < G; ++gr) sv[nb][e][gr] = 0u;
+                    }
                     // 16-bit entries [g][0 .. G): nibble j is channel 4 g + j of a group.
                     if constexpr (G == 1) {
                         uint16_t h;
@@ -528,9 +577,8 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
                         low0 = fmaf(-128.0f, step0, low0);
                         low1 = fmaf(-128.0f, step1, low1);
                     }
-                    // A key this query does not see may hold a NaN that another one does see.
-                    low_sum[gr] = fmaf(p[nb][0], ok[nb][0] ? low0 : 0.0f, low_sum[gr]);
-                    low_sum[gr] = fmaf(p[nb][1], ok[nb][1] ? low1 : 0.0f, low_sum[gr]);
+                    low_sum[gr] = fmaf(p[nb][0], low0, low_sum[gr]);
+                    low_sum[gr] = fmaf(p[nb][1], low1, low_sum[gr]);
                     terms_of<kTerms>(p[nb][0] * step0, p[nb][1] * step1, pa[nb]);
                     x[nb] = __byte_perm(wv[nb][0][gr / 2], wv[nb][1][gr / 2], gr & 1 ? 0x7632 : 0x5410);
                 }
@@ -639,47 +687,68 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
     }
 }
 
-// Joins the splits of a query, one warp each: the largest maximum, then the weighted sums.
+// Joins the splits of a query, one CTA each: the splits' factors first, then every warp sums its
+// share of the splits with all loads independent of one another.
+constexpr int kMaxSplits = 512;
+
 template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads)
 k_cached_join(Cache c, Batch b, AttnSpec a, T* __restrict__ out, int64_t out_stride, int splits,
               const float* __restrict__ part) {
     constexpr int C = HD / 32;
-    const int64_t unit = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (unit >= static_cast<int64_t>(b.tokens) * a.heads) return;
-    const int token = static_cast<int>(unit / a.heads), head = static_cast<int>(unit % a.heads);
+    __shared__ float factor[kMaxSplits], tops[kWarps], sums[kWarps], values[kWarps][HD];
+    const int token = blockIdx.x, head = blockIdx.y;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int seq, first, n;
     if (!find_sequence(b, token, &seq, &first, &n)) return;
     // How many splits the query's tile used, as k_cached found it.
     n = min(n, b.tokens - first);
     const int group = a.heads / a.kv_heads;
     const int row = b.rows ? __ldg(b.rows + seq) : seq;
-    const int64_t length = __ldg(b.lengths + seq);
+    const int length = max(0, __ldg(b.lengths + seq));
     const int r0 = ((token - first) * group + head % group) / kRows * kRows;
     const int rows = min(kRows, n * group - r0);
-    const int64_t p_last = row >= 0 && row < c.rows ? length - n + (r0 + rows - 1) / group : -1;
+    const int p_last = row >= 0 && row < c.rows ? length - n + (r0 + rows - 1) / group : -1;
     const Visible seen(length - n + r0 / group, p_last, c.slots, a.window, a.sinks);
     const int use = useful_splits(seen.blocks, splits);
     pdl_wait();
-    const float* from = part + unit * splits * (HD + 2);
+    const float* from =
+        part + (static_cast<int64_t>(token) * a.heads + head) * splits * (HD + 2);
     float m = -INFINITY;
-    for (int s = lane; s < use; s += 32) m = fmaxf(m, from[s * (HD + 2) + HD]);
+    for (int s = threadIdx.x; s < use; s += kThreads) m = fmaxf(m, from[s * (HD + 2) + HD]);
     m = warp_max(m);
-    float sum = 0.0f, value[C] = {};
-    for (int s = 0; s < use; ++s) {
-        const float* x = from + s * (HD + 2);
-        const float top = x[HD];
-        const float f = top == -INFINITY ? 0.0f : exp2_fast(top - m);
-        sum = fmaf(x[HD + 1], f, sum);
-        if (top != -INFINITY || x[HD + 1] != 0.0f) {
-#pragma unroll
-            for (int i = 0; i < C; ++i) value[i] = fmaf(x[lane + 32 * i], f, value[i]);
-        }
+    if (lane == 0) tops[warp] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    float sum = 0.0f;
+    for (int s = threadIdx.x; s < use; s += kThreads) {
+        const float top = from[s * (HD + 2) + HD], total = from[s * (HD + 2) + HD + 1];
+        // A split that saw nothing has nothing to add; one whose scores are NaN has.
+        const float f = top == -INFINITY ? (total == 0.0f ? 0.0f : total) : exp2_fast(top - m);
+        factor[s] = f;
+        sum = fmaf(total, f, sum);
     }
-    T* to = out + token * out_stride + head * HD;
+    sum = warp_sum(sum);
+    if (lane == 0) sums[warp] = sum;
+    __syncthreads();
+    sum = sums[0] + sums[1] + sums[2] + sums[3];
+    float value[C] = {};
+#pragma unroll 8
+    for (int s = warp; s < use; s += kWarps) {
+        const float f = factor[s];
+        const float* x = from + s * (HD + 2);
 #pragma unroll
-    for (int i = 0; i < C; ++i) put(to + lane + 32 * i, sum == 0.0f ? 0.0f : value[i] / sum);
+        for (int i = 0; i < C; ++i) value[i] = fmaf(x[lane + 32 * i], f, value[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < C; ++i) values[warp][lane + 32 * i] = value[i];
+    __syncthreads();
+    T* to = out + token * out_stride + head * HD;
+    if (threadIdx.x < HD) {
+        const int ch = threadIdx.x;
+        const float v = values[0][ch] + values[1][ch] + values[2][ch] + values[3][ch];
+        put(to + ch, sum == 0.0f ? 0.0f : v / sum);
+    }
 }
 
 // Tiles of eight query rows: exact without starts, at most one partial tile a sequence with them.
@@ -700,7 +769,7 @@ int split_count(const Cache& c, const Batch& b, const AttnSpec& a) {
     const int64_t fill = (148 * 4 + units - 1) / std::max<int64_t>(units, 1);
     const int64_t even = (keys + 2047) / 2048;
     const int64_t most = std::max<int64_t>(1, keys / 128);
-    return static_cast<int>(std::min<int64_t>({std::max(fill, even), most, 512}));
+    return static_cast<int>(std::min<int64_t>({std::max(fill, even), most, kMaxSplits}));
 }
 
 }  // namespace
@@ -733,10 +802,7 @@ cudaError_t launch_attention_cached(cudaStream_t s, const Cache& c, const Batch&
                     splits, static_cast<float*>(workspace));
                 e = cudaGetLastError();
                 if (e || splits == 1) return e;
-                const int64_t units = static_cast<int64_t>(b.tokens) * a.heads;
-                return launch_pdl(k_cached_join<T, HD>,
-                                  dim3(static_cast<unsigned>((units + kWarps - 1) / kWarps)),
-                                  dim3(kThreads), 0, s, c, b, a, static_cast<T*>(out), out_stride,
+                return launch_pdl(k_cached_join<T, HD>, dim3(b.tokens, a.heads), dim3(kThreads), 0, s, c, b, a, static_cast<T*>(out), out_stride,
                                   splits, static_cast<const float*>(workspace));
             });
         });

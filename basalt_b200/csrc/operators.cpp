@@ -155,6 +155,12 @@ int check_spec(const bst_attention_spec* a, AttnSpec* out, std::string* why) {
     return BST_OK;
 }
 
+// Positions and keys stay below `keys`: a window that wide hides nothing.
+void limit_window(int keys, AttnSpec* a) {
+    if (a->window >= keys || a->sinks >= keys) a->window = 0;
+    if (a->window == 0) a->sinks = 0;
+}
+
 int check_cached(const bst_kv_cache* cache, const bst_sequences* sequences,
                  const bst_attention_spec* spec, Cache* c, Batch* b, AttnSpec* a,
                  std::string* why) {
@@ -166,6 +172,7 @@ int check_cached(const bst_kv_cache* cache, const bst_sequences* sequences,
         *why = "spec and cache disagree on kv_heads or head_dim";
         return BST_SHAPE;
     }
+    limit_window(c->slots, a);
     if (b->starts && c->storage != BST_DTYPE_U4) {
         *why = "a float32 or bf16 cache takes one token per sequence (starts must be null)";
         return BST_UNSUPPORTED;
@@ -186,6 +193,7 @@ int check_packed(const bst_sequences* sequences, const bst_attention_spec* spec,
         *why = "packed attention takes no rows and no lengths";
         return BST_INVALID;
     }
+    limit_window(b->tokens, a);
     return BST_OK;
 }
 
