@@ -43,7 +43,6 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kBlock = 16;   // keys a warp takes at a time
-constexpr int kRows = 8;     // query rows of a tile
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int STORAGE, int HD>
@@ -51,14 +50,14 @@ struct Layout {
     static constexpr int kGroups = HD / 32;
     static constexpr bool kCodes = STORAGE == BST_DTYPE_U4;
     static constexpr int kRowBytes = kCodes ? HD / 2 : (STORAGE == BST_DTYPE_F32 ? 4 : 2) * HD;
-    static constexpr int kChunks = kRowBytes / 16;
     static constexpr int kScaleBytes = kCodes ? kBlock * kGroups * 4 : 0;
     static constexpr int kStage = 2 * (kBlock * kRowBytes + kScaleBytes);
     // Enough in flight to cover the memory's latency from every SM: 20 to 130 KB a CTA.
     static constexpr int kStages = kStage <= 2560 ? 4 : (kStage <= 8192 ? 3 : 2);
     static constexpr int kRing = kWarps * kStages * kStage;
-    static constexpr int kMerge = kWarps * kRows * (HD + 2) * 4;
-    static constexpr int kSmem = kRing > kMerge ? kRing : kMerge;
+    static constexpr int smem(int rows) {
+        return kRing > kWarps * rows * (HD + 2) * 4 ? kRing : kWarps * rows * (HD + 2) * 4;
+    }
 };
 
 // Where 16-byte chunk `chunk` of key row `row` of a block lies in its row in shared memory, so that
@@ -104,11 +103,21 @@ __device__ __forceinline__ void cp_wait() {
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                          uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
         "{%8, %9}, {%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The same from zero.
+__device__ __forceinline__ void mma_bf16_start(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                               uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -194,22 +203,22 @@ __host__ __device__ __forceinline__ int useful_splits(int blocks, int splits) {
     return most < 1 ? 1 : (most < splits ? most : splits);
 }
 
-// One tile of eight query rows of one key head.
+// One tile of query rows of one key head.
 struct Tile {
     int seq, first, n;   // the sequence, its first packed token and its tokens
     int r0;              // the tile's first query row: row r is token r / group, head r % group
 };
 
-// Tile number `index` of a batch whose sequences have n group rows each, eight to a tile. Without
+// Tile number `index` of a batch whose sequences have n group rows each, tile_rows to a tile. Without
 // starts every sequence has the same number of tiles; with them the tiles before each sequence are
 // summed, 32 sequences at a time.
-__device__ __forceinline__ bool find_tile(const Batch& b, int group, int index, Tile* t) {
+__device__ __forceinline__ bool find_tile(const Batch& b, int group, int tile_rows, int index, Tile* t) {
     if (!b.starts) {
-        const int per = (group + kRows - 1) / kRows;
+        const int per = (group + tile_rows - 1) / tile_rows;
         t->seq = index / per;
         t->first = t->seq;
         t->n = 1;
-        t->r0 = (index - t->seq * per) * kRows;
+        t->r0 = (index - t->seq * per) * tile_rows;
         return t->seq < b.count;
     }
     const int lane = threadIdx.x & 31;
@@ -221,7 +230,7 @@ __device__ __forceinline__ bool find_tile(const Batch& b, int group, int index, 
             from = __ldg(b.starts + s);
             n = max(0, min(__ldg(b.starts + s + 1), b.tokens) - from);
         }
-        const int tiles = (n * group + kRows - 1) / kRows;
+        const int tiles = (n * group + tile_rows - 1) / tile_rows;
         int run = tiles;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -234,7 +243,7 @@ __device__ __forceinline__ bool find_tile(const Batch& b, int group, int index, 
             t->seq = s0 + who;
             t->first = __shfl_sync(kFull, from, who);
             t->n = __shfl_sync(kFull, n, who);
-            t->r0 = (index - before - __shfl_sync(kFull, run - tiles, who)) * kRows;
+            t->r0 = (index - before - __shfl_sync(kFull, run - tiles, who)) * tile_rows;
             return true;
         }
         before += __shfl_sync(kFull, run, 31);
@@ -242,12 +251,64 @@ __device__ __forceinline__ bool find_tile(const Batch& b, int group, int index, 
     return false;
 }
 
-template <typename T, int STORAGE, int HD>
-__global__ void __launch_bounds__(kThreads)
+// CTAs an SM must hold, which caps the registers: measured, more warps beat the few spills.
+template <typename T, int STORAGE, int HD, int ROWS>
+constexpr int min_ctas() {
+    if (STORAGE == BST_DTYPE_F32) return 1;
+    return HD == 128 ? 2 : (HD == 64 ? 4 : 5);
+}
+
+// The A fragment's terms times (b0, b1). With one query row a lane, the tile's rows 8-15 carry the
+// second term of rows 0-7; with two they are queries of their own and every term is a product.
+template <bool START, int R, int N>
+__device__ __forceinline__ void product(float (&c)[4], const uint32_t (&a)[R][2][N], uint32_t b0,
+                                        uint32_t b1) {
+    auto one = [&](bool first, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+        if (START && first) {
+            mma_bf16_start(c, a0, a1, a2, a3, b0, b1);
+        } else {
+            mma_bf16(c, a0, a1, a2, a3, b0, b1);
+        }
+    };
+    if constexpr (R == 2) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) one(i == 0, a[0][0][i], a[1][0][i], a[0][1][i], a[1][1][i]);
+    } else if constexpr (N == 1) {
+        one(true, a[0][0][0], 0u, a[0][1][0], 0u);
+    } else {
+        one(true, a[0][0][0], a[0][0][1], a[0][1][0], a[0][1][1]);
+        if constexpr (N == 3) one(false, a[0][0][2], 0u, a[0][1][2], 0u);
+    }
+}
+// One product with the leading term of every query (and the second where it is free).
+template <int R, int N>
+__device__ __forceinline__ void leading(float (&c)[4], const uint32_t (&a)[R][2][N], uint32_t b0,
+                                        uint32_t b1) {
+    if constexpr (R == 2) {
+        mma_bf16(c, a[0][0][0], a[1][0][0], a[0][1][0], a[1][1][0], b0, b1);
+    } else if constexpr (N == 1) {
+        mma_bf16(c, a[0][0][0], 0u, a[0][1][0], 0u, b0, b1);
+    } else {
+        mma_bf16(c, a[0][0][0], a[0][0][1], a[0][1][0], a[0][1][1], b0, b1);
+    }
+}
+// Column e of such a product for this lane's query row r.
+template <int R, int N>
+__device__ __forceinline__ float entry(const float (&c)[4], int r, int e) {
+    if constexpr (R == 2) return c[2 * r + e];
+    if constexpr (N == 1) return c[e];
+    return c[e] + c[2 + e];
+}
+
+// ROWS queries a tile: 8, or 16 for bf16 batches that have more than eight to a key head, so that
+// unpacking the codes, which bounds the kernel, is shared by twice as many.
+template <typename T, int STORAGE, int HD, int ROWS>
+__global__ void __launch_bounds__(kThreads, min_ctas<T, STORAGE, HD, ROWS>())
 k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride,
          T* __restrict__ out, int64_t out_stride, int splits, float* __restrict__ part) {
     using L = Layout<STORAGE, HD>;
     constexpr int G = L::kGroups;
+    constexpr int R = ROWS / 8;                  // query rows of a lane: g, and g + 8
     constexpr bool kExact = sizeof(T) == 4;      // float32: 24-bit operands
     constexpr int kTerms = kExact ? 3 : 2;       // of the weights
     constexpr int kQ = kExact ? 3 : 1;           // of the queries (a bf16 query is one)
@@ -260,35 +321,103 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
     const int split = blockIdx.z;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     Tile tile;
-    if (!find_tile(b, group, blockIdx.x, &tile)) return;
+    if (!find_tile(b, group, ROWS, blockIdx.x, &tile)) return;
     const int row = b.rows ? __ldg(b.rows + tile.seq) : tile.seq;
     const int length = max(0, __ldg(b.lengths + tile.seq));
-    const int rows = min(kRows, tile.n * group - tile.r0);
+    const int rows = min(ROWS, tile.n * group - tile.r0);
     // Positions of the tile's tokens; a row or slot outside the cache sees nothing.
     const bool inside = row >= 0 && row < c.rows;
-    const int p_first = length - tile.n + tile.r0 / group;
-    const int p_last = length - tile.n + (tile.r0 + rows - 1) / group;
+    // A sequence's only token, or token row / group of several.
+    const int first_token = tile.n == 1 ? 0 : tile.r0 / group;
+    const int last_token = tile.n == 1 ? 0 : (tile.r0 + rows - 1) / group;
+    const int p_first = length - tile.n + first_token, p_last = length - tile.n + last_token;
     const Visible seen(p_first, inside ? p_last : -1, c.slots, a.window, a.sinks);
     const int use = useful_splits(seen.blocks, splits);
     if (split >= use) return;
     const int b0 = static_cast<int>(static_cast<int64_t>(seen.blocks) * split / use);
     const int b1 = static_cast<int>(static_cast<int64_t>(seen.blocks) * (split + 1) / use);
 
-    const int my_row = tile.r0 + g;
-    const bool live = g < rows;
-    int position = length - tile.n + my_row / group;
-    if (!live || !inside || position >= c.slots) position = -1;
-    const float to_log2 = a.scale * kLog2e;
+    const int64_t at = (static_cast<int64_t>(inside ? row : 0) * c.kv_heads + kvh) * c.slots;
+    const char* kb = static_cast<const char*>(c.k) + at * L::kRowBytes;
+    const char* vb = static_cast<const char*>(c.v) + at * L::kRowBytes;
+    const char* ksb = static_cast<const char*>(c.k_scale) + at * (G * 4);
+    const char* vsb = static_cast<const char*>(c.v_scale) + at * (G * 4);
+    const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) +
+                          warp * L::kStages * L::kStage;
+    // A block is contiguous in its source: chunk i of this lane lies 512 i bytes after chunk 0.
+    const int lane_row = lane / (L::kRowBytes / 16), lane_chunk = lane % (L::kRowBytes / 16);
+    constexpr int kHalf = kBlock * L::kRowBytes;          // bytes of a block's keys
+    constexpr int kLoads = kHalf / 512 ? kHalf / 512 : 1;  // of each lane, for the keys
+    auto lane_to = [&](int i) {
+        const int r = lane_row + i * (512 / L::kRowBytes);
+        return r * L::kRowBytes + swizzled<STORAGE, HD>(r, lane_chunk) * 16;
+    };
+    // Rows of 16 bytes: sixteen lanes take the keys, sixteen the values.
+    constexpr bool kShared = kHalf < 512;
+    const char* const k_lane = (kShared && lane >= 16 ? vb - kHalf : kb) + lane * 16;
+    const char* const v_lane = vb + lane * 16;
+    const char* const s_lane = (lane >= 16 ? vsb : ksb) + (lane & 15) * (G * 4);
+    auto fetch = [&](int block, int stage) {
+        if (block < b1) {
+            const int key0 = seen.key(block);
+            const uint32_t dst = ring + stage * L::kStage;
+            const char* const ks = k_lane + static_cast<int64_t>(key0) * L::kRowBytes;
+            const char* const vs = v_lane + static_cast<int64_t>(key0) * L::kRowBytes;
+            const char* const ss = s_lane + static_cast<int64_t>(key0) * (G * 4);
+            const uint32_t scale_to = dst + 2 * kHalf + lane * (G * 4);
+            if (seen.whole(key0)) {
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) cp_async16(dst + lane_to(i), ks + 512 * i, 16);
+                if constexpr (!kShared) {
+#pragma unroll
+                    for (int i = 0; i < kLoads; ++i) {
+                        cp_async16(dst + kHalf + lane_to(i), vs + 512 * i, 16);
+                    }
+                }
+                if constexpr (L::kCodes) cp_async_small<G * 4>(scale_to, ss, G * 4);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) {
+                    const int r = lane_row + i * (512 / L::kRowBytes);
+                    const bool ok = seen.holds(key0 + (kShared ? r & 15 : r));
+                    cp_async16(dst + lane_to(i), ok ? ks + 512 * i : kb, ok ? 16 : 0);
+                    if constexpr (!kShared) {
+                        cp_async16(dst + kHalf + lane_to(i), ok ? vs + 512 * i : vb, ok ? 16 : 0);
+                    }
+                }
+                if constexpr (L::kCodes) {
+                    const bool ok = seen.holds(key0 + (lane & 15));
+                    cp_async_small<G * 4>(scale_to, ok ? ss : ksb, ok ? G * 4 : 0);
+                }
+            }
+        }
+        cp_commit();
+    };
+    int next = b0 + warp;
+#pragma unroll
+    for (int i = 0; i < L::kStages - 1; ++i) {
+        fetch(next, i);
+        next += kWarps;
+    }
 
     // This lane's part of the queries as A fragments: product m of group gr takes, for 4-bit
     // keys, channels 8 t + {2 m, 2 m + 4} and {2 m + 1, 2 m + 5} (the order in which nibbles
     // unpack, the second pair 16 times too large), otherwise 8 t + 4 m + {0, 1} and {2, 3}.
-    // to_score takes a product to the base-2 logarithm of its weight.
-    uint32_t qa[kMma][2][kQ];
-    float qsum[G], to_score = a.scale * kLog2e;
-    {
-        const int token = tile.first + my_row / group;
-        const T* src = q + token * q_stride + (kvh * group + my_row % group) * HD + 8 * t;
+    // to_score takes a product to the base-2 logarithm of its weight. With codes, one more product
+    // (qs) of the groups' query sums and the keys' lows completes a score.
+    uint32_t qa[kMma][R][2][kQ], qs[R][2][kTerms] = {};
+    float to_score[R];
+    int position[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int my_row = tile.r0 + g + 8 * r;
+        const bool live = g + 8 * r < rows;
+        const int my_token = tile.n == 1 ? 0 : my_row / group;
+        position[r] = length - tile.n + my_token;
+        if (!live || !inside || position[r] >= c.slots) position[r] = -1;
+        to_score[r] = a.scale * kLog2e;
+        const int64_t token = tile.first + my_token;
+        const T* src = q + token * q_stride + (kvh * group + my_row - my_token * group) * HD + 8 * t;
         float x[G][8], largest = 0.0f;
 #pragma unroll
         for (int gr = 0; gr < G; ++gr) {
@@ -304,120 +433,104 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
             largest = fmaxf(largest, __shfl_xor_sync(kFull, largest, 2));
             const int e = max(min(ilogbf(fmaxf(largest, FLT_MIN)), 126) + 1, -100);
             const float shrink = exp2f(static_cast<float>(-e));
-            to_score *= exp2f(static_cast<float>(e));
-            to_score *= 64.0f;
+            to_score[r] *= exp2f(static_cast<float>(e));
+            to_score[r] *= 64.0f;
+            float mine[2] = {0.0f, 0.0f};  // sums of groups 2 t and 2 t + 1
 #pragma unroll
             for (int gr = 0; gr < G; ++gr) {
+                float sum = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[gr][i] *= shrink;
+                for (int i = 0; i < 8; ++i) sum += x[gr][i] *= shrink;
+                sum += __shfl_xor_sync(kFull, sum, 1);
+                sum += __shfl_xor_sync(kFull, sum, 2);
+                if (t == gr / 2) mine[gr & 1] = sum * 0.015625f;
             }
+            terms_of<kTerms>(mine[0], mine[1], qs[r][0]);
         }
 #pragma unroll
         for (int gr = 0; gr < G; ++gr) {
-            float sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sum += x[gr][i];
-            sum += __shfl_xor_sync(kFull, sum, 1);
-            sum += __shfl_xor_sync(kFull, sum, 2);
-            qsum[gr] = sum * 0.015625f;
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
                 if constexpr (L::kCodes) {
                     terms_of<kQ>(x[gr][2 * m] * 0x1p127f, x[gr][2 * m + 4] * 0x1p127f,
-                                 qa[2 * gr + m][0]);
+                                 qa[2 * gr + m][r][0]);
                     terms_of<kQ>(x[gr][2 * m + 1] * 0x1p123f, x[gr][2 * m + 5] * 0x1p123f,
-                                 qa[2 * gr + m][1]);
+                                 qa[2 * gr + m][r][1]);
                 } else {
-                    terms_of<kQ>(x[gr][4 * m], x[gr][4 * m + 1], qa[2 * gr + m][0]);
-                    terms_of<kQ>(x[gr][4 * m + 2], x[gr][4 * m + 3], qa[2 * gr + m][1]);
+                    terms_of<kQ>(x[gr][4 * m], x[gr][4 * m + 1], qa[2 * gr + m][r][0]);
+                    terms_of<kQ>(x[gr][4 * m + 2], x[gr][4 * m + 3], qa[2 * gr + m][r][1]);
                 }
             }
         }
     }
 
-    const int64_t at = (static_cast<int64_t>(inside ? row : 0) * c.kv_heads + kvh) * c.slots;
-    const char* kb = static_cast<const char*>(c.k) + at * L::kRowBytes;
-    const char* vb = static_cast<const char*>(c.v) + at * L::kRowBytes;
-    const char* ksb = static_cast<const char*>(c.k_scale) + at * (G * 4);
-    const char* vsb = static_cast<const char*>(c.v_scale) + at * (G * 4);
-    const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) +
-                          warp * L::kStages * L::kStage;
-    // This lane's chunks of a block: row and byte offsets, in its source and in a stage.
-    int from_row[L::kChunks], from[L::kChunks], to[L::kChunks];
-#pragma unroll
-    for (int i = 0; i < L::kChunks; ++i) {
-        const int index = lane + 32 * i;
-        const int half = index / (kBlock * L::kChunks), rest = index % (kBlock * L::kChunks);
-        const int r = rest / L::kChunks, chunk = rest % L::kChunks;
-        from_row[i] = r;
-        from[i] = r * L::kRowBytes + chunk * 16;
-        to[i] = half * (kBlock * L::kRowBytes) + r * L::kRowBytes + swizzled<STORAGE, HD>(r, chunk) * 16;
-    }
-    // Chunk i lies in the keys or in the values: by the lane where a row is one chunk.
-    const char* const first_base = L::kChunks == 1 && lane >= 16 ? vb : kb;
-    const char* const scale_base = (lane >= 16 ? vsb : ksb) + (lane & 15) * (G * 4);
-    auto fetch = [&](int block, int stage) {
-        if (block < b1) {
-            const int key0 = seen.key(block);
-            const uint32_t dst = ring + stage * L::kStage;
-            const int64_t bytes = static_cast<int64_t>(key0) * L::kRowBytes;
-            const bool whole = seen.whole(key0);
-#pragma unroll
-            for (int i = 0; i < L::kChunks; ++i) {
-                const char* src = (L::kChunks == 1 ? first_base : (i < L::kChunks / 2 ? kb : vb));
-                const bool ok = whole || seen.holds(key0 + from_row[i]);
-                cp_async16(dst + to[i], src + (ok ? bytes + from[i] : 0), ok ? 16 : 0);
-            }
-            if constexpr (L::kCodes) {
-                const bool ok = whole || seen.holds(key0 + (lane & 15));
-                const char* src = ok ? scale_base + static_cast<int64_t>(key0) * (G * 4) : ksb;
-                cp_async_small<G * 4>(dst + 2 * kBlock * L::kRowBytes + lane * (G * 4), src,
-                                      ok ? G * 4 : 0);
-            }
-        }
-        cp_commit();
-    };
-
-    float o[G * 4][4], low_sum[G], top = -INFINITY, total = 0.0f;
+    // Output columns, and with codes the sums over keys of weight x (step, low) of group t.
+    float o[G * 4][4], scales[4] = {}, top[R], total[R];
+    unsigned poison[R];  // groups in which a key that the query sees holds a NaN
 #pragma unroll
     for (int i = 0; i < G * 4; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
 #pragma unroll
-    for (int i = 0; i < G; ++i) low_sum[i] = 0.0f;
-
-    int next = b0 + warp;
-#pragma unroll
-    for (int i = 0; i < L::kStages - 1; ++i) {
-        fetch(next, i);
-        next += kWarps;
+    for (int r = 0; r < R; ++r) {
+        top[r] = -INFINITY;
+        total[r] = 0.0f;
+        poison[r] = 0u;
     }
+    // The key rows of this lane's score columns 2 t and 2 t + 1, and of the key that it loads.
+    const int key_row[2] = {row_of_column<STORAGE, HD>(2 * t), row_of_column<STORAGE, HD>(2 * t + 1)};
+    const int load_row = row_of_column<STORAGE, HD>(g);
+    // Offsets of this lane's reads in a stage, for the first eight keys (the other eight follow at
+    // eight rows' distance, which the swizzle does not look at): its keys' codes, the lows of groups
+    // 2 t and 2 t + 1, the scales of its score columns, its entries of the values.
+    int k_at = 0, lows_at = 0, scale_at[2] = {}, v_at[2] = {};
+    if constexpr (L::kCodes) {
+        k_at = load_row * L::kRowBytes + swizzled<STORAGE, HD>(load_row, t * 4 * G / 16) * 16 + t * 4 * G % 16;
+        lows_at = 2 * kHalf + load_row * (G * 4) + (2 * t < G ? t * 8 : 0);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            scale_at[e] = 2 * kHalf + key_row[e] * (G * 4);
+            v_at[e] = kHalf + key_row[e] * L::kRowBytes +
+                      swizzled<STORAGE, HD>(key_row[e], g * 2 * G / 16) * 16 + g * 2 * G % 16;
+        }
+    }
+
     int stage = 0;
     for (int block = b0 + warp; block < b1; block += kWarps) {
         cp_wait<L::kStages - 2>();
         __syncwarp();
         const uint32_t ks = ring + stage * L::kStage;
-        const uint32_t vs = ks + kBlock * L::kRowBytes;
-        const uint32_t kss = ks + 2 * kBlock * L::kRowBytes, vss = kss + L::kScaleBytes;
+        const uint32_t vs = ks + kHalf;
+        const uint32_t vss = ks + 2 * kHalf + L::kScaleBytes;
         const int key0 = seen.key(block);
 
-        // Scores of keys key0 + 8 nb + row_of_column(2 t + e), this lane's query row.
-        float s[2][2];
-        int key_row[2];
-        key_row[0] = row_of_column<STORAGE, HD>(2 * t);
-        key_row[1] = row_of_column<STORAGE, HD>(2 * t + 1);
+        // Scores of keys key0 + 8 nb + key_row[e].
+        float s[R][2][2];
 #pragma unroll
         for (int nb = 0; nb < 2; ++nb) {
-            const int r = 8 * nb + row_of_column<STORAGE, HD>(g);  // the key this lane loads
+            const int lr = 8 * nb + load_row;
             if constexpr (L::kCodes) {
                 // Bytes [t * 4 G, ...) of the row: half 2 t of every group, then half 2 t + 1.
-                uint32_t w[G];
-                {
-                    const int chunk = t * 4 * G / 16, rest = t * 4 * G % 16;
-                    load_words<G>(ks + r * L::kRowBytes + swizzled<STORAGE, HD>(r, chunk) * 16 + rest, w);
+                uint32_t w[G], sa[G], sb[G];
+                load_words<G>(ks + k_at + nb * 8 * L::kRowBytes, w);
+                load_words<G>(ks + scale_at[0] + nb * 8 * (G * 4), sa);  // (step, low) of the two
+                load_words<G>(ks + scale_at[1] + nb * 8 * (G * 4), sb);  // keys this lane scores
+                uint32_t lows;
+                if constexpr (G == 1) {
+                    uint32_t w1[1];
+                    load_words<1>(ks + lows_at + nb * 8 * (G * 4), w1);
+                    lows = w1[0] >> 16;
+                } else {
+                    uint32_t w2[2];
+                    load_words<2>(ks + lows_at + nb * 8 * (G * 4), w2);
+                    lows = __byte_perm(w2[0], w2[1], 0x7632);
                 }
-                uint32_t sa[G], sb[G];  // (step, low) of the two keys this lane scores
-                load_words<G>(kss + (8 * nb + key_row[0]) * (G * 4), sa);
-                load_words<G>(kss + (8 * nb + key_row[1]) * (G * 4), sb);
-                s[nb][0] = s[nb][1] = 0.0f;
+                if (2 * t >= G) lows = 0u;
+                float low[4];
+                product<true>(low, qs, lows, 0u);
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    s[r][nb][0] = entry<R, kTerms>(low, r, 0);
+                    s[r][nb][1] = entry<R, kTerms>(low, r, 1);
+                }
 #pragma unroll
                 for (int gr = 0; gr < G; ++gr) {
                     uint32_t x;
@@ -427,172 +540,181 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
                         // 16-bit entries gr and G + gr of the lane's 2 G.
                         x = __byte_perm(w[gr / 2], w[G / 2 + gr / 2], gr & 1 ? 0x7632 : 0x5410);
                     }
-                    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int m = 0; m < 2; ++m) {
-                        const uint32_t y = m ? __umulhi(x, 1u << 24) : x;  // x >> 8
-                        const uint32_t k0 = y & 0x000f000fu, k1 = y & 0x00f000f0u;
-                        uint32_t(&A)[2][kQ] = qa[2 * gr + m];
-                        if constexpr (kExact) {
-                            mma_bf16(acc, A[0][0], A[0][1], A[1][0], A[1][1], k0, k1);
-                            mma_bf16(acc, A[0][2], 0u, A[1][2], 0u, k0, k1);
-                        } else {
-                            mma_bf16(acc, A[0][0], 0u, A[1][0], 0u, k0, k1);
-                        }
-                    }
-                    const float pa = kExact ? acc[0] + acc[2] : acc[0];
-                    const float pb = kExact ? acc[1] + acc[3] : acc[1];
+                    float acc[4];
+                    product<true>(acc, qa[2 * gr], x & 0x000f000fu, x & 0x00f000f0u);
+                    x = __umulhi(x, 1u << 24);  // x >> 8
+                    product<false>(acc, qa[2 * gr + 1], x & 0x000f000fu, x & 0x00f000f0u);
                     const float step_a = low_of(sa[gr]), step_b = low_of(sb[gr]);
-                    const float low_a = high_of(sa[gr]), low_b = high_of(sb[gr]);
-                    s[nb][0] = fmaf(step_a, pa, fmaf(low_a, qsum[gr], s[nb][0]));
-                    s[nb][1] = fmaf(step_b, pb, fmaf(low_b, qsum[gr], s[nb][1]));
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        s[r][nb][0] = fmaf(step_a, entry<R, kQ>(acc, r, 0), s[r][nb][0]);
+                        s[r][nb][1] = fmaf(step_b, entry<R, kQ>(acc, r, 1), s[r][nb][1]);
+                    }
                 }
             } else {
-                float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                float acc[4] = {};
 #pragma unroll
                 for (int gr = 0; gr < G; ++gr) {
                     uint32_t kw[4][kK];  // channels 8 t .. 8 t + 7 of the group, in pairs
                     if constexpr (STORAGE == BST_DTYPE_BF16) {
                         uint32_t w[4];
-                        load_words<4>(ks + r * L::kRowBytes + swizzled<STORAGE, HD>(r, 4 * gr + t) * 16, w);
+                        load_words<4>(ks + lr * L::kRowBytes + swizzled<STORAGE, HD>(lr, 4 * gr + t) * 16, w);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) kw[i][0] = w[i];
                     } else {
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             uint32_t w[4];
-                            load_words<4>(ks + r * L::kRowBytes +
-                                              swizzled<STORAGE, HD>(r, 8 * gr + 2 * t + h) * 16, w);
+                            load_words<4>(ks + lr * L::kRowBytes +
+                                              swizzled<STORAGE, HD>(lr, 8 * gr + 2 * t + h) * 16, w);
                             terms_of<kK>(__uint_as_float(w[0]), __uint_as_float(w[1]), kw[2 * h]);
                             terms_of<kK>(__uint_as_float(w[2]), __uint_as_float(w[3]), kw[2 * h + 1]);
                         }
                     }
 #pragma unroll
                     for (int m = 0; m < 2; ++m) {
-                        uint32_t(&A)[2][kQ] = qa[2 * gr + m];
+                        // All of the query's terms with the key's first, its leading ones with the
+                        // others.
+                        product<false>(acc, qa[2 * gr + m], kw[2 * m][0], kw[2 * m + 1][0]);
 #pragma unroll
-                        for (int i = 0; i < kK; ++i) {
-                            if constexpr (kExact) {
-                                mma_bf16(acc, A[0][0], A[0][1], A[1][0], A[1][1], kw[2 * m][i],
-                                         kw[2 * m + 1][i]);
-                            } else {
-                                mma_bf16(acc, A[0][0], 0u, A[1][0], 0u, kw[2 * m][i],
-                                         kw[2 * m + 1][i]);
-                            }
-                        }
-                        if constexpr (kExact) {
-                            mma_bf16(acc, A[0][2], 0u, A[1][2], 0u, kw[2 * m][0], kw[2 * m + 1][0]);
+                        for (int i = 1; i < kK; ++i) {
+                            leading<R, kQ>(acc, qa[2 * gr + m], kw[2 * m][i], kw[2 * m + 1][i]);
                         }
                     }
                 }
-                s[nb][0] = kExact ? acc[0] + acc[2] : acc[0];
-                s[nb][1] = kExact ? acc[1] + acc[3] : acc[1];
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    s[r][nb][0] = entry<R, kQ>(acc, r, 0);
+                    s[r][nb][1] = entry<R, kQ>(acc, r, 1);
+                }
             }
         }
         // Mask, running maximum. Every query of the tile sees all of a block in the middle.
         const bool all = key0 + kBlock - 1 <= p_first && p_last < c.slots &&
                          (a.window == 0 || p_last - key0 < a.window || key0 + kBlock <= a.sinks);
-        bool hidden[2][2] = {};
-        float block_top = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[r][i / 2][i % 2] *= to_score[r];
+        }
         if (!all) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int key_at = 8 * (i / 2) + key_row[i % 2], key = key0 + key_at;
+                // A NaN that some query does not see is taken out of the products below; the
+                // queries that see it remember.
+                unsigned bad = 0u;
+                if constexpr (L::kCodes) {
+                    uint32_t w[G];
+                    load_words<G>(vss + key_at * (G * 4), w);
+#pragma unroll
+                    for (int gr = 0; gr < G; ++gr) {
+                        bad |= (w[gr] & 0x7f800000u) == 0x7f800000u ? 1u << gr : 0u;
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    if (key > position[r] || (a.window != 0 && position[r] - key >= a.window &&
+                                              key >= a.sinks)) {
+                        s[r][i / 2][i % 2] = -INFINITY;
+                    } else {
+                        poison[r] |= bad;
+                    }
+                }
+            }
+        }
+        bool grows = false;
+        float keep[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float block_top = fmaxf(fmaxf(s[r][0][0], s[r][0][1]), fmaxf(s[r][1][0], s[r][1][1]));
+            block_top = fmaxf(block_top, __shfl_xor_sync(kFull, block_top, 1));
+            block_top = fmaxf(block_top, __shfl_xor_sync(kFull, block_top, 2));
+            const bool up = block_top > top[r];
+            keep[r] = up ? (top[r] == -INFINITY ? 0.0f : exp2_fast(top[r] - block_top)) : 1.0f;
+            top[r] = up ? block_top : top[r];
+            grows |= up;
+        }
+        if (__any_sync(kFull, grows)) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) total[r] *= keep[r];
+            // Columns 2 and 3 are row g + 8: of the same query, or of the second.
+#pragma unroll
+            for (int j = 0; j < 4; ++j) scales[j] *= keep[R == 2 ? j / 2 : 0];
+#pragma unroll
+            for (int i = 0; i < G * 4; ++i) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[i][j] *= keep[R == 2 ? j / 2 : 0];
+            }
+        }
+        float p[R][2][2];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const float base = top[r] == -INFINITY ? 0.0f : top[r];
 #pragma unroll
             for (int nb = 0; nb < 2; ++nb) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const int key = key0 + 8 * nb + key_row[e];
-                    hidden[nb][e] = key > position || (a.window != 0 && position - key >= a.window &&
-                                                       key >= a.sinks);
+                    p[r][nb][e] = exp2_fast(s[r][nb][e] - base);
+                    total[r] += p[r][nb][e];
                 }
-            }
-        }
-#pragma unroll
-        for (int nb = 0; nb < 2; ++nb) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                s[nb][e] = hidden[nb][e] ? -INFINITY : s[nb][e] * to_score;
-                block_top = fmaxf(block_top, s[nb][e]);
-            }
-        }
-        block_top = fmaxf(block_top, __shfl_xor_sync(kFull, block_top, 1));
-        block_top = fmaxf(block_top, __shfl_xor_sync(kFull, block_top, 2));
-        const bool grows = block_top > top;
-        if (__any_sync(kFull, grows)) {
-            const float keep = grows ? (top == -INFINITY ? 0.0f : exp2_fast(top - block_top)) : 1.0f;
-            top = grows ? block_top : top;
-            total *= keep;
-#pragma unroll
-            for (int i = 0; i < G; ++i) low_sum[i] *= keep;
-#pragma unroll
-            for (int i = 0; i < G * 4; ++i) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) o[i][j] *= keep;
-            }
-        }
-        const float base = top == -INFINITY ? 0.0f : top;
-        float p[2][2];
-#pragma unroll
-        for (int nb = 0; nb < 2; ++nb) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                p[nb][e] = exp2_fast(s[nb][e] - base);
-                total += p[nb][e];
             }
         }
 
         // Weights times values.
+        uint32_t pa[R][2][kTerms];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            terms_of<kTerms>(p[r][0][0], p[r][0][1], pa[r][0]);
+            terms_of<kTerms>(p[r][1][0], p[r][1][1], pa[r][1]);
+        }
         if constexpr (L::kCodes) {
             uint32_t sv[2][2][G];
             uint32_t wv[2][2][(G + 1) / 2];
+            uint16_t column[2][2];  // entry g of the keys' (step, low) pairs
 #pragma unroll
             for (int nb = 0; nb < 2; ++nb) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const int r = 8 * nb + key_row[e];
-                    load_words<G>(vss + r * (G * 4), sv[nb][e]);
-                    if (hidden[nb][e]) {
-                        // Its low may be a NaN that another query sees.
-#pragma unroll
-                        for (int gr = 0; gr < G; ++gr) sv[nb][e][gr] = 0u;
-                    }
+                    load_words<G>(ks + scale_at[e] + L::kScaleBytes + nb * 8 * (G * 4), sv[nb][e]);
+                    asm volatile("ld.shared.u16 %0, [%1];"
+                                 : "=h"(column[nb][e])
+                                 : "r"(ks + scale_at[e] + L::kScaleBytes + nb * 8 * (G * 4) +
+                                       (g & (2 * G - 1)) * 2));
+                    if (G < 4 && g >= 2 * G) column[nb][e] = 0;
+                    if (!all && (column[nb][e] & 0x7f80u) == 0x7f80u) column[nb][e] = 0;
                     // 16-bit entries [g][0 .. G): nibble j is channel 4 g + j of a group.
+                    const uint32_t va = ks + v_at[e] + nb * 8 * L::kRowBytes;
                     if constexpr (G == 1) {
                         uint16_t h;
-                        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(vs + r * L::kRowBytes + g * 2));
+                        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(va));
                         wv[nb][e][0] = h;
                     } else {
-                        const int chunk = g * 2 * G / 16, rest = g * 2 * G % 16;
-                        load_words<G / 2>(vs + r * L::kRowBytes + swizzled<STORAGE, HD>(r, chunk) * 16 + rest,
-                                          wv[nb][e]);
+                        load_words<G / 2>(va, wv[nb][e]);
                     }
                 }
             }
+            product<false>(scales, pa, __byte_perm(column[0][0], column[0][1], 0x5410),
+                               __byte_perm(column[1][0], column[1][1], 0x5410));
 #pragma unroll
             for (int gr = 0; gr < G; ++gr) {
-                uint32_t pa[2][kTerms], x[2];
+                uint32_t ps[R][2][kTerms], x[2];
 #pragma unroll
                 for (int nb = 0; nb < 2; ++nb) {
                     const float step0 = low_of(sv[nb][0][gr]), step1 = low_of(sv[nb][1][gr]);
-                    float low0 = high_of(sv[nb][0][gr]), low1 = high_of(sv[nb][1][gr]);
-                    if constexpr (!kExact) {
-                        low0 = fmaf(-128.0f, step0, low0);
-                        low1 = fmaf(-128.0f, step1, low1);
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        terms_of<kTerms>(p[r][nb][0] * step0, p[r][nb][1] * step1, ps[r][nb]);
                     }
-                    low_sum[gr] = fmaf(p[nb][0], low0, low_sum[gr]);
-                    low_sum[gr] = fmaf(p[nb][1], low1, low_sum[gr]);
-                    terms_of<kTerms>(p[nb][0] * step0, p[nb][1] * step1, pa[nb]);
                     x[nb] = __byte_perm(wv[nb][0][gr / 2], wv[nb][1][gr / 2], gr & 1 ? 0x7632 : 0x5410);
                 }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const uint32_t v0 = nibbles<!kExact>(x[0], j), v1 = nibbles<!kExact>(x[1], j);
-                    mma_bf16(o[4 * gr + j], pa[0][0], pa[0][1], pa[1][0], pa[1][1], v0, v1);
-                    if constexpr (kExact) mma_bf16(o[4 * gr + j], pa[0][2], 0u, pa[1][2], 0u, v0, v1);
+                    product<false>(o[4 * gr + j], ps, nibbles<!kExact>(x[0], j),
+                                       nibbles<!kExact>(x[1], j));
                 }
             }
         } else {
-            uint32_t pa[2][kTerms];
-            terms_of<kTerms>(p[0][0], p[0][1], pa[0]);
-            terms_of<kTerms>(p[1][0], p[1][1], pa[1]);
 #pragma unroll
             for (int j = 0; j < G * 4; ++j) {  // channels 8 j .. 8 j + 7, column n of them at lane n = g
                 uint32_t v0[kK], v1[kK];
@@ -616,11 +738,11 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
                     terms_of<kK>(v[0], v[1], v0);
                     terms_of<kK>(v[2], v[3], v1);
                 }
+                product<false>(o[j], pa, v0[0], v1[0]);
 #pragma unroll
-                for (int i = 0; i < kK; ++i) {
-                    mma_bf16(o[j], pa[0][0], pa[0][1], pa[1][0], pa[1][1], v0[i], v1[i]);
+                for (int i = 1; i < kK; ++i) {
+                    leading<R, kTerms>(o[j], pa, v0[i], v1[i]);
                 }
-                if constexpr (kExact) mma_bf16(o[j], pa[0][2], 0u, pa[1][2], 0u, v0[0], v1[0]);
             }
         }
         __syncwarp();
@@ -632,48 +754,59 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
     __syncthreads();  // the rings become the merge buffer
 
     // The warps' results: [warp][row][HD outputs, maximum, sum].
-    total += __shfl_xor_sync(kFull, total, 1);
-    total += __shfl_xor_sync(kFull, total, 2);
     float* merge = reinterpret_cast<float*>(smem);
-    float* mine = merge + (warp * kRows + g) * (HD + 2);
 #pragma unroll
-    for (int gr = 0; gr < G; ++gr) {
-        float low = low_sum[gr];
+    for (int r = 0; r < R; ++r) {
+        total[r] += __shfl_xor_sync(kFull, total[r], 1);
+        total[r] += __shfl_xor_sync(kFull, total[r], 2);
         if constexpr (L::kCodes) {
-            low += __shfl_xor_sync(kFull, low, 1);
-            low += __shfl_xor_sync(kFull, low, 2);
+            poison[r] |= __shfl_xor_sync(kFull, poison[r], 1);
+            poison[r] |= __shfl_xor_sync(kFull, poison[r], 2);
         }
+        float* mine = merge + (warp * ROWS + g + 8 * r) * (HD + 2);
+        // What the codes of group t stand above: its lows, less the 128 that the codes carry.
+        const float step_sum = entry<R, kTerms>(scales, r, 0), low_sum = entry<R, kTerms>(scales, r, 1);
+        const float below = kExact ? low_sum : fmaf(-128.0f, step_sum, low_sum);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float(&x)[4] = o[4 * gr + j];
-            // Columns 2 t and 2 t + 1: channels 4 n + j of the group (codes) or 8 j + n.
-            const int c0 = L::kCodes ? 32 * gr + 8 * t + j : 32 * gr + 8 * j + 2 * t;
-            mine[c0] = x[0] + x[2] + low;
-            mine[c0 + (L::kCodes ? 4 : 1)] = x[1] + x[3] + low;
+        for (int gr = 0; gr < G; ++gr) {
+            float low = 0.0f;
+            if constexpr (L::kCodes) {
+                low = __shfl_sync(kFull, below, (lane & ~3) | gr);
+                if ((poison[r] >> gr) & 1u) low = NAN;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                // Columns 2 t and 2 t + 1: channels 4 n + j of the group (codes) or 8 j + n.
+                const int c0 = L::kCodes ? 32 * gr + 8 * t + j : 32 * gr + 8 * j + 2 * t;
+                mine[c0] = entry<R, kTerms>(o[4 * gr + j], r, 0) + low;
+                mine[c0 + (L::kCodes ? 4 : 1)] = entry<R, kTerms>(o[4 * gr + j], r, 1) + low;
+            }
         }
-    }
-    if (t == 0) {
-        mine[HD] = top;
-        mine[HD + 1] = total;
+        if (t == 0) {
+            mine[HD] = top[r];
+            mine[HD + 1] = total[r];
+        }
     }
     __syncthreads();
     for (int i = threadIdx.x; i < rows * HD; i += kThreads) {
         const int r = i / HD, ch = i % HD;
         float m = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, merge[(w * kRows + r) * (HD + 2) + HD]);
+        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, merge[(w * ROWS + r) * (HD + 2) + HD]);
         float sum = 0.0f, value = 0.0f;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-            const float* from = merge + (w * kRows + r) * (HD + 2);
+            const float* from = merge + (w * ROWS + r) * (HD + 2);
             const float f = from[HD] == -INFINITY ? 0.0f : exp2_fast(from[HD] - m);
-            sum = fmaf(from[HD + 1], f, sum);
             // A warp that saw no key has nothing to add, not even zero times its output.
-            if (from[HD] != -INFINITY || from[HD + 1] != 0.0f) value = fmaf(from[ch], f, value);
+            if (from[HD] != -INFINITY || from[HD + 1] != 0.0f) {
+                sum = fmaf(from[HD + 1], f, sum);
+                value = fmaf(from[ch], f, value);
+            }
         }
-        const int query = tile.r0 + r;
-        const int64_t token = tile.first + query / group;
-        const int head = kvh * group + query % group;
+        const int query = tile.r0 + r, my_token = tile.n == 1 ? 0 : query / group;
+        const int64_t token = tile.first + my_token;
+        const int head = kvh * group + query - my_token * group;
         if (splits == 1) {
             put(out + token * out_stride + head * HD + ch, sum == 0.0f ? 0.0f : value / sum);
         } else {
@@ -693,8 +826,8 @@ constexpr int kMaxSplits = 512;
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads)
-k_cached_join(Cache c, Batch b, AttnSpec a, T* __restrict__ out, int64_t out_stride, int splits,
-              const float* __restrict__ part) {
+k_cached_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out,
+              int64_t out_stride, int splits, const float* __restrict__ part) {
     constexpr int C = HD / 32;
     __shared__ float factor[kMaxSplits], tops[kWarps], sums[kWarps], values[kWarps][HD];
     const int token = blockIdx.x, head = blockIdx.y;
@@ -706,8 +839,8 @@ k_cached_join(Cache c, Batch b, AttnSpec a, T* __restrict__ out, int64_t out_str
     const int group = a.heads / a.kv_heads;
     const int row = b.rows ? __ldg(b.rows + seq) : seq;
     const int length = max(0, __ldg(b.lengths + seq));
-    const int r0 = ((token - first) * group + head % group) / kRows * kRows;
-    const int rows = min(kRows, n * group - r0);
+    const int r0 = ((token - first) * group + head % group) / tile_rows * tile_rows;
+    const int rows = min(tile_rows, n * group - r0);
     const int p_last = row >= 0 && row < c.rows ? length - n + (r0 + rows - 1) / group : -1;
     const Visible seen(length - n + r0 / group, p_last, c.slots, a.window, a.sinks);
     const int use = useful_splits(seen.blocks, splits);
@@ -751,11 +884,18 @@ k_cached_join(Cache c, Batch b, AttnSpec a, T* __restrict__ out, int64_t out_str
     }
 }
 
-// Tiles of eight query rows: exact without starts, at most one partial tile a sequence with them.
-int tile_bound(const Batch& b, const AttnSpec& a) {
+// Query rows a tile: 16 where bf16 sequences have more than eight to a key head on average. For
+// four tokens of four heads that took a step over 24 caches of up to 16 384 keys from 330 to @@ us.
+int rows_of_tile(const Batch& b, const AttnSpec& a) {
     const int64_t group = a.heads / a.kv_heads;
-    if (!b.starts) return static_cast<int>(b.count * ((group + kRows - 1) / kRows));
-    return static_cast<int>(std::min<int64_t>((b.tokens * group) / kRows + b.count, b.tokens * group));
+    return a.dtype == BST_DTYPE_BF16 && b.tokens * group > 8ll * b.count ? 16 : 8;
+}
+
+// Tiles: exact without starts, at most one partial tile a sequence with them.
+int tile_bound(const Batch& b, const AttnSpec& a) {
+    const int64_t group = a.heads / a.kv_heads, rows = rows_of_tile(b, a);
+    if (!b.starts) return static_cast<int>(b.count * ((group + rows - 1) / rows));
+    return static_cast<int>(std::min<int64_t>((b.tokens * group) / rows + b.count, b.tokens * group));
 }
 
 // CTAs for about four on every SM, and splits of at most 2048 keys so that a few long sequences
@@ -791,18 +931,28 @@ cudaError_t launch_attention_cached(cudaStream_t s, const Cache& c, const Batch&
             return by_storage(c.storage, [&](auto st) {
                 constexpr int STORAGE = decltype(st)::value;
                 using L = Layout<STORAGE, HD>;
-                const int splits = split_count(c, b, a);
+                const int splits = split_count(c, b, a), rows = rows_of_tile(b, a);
                 const dim3 grid(tile_bound(b, a), a.kv_heads, splits);
-                cudaError_t e = cudaFuncSetAttribute(k_cached<T, STORAGE, HD>,
-                                                     cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                     L::kSmem);
-                if (e) return e;
-                k_cached<T, STORAGE, HD><<<grid, kThreads, L::kSmem, s>>>(
-                    c, b, a, static_cast<const T*>(q), q_stride, static_cast<T*>(out), out_stride,
-                    splits, static_cast<float*>(workspace));
-                e = cudaGetLastError();
+                auto run = [&](auto tile_rows) {
+                    constexpr int ROWS = decltype(tile_rows)::value;
+                    const auto kernel = k_cached<T, STORAGE, HD, ROWS>;
+                    const cudaError_t err = cudaFuncSetAttribute(
+                        kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::smem(ROWS));
+                    if (err) return err;
+                    kernel<<<grid, kThreads, L::smem(ROWS), s>>>(
+                        c, b, a, static_cast<const T*>(q), q_stride, static_cast<T*>(out), out_stride,
+                        splits, static_cast<float*>(workspace));
+                    return cudaGetLastError();
+                };
+                cudaError_t e;
+                if constexpr (sizeof(T) == 2) {
+                    e = rows == 16 ? run(std::integral_constant<int, 16>())
+                                   : run(std::integral_constant<int, 8>());
+                } else {
+                    e = run(std::integral_constant<int, 8>());
+                }
                 if (e || splits == 1) return e;
-                return launch_pdl(k_cached_join<T, HD>, dim3(b.tokens, a.heads), dim3(kThreads), 0, s, c, b, a, static_cast<T*>(out), out_stride,
+                return launch_pdl(k_cached_join<T, HD>, dim3(b.tokens, a.heads), dim3(kThreads), 0, s, c, b, a, rows, static_cast<T*>(out), out_stride,
                                   splits, static_cast<const float*>(workspace));
             });
         });
