@@ -23,7 +23,8 @@ COMMON = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-I", str(INC
 SOURCES = ["kernels.cu", "gemm_tc.cu", "decode_fused.cu", "ops.cu", "ops_static.cu", "tensors.cu",
            "kv_cache.cu", "attention_cached.cu", "attention_packed.cu", "sample.cu", "operators.cpp", "engine.cpp"]
 HEADERS = ["kernels.h", "java_random.h", "epilogue.cuh", "device.cuh", "select.cuh",
-           "operators.h", "attention.cuh"]
+           "operators.h", "attention.cuh",
+           "sm100.cuh"]
 
 
 def nvcc() -> str:

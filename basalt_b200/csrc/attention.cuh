@@ -5,7 +5,10 @@
 
 #include <type_traits>
 
-#include "basalt_cuda.h"
+#include <algorithm>
+
+#include "device.cuh"
+#include "operators.h"
 
 namespace bst {
 
@@ -16,6 +19,74 @@ __device__ __forceinline__ void put<float>(float* p, float v) { *p = v; }
 template <>
 __device__ __forceinline__ void put<__nv_bfloat16>(__nv_bfloat16* p, float v) {
     *p = __float2bfloat16_rn(v);
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {  // lo in the low half
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// One tile of query rows of one key head.
+struct Tile {
+    int seq, first, n;   // the sequence, its first packed token and its tokens
+    int r0;              // the tile's first query row: row r is token r / group, head r % group
+};
+
+// Tile number `index` of a batch whose sequences have n group rows each, tile_rows to a tile. Without
+// starts every sequence has the same number of tiles; with them the tiles before each sequence are
+// summed, 32 sequences at a time.
+__device__ __forceinline__ bool find_tile(const Batch& b, int group, int tile_rows, int index, Tile* t) {
+    if (!b.starts) {
+        const int per = (group + tile_rows - 1) / tile_rows;
+        t->seq = index / per;
+        t->first = t->seq;
+        t->n = 1;
+        t->r0 = (index - t->seq * per) * tile_rows;
+        return t->seq < b.count;
+    }
+    const int lane = threadIdx.x & 31;
+    int before = 0;
+    for (int s0 = 0; s0 < b.count; s0 += 32) {
+        const int s = s0 + lane;
+        int from = 0, n = 0;
+        if (s < b.count) {
+            from = __ldg(b.starts + s);
+            n = max(0, min(__ldg(b.starts + s + 1), b.tokens) - from);
+        }
+        const int tiles = (n * group + tile_rows - 1) / tile_rows;
+        int run = tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(kFull, run, o);
+            if (lane >= o) run += v;
+        }
+        const unsigned hit = __ballot_sync(kFull, before + run > index);
+        if (hit) {
+            const int who = __ffs(hit) - 1;
+            t->seq = s0 + who;
+            t->first = __shfl_sync(kFull, from, who);
+            t->n = __shfl_sync(kFull, n, who);
+            t->r0 = (index - before - __shfl_sync(kFull, run - tiles, who)) * tile_rows;
+            return true;
+        }
+        before += __shfl_sync(kFull, run, 31);
+    }
+    return false;
+}
+
+// Tiles of `rows` query rows: exact without starts, at most one partial tile a sequence with them.
+inline int tile_bound(const Batch& b, const AttnSpec& a, int64_t rows) {
+    const int64_t group = a.heads / a.kv_heads;
+    if (!b.starts) return static_cast<int>(b.count * ((group + rows - 1) / rows));
+    return static_cast<int>(std::min<int64_t>((b.tokens * group) / rows + b.count, b.tokens * group));
 }
 
 // Calls fn with the value as a constant or type.

@@ -43,7 +43,6 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kBlock = 16;   // keys a warp takes at a time
-constexpr float kLog2e = 1.4426950408889634f;
 
 template <int STORAGE, int HD>
 struct Layout {
@@ -120,17 +119,6 @@ __device__ __forceinline__ void mma_bf16_start(float (&c)[4], uint32_t a0, uint3
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {  // lo in the low half
-    uint32_t r;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
 __device__ __forceinline__ float low_of(uint32_t p) { return __uint_as_float(p << 16); }
 __device__ __forceinline__ float high_of(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
 
@@ -201,54 +189,6 @@ struct Visible {
 __host__ __device__ __forceinline__ int useful_splits(int blocks, int splits) {
     const int most = blocks / 8;
     return most < 1 ? 1 : (most < splits ? most : splits);
-}
-
-// One tile of query rows of one key head.
-struct Tile {
-    int seq, first, n;   // the sequence, its first packed token and its tokens
-    int r0;              // the tile's first query row: row r is token r / group, head r % group
-};
-
-// Tile number `index` of a batch whose sequences have n group rows each, tile_rows to a tile. Without
-// starts every sequence has the same number of tiles; with them the tiles before each sequence are
-// summed, 32 sequences at a time.
-__device__ __forceinline__ bool find_tile(const Batch& b, int group, int tile_rows, int index, Tile* t) {
-    if (!b.starts) {
-        const int per = (group + tile_rows - 1) / tile_rows;
-        t->seq = index / per;
-        t->first = t->seq;
-        t->n = 1;
-        t->r0 = (index - t->seq * per) * tile_rows;
-        return t->seq < b.count;
-    }
-    const int lane = threadIdx.x & 31;
-    int before = 0;
-    for (int s0 = 0; s0 < b.count; s0 += 32) {
-        const int s = s0 + lane;
-        int from = 0, n = 0;
-        if (s < b.count) {
-            from = __ldg(b.starts + s);
-            n = max(0, min(__ldg(b.starts + s + 1), b.tokens) - from);
-        }
-        const int tiles = (n * group + tile_rows - 1) / tile_rows;
-        int run = tiles;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(kFull, run, o);
-            if (lane >= o) run += v;
-        }
-        const unsigned hit = __ballot_sync(kFull, before + run > index);
-        if (hit) {
-            const int who = __ffs(hit) - 1;
-            t->seq = s0 + who;
-            t->first = __shfl_sync(kFull, from, who);
-            t->n = __shfl_sync(kFull, n, who);
-            t->r0 = (index - before - __shfl_sync(kFull, run - tiles, who)) * tile_rows;
-            return true;
-        }
-        before += __shfl_sync(kFull, run, 31);
-    }
-    return false;
 }
 
 // CTAs an SM must hold, which caps the registers: measured, more warps beat the few spills.
@@ -891,13 +831,6 @@ int rows_of_tile(const Batch& b, const AttnSpec& a) {
     return a.dtype == BST_DTYPE_BF16 && b.tokens * group > 8ll * b.count ? 16 : 8;
 }
 
-// Tiles: exact without starts, at most one partial tile a sequence with them.
-int tile_bound(const Batch& b, const AttnSpec& a) {
-    const int64_t group = a.heads / a.kv_heads, rows = rows_of_tile(b, a);
-    if (!b.starts) return static_cast<int>(b.count * ((group + rows - 1) / rows));
-    return static_cast<int>(std::min<int64_t>((b.tokens * group) / rows + b.count, b.tokens * group));
-}
-
 // CTAs for about four on every SM, and splits of at most 2048 keys so that a few long sequences
 // among short ones are spread over the SMs too; never less than 128 keys a split. The lengths are
 // on the device, so the bound is what the cache and the window allow; tiles with fewer keys use
@@ -905,7 +838,7 @@ int tile_bound(const Batch& b, const AttnSpec& a) {
 int split_count(const Cache& c, const Batch& b, const AttnSpec& a) {
     int64_t keys = c.slots;
     if (a.window) keys = std::min<int64_t>(keys, static_cast<int64_t>(a.window) + a.sinks + 2 * kBlock);
-    const int64_t units = static_cast<int64_t>(tile_bound(b, a)) * a.kv_heads;
+    const int64_t units = static_cast<int64_t>(tile_bound(b, a, rows_of_tile(b, a))) * a.kv_heads;
     const int64_t fill = (148 * 4 + units - 1) / std::max<int64_t>(units, 1);
     const int64_t even = (keys + 2047) / 2048;
     const int64_t most = std::max<int64_t>(1, keys / 128);
@@ -932,7 +865,7 @@ cudaError_t launch_attention_cached(cudaStream_t s, const Cache& c, const Batch&
                 constexpr int STORAGE = decltype(st)::value;
                 using L = Layout<STORAGE, HD>;
                 const int splits = split_count(c, b, a), rows = rows_of_tile(b, a);
-                const dim3 grid(tile_bound(b, a), a.kv_heads, splits);
+                const dim3 grid(tile_bound(b, a, rows_of_tile(b, a)), a.kv_heads, splits);
                 auto run = [&](auto tile_rows) {
                     constexpr int ROWS = decltype(tile_rows)::value;
                     const auto kernel = k_cached<T, STORAGE, HD, ROWS>;

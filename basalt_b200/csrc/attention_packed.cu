@@ -14,9 +14,428 @@
 #include "attention.cuh"
 #include "device.cuh"
 #include "operators.h"
+#include "sm100.cuh"
 
 namespace bst {
 namespace {
+
+// ---- bf16 on the tensor cores ----------------------------------------------------------------
+// A CTA takes 256 query rows of one key head: tokens x heads of its group, so that heads sharing keys
+// share their tiles, and a tile of few tokens wastes little of a window. They are two M = 128 tiles
+// whose products alternate with their softmaxes: while eight warps (a thread a row) turn one tile's
+// scores into weights, the tensor cores work on the other's. Keys and values come in tiles of 128 by
+// TMA through a ring of 128-byte-swizzled buffers.
+//   TMEM, per tile: scores S (128 columns, float32), whose place the weights P take as bf16 and from
+//   where the second product reads them as its A operand, and the output O (head_dim columns).
+//   O = P V reads V as it lies in memory (its B operand is MN-major).
+// The maximum that weights are taken against moves only when a row's grows by more than 2^8: the
+// softmax then rescales O itself, which is idle at that moment, because the scores it waits for were
+// issued behind the last product into O.
+// What bounds it: at head_dim 128 the products (4 x 128 x 128 x 128 multiply-adds a step, ~2900
+// cycles at the measured rate) outweigh the exponentials (32 768 at 16 a cycle, 2048 cycles).
+//
+// Weights of keys that a row does not see are zero, but zero times a NaN or infinity is NaN. Tiles
+// that are partly hidden are searched for such values first; a CTA that meets one, or whose waits
+// run out, raises its flag, and the plain kernel behind this one computes its rows again.
+
+constexpr int kTcRows = 256;
+constexpr int kTcThreads = 320;  // warps 0-3 and 4-7: a tile's rows; 8: products; 9: copies
+constexpr int kTcKeys = 128;
+
+template <int HD>
+struct TcLayout {
+    static constexpr int kTile = kTcKeys * HD * 2;    // a tile of keys, values or 128 query rows
+    static constexpr int kSlots = 4;
+    static constexpr int kBars = 2 * kTile + kSlots * kTile;
+    // More than half of an SM's shared memory: one CTA an SM, which owns all of TMEM.
+    static constexpr int kBytes = kBars + 256 > 120 * 1024 ? kBars + 256 : 120 * 1024;
+    static constexpr int kSmem = kBytes + 1024;       // the base is aligned to 1024 bytes
+};
+
+// The key tiles of a CTA: the sinks before its window, then the window; a tile is up to 128 keys
+// from `key`, `cols` of them (a multiple of 32) multiplied.
+struct TcKeys {
+    int first, end;      // the window's keys
+    int sink_end;        // sinks before it
+    int sink_tiles, tiles;
+    __device__ TcKeys(int p0, int p1, int window, int sinks) {
+        end = p1 + 1;
+        first = window ? max(0, p0 - window + 1) : 0;
+        sink_end = min(sinks, first);
+        sink_tiles = (sink_end + kTcKeys - 1) / kTcKeys;
+        tiles = sink_tiles + (end - first + kTcKeys - 1) / kTcKeys;
+    }
+    __device__ int key(int i) const {
+        return i < sink_tiles ? i * kTcKeys : first + (i - sink_tiles) * kTcKeys;
+    }
+    __device__ int cols(int i) const {
+        const int left = (i < sink_tiles ? sink_end : end) - key(i);
+        return min(kTcKeys, (left + 31) & ~31);
+    }
+};
+
+// Accumulating or fresh product of kind::f16 with A from shared memory (a descriptor) or TMEM.
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                          uint32_t accumulate) {
+    const uint32_t z = 0;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(z));
+}
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                          uint32_t accumulate) {
+    const uint32_t z = 0;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(z));
+}
+
+// bf16 x bf16 -> float32, M = 128; b_mn: B is MN-major.
+__device__ __forceinline__ uint32_t tc_idesc(int n, bool b_mn) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn ? 1u << 16 : 0u) |
+           (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
+}
+
+// MN-major tile in the 128-byte swizzle: 64-channel columns of atoms 16 KB apart (leading offset),
+// atoms of eight keys 1024 bytes apart.
+__device__ __forceinline__ uint64_t tc_desc_mn(uint32_t addr) {
+    return static_cast<uint64_t>((addr >> 4) & 0x3fff) | (static_cast<uint64_t>(16384 >> 4) << 16) |
+           (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) |
+           (static_cast<uint64_t>(2) << 61);
+}
+
+// 32 columns of this thread's TMEM lane, without waiting for them.
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+        "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+        "%30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+          "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+          "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_ld_wait() {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+        "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, "
+        "%29, %30, %31, %32};" ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+        "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
+        "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+        "r"(r[29]), "r"(r[30]), "r"(r[31]));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+        "%11, %12, %13, %14, %15, %16};" ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+        "r"(r[15]));
+}
+__device__ __forceinline__ void tmem_st_wait() {
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ bool not_finite(uint32_t pair) {  // of two bf16
+    return (pair & 0x7f80u) == 0x7f80u || (pair & 0x7f800000u) == 0x7f800000u;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kTcThreads, 1)
+k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+            Batch b, AttnSpec a, const __nv_bfloat16* __restrict__ q, int64_t q_stride,
+            __nv_bfloat16* __restrict__ out, int64_t out_stride, int* __restrict__ flags) {
+    using L = TcLayout<HD>;
+    constexpr int kBlocks = HD / 64;     // 128-byte columns of a tile, 16 KB each
+    extern __shared__ unsigned char raw[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int group = a.heads / a.kv_heads, kvh = blockIdx.y;
+    // The last tiles first: without a window they see the most keys.
+    const int index = gridDim.x - 1 - blockIdx.x;
+    int* const flag = flags + kvh * gridDim.x + index;
+    Tile tile;
+    if (!find_tile(b, group, kTcRows, index, &tile)) {
+        if (threadIdx.x == 0) *flag = 0;
+        return;
+    }
+    const int rows = min(kTcRows, tile.n * group - tile.r0);
+    const int p0 = tile.r0 / group, p1 = (tile.r0 + rows - 1) / group;
+    const TcKeys keys(p0, p1, a.window, a.sinks);
+    // The second tile of a short CTA has no rows: then all is done for the first alone.
+    const int halves = rows > 128 ? 2 : 1;
+
+    const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+    unsigned char* const smem = raw + (base - smem_u32(raw));
+    uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
+    uint64_t* const full = bars;                 // [kSlots] a copy has arrived
+    uint64_t* const empty = full + L::kSlots;    // [kSlots] its readers are done
+    uint64_t* const s_full = empty + L::kSlots;  // [2] scores (and all products before) are done
+    uint64_t* const p_full = s_full + 2;         // [2] weights are written
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(p_full + 2);
+    int* const status = reinterpret_cast<int*>(tmem_slot + 1);  // [0] error code, [1] abort, [2] redo
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < L::kSlots; ++i) {
+            mbar_init(full + i, 1);
+            mbar_init(empty + i, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(s_full + i, 1);
+            mbar_init(p_full + i, 128);
+        }
+        status[0] = status[1] = status[2] = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         smem_u32(tmem_slot)),
+                     "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    // Queries: a thread a row, 16-byte chunks into the swizzle. A negative scale moves into them.
+    const int my_row = tile.r0 + threadIdx.x;
+    const int my_token = my_row / group, my_head = kvh * group + my_row - my_token * group;
+    const bool live = static_cast<int>(threadIdx.x) < rows;
+    if (threadIdx.x < kTcRows) {
+        const uint4* src = reinterpret_cast<const uint4*>(
+            q + (tile.first + static_cast<int64_t>(my_token)) * q_stride + my_head * HD);
+        const int r = threadIdx.x & 127;
+        unsigned char* to = smem + (threadIdx.x >> 7) * L::kTile + r * 128;
+        const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+#pragma unroll
+        for (int i = 0; i < HD / 8; ++i) {
+            uint4 x = live ? src[i] : make_uint4(0u, 0u, 0u, 0u);
+            x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
+            *reinterpret_cast<uint4*>(to + (i >> 3) * 16384 + (((i & 7) ^ (r & 7)) << 4)) = x;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *tmem_slot;
+    volatile int* const abort = status + 1;
+    auto slot_at = [&](int i) { return base + 2 * L::kTile + (i % L::kSlots) * L::kTile; };
+    // Tile i's keys are copy 2 i, its values copy 2 i + 1.
+    const int copies = 2 * keys.tiles;
+
+    if (warp == 9) {
+        if (lane == 0) {
+            for (int i = 0; i < copies; ++i) {
+                const int slot = i % L::kSlots;
+                if (i >= L::kSlots &&
+                    !mbar_wait(empty + slot, ((i / L::kSlots) - 1) & 1, status, 1, abort)) {
+                    break;
+                }
+                mbar_expect_tx(full + slot, L::kTile);
+                for (int x = 0; x < kBlocks; ++x) {
+                    tma_load_2d(i & 1 ? &v_map : &k_map, full + slot,
+                                smem + 2 * L::kTile + slot * L::kTile + x * 16384,
+                                kvh * HD + 64 * x, tile.first + keys.key(i >> 1));
+                }
+            }
+        }
+    } else if (warp == 8) {
+        if (lane == 0) {
+            auto scores = [&](int half, int i) {  // S = Q K^T
+                const uint32_t d = tmem + half * 256;
+                const uint32_t qa = base + half * L::kTile, ka = slot_at(2 * i);
+                const uint32_t idesc = tc_idesc(keys.cols(i), false);
+#pragma unroll
+                for (int k = 0; k < HD / 16; ++k) {
+                    const uint32_t at = (k >> 2) * 16384 + (k & 3) * 32;
+                    tc_mma_ss(d, smem_desc(qa + at), smem_desc(ka + at), idesc, k > 0);
+                }
+                mma_commit(s_full + half);
+            };
+            bool ok = mbar_wait(full, 0, status, 2, abort);
+            if (ok) {
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                for (int h = 0; h < halves; ++h) scores(h, 0);
+                mma_commit(empty);
+            }
+            for (int i = 0; ok && i < keys.tiles; ++i) {
+                const int vc = 2 * i + 1, kc = 2 * i + 2;
+                const bool more = i + 1 < keys.tiles;
+                ok = mbar_wait(full + vc % L::kSlots, (vc / L::kSlots) & 1, status, 3, abort) &&
+                     (!more || mbar_wait(full + kc % L::kSlots, (kc / L::kSlots) & 1, status, 4, abort));
+                const uint32_t idesc = tc_idesc(HD, true);
+                const int steps = keys.cols(i) / 16;
+                for (int h = 0; ok && h < halves; ++h) {
+                    ok = mbar_wait(p_full + h, i & 1, status, 5, abort);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t d = tmem + h * 256 + 128, p = tmem + h * 256;
+                    const uint32_t va = slot_at(vc);
+                    for (int k = 0; k < steps; ++k) {  // O += P V
+                        tc_mma_ts(d, p + 8 * k, tc_desc_mn(va + k * 2048), idesc, i > 0 || k > 0);
+                    }
+                    if (more) {
+                        scores(h, i + 1);
+                    } else {
+                        mma_commit(s_full + h);
+                    }
+                }
+                if (ok) {
+                    mma_commit(empty + vc % L::kSlots);
+                    if (more) mma_commit(empty + kc % L::kSlots);
+                }
+            }
+        }
+    } else {
+        const int half = warp >> 2;
+        const uint32_t s_at = tmem + half * 256 + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
+        const uint32_t o_at = s_at + 128;
+        const float scale = fabsf(a.scale) * kLog2e;
+        // Rows behind the last query see nothing.
+        const int position = live ? my_token : -1;
+        const int low = a.window ? position - a.window + 1 : 0;  // the window's first key
+        const float slack = 8.0f / scale;                        // scale 0: infinite, never moved
+        float top = -INFINITY, total = 0.0f;
+        bool ok = half < halves;
+        for (int i = 0; ok && i < keys.tiles; ++i) {
+            const int key0 = keys.key(i), cols = keys.cols(i);
+            // Whether all rows of the CTA see all of the tile's columns.
+            const bool all = key0 + cols - 1 <= p0 &&
+                             (i < keys.sink_tiles ? key0 + cols <= keys.sink_end
+                                                  : a.window == 0 || p1 - key0 < a.window);
+            if (!all) {
+                // The CTA's rows (256 or 128 of them) search the values for what is not finite.
+                const int vc = 2 * i + 1;
+                ok = mbar_wait(full + vc % L::kSlots, (vc / L::kSlots) & 1, status, 6, abort);
+                if (!ok) break;
+                const uint4* v = reinterpret_cast<const uint4*>(smem + 2 * L::kTile +
+                                                                (vc % L::kSlots) * L::kTile);
+                bool bad = false;
+                for (int x = threadIdx.x; x < L::kTile / 16; x += 128 * halves) {
+                    const uint4 u = v[x];
+                    bad |= not_finite(u.x) || not_finite(u.y) || not_finite(u.z) || not_finite(u.w);
+                }
+                if (bad) status[2] = 1;
+            }
+            ok = mbar_wait(s_full + half, i & 1, status, 7, abort);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            // Two passes over the scores, 32 columns at a time with the next 32 on their way: the
+            // maximum, then the weights (which fall on columns that have been read).
+            const int last = i < keys.sink_tiles ? min(position, keys.sink_end - 1) : position;
+            auto mask = [&](uint32_t(&s)[32], int c) {
+                const int at = key0 + 32 * c;
+#pragma unroll
+                for (int x = 0; x < 32; ++x) {
+                    const int key = at + x;
+                    const bool see = key <= last && (key >= low || key < a.sinks);
+                    if (!see) s[x] = 0xff800000u;
+                }
+            };
+            const int chunks = cols >> 5;
+            uint32_t s[2][32];
+            float most = -INFINITY;
+            tmem_ld32(s_at, s[0]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                if (c < chunks) {
+                    tmem_ld_wait();
+                    if (c + 1 < chunks) tmem_ld32(s_at + 32 * (c + 1), s[(c + 1) & 1]);
+                    if (!all) mask(s[c & 1], c);
+                    float m[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) m[x & 1] = fmaxf(m[x & 1], __uint_as_float(s[c & 1][x]));
+                    most = fmaxf(most, fmaxf(m[0], m[1]));
+                }
+            }
+            tmem_ld32(s_at, s[0]);
+            const bool move = most > top + slack || (top == -INFINITY && most > top);
+            if (__any_sync(kFull, move)) {
+                const float keep = move ? (top == -INFINITY ? 0.0f : exp2_fast((top - most) * scale)) : 1.0f;
+                if (move) top = most;
+                total *= keep;
+                if (i > 0) {
+#pragma unroll
+                    for (int c = 0; c < HD / 32; ++c) {
+                        uint32_t o[32];
+                        tmem_ld32(o_at + 32 * c, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * keep);
+                        tmem_st32(o_at + 32 * c, o);
+                    }
+                }
+            }
+            const float from = top == -INFINITY ? 0.0f : top * scale;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                if (c < chunks) {
+                    tmem_ld_wait();
+                    if (c + 1 < chunks) tmem_ld32(s_at + 32 * (c + 1), s[(c + 1) & 1]);
+                    if (!all) mask(s[c & 1], c);
+                    uint32_t p[16];
+                    float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) {
+                        const float e0 = exp2_fast(fmaf(__uint_as_float(s[c & 1][2 * x]), scale, -from));
+                        const float e1 = exp2_fast(fmaf(__uint_as_float(s[c & 1][2 * x + 1]), scale, -from));
+                        sum[0] += e0;
+                        sum[1] += e1;
+                        p[x] = pack2(e0, e1);
+                    }
+                    total += sum[0] + sum[1];
+                    tmem_st16(s_at + 16 * c, p);
+                }
+            }
+            tmem_st_wait();
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            mbar_arrive(p_full + half);
+        }
+        if (ok) ok = mbar_wait(s_full + half, keys.tiles & 1, status, 8, abort);
+        if (ok) {
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const float by = total == 0.0f ? 0.0f : 1.0f / total;
+            uint4* to = reinterpret_cast<uint4*>(
+                out + (tile.first + static_cast<int64_t>(my_token)) * out_stride + my_head * HD);
+#pragma unroll
+            for (int c = 0; c < HD / 32; ++c) {
+                uint32_t o[32];
+                tmem_ld32(o_at + 32 * c, o);
+                tmem_ld_wait();
+                if (live) {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) {
+                            w[y] = pack2(__uint_as_float(o[8 * x + 2 * y]) * by,
+                                         __uint_as_float(o[8 * x + 2 * y + 1]) * by);
+                        }
+                        to[4 * c + x] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+            }
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (status[0] != 0 && threadIdx.x == 0) {
+        // A wait ran out: let the copies that were issued land before the memory goes away.
+        const uint64_t start = global_ns();
+        while (global_ns() - start < 2000000ull) {
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) *flag = status[0] != 0 || status[2] != 0;
+    if (warp == 8) {
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    }
+}
 
 // One query by one warp: lanes over the channels, one key at a time.
 template <typename T, int HD>
@@ -70,18 +489,88 @@ k_packed_plain(Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride,
                         threadIdx.x & 31);
 }
 
+// The rows of CTAs of k_packed_tc that raised their flag, computed plainly.
+template <int HD>
+__global__ void __launch_bounds__(256)
+k_packed_again(Batch b, AttnSpec a, const __nv_bfloat16* __restrict__ q, int64_t q_stride,
+               const __nv_bfloat16* __restrict__ k, int64_t k_stride,
+               const __nv_bfloat16* __restrict__ v, int64_t v_stride,
+               __nv_bfloat16* __restrict__ out, int64_t out_stride, const int* __restrict__ flags,
+               int tiles) {
+    pdl_wait();
+    for (int i = blockIdx.x; i < tiles * a.kv_heads; i += gridDim.x) {
+        if (flags[i] == 0) continue;
+        const int kvh = i / tiles, group = a.heads / a.kv_heads;
+        Tile tile;
+        if (!find_tile(b, group, kTcRows, i % tiles, &tile)) continue;
+        const int rows = min(kTcRows, tile.n * group - tile.r0);
+        for (int r = threadIdx.x >> 5; r < rows; r += 8) {
+            const int row = tile.r0 + r;
+            const int64_t token = row / group, head = kvh * group + row % group;
+            attend_query<__nv_bfloat16, HD>(
+                q + (tile.first + token) * q_stride + head * HD,
+                k + tile.first * k_stride + kvh * HD, k_stride,
+                v + tile.first * v_stride + kvh * HD, v_stride,
+                out + (tile.first + token) * out_stride + head * HD, token, a.window, a.sinks,
+                a.scale, threadIdx.x & 31);
+        }
+    }
+}
+
+// Whether the tensor-core kernel takes this call: bf16, what TMA and 16-byte accesses can address.
+bool tc_takes(const AttnSpec& a, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+              const void* v, int64_t v_stride, const void* out, int64_t out_stride) {
+    auto aligned = [](const void* p, int64_t stride) {
+        return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 8 == 0;
+    };
+    return a.dtype == BST_DTYPE_BF16 && a.head_dim >= 64 && aligned(q, q_stride) &&
+           aligned(k, k_stride) && aligned(v, v_stride) && aligned(out, out_stride);
+}
+
 unsigned plain_grid(const Batch& b, const AttnSpec& a) {
     return static_cast<unsigned>((static_cast<int64_t>(b.tokens) * a.heads + 3) / 4);
 }
 
 }  // namespace
 
-size_t attention_packed_workspace(const Batch&, const AttnSpec&) { return 0; }
+// A flag for every CTA of the tensor-core kernel.
+size_t attention_packed_workspace(const Batch& b, const AttnSpec& a) {
+    if (a.dtype != BST_DTYPE_BF16 || a.head_dim < 64) return 0;
+    return static_cast<size_t>(tile_bound(b, a, kTcRows)) * a.kv_heads * sizeof(int);
+}
 
 cudaError_t launch_attention_packed(cudaStream_t s, const Batch& b, const AttnSpec& a,
                                     const void* q, int64_t q_stride, const void* k,
                                     int64_t k_stride, const void* v, int64_t v_stride, void* out,
-                                    int64_t out_stride, void*) {
+                                    int64_t out_stride, void* workspace) {
+    if (b.tokens < 1 || b.count < 1) return cudaSuccess;
+    if (tc_takes(a, q, q_stride, k, k_stride, v, v_stride, out, out_stride)) {
+        auto run = [&](auto hd) {
+            constexpr int HD = decltype(hd)::value;
+            using T = __nv_bfloat16;
+            CUtensorMap k_map, v_map;
+            const int width = a.kv_heads * HD;
+            cudaError_t e = make_tile_map(&k_map, k, b.tokens, width, k_stride * 2, true, kTcKeys);
+            if (!e) e = make_tile_map(&v_map, v, b.tokens, width, v_stride * 2, true, kTcKeys);
+            if (!e) {
+                e = cudaFuncSetAttribute(k_packed_tc<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         TcLayout<HD>::kSmem);
+            }
+            if (e) return e;
+            const int tiles = tile_bound(b, a, kTcRows);
+            int* flags = static_cast<int*>(workspace);
+            k_packed_tc<HD><<<dim3(tiles, a.kv_heads), kTcThreads, TcLayout<HD>::kSmem, s>>>(
+                k_map, v_map, b, a, static_cast<const T*>(q), q_stride, static_cast<T*>(out),
+                out_stride, flags);
+            if ((e = cudaGetLastError())) return e;
+            return launch_pdl(k_packed_again<HD>, dim3(std::min(148, tiles * a.kv_heads)), dim3(256), 0,
+                              s, b, a, static_cast<const T*>(q), q_stride, static_cast<const T*>(k),
+                              k_stride, static_cast<const T*>(v), v_stride, static_cast<T*>(out),
+                              out_stride, static_cast<const int*>(flags), tiles);
+        };
+        return a.head_dim == 64 ? run(std::integral_constant<int, 64>())
+                                : run(std::integral_constant<int, 128>());
+    }
     return by_dtype(a.dtype, [&](auto t) {
         using T = decltype(t);
         return by_head_dim(a.head_dim, [&](auto hd) {

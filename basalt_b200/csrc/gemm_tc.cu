@@ -29,6 +29,7 @@
 #include "epilogue.cuh"
 #include "kernels.h"
 #include "select.cuh"
+#include "sm100.cuh"
 
 namespace bst {
 namespace {
@@ -36,83 +37,6 @@ namespace {
 constexpr int BM = 128;
 constexpr int kRowBytes = 128;                 // one swizzle atom row
 constexpr int kTileRowsA = BM;
-constexpr uint64_t kWaitNs = 2000000000ull;    // 2 s bound on any single wait
-
-__device__ __forceinline__ uint32_t smem_u32(const void* p) {
-    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-
-__device__ __forceinline__ uint64_t global_ns() {
-    uint64_t t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-
-__device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
-}
-
-__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)),
-                 "r"(bytes)
-                 : "memory");
-}
-
-__device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-
-// Waits for the phase of `bar` with the given parity. False on timeout (the error code is
-// recorded and `abort` raised for the other roles of the CTA) or once another role has raised
-// `abort`.
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* err, int code,
-                                          volatile int* abort) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const uint64_t start = global_ns();
-    while (!mbar_try_wait(bar, parity)) {
-        if (*abort) return false;
-        if (global_ns() - start > kWaitNs) {
-            atomicCAS(err, 0, code);
-            *abort = 1;
-            return false;
-        }
-    }
-    return true;
-}
-
-// Bounded wait that ignores `abort`: used on the way out, to let copies and MMAs already issued
-// finish before their shared memory or TMEM is released.
-__device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity, int* err, int code) {
-    const uint64_t start = global_ns();
-    while (!mbar_try_wait(bar, parity)) {
-        if (global_ns() - start > kWaitNs) {
-            atomicCAS(err, 0, code);
-            return;
-        }
-    }
-}
-
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-
-__device__ __forceinline__ void tma_load_2d(const CUtensorMap* map, uint64_t* bar, void* dst,
-                                            int x, int y) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y)
-        : "memory");
-}
-
 // Tiled bulk store of one box from shared memory into a 3-D tensor (the split-K partials), then
 // the wait until the box has been read out of shared memory. Elements outside the tensor are not
 // written.
@@ -128,17 +52,6 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void*
 __device__ __forceinline__ void tma_store_commit_and_drain() {
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
     asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-}
-
-// Shared-memory matrix descriptor for a K-major tile of 128-byte rows with the 128-byte swizzle:
-// 8-row groups 1024 bytes apart (SBO), leading offset unused (1), descriptor version 1.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {
-    uint64_t d = static_cast<uint64_t>((addr >> 4) & 0x3FFF);
-    d |= static_cast<uint64_t>(1) << 16;
-    d |= static_cast<uint64_t>(1024 >> 4) << 32;
-    d |= static_cast<uint64_t>(1) << 46;
-    d |= static_cast<uint64_t>(2) << 61;
-    return d;
 }
 
 // Instruction descriptor: fp32 accumulate, A/B format (2 = tf32, 1 = bf16), both K-major,
@@ -164,43 +77,6 @@ __device__ __forceinline__ void mma(uint32_t tmem_d, uint64_t a, uint64_t b, uin
             "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(tmem_d),
             "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(z), "r"(z), "r"(z), "r"(z));
     }
-}
-
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                     smem_u32(bar))
-                 : "memory");
-}
-
-// CW (16 or 32) consecutive accumulator columns of this thread's TMEM lane (one row of the tile).
-template <int CW>
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, float* v) {
-    uint32_t r[CW];
-    if constexpr (CW == 32) {
-        asm volatile(
-            "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
-            "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, "
-            "%28, %29, %30, %31}, [%32];"
-            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-              "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
-              "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
-              "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-              "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
-              "=r"(r[31])
-            : "r"(taddr));
-    } else {
-        static_assert(CW == 16, "chunk width");
-        asm volatile(
-            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
-            "%11, %12, %13, %14, %15}, [%16];"
-            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-              "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
-              "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-            : "r"(taddr));
-    }
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < CW; ++i) v[i] = __uint_as_float(r[i]);
 }
 
 template <int FMT, int BN, int ST = 0>
@@ -1089,12 +965,13 @@ cudaError_t encoder() {
     return g_encode ? cudaSuccess : cudaErrorNotSupported;
 }
 
-// 2-D row-major [rows, K] map with a (128-byte-row x box_rows) box, 128-byte swizzle, zero fill.
-cudaError_t make_map(CUtensorMap* map, const void* ptr, int rows, int K, bool bf16,
-                     int box_rows) {
+// 2-D map of [rows, K], rows `pitch` bytes apart, with a (128-byte-row x box_rows) box, 128-byte
+// swizzle, zero fill.
+cudaError_t make_pitched_map(CUtensorMap* map, const void* ptr, int rows, int K, int64_t pitch,
+                             bool bf16, int box_rows) {
     const size_t elem = bf16 ? 2 : 4;
     cuuint64_t dims[2] = {static_cast<cuuint64_t>(K), static_cast<cuuint64_t>(rows)};
-    cuuint64_t strides[1] = {static_cast<cuuint64_t>(K) * elem};
+    cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch)};
     cuuint32_t box[2] = {static_cast<cuuint32_t>(kRowBytes / elem),
                          static_cast<cuuint32_t>(box_rows)};
     cuuint32_t estr[2] = {1, 1};
@@ -1104,6 +981,12 @@ cudaError_t make_map(CUtensorMap* map, const void* ptr, int rows, int K, bool bf
                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+cudaError_t make_map(CUtensorMap* map, const void* ptr, int rows, int K, bool bf16,
+                     int box_rows) {
+    return make_pitched_map(map, ptr, rows, K, static_cast<int64_t>(K) * (bf16 ? 2 : 4), bf16,
+                            box_rows);
 }
 
 // 3-D map over split-K partials part[splits][M][N] (fp32) with a 32-column x 128-row box in the
@@ -1347,6 +1230,12 @@ cudaError_t launch_gemm_tc(cudaStream_t s, const void* x_hi, const void* x_lo, c
     }
     return bn == 128 ? launch_epi<2, 128>(s, a0, a1, b0, b1, bias, M, N, K, epi, ea, err, sk)
                      : launch_epi<2, 64>(s, a0, a1, b0, b1, bias, M, N, K, epi, ea, err, sk);
+}
+
+cudaError_t make_tile_map(CUtensorMap* map, const void* ptr, int rows, int K, int64_t pitch, bool bf16,
+                          int box_rows) {
+    const cudaError_t e = encoder();
+    return e ? e : make_pitched_map(map, ptr, rows, K, pitch, bf16, box_rows);
 }
 
 }  // namespace bst
