@@ -21,6 +21,19 @@ __device__ __forceinline__ void put<__nv_bfloat16>(__nv_bfloat16* p, float v) {
     *p = __float2bfloat16_rn(v);
 }
 
+// An asynchronous copy of N bytes to shared memory of which the first `bytes` are read, the rest zero.
+template <int N>
+__device__ __forceinline__ void cp_async(uint32_t dst, const void* src, int bytes) {
+    if constexpr (N == 16) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+                     : "memory");
+    } else {
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N),
+                     "r"(bytes)
+                     : "memory");
+    }
+}
+
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float exp2_fast(float x) {

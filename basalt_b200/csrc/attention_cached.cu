@@ -84,16 +84,6 @@ __device__ __forceinline__ int row_of_column(int n) {
     }
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
-                 : "memory");
-}
-template <int N>
-__device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src, int bytes) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N),
-                 "r"(bytes)
-                 : "memory");
-}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() {
@@ -307,27 +297,27 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
             const uint32_t scale_to = dst + 2 * kHalf + lane * (G * 4);
             if (seen.whole(key0)) {
 #pragma unroll
-                for (int i = 0; i < kLoads; ++i) cp_async16(dst + lane_to(i), ks + 512 * i, 16);
+                for (int i = 0; i < kLoads; ++i) cp_async<16>(dst + lane_to(i), ks + 512 * i, 16);
                 if constexpr (!kShared) {
 #pragma unroll
                     for (int i = 0; i < kLoads; ++i) {
-                        cp_async16(dst + kHalf + lane_to(i), vs + 512 * i, 16);
+                        cp_async<16>(dst + kHalf + lane_to(i), vs + 512 * i, 16);
                     }
                 }
-                if constexpr (L::kCodes) cp_async_small<G * 4>(scale_to, ss, G * 4);
+                if constexpr (L::kCodes) cp_async<G * 4>(scale_to, ss, G * 4);
             } else {
 #pragma unroll
                 for (int i = 0; i < kLoads; ++i) {
                     const int r = lane_row + i * (512 / L::kRowBytes);
                     const bool ok = seen.holds(key0 + (kShared ? r & 15 : r));
-                    cp_async16(dst + lane_to(i), ok ? ks + 512 * i : kb, ok ? 16 : 0);
+                    cp_async<16>(dst + lane_to(i), ok ? ks + 512 * i : kb, ok ? 16 : 0);
                     if constexpr (!kShared) {
-                        cp_async16(dst + kHalf + lane_to(i), ok ? vs + 512 * i : vb, ok ? 16 : 0);
+                        cp_async<16>(dst + kHalf + lane_to(i), ok ? vs + 512 * i : vb, ok ? 16 : 0);
                     }
                 }
                 if constexpr (L::kCodes) {
                     const bool ok = seen.holds(key0 + (lane & 15));
-                    cp_async_small<G * 4>(scale_to, ok ? ss : ksb, ok ? G * 4 : 0);
+                    cp_async<G * 4>(scale_to, ok ? ss : ksb, ok ? G * 4 : 0);
                 }
             }
         }

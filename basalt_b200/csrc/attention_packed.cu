@@ -10,6 +10,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <cfloat>
 
 #include "attention.cuh"
 #include "device.cuh"
@@ -18,6 +19,33 @@
 
 namespace bst {
 namespace {
+
+// The key tiles of a CTA: the sinks before its window, then the window; a tile is up to KEYS keys
+// from key(i), cols(i) of them (a multiple of STEP) multiplied.
+template <int KEYS, int STEP>
+struct KeyTiles {
+    int first, end;      // the window's keys
+    int sink_end;        // sinks before it
+    int sink_tiles, tiles;
+    __device__ KeyTiles(int p0, int p1, int window, int sinks) {
+        end = p1 + 1;
+        first = window ? max(0, p0 - window + 1) : 0;
+        sink_end = min(sinks, first);
+        sink_tiles = (sink_end + KEYS - 1) / KEYS;
+        tiles = sink_tiles + (end - first + KEYS - 1) / KEYS;
+    }
+    __device__ int key(int i) const {
+        return i < sink_tiles ? i * KEYS : first + (i - sink_tiles) * KEYS;
+    }
+    __device__ int stop(int i) const { return i < sink_tiles ? sink_end : end; }
+    __device__ int cols(int i) const { return min(KEYS, (stop(i) - key(i) + STEP - 1) / STEP * STEP); }
+    // Whether queries at positions p0..p1 see all of the tile's columns.
+    __device__ bool whole(int i, int p0, int p1, int window) const {
+        const int at = key(i), n = cols(i);
+        return at + n - 1 <= p0 && (i < sink_tiles ? at + n <= sink_end
+                                                   : window == 0 || p1 - at < window);
+    }
+};
 
 // ---- bf16 on the tensor cores ----------------------------------------------------------------
 // A CTA takes 256 query rows of one key head: tokens x heads of its group, so that heads sharing keys
@@ -50,28 +78,6 @@ struct TcLayout {
     // More than half of an SM's shared memory: one CTA an SM, which owns all of TMEM.
     static constexpr int kBytes = kBars + 256 > 120 * 1024 ? kBars + 256 : 120 * 1024;
     static constexpr int kSmem = kBytes + 1024;       // the base is aligned to 1024 bytes
-};
-
-// The key tiles of a CTA: the sinks before its window, then the window; a tile is up to 128 keys
-// from `key`, `cols` of them (a multiple of 32) multiplied.
-struct TcKeys {
-    int first, end;      // the window's keys
-    int sink_end;        // sinks before it
-    int sink_tiles, tiles;
-    __device__ TcKeys(int p0, int p1, int window, int sinks) {
-        end = p1 + 1;
-        first = window ? max(0, p0 - window + 1) : 0;
-        sink_end = min(sinks, first);
-        sink_tiles = (sink_end + kTcKeys - 1) / kTcKeys;
-        tiles = sink_tiles + (end - first + kTcKeys - 1) / kTcKeys;
-    }
-    __device__ int key(int i) const {
-        return i < sink_tiles ? i * kTcKeys : first + (i - sink_tiles) * kTcKeys;
-    }
-    __device__ int cols(int i) const {
-        const int left = (i < sink_tiles ? sink_end : end) - key(i);
-        return min(kTcKeys, (left + 31) & ~31);
-    }
 };
 
 // Accumulating or fresh product of kind::f16 with A from shared memory (a descriptor) or TMEM.
@@ -169,7 +175,7 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
     }
     const int rows = min(kTcRows, tile.n * group - tile.r0);
     const int p0 = tile.r0 / group, p1 = (tile.r0 + rows - 1) / group;
-    const TcKeys keys(p0, p1, a.window, a.sinks);
+    const KeyTiles<kTcKeys, 32> keys(p0, p1, a.window, a.sinks);
     // The second tile of a short CTA has no rows: then all is done for the first alone.
     const int halves = rows > 128 ? 2 : 1;
 
@@ -305,9 +311,7 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
         for (int i = 0; ok && i < keys.tiles; ++i) {
             const int key0 = keys.key(i), cols = keys.cols(i);
             // Whether all rows of the CTA see all of the tile's columns.
-            const bool all = key0 + cols - 1 <= p0 &&
-                             (i < keys.sink_tiles ? key0 + cols <= keys.sink_end
-                                                  : a.window == 0 || p1 - key0 < a.window);
+            const bool all = keys.whole(i, p0, p1, a.window);
             if (!all) {
                 // The CTA's rows (256 or 128 of them) search the values for what is not finite.
                 const int vc = 2 * i + 1;
@@ -471,43 +475,271 @@ __device__ __forceinline__ void attend_query(const T* q, const T* k, int64_t k_s
     for (int i = 0; i < C; ++i) put(out + lane + 32 * i, l == 0.0f ? 0.0f : acc[i] / l);
 }
 
-// The plain kernel: one warp per (token, head). Right for every case.
+// ---- float32, and bf16 that the kernel above does not take --------------------------------------
+// The same scheme on mma.sync m16n8k8 (tf32): a CTA takes 64 query rows, a warp 16 of them, keys and
+// values pass through shared memory in tiles, double-buffered with cp.async. float32 operands are
+// split in two tf32 parts, x = h + l with h the upper 10 mantissa bits, and multiplied as
+// h h + h l + l h (2^-21 of a product is left out); bf16 ones are tf32 numbers as they are, their
+// weights rounded to tf32. Splitting happens in registers after the load, so the tiles stay float32.
+// Rows of keys are padded to HD + 8 floats and of values to HD + 4, which keeps the fragments' reads
+// (pairs of channels of eight keys; one channel of four keys two apart) free of bank conflicts.
+// Bound by the tensor cores' mma.sync rate: 6 x 64 x 64 x HD multiply-adds a 64-key tile and warp row.
+
 template <typename T, int HD>
-__global__ void __launch_bounds__(128)
-k_packed_plain(Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride,
-               const T* __restrict__ k, int64_t k_stride, const T* __restrict__ v, int64_t v_stride,
-               T* __restrict__ out, int64_t out_stride) {
-    const int64_t unit = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-    if (unit >= static_cast<int64_t>(b.tokens) * a.heads) return;
-    const int t = static_cast<int>(unit / a.heads), head = static_cast<int>(unit % a.heads);
-    int seq, first, n;
-    if (!find_sequence(b, t, &seq, &first, &n)) return;
-    const int kvh = head / (a.heads / a.kv_heads);
-    attend_query<T, HD>(q + t * q_stride + head * HD, k + first * k_stride + kvh * HD, k_stride,
-                        v + first * v_stride + kvh * HD, v_stride,
-                        out + t * out_stride + head * HD, t - first, a.window, a.sinks, a.scale,
-                        threadIdx.x & 31);
+struct MmaLayout {
+    static constexpr int kRows = 64, kThreads = 128;
+    static constexpr int kKeys = HD == 128 ? 32 : 64;   // three CTAs an SM
+    static constexpr int kKPitch = HD + 8, kVPitch = HD + 4;
+    static constexpr int kStage = kKeys * (kKPitch + kVPitch);  // floats
+    static constexpr int kQPitch = HD + 8;
+    static constexpr int kSmem = (2 * kStage + kRows * kQPitch) * 4;
+};
+
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// The rows of CTAs of k_packed_tc that raised their flag, computed plainly.
-template <int HD>
+// x = high + low, high with tf32's mantissa; low is rounded by the product itself.
+__device__ __forceinline__ void tf32_parts(float x, uint32_t* high, uint32_t* low) {
+    *high = __float_as_uint(x) & 0xffffe000u;
+    *low = __float_as_uint(x - __uint_as_float(*high));
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(128, HD == 128 ? 2 : 3)
+k_packed_mma(Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride, const T* __restrict__ k,
+             int64_t k_stride, const T* __restrict__ v, int64_t v_stride, T* __restrict__ out,
+             int64_t out_stride, bool vector, int* __restrict__ flags) {
+    using L = MmaLayout<T, HD>;
+    constexpr bool kSplit = sizeof(T) == 4;
+    extern __shared__ __align__(16) float shared[];
+    __shared__ int redo;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int group = a.heads / a.kv_heads, kvh = blockIdx.y;
+    const int index = gridDim.x - 1 - blockIdx.x;
+    int* const flag = flags + kvh * gridDim.x + index;
+    Tile tile;
+    if (!find_tile(b, group, L::kRows, index, &tile)) {
+        if (threadIdx.x == 0) *flag = 0;
+        return;
+    }
+    const int rows = min(L::kRows, tile.n * group - tile.r0);
+    const int p0 = tile.r0 / group, p1 = (tile.r0 + rows - 1) / group;
+    const KeyTiles<L::kKeys, 8> keys(p0, p1, a.window, a.sinks);
+    if (threadIdx.x == 0) redo = 0;
+
+    const T* const kb = k + tile.first * k_stride + kvh * HD;
+    const T* const vb = v + tile.first * v_stride + kvh * HD;
+    float* const queries = shared + 2 * L::kStage;
+    // Keys and values of tile i into stage i & 1; keys behind the sequence read as zeros.
+    auto fetch = [&](int i) {
+        if (i < keys.tiles) {
+            float* const ks = shared + (i & 1) * L::kStage;
+            float* const vs = ks + L::kKeys * L::kKPitch;
+            const int key0 = keys.key(i);
+            for (int x = threadIdx.x; x < L::kKeys * (HD / 4); x += L::kThreads) {
+                const int r = x / (HD / 4), c = x % (HD / 4) * 4;
+                const bool ok = key0 + r < tile.n;
+                const T* from_k = kb + (ok ? (key0 + r) * k_stride + c : 0);
+                const T* from_v = vb + (ok ? (key0 + r) * v_stride + c : 0);
+                float* to_k = ks + r * L::kKPitch + c;
+                float* to_v = vs + r * L::kVPitch + c;
+                if constexpr (kSplit) {
+                    const int bytes = ok ? 16 : 0;
+                    if (vector) {
+                        cp_async<16>(smem_u32(to_k), from_k, bytes);
+                        cp_async<16>(smem_u32(to_v), from_v, bytes);
+                    } else {
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) {
+                            cp_async<4>(smem_u32(to_k + y), from_k + (ok ? y : 0), bytes / 4);
+                            cp_async<4>(smem_u32(to_v + y), from_v + (ok ? y : 0), bytes / 4);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) {
+                        to_k[y] = ok ? to_f(from_k[y]) : 0.0f;
+                        to_v[y] = ok ? to_f(from_v[y]) : 0.0f;
+                    }
+                }
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    fetch(0);
+    const float to_log2 = a.scale * kLog2e;
+    for (int x = threadIdx.x; x < L::kRows * HD; x += L::kThreads) {
+        const int r = x / HD, c = x % HD, row = tile.r0 + r;
+        float value = 0.0f;
+        if (r < rows) {
+            const int token = row / group;
+            value = to_f(q[(tile.first + static_cast<int64_t>(token)) * q_stride +
+                           (kvh * group + row - token * group) * HD + c]);
+        }
+        queries[r * L::kQPitch + c] = value;
+    }
+    int position[2], low[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        const int row = 16 * warp + g + 8 * r;
+        position[r] = row < rows ? (tile.r0 + row) / group : -1;
+        low[r] = a.window ? position[r] - a.window + 1 : 0;
+    }
+    float o[HD / 8][4], top[2] = {-INFINITY, -INFINITY}, total[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+
+    for (int i = 0; i < keys.tiles; ++i) {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();  // tile i is there, and everyone has left tile i - 1
+        fetch(i + 1);
+        const float* const ks = shared + (i & 1) * L::kStage;
+        const float* const vs = ks + L::kKeys * L::kKPitch;
+        const int key0 = keys.key(i), blocks = keys.cols(i) / 8;
+        const bool all = keys.whole(i, p0, p1, a.window);
+        if (!all) {
+            bool bad = false;
+            for (int x = threadIdx.x; x < L::kKeys * HD; x += L::kThreads) {
+                bad |= !(fabsf(vs[x / HD * L::kVPitch + x % HD]) <= FLT_MAX);
+            }
+            if (bad) redo = 1;
+        }
+        constexpr int kBlocks = L::kKeys / 8;
+        float s[kBlocks][4];
+#pragma unroll
+        for (int n = 0; n < kBlocks; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < HD / 8; ++c) {  // channels 8 c + {2 t, 2 t + 1} are k = t and t + 4
+            uint32_t qh[4], ql[4];
+            const float* from = queries + (16 * warp + g) * L::kQPitch + 8 * c + 2 * t;
+            const float2 q0 = *reinterpret_cast<const float2*>(from);
+            const float2 q1 = *reinterpret_cast<const float2*>(from + 8 * L::kQPitch);
+            tf32_parts(q0.x, &qh[0], &ql[0]);
+            tf32_parts(q1.x, &qh[1], &ql[1]);
+            tf32_parts(q0.y, &qh[2], &ql[2]);
+            tf32_parts(q1.y, &qh[3], &ql[3]);
+#pragma unroll
+            for (int n = 0; n < kBlocks; ++n) {
+                if (n < blocks) {
+                    const float2 x = *reinterpret_cast<const float2*>(ks + (8 * n + g) * L::kKPitch +
+                                                                      8 * c + 2 * t);
+                    uint32_t h0, l0, h1, l1;
+                    tf32_parts(x.x, &h0, &l0);
+                    tf32_parts(x.y, &h1, &l1);
+                    mma_tf32(s[n], qh, h0, h1);
+                    if constexpr (kSplit) {
+                        mma_tf32(s[n], qh, l0, l1);
+                        mma_tf32(s[n], ql, h0, h1);
+                    }
+                }
+            }
+        }
+        float most[2] = {-INFINITY, -INFINITY};
+        const int stop = keys.stop(i);
+#pragma unroll
+        for (int n = 0; n < kBlocks; ++n) {
+            if (n < blocks) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = e >> 1, key = key0 + 8 * n + 2 * t + (e & 1);
+                    s[n][e] *= to_log2;
+                    if (!all && !(key <= position[r] && key < stop && (key >= low[r] || key < a.sinks))) {
+                        s[n][e] = -INFINITY;
+                    }
+                    most[r] = fmaxf(most[r], s[n][e]);
+                }
+            }
+        }
+        float from[2], keep[2];
+        bool grows = false;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            most[r] = fmaxf(most[r], __shfl_xor_sync(kFull, most[r], 1));
+            most[r] = fmaxf(most[r], __shfl_xor_sync(kFull, most[r], 2));
+            const bool up = most[r] > top[r];
+            keep[r] = up ? (top[r] == -INFINITY ? 0.0f : exp2_fast(top[r] - most[r])) : 1.0f;
+            if (up) top[r] = most[r];
+            from[r] = top[r] == -INFINITY ? 0.0f : top[r];
+            total[r] *= keep[r];
+            grows |= up;
+        }
+        if (__any_sync(kFull, grows)) {
+#pragma unroll
+            for (int c = 0; c < HD / 8; ++c) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[c][e] *= keep[e >> 1];
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < kBlocks; ++n) {
+            if (n < blocks) {
+                uint32_t ph[4], pl[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float p = exp2_fast(s[n][e] - from[e >> 1]);
+                    total[e >> 1] += p;
+                    // Column 2 t is k = t, column 2 t + 1 is k = t + 4; rows g and g + 8.
+                    const int at = (e >> 1) + 2 * (e & 1);
+                    tf32_parts(p, &ph[at], &pl[at]);
+                    if constexpr (!kSplit) ph[at] = __float_as_uint(p) + 0x1000u;  // to the nearest
+                }
+#pragma unroll
+                for (int c = 0; c < HD / 8; ++c) {
+                    const float* x = vs + (8 * n + 2 * t) * L::kVPitch + 8 * c + g;
+                    uint32_t h0, l0, h1, l1;
+                    tf32_parts(x[0], &h0, &l0);
+                    tf32_parts(x[L::kVPitch], &h1, &l1);
+                    mma_tf32(o[c], ph, h0, h1);
+                    if constexpr (kSplit) {
+                        mma_tf32(o[c], ph, l0, l1);
+                        mma_tf32(o[c], pl, h0, h1);
+                    }
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        total[r] += __shfl_xor_sync(kFull, total[r], 1);
+        total[r] += __shfl_xor_sync(kFull, total[r], 2);
+        const float by = total[r] == 0.0f ? 0.0f : 1.0f / total[r];
+        const int row = 16 * warp + g + 8 * r;
+        if (row < rows) {
+            const int token = position[r], head = kvh * group + tile.r0 + row - token * group;
+            T* to = out + (tile.first + static_cast<int64_t>(token)) * out_stride + head * HD + 2 * t;
+#pragma unroll
+            for (int c = 0; c < HD / 8; ++c) {
+                put(to + 8 * c, o[c][2 * r] * by);
+                put(to + 8 * c + 1, o[c][2 * r + 1] * by);
+            }
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) *flag = redo;
+}
+
+// The rows of CTAs that raised their flag, computed plainly.
+template <typename T, int HD>
 __global__ void __launch_bounds__(256)
-k_packed_again(Batch b, AttnSpec a, const __nv_bfloat16* __restrict__ q, int64_t q_stride,
-               const __nv_bfloat16* __restrict__ k, int64_t k_stride,
-               const __nv_bfloat16* __restrict__ v, int64_t v_stride,
-               __nv_bfloat16* __restrict__ out, int64_t out_stride, const int* __restrict__ flags,
-               int tiles) {
+k_packed_again(Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride,
+               const T* __restrict__ k, int64_t k_stride, const T* __restrict__ v, int64_t v_stride,
+               T* __restrict__ out, int64_t out_stride, const int* __restrict__ flags, int tiles,
+               int tile_rows) {
     pdl_wait();
     for (int i = blockIdx.x; i < tiles * a.kv_heads; i += gridDim.x) {
         if (flags[i] == 0) continue;
         const int kvh = i / tiles, group = a.heads / a.kv_heads;
         Tile tile;
-        if (!find_tile(b, group, kTcRows, i % tiles, &tile)) continue;
-        const int rows = min(kTcRows, tile.n * group - tile.r0);
+        if (!find_tile(b, group, tile_rows, i % tiles, &tile)) continue;
+        const int rows = min(tile_rows, tile.n * group - tile.r0);
         for (int r = threadIdx.x >> 5; r < rows; r += 8) {
             const int row = tile.r0 + r;
             const int64_t token = row / group, head = kvh * group + row % group;
-            attend_query<__nv_bfloat16, HD>(
+            attend_query<T, HD>(
                 q + (tile.first + token) * q_stride + head * HD,
                 k + tile.first * k_stride + kvh * HD, k_stride,
                 v + tile.first * v_stride + kvh * HD, v_stride,
@@ -517,67 +749,72 @@ k_packed_again(Batch b, AttnSpec a, const __nv_bfloat16* __restrict__ q, int64_t
     }
 }
 
-// Whether the tensor-core kernel takes this call: bf16, what TMA and 16-byte accesses can address.
-bool tc_takes(const AttnSpec& a, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
-              const void* v, int64_t v_stride, const void* out, int64_t out_stride) {
+// Whether TMA and 16-byte accesses can address these bf16 tensors.
+bool tc_takes(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+              int64_t v_stride, const void* out, int64_t out_stride) {
     auto aligned = [](const void* p, int64_t stride) {
         return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 8 == 0;
     };
-    return a.dtype == BST_DTYPE_BF16 && a.head_dim >= 64 && aligned(q, q_stride) &&
-           aligned(k, k_stride) && aligned(v, v_stride) && aligned(out, out_stride);
-}
-
-unsigned plain_grid(const Batch& b, const AttnSpec& a) {
-    return static_cast<unsigned>((static_cast<int64_t>(b.tokens) * a.heads + 3) / 4);
+    return aligned(q, q_stride) && aligned(k, k_stride) && aligned(v, v_stride) &&
+           aligned(out, out_stride);
 }
 
 }  // namespace
 
-// A flag for every CTA of the tensor-core kernel.
+// A flag for every CTA, of the kernel with the smaller tiles.
 size_t attention_packed_workspace(const Batch& b, const AttnSpec& a) {
-    if (a.dtype != BST_DTYPE_BF16 || a.head_dim < 64) return 0;
-    return static_cast<size_t>(tile_bound(b, a, kTcRows)) * a.kv_heads * sizeof(int);
+    return static_cast<size_t>(tile_bound(b, a, 64)) * a.kv_heads * sizeof(int);
 }
 
 cudaError_t launch_attention_packed(cudaStream_t s, const Batch& b, const AttnSpec& a,
-                                    const void* q, int64_t q_stride, const void* k,
-                                    int64_t k_stride, const void* v, int64_t v_stride, void* out,
+                                    const void* q_, int64_t q_stride, const void* k_,
+                                    int64_t k_stride, const void* v_, int64_t v_stride, void* out_,
                                     int64_t out_stride, void* workspace) {
     if (b.tokens < 1 || b.count < 1) return cudaSuccess;
-    if (tc_takes(a, q, q_stride, k, k_stride, v, v_stride, out, out_stride)) {
-        auto run = [&](auto hd) {
-            constexpr int HD = decltype(hd)::value;
-            using T = __nv_bfloat16;
-            CUtensorMap k_map, v_map;
-            const int width = a.kv_heads * HD;
-            cudaError_t e = make_tile_map(&k_map, k, b.tokens, width, k_stride * 2, true, kTcKeys);
-            if (!e) e = make_tile_map(&v_map, v, b.tokens, width, v_stride * 2, true, kTcKeys);
-            if (!e) {
-                e = cudaFuncSetAttribute(k_packed_tc<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         TcLayout<HD>::kSmem);
-            }
-            if (e) return e;
-            const int tiles = tile_bound(b, a, kTcRows);
-            int* flags = static_cast<int*>(workspace);
-            k_packed_tc<HD><<<dim3(tiles, a.kv_heads), kTcThreads, TcLayout<HD>::kSmem, s>>>(
-                k_map, v_map, b, a, static_cast<const T*>(q), q_stride, static_cast<T*>(out),
-                out_stride, flags);
-            if ((e = cudaGetLastError())) return e;
-            return launch_pdl(k_packed_again<HD>, dim3(std::min(148, tiles * a.kv_heads)), dim3(256), 0,
-                              s, b, a, static_cast<const T*>(q), q_stride, static_cast<const T*>(k),
-                              k_stride, static_cast<const T*>(v), v_stride, static_cast<T*>(out),
-                              out_stride, static_cast<const int*>(flags), tiles);
-        };
-        return a.head_dim == 64 ? run(std::integral_constant<int, 64>())
-                                : run(std::integral_constant<int, 128>());
-    }
-    return by_dtype(a.dtype, [&](auto t) {
-        using T = decltype(t);
+    int* const flags = static_cast<int*>(workspace);
+    return by_dtype(a.dtype, [&](auto type) {
+        using T = decltype(type);
         return by_head_dim(a.head_dim, [&](auto hd) {
-            k_packed_plain<T, decltype(hd)::value><<<plain_grid(b, a), 128, 0, s>>>(
-                b, a, static_cast<const T*>(q), q_stride, static_cast<const T*>(k), k_stride,
-                static_cast<const T*>(v), v_stride, static_cast<T*>(out), out_stride);
-            return cudaGetLastError();
+            constexpr int HD = decltype(hd)::value;
+            const T *q = static_cast<const T*>(q_), *k = static_cast<const T*>(k_),
+                    *v = static_cast<const T*>(v_);
+            T* const out = static_cast<T*>(out_);
+            int tile_rows = 0, tiles = 0;
+            cudaError_t e = cudaSuccess;
+            if constexpr (sizeof(T) == 2 && HD >= 64) {
+                if (tc_takes(q, q_stride, k, k_stride, v, v_stride, out, out_stride)) {
+                    tile_rows = kTcRows;
+                    tiles = tile_bound(b, a, tile_rows);
+                    CUtensorMap k_map, v_map;
+                    const int width = a.kv_heads * HD;
+                    e = make_tile_map(&k_map, k, b.tokens, width, k_stride * 2, true, kTcKeys);
+                    if (!e) e = make_tile_map(&v_map, v, b.tokens, width, v_stride * 2, true, kTcKeys);
+                    if (!e) {
+                        e = cudaFuncSetAttribute(k_packed_tc<HD>,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 TcLayout<HD>::kSmem);
+                    }
+                    if (e) return e;
+                    k_packed_tc<HD><<<dim3(tiles, a.kv_heads), kTcThreads, TcLayout<HD>::kSmem, s>>>(
+                        k_map, v_map, b, a, q, q_stride, out, out_stride, flags);
+                }
+            }
+            if (tile_rows == 0) {
+                using L = MmaLayout<T, HD>;
+                tile_rows = L::kRows;
+                tiles = tile_bound(b, a, tile_rows);
+                const bool vector = (reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16 == 0 &&
+                                    k_stride % 4 == 0 && v_stride % 4 == 0;
+                e = cudaFuncSetAttribute(k_packed_mma<T, HD>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
+                if (e) return e;
+                k_packed_mma<T, HD><<<dim3(tiles, a.kv_heads), L::kThreads, L::kSmem, s>>>(
+                    b, a, q, q_stride, k, k_stride, v, v_stride, out, out_stride, vector, flags);
+            }
+            if ((e = cudaGetLastError())) return e;
+            return launch_pdl(k_packed_again<T, HD>, dim3(std::min(148, tiles * a.kv_heads)), dim3(256),
+                              0, s, b, a, q, q_stride, k, k_stride, v, v_stride, out, out_stride,
+                              static_cast<const int*>(flags), tiles, tile_rows);
         });
     });
 }

@@ -304,6 +304,22 @@ def test_packed_prompts(ops, dtype, heads, kv_heads, dim, lengths, window, sinks
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [32, 64, 128])
+def test_packed_tensors_of_any_alignment(ops, dtype, dim):
+    rng = np.random.default_rng(dim)
+    starts = [0, 150, 150, 201]
+    wide = tensor(rng.standard_normal((201, 6 * dim + 3)).astype(np.float32), dtype)
+    q, k, v = (wide[:, 1 + a * dim:1 + b * dim].unflatten(-1, (-1, dim)) for a, b in
+               ((0, 4), (4, 5), (5, 6)))
+    got = host(ops.attention_packed(q, k, v, ints(starts), window=70, sinks=3, scale=-0.2))
+    qh, kh, vh = host(q), host(k), host(v)
+    for a, b in ((0, 150), (150, 201)):
+        want, size = ref.attend(qh[a:b], kh[a:b], vh[a:b], 0, 70, 3, -0.2)
+        tol = bound(size, dim, b - a, np.abs(vh[a:b]).max(), want, dtype)
+        assert np.all(np.abs(got[a:b] - want) <= tol)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("value", [float("nan"), float("inf")])
 def test_packed_values_that_are_not_finite_reach_only_those_that_see_them(ops, dtype, dim, value):
