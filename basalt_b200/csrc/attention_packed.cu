@@ -50,7 +50,7 @@ struct KeyTiles {
 // ---- bf16 on the tensor cores ----------------------------------------------------------------
 // A CTA takes 256 query rows of one key head: tokens x heads of its group, so that heads sharing keys
 // share their tiles, and a tile of few tokens wastes little of a window. They are two M = 128 tiles
-// whose products alternate with their softmaxes: while eight warps (a thread a row) turn one tile's
+// whose products alternate with their softmaxes: while eight warps turn one tile's
 // scores into weights, the tensor cores work on the other's. Keys and values come in tiles of 128 by
 // TMA through a ring of 128-byte-swizzled buffers.
 //   TMEM, per tile: scores S (128 columns, float32), whose place the weights P take as bf16 and from
@@ -67,7 +67,10 @@ struct KeyTiles {
 // run out, raises its flag, and the plain kernel behind this one computes its rows again.
 
 constexpr int kTcRows = 256;
-constexpr int kTcThreads = 320;  // warps 0-3 and 4-7: a tile's rows; 8: products; 9: copies
+// Warps 0-7 and 8-15: a tile's rows, the first four of them columns 0-63, the others 64-127 (two
+// threads a row halve the time from scores to weights, which is what the other tile's products have
+// to cover; with one thread a row this took 143 us where it takes @@); 16: products; 17: copies.
+constexpr int kTcSoft = 512, kTcThreads = kTcSoft + 64;
 constexpr int kTcKeys = 128;
 
 template <int HD>
@@ -76,7 +79,9 @@ struct TcLayout {
     static constexpr int kSlots = 4;
     static constexpr int kBars = 2 * kTile + kSlots * kTile;
     // More than half of an SM's shared memory: one CTA an SM, which owns all of TMEM.
-    static constexpr int kBytes = kBars + 256 > 120 * 1024 ? kBars + 256 : 120 * 1024;
+    static constexpr int kExchange = kBars + 256;     // [2 tiles][2 parts][128] maxima or sums
+    static constexpr int kEnd = kExchange + 2 * 2 * 128 * 4;
+    static constexpr int kBytes = kEnd > 120 * 1024 ? kEnd : 120 * 1024;
     static constexpr int kSmem = kBytes + 1024;       // the base is aligned to 1024 bytes
 };
 
@@ -128,16 +133,14 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
 __device__ __forceinline__ void tmem_ld_wait() {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&r)[16]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
-        "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, "
-        "%29, %30, %31, %32};" ::"r"(addr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
-        "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
-        "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
-        "r"(r[29]), "r"(r[30]), "r"(r[31]));
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+        "%12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15])
+        : "r"(addr));
 }
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
     asm volatile(
@@ -149,6 +152,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_st_wait() {
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// The lowest n of 32 bits, for any n.
+__device__ __forceinline__ uint32_t first_bits(int n) {
+    return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u);
 }
 
 __device__ __forceinline__ bool not_finite(uint32_t pair) {  // of two bf16
@@ -196,32 +204,64 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(s_full + i, 1);
-            mbar_init(p_full + i, 128);
+            mbar_init(p_full + i, kTcSoft / 2);
         }
         status[0] = status[1] = status[2] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) {
+    if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                          smem_u32(tmem_slot)),
                      "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-    // Queries: a thread a row, 16-byte chunks into the swizzle. A negative scale moves into them.
-    const int my_row = tile.r0 + threadIdx.x;
-    const int my_token = my_row / group, my_head = kvh * group + my_row - my_token * group;
-    const bool live = static_cast<int>(threadIdx.x) < rows;
-    if (threadIdx.x < kTcRows) {
-        const uint4* src = reinterpret_cast<const uint4*>(
-            q + (tile.first + static_cast<int64_t>(my_token)) * q_stride + my_head * HD);
-        const int r = threadIdx.x & 127;
-        unsigned char* to = smem + (threadIdx.x >> 7) * L::kTile + r * 128;
+    // Token and head of the CTA's query row `at`: the quotient of two small numbers, in float.
+    const int r_first = tile.r0 - p0 * group;
+    const float by_group = 1.0f / static_cast<float>(group);
+    auto place = [&](int at, int* token, int* head) {
+        const int n = static_cast<int>((static_cast<float>(r_first + at) + 0.5f) * by_group);
+        *token = p0 + n;
+        *head = kvh * group + r_first + at - n * group;
+    };
+    __syncthreads();  // the barriers are there: copies may start
+    auto slot_at = [&](int i) { return base + 2 * L::kTile + (i % L::kSlots) * L::kTile; };
+    // Tile i's keys are copy 2 i, its values copy 2 i + 1.
+    const int copies = 2 * keys.tiles;
+    auto copy = [&](int i) {
+        const int slot = i % L::kSlots;
+        mbar_expect_tx(full + slot, L::kTile);
+        for (int x = 0; x < kBlocks; ++x) {
+            tma_load_2d(i & 1 ? &v_map : &k_map, full + slot,
+                        smem + 2 * L::kTile + slot * L::kTile + x * 16384, kvh * HD + 64 * x,
+                        tile.first + keys.key(i >> 1));
+        }
+    };
+    if (threadIdx.x == 17 * 32) {
+        for (int i = 0; i < min(copies, L::kSlots); ++i) copy(i);
+    }
+    // Queries, 16-byte chunks into the swizzle, all loads of a thread at once. A negative scale moves
+    // into them.
+    if (threadIdx.x < kTcSoft) {
         const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+        constexpr int kLoads = kTcRows * (HD / 8) / kTcSoft;
+        uint4 x[kLoads];
 #pragma unroll
-        for (int i = 0; i < HD / 8; ++i) {
-            uint4 x = live ? src[i] : make_uint4(0u, 0u, 0u, 0u);
-            x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
-            *reinterpret_cast<uint4*>(to + (i >> 3) * 16384 + (((i & 7) ^ (r & 7)) << 4)) = x;
+        for (int i = 0; i < kLoads; ++i) {
+            const int at = (threadIdx.x + i * kTcSoft) / (HD / 8), c = threadIdx.x % (HD / 8);
+            int token, head;
+            place(at, &token, &head);
+            x[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (at < rows) {
+                x[i] = *reinterpret_cast<const uint4*>(
+                    q + (tile.first + static_cast<int64_t>(token)) * q_stride + head * HD + 8 * c);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int at = (threadIdx.x + i * kTcSoft) / (HD / 8), c = threadIdx.x % (HD / 8), r = at & 127;
+            x[i].x ^= flip; x[i].y ^= flip; x[i].z ^= flip; x[i].w ^= flip;
+            *reinterpret_cast<uint4*>(smem + (at >> 7) * L::kTile + r * 128 + (c >> 3) * 16384 +
+                                      (((c & 7) ^ (r & 7)) << 4)) = x[i];
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -230,27 +270,14 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
     volatile int* const abort = status + 1;
-    auto slot_at = [&](int i) { return base + 2 * L::kTile + (i % L::kSlots) * L::kTile; };
-    // Tile i's keys are copy 2 i, its values copy 2 i + 1.
-    const int copies = 2 * keys.tiles;
-
-    if (warp == 9) {
+    if (warp == 17) {
         if (lane == 0) {
-            for (int i = 0; i < copies; ++i) {
-                const int slot = i % L::kSlots;
-                if (i >= L::kSlots &&
-                    !mbar_wait(empty + slot, ((i / L::kSlots) - 1) & 1, status, 1, abort)) {
-                    break;
-                }
-                mbar_expect_tx(full + slot, L::kTile);
-                for (int x = 0; x < kBlocks; ++x) {
-                    tma_load_2d(i & 1 ? &v_map : &k_map, full + slot,
-                                smem + 2 * L::kTile + slot * L::kTile + x * 16384,
-                                kvh * HD + 64 * x, tile.first + keys.key(i >> 1));
-                }
+            for (int i = L::kSlots; i < copies; ++i) {
+                if (!mbar_wait(empty + i % L::kSlots, ((i / L::kSlots) - 1) & 1, status, 1, abort)) break;
+                copy(i);
             }
         }
-    } else if (warp == 8) {
+    } else if (warp == 16) {
         if (lane == 0) {
             auto scores = [&](int half, int i) {  // S = Q K^T
                 const uint32_t d = tmem + half * 256;
@@ -298,29 +325,33 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
             }
         }
     } else {
-        const int half = warp >> 2;
+        const int half = warp >> 3, part = (warp >> 2) & 1, in_tile = 32 * (warp & 3) + lane;
+        const int at = 128 * half + in_tile;
+        int my_token, my_head;
+        place(at, &my_token, &my_head);
         const uint32_t s_at = tmem + half * 256 + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
-        const uint32_t o_at = s_at + 128;
+        const uint32_t o_at = s_at + 128 + part * (HD / 2);
+        float* const exchange = reinterpret_cast<float*>(smem + L::kExchange) + half * 256 + in_tile;
         const float scale = fabsf(a.scale) * kLog2e;
         // Rows behind the last query see nothing.
-        const int position = live ? my_token : -1;
+        const int position = at < rows ? my_token : -1;
         const int low = a.window ? position - a.window + 1 : 0;  // the window's first key
         const float slack = 8.0f / scale;                        // scale 0: infinite, never moved
         float top = -INFINITY, total = 0.0f;
         bool ok = half < halves;
         for (int i = 0; ok && i < keys.tiles; ++i) {
-            const int key0 = keys.key(i), cols = keys.cols(i);
-            // Whether all rows of the CTA see all of the tile's columns.
+            const int key0 = keys.key(i) + 64 * part;
+            const int chunks = min(2, (keys.cols(i) >> 5) - 2 * part);  // this thread's 32 columns
             const bool all = keys.whole(i, p0, p1, a.window);
             if (!all) {
-                // The CTA's rows (256 or 128 of them) search the values for what is not finite.
+                // The CTA's softmax threads search the values for what is not finite.
                 const int vc = 2 * i + 1;
                 ok = mbar_wait(full + vc % L::kSlots, (vc / L::kSlots) & 1, status, 6, abort);
                 if (!ok) break;
                 const uint4* v = reinterpret_cast<const uint4*>(smem + 2 * L::kTile +
                                                                 (vc % L::kSlots) * L::kTile);
                 bool bad = false;
-                for (int x = threadIdx.x; x < L::kTile / 16; x += 128 * halves) {
+                for (int x = threadIdx.x; x < L::kTile / 16; x += kTcSoft / 2 * halves) {
                     const uint4 u = v[x];
                     bad |= not_finite(u.x) || not_finite(u.y) || not_finite(u.z) || not_finite(u.w);
                 }
@@ -329,35 +360,38 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
             ok = mbar_wait(s_full + half, i & 1, status, 7, abort);
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            // Two passes over the scores, 32 columns at a time with the next 32 on their way: the
-            // maximum, then the weights (which fall on columns that have been read).
-            const int last = i < keys.sink_tiles ? min(position, keys.sink_end - 1) : position;
-            auto mask = [&](uint32_t(&s)[32], int c) {
-                const int at = key0 + 32 * c;
-#pragma unroll
-                for (int x = 0; x < 32; ++x) {
-                    const int key = at + x;
-                    const bool see = key <= last && (key >= low || key < a.sinks);
-                    if (!see) s[x] = 0xff800000u;
-                }
-            };
-            const int chunks = cols >> 5;
             uint32_t s[2][32];
-            float most = -INFINITY;
-            tmem_ld32(s_at, s[0]);
+            if (chunks > 0) tmem_ld32(s_at + 64 * part, s[0]);
+            if (chunks > 1) tmem_ld32(s_at + 64 * part + 32, s[1]);
+            tmem_ld_wait();
+            if (!all) {
+                // 32 columns' visibility as bits: below `last`, and from `low` on or below the sinks.
+                const int last = i < keys.sink_tiles ? min(position, keys.sink_end - 1) : position;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                if (c < chunks) {
-                    tmem_ld_wait();
-                    if (c + 1 < chunks) tmem_ld32(s_at + 32 * (c + 1), s[(c + 1) & 1]);
-                    if (!all) mask(s[c & 1], c);
-                    float m[2] = {-INFINITY, -INFINITY};
+                for (int c = 0; c < 2; ++c) {
+                    const int from = key0 + 32 * c;
+                    const uint32_t see = first_bits(last + 1 - from) &
+                                         (~first_bits(low - from) | first_bits(a.sinks - from));
 #pragma unroll
-                    for (int x = 0; x < 32; ++x) m[x & 1] = fmaxf(m[x & 1], __uint_as_float(s[c & 1][x]));
-                    most = fmaxf(most, fmaxf(m[0], m[1]));
+                    for (int x = 0; x < 32; ++x) {
+                        if (!((see >> x) & 1u)) s[c][x] = 0xff800000u;
+                    }
                 }
             }
-            tmem_ld32(s_at, s[0]);
+            float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                if (c < chunks) {
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) m[x & 3] = fmaxf(m[x & 3], __uint_as_float(s[c][x]));
+                }
+            }
+            // The row's other thread has the other columns. Behind the barrier both have read their
+            // scores, so that weights may be written over them.
+            float most = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+            exchange[128 * part] = most;
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + half), "n"(kTcSoft / 2) : "memory");
+            most = fmaxf(most, exchange[128 * (part ^ 1)]);
             const bool move = most > top + slack || (top == -INFINITY && most > top);
             if (__any_sync(kFull, move)) {
                 const float keep = move ? (top == -INFINITY ? 0.0f : exp2_fast((top - most) * scale)) : 1.0f;
@@ -366,34 +400,30 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
                 if (i > 0) {
 #pragma unroll
                     for (int c = 0; c < HD / 32; ++c) {
-                        uint32_t o[32];
-                        tmem_ld32(o_at + 32 * c, o);
+                        uint32_t o[16];
+                        tmem_ld16(o_at + 16 * c, o);
                         tmem_ld_wait();
 #pragma unroll
-                        for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * keep);
-                        tmem_st32(o_at + 32 * c, o);
+                        for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * keep);
+                        tmem_st16(o_at + 16 * c, o);
                     }
                 }
             }
             const float from = top == -INFINITY ? 0.0f : top * scale;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
+            for (int c = 0; c < 2; ++c) {
                 if (c < chunks) {
-                    tmem_ld_wait();
-                    if (c + 1 < chunks) tmem_ld32(s_at + 32 * (c + 1), s[(c + 1) & 1]);
-                    if (!all) mask(s[c & 1], c);
-                    uint32_t p[16];
                     float sum[2] = {0.0f, 0.0f};
 #pragma unroll
                     for (int x = 0; x < 16; ++x) {
-                        const float e0 = exp2_fast(fmaf(__uint_as_float(s[c & 1][2 * x]), scale, -from));
-                        const float e1 = exp2_fast(fmaf(__uint_as_float(s[c & 1][2 * x + 1]), scale, -from));
+                        const float e0 = exp2_fast(fmaf(__uint_as_float(s[c][2 * x]), scale, -from));
+                        const float e1 = exp2_fast(fmaf(__uint_as_float(s[c][2 * x + 1]), scale, -from));
                         sum[0] += e0;
                         sum[1] += e1;
-                        p[x] = pack2(e0, e1);
+                        s[c][x] = pack2(e0, e1);
                     }
                     total += sum[0] + sum[1];
-                    tmem_st16(s_at + 16 * c, p);
+                    tmem_st16(s_at + 32 * part + 16 * c, s[c]);
                 }
             }
             tmem_st_wait();
@@ -403,25 +433,42 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
         if (ok) ok = mbar_wait(s_full + half, keys.tiles & 1, status, 8, abort);
         if (ok) {
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            exchange[128 * part] = total;
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + half), "n"(kTcSoft / 2) : "memory");
+            total += exchange[128 * (part ^ 1)];
             const float by = total == 0.0f ? 0.0f : 1.0f / total;
-            uint4* to = reinterpret_cast<uint4*>(
-                out + (tile.first + static_cast<int64_t>(my_token)) * out_stride + my_head * HD);
+            // Through the queries' place in shared memory, so that rows are written whole.
+            unsigned char* const rows_at = smem + half * L::kTile;
 #pragma unroll
-            for (int c = 0; c < HD / 32; ++c) {
+            for (int c = 0; c < HD / 64; ++c) {
                 uint32_t o[32];
                 tmem_ld32(o_at + 32 * c, o);
                 tmem_ld_wait();
-                if (live) {
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        uint32_t w[4];
+                for (int x = 0; x < 4; ++x) {
+                    uint32_t w[4];
 #pragma unroll
-                        for (int y = 0; y < 4; ++y) {
-                            w[y] = pack2(__uint_as_float(o[8 * x + 2 * y]) * by,
-                                         __uint_as_float(o[8 * x + 2 * y + 1]) * by);
-                        }
-                        to[4 * c + x] = make_uint4(w[0], w[1], w[2], w[3]);
+                    for (int y = 0; y < 4; ++y) {
+                        w[y] = pack2(__uint_as_float(o[8 * x + 2 * y]) * by,
+                                     __uint_as_float(o[8 * x + 2 * y + 1]) * by);
                     }
+                    const int chunk = part * (HD / 16) + 4 * c + x;
+                    *reinterpret_cast<uint4*>(rows_at + in_tile * (HD * 2) +
+                                              ((chunk ^ (in_tile & 7)) << 4)) =
+                        make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + half), "n"(kTcSoft / 2) : "memory");
+#pragma unroll
+            for (int i = 0; i < 128 * (HD / 8) / (kTcSoft / 2); ++i) {
+                const int x = (threadIdx.x & (kTcSoft / 2 - 1)) + i * (kTcSoft / 2);
+                const int r = x / (HD / 8), c = x % (HD / 8);
+                if (128 * half + r < rows) {
+                    int token, head;
+                    place(128 * half + r, &token, &head);
+                    *reinterpret_cast<uint4*>(out + (tile.first + static_cast<int64_t>(token)) * out_stride +
+                                              head * HD + 8 * c) =
+                        *reinterpret_cast<const uint4*>(rows_at + r * (HD * 2) + ((c ^ (r & 7)) << 4));
                 }
             }
         }
@@ -436,7 +483,7 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
     }
     __syncthreads();
     if (threadIdx.x == 0) *flag = status[0] != 0 || status[2] != 0;
-    if (warp == 8) {
+    if (warp == 16) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
 }
@@ -488,7 +535,7 @@ __device__ __forceinline__ void attend_query(const T* q, const T* k, int64_t k_s
 template <typename T, int HD>
 struct MmaLayout {
     static constexpr int kRows = 64, kThreads = 128;
-    static constexpr int kKeys = HD == 128 ? 32 : 64;   // three CTAs an SM
+    static constexpr int kKeys = HD == 32 ? 64 : 32;    // three CTAs an SM
     static constexpr int kKPitch = HD + 8, kVPitch = HD + 4;
     static constexpr int kStage = kKeys * (kKPitch + kVPitch);  // floats
     static constexpr int kQPitch = HD + 8;
@@ -603,8 +650,11 @@ k_packed_mma(Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride, con
         const bool all = keys.whole(i, p0, p1, a.window);
         if (!all) {
             bool bad = false;
-            for (int x = threadIdx.x; x < L::kKeys * HD; x += L::kThreads) {
-                bad |= !(fabsf(vs[x / HD * L::kVPitch + x % HD]) <= FLT_MAX);
+            for (int x = threadIdx.x; x < L::kKeys * (HD / 4); x += L::kThreads) {
+                const float4 y = *reinterpret_cast<const float4*>(vs + x / (HD / 4) * L::kVPitch +
+                                                                  x % (HD / 4) * 4);
+                bad |= !(fabsf(y.x) <= FLT_MAX) || !(fabsf(y.y) <= FLT_MAX) ||
+                       !(fabsf(y.z) <= FLT_MAX) || !(fabsf(y.w) <= FLT_MAX);
             }
             if (bad) redo = 1;
         }
