@@ -49,35 +49,36 @@ struct KeyTiles {
 
 // ---- bf16 on the tensor cores ----------------------------------------------------------------
 // A CTA takes 256 query rows of one key head: tokens x heads of its group, so that heads sharing keys
-// share their tiles, and a tile of few tokens wastes little of a window. They are two M = 128 tiles
-// whose products alternate with their softmaxes: while eight warps turn one tile's
-// scores into weights, the tensor cores work on the other's. Keys and values come in tiles of 128 by
-// TMA through a ring of 128-byte-swizzled buffers.
-//   TMEM, per tile: scores S (128 columns, float32), whose place the weights P take as bf16 and from
-//   where the second product reads them as its A operand, and the output O (head_dim columns).
+// share their tiles, and a tile of few tokens wastes little of a window. They are two M = 128 tiles;
+// eight warps a tile turn scores into weights. Keys and values come in tiles of 64 by TMA through a
+// ring of 128-byte-swizzled buffers.
+//   TMEM, per tile: two buffers of scores S (64 columns each, float32), whose place the weights P
+//   take as bf16 and from where the second product reads them as its A operand, and the output O
+//   (head_dim columns). The next tile's scores are computed while a tile's weights are, so that the
+//   softmax, which is the longer part, never waits for a product it has just fed.
 //   O = P V reads V as it lies in memory (its B operand is MN-major).
 // The maximum that weights are taken against moves only when a row's grows by more than 2^8: the
-// softmax then rescales O itself, which is idle at that moment, because the scores it waits for were
-// issued behind the last product into O.
-// What bounds it: at head_dim 128 the products (4 x 128 x 128 x 128 multiply-adds a step, ~2900
-// cycles at the measured rate) outweigh the exponentials (32 768 at 16 a cycle, 2048 cycles).
+// softmax then waits for the last product into O and rescales O itself.
+// What bounds it: per 128 keys the exponentials (32 768 at 16 a cycle, 2048 cycles) beside the
+// products (4 x 128 x 128 x 128 multiply-adds, 2048 cycles at the nominal rate; the scores' half
+// takes half as long again, because 64 columns a product read Q from shared memory twice as often).
 //
 // Weights of keys that a row does not see are zero, but zero times a NaN or infinity is NaN. Tiles
 // that are partly hidden are searched for such values first; a CTA that meets one, or whose waits
 // run out, raises its flag, and the plain kernel behind this one computes its rows again.
 
 constexpr int kTcRows = 256;
-// Warps 0-7 and 8-15: a tile's rows, the first four of them columns 0-63, the others 64-127 (two
-// threads a row halve the time from scores to weights, which is what the other tile's products have
-// to cover; with one thread a row this took 143 us where it takes @@); 16: products; 17: copies.
+// Warps 0-7 and 8-15: a tile's rows, the first four of them columns 0-31, the others 32-63; 16:
+// products; 17: copies.
 constexpr int kTcSoft = 512, kTcThreads = kTcSoft + 64;
-constexpr int kTcKeys = 128;
+constexpr int kTcKeys = 64;
 
 template <int HD>
 struct TcLayout {
-    static constexpr int kTile = kTcKeys * HD * 2;    // a tile of keys, values or 128 query rows
-    static constexpr int kSlots = 4;
-    static constexpr int kBars = 2 * kTile + kSlots * kTile;
+    static constexpr int kQuery = 128 * HD * 2;       // a tile of query rows
+    static constexpr int kTile = kTcKeys * HD * 2;    // a tile of keys or values
+    static constexpr int kSlots = 8;
+    static constexpr int kBars = 2 * kQuery + kSlots * kTile;
     // More than half of an SM's shared memory: one CTA an SM, which owns all of TMEM.
     static constexpr int kExchange = kBars + 256;     // [2 tiles][2 parts][128] maxima or sums
     static constexpr int kEnd = kExchange + 2 * 2 * 128 * 4;
@@ -85,22 +86,33 @@ struct TcLayout {
     static constexpr int kSmem = kBytes + 1024;       // the base is aligned to 1024 bytes
 };
 
-// Accumulating or fresh product of kind::f16 with A from shared memory (a descriptor) or TMEM.
-__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                          uint32_t accumulate) {
-    const uint32_t z = 0;
+// Accumulating or fresh product of kind::f16 with A from shared memory or TMEM. Descriptors come as
+// their low words (the addresses, which move) and constant high words.
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t high,
+                                          uint32_t idesc, bool accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(z));
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(high), "r"(idesc), "r"(static_cast<uint32_t>(accumulate)));
 }
-__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
-                                          uint32_t accumulate) {
-    const uint32_t z = 0;
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t high,
+                                          uint32_t idesc, bool accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(z));
+        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "mov.b64 b, {%2, %3};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(high), "r"(idesc), "r"(static_cast<uint32_t>(accumulate)));
+}
+
+// One lane of a converged warp, in a way that leaves the warp's uniform registers usable (operands of
+// tcgen05.mma live there: behind a test of the lane number they have to be moved for every product,
+// which halved the rate).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}"
+                 : "=r"(one));
+    return one != 0;
 }
 
 // bf16 x bf16 -> float32, M = 128; b_mn: B is MN-major.
@@ -109,12 +121,13 @@ __device__ __forceinline__ uint32_t tc_idesc(int n, bool b_mn) {
            (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
 }
 
-// MN-major tile in the 128-byte swizzle: 64-channel columns of atoms 16 KB apart (leading offset),
-// atoms of eight keys 1024 bytes apart.
-__device__ __forceinline__ uint64_t tc_desc_mn(uint32_t addr) {
-    return static_cast<uint64_t>((addr >> 4) & 0x3fff) | (static_cast<uint64_t>(16384 >> 4) << 16) |
-           (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) |
-           (static_cast<uint64_t>(2) << 61);
+// Descriptor words. Both tiles' atoms of eight rows are 1024 bytes apart, in the 128-byte swizzle
+// (high word). Low words: a K-major tile; an MN-major tile, whose 64-channel columns of atoms are a
+// tile's 64 rows apart. A step of 16 channels is 32 bytes in the first, of 16 keys 2048 in the second.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_k(uint32_t addr) { return ((addr >> 4) & 0x3fffu) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_mn(uint32_t addr) {
+    return ((addr >> 4) & 0x3fffu) | ((kTcKeys * 128u >> 4) << 16);
 }
 
 // 32 columns of this thread's TMEM lane, without waiting for them.
@@ -169,7 +182,7 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
             Batch b, AttnSpec a, const __nv_bfloat16* __restrict__ q, int64_t q_stride,
             __nv_bfloat16* __restrict__ out, int64_t out_stride, int* __restrict__ flags) {
     using L = TcLayout<HD>;
-    constexpr int kBlocks = HD / 64;     // 128-byte columns of a tile, 16 KB each
+    constexpr int kBlocks = HD / 64;     // 128-byte columns of a tile
     extern __shared__ unsigned char raw[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int group = a.heads / a.kv_heads, kvh = blockIdx.y;
@@ -192,9 +205,10 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
     uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
     uint64_t* const full = bars;                 // [kSlots] a copy has arrived
     uint64_t* const empty = full + L::kSlots;    // [kSlots] its readers are done
-    uint64_t* const s_full = empty + L::kSlots;  // [2] scores (and all products before) are done
-    uint64_t* const p_full = s_full + 2;         // [2] weights are written
-    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(p_full + 2);
+    uint64_t* const s_full = empty + L::kSlots;  // [tile][buffer] scores are done
+    uint64_t* const p_full = s_full + 4;         // [tile][buffer] weights are written
+    uint64_t* const o_done = p_full + 4;         // [tile] a product into O is done
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(o_done + 2);
     int* const status = reinterpret_cast<int*>(tmem_slot + 1);  // [0] error code, [1] abort, [2] redo
 
     if (threadIdx.x == 0) {
@@ -202,10 +216,12 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
             mbar_init(full + i, 1);
             mbar_init(empty + i, 1);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < 4; ++i) {
             mbar_init(s_full + i, 1);
             mbar_init(p_full + i, kTcSoft / 2);
         }
+        mbar_init(o_done, 1);
+        mbar_init(o_done + 1, 1);
         status[0] = status[1] = status[2] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -224,17 +240,24 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
         *head = kvh * group + r_first + at - n * group;
     };
     __syncthreads();  // the barriers are there: copies may start
-    auto slot_at = [&](int i) { return base + 2 * L::kTile + (i % L::kSlots) * L::kTile; };
-    // Tile i's keys are copy 2 i, its values copy 2 i + 1.
+    auto slot_at = [&](int i) { return base + 2 * L::kQuery + (i % L::kSlots) * L::kTile; };
+    // The copies in the order in which they are used: K0 K1 V0 K2 V1 K3 ... V(n-1).
     const int copies = 2 * keys.tiles;
+    auto k_copy = [&](int i) { return i == 0 ? 0 : 2 * i - 1; };
+    auto v_copy = [&](int i) { return i == keys.tiles - 1 ? 2 * i + 1 : 2 * i + 2; };
     auto copy = [&](int i) {
+        const bool of_keys = i == 0 || ((i & 1) && i != copies - 1);
+        const int at = i == 0 ? 0 : (of_keys ? (i + 1) / 2 : (i == copies - 1 ? keys.tiles - 1 : i / 2 - 1));
         const int slot = i % L::kSlots;
         mbar_expect_tx(full + slot, L::kTile);
         for (int x = 0; x < kBlocks; ++x) {
-            tma_load_2d(i & 1 ? &v_map : &k_map, full + slot,
-                        smem + 2 * L::kTile + slot * L::kTile + x * 16384, kvh * HD + 64 * x,
-                        tile.first + keys.key(i >> 1));
+            tma_load_2d(of_keys ? &k_map : &v_map, full + slot,
+                        smem + 2 * L::kQuery + slot * L::kTile + x * (kTcKeys * 128),
+                        kvh * HD + 64 * x, tile.first + keys.key(at));
         }
+    };
+    auto await = [&](int i, int code, volatile int* abort) {
+        return mbar_wait(full + i % L::kSlots, (i / L::kSlots) & 1, status, code, abort);
     };
     if (threadIdx.x == 17 * 32) {
         for (int i = 0; i < min(copies, L::kSlots); ++i) copy(i);
@@ -260,7 +283,7 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
         for (int i = 0; i < kLoads; ++i) {
             const int at = (threadIdx.x + i * kTcSoft) / (HD / 8), c = threadIdx.x % (HD / 8), r = at & 127;
             x[i].x ^= flip; x[i].y ^= flip; x[i].z ^= flip; x[i].w ^= flip;
-            *reinterpret_cast<uint4*>(smem + (at >> 7) * L::kTile + r * 128 + (c >> 3) * 16384 +
+            *reinterpret_cast<uint4*>(smem + (at >> 7) * L::kQuery + r * 128 + (c >> 3) * 16384 +
                                       (((c & 7) ^ (r & 7)) << 4)) = x[i];
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -278,51 +301,63 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
             }
         }
     } else if (warp == 16) {
-        if (lane == 0) {
-            auto scores = [&](int half, int i) {  // S = Q K^T
-                const uint32_t d = tmem + half * 256;
-                const uint32_t qa = base + half * L::kTile, ka = slot_at(2 * i);
-                const uint32_t idesc = tc_idesc(keys.cols(i), false);
+        // The whole warp keeps time; one lane issues. All of it is the same in every lane.
+        const uint32_t u_tmem = __shfl_sync(kFull, tmem, 0), u_base = __shfl_sync(kFull, base, 0);
+        const int n_tiles = __shfl_sync(kFull, keys.tiles, 0), n_halves = __shfl_sync(kFull, halves, 0);
+        auto slot = [&](int i) { return u_base + 2 * L::kQuery + (i % L::kSlots) * L::kTile; };
+        auto scores = [&](int half, int i, int cols) {  // S = Q K^T
+            const uint32_t d = u_tmem + half * 256 + (i & 1) * 64;
+            const uint32_t qa = desc_k(u_base + half * L::kQuery), ka = desc_k(slot(k_copy(i)));
+            const uint32_t idesc = tc_idesc(cols, false);
 #pragma unroll
-                for (int k = 0; k < HD / 16; ++k) {
-                    const uint32_t at = (k >> 2) * 16384 + (k & 3) * 32;
-                    tc_mma_ss(d, smem_desc(qa + at), smem_desc(ka + at), idesc, k > 0);
-                }
-                mma_commit(s_full + half);
-            };
-            bool ok = mbar_wait(full, 0, status, 2, abort);
-            if (ok) {
+            for (int k = 0; k < HD / 16; ++k) {
+                tc_mma_ss(d, qa + (k >> 2) * (16384 >> 4) + (k & 3) * 2,
+                          ka + (k >> 2) * (kTcKeys * 128 >> 4) + (k & 3) * 2, kDescHigh, idesc, k > 0);
+            }
+            mma_commit(s_full + 2 * half + (i & 1));
+        };
+        bool ok = true;
+        for (int i = 0; ok && i < min(2, n_tiles); ++i) {
+            ok = await(k_copy(i), 2, abort);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const int cols = __shfl_sync(kFull, keys.cols(i), 0);
+            if (elect_one()) {
+                for (int h = 0; h < n_halves; ++h) scores(h, i, cols);
+                mma_commit(empty + k_copy(i) % L::kSlots);
+            }
+            __syncwarp();
+        }
+        const uint32_t idesc = tc_idesc(HD, true);
+        for (int i = 0; ok && i < n_tiles; ++i) {
+            const bool more = i + 2 < n_tiles;
+            ok = await(v_copy(i), 3, abort) && (!more || await(k_copy(i + 2), 4, abort));
+            const int steps = __shfl_sync(kFull, keys.cols(i), 0) / 16;
+            const int cols = more ? __shfl_sync(kFull, keys.cols(i + 2), 0) : 0;
+            const uint32_t va = desc_mn(slot(v_copy(i)));
+            for (int h = 0; ok && h < n_halves; ++h) {
+                ok = mbar_wait(p_full + 2 * h + (i & 1), (i >> 1) & 1, status, 5, abort);
+                if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                for (int h = 0; h < halves; ++h) scores(h, 0);
-                mma_commit(empty);
-            }
-            for (int i = 0; ok && i < keys.tiles; ++i) {
-                const int vc = 2 * i + 1, kc = 2 * i + 2;
-                const bool more = i + 1 < keys.tiles;
-                ok = mbar_wait(full + vc % L::kSlots, (vc / L::kSlots) & 1, status, 3, abort) &&
-                     (!more || mbar_wait(full + kc % L::kSlots, (kc / L::kSlots) & 1, status, 4, abort));
-                const uint32_t idesc = tc_idesc(HD, true);
-                const int steps = keys.cols(i) / 16;
-                for (int h = 0; ok && h < halves; ++h) {
-                    ok = mbar_wait(p_full + h, i & 1, status, 5, abort);
-                    if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t d = tmem + h * 256 + 128, p = tmem + h * 256;
-                    const uint32_t va = slot_at(vc);
-                    for (int k = 0; k < steps; ++k) {  // O += P V
-                        tc_mma_ts(d, p + 8 * k, tc_desc_mn(va + k * 2048), idesc, i > 0 || k > 0);
+                const uint32_t d = u_tmem + h * 256 + 128, p = u_tmem + h * 256 + (i & 1) * 64;
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < kTcKeys / 16; ++k) {  // O += P V
+                        if (k < steps) {
+                            tc_mma_ts(d, p + 8 * k, va + k * (2048 >> 4), kDescHigh, idesc, i > 0 || k > 0);
+                        }
                     }
-                    if (more) {
-                        scores(h, i + 1);
-                    } else {
-                        mma_commit(s_full + h);
-                    }
+                    mma_commit(o_done + h);
+                    // Into the buffer that the product above has just read.
+                    if (more) scores(h, i + 2, cols);
                 }
-                if (ok) {
-                    mma_commit(empty + vc % L::kSlots);
-                    if (more) mma_commit(empty + kc % L::kSlots);
-                }
+                __syncwarp();
             }
+            if (ok && elect_one()) {
+                mma_commit(empty + v_copy(i) % L::kSlots);
+                if (more) mma_commit(empty + k_copy(i + 2) % L::kSlots);
+            }
+            __syncwarp();
         }
     } else {
         const int half = warp >> 3, part = (warp >> 2) & 1, in_tile = 32 * (warp & 3) + lane;
@@ -338,18 +373,19 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
         const int low = a.window ? position - a.window + 1 : 0;  // the window's first key
         const float slack = 8.0f / scale;                        // scale 0: infinite, never moved
         float top = -INFINITY, total = 0.0f;
-        bool ok = half < halves;
-        for (int i = 0; ok && i < keys.tiles; ++i) {
-            const int key0 = keys.key(i) + 64 * part;
-            const int chunks = min(2, (keys.cols(i) >> 5) - 2 * part);  // this thread's 32 columns
+        // A wait that runs out ends no loop here: the tile's threads meet at barriers in every step,
+        // and what they write then is computed again.
+        bool ok = true;
+        for (int i = 0; half < halves && i < keys.tiles; ++i) {
+            const int key0 = keys.key(i) + 32 * part;
+            const uint32_t buffer = s_at + (i & 1) * 64;
+            const bool mine = keys.cols(i) > 32 * part;  // this thread's 32 columns are there
             const bool all = keys.whole(i, p0, p1, a.window);
             if (!all) {
                 // The CTA's softmax threads search the values for what is not finite.
-                const int vc = 2 * i + 1;
-                ok = mbar_wait(full + vc % L::kSlots, (vc / L::kSlots) & 1, status, 6, abort);
-                if (!ok) break;
-                const uint4* v = reinterpret_cast<const uint4*>(smem + 2 * L::kTile +
-                                                                (vc % L::kSlots) * L::kTile);
+                ok = ok && await(v_copy(i), 6, abort);
+                const uint4* v = reinterpret_cast<const uint4*>(smem + 2 * L::kQuery +
+                                                                (v_copy(i) % L::kSlots) * L::kTile);
                 bool bad = false;
                 for (int x = threadIdx.x; x < L::kTile / 16; x += kTcSoft / 2 * halves) {
                     const uint4 u = v[x];
@@ -357,34 +393,28 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
                 }
                 if (bad) status[2] = 1;
             }
-            ok = mbar_wait(s_full + half, i & 1, status, 7, abort);
-            if (!ok) break;
+            ok = ok && mbar_wait(s_full + 2 * half + (i & 1), (i >> 1) & 1, status, 7, abort);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            uint32_t s[2][32];
-            if (chunks > 0) tmem_ld32(s_at + 64 * part, s[0]);
-            if (chunks > 1) tmem_ld32(s_at + 64 * part + 32, s[1]);
-            tmem_ld_wait();
-            if (!all) {
-                // 32 columns' visibility as bits: below `last`, and from `low` on or below the sinks.
-                const int last = i < keys.sink_tiles ? min(position, keys.sink_end - 1) : position;
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const int from = key0 + 32 * c;
-                    const uint32_t see = first_bits(last + 1 - from) &
-                                         (~first_bits(low - from) | first_bits(a.sinks - from));
+            uint32_t s[32];
+            if (mine) {
+                tmem_ld32(buffer + 32 * part, s);
+                tmem_ld_wait();
+                if (!all) {
+                    // The columns' visibility as bits: below `last`, and from `low` on or below the
+                    // sinks.
+                    const int last = i < keys.sink_tiles ? min(position, keys.sink_end - 1) : position;
+                    const uint32_t see = first_bits(last + 1 - key0) &
+                                         (~first_bits(low - key0) | first_bits(a.sinks - key0));
 #pragma unroll
                     for (int x = 0; x < 32; ++x) {
-                        if (!((see >> x) & 1u)) s[c][x] = 0xff800000u;
+                        if (!((see >> x) & 1u)) s[x] = 0xff800000u;
                     }
                 }
             }
             float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            if (mine) {
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                if (c < chunks) {
-#pragma unroll
-                    for (int x = 0; x < 32; ++x) m[x & 3] = fmaxf(m[x & 3], __uint_as_float(s[c][x]));
-                }
+                for (int x = 0; x < 32; ++x) m[x & 3] = fmaxf(m[x & 3], __uint_as_float(s[x]));
             }
             // The row's other thread has the other columns. Behind the barrier both have read their
             // scores, so that weights may be written over them.
@@ -398,6 +428,8 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
                 if (move) top = most;
                 total *= keep;
                 if (i > 0) {
+                    ok = ok && mbar_wait(o_done + half, (i - 1) & 1, status, 8, abort);
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
                     for (int c = 0; c < HD / 32; ++c) {
                         uint32_t o[16];
@@ -410,35 +442,34 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
                 }
             }
             const float from = top == -INFINITY ? 0.0f : top * scale;
+            if (mine) {
+                float sum[2] = {0.0f, 0.0f};
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                if (c < chunks) {
-                    float sum[2] = {0.0f, 0.0f};
-#pragma unroll
-                    for (int x = 0; x < 16; ++x) {
-                        const float e0 = exp2_fast(fmaf(__uint_as_float(s[c][2 * x]), scale, -from));
-                        const float e1 = exp2_fast(fmaf(__uint_as_float(s[c][2 * x + 1]), scale, -from));
-                        sum[0] += e0;
-                        sum[1] += e1;
-                        s[c][x] = pack2(e0, e1);
-                    }
-                    total += sum[0] + sum[1];
-                    tmem_st16(s_at + 32 * part + 16 * c, s[c]);
+                for (int x = 0; x < 16; ++x) {
+                    const float e0 = exp2_fast(fmaf(__uint_as_float(s[2 * x]), scale, -from));
+                    const float e1 = exp2_fast(fmaf(__uint_as_float(s[2 * x + 1]), scale, -from));
+                    sum[0] += e0;
+                    sum[1] += e1;
+                    s[x] = pack2(e0, e1);
                 }
+                total += sum[0] + sum[1];
+                tmem_st16(buffer + 16 * part, s);
             }
             tmem_st_wait();
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            mbar_arrive(p_full + half);
+            mbar_arrive(p_full + 2 * half + (i & 1));
         }
-        if (ok) ok = mbar_wait(s_full + half, keys.tiles & 1, status, 8, abort);
-        if (ok) {
+        if (half < halves) {
+            // The last two products into O (those before were done when the last scores were).
+            if (keys.tiles > 1) ok = ok && mbar_wait(o_done + half, keys.tiles & 1, status, 9, abort);
+            ok = ok && mbar_wait(o_done + half, (keys.tiles - 1) & 1, status, 10, abort);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             exchange[128 * part] = total;
             asm volatile("bar.sync %0, %1;" ::"r"(1 + half), "n"(kTcSoft / 2) : "memory");
             total += exchange[128 * (part ^ 1)];
             const float by = total == 0.0f ? 0.0f : 1.0f / total;
             // Through the queries' place in shared memory, so that rows are written whole.
-            unsigned char* const rows_at = smem + half * L::kTile;
+            unsigned char* const rows_at = smem + half * L::kQuery;
 #pragma unroll
             for (int c = 0; c < HD / 64; ++c) {
                 uint32_t o[32];
