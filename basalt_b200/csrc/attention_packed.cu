@@ -50,7 +50,7 @@ struct KeyTiles {
 // ---- bf16 on the tensor cores ----------------------------------------------------------------
 // A CTA takes 256 query rows of one key head: tokens x heads of its group, so that heads sharing keys
 // share their tiles, and a tile of few tokens wastes little of a window. They are two M = 128 tiles;
-// eight warps a tile turn scores into weights. Keys and values come in tiles of 64 by TMA through a
+// four warps a tile turn scores into weights. Keys and values come in tiles of 64 by TMA through a
 // ring of 128-byte-swizzled buffers.
 //   TMEM, per tile: two buffers of scores S (64 columns each, float32), whose place the weights P
 //   take as bf16 and from where the second product reads them as its A operand, and the output O
@@ -68,9 +68,9 @@ struct KeyTiles {
 // run out, raises its flag, and the plain kernel behind this one computes its rows again.
 
 constexpr int kTcRows = 256;
-// Warps 0-7 and 8-15: a tile's rows, the first four of them columns 0-31, the others 32-63; 16:
-// products; 17: copies.
-constexpr int kTcSoft = 512, kTcThreads = kTcSoft + 64;
+// Warps 0-3 and 4-7: a tile's rows, a thread each; 8: products; 9: copies. (Two threads a row were
+// slower: their meeting in every step kept both tiles' softmaxes in step with one another.)
+constexpr int kTcSoft = 256, kTcThreads = kTcSoft + 64;
 constexpr int kTcKeys = 64;
 
 template <int HD>
@@ -80,8 +80,7 @@ struct TcLayout {
     static constexpr int kSlots = 8;
     static constexpr int kBars = 2 * kQuery + kSlots * kTile;
     // More than half of an SM's shared memory: one CTA an SM, which owns all of TMEM.
-    static constexpr int kExchange = kBars + 256;     // [2 tiles][2 parts][128] maxima or sums
-    static constexpr int kEnd = kExchange + 2 * 2 * 128 * 4;
+    static constexpr int kEnd = kBars + 256;
     static constexpr int kBytes = kEnd > 120 * 1024 ? kEnd : 120 * 1024;
     static constexpr int kSmem = kBytes + 1024;       // the base is aligned to 1024 bytes
 };
@@ -145,15 +144,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
 }
 __device__ __forceinline__ void tmem_ld_wait() {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
-        "%12, %13, %14, %15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-          "=r"(r[14]), "=r"(r[15])
-        : "r"(addr));
 }
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
     asm volatile(
@@ -225,7 +215,7 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
         status[0] = status[1] = status[2] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 16) {
+    if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                          smem_u32(tmem_slot)),
                      "r"(512));
@@ -259,7 +249,7 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
     auto await = [&](int i, int code, volatile int* abort) {
         return mbar_wait(full + i % L::kSlots, (i / L::kSlots) & 1, status, code, abort);
     };
-    if (threadIdx.x == 17 * 32) {
+    if (threadIdx.x == 9 * 32) {
         for (int i = 0; i < min(copies, L::kSlots); ++i) copy(i);
     }
     // Queries, 16-byte chunks into the swizzle, all loads of a thread at once. A negative scale moves
@@ -293,14 +283,14 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
     volatile int* const abort = status + 1;
-    if (warp == 17) {
+    if (warp == 9) {
         if (lane == 0) {
             for (int i = L::kSlots; i < copies; ++i) {
                 if (!mbar_wait(empty + i % L::kSlots, ((i / L::kSlots) - 1) & 1, status, 1, abort)) break;
                 copy(i);
             }
         }
-    } else if (warp == 16) {
+    } else if (warp == 8) {
         // The whole warp keeps time; one lane issues. All of it is the same in every lane.
         const uint32_t u_tmem = __shfl_sync(kFull, tmem, 0), u_base = __shfl_sync(kFull, base, 0);
         const int n_tiles = __shfl_sync(kFull, keys.tiles, 0), n_halves = __shfl_sync(kFull, halves, 0);
@@ -360,28 +350,34 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
             __syncwarp();
         }
     } else {
-        const int half = warp >> 3, part = (warp >> 2) & 1, in_tile = 32 * (warp & 3) + lane;
-        const int at = 128 * half + in_tile;
+        const int half = warp >> 2, in_tile = threadIdx.x & 127, at = 128 * half + in_tile;
         int my_token, my_head;
         place(at, &my_token, &my_head);
         const uint32_t s_at = tmem + half * 256 + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
-        const uint32_t o_at = s_at + 128 + part * (HD / 2);
-        float* const exchange = reinterpret_cast<float*>(smem + L::kExchange) + half * 256 + in_tile;
+        const uint32_t o_at = s_at + 128;
         const float scale = fabsf(a.scale) * kLog2e;
         // Rows behind the last query see nothing.
         const int position = at < rows ? my_token : -1;
         const int low = a.window ? position - a.window + 1 : 0;  // the window's first key
         const float slack = 8.0f / scale;                        // scale 0: infinite, never moved
-        float top = -INFINITY, total = 0.0f;
-        // A wait that runs out ends no loop here: the tile's threads meet at barriers in every step,
-        // and what they write then is computed again.
+        float top = -INFINITY, from = 0.0f, total = 0.0f;
+        // A wait that runs out ends no loop here: the tile's threads meet at a barrier behind it, and
+        // what they write then is computed again.
         bool ok = true;
+        int key0 = keys.key(0);
         for (int i = 0; half < halves && i < keys.tiles; ++i) {
-            const int key0 = keys.key(i) + 32 * part;
             const uint32_t buffer = s_at + (i & 1) * 64;
-            const bool mine = keys.cols(i) > 32 * part;  // this thread's 32 columns are there
-            const bool all = keys.whole(i, p0, p1, a.window);
-            if (!all) {
+            // Most tiles lie inside every row's window and have all of their columns.
+            const bool inside = i >= keys.sink_tiles && key0 + kTcKeys - 1 <= p0 &&
+                                (a.window == 0 || p1 - key0 < a.window);
+            uint32_t s[2][32];
+            if (inside) {
+                ok = ok && mbar_wait(s_full + 2 * half + (i & 1), (i >> 1) & 1, status, 7, abort);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                tmem_ld32(buffer, s[0]);
+                tmem_ld32(buffer + 32, s[1]);
+                tmem_ld_wait();
+            } else {
                 // The CTA's softmax threads search the values for what is not finite.
                 ok = ok && await(v_copy(i), 6, abort);
                 const uint4* v = reinterpret_cast<const uint4*>(smem + 2 * L::kQuery +
@@ -392,86 +388,82 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
                     bad |= not_finite(u.x) || not_finite(u.y) || not_finite(u.z) || not_finite(u.w);
                 }
                 if (bad) status[2] = 1;
-            }
-            ok = ok && mbar_wait(s_full + 2 * half + (i & 1), (i >> 1) & 1, status, 7, abort);
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            uint32_t s[32];
-            if (mine) {
-                tmem_ld32(buffer + 32 * part, s);
+                ok = ok && mbar_wait(s_full + 2 * half + (i & 1), (i >> 1) & 1, status, 7, abort);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                tmem_ld32(buffer, s[0]);
+                tmem_ld32(buffer + 32, s[1]);
                 tmem_ld_wait();
-                if (!all) {
-                    // The columns' visibility as bits: below `last`, and from `low` on or below the
-                    // sinks.
-                    const int last = i < keys.sink_tiles ? min(position, keys.sink_end - 1) : position;
-                    const uint32_t see = first_bits(last + 1 - key0) &
-                                         (~first_bits(low - key0) | first_bits(a.sinks - key0));
+                // The columns' visibility as bits: below `last`, and from `low` on or below the sinks.
+                // Columns that were not multiplied are behind `last` for every row.
+                const int last = i < keys.sink_tiles ? min(position, keys.sink_end - 1) : position;
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int first = key0 + 32 * c;
+                    const uint32_t see = first_bits(last + 1 - first) &
+                                         (~first_bits(low - first) | first_bits(a.sinks - first));
 #pragma unroll
                     for (int x = 0; x < 32; ++x) {
-                        if (!((see >> x) & 1u)) s[x] = 0xff800000u;
+                        if (!((see >> x) & 1u)) s[c][x] = 0xff800000u;
                     }
                 }
             }
             float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            if (mine) {
 #pragma unroll
-                for (int x = 0; x < 32; ++x) m[x & 3] = fmaxf(m[x & 3], __uint_as_float(s[x]));
-            }
-            // The row's other thread has the other columns. Behind the barrier both have read their
-            // scores, so that weights may be written over them.
-            float most = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-            exchange[128 * part] = most;
-            asm volatile("bar.sync %0, %1;" ::"r"(1 + half), "n"(kTcSoft / 2) : "memory");
-            most = fmaxf(most, exchange[128 * (part ^ 1)]);
+            for (int x = 0; x < 64; ++x) m[x & 3] = fmaxf(m[x & 3], __uint_as_float(s[x >> 5][x & 31]));
+            const float most = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
             const bool move = most > top + slack || (top == -INFINITY && most > top);
             if (__any_sync(kFull, move)) {
                 const float keep = move ? (top == -INFINITY ? 0.0f : exp2_fast((top - most) * scale)) : 1.0f;
-                if (move) top = most;
+                if (move) {
+                    top = most;
+                    from = top * scale;
+                }
                 total *= keep;
                 if (i > 0) {
                     ok = ok && mbar_wait(o_done + half, (i - 1) & 1, status, 8, abort);
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
                     for (int c = 0; c < HD / 32; ++c) {
-                        uint32_t o[16];
-                        tmem_ld16(o_at + 16 * c, o);
+                        uint32_t o[32];
+                        tmem_ld32(o_at + 32 * c, o);
                         tmem_ld_wait();
 #pragma unroll
-                        for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * keep);
-                        tmem_st16(o_at + 16 * c, o);
+                        for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * keep);
+                        tmem_st16(o_at + 32 * c, o);
+                        tmem_st16(o_at + 32 * c + 16, o + 16);
                     }
                 }
             }
-            const float from = top == -INFINITY ? 0.0f : top * scale;
-            if (mine) {
-                float sum[2] = {0.0f, 0.0f};
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                uint32_t p[16];
 #pragma unroll
                 for (int x = 0; x < 16; ++x) {
-                    const float e0 = exp2_fast(fmaf(__uint_as_float(s[2 * x]), scale, -from));
-                    const float e1 = exp2_fast(fmaf(__uint_as_float(s[2 * x + 1]), scale, -from));
-                    sum[0] += e0;
-                    sum[1] += e1;
-                    s[x] = pack2(e0, e1);
+                    const float e0 = exp2_fast(fmaf(__uint_as_float(s[c][2 * x]), scale, -from));
+                    const float e1 = exp2_fast(fmaf(__uint_as_float(s[c][2 * x + 1]), scale, -from));
+                    sum[(2 * x) & 3] += e0;
+                    sum[(2 * x + 1) & 3] += e1;
+                    p[x] = pack2(e0, e1);
                 }
-                total += sum[0] + sum[1];
-                tmem_st16(buffer + 16 * part, s);
+                tmem_st16(buffer + 16 * c, p);
             }
+            total += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             tmem_st_wait();
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             mbar_arrive(p_full + 2 * half + (i & 1));
+            key0 = i + 1 == keys.sink_tiles ? keys.first : key0 + kTcKeys;
         }
         if (half < halves) {
             // The last two products into O (those before were done when the last scores were).
             if (keys.tiles > 1) ok = ok && mbar_wait(o_done + half, keys.tiles & 1, status, 9, abort);
             ok = ok && mbar_wait(o_done + half, (keys.tiles - 1) & 1, status, 10, abort);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            exchange[128 * part] = total;
-            asm volatile("bar.sync %0, %1;" ::"r"(1 + half), "n"(kTcSoft / 2) : "memory");
-            total += exchange[128 * (part ^ 1)];
             const float by = total == 0.0f ? 0.0f : 1.0f / total;
             // Through the queries' place in shared memory, so that rows are written whole.
             unsigned char* const rows_at = smem + half * L::kQuery;
 #pragma unroll
-            for (int c = 0; c < HD / 64; ++c) {
+            for (int c = 0; c < HD / 32; ++c) {
                 uint32_t o[32];
                 tmem_ld32(o_at + 32 * c, o);
                 tmem_ld_wait();
@@ -483,16 +475,15 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
                         w[y] = pack2(__uint_as_float(o[8 * x + 2 * y]) * by,
                                      __uint_as_float(o[8 * x + 2 * y + 1]) * by);
                     }
-                    const int chunk = part * (HD / 16) + 4 * c + x;
                     *reinterpret_cast<uint4*>(rows_at + in_tile * (HD * 2) +
-                                              ((chunk ^ (in_tile & 7)) << 4)) =
+                                              (((4 * c + x) ^ (in_tile & 7)) << 4)) =
                         make_uint4(w[0], w[1], w[2], w[3]);
                 }
             }
             asm volatile("bar.sync %0, %1;" ::"r"(1 + half), "n"(kTcSoft / 2) : "memory");
-#pragma unroll
+#pragma unroll 4
             for (int i = 0; i < 128 * (HD / 8) / (kTcSoft / 2); ++i) {
-                const int x = (threadIdx.x & (kTcSoft / 2 - 1)) + i * (kTcSoft / 2);
+                const int x = in_tile + i * (kTcSoft / 2);
                 const int r = x / (HD / 8), c = x % (HD / 8);
                 if (128 * half + r < rows) {
                     int token, head;
@@ -514,7 +505,7 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
     }
     __syncthreads();
     if (threadIdx.x == 0) *flag = status[0] != 0 || status[2] != 0;
-    if (warp == 16) {
+    if (warp == 8) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
 }
