@@ -38,29 +38,30 @@ __device__ __forceinline__ float bf16_up_positive(float x) {
     return __uint_as_float((u & 0xffffu) ? (u & 0xffff0000u) + 0x10000u : u);
 }
 
-// step of a group with this low and maximum. The quotient in double, rounded up to bf16. In float
-// with directed roundings the two bounds nearly always round to the same bf16; only where they do
-// not is the double quotient taken.
+// step of a group with this low and maximum: the quotient in double, rounded up to bf16. Products
+// with the two floats around 1 / 15 enclose the quotient; nearly always both round up to the same
+// bf16, and only where they do not is the double quotient taken.
 __device__ __forceinline__ float group_step(float low, float high) {
-    const float up = bf16_up_positive(__fdiv_ru(__fsub_ru(high, low), 15.0f));
-    const float down = bf16_up_positive(__fdiv_rd(__fsub_rd(high, low), 15.0f));
+    const float up = bf16_up_positive(__fmul_ru(__fsub_ru(high, low), __uint_as_float(0x3d888889u)));
+    const float down = bf16_up_positive(__fmul_rd(__fsub_rd(high, low), __uint_as_float(0x3d888888u)));
     if (up == down) return up;
     const double d = (static_cast<double>(high) - static_cast<double>(low)) / 15.0;
-    float f = __double2float_ru(d);
-    return bf16_up_positive(f);
+    return bf16_up_positive(__double2float_ru(d));
 }
 
-// rint((x - low) / step) of the double quotient, in 0..15. The float quotient is within
-// 15 * 3 * 2^-24 < 3e-6 of it, so only quotients within 1e-5 of a tie need the double.
+// rint((x - low) / step) of the double quotient, in 0..15. The float quotient q is within
+// 15 * 3 * 2^-24 < 3e-6 of it, so only a q within 1e-5 of a tie needs the double (and one that is no
+// number, where step's reciprocal overflows). Adding 1.5 * 2^23 rounds q to nearest even and leaves
+// it in the lowest bits.
 __device__ __forceinline__ uint32_t code_of(float x, float low, float step, float inverse) {
-    float q = __fmul_rn(__fsub_rn(x, low), inverse);
-    const float f = q - floorf(q);
-    if (!(fabsf(f - 0.5f) > 1e-5f) || !(q < 16.0f)) {
+    const float q = __fmul_rn(__fsub_rn(x, low), inverse);
+    const float moved = __fadd_rn(q, 12582912.0f);
+    if (!(fabsf(__fsub_rn(q, __fsub_rn(moved, 12582912.0f))) <= 0.49999f)) {
         const double d = (static_cast<double>(x) - static_cast<double>(low)) /
                          static_cast<double>(step);
-        q = static_cast<float>(fmin(rint(d), 15.0));
+        return static_cast<uint32_t>(fmin(rint(d), 15.0));
     }
-    return static_cast<uint32_t>(fminf(rintf(q), 15.0f));
+    return __float_as_uint(moved) & 15u;
 }
 
 template <typename T>
@@ -123,149 +124,179 @@ __device__ __forceinline__ int64_t entry_of(const Cache& c, const Batch& b, int 
     return static_cast<int64_t>(row) * c.kv_heads * c.slots + slot;  // head h adds h * slots
 }
 
-// blockIdx.y: 0 keys, 1 values. Eight lanes per (token, head).
+// A CTA's tokens: `per` of them from blockIdx.x * per on, whose entries its first threads look up.
+// Eight lanes take a head of a token (a unit); blockIdx.y: 0 keys, 1 values.
+constexpr int kMaxTokens = 32;
+
+struct Units {
+    int first, count;   // tokens
+    int heads;
+    __device__ Units(const Cache& c, const Batch& b, int per, int64_t* entries) {
+        first = blockIdx.x * per;
+        count = min(per, b.tokens - first);
+        heads = c.kv_heads;
+        if (static_cast<int>(threadIdx.x) < count) {
+            entries[threadIdx.x] = entry_of(c, b, first + threadIdx.x);
+        }
+        __syncthreads();
+    }
+};
+
 template <typename T, int HD, int STORAGE>
 __global__ void __launch_bounds__(kThreads)
-k_kv_append(Cache c, Batch b, const T* __restrict__ k, int64_t k_stride, const T* __restrict__ v,
-            int64_t v_stride, bool vector) {
+k_kv_append(Cache c, Batch b, int per, const T* __restrict__ k, int64_t k_stride,
+            const T* __restrict__ v, int64_t v_stride, bool vector) {
     constexpr int G = HD / 32;
-    const int64_t unit = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) >> 3;
+    __shared__ int64_t entries[kMaxTokens];
     const int h8 = threadIdx.x & 7;
     const bool values = blockIdx.y != 0;
-    const bool live = unit < static_cast<int64_t>(b.tokens) * c.kv_heads;
-    const int t = live ? static_cast<int>(unit / c.kv_heads) : 0;
-    const int head = live ? static_cast<int>(unit - static_cast<int64_t>(t) * c.kv_heads) : 0;
-    const int64_t entry = live ? entry_of(c, b, t) : -1;
-    // Lanes without an entry keep running: the shuffles below take the whole warp.
-    float x[G][4];
-    const T* src = (values ? v + t * v_stride : k + t * k_stride) + head * HD + 4 * h8;
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-        if (entry >= 0) {
-            load4<T>(src + 32 * g, vector, x[g]);
-        } else {
-            x[g][0] = x[g][1] = x[g][2] = x[g][3] = 0.0f;
-        }
-    }
-    const int64_t at = entry + static_cast<int64_t>(head) * c.slots;
-    if constexpr (STORAGE == BST_DTYPE_U4) {
-        uint32_t half[G];
-        uint32_t scale = 0;
+    const Units units(c, b, per, entries);
+    const int most = (units.count * units.heads + kThreads / 8 - 1) / (kThreads / 8);
+    for (int turn = 0; turn < most; ++turn) {
+        const unsigned unit = turn * (kThreads / 8) + (threadIdx.x >> 3);
+        const int at_token = unit / static_cast<unsigned>(units.heads);
+        const int head = unit - at_token * units.heads;
+        const int64_t t = units.first + at_token;
+        const int64_t entry = at_token < units.count ? entries[at_token] : -1;
+        // Lanes without an entry keep running: the shuffles below take the whole warp.
+        float x[G][4];
+        const T* src = (values ? v + t * v_stride : k + t * k_stride) + head * HD + 4 * h8;
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-            float lo = x[g][0], hi = x[g][0], worst = fabsf(x[g][0]);
-            bool bad = !(worst <= FLT_MAX);
-#pragma unroll
-            for (int i = 1; i < 4; ++i) {
-                lo = fminf(lo, x[g][i]);
-                hi = fmaxf(hi, x[g][i]);
-                bad |= !(fabsf(x[g][i]) <= FLT_MAX);
-            }
-#pragma unroll
-            for (int o = 4; o > 0; o >>= 1) {
-                lo = fminf(lo, __shfl_xor_sync(kFull, lo, o));
-                hi = fmaxf(hi, __shfl_xor_sync(kFull, hi, o));
-                bad |= __shfl_xor_sync(kFull, static_cast<int>(bad), o) != 0;
-            }
-            const float low = bf16_down(lo);
-            bad |= isinf(low);
-            const float step = bad ? 0.0f : group_step(low, hi);
-            uint32_t codes = 0;
-            if (step > 0.0f) {
-                // A reciprocal of a step below the normal range is no float: code_of then sees a
-                // quotient that is not below 16 and takes the double.
-                const float inverse = __frcp_rn(step);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) codes |= code_of(x[g][i], low, step, inverse) << (4 * i);
-            }
-            half[g] = codes;
-            if (h8 == g) {
-                scale = bad ? (0x7fc0u << 16)
-                            : (__float_as_uint(step) >> 16) | (__float_as_uint(low) & 0xffff0000u);
+            if (entry >= 0) {
+                load4<T>(src + 32 * g, vector, x[g]);
+            } else {
+                x[g][0] = x[g][1] = x[g][2] = x[g][3] = 0.0f;
             }
         }
-        if (entry < 0) return;
-        unsigned char* codes = static_cast<unsigned char*>(values ? c.v : c.k) + at * (HD / 2);
-        if constexpr (G == 1) {
-            reinterpret_cast<uint16_t*>(codes)[h8] = static_cast<uint16_t>(half[0]);
-        } else if constexpr (G == 2) {
-            reinterpret_cast<uint32_t*>(codes)[h8] = half[0] | (half[1] << 16);
+        const int64_t at = entry + static_cast<int64_t>(head) * c.slots;
+        if constexpr (STORAGE == BST_DTYPE_U4) {
+            // Extremes of the groups; then lane g computes the scale of group g for all eight.
+            float low_mine = 0.0f, high_mine = 0.0f;
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                float lo = fminf(fminf(x[g][0], x[g][1]), fminf(x[g][2], x[g][3]));
+                float hi = fmaxf(fmaxf(x[g][0], x[g][1]), fmaxf(x[g][2], x[g][3]));
+                // fminf and fmaxf pass over a NaN.
+                bool bad = !(fabsf(x[g][0]) <= FLT_MAX) || !(fabsf(x[g][1]) <= FLT_MAX) ||
+                           !(fabsf(x[g][2]) <= FLT_MAX) || !(fabsf(x[g][3]) <= FLT_MAX);
+                if (bad) hi = INFINITY;
+#pragma unroll
+                for (int o = 4; o > 0; o >>= 1) {
+                    lo = fminf(lo, __shfl_xor_sync(kFull, lo, o));
+                    hi = fmaxf(hi, __shfl_xor_sync(kFull, hi, o));
+                }
+                if (h8 == g) {
+                    low_mine = bf16_down(lo);
+                    high_mine = hi;
+                }
+            }
+            const bool bad = !(high_mine <= FLT_MAX) || isinf(low_mine);
+            const float step_mine = bad ? 0.0f : group_step(low_mine, high_mine);
+            const uint32_t scale = bad ? (0x7fc0u << 16)
+                                       : (__float_as_uint(step_mine) >> 16) |
+                                             (__float_as_uint(low_mine) & 0xffff0000u);
+            uint32_t half[G];
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const uint32_t pair = __shfl_sync(kFull, scale, (threadIdx.x & 24) | g);
+                const float step = bf16_bits_to_f(pair & 0xffffu), low = bf16_bits_to_f(pair >> 16);
+                half[g] = 0u;
+                if (step > 0.0f) {
+                    const float inverse = __frcp_rn(step);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) half[g] |= code_of(x[g][i], low, step, inverse) << (4 * i);
+                }
+            }
+            if (entry < 0) continue;
+            unsigned char* codes = static_cast<unsigned char*>(values ? c.v : c.k) + at * (HD / 2);
+            if constexpr (G == 1) {
+                reinterpret_cast<uint16_t*>(codes)[h8] = static_cast<uint16_t>(half[0]);
+            } else if constexpr (G == 2) {
+                reinterpret_cast<uint32_t*>(codes)[h8] = half[0] | (half[1] << 16);
+            } else {
+                reinterpret_cast<uint2*>(codes)[h8] =
+                    make_uint2(half[0] | (half[1] << 16), half[2] | (half[3] << 16));
+            }
+            if (h8 < G) static_cast<uint32_t*>(values ? c.v_scale : c.k_scale)[at * G + h8] = scale;
         } else {
-            reinterpret_cast<uint2*>(codes)[h8] =
-                make_uint2(half[0] | (half[1] << 16), half[2] | (half[3] << 16));
-        }
-        if (h8 < G) static_cast<uint32_t*>(values ? c.v_scale : c.k_scale)[at * G + h8] = scale;
-    } else {
-        using S = typename std::conditional<STORAGE == BST_DTYPE_F32, float, __nv_bfloat16>::type;
-        if (entry < 0) return;
-        S* dst = static_cast<S*>(values ? c.v : c.k) + at * HD + 4 * h8;
+            using S = typename std::conditional<STORAGE == BST_DTYPE_F32, float, __nv_bfloat16>::type;
+            if (entry < 0) continue;
+            S* dst = static_cast<S*>(values ? c.v : c.k) + at * HD + 4 * h8;
 #pragma unroll
-        for (int g = 0; g < G; ++g) store4<S>(dst + 32 * g, true, x[g]);
+            for (int g = 0; g < G; ++g) store4<S>(dst + 32 * g, true, x[g]);
+        }
     }
 }
 
 template <typename T, int HD, int STORAGE>
 __global__ void __launch_bounds__(kThreads)
-k_kv_read(Cache c, Batch b, T* __restrict__ k, int64_t k_stride, T* __restrict__ v,
+k_kv_read(Cache c, Batch b, int per, T* __restrict__ k, int64_t k_stride, T* __restrict__ v,
           int64_t v_stride, bool vector) {
     constexpr int G = HD / 32;
-    const int64_t unit = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) >> 3;
+    __shared__ int64_t entries[kMaxTokens];
     const int h8 = threadIdx.x & 7;
     const bool values = blockIdx.y != 0;
-    if (unit >= static_cast<int64_t>(b.tokens) * c.kv_heads) return;
-    const int t = static_cast<int>(unit / c.kv_heads);
-    const int head = static_cast<int>(unit - static_cast<int64_t>(t) * c.kv_heads);
-    const int64_t entry = entry_of(c, b, t);
-    if (entry == -1) return;
-    T* dst = (values ? v + t * v_stride : k + t * k_stride) + head * HD + 4 * h8;
-    const int64_t at = entry + static_cast<int64_t>(head) * c.slots;
-    float x[G][4] = {};
-    if (entry >= 0) {
-        if constexpr (STORAGE == BST_DTYPE_U4) {
-            const unsigned char* codes =
-                static_cast<const unsigned char*>(values ? c.v : c.k) + at * (HD / 2);
-            const uint32_t* scale =
-                static_cast<const uint32_t*>(values ? c.v_scale : c.k_scale) + at * G;
-            uint32_t half[G];
-            if constexpr (G == 1) {
-                half[0] = reinterpret_cast<const uint16_t*>(codes)[h8];
-            } else if constexpr (G == 2) {
-                const uint32_t w = reinterpret_cast<const uint32_t*>(codes)[h8];
-                half[0] = w & 0xffffu;
-                half[1] = w >> 16;
-            } else {
-                const uint2 w = reinterpret_cast<const uint2*>(codes)[h8];
-                half[0] = w.x & 0xffffu;
-                half[1] = w.x >> 16;
-                half[2] = w.y & 0xffffu;
-                half[3] = w.y >> 16;
-            }
-#pragma unroll
-            for (int g = 0; g < G; ++g) {
-                const uint32_t s = scale[g];
-                const float step = bf16_bits_to_f(s & 0xffffu), low = bf16_bits_to_f(s >> 16);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    // code * step is exact, so this rounds once.
-                    x[g][i] = fmaf(static_cast<float>((half[g] >> (4 * i)) & 15u), step, low);
+    const Units units(c, b, per, entries);
+#pragma unroll 2
+    for (unsigned unit = threadIdx.x >> 3; unit < static_cast<unsigned>(units.count * units.heads);
+         unit += kThreads / 8) {
+        const int at_token = unit / static_cast<unsigned>(units.heads);
+        const int head = unit - at_token * units.heads;
+        const int64_t t = units.first + at_token, entry = entries[at_token];
+        if (entry == -1) continue;
+        T* dst = (values ? v + t * v_stride : k + t * k_stride) + head * HD + 4 * h8;
+        const int64_t at = entry + static_cast<int64_t>(head) * c.slots;
+        float x[G][4] = {};
+        if (entry >= 0) {
+            if constexpr (STORAGE == BST_DTYPE_U4) {
+                const unsigned char* codes =
+                    static_cast<const unsigned char*>(values ? c.v : c.k) + at * (HD / 2);
+                const uint32_t* scale =
+                    static_cast<const uint32_t*>(values ? c.v_scale : c.k_scale) + at * G;
+                uint32_t half[G];
+                if constexpr (G == 1) {
+                    half[0] = reinterpret_cast<const uint16_t*>(codes)[h8];
+                } else if constexpr (G == 2) {
+                    const uint32_t w = reinterpret_cast<const uint32_t*>(codes)[h8];
+                    half[0] = w & 0xffffu;
+                    half[1] = w >> 16;
+                } else {
+                    const uint2 w = reinterpret_cast<const uint2*>(codes)[h8];
+                    half[0] = w.x & 0xffffu;
+                    half[1] = w.x >> 16;
+                    half[2] = w.y & 0xffffu;
+                    half[3] = w.y >> 16;
                 }
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    const uint32_t s = scale[g];
+                    const float step = bf16_bits_to_f(s & 0xffffu), low = bf16_bits_to_f(s >> 16);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        // code * step is exact, so this rounds once.
+                        x[g][i] = fmaf(static_cast<float>((half[g] >> (4 * i)) & 15u), step, low);
+                    }
+                }
+            } else {
+                using S = typename std::conditional<STORAGE == BST_DTYPE_F32, float, __nv_bfloat16>::type;
+                const S* src = static_cast<const S*>(values ? c.v : c.k) + at * HD + 4 * h8;
+#pragma unroll
+                for (int g = 0; g < G; ++g) load4<S>(src + 32 * g, true, x[g]);
             }
-        } else {
-            using S = typename std::conditional<STORAGE == BST_DTYPE_F32, float, __nv_bfloat16>::type;
-            const S* src = static_cast<const S*>(values ? c.v : c.k) + at * HD + 4 * h8;
-#pragma unroll
-            for (int g = 0; g < G; ++g) load4<S>(src + 32 * g, true, x[g]);
         }
-    }
 #pragma unroll
-    for (int g = 0; g < G; ++g) store4<T>(dst + 32 * g, vector, x[g]);
+        for (int g = 0; g < G; ++g) store4<T>(dst + 32 * g, vector, x[g]);
+    }
 }
 
 template <typename T, int HD, bool APPEND>
 cudaError_t launch_storage(cudaStream_t s, const Cache& c, const Batch& b, void* k, int64_t ks,
                            void* v, int64_t vs) {
-    const int64_t units = static_cast<int64_t>(b.tokens) * c.kv_heads;
-    const dim3 grid(static_cast<unsigned>((units * 8 + kThreads - 1) / kThreads), 2);
+    // Tokens a CTA: one while that fills the SMs, then up to 32, at least two units a thread.
+    int per = std::max(1, 64 / c.kv_heads);
+    per = std::max(1, std::min({per, kMaxTokens, b.tokens / (148 * 4)}));
+    const dim3 grid(static_cast<unsigned>((b.tokens + per - 1) / per), 2);
     const size_t four = 4 * sizeof(T);
     const bool vector = reinterpret_cast<uintptr_t>(k) % four == 0 &&
                         reinterpret_cast<uintptr_t>(v) % four == 0 && ks % 4 == 0 && vs % 4 == 0;
@@ -273,9 +304,9 @@ cudaError_t launch_storage(cudaStream_t s, const Cache& c, const Batch& b, void*
     T* vv = static_cast<T*>(v);
 #define BST_KV(STORAGE)                                                                     \
     if constexpr (APPEND) {                                                                 \
-        k_kv_append<T, HD, STORAGE><<<grid, kThreads, 0, s>>>(c, b, kk, ks, vv, vs, vector); \
+        k_kv_append<T, HD, STORAGE><<<grid, kThreads, 0, s>>>(c, b, per, kk, ks, vv, vs, vector); \
     } else {                                                                                \
-        k_kv_read<T, HD, STORAGE><<<grid, kThreads, 0, s>>>(c, b, kk, ks, vv, vs, vector);   \
+        k_kv_read<T, HD, STORAGE><<<grid, kThreads, 0, s>>>(c, b, per, kk, ks, vv, vs, vector);   \
     }
     if (c.storage == BST_DTYPE_U4) {
         BST_KV(BST_DTYPE_U4)

@@ -16,23 +16,29 @@ new output is undefined, in a given one it stays.
 from __future__ import annotations
 
 import ctypes
-import math
 
 from . import _lib
 from .text_engine import (BasaltShapeException, BasaltUnsupportedOperationException,
                           IllegalArgumentException, _raise)
 
-_CODES = {"torch.float32": _lib.DTYPE_F32, "torch.bfloat16": _lib.DTYPE_BF16}
+_CODES = {}   # torch dtype -> BST_DTYPE_*, filled with the module below
+_module = None
 
 
 def _torch():
-    import torch
+    global _module
+    if _module is None:
+        import torch
 
-    return torch
+        _CODES.update({torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16})
+        _module = torch
+    return _module
 
 
 def _dtype(name, t):
-    code = _CODES.get(str(t.dtype))
+    if _module is None:
+        _torch()
+    code = _CODES.get(t.dtype)
     if code is None:
         raise BasaltUnsupportedOperationException(
             f"{name}: {t.dtype} is not float32 or bfloat16", _lib.BST_UNSUPPORTED)
@@ -40,8 +46,9 @@ def _dtype(name, t):
 
 
 def _on(device, name, t):
-    if not t.is_cuda or t.device != device:
-        raise IllegalArgumentException(f"{name} is on {t.device}, expected {device}",
+    if t.device != device or not t.is_cuda:
+        raise IllegalArgumentException(f"{name} is on {t.device}, expected "
+                                       f"{device if device.type == 'cuda' else 'a CUDA device'}",
                                        _lib.BST_INVALID)
 
 
@@ -49,8 +56,9 @@ def _index(device, name, t, size=None):
     """The pointer of an int32 index tensor, or None."""
     if t is None:
         return None
-    _on(device, name, t)
-    if str(t.dtype) != "torch.int32" or t.dim() != 1 or not t.is_contiguous():
+    if t.device != device:
+        _on(device, name, t)
+    if t.dtype is not _module.int32 or t.dim() != 1 or not t.is_contiguous():
         raise IllegalArgumentException(f"{name} must be a contiguous int32 vector",
                                        _lib.BST_INVALID)
     if size is not None and t.shape[0] != size:
@@ -61,13 +69,15 @@ def _index(device, name, t, size=None):
 
 def _packed(device, name, t, heads=None, head_dim=None):
     """Checks a [tokens, heads, head_dim] tensor whose heads are contiguous; its token stride."""
-    _on(device, name, t)
-    if t.dim() != 3:
+    if t.device != device:
+        _on(device, name, t)
+    shape = t.shape
+    if len(shape) != 3:
         raise BasaltShapeException(f"{name} must be [tokens, heads, head_dim], got "
-                                   f"{tuple(t.shape)}", _lib.BST_SHAPE)
-    n, h, d = t.shape
+                                   f"{tuple(shape)}", _lib.BST_SHAPE)
+    n, h, d = shape
     if (heads is not None and h != heads) or (head_dim is not None and d != head_dim):
-        raise BasaltShapeException(f"{name} is {tuple(t.shape)}, expected [tokens, {heads}, "
+        raise BasaltShapeException(f"{name} is {tuple(shape)}, expected [tokens, {heads}, "
                                    f"{head_dim}]", _lib.BST_SHAPE)
     stride = t.stride()
     if (d > 1 and stride[2] != 1) or (h > 1 and stride[1] != d):
@@ -77,7 +87,9 @@ def _packed(device, name, t, heads=None, head_dim=None):
 
 
 def _stream(device, stream):
-    return _torch().cuda.current_stream(device).cuda_stream if stream is None else stream
+    if stream is not None:
+        return stream
+    return _module.cuda.current_stream(device).cuda_stream
 
 
 class KvCache:
@@ -89,8 +101,10 @@ class KvCache:
     """
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
+        _torch()
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.device = k.device
+        self._sizes = {}  # workspace bytes by what they depend on
         u4 = str(k.dtype) == "torch.uint8"
         if u4 != (k_scale is not None) or u4 != (v_scale is not None):
             raise IllegalArgumentException("a 4-bit cache, and only that, has scales",
@@ -143,22 +157,16 @@ class KvCache:
 
 def _sequences(device, tokens, lengths, starts, rows):
     """The batch's struct; the tensors it points to belong to the caller."""
-    s = _lib.SequencesStruct()
     if lengths is not None:
-        s.lengths = _index(device, "lengths", lengths)
-        s.count = lengths.shape[0]
-        if starts is not None:
-            s.starts = _index(device, "starts", starts, s.count + 1)
+        at = _index(device, "lengths", lengths)
+        count = lengths.shape[0]
     else:
-        s.starts = _index(device, "starts", starts)
-        s.count = starts.shape[0] - 1
-        if s.count < 0:
+        at, count = None, starts.shape[0] - 1
+        if count < 0:
             raise BasaltShapeException("starts must have one entry more than there are sequences",
                                        _lib.BST_SHAPE)
-    if rows is not None:
-        s.rows = _index(device, "rows", rows, s.count)
-    s.tokens = tokens
-    return s
+    return _lib.SequencesStruct(count, tokens, _index(device, "rows", rows, count),
+                                _index(device, "starts", starts, count + 1), at)
 
 
 def kv_append(cache: KvCache, k, v, lengths, starts=None, rows=None, stream=None):
@@ -182,20 +190,25 @@ def kv_read(cache: KvCache, lengths, starts=None, rows=None, tokens=None, dtype=
     fill; otherwise new ones of ``dtype`` (float32)."""
     device = cache.device
     if out is None:
-        torch = _torch()
         if tokens is None:
             if starts is not None:
                 raise IllegalArgumentException("kv_read needs tokens or out beside starts",
                                                _lib.BST_INVALID)
             tokens = lengths.shape[0]
         shape = (tokens, cache.kv_heads, cache.head_dim)
-        out = tuple(torch.empty(shape, dtype=dtype or torch.float32, device=device) for _ in range(2))
-    k, v = out
-    k_stride = _packed(device, "k", k, cache.kv_heads, cache.head_dim)
-    v_stride = _packed(device, "v", v, cache.kv_heads, cache.head_dim)
-    if k.dtype != v.dtype or k.shape[0] != v.shape[0]:
-        raise BasaltShapeException("k and v must have the same type and tokens", _lib.BST_SHAPE)
-    s = _sequences(device, k.shape[0], lengths, starts, rows)
+        dtype = dtype or _module.float32
+        k = _module.empty(shape, dtype=dtype, device=device)
+        v = _module.empty(shape, dtype=dtype, device=device)
+        k_stride = v_stride = cache.kv_heads * cache.head_dim
+    else:
+        k, v = out
+        k_stride = _packed(device, "k", k, cache.kv_heads, cache.head_dim)
+        v_stride = _packed(device, "v", v, cache.kv_heads, cache.head_dim)
+        tokens = k.shape[0]
+        if k.dtype != v.dtype or tokens != v.shape[0]:
+            raise BasaltShapeException("k and v must have the same type and tokens",
+                                       _lib.BST_SHAPE)
+    s = _sequences(device, tokens, lengths, starts, rows)
     _raise(_lib.load().bst_kv_read(device.index, _stream(device, stream), cache._ref, s,
                                    k.data_ptr(), k_stride, v.data_ptr(), v_stride,
                                    _dtype("k", k)))
@@ -203,17 +216,16 @@ def kv_read(cache: KvCache, lengths, starts=None, rows=None, tokens=None, dtype=
 
 
 def _spec(q, kv_heads, window, sinks, scale):
-    a = _lib.AttentionSpecStruct()
-    a.heads, a.kv_heads, a.head_dim = q.shape[1], kv_heads, q.shape[2]
-    a.dtype, a.window, a.sinks = _dtype("q", q), window, sinks
-    a.scale = 1.0 / math.sqrt(max(1, q.shape[2])) if scale is None else scale
-    return a
+    _, heads, dim = q.shape
+    return _lib.AttentionSpecStruct(heads, kv_heads, dim, _dtype("q", q), window, sinks,
+                                    dim ** -0.5 if scale is None and dim else scale or 0.0, 0)
 
 
 def _out(device, q, out):
     if out is None:
-        out = _torch().empty(q.shape, dtype=q.dtype, device=device)
-    elif out.dtype != q.dtype or out.shape != q.shape:
+        out = _module.empty(q.shape, dtype=q.dtype, device=device)
+        return out, q.shape[1] * q.shape[2]
+    if out.dtype != q.dtype or out.shape != q.shape:
         raise BasaltShapeException("out must be like q", _lib.BST_SHAPE)
     return out, _packed(device, "out", out)
 
@@ -223,7 +235,8 @@ def _workspace(device, size, workspace):
     if workspace is None:
         if size == 0:
             return None, 0, None
-        workspace = _torch().empty(size, dtype=_torch().uint8, device=device)
+        workspace = _module.empty(size, dtype=_module.uint8, device=device)
+        return workspace.data_ptr(), size, workspace
     _on(device, "workspace", workspace)
     return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
 
@@ -239,9 +252,13 @@ def attention_cached(cache: KvCache, q, lengths, starts=None, rows=None, window:
     s = _sequences(device, q.shape[0], lengths, starts, rows)
     a = _spec(q, cache.kv_heads, window, sinks, scale)
     lib = _lib.load()
-    size = ctypes.c_int64(0)
-    _raise(lib.bst_attention_cached_workspace(cache._ref, s, a, size))
-    pointer, room, workspace = _workspace(device, size.value, workspace)
+    key = (s.count, s.tokens, starts is None, a.heads, a.dtype, window, sinks)
+    needed = cache._sizes.get(key)
+    if needed is None:
+        size = ctypes.c_int64(0)
+        _raise(lib.bst_attention_cached_workspace(cache._ref, s, a, size))
+        needed = cache._sizes[key] = size.value
+    pointer, room, workspace = _workspace(device, needed, workspace)
     _raise(lib.bst_attention_cached(device.index, _stream(device, stream), cache._ref, s, a,
                                     q.data_ptr(), q_stride, out.data_ptr(), out_stride, pointer,
                                     room))
@@ -252,7 +269,9 @@ def attention_packed(q, k, v, starts, window: int = 0, sinks: int = 0, scale=Non
                      workspace=None, stream=None):
     """Causal attention of packed sequences over their own keys and values: q [tokens, heads,
     head_dim], k and v [tokens, kv_heads, head_dim], all of one type."""
+    _torch()
     device = q.device
+    _on(device, "q", q)
     q_stride = _packed(device, "q", q)
     k_stride = _packed(device, "k", k, None, q.shape[2])
     v_stride = _packed(device, "v", v, k.shape[1], q.shape[2])
@@ -287,6 +306,7 @@ def sample_tokens(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0
     """int32 tokens drawn from logits [rows, vocabulary] (float32 or bfloat16) with ``uniforms``
     (float64, one in [0, 1) per row). Each setting is a number or one value per row (float32, top_k
     int32, on the device). Rows with nothing to draw give -1."""
+    _torch()
     device = logits.device
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise BasaltShapeException("logits must be [rows, vocabulary] with contiguous rows",
@@ -294,12 +314,12 @@ def sample_tokens(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0
     _on(device, "logits", logits)
     rows, vocabulary = logits.shape
     _on(device, "uniforms", uniforms)
-    if str(uniforms.dtype) != "torch.float64" or tuple(uniforms.shape) != (rows,) or \
+    if uniforms.dtype is not _module.float64 or tuple(uniforms.shape) != (rows,) or \
             not uniforms.is_contiguous():
         raise IllegalArgumentException(f"uniforms must be a contiguous float64 vector of {rows}",
                                        _lib.BST_INVALID)
     if out is None:
-        out = _torch().empty(rows, dtype=_torch().int32, device=device)
+        out = _module.empty(rows, dtype=_module.int32, device=device)
     else:
         _index(device, "out", out, rows)
     p = _lib.SamplingStruct()
