@@ -3,17 +3,24 @@
 // With z = (logit - largest) / temperature the weight of a token is exp(z), held as a 64-bit whole
 // number of units of 2^-42 (so 2^20 tokens cannot overflow it). Sums of whole numbers do not depend
 // on their order: any number of threads may add in any order, with atomics, and a draw still comes
-// out the same. Weights below 2^-40 count as nothing.
+// out the same. Weights below 2^-40 count as nothing. The exponential is a double one, because a
+// draw among 10^5 tokens is decided by differences of 10^-10 of their sum: 2^(k / 32) from a table
+// times the Taylor polynomial of 2^r, |r| <= 1/64, of degree five (2^-48): eleven double operations,
+// where the library's function for all arguments takes four times as many.
 //
-// No sort. All filters keep a prefix of the order (logit descending, index ascending), so each is a
-// threshold: the smallest logit kept and how many of the tokens with exactly that logit. A threshold
-// is found by histograms of 2048 bins: the first over the distance from the largest logit (spreads
-// the tokens evenly, where bits of the float would pile them on a few bins), then over the bits of
-// the logits inside the bin where the sum crosses, until a bin is one value. The draw itself is a
-// running sum over slices of the row, then inside one slice.
+// No sort of the row. All filters keep a prefix of the order (logit descending, index ascending), so
+// each is a threshold: the smallest logit kept and how many of the tokens with exactly that logit. A
+// histogram of 2048 bins over the distance from the largest logit (which spreads the tokens evenly,
+// where bits of the float would pile them on a few bins) finds the bin in which the sum of counts or
+// weights crosses, and the few tokens in that bin are sorted. (Should it hold more than fit, more
+// histograms follow, over the bits of its logits.) A top_k that fits the list itself needs no more:
+// its candidates are collected with their indices and one CTA finishes on them. Otherwise the draw is
+// a running sum over slices of the row, then inside one slice.
 //
-// A row is worked on by a cluster of CTAs, each with a slice of the row in its shared memory; sums
-// and histograms meet through distributed shared memory.
+// A row is worked on by a cluster of CTAs, each with a slice of the row in its shared memory; sums,
+// histograms and lists meet through distributed shared memory. The row is read once; what bounds the
+// kernel are its passes over the slices in shared memory, the double operations, and for few rows the
+// latency of the steps between them.
 
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -49,13 +56,48 @@ __device__ __forceinline__ float float_of(uint32_t key) {
     return __uint_as_float(key ^ ((key >> 31) ? 0x80000000u : 0xffffffffu));
 }
 
+constexpr int kList = 2048;   // tokens that a list holds
+
 struct Shared {
-    u64 bins[kBins];
+    uint32_t low[kBins], high[kBins];  // a histogram's 64-bit sums; both halves are a list otherwise
     u64 coarse[kCoarse];
+    double powers[32];                 // 2^(k / 32)
+    unsigned listed;                   // tokens that asked for a place in the list
     u64 exchange[2][2];     // this CTA's value of a reduction over the cluster, two pairs in turn
     u64 warp_a[kWarps], warp_b[kWarps];
     u64 result[4];
+    u64 padding;  // the slice behind it is 16-byte aligned
 };
+static_assert(kList * 8 == kBins * 8, "a list lies in the histogram's place");
+
+// A histogram's 64-bit sum grows by v: two native 32-bit additions, the carry by hand.
+__device__ __forceinline__ void add_to(Shared& sh, int bin, u64 v) {
+    const uint32_t lo = static_cast<uint32_t>(v);
+    uint32_t hi = static_cast<uint32_t>(v >> 32);
+    if (lo && atomicAdd(&sh.low[bin], lo) > 0xffffffffu - lo) ++hi;
+    if (hi) atomicAdd(&sh.high[bin], hi);
+}
+
+// A list lies in the histogram's place.
+__device__ __forceinline__ u64* list_of(Shared* sh) { return reinterpret_cast<u64*>(sh->low); }
+
+// Sorts v[0 .. n) (n a power of two) in descending order, with the whole CTA.
+__device__ __forceinline__ void sort_descending(u64* v, int n) {
+    for (int size = 2; size <= n; size <<= 1) {
+        for (int stride = size >> 1; stride > 0; stride >>= 1) {
+            __syncthreads();
+            for (int x = threadIdx.x; x < n / 2; x += kThreads) {
+                const int i = 2 * x - (x & (stride - 1)), j = i + stride;
+                const u64 p = v[i], q = v[j];
+                if ((p < q) == ((i & size) == 0)) {
+                    v[i] = q;
+                    v[j] = p;
+                }
+            }
+        }
+    }
+    __syncthreads();
+}
 
 __device__ __forceinline__ u64 warp_sum_u(u64 v) {
 #pragma unroll
@@ -117,7 +159,86 @@ struct Row {
 struct Threshold {
     uint32_t key;  // the smallest key kept; 0: everything
     u64 above;     // the sum over larger keys
-    u64 total;     // the sum over this key's tokens
+    u64 total;     // the sum over this key's tokens, where it is known
+};
+
+// Clears the histogram.
+__device__ __forceinline__ void clear_bins(Shared& sh) {
+    for (int i = threadIdx.x; i < kBins; i += kThreads) sh.low[i] = sh.high[i] = 0u;
+    __syncthreads();
+}
+
+// The first bin at which the cluster's histogram, summed from bin 0 on top of `above`, reaches
+// `target`; sh.result = bin, the sum before it, its own sum.
+template <typename T>
+__device__ void find_bin(Row<T>& row, u64 above, u64 target) {
+    Shared& sh = row.sh;
+    auto bin = [](const Shared* s, int i) { return (static_cast<u64>(s->high[i]) << 32) + s->low[i]; };
+    __syncthreads();
+    for (int i = threadIdx.x >> 5; i < kCoarse; i += kWarps) {
+        const u64 v = warp_sum_u(bin(&sh, i * 32 + (threadIdx.x & 31)));
+        if ((threadIdx.x & 31) == 0) sh.coarse[i] = v;
+    }
+    row.cluster.sync();
+    if (threadIdx.x < 32) {
+        const int lane = threadIdx.x;
+        u64 c0 = 0, c1 = 0;
+        for (int r = 0; r < row.ranks; ++r) {
+            const u64* c = row.cluster.map_shared_rank(sh.coarse, r);
+            c0 += c[2 * lane];
+            c1 += c[2 * lane + 1];
+        }
+        u64 run = c0 + c1;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const u64 v = __shfl_up_sync(kFull, run, o);
+            if (lane >= o) run += v;
+        }
+        const unsigned hit = __ballot_sync(kFull, above + run >= target);
+        const int who = hit ? __ffs(hit) - 1 : 31;
+        u64 before = above + run - c0 - c1;
+        int coarse = 2 * lane;
+        if (before + c0 < target) {
+            before += c0;
+            ++coarse;
+        }
+        before = __shfl_sync(kFull, before, who);
+        coarse = __shfl_sync(kFull, coarse, who);
+        u64 fine = 0;
+        for (int r = 0; r < row.ranks; ++r) {
+            fine += bin(row.cluster.map_shared_rank(&sh, r), coarse * 32 + lane);
+        }
+        run = fine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const u64 v = __shfl_up_sync(kFull, run, o);
+            if (lane >= o) run += v;
+        }
+        const unsigned hit2 = __ballot_sync(kFull, before + run >= target);
+        const int who2 = hit2 ? __ffs(hit2) - 1 : 31;
+        if (lane == who2) {
+            sh.result[0] = coarse * 32 + lane;
+            sh.result[1] = before + run - fine;
+            sh.result[2] = fine;
+        }
+    }
+    row.cluster.sync();  // every CTA has read the others' bins
+}
+
+// Bins by the distance from the largest logit, over [least, top].
+struct Distance {
+    float largest, per;
+    bool usable;  // the distance tells tokens apart (not over an infinite span, nor one key)
+    __device__ Distance(uint32_t top, uint32_t least) {
+        largest = float_of(top);
+        const float span = largest - float_of(least);
+        usable = span > 0.0f && span < FLT_MAX;
+        per = usable ? static_cast<float>(kBins) / span : 0.0f;
+    }
+    __device__ int bin(float x) const {
+        return min(kBins - 1, static_cast<int>((largest - x) * per));
+    }
+    __device__ int bin(uint32_t key) const { return bin(float_of(key)); }
 };
 
 // The key at which the sum of weight(key), over the tokens with key >= least, reaches target (which
@@ -127,11 +248,8 @@ template <typename T, typename W>
 __device__ Threshold find_threshold(Row<T>& row, uint32_t top, uint32_t least, u64 target,
                                     uint32_t extra_key, u64 extra, W&& weight) {
     Shared& sh = row.sh;
-    const float largest = float_of(top);
-    const float span = largest - float_of(least);
-    // Distance bins first, unless they could not tell anything apart (an infinite span, one key).
-    bool by_distance = span > 0.0f && span < FLT_MAX;
-    const float per = by_distance ? static_cast<float>(kBins) / span : 0.0f;
+    const Distance distance(top, least);
+    bool by_distance = distance.usable;
     uint32_t lo = least, hi = top;
     u64 above = 0;
     while (true) {
@@ -139,95 +257,102 @@ __device__ Threshold find_threshold(Row<T>& row, uint32_t top, uint32_t least, u
         while (((hi - lo) >> shift) >= kBins) ++shift;
         if (shift == 0) by_distance = false;  // a bin is one key already
         auto bin_of = [&](uint32_t key) {
-            return by_distance ? min(kBins - 1, static_cast<int>((largest - float_of(key)) * per))
-                               : static_cast<int>((hi - key) >> shift);
+            return by_distance ? distance.bin(key) : static_cast<int>((hi - key) >> shift);
         };
-        for (int i = threadIdx.x; i < kBins; i += kThreads) sh.bins[i] = 0;
-        __syncthreads();
+        clear_bins(sh);
         for (int i = threadIdx.x; i < row.count; i += kThreads) {
             const uint32_t key = key_of(row.at(i));
             if (key < lo || key > hi) continue;
             const u64 w = weight(key);
-            if (w) atomicAdd(&sh.bins[bin_of(key)], w);
+            if (w) add_to(sh, bin_of(key), w);
         }
         if (extra && row.rank == 0 && threadIdx.x == 0 && extra_key >= lo && extra_key <= hi) {
-            atomicAdd(&sh.bins[bin_of(extra_key)], extra);
+            add_to(sh, bin_of(extra_key), extra);
         }
-        __syncthreads();
-        for (int i = threadIdx.x >> 5; i < kCoarse; i += kWarps) {
-            const u64 v = warp_sum_u(sh.bins[i * 32 + (threadIdx.x & 31)]);
-            if ((threadIdx.x & 31) == 0) sh.coarse[i] = v;
-        }
-        row.cluster.sync();
-        // The first coarse bin, then the first bin, where the sum from above reaches the target.
-        if (threadIdx.x < 32) {
-            const int lane = threadIdx.x;
-            u64 c0 = 0, c1 = 0;
-            for (int r = 0; r < row.ranks; ++r) {
-                const u64* c = row.cluster.map_shared_rank(sh.coarse, r);
-                c0 += c[2 * lane];
-                c1 += c[2 * lane + 1];
-            }
-            u64 run = c0 + c1;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const u64 v = __shfl_up_sync(kFull, run, o);
-                if (lane >= o) run += v;
-            }
-            const unsigned hit = __ballot_sync(kFull, above + run >= target);
-            const int who = hit ? __ffs(hit) - 1 : 31;
-            u64 before = above + run - c0 - c1;
-            int coarse = 2 * lane;
-            if (before + c0 < target) {
-                before += c0;
-                ++coarse;
-            }
-            before = __shfl_sync(kFull, before, who);
-            coarse = __shfl_sync(kFull, coarse, who);
-            u64 fine = 0;
-            for (int r = 0; r < row.ranks; ++r) {
-                fine += row.cluster.map_shared_rank(sh.bins, r)[coarse * 32 + lane];
-            }
-            run = fine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const u64 v = __shfl_up_sync(kFull, run, o);
-                if (lane >= o) run += v;
-            }
-            const unsigned hit2 = __ballot_sync(kFull, before + run >= target);
-            const int who2 = hit2 ? __ffs(hit2) - 1 : 31;
-            if (lane == who2) {
-                sh.result[0] = coarse * 32 + lane;
-                sh.result[1] = before + run - fine;
-                sh.result[2] = fine;
-            }
-        }
-        row.cluster.sync();  // every CTA has read the others' bins
+        find_bin(row, above, target);
         const int bin = static_cast<int>(sh.result[0]);
         above = sh.result[1];
         const u64 total = sh.result[2];
         if (!by_distance && shift == 0) {
             return Threshold{hi - static_cast<uint32_t>(bin), above, total};
         }
-        if (by_distance) {
-            // The keys that fell into the bin, as a range.
-            u64 high = 0, low = 0;  // low as its complement, so that both are maxima
-            for (int i = threadIdx.x; i < row.count; i += kThreads) {
-                const uint32_t key = key_of(row.at(i));
-                if (key < lo || key > hi || bin_of(key) != bin) continue;
-                high = max(high, static_cast<u64>(key));
-                low = max(low, static_cast<u64>(~key));
-            }
-            row.template reduce<true>(high, low);
-            hi = static_cast<uint32_t>(high);
-            lo = ~static_cast<uint32_t>(low);
-            by_distance = false;
-        } else {
+        if (!by_distance) {
             const uint32_t new_hi = hi - (static_cast<uint32_t>(bin) << shift);
             const uint32_t width = (1u << shift) - 1u;
             lo = new_hi - lo > width ? new_hi - width : lo;
             hi = new_hi;
+            continue;
         }
+        // The bin's tokens, collected by CTA 0 (their keys; weights follow from those).
+        __syncthreads();
+        if (threadIdx.x == 0) sh.listed = 0;
+        row.cluster.sync();
+        Shared* const home = row.cluster.map_shared_rank(&sh, 0);
+        u64 high = 0, low = 0;  // the keys' range; low as its complement, so that both are maxima
+        for (int i = threadIdx.x; i < row.count; i += kThreads) {
+            const uint32_t key = key_of(row.at(i));
+            if (key < lo || key > hi || bin_of(key) != bin) continue;
+            high = max(high, static_cast<u64>(key));
+            low = max(low, static_cast<u64>(~key));
+            const unsigned at = atomicAdd(&home->listed, 1u);
+            if (at < kList) list_of(home)[at] = key;
+        }
+        row.template reduce<true>(high, low);  // its barrier completes the list, too
+        const int n = static_cast<int>(min(home->listed, 1u + kList));
+        hi = static_cast<uint32_t>(high);
+        lo = ~static_cast<uint32_t>(low);
+        by_distance = false;
+        if (n > kList) {
+            row.cluster.sync();  // the list's place is cleared next
+            continue;
+        }
+        if (row.rank == 0) {
+            int size = 2;
+            while (size < n) size <<= 1;
+            u64* const list = list_of(&sh);
+            for (int i = n + threadIdx.x; i < size; i += kThreads) list[i] = 0;
+            sort_descending(list, size);
+            if (threadIdx.x < 32) {
+                // Lanes walk the sorted keys, 32 at a time, until the running sum reaches the target.
+                u64 run = above;
+                for (int i0 = 0; i0 < n; i0 += 32) {
+                    const int i = i0 + static_cast<int>(threadIdx.x);
+                    const uint32_t key = i < n ? static_cast<uint32_t>(list[i]) : 0u;
+                    u64 w = i < n ? weight(key) : 0;
+                    // What belongs to the extra key counts at its first token here.
+                    if (extra && i < n && key == extra_key && (i == 0 || list[i - 1] != key)) w += extra;
+                    u64 upto = w;
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const u64 v = __shfl_up_sync(kFull, upto, o);
+                        if (threadIdx.x >= o) upto += v;
+                    }
+                    const unsigned hit = __ballot_sync(kFull, i < n && run + upto >= target);
+                    if (hit) {
+                        const uint32_t edge = __shfl_sync(kFull, key, __ffs(hit) - 1);
+                        // The sum over larger keys: before the first token with this key.
+                        u64 larger = 0;
+                        for (int x = static_cast<int>(threadIdx.x); x < n; x += 32) {
+                            const uint32_t other = static_cast<uint32_t>(list[x]);
+                            if (other > edge) larger += weight(other);
+                        }
+                        larger = warp_sum_u(larger);
+                        if (extra && extra_key > edge && extra_key <= hi) larger += extra;
+                        if (threadIdx.x == 0) {
+                            sh.result[0] = edge;
+                            sh.result[1] = above + larger;
+                        }
+                        break;
+                    }
+                    run += __shfl_sync(kFull, upto, 31);
+                }
+            }
+        }
+        row.cluster.sync();
+        const uint32_t edge = static_cast<uint32_t>(home->result[0]);
+        const u64 larger = home->result[1];
+        row.cluster.sync();  // read by all before it is written again
+        return Threshold{edge, larger, 0};
     }
 }
 
@@ -248,6 +373,76 @@ __device__ uint32_t smallest_key(uint32_t lo, uint32_t hi, uint32_t guess, P&& h
         lo += static_cast<uint32_t>(f) * step;
     }
     return hi;
+}
+
+// The draw from a list of n tokens (key, ~index), of which the first top_k in order count: sorted by
+// logit for the filters, then by index for the draw. One CTA; warp 0 walks the sums.
+template <typename W, typename F, typename U>
+__device__ void finish_list(Shared& sh, int n, int top_k, float top_p, bool floored, W&& weight,
+                            F&& above_floor, U&& target_of, int* token) {
+    u64* const list = list_of(&sh);
+    int size = 2;
+    while (size < n) size <<= 1;
+    for (int i = n + threadIdx.x; i < size; i += kThreads) list[i] = 0;
+    sort_descending(list, size);
+    const int lane = threadIdx.x & 31;
+    // Running sums of w(i), i < m, 32 at a time: the first i at which they reach `target` (m: none),
+    // and with it the sum of all before the walk ended.
+    auto walk = [&](int m, u64 target, auto&& w, u64* sum) {
+        u64 run = 0;
+        for (int i0 = 0; i0 < m; i0 += 32) {
+            const int i = i0 + lane;
+            u64 upto = i < m ? w(i) : 0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const u64 v = __shfl_up_sync(kFull, upto, o);
+                if (lane >= o) upto += v;
+            }
+            const unsigned hit = __ballot_sync(kFull, i < m && run + upto >= target);
+            if (hit) return i0 + __ffs(hit) - 1;
+            run += __shfl_sync(kFull, upto, 31);
+        }
+        *sum = run;
+        return m;
+    };
+    auto by_logit = [&](int i) { return weight(static_cast<uint32_t>(list[i] >> 32)); };
+    if (threadIdx.x < 32) {
+        int m = min(n, top_k);
+        u64 sum = 0;
+        if (top_p < 1.0f) {
+            walk(m, ~0ull, by_logit, &sum);
+            const double want = static_cast<double>(top_p) * static_cast<double>(sum);
+            const u64 target = want > 0.0 ? min(sum, static_cast<u64>(ceil(want))) : 0;
+            m = target <= 1 ? 1 : walk(m, target, by_logit, &sum) + 1;
+        }
+        if (floored) {
+            int kept = 0;
+            for (int i0 = 0; i0 < m; i0 += 32) {
+                const int i = i0 + lane;
+                kept += __popc(__ballot_sync(
+                    kFull, i < m && above_floor(static_cast<uint32_t>(list[i] >> 32))));
+            }
+            m = kept;
+        }
+        if (lane == 0) sh.result[0] = m;
+    }
+    __syncthreads();
+    const int m = static_cast<int>(sh.result[0]);
+    size = 2;
+    while (size < m) size <<= 1;
+    for (int i = threadIdx.x; i < size; i += kThreads) {
+        const u64 v = list[i];
+        list[i] = i < m ? (v << 32) | (v >> 32) : 0;
+    }
+    sort_descending(list, size);
+    if (threadIdx.x < 32) {
+        auto by_index = [&](int i) { return weight(static_cast<uint32_t>(list[i])); };
+        u64 sum = 0;
+        walk(m, ~0ull, by_index, &sum);
+        // The first whose running sum exceeds the target.
+        const int i = walk(m, target_of(sum) + 1, by_index, &sum);
+        if (lane == 0) *token = static_cast<int>(~static_cast<uint32_t>(list[min(i, m - 1)] >> 32));
+    }
 }
 
 struct Args {
@@ -280,15 +475,35 @@ __global__ void __launch_bounds__(kThreads) k_sample_tokens(Args a) {
     const float min_p = a.p.min_ps ? a.p.min_ps[r] : a.p.min_p;
     const int top_k = a.p.top_ks ? a.p.top_ks[r] : a.p.top_k;
 
+    if (threadIdx.x < 32) sh.powers[threadIdx.x] = exp2(threadIdx.x / 32.0);
     // The largest logit and its first index: the maximum of (key, V - index).
-    u64 best = 0, unused = 0;
-    for (int i = threadIdx.x; i < row.count; i += kThreads) {
+    uint32_t best_key = 0u;
+    int best_at = 0;
+    auto look = [&](int i, T x) {
+        const uint32_t key = key_of(to_f(x));
+        if (key > best_key) {
+            best_key = key;
+            best_at = i;
+        }
+    };
+    constexpr int kWide = 16 / sizeof(T);
+    const int wide = reinterpret_cast<uintptr_t>(global) % 16 == 0 ? row.count / kWide : 0;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < wide; i += kThreads) {
+        const uint4 chunk = reinterpret_cast<const uint4*>(global)[i];
+        if (a.staged) reinterpret_cast<uint4*>(staged)[i] = chunk;
+        const T* x = reinterpret_cast<const T*>(&chunk);
+#pragma unroll
+        for (int j = 0; j < kWide; ++j) look(i * kWide + j, x[j]);
+    }
+    for (int i = wide * kWide + threadIdx.x; i < row.count; i += kThreads) {
         const T x = global[i];
         if (a.staged) staged[i] = x;
-        const u64 v = (static_cast<u64>(key_of(to_f(x))) << 32) |
-                      static_cast<uint32_t>(a.V - (begin + i));
-        best = max(best, v);
+        look(i, x);
     }
+    u64 unused = 0, best = row.count > 0 ? (static_cast<u64>(best_key) << 32) |
+                                               static_cast<uint32_t>(a.V - (begin + best_at))
+                                         : 0;
     row.template reduce<true>(best, unused);
     const uint32_t top = static_cast<uint32_t>(best >> 32);
     const float largest = float_of(top);
@@ -299,15 +514,7 @@ __global__ void __launch_bounds__(kThreads) k_sample_tokens(Args a) {
         return;
     }
 
-    const double T_ = temperature, top_d = largest;
-    auto real_weight = [&](uint32_t key) -> double {
-        if (key == top) return 1.0;
-        const double z = (static_cast<double>(float_of(key)) - top_d) / T_;
-        return z >= kCut ? exp(z) : 0.0;
-    };
-    auto weight = [&](uint32_t key) -> u64 {
-        return static_cast<u64>(__double2ll_rn(real_weight(key) * kUnit));
-    };
+    const double T_ = temperature, top_d = largest, per_two = 1.4426950408889634 / T_;
     // The smallest key with a weight (everything, down to the lowest finite logit, at an infinite
     // temperature; the largest alone when that is infinite).
     if (threadIdx.x < 32) {
@@ -322,6 +529,86 @@ __global__ void __launch_bounds__(kThreads) k_sample_tokens(Args a) {
     }
     __syncthreads();
     const uint32_t least = static_cast<uint32_t>(sh.result[3]);
+
+    // exp((x - largest) / temperature) of a key from `least` on, in [2^-40, 1]: 2^(k / 32 + r).
+    auto real_weight = [&](uint32_t key, int* shift) -> double {
+        const double y = key == top ? 0.0 : (static_cast<double>(float_of(key)) - top_d) * per_two;
+        const double moved = y + 211106232532992.0;  // 1.5 * 2^47: y in whole 32nds in the low bits
+        const int k = __double2loint(moved);
+        const double r = y - (moved - 211106232532992.0);
+        double p = fma(r, 0.0013333558146428441, 0.009618129107628477);
+        p = fma(r, p, 0.055504108664821576);
+        p = fma(r, p, 0.2402265069591007);
+        p = fma(r, p, 0.6931471805599453);
+        p = fma(r, p, 1.0);
+        *shift = -(k >> 5);
+        return p * sh.powers[k & 31];
+    };
+    // In units of 2^-42, to the nearest: adding 2^52 leaves them in the low bits.
+    auto weight = [&](uint32_t key) -> u64 {
+        if (key < least) return 0;
+        int shift;
+        const double w = real_weight(key, &shift);
+        const double units = fma(w, __hiloint2double((1023 + 42 - shift) << 20, 0), 4503599627370496.0);
+        return static_cast<u64>(__double_as_longlong(units)) & 0xfffffffffffffull;
+    };
+    const double floor_w = fmin(static_cast<double>(min_p), 1.0);
+    const bool floored = min_p > 0.0f;  // a NaN is no filter
+    auto above_floor = [&](uint32_t key) {
+        int shift;
+        const double w = real_weight(key, &shift);
+        return key == top || w * __hiloint2double((1023 - shift) << 20, 0) >= floor_w;
+    };
+    double u = a.uniforms[r * a.uniform_stride + (a.step ? *a.step : 0)];
+    u = u >= 0.0 ? fmin(u, 1.0) : 0.0;  // NaN too
+    auto target_of = [&](u64 whole) {
+        return min(static_cast<u64>(u * static_cast<double>(whole)), whole - 1);
+    };
+
+    // A top_k whose candidates fit a list: collected, sorted and finished by CTA 0.
+    const Distance distance(top, least);
+    if (top_k > 0 && top_k <= kList / 2 && distance.usable) {
+        clear_bins(sh);
+        const float least_f = float_of(least);
+        u64 n = 0;
+        for (int i = threadIdx.x; i < row.count; i += kThreads) {
+            const float x = row.at(i);
+            if (x >= least_f) {
+                ++n;
+                atomicAdd(&sh.low[distance.bin(x)], 1u);
+            }
+        }
+        unused = 0;
+        row.template reduce<false>(n, unused);
+        int last = kBins - 1;
+        u64 candidates = n;
+        if (n > static_cast<u64>(top_k)) {
+            find_bin(row, 0, static_cast<u64>(top_k));
+            last = static_cast<int>(sh.result[0]);
+            candidates = sh.result[1] + sh.result[2];
+            __syncthreads();
+        }
+        if (candidates <= kList) {
+            if (threadIdx.x == 0) sh.listed = 0;
+            cluster.sync();
+            Shared* const home = cluster.map_shared_rank(&sh, 0);
+            for (int i = threadIdx.x; i < row.count; i += kThreads) {
+                const float x = row.at(i);
+                if (x >= least_f && distance.bin(x) <= last) {
+                    const unsigned at = atomicAdd(&home->listed, 1u);
+                    list_of(home)[at] = (static_cast<u64>(key_of(x)) << 32) |
+                                        static_cast<uint32_t>(~(begin + i));
+                }
+            }
+            cluster.sync();  // the last access to other CTAs' memory
+            if (rank == 0) {
+                finish_list(sh, static_cast<int>(candidates), top_k, top_p, floored, weight,
+                            above_floor, target_of, a.tokens + r);
+            }
+            return;
+        }
+        cluster.sync();
+    }
 
     // Kept: keys above `edge` and the first `ties` tokens, by index, with exactly that key.
     uint32_t edge = 0;
@@ -367,16 +654,15 @@ __global__ void __launch_bounds__(kThreads) k_sample_tokens(Args a) {
             ties = need;
         }
     }
-    if (!(min_p <= 0.0f) && !isnan(min_p)) {
+    if (floored) {
         // The smallest key with a weight of at least min_p; all of its tokens are kept.
-        const double floor_w = fmin(static_cast<double>(min_p), 1.0);
         if (threadIdx.x < 32) {
             uint32_t low = top;
             if (!isinf(largest) && floor_w < 1.0) {
                 const float guess = static_cast<float>(
                     fmax(top_d + log(floor_w) * T_, -static_cast<double>(FLT_MAX)));
                 low = smallest_key(least, top, max(least, min(top, key_of(guess))),
-                                   [&](uint32_t key) { return real_weight(key) >= floor_w; });
+                                   [&](uint32_t key) { return above_floor(max(key, least)); });
             }
             if (threadIdx.x == 0) sh.result[3] = low;
         }
@@ -417,10 +703,7 @@ __global__ void __launch_bounds__(kThreads) k_sample_tokens(Args a) {
     u64 sum = lane == 0 ? my_sum : 0, tied = lane == 0 ? my_ties : 0;
     row.template reduce<false>(sum, tied);
     const u64 whole = joined(sum, tied);
-    double u = a.uniforms[r * a.uniform_stride + (a.step ? *a.step : 0)];
-    u = u >= 0.0 ? u : 0.0;  // NaN too
-    u64 target = static_cast<u64>(fmin(u, 1.0) * static_cast<double>(whole));
-    target = min(target, whole - 1);
+    const u64 target = target_of(whole);
     // The CTA that holds the target: sums before it by rank. The slots written by the reduction
     // above are the ones of the other turn.
     u64 before_sum = 0, before_ties = 0;
@@ -490,7 +773,7 @@ cudaError_t launch_typed(cudaStream_t s, Args a, int rows) {
     // portable cluster) slices grow, and past the shared memory they are read through L2.
     int cluster = 1;
     while (cluster < kMaxCluster && (a.V + cluster - 1) / cluster > (1 << 14)) cluster *= 2;
-    a.per = (a.V + cluster - 1) / cluster;
+    a.per = ((a.V + cluster - 1) / cluster + 7) / 8 * 8;  // 16-byte chunks do not straddle slices
     const size_t slice = static_cast<size_t>(a.per) * sizeof(T);
     a.staged = sizeof(Shared) + slice <= 200 * 1024;
     const size_t smem = sizeof(Shared) + (a.staged ? slice : 0);
