@@ -36,14 +36,18 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
+// Threads a CTA: half as many where a CTA has a whole row, so that more rows share an SM and cover one
+// another's steps (2048 rows of 8192: 101 -> 78 us; 64 rows of 131 072 are slower so).
+constexpr int kMaxThreads = 512;
 constexpr int kBins = 2048;
 constexpr int kCoarse = 64;                  // bins / kCoarse = 32 bins, a lane each
 constexpr int kMaxCluster = 8;
 constexpr double kUnit = 4398046511104.0;    // 2^42 units in the largest weight
 constexpr double kCut = -27.725887222397812; // ln 2^-40
 using u64 = unsigned long long;
+
+__device__ __forceinline__ int threads() { return static_cast<int>(blockDim.x); }
+__device__ __forceinline__ int warps() { return static_cast<int>(blockDim.x >> 5); }
 
 // Floats in an order of whole numbers: a < b as floats <=> key(a) < key(b); -0 and 0 are one, NaN
 // is -infinity.
@@ -64,7 +68,7 @@ struct Shared {
     double powers[32];                 // 2^(k / 32)
     unsigned listed;                   // tokens that asked for a place in the list
     u64 exchange[2][2];     // this CTA's value of a reduction over the cluster, two pairs in turn
-    u64 warp_a[kWarps], warp_b[kWarps];
+    u64 warp_a[kMaxThreads / 32], warp_b[kMaxThreads / 32];
     u64 result[4];
     u64 padding;  // the slice behind it is 16-byte aligned
 };
@@ -86,7 +90,7 @@ __device__ __forceinline__ void sort_descending(u64* v, int n) {
     for (int size = 2; size <= n; size <<= 1) {
         for (int stride = size >> 1; stride > 0; stride >>= 1) {
             __syncthreads();
-            for (int x = threadIdx.x; x < n / 2; x += kThreads) {
+            for (int x = threadIdx.x; x < n / 2; x += threads()) {
                 const int i = 2 * x - (x & (stride - 1)), j = i + stride;
                 const u64 p = v[i], q = v[j];
                 if ((p < q) == ((i & size) == 0)) {
@@ -133,7 +137,7 @@ struct Row {
         }
         __syncthreads();
         if (warp == 0) {
-            u64 x = lane < kWarps ? sh.warp_a[lane] : 0, y = lane < kWarps ? sh.warp_b[lane] : 0;
+            u64 x = lane < warps() ? sh.warp_a[lane] : 0, y = lane < warps() ? sh.warp_b[lane] : 0;
             x = MAX ? warp_max_u(x) : warp_sum_u(x);
             y = MAX ? warp_max_u(y) : warp_sum_u(y);
             if (lane == 0) {
@@ -164,7 +168,7 @@ struct Threshold {
 
 // Clears the histogram.
 __device__ __forceinline__ void clear_bins(Shared& sh) {
-    for (int i = threadIdx.x; i < kBins; i += kThreads) sh.low[i] = sh.high[i] = 0u;
+    for (int i = threadIdx.x; i < kBins; i += threads()) sh.low[i] = sh.high[i] = 0u;
     __syncthreads();
 }
 
@@ -175,7 +179,7 @@ __device__ void find_bin(Row<T>& row, u64 above, u64 target) {
     Shared& sh = row.sh;
     auto bin = [](const Shared* s, int i) { return (static_cast<u64>(s->high[i]) << 32) + s->low[i]; };
     __syncthreads();
-    for (int i = threadIdx.x >> 5; i < kCoarse; i += kWarps) {
+    for (int i = threadIdx.x >> 5; i < kCoarse; i += warps()) {
         const u64 v = warp_sum_u(bin(&sh, i * 32 + (threadIdx.x & 31)));
         if ((threadIdx.x & 31) == 0) sh.coarse[i] = v;
     }
@@ -260,7 +264,7 @@ __device__ Threshold find_threshold(Row<T>& row, uint32_t top, uint32_t least, u
             return by_distance ? distance.bin(key) : static_cast<int>((hi - key) >> shift);
         };
         clear_bins(sh);
-        for (int i = threadIdx.x; i < row.count; i += kThreads) {
+        for (int i = threadIdx.x; i < row.count; i += threads()) {
             const uint32_t key = key_of(row.at(i));
             if (key < lo || key > hi) continue;
             const u64 w = weight(key);
@@ -289,7 +293,7 @@ __device__ Threshold find_threshold(Row<T>& row, uint32_t top, uint32_t least, u
         row.cluster.sync();
         Shared* const home = row.cluster.map_shared_rank(&sh, 0);
         u64 high = 0, low = 0;  // the keys' range; low as its complement, so that both are maxima
-        for (int i = threadIdx.x; i < row.count; i += kThreads) {
+        for (int i = threadIdx.x; i < row.count; i += threads()) {
             const uint32_t key = key_of(row.at(i));
             if (key < lo || key > hi || bin_of(key) != bin) continue;
             high = max(high, static_cast<u64>(key));
@@ -310,7 +314,7 @@ __device__ Threshold find_threshold(Row<T>& row, uint32_t top, uint32_t least, u
             int size = 2;
             while (size < n) size <<= 1;
             u64* const list = list_of(&sh);
-            for (int i = n + threadIdx.x; i < size; i += kThreads) list[i] = 0;
+            for (int i = n + threadIdx.x; i < size; i += threads()) list[i] = 0;
             sort_descending(list, size);
             if (threadIdx.x < 32) {
                 // Lanes walk the sorted keys, 32 at a time, until the running sum reaches the target.
@@ -383,7 +387,7 @@ __device__ void finish_list(Shared& sh, int n, int top_k, float top_p, bool floo
     u64* const list = list_of(&sh);
     int size = 2;
     while (size < n) size <<= 1;
-    for (int i = n + threadIdx.x; i < size; i += kThreads) list[i] = 0;
+    for (int i = n + threadIdx.x; i < size; i += threads()) list[i] = 0;
     sort_descending(list, size);
     const int lane = threadIdx.x & 31;
     // Running sums of w(i), i < m, 32 at a time: the first i at which they reach `target` (m: none),
@@ -430,7 +434,7 @@ __device__ void finish_list(Shared& sh, int n, int top_k, float top_p, bool floo
     const int m = static_cast<int>(sh.result[0]);
     size = 2;
     while (size < m) size <<= 1;
-    for (int i = threadIdx.x; i < size; i += kThreads) {
+    for (int i = threadIdx.x; i < size; i += threads()) {
         const u64 v = list[i];
         list[i] = i < m ? (v << 32) | (v >> 32) : 0;
     }
@@ -458,7 +462,7 @@ struct Args {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) k_sample_tokens(Args a) {
+__global__ void __launch_bounds__(kMaxThreads) k_sample_tokens(Args a) {
     extern __shared__ __align__(16) unsigned char smem[];
     Shared& sh = *reinterpret_cast<Shared*>(smem);
     T* staged = reinterpret_cast<T*>(smem + sizeof(Shared));
@@ -476,40 +480,37 @@ __global__ void __launch_bounds__(kThreads) k_sample_tokens(Args a) {
     const int top_k = a.p.top_ks ? a.p.top_ks[r] : a.p.top_k;
 
     if (threadIdx.x < 32) sh.powers[threadIdx.x] = exp2(threadIdx.x / 32.0);
-    // The largest logit and its first index: the maximum of (key, V - index).
-    uint32_t best_key = 0u;
-    int best_at = 0;
-    auto look = [&](int i, T x) {
-        const uint32_t key = key_of(to_f(x));
-        if (key > best_key) {
-            best_key = key;
-            best_at = i;
-        }
-    };
+    // The largest logit (fmaxf passes over NaN).
+    float most = -INFINITY;
     constexpr int kWide = 16 / sizeof(T);
     const int wide = reinterpret_cast<uintptr_t>(global) % 16 == 0 ? row.count / kWide : 0;
 #pragma unroll 4
-    for (int i = threadIdx.x; i < wide; i += kThreads) {
+    for (int i = threadIdx.x; i < wide; i += threads()) {
         const uint4 chunk = reinterpret_cast<const uint4*>(global)[i];
         if (a.staged) reinterpret_cast<uint4*>(staged)[i] = chunk;
         const T* x = reinterpret_cast<const T*>(&chunk);
 #pragma unroll
-        for (int j = 0; j < kWide; ++j) look(i * kWide + j, x[j]);
+        for (int j = 0; j < kWide; ++j) most = fmaxf(most, to_f(x[j]));
     }
-    for (int i = wide * kWide + threadIdx.x; i < row.count; i += kThreads) {
+    for (int i = wide * kWide + threadIdx.x; i < row.count; i += threads()) {
         const T x = global[i];
         if (a.staged) staged[i] = x;
-        look(i, x);
+        most = fmaxf(most, to_f(x));
     }
-    u64 unused = 0, best = row.count > 0 ? (static_cast<u64>(best_key) << 32) |
-                                               static_cast<uint32_t>(a.V - (begin + best_at))
-                                         : 0;
+    u64 unused = 0, best = key_of(most);
     row.template reduce<true>(best, unused);
-    const uint32_t top = static_cast<uint32_t>(best >> 32);
+    const uint32_t top = static_cast<uint32_t>(best);
     const float largest = float_of(top);
-    const int first = a.V - static_cast<int>(best & 0xffffffffu);
     if (largest == -INFINITY || !(temperature > 0.0f)) {
-        if (rank == 0 && threadIdx.x == 0) a.tokens[r] = largest == -INFINITY ? -1 : first;
+        // Nothing to draw, or the first of the largest: the most tokens from it to the row's end.
+        u64 rest = 0;
+        for (int i = threadIdx.x; i < row.count; i += threads()) {
+            if (row.at(i) == largest) rest = max(rest, static_cast<u64>(a.V - (begin + i)));
+        }
+        row.template reduce<true>(rest, unused);
+        if (rank == 0 && threadIdx.x == 0) {
+            a.tokens[r] = largest == -INFINITY ? -1 : a.V - static_cast<int>(rest);
+        }
         cluster.sync();  // the exchange slots are read by others until here
         return;
     }
@@ -530,9 +531,9 @@ __global__ void __launch_bounds__(kThreads) k_sample_tokens(Args a) {
     __syncthreads();
     const uint32_t least = static_cast<uint32_t>(sh.result[3]);
 
-    // exp((x - largest) / temperature) of a key from `least` on, in [2^-40, 1]: 2^(k / 32 + r).
-    auto real_weight = [&](uint32_t key, int* shift) -> double {
-        const double y = key == top ? 0.0 : (static_cast<double>(float_of(key)) - top_d) * per_two;
+    // exp((x - largest) / temperature) of a logit from `least` on, in [2^-40, 1]: 2^(k / 32 + r).
+    auto real_weight = [&](float x, int* shift) -> double {
+        const double y = x == largest ? 0.0 : (static_cast<double>(x) - top_d) * per_two;
         const double moved = y + 211106232532992.0;  // 1.5 * 2^47: y in whole 32nds in the low bits
         const int k = __double2loint(moved);
         const double r = y - (moved - 211106232532992.0);
@@ -545,18 +546,18 @@ __global__ void __launch_bounds__(kThreads) k_sample_tokens(Args a) {
         return p * sh.powers[k & 31];
     };
     // In units of 2^-42, to the nearest: adding 2^52 leaves them in the low bits.
-    auto weight = [&](uint32_t key) -> u64 {
-        if (key < least) return 0;
+    auto weight_of = [&](float x) -> u64 {
         int shift;
-        const double w = real_weight(key, &shift);
+        const double w = real_weight(x, &shift);
         const double units = fma(w, __hiloint2double((1023 + 42 - shift) << 20, 0), 4503599627370496.0);
         return static_cast<u64>(__double_as_longlong(units)) & 0xfffffffffffffull;
     };
+    auto weight = [&](uint32_t key) -> u64 { return key < least ? 0 : weight_of(float_of(key)); };
     const double floor_w = fmin(static_cast<double>(min_p), 1.0);
     const bool floored = min_p > 0.0f;  // a NaN is no filter
     auto above_floor = [&](uint32_t key) {
         int shift;
-        const double w = real_weight(key, &shift);
+        const double w = real_weight(float_of(key), &shift);
         return key == top || w * __hiloint2double((1023 - shift) << 20, 0) >= floor_w;
     };
     double u = a.uniforms[r * a.uniform_stride + (a.step ? *a.step : 0)];
@@ -571,7 +572,7 @@ __global__ void __launch_bounds__(kThreads) k_sample_tokens(Args a) {
         clear_bins(sh);
         const float least_f = float_of(least);
         u64 n = 0;
-        for (int i = threadIdx.x; i < row.count; i += kThreads) {
+        for (int i = threadIdx.x; i < row.count; i += threads()) {
             const float x = row.at(i);
             if (x >= least_f) {
                 ++n;
@@ -592,7 +593,7 @@ __global__ void __launch_bounds__(kThreads) k_sample_tokens(Args a) {
             if (threadIdx.x == 0) sh.listed = 0;
             cluster.sync();
             Shared* const home = cluster.map_shared_rank(&sh, 0);
-            for (int i = threadIdx.x; i < row.count; i += kThreads) {
+            for (int i = threadIdx.x; i < row.count; i += threads()) {
                 const float x = row.at(i);
                 if (x >= least_f && distance.bin(x) <= last) {
                     const unsigned at = atomicAdd(&home->listed, 1u);
@@ -615,7 +616,7 @@ __global__ void __launch_bounds__(kThreads) k_sample_tokens(Args a) {
     u64 ties = 0;
     if (top_k > 0 && top_k < a.V) {
         u64 n = 0;
-        for (int i = threadIdx.x; i < row.count; i += kThreads) n += key_of(row.at(i)) >= least;
+        for (int i = threadIdx.x; i < row.count; i += threads()) n += key_of(row.at(i)) >= least;
         unused = 0;
         row.template reduce<false>(n, unused);
         if (n > static_cast<u64>(top_k)) {
@@ -629,7 +630,7 @@ __global__ void __launch_bounds__(kThreads) k_sample_tokens(Args a) {
         u64 sum = 0;
         unused = 0;
         const uint32_t from = max(least, edge + (edge ? 1u : 0u));
-        for (int i = threadIdx.x; i < row.count; i += kThreads) {
+        for (int i = threadIdx.x; i < row.count; i += threads()) {
             const uint32_t key = key_of(row.at(i));
             if (key >= from) sum += weight(key);
         }
@@ -681,21 +682,28 @@ __global__ void __launch_bounds__(kThreads) k_sample_tokens(Args a) {
     // The draw: sums of slices in index order, then inside the slice that the target falls into.
     const u64 tie_weight = weight(edge);
     auto joined = [&](u64 sum, u64 tied) { return sum + tie_weight * min(tied, ties); };
+    const float edge_f = float_of(edge);
+    const bool all_ties = ties == ~0ull;  // then tokens at the edge are like the others
     auto count_range = [&](int from, int to, u64* sum, u64* tied) {  // one warp, [from, to)
         u64 s = 0, n = 0;
-        for (int i = from + (threadIdx.x & 31); i < to; i += 32) {
-            const uint32_t key = key_of(row.at(i));
-            if (key > edge) {
-                s += weight(key);
-            } else if (key == edge) {
-                ++n;
+        if (all_ties) {
+#pragma unroll 4
+            for (int i = from + (threadIdx.x & 31); i < to; i += 32) {
+                const float x = row.at(i);
+                if (x >= edge_f) s += weight_of(x);
+            }
+        } else {
+            for (int i = from + (threadIdx.x & 31); i < to; i += 32) {
+                const float x = row.at(i);
+                if (x > edge_f) s += weight_of(x);
+                n += x == edge_f;
             }
         }
         *sum = warp_sum_u(s);
         *tied = warp_sum_u(n);
     };
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int part = (row.count + kWarps - 1) / kWarps;
+    const int part = (row.count + warps() - 1) / warps();
     const int w0 = min(row.count, warp * part), w1 = min(row.count, w0 + part);
     u64 my_sum, my_ties;
     count_range(w0, w1, &my_sum, &my_ties);
@@ -724,7 +732,7 @@ __global__ void __launch_bounds__(kThreads) k_sample_tokens(Args a) {
     // Twice: the sums of the warps' parts pick one, and its elements become the next parts.
     int from = 0, to = row.count;
     for (int round = 0; round < 2; ++round) {
-        const int step = (to - from + kWarps - 1) / kWarps;
+        const int step = (to - from + warps() - 1) / warps();
         const int p0 = min(to, from + warp * step), p1 = min(to, p0 + step);
         if (round > 0) count_range(p0, p1, &my_sum, &my_ties);
         __syncthreads();
@@ -734,7 +742,7 @@ __global__ void __launch_bounds__(kThreads) k_sample_tokens(Args a) {
         }
         __syncthreads();
         int pick = 0;
-        for (; pick < kWarps - 1; ++pick) {
+        for (; pick < warps() - 1; ++pick) {
             const u64 s = before_sum + sh.warp_a[pick], n = before_ties + sh.warp_b[pick];
             if (joined(s, n) > target) break;
             before_sum = s;
@@ -747,8 +755,9 @@ __global__ void __launch_bounds__(kThreads) k_sample_tokens(Args a) {
     if (warp != 0) return;
     for (int i0 = from; i0 < to; i0 += 32) {
         const int i = i0 + lane;
-        const uint32_t key = i < to ? key_of(row.at(i)) : 0u;
-        u64 s = i < to && key > edge ? weight(key) : 0, n = i < to && key == edge ? 1 : 0;
+        const float x = i < to ? row.at(i) : -INFINITY;
+        u64 s = x > edge_f || (all_ties && x == edge_f) ? weight_of(x) : 0;
+        u64 n = !all_ties && x == edge_f ? 1 : 0;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const u64 vs = __shfl_up_sync(kFull, s, o), vn = __shfl_up_sync(kFull, n, o);
@@ -782,7 +791,7 @@ cudaError_t launch_typed(cudaStream_t s, Args a, int rows) {
     if (e) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(rows) * cluster);
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(cluster == 1 ? kMaxThreads / 2 : kMaxThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
