@@ -41,7 +41,8 @@ class ModelSpecStruct(ctypes.Structure):
                 ("layers", ctypes.c_int32), ("heads", ctypes.c_int32),
                 ("hidden", ctypes.c_int32), ("weight_dtype", ctypes.c_int32),
                 ("kv_dtype", ctypes.c_int32), ("max_rows", ctypes.c_int32),
-                ("reserved", ctypes.c_int32 * 6)]
+                ("attention_window", ctypes.c_int32), ("attention_sinks", ctypes.c_int32),
+                ("reserved", ctypes.c_int32 * 4)]
 
 
 class SequencesStruct(ctypes.Structure):
@@ -100,6 +101,12 @@ SIGNATURES = {
     "bst_sample": (ctypes.c_int32, [_u64, _i32p, ctypes.c_int32, ctypes.c_int32,
                                     ctypes.c_int32, ctypes.c_float, ctypes.c_int32, _i32p,
                                     TOKEN_SINK, ctypes.c_void_p]),
+    "bst_sample_filtered": (ctypes.c_int32, [_u64, _i32p, ctypes.c_int32, ctypes.c_int32,
+                                             ctypes.c_int32, _P(SamplingStruct), _f64p, _i32p,
+                                             TOKEN_SINK, ctypes.c_void_p]),
+    "bst_sample_filtered_logits": (ctypes.c_int32, [_u64, _i32p, ctypes.c_int32, ctypes.c_int32,
+                                                    ctypes.c_int32, _P(SamplingStruct), _f64p,
+                                                    _i32p, _f32p]),
     "bst_generate_logits": (ctypes.c_int32, [_u64, _i32p, ctypes.c_int32, ctypes.c_int32,
                                              ctypes.c_int32, _i32p, _f32p]),
     "bst_sample_logits": (ctypes.c_int32, [_u64, _i32p, ctypes.c_int32, ctypes.c_int32,

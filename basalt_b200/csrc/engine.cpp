@@ -31,6 +31,7 @@
 
 #include "java_random.h"
 #include "kernels.h"
+#include "operators.h"
 
 namespace {
 
@@ -140,8 +141,15 @@ Failure validate_spec(const bst_model_spec& s) {
     if (s.weight_dtype != BST_DTYPE_F32 && s.weight_dtype != BST_DTYPE_BF16) {
         return {BST_INVALID, "weight_dtype must be BST_DTYPE_F32 or BST_DTYPE_BF16"};
     }
-    if (s.kv_dtype != BST_DTYPE_F32 && s.kv_dtype != BST_DTYPE_BF16) {
-        return {BST_INVALID, "kv_dtype must be BST_DTYPE_F32 or BST_DTYPE_BF16"};
+    if (s.kv_dtype != BST_DTYPE_F32 && s.kv_dtype != BST_DTYPE_BF16 && s.kv_dtype != BST_DTYPE_U4) {
+        return {BST_INVALID, "kv_dtype must be BST_DTYPE_F32, BST_DTYPE_BF16 or BST_DTYPE_U4"};
+    }
+    if (s.attention_window < 0 || s.attention_sinks < 0) {
+        return {BST_INVALID, "attention_window and attention_sinks must not be negative"};
+    }
+    if (!decoder_family(s.family) &&
+        (s.attention_window > 0 || s.attention_sinks > 0 || s.kv_dtype == BST_DTYPE_U4)) {
+        return {BST_INVALID, "only decoders have an attention window or a 4-bit cache"};
     }
     if (s.max_rows < 0) return {BST_INVALID, "max_rows must be non-negative"};
     if (decoder_family(s.family)) {
@@ -472,6 +480,18 @@ struct Workspace {
     bst::FusedLayer* fused_layers = nullptr;  // fused decode step: per-layer table [L]
     void *k_cache = nullptr, *v_cache = nullptr;
     size_t kv_layer_elems = 0;
+    // Engines whose attention runs through the serving operators (4-bit cache, attention window):
+    // the scales of a 4-bit cache, a step's keys and values as they leave the projection
+    // ([tokens][d]), the token list 0, 1, .. and slot zeros that put them there, the rows' lengths
+    // in the step's order, and the attention's workspace.
+    void *k_scale = nullptr, *v_scale = nullptr;
+    float *k_new = nullptr, *v_new = nullptr;
+    int *token_list = nullptr, *zero_slots = nullptr, *step_len = nullptr;
+    void* attn_space = nullptr;
+    // Filtered sampling: uniforms [rows][steps] and the step's draws.
+    double* uniforms = nullptr;
+    int* drawn = nullptr;
+    size_t uniform_capacity = 0;
     uint64_t generation = 0;
 };
 
@@ -486,7 +506,7 @@ struct PendingTiming {
     double bytes, flops;
 };
 
-enum class Mode { kGreedy, kSample, kScores };
+enum class Mode { kGreedy, kSample, kScores, kFiltered };
 
 class Engine {
    public:
@@ -500,6 +520,11 @@ class Engine {
     cudaEvent_t lane_fork = nullptr, lane_join[kLanes] = {};
     int V = 0, W = 0, d = 0, L = 0, H = 0, hd = 0, F = 0;
     bool wbf16 = false, kvbf16 = false;
+    // Attention through the serving operators: a 4-bit cache or an attention window.
+    bool op_attention = false;
+    // Mode::kFiltered: the filters, and the caller's uniforms [rows][steps].
+    bst::Sampling filters;
+    const double* filter_uniforms = nullptr;
     std::vector<std::string> names;
     std::vector<std::vector<float>> values;
     std::unordered_map<std::string, size_t> index;
@@ -655,7 +680,12 @@ class Engine {
     int upload_weights();
     // hist_rows: rows whose per-step logits this run keeps (0: none).
     int ensure_workspace(int rows, int steps, int slots, int tokens, int splits, int hist_rows,
-                         bool sampling);
+                         Mode mode);
+    // The serving operators' views of layer l's cache and of this model's attention.
+    bst::Cache layer_cache(int l) const;
+    bst::AttnSpec attention_spec() const;
+    // Stores the keys and values in ws.k_new and ws.v_new ([tokens][d]) in layer l's cache.
+    int append_step(int l, const bst::Batch& batch);
     void free_workspace();
 
     // ---- runs ----
@@ -704,7 +734,8 @@ class Engine {
     // from the projection's split-K partials), output projection, LN2, FFN, and the next LN.
     // attn_class: the profiling class of its attention launch (the prefill's last layer counts
     // as prefill attention).
-    int decode_after_qkv(int l, int R, const int* rowmap, const DecodePlan& dp,
+    // lengths: the rows' cached tokens in rowmap's order (the operators' attention reads those).
+    int decode_after_qkv(int l, int R, const int* rowmap, const int* lengths, const DecodePlan& dp,
                          const bst::QkvParts& qparts, bool* x_normalised,
                          int attn_class = bst::kAttnDecode);
     int decode_head(int R, const int* rowmap, bool x_normalised);
@@ -948,13 +979,15 @@ void Engine::free_workspace() {
 }
 
 int Engine::ensure_workspace(int rows, int steps, int slots, int tokens, int splits,
-                             int hist_rows, bool sampling) {
+                             int hist_rows, Mode mode) {
+    const bool sampling = mode == Mode::kSample;
+    const size_t uniforms = mode == Mode::kFiltered ? static_cast<size_t>(rows) * steps : 0;
     const size_t hist_floats = static_cast<size_t>(hist_rows) * steps * V;
     // The split draw pays off once the rows outnumber the SMs (one sorting CTA per row).
     const size_t sorted = sampling && rows > 148 ? static_cast<size_t>(rows) * V : 0;
     if (ws.arena.ptr && ws.rows >= rows && ws.steps >= steps && ws.slots == slots &&
         ws.tokens >= tokens && ws.splits >= splits && ws.hist_capacity >= hist_floats &&
-        ws.sorted_capacity >= sorted) {
+        ws.sorted_capacity >= sorted && ws.uniform_capacity >= uniforms) {
         return BST_OK;
     }
     free_workspace();
@@ -1003,6 +1036,10 @@ int Engine::ensure_workspace(int rows, int steps, int slots, int tokens, int spl
         add(reinterpret_cast<void**>(&ws.sorted_w), sizeof(double) * sorted);
         add(reinterpret_cast<void**>(&ws.sorted_ids), sizeof(int) * sorted);
     }
+    if (uniforms) {
+        add(reinterpret_cast<void**>(&ws.uniforms), sizeof(double) * uniforms);
+        add(reinterpret_cast<void**>(&ws.drawn), sizeof(int) * rows);
+    }
     if (hist_floats) {
         add(reinterpret_cast<void**>(&ws.history), sizeof(float) * hist_floats);
         add(reinterpret_cast<void**>(&ws.hist_rows_of), sizeof(int) * rows);
@@ -1010,7 +1047,7 @@ int Engine::ensure_workspace(int rows, int steps, int slots, int tokens, int spl
     if (decoder_family(spec.family)) {
         add(reinterpret_cast<void**>(&ws.seg_row), sizeof(int) * rows);
         add(reinterpret_cast<void**>(&ws.seg_npad), sizeof(int) * rows);
-        add(reinterpret_cast<void**>(&ws.seg_start), sizeof(int) * rows);
+        add(reinterpret_cast<void**>(&ws.seg_start), sizeof(int) * (rows + 1));
         add(reinterpret_cast<void**>(&ws.seg_len), sizeof(int) * rows);
         add(reinterpret_cast<void**>(&ws.tok_id), sizeof(int) * act_rows);
         add(reinterpret_cast<void**>(&ws.tok_pos), sizeof(int) * act_rows);
@@ -1027,9 +1064,42 @@ int Engine::ensure_workspace(int rows, int steps, int slots, int tokens, int spl
         add(reinterpret_cast<void**>(&ws.attn_tickets), sizeof(int) * static_cast<size_t>(rows) * H);
         add(reinterpret_cast<void**>(&ws.fused_layers), sizeof(bst::FusedLayer) * L);
         ws.kv_layer_elems = static_cast<size_t>(rows) * H * slots * hd;
-        const size_t kvb = (kvbf16 ? 2 : 4) * ws.kv_layer_elems * L;
+        const bool u4 = spec.kv_dtype == BST_DTYPE_U4;
+        const size_t kvb = u4 ? ws.kv_layer_elems / 2 * L : (kvbf16 ? 2 : 4) * ws.kv_layer_elems * L;
         add(&ws.k_cache, kvb);
         add(&ws.v_cache, kvb);
+        if (u4) {
+            add(&ws.k_scale, ws.kv_layer_elems / 8 * L);
+            add(&ws.v_scale, ws.kv_layer_elems / 8 * L);
+        }
+        if (op_attention) {
+            const size_t per_token = sizeof(float) * static_cast<size_t>(act_rows);
+            add(reinterpret_cast<void**>(&ws.k_new), per_token * d);
+            add(reinterpret_cast<void**>(&ws.v_new), per_token * d);
+            add(reinterpret_cast<void**>(&ws.token_list), per_token);
+            add(reinterpret_cast<void**>(&ws.zero_slots), per_token);
+            add(reinterpret_cast<void**>(&ws.step_len), sizeof(int) * rows);
+            // The most that a step of any number of rows, or a prompt's pass, asks for.
+            bst::Cache cache;
+            cache.storage = spec.kv_dtype;
+            cache.rows = rows;
+            cache.kv_heads = H;
+            cache.slots = slots;
+            cache.head_dim = hd;
+            size_t space = 16;
+            static const int kSomeStarts = 0;  // only told apart from null
+            for (int r = 1; r <= rows; ++r) {
+                bst::Batch step;
+                step.count = step.tokens = r;
+                space = std::max(space, bst::attention_cached_workspace(cache, step, attention_spec()));
+            }
+            bst::Batch prompts;
+            prompts.count = rows;
+            prompts.tokens = act_rows;
+            prompts.starts = &kSomeStarts;
+            space = std::max(space, bst::attention_packed_workspace(prompts, attention_spec()));
+            add(&ws.attn_space, space);
+        }
     } else if (spec.family == BST_FAMILY_CHAR_LM) {
         add(reinterpret_cast<void**>(&ws.flat), sizeof(float) * static_cast<size_t>(rows) * flat);
         add(reinterpret_cast<void**>(&ws.ffn), sizeof(float) * static_cast<size_t>(rows) * F);
@@ -1057,14 +1127,60 @@ int Engine::ensure_workspace(int rows, int steps, int slots, int tokens, int spl
     ws.splits = splits;
     ws.hist_capacity = hist_floats;
     ws.sorted_capacity = sorted;
+    ws.uniform_capacity = uniforms;
     ws.generation = next_generation++;
     err = bst::launch_iota(stream, ws.rowmap_all, rows);
     if (!err && ws.attn_tickets) {
         err = cudaMemsetAsync(ws.attn_tickets, 0, sizeof(int) * static_cast<size_t>(rows) * H,
                               stream);
     }
+    if (!err && ws.token_list) {
+        err = bst::launch_iota(stream, ws.token_list, act_rows);
+        if (!err) err = bst::launch_fill_int(stream, ws.zero_slots, 0, act_rows);
+    }
     if (err != cudaSuccess) return cuda_fail(err, "initialising the workspace");
     return BST_OK;
+}
+
+bst::Cache Engine::layer_cache(int l) const {
+    const size_t elems = ws.kv_layer_elems * l;
+    const size_t bytes = spec.kv_dtype == BST_DTYPE_U4 ? elems / 2 : elems * (kvbf16 ? 2 : 4);
+    bst::Cache c;
+    c.storage = spec.kv_dtype;
+    c.rows = ws.rows;
+    c.kv_heads = H;
+    c.slots = ws.slots;
+    c.head_dim = hd;
+    c.k = static_cast<char*>(ws.k_cache) + bytes;
+    c.v = static_cast<char*>(ws.v_cache) + bytes;
+    if (spec.kv_dtype == BST_DTYPE_U4) {
+        c.k_scale = static_cast<char*>(ws.k_scale) + elems / 8;
+        c.v_scale = static_cast<char*>(ws.v_scale) + elems / 8;
+    }
+    return c;
+}
+
+bst::AttnSpec Engine::attention_spec() const {
+    bst::AttnSpec a;
+    a.heads = a.kv_heads = H;
+    a.head_dim = hd;
+    a.dtype = BST_DTYPE_F32;
+    // Positions stay below the context length: a wider window hides nothing.
+    if (spec.attention_window < W && spec.attention_sinks < W) {
+        a.window = spec.attention_window;
+        a.sinks = a.window ? spec.attention_sinks : 0;
+    }
+    a.scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(hd)));
+    return a;
+}
+
+int Engine::append_step(int l, const bst::Batch& batch) {
+    const double bytes = 2.0 * batch.tokens * d * (4.0 + 4.0);
+    const cudaError_t err = launch(bst::kMisc, bytes, 0, 1, [&] {
+        return bst::launch_kv_append(stream, layer_cache(l), batch, ws.k_new, d, ws.v_new, d,
+                                     BST_DTYPE_F32);
+    });
+    return err ? cuda_fail(err, "storing keys and values") : BST_OK;
 }
 
 // Plans every step of every row (padded and stock decoders). A row extends its cache at step g
@@ -1254,7 +1370,8 @@ int Engine::enqueue_prefill(const StepPlan& p, size_t begin, size_t end) {
                           cudaMemcpyHostToDevice, stream);
     if (!err) err = cudaMemcpyAsync(ws.seg_npad, p.prefill_npad.data() + begin, sizeof(int) * segs,
                                     cudaMemcpyHostToDevice, stream);
-    if (!err) err = cudaMemcpyAsync(ws.seg_start, start.data(), sizeof(int) * segs,
+    start.push_back(total);
+    if (!err) err = cudaMemcpyAsync(ws.seg_start, start.data(), sizeof(int) * (segs + 1),
                                     cudaMemcpyHostToDevice, stream);
     if (!err) err = cudaMemcpyAsync(ws.seg_len, p.prefill_len.data() + begin, sizeof(int) * segs,
                                     cudaMemcpyHostToDevice, stream);
@@ -1300,8 +1417,27 @@ int Engine::enqueue_prefill(const StepPlan& p, size_t begin, size_t end) {
         qkv.head_dim = hd;
         qkv.slots = slots;
         qkv.kv_bf16 = kvbf16;
+        if (op_attention) {
+            // Keys and values of token t leave the projection as row t of [tokens][d].
+            qkv.rowmap = ws.token_list;
+            qkv.slot = ws.zero_slots;
+            qkv.k_cache = ws.k_new;
+            qkv.v_cache = ws.v_new;
+            qkv.slots = 1;
+            qkv.kv_bf16 = 0;
+        }
         st = linear(ws.x, d, lw.wqkv, lw.bqkv, T, 3 * d, d, Epi::kQkv, qkv, "qkv projection", &ln1);
         if (st) return st;
+        bst::Batch prompts;
+        if (op_attention) {
+            prompts.count = segs;
+            prompts.tokens = T;
+            prompts.rows = ws.seg_row;
+            prompts.starts = ws.seg_start;
+            prompts.lengths = ws.seg_len;
+            st = append_step(l, prompts);
+            if (st) return st;
+        }
         if (l == L - 1 && T > segs) {
             // Only each segment's last position feeds the head, and the cache now holds every
             // key and value of the segment: the rest of the last layer runs as a decode step
@@ -1322,8 +1458,8 @@ int Engine::enqueue_prefill(const StepPlan& p, size_t begin, size_t end) {
             st = decode_plan(segs, std::vector<int>(p.prefill_len.begin() + begin,
                                                     p.prefill_len.begin() + end), &dp);
             if (!st) {
-                st = decode_after_qkv(l, segs, ws.seg_row, dp, bst::QkvParts{}, &normalised,
-                                      bst::kAttnPrefill);
+                st = decode_after_qkv(l, segs, ws.seg_row, ws.seg_len, dp, bst::QkvParts{},
+                                      &normalised, bst::kAttnPrefill);
             }
             ws = saved;
             if (st) return st;
@@ -1339,7 +1475,26 @@ int Engine::enqueue_prefill(const StepPlan& p, size_t begin, size_t end) {
             const bst::LnArgs lnf{lnf_g, lnf_b, kLayerNormEps};
             return linear(ws.last, d, head_w, head_b, segs, V, d, Epi::kLogits, lg, "head", &lnf);
         }
-        const bst::PlaneOut att_planes = planes_for(lw.wo, T, d, d);
+        bst::PlaneOut att_planes = planes_for(lw.wo, T, d, d);
+        if (op_attention) {
+            att_planes = bst::PlaneOut{};
+            // The prompt sees the values that later steps will read.
+            if (spec.kv_dtype != BST_DTYPE_F32) {
+                err = launch(bst::kMisc, 2.0 * T * d * 8.0, 0, 1, [&] {
+                    return bst::launch_kv_read(stream, layer_cache(l), prompts, ws.k_new, d, ws.v_new,
+                                               d, BST_DTYPE_F32);
+                });
+                if (err) return cuda_fail(err, "reading keys and values");
+            }
+            bst::Batch packed = prompts;
+            packed.rows = nullptr;
+            packed.lengths = nullptr;
+            st = check(launch(bst::kAttnPrefill, attn_bytes, attn_flops, 2, [&] {
+                           return bst::launch_attention_packed(stream, packed, attention_spec(), ws.q, d,
+                                                               ws.k_new, d, ws.v_new, d, ws.att, d,
+                                                               ws.attn_space);
+                       }), "prefill attention");
+        } else
         st = check(launch(bst::kAttnPrefill, attn_bytes, attn_flops, 1, [&] {
                        return bst::launch_attn_prefill(stream, ws.q, qkv.k_cache, qkv.v_cache,
                                                        kvbf16, ws.seg_row, ws.seg_start,
@@ -1405,7 +1560,7 @@ int Engine::enqueue_decode(int R, const int* rowmap, const std::vector<int>& len
     // than 8 rows (the tensor-core path).
     int nl = 2;
     if (const char* env = std::getenv("BST_DECODE_LANES")) nl = std::atoi(env);
-    nl = std::max(1, std::min(nl, kLanes));
+    nl = op_attention ? 1 : std::max(1, std::min(nl, kLanes));
     while (nl > 1 && (R / nl <= 8 || !ws.lane_part[nl - 1] ||
                       !linear_on_tc(layers[0].wqkv, R / nl, 3 * d, d))) {
         nl /= 2;
@@ -1421,6 +1576,12 @@ int Engine::enqueue_decode(int R, const int* rowmap, const std::vector<int>& len
         // operand planes; the GEMV path normalises inside its own projection.
         const bool normalise = linear_on_tc(layers[0].wqkv, R, 3 * d, d) && d <= 1024;
         st = embed_rows(R, rowmap, normalise);
+        if (!st && op_attention) {
+            const cudaError_t e = launch(bst::kGather, R * 12.0, 0, 1, [&] {
+                return bst::launch_gather_int(stream, ws.len, rowmap, R, ws.step_len);
+            });
+            if (e) return cuda_fail(e, "row lengths");
+        }
         return st ? st : decode_layers(R, rowmap, lens, normalise);
     }
     // Lane i takes rows [i R / nl, (i + 1) R / nl) with every per-row workspace view shifted to
@@ -1568,7 +1729,14 @@ int Engine::decode_layer(int l, int R, const int* rowmap, const DecodePlan& dp,
     // A split-K QKV projection leaves its partial sums to the attention kernel, which sums
     // q per head and appends the step's key and value to the cache itself.
     bst::QkvParts qparts;
-    if (linear_on_tc(lw.wqkv, R, 3 * d, d)) {
+    if (op_attention) {
+        qkv.rowmap = ws.token_list;
+        qkv.slot = ws.zero_slots;
+        qkv.k_cache = ws.k_new;
+        qkv.v_cache = ws.v_new;
+        qkv.slots = 1;
+        qkv.kv_bf16 = 0;
+    } else if (linear_on_tc(lw.wqkv, R, 3 * d, d)) {
         const int qkv_splits = bst::tc_plan(R, 3 * d, d, wbf16, bst::tc_part_bytes_max(), nullptr);
         if (qkv_splits > 1) qparts = bst::QkvParts{ws.tc_part, qkv_splits, lw.bqkv};
     }
@@ -1581,11 +1749,20 @@ int Engine::decode_layer(int l, int R, const int* rowmap, const DecodePlan& dp,
                                     "qkv projection", &ln1);
     }
     if (st) return st;
-    return decode_after_qkv(l, R, rowmap, dp, qparts, x_normalised);
+    if (op_attention) {
+        bst::Batch step;
+        step.count = step.tokens = R;
+        step.rows = rowmap;
+        step.lengths = ws.step_len;
+        st = append_step(l, step);
+        if (st) return st;
+    }
+    return decode_after_qkv(l, R, rowmap, ws.step_len, dp, qparts, x_normalised);
 }
 
-int Engine::decode_after_qkv(int l, int R, const int* rowmap, const DecodePlan& dp,
-                             const bst::QkvParts& qparts, bool* x_normalised, int attn_class) {
+int Engine::decode_after_qkv(int l, int R, const int* rowmap, const int* lengths,
+                             const DecodePlan& dp, const bst::QkvParts& qparts, bool* x_normalised,
+                             int attn_class) {
     const double kvb = kvbf16 ? 2.0 : 4.0;
     const int slots = ws.slots;
     const float scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(hd)));
@@ -1598,7 +1775,19 @@ int Engine::decode_after_qkv(int l, int R, const int* rowmap, const DecodePlan& 
         static_cast<char*>(ws.v_cache) + l * ws.kv_layer_elems * static_cast<size_t>(kvb);
     const double kv_bytes = dp.sum_len * 2.0 * d * kvb + R * d * 4.0 +
                             (qparts.part ? qparts.splits * R * 3.0 * d * 4.0 : 0.0);
-    const bst::PlaneOut att_planes = planes_for(lw.wo, R, d, d);
+    bst::PlaneOut att_planes = planes_for(lw.wo, R, d, d);
+    if (op_attention) {
+        att_planes = bst::PlaneOut{};
+        bst::Batch step;
+        step.count = step.tokens = R;
+        step.rows = rowmap;
+        step.lengths = lengths;
+        st = check(launch(attn_class, kv_bytes, 4.0 * dp.sum_len * d, 1, [&] {
+                       return bst::launch_attention_cached(stream, layer_cache(l), step,
+                                                           attention_spec(), ws.q, d, ws.att, d,
+                                                           ws.attn_space);
+                   }), "decode attention");
+    } else
     st = check(launch(attn_class, kv_bytes, 4.0 * dp.sum_len * d, 1, [&] {
                    return bst::launch_attn_decode(stream, ws.q, k_cache, v_cache,
                                                   kvbf16, rowmap, ws.len, R, H, hd, slots,
@@ -1693,6 +1882,7 @@ int Engine::enqueue_direct(int rows) {
 int Engine::prepare_fused(int rows) {
     const char* env = std::getenv("BST_FUSED_DECODE");
     if (env && std::strcmp(env, "0") == 0) return 0;
+    if (op_attention) return 0;
     if (!decoder_family(spec.family) || !bst::fused_decode_supported(rows, d, F, W, hd, wbf16)) {
         return 0;
     }
@@ -1804,6 +1994,15 @@ int Engine::enqueue_select(Mode mode, int rows, int steps, float temperature, in
         return BST_OK;
     }
     push_in_head = false;
+    if (mode == Mode::kFiltered) {
+        err = launch(bst::kSelectSample, rows * V * 4.0, 0, 2, [&] {
+            cudaError_t e = bst::launch_sample_tokens(stream, ws.logits, BST_DTYPE_F32, rows, V, V,
+                                                      filters, ws.uniforms, steps, ws.step, ws.drawn);
+            return e ? e : bst::launch_push_tokens(stream, ws.drawn, rows, W, steps, ws.step, ws.done,
+                                                   ws.tokens_out, ws.next, ws.window);
+        });
+        return err ? cuda_fail(err, "token selection") : BST_OK;
+    }
     if (mode == Mode::kGreedy) {
         err = launch(bst::kSelectGreedy, rows * V * 4.0, 0, 1, [&] {
             return bst::launch_select_greedy(stream, ws.logits, rows, V, W, steps, ws.step, ws.done,
@@ -1863,8 +2062,7 @@ int Engine::run_wave(Mode mode, const std::vector<int32_t>& all_windows, int row
     const bool transformer = decoder_family(spec.family);
     if (transformer) plan(windows, rows, run_steps, &plans, &max_slots, &max_tokens);
     const int splits_cap = std::max(1, (max_slots + 31) / 32);
-    int st = ensure_workspace(rows, run_steps, max_slots, max_tokens, splits_cap, hist_rows,
-                              mode == Mode::kSample);
+    int st = ensure_workspace(rows, run_steps, max_slots, max_tokens, splits_cap, hist_rows, mode);
     if (st) return st;
     hist_count = hist_rows;
     push_steps = run_steps;
@@ -1905,6 +2103,11 @@ int Engine::run_wave(Mode mode, const std::vector<int32_t>& all_windows, int row
                               cudaMemcpyHostToDevice, stream);
         if (!err) err = cudaStreamSynchronize(stream);
     }
+    if (!err && mode == Mode::kFiltered) {
+        err = cudaMemcpyAsync(ws.uniforms, filter_uniforms + static_cast<size_t>(row0) * steps,
+                              sizeof(double) * static_cast<size_t>(rows) * steps,
+                              cudaMemcpyHostToDevice, stream);
+    }
     if (!err) err = cudaStreamSynchronize(stream);
     if (err) return cuda_fail(err, "uploading contexts");
 
@@ -1937,11 +2140,13 @@ int Engine::run_wave(Mode mode, const std::vector<int32_t>& all_windows, int row
         } else if (graphable) {
             // One CUDA graph per (shape, mode): the step body plus selection reads every
             // step-dependent value (lengths, step counter, RNG state) from device memory.
-            char key[160];
-            std::snprintf(key, sizeof(key), "%d/%d/%d/%d/%08x/%d/%d/%llu", static_cast<int>(mode),
-                          rows, run_steps, ws.slots,
-                          [&] { uint32_t b; std::memcpy(&b, &temperature, 4); return b; }(),
-                          top_k, hist_rows, static_cast<unsigned long long>(ws.generation));
+            char key[192];
+            auto bits = [](float f) { uint32_t b; std::memcpy(&b, &f, 4); return b; };
+            std::snprintf(key, sizeof(key), "%d/%d/%d/%d/%08x/%d/%d/%llu/%08x/%08x",
+                          static_cast<int>(mode), rows, run_steps, ws.slots, bits(temperature),
+                          top_k, hist_rows, static_cast<unsigned long long>(ws.generation),
+                          bits(mode == Mode::kFiltered ? filters.top_p : 0.0f),
+                          bits(mode == Mode::kFiltered ? filters.min_p : 0.0f));
             if (!graph || graph_key != key) {
                 if (graph) {
                     cudaGraphExecDestroy(graph);
@@ -2076,6 +2281,9 @@ int Engine::run(Mode mode, const int32_t* contexts, int32_t rows, int32_t length
             return fail(BST_UNSUPPORTED, "sampling supports vocabularies up to 16384");
         }
     }
+    if (mode == Mode::kFiltered && !filter_uniforms) {
+        return fail(BST_INVALID, "uniforms must not be null");
+    }
     if (!contexts) return fail(BST_INVALID, "contexts must not be null");
     if (rows < 1) return fail(BST_INVALID, "contexts must not be empty");
     if (length < W) {
@@ -2208,6 +2416,7 @@ int32_t bst_engine_create(const bst_model_spec* spec, int32_t device, bst_engine
         e->F = spec->hidden;
         e->wbf16 = spec->weight_dtype == BST_DTYPE_BF16;
         e->kvbf16 = spec->kv_dtype == BST_DTYPE_BF16;
+        e->op_attention = spec->kv_dtype == BST_DTYPE_U4 || spec->attention_window > 0;
         std::vector<int64_t> sizes;
         declare_parameters(*spec, &e->names, &sizes);
         for (size_t i = 0; i < e->names.size(); ++i) {
@@ -2448,6 +2657,54 @@ int32_t bst_sample(bst_engine h, const int32_t* contexts, int32_t rows, int32_t 
         return set_error(e, e->run(Mode::kSample, contexts, rows, length, steps, temperature,
                                    top_k, tokens, false, sink, user, nullptr));
     })
+}
+
+static int32_t filtered_call(bst_engine h, const int32_t* contexts, int32_t rows, int32_t length,
+                             int32_t steps, const bst_sampling* sampling, const double* uniforms,
+                             int32_t* tokens, bst_token_sink sink, void* user, float* logits) {
+    auto e = find_engine(h);
+    if (!e) return unknown(h);
+    BST_GUARDED({
+        std::lock_guard<std::mutex> lock(e->mu);
+        if (!sampling) return set_error(e, e->fail(BST_INVALID, "sampling must not be null"));
+        if (sampling->temperatures || sampling->top_ks || sampling->top_ps || sampling->min_ps) {
+            return set_error(e, e->fail(BST_INVALID, "an engine's rows share their sampling settings"));
+        }
+        // The caller's uniforms are borrowed for this call only, however it ends.
+        struct UniformScope {
+            const double*& u;
+            ~UniformScope() { u = nullptr; }
+        } scope{e->filter_uniforms};
+        e->filter_uniforms = uniforms;
+        e->filters = bst::Sampling{};
+        e->filters.temperature = sampling->temperature;
+        e->filters.top_k = sampling->top_k;
+        e->filters.top_p = sampling->top_p;
+        e->filters.min_p = sampling->min_p;
+        return set_error(e, e->run(Mode::kFiltered, contexts, rows, length, steps,
+                                   sampling->temperature, sampling->top_k, tokens, false, sink,
+                                   user, nullptr, logits));
+    })
+}
+
+int32_t bst_sample_filtered(bst_engine h, const int32_t* contexts, int32_t rows, int32_t length,
+                            int32_t steps, const bst_sampling* sampling, const double* uniforms,
+                            int32_t* tokens, bst_token_sink sink, void* user) {
+    return filtered_call(h, contexts, rows, length, steps, sampling, uniforms, tokens, sink, user,
+                         nullptr);
+}
+
+int32_t bst_sample_filtered_logits(bst_engine h, const int32_t* contexts, int32_t rows,
+                                   int32_t length, int32_t steps, const bst_sampling* sampling,
+                                   const double* uniforms, int32_t* tokens, float* logits) {
+    auto e = find_engine(h);
+    if (!e) return unknown(h);
+    if (!logits) {
+        t_last_error = "logits must not be null";
+        return BST_INVALID;
+    }
+    return filtered_call(h, contexts, rows, length, steps, sampling, uniforms, tokens, nullptr,
+                         nullptr, logits);
 }
 
 int32_t bst_generate_logits(bst_engine h, const int32_t* contexts, int32_t rows, int32_t length,

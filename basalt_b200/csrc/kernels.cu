@@ -1059,6 +1059,28 @@ __global__ __launch_bounds__(256) void k_select_greedy(const float* __restrict__
     finish_row(r, token, s_step, rows, W, steps, step, done, tokens, next, window);
 }
 
+// Tokens drawn by another kernel: the bookkeeping of a step alone.
+__global__ __launch_bounds__(256) void k_push_tokens(const int* __restrict__ drawn, int W, int steps,
+                                                     int rows, int* step, int* done, int* tokens,
+                                                     int* next, int* window) {
+    pdl_trigger();
+    pdl_wait();
+    const int r = blockIdx.x;
+    __shared__ int s_step;
+    if (threadIdx.x == 0) s_step = *reinterpret_cast<volatile int*>(step);
+    __syncthreads();
+    finish_row(r, max(drawn[r], 0), s_step, rows, W, steps, step, done, tokens, next, window);
+}
+
+__global__ __launch_bounds__(256) void k_gather_int(const int* __restrict__ values,
+                                                    const int* __restrict__ at, int count,
+                                                    int* __restrict__ out) {
+    pdl_trigger();
+    pdl_wait();
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i < count) out[i] = values[at[i]];
+}
+
 // Greedy selection when the head's epilogue already folded each row's first maximum into best[r]
 // (pack_best): the logits are not read again, except the row's score at index 0, which wins when
 // it is NaN (TextEngine.argmax only moves on to a larger score). best[r] is cleared for the next
@@ -1792,6 +1814,19 @@ cudaError_t launch_select_greedy(cudaStream_t s, const float* logits, int rows, 
     }
     return launch_pdl(k_select_greedy, rows, 256, 0, s, logits, V, W, steps, rows, step, done, tokens, next,
                                          window);
+}
+
+cudaError_t launch_push_tokens(cudaStream_t s, const int* drawn, int rows, int W, int steps, int* step,
+                               int* done, int* tokens, int* next, int* window) {
+    if (rows <= 0) return cudaSuccess;
+    if (W > 8 * 256) return cudaErrorInvalidValue;
+    return launch_pdl(k_push_tokens, rows, 256, 0, s, drawn, W, steps, rows, step, done, tokens, next,
+                      window);
+}
+
+cudaError_t launch_gather_int(cudaStream_t s, const int* values, const int* at, int count, int* out) {
+    if (count <= 0) return cudaSuccess;
+    return launch_pdl(k_gather_int, (count + 255) / 256, 256, 0, s, values, at, count, out);
 }
 
 size_t sample_draw_smem(int top_k) {

@@ -179,6 +179,9 @@ cudaError_t launch_select_sample(cudaStream_t s, const float* logits, int rows, 
                                  int steps, float temperature, int top_k, uint64_t* rng,
                                  int* step, int* done, int* tokens, int* next, int* window,
                                  double* sorted_w = nullptr, int* sorted_ids = nullptr);
+// Takes tokens chosen elsewhere (drawn[r]; a negative one counts as 0) through the same bookkeeping.
+cudaError_t launch_push_tokens(cudaStream_t s, const int* drawn, int rows, int W, int steps, int* step,
+                               int* done, int* tokens, int* next, int* window);
 size_t select_sample_smem(int V);
 size_t sample_draw_smem(int top_k);
 
@@ -279,5 +282,7 @@ cudaError_t launch_decode_fused(cudaStream_t s, const FusedStep& p, const FusedL
 
 cudaError_t launch_fill_int(cudaStream_t s, int* p, int value, int count);
 cudaError_t launch_iota(cudaStream_t s, int* p, int count);
+// out[i] = values[at[i]].
+cudaError_t launch_gather_int(cudaStream_t s, const int* values, const int* at, int count, int* out);
 
 }  // namespace bst

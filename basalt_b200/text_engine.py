@@ -73,7 +73,7 @@ FAMILIES = {
     "char_lm": _lib.FAMILY_CHAR_LM,
     "last_token": _lib.FAMILY_LAST_TOKEN,
 }
-DTYPES = {"f32": _lib.DTYPE_F32, "bf16": _lib.DTYPE_BF16}
+DTYPES = {"f32": _lib.DTYPE_F32, "bf16": _lib.DTYPE_BF16, "u4": _lib.DTYPE_U4}
 
 
 @dataclass(frozen=True)
@@ -90,6 +90,10 @@ class ModelSpec:
     * ``char_lm`` — Zoo.charLm (zoo/Zoo.java:80-168): ``dimension`` is the embedding width and
       ``hidden`` the bottleneck.
     * ``last_token`` — TextEngineTest.LastTokenModel, the reference's decode-loop fixture.
+
+    Decoders may keep their attention cache in 4 bits (``kv_dtype="u4"``: 5 bits a value with its
+    scale, see ``basalt_b200.operators``; a prompt attends to the values that are kept) and may look
+    at the last ``attention_window`` tokens only (0: all) and the first ``attention_sinks``.
     """
 
     family: str
@@ -102,6 +106,8 @@ class ModelSpec:
     weight_dtype: str = "f32"
     kv_dtype: str = "f32"
     max_rows: int = 0
+    attention_window: int = 0
+    attention_sinks: int = 0
 
     def struct(self) -> _lib.ModelSpecStruct:
         if self.family not in FAMILIES:
@@ -117,6 +123,8 @@ class ModelSpec:
         s.weight_dtype = DTYPES[self.weight_dtype]
         s.kv_dtype = DTYPES[self.kv_dtype]
         s.max_rows = self.max_rows
+        s.attention_window = self.attention_window
+        s.attention_sinks = self.attention_sinks
         return s
 
 
@@ -300,6 +308,45 @@ class TextEngine:
         """Rows sampled together; the tokens equal ``len(contexts)`` successive ``sample`` calls
         on this engine, and the generator ends where those calls would leave it."""
         return self._sample(contexts, steps, temperature, topK, sink)
+
+    def sampleFiltered(self, contexts, steps: int, uniforms, temperature: float = 1.0,
+                       topK: int = 0, topP: float = 1.0, minP: float = 0.0,
+                       sink: Optional[Callable[[int, int, int], None]] = None) -> np.ndarray:
+        """Tokens [rows, steps] drawn after temperature, topK (0: all), topP and minP with the given
+        ``uniforms`` ([rows, steps] in [0, 1)); the filters are those of
+        ``basalt_b200.operators.sample_tokens``. The engine's own generator is not used."""
+        arr, u, p = self._filtered(contexts, steps, uniforms, temperature, topK, topP, minP)
+        out = np.zeros((arr.shape[0], steps), dtype=np.int32)
+        cb, errors = self._sink(sink)
+        code = self._lib.bst_sample_filtered(self._h, arr.ctypes.data_as(_lib._i32p), arr.shape[0],
+                                             arr.shape[1], steps, p, u.ctypes.data_as(_lib._f64p),
+                                             out.ctypes.data_as(_lib._i32p), cb, None)
+        if errors:
+            raise errors[0]
+        self._call(code)
+        return out
+
+    def sampleFilteredWithLogits(self, contexts, steps: int, uniforms, temperature: float = 1.0,
+                                 topK: int = 0, topP: float = 1.0, minP: float = 0.0):
+        """sampleFiltered, and the logits [rows, steps, V] each token was drawn from."""
+        arr, u, p = self._filtered(contexts, steps, uniforms, temperature, topK, topP, minP)
+        tokens = np.zeros((arr.shape[0], steps), dtype=np.int32)
+        logits = np.zeros((arr.shape[0], steps, self.vocabulary()), dtype=np.float32)
+        self._call(self._lib.bst_sample_filtered_logits(
+            self._h, arr.ctypes.data_as(_lib._i32p), arr.shape[0], arr.shape[1], steps, p,
+            u.ctypes.data_as(_lib._f64p), tokens.ctypes.data_as(_lib._i32p),
+            logits.ctypes.data_as(_lib._f32p)))
+        return tokens, logits
+
+    def _filtered(self, contexts, steps, uniforms, temperature, topK, topP, minP):
+        arr = self._prepare(contexts, steps)
+        u = np.ascontiguousarray(uniforms, dtype=np.float64)
+        if u.shape != (arr.shape[0], steps):
+            raise IllegalArgumentException(f"uniforms must be [{arr.shape[0]}, {steps}], got "
+                                           f"{list(u.shape)}", _lib.BST_INVALID)
+        if not np.all((u >= 0) & (u < 1)):
+            raise IllegalArgumentException("uniforms must lie in [0, 1)", _lib.BST_INVALID)
+        return arr, u, _lib.SamplingStruct(temperature, topP, minP, topK)
 
     def seed(self, seed: int):
         self._call(self._lib.bst_seed(self._h, int(seed)))

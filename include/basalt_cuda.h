@@ -65,7 +65,11 @@ typedef struct bst_model_spec {
     int32_t weight_dtype; /* BST_DTYPE_*: storage of matrices and embedding tables */
     int32_t kv_dtype;     /* BST_DTYPE_*: storage of the attention cache */
     int32_t max_rows;     /* rows decoded together per wave; 0 = sized from free memory */
-    int32_t reserved[6];  /* must be zero */
+    /* Decoders: a token attends to the last attention_window tokens (0: all of the context) and,
+     * with a window, to the first attention_sinks. No counterpart in the reference. */
+    int32_t attention_window;
+    int32_t attention_sinks;
+    int32_t reserved[4];  /* must be zero */
 } bst_model_spec;
 
 /* Per-token callback (java.util.function.IntConsumer of TextEngine.stream / streamSampled,
@@ -133,6 +137,21 @@ int32_t bst_generate(bst_engine engine, const int32_t* contexts, int32_t rows, i
 int32_t bst_sample(bst_engine engine, const int32_t* contexts, int32_t rows, int32_t length,
                    int32_t steps, float temperature, int32_t top_k, int32_t* tokens,
                    bst_token_sink sink, void* user);
+
+/* Sampling with bst_sampling's filters (below; its per-row arrays must be NULL) from the caller's
+ * random numbers: step g of row r draws with uniforms[r * steps + g] (host memory, [rows, steps]).
+ * A row whose logits leave nothing to draw (NaN only) takes token 0. The engine's java.util.Random is
+ * not touched. No counterpart in the reference. */
+struct bst_sampling;
+int32_t bst_sample_filtered(bst_engine engine, const int32_t* contexts, int32_t rows, int32_t length,
+                            int32_t steps, const struct bst_sampling* sampling,
+                            const double* uniforms, int32_t* tokens, bst_token_sink sink,
+                            void* user);
+/* The same, also returning the logits each step was decided on ([rows, steps, vocabulary]). */
+int32_t bst_sample_filtered_logits(bst_engine engine, const int32_t* contexts, int32_t rows,
+                                   int32_t length, int32_t steps,
+                                   const struct bst_sampling* sampling, const double* uniforms,
+                                   int32_t* tokens, float* logits);
 
 /* bst_generate / bst_sample that also return the logits each step was decided on:
  * logits [rows, steps, vocabulary] float32 (the scores TextEngine.scores would have returned for

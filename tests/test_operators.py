@@ -149,3 +149,21 @@ def test_reference_draw_known_answers():
     assert ref.draw_token(x, 0.99, 1.0, 0, 1.0, 0.0)[0] == 2
     assert ref.draw_token(x, 0.99, 1.0, 1, 1.0, 0.0)[0] == 1       # ties: lowest index
     assert ref.draw_token([-np.inf] * 3, 0.5, 1.0, 0, 1.0, 0.0)[0] == -1
+
+
+def test_specs_with_a_window_or_a_4_bit_cache():
+    from basalt_b200 import ModelSpec
+
+    def create(spec):
+        s, h = spec.struct(), ctypes.c_uint64(0)
+        return _lib.load().bst_engine_create(s, 10 ** 6, ctypes.byref(h))
+
+    decoder = ("padded_decoder", 10, 8, 64, 1, 2, 32)
+    assert create(ModelSpec(*decoder, attention_window=-1)) == _lib.BST_INVALID
+    assert create(ModelSpec(*decoder, attention_sinks=-1)) == _lib.BST_INVALID
+    assert create(ModelSpec(*decoder, weight_dtype="u4")) == _lib.BST_INVALID
+    assert create(ModelSpec("last_token", 5, 3, attention_window=2)) == _lib.BST_INVALID
+    assert create(ModelSpec("last_token", 5, 3, kv_dtype="u4")) == _lib.BST_INVALID
+    # accepted specs get as far as the device, which does not exist
+    assert create(ModelSpec(*decoder, kv_dtype="u4", attention_window=3,
+                            attention_sinks=1)) == _lib.BST_UNSUPPORTED
