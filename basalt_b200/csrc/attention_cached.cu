@@ -8,19 +8,23 @@
 //   s_ij    = sum_g step_jg (q_ig . c_jg) + low_jg sum(q_ig)         g: groups of 32 channels
 //   out_icg = sum_j (p_ij step_jg) c_jgc + sum_j p_ij low_jg
 //
-// A nibble becomes a bf16 number without a conversion. Keys: the bits themselves, c or 16 c in the
-// lowest mantissa bits, are c 2^-133 or 16 c 2^-133 (bf16's subnormals and its first binade have the
-// same spacing); the queries carry the 2^127 and 2^123 that bring them back, normalised by a power
-// of two per row so that nothing overflows. Values: 0x4300 | c is 128 + c; bf16 queries keep the 128
-// and take it out through low - 128 step, float32 ones subtract it (it would cost them four bits).
+// A nibble becomes an fp16 number without a conversion: its bits in the lowest mantissa bits, c or
+// 16 c, are the subnormals c 2^-24 and 16 c 2^-24. The other operand carries the 2^15 or 2^11 that
+// bring them near one: queries, normalised by a power of two per row so that nothing overflows, and
+// weights p step, normalised by the power of two above the largest step of the group so far (which
+// moves as the maximum of the scores does, by rescaling). fp16 has 11 bits where bf16 has 8: one
+// term is more than bf16 outputs show, and two carry 22 bits for float32. float32 also takes
+// 1024 + c, or 1024 + 16 c, to c - 8 with one fp16 operation: sums of low and of step c would
+// otherwise cancel one another (over 42 000 keys that left 7e-5 of the output where this leaves @@),
+// and the tensor cores add subnormals with fewer bits.
 // mma.sync m16n8k16 reads its B operand from registers, which is where unpacked codes are;
 // tcgen05 would need them written to shared memory at four times their size first, and a tile
 // of at most eight query rows would leave 120 of its 128 rows empty.
 //
-// The sixteen rows of the A operand hold eight queries (tokens x heads of one key head) twice: rows
-// 0-7 the leading bf16 part of the weights p step (and of float32 q), rows 8-15 what that rounding
-// left, so one product carries 16 bits; float32 adds a second product for the next eight. Weights,
-// sums and the running maximum are float32.
+// The sixteen rows of the A operand hold sixteen queries (tokens x heads of one key head), or eight:
+// then rows 8-15 hold what rounding the weights (and float32 q) of rows 0-7 left, so that one product
+// carries both terms. The lows, and caches that are not in 4 bits, are multiplied in bf16 the same way,
+// float32 ones in three terms. Weights, sums and the running maximum are float32.
 //
 // A warp works on 16 keys at a time and alone: it copies its keys into its own ring in shared memory
 // with cp.async (keys that nobody sees are filled with zeros there, whatever their slots hold), and
@@ -29,6 +33,7 @@
 // and output in the workspace and a second kernel joins them.
 
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 
 #include <algorithm>
 #include <cfloat>
@@ -99,11 +104,25 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                        uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
 // The same from zero.
 __device__ __forceinline__ void mma_bf16_start(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                                uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+__device__ __forceinline__ void mma_f16_start(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                              uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
         "{%8, %9}, {%10, %10, %10, %10};"
         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
@@ -124,15 +143,41 @@ __device__ __forceinline__ void terms_of(float a, float b, uint32_t* out) {
     }
 }
 
-// Nibble i of both halves of x as bf16 numbers: c or, with OFFSET, 128 + c. The shifts are high
-// halves of products, which run beside the logic operations instead of among them.
-template <bool OFFSET>
-__device__ __forceinline__ uint32_t nibbles(uint32_t x, int i) {
-    const uint32_t v = ((i ? __umulhi(x, 1u << (32 - 4 * i)) : x) & 0x000f000fu) | 0x43004300u;
-    if constexpr (OFFSET) return v;
+// The same as fp16 pairs, 11 bits a term.
+template <int TERMS>
+__device__ __forceinline__ void half_terms_of(float a, float b, uint32_t* out) {
+#pragma unroll
+    for (int i = 0; i < TERMS; ++i) {
+        const __half2 h = __floats2half2_rn(a, b);
+        out[i] = *reinterpret_cast<const uint32_t*>(&h);
+        if (i + 1 < TERMS) {
+            a -= __low2float(h);
+            b -= __high2float(h);
+        }
+    }
+}
+
+// Nibbles 0 and 1 of both halves of x as fp16 pairs c - 8.
+__device__ __forceinline__ uint32_t centred0(uint32_t x) {
     uint32_t r;
-    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(0x43004300u));
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"((x & 0x000f000fu) | 0x64006400u), "r"(0x64086408u));
     return r;
+}
+__device__ __forceinline__ uint32_t centred1(uint32_t x) {  // (1024 + 16 c) / 16 - 72
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;"
+        : "=r"(r)
+        : "r"((x & 0x00f000f0u) | 0x64006400u), "r"(0x2c002c00u), "r"(0xd480d480u));
+    return r;
+}
+// The same as c 2^-24 and 16 c 2^-24, or centred.
+template <bool CENTRED>
+__device__ __forceinline__ uint32_t nibble0(uint32_t x) {
+    return CENTRED ? centred0(x) : x & 0x000f000fu;
+}
+template <bool CENTRED>
+__device__ __forceinline__ uint32_t nibble1(uint32_t x) {
+    return CENTRED ? centred1(x) : x & 0x00f000f0u;
 }
 
 template <int G>
@@ -190,12 +235,18 @@ constexpr int min_ctas() {
 
 // The A fragment's terms times (b0, b1). With one query row a lane, the tile's rows 8-15 carry the
 // second term of rows 0-7; with two they are queries of their own and every term is a product.
-template <bool START, int R, int N>
+template <bool HALF, bool START, int R, int N>
 __device__ __forceinline__ void product(float (&c)[4], const uint32_t (&a)[R][2][N], uint32_t b0,
                                         uint32_t b1) {
     auto one = [&](bool first, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
         if (START && first) {
-            mma_bf16_start(c, a0, a1, a2, a3, b0, b1);
+            if constexpr (HALF) {
+                mma_f16_start(c, a0, a1, a2, a3, b0, b1);
+            } else {
+                mma_bf16_start(c, a0, a1, a2, a3, b0, b1);
+            }
+        } else if constexpr (HALF) {
+            mma_f16(c, a0, a1, a2, a3, b0, b1);
         } else {
             mma_bf16(c, a0, a1, a2, a3, b0, b1);
         }
@@ -240,10 +291,14 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
     constexpr int G = L::kGroups;
     constexpr int R = ROWS / 8;                  // query rows of a lane: g, and g + 8
     constexpr bool kExact = sizeof(T) == 4;      // float32: 24-bit operands
-    constexpr int kTerms = kExact ? 3 : 2;       // of the weights
-    constexpr int kQ = kExact ? 3 : 1;           // of the queries (a bf16 query is one)
+    constexpr int kTerms = kExact ? 3 : 2;       // of the weights and query sums, in bf16
+    constexpr int kHalf = kExact ? 2 : 1;        // of weights x steps, in fp16
+    // Of the queries: in fp16 for codes, in bf16 otherwise; a bf16 query is one term of either.
+    constexpr int kQ = kExact ? (L::kCodes ? 2 : 3) : 1;
     constexpr int kK = STORAGE == BST_DTYPE_F32 ? (kExact ? 3 : 2) : 1;  // of keys and values
     constexpr int kMma = HD / 16;
+    constexpr float kOdd = kExact ? 0x1p15f : 0x1p11f;  // takes the 16 of nibbles 1 and 3 back
+    static_assert(!kExact || R == 1, "float32 tiles have eight rows");
     extern __shared__ __align__(16) unsigned char smem[];
 
     const int group = a.heads / a.kv_heads;
@@ -276,15 +331,15 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
                           warp * L::kStages * L::kStage;
     // A block is contiguous in its source: chunk i of this lane lies 512 i bytes after chunk 0.
     const int lane_row = lane / (L::kRowBytes / 16), lane_chunk = lane % (L::kRowBytes / 16);
-    constexpr int kHalf = kBlock * L::kRowBytes;          // bytes of a block's keys
-    constexpr int kLoads = kHalf / 512 ? kHalf / 512 : 1;  // of each lane, for the keys
+    constexpr int kKeyBytes = kBlock * L::kRowBytes;      // bytes of a block's keys
+    constexpr int kLoads = kKeyBytes / 512 ? kKeyBytes / 512 : 1;  // of each lane, for the keys
     auto lane_to = [&](int i) {
         const int r = lane_row + i * (512 / L::kRowBytes);
         return r * L::kRowBytes + swizzled<STORAGE, HD>(r, lane_chunk) * 16;
     };
     // Rows of 16 bytes: sixteen lanes take the keys, sixteen the values.
-    constexpr bool kShared = kHalf < 512;
-    const char* const k_lane = (kShared && lane >= 16 ? vb - kHalf : kb) + lane * 16;
+    constexpr bool kShared = kKeyBytes < 512;
+    const char* const k_lane = (kShared && lane >= 16 ? vb - kKeyBytes : kb) + lane * 16;
     const char* const v_lane = vb + lane * 16;
     const char* const s_lane = (lane >= 16 ? vsb : ksb) + (lane & 15) * (G * 4);
     auto fetch = [&](int block, int stage) {
@@ -294,14 +349,14 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
             const char* const ks = k_lane + static_cast<int64_t>(key0) * L::kRowBytes;
             const char* const vs = v_lane + static_cast<int64_t>(key0) * L::kRowBytes;
             const char* const ss = s_lane + static_cast<int64_t>(key0) * (G * 4);
-            const uint32_t scale_to = dst + 2 * kHalf + lane * (G * 4);
+            const uint32_t scale_to = dst + 2 * kKeyBytes + lane * (G * 4);
             if (seen.whole(key0)) {
 #pragma unroll
                 for (int i = 0; i < kLoads; ++i) cp_async<16>(dst + lane_to(i), ks + 512 * i, 16);
                 if constexpr (!kShared) {
 #pragma unroll
                     for (int i = 0; i < kLoads; ++i) {
-                        cp_async<16>(dst + kHalf + lane_to(i), vs + 512 * i, 16);
+                        cp_async<16>(dst + kKeyBytes + lane_to(i), vs + 512 * i, 16);
                     }
                 }
                 if constexpr (L::kCodes) cp_async<G * 4>(scale_to, ss, G * 4);
@@ -312,7 +367,7 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
                     const bool ok = seen.holds(key0 + (kShared ? r & 15 : r));
                     cp_async<16>(dst + lane_to(i), ok ? ks + 512 * i : kb, ok ? 16 : 0);
                     if constexpr (!kShared) {
-                        cp_async<16>(dst + kHalf + lane_to(i), ok ? vs + 512 * i : vb, ok ? 16 : 0);
+                        cp_async<16>(dst + kKeyBytes + lane_to(i), ok ? vs + 512 * i : vb, ok ? 16 : 0);
                     }
                 }
                 if constexpr (L::kCodes) {
@@ -336,7 +391,7 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
     // to_score takes a product to the base-2 logarithm of its weight. With codes, one more product
     // (qs) of the groups' query sums and the keys' lows completes a score.
     uint32_t qa[kMma][R][2][kQ], qs[R][2][kTerms] = {};
-    float to_score[R];
+    float to_score[R], qsum[G] = {};
     int position[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -358,13 +413,14 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
             }
         }
         if constexpr (L::kCodes) {
-            // Normalised to |q| < 1; products come out 2^-6 too small (2^127 for 2^133).
+            // Normalised to |q| < 1; products come out 2^-9 too small (2^15 for 2^24), or 2^15 too
+            // large.
             largest = fmaxf(largest, __shfl_xor_sync(kFull, largest, 1));
             largest = fmaxf(largest, __shfl_xor_sync(kFull, largest, 2));
             const int e = max(min(ilogbf(fmaxf(largest, FLT_MIN)), 126) + 1, -100);
             const float shrink = exp2f(static_cast<float>(-e));
             to_score[r] *= exp2f(static_cast<float>(e));
-            to_score[r] *= 64.0f;
+            to_score[r] *= kExact ? 0x1p-15f : 512.0f;
             float mine[2] = {0.0f, 0.0f};  // sums of groups 2 t and 2 t + 1
 #pragma unroll
             for (int gr = 0; gr < G; ++gr) {
@@ -373,19 +429,20 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
                 for (int i = 0; i < 8; ++i) sum += x[gr][i] *= shrink;
                 sum += __shfl_xor_sync(kFull, sum, 1);
                 sum += __shfl_xor_sync(kFull, sum, 2);
-                if (t == gr / 2) mine[gr & 1] = sum * 0.015625f;
+                if (t == gr / 2) mine[gr & 1] = sum * 0.001953125f;
+                qsum[gr] = sum * 0x1p15f;
             }
-            terms_of<kTerms>(mine[0], mine[1], qs[r][0]);
+            if constexpr (!kExact) terms_of<kTerms>(mine[0], mine[1], qs[r][0]);
         }
 #pragma unroll
         for (int gr = 0; gr < G; ++gr) {
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
                 if constexpr (L::kCodes) {
-                    terms_of<kQ>(x[gr][2 * m] * 0x1p127f, x[gr][2 * m + 4] * 0x1p127f,
-                                 qa[2 * gr + m][r][0]);
-                    terms_of<kQ>(x[gr][2 * m + 1] * 0x1p123f, x[gr][2 * m + 5] * 0x1p123f,
-                                 qa[2 * gr + m][r][1]);
+                    half_terms_of<kQ>(x[gr][2 * m] * 0x1p15f, x[gr][2 * m + 4] * 0x1p15f,
+                                      qa[2 * gr + m][r][0]);
+                    half_terms_of<kQ>(x[gr][2 * m + 1] * kOdd, x[gr][2 * m + 5] * kOdd,
+                                      qa[2 * gr + m][r][1]);
                 } else {
                     terms_of<kQ>(x[gr][4 * m], x[gr][4 * m + 1], qa[2 * gr + m][r][0]);
                     terms_of<kQ>(x[gr][4 * m + 2], x[gr][4 * m + 3], qa[2 * gr + m][r][1]);
@@ -394,8 +451,9 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
         }
     }
 
-    // Output columns, and with codes the sums over keys of weight x (step, low) of group t.
-    float o[G * 4][4], scales[4] = {}, top[R], total[R];
+    // Output columns, and with codes the sums over keys of weight x low (column n: of group n) and the
+    // steps' normalisation: 2^14 over the power of two above a group's largest step so far.
+    float o[G * 4][4], lows[4] = {}, middles[G] = {}, top[R], total[R], shrink[G];
     unsigned poison[R];  // groups in which a key that the query sees holds a NaN
 #pragma unroll
     for (int i = 0; i < G * 4; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
@@ -405,6 +463,8 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
         total[r] = 0.0f;
         poison[r] = 0u;
     }
+#pragma unroll
+    for (int gr = 0; gr < G; ++gr) shrink[gr] = 0x1p114f;  // steps below 2^-100
     // The key rows of this lane's score columns 2 t and 2 t + 1, and of the key that it loads.
     const int key_row[2] = {row_of_column<STORAGE, HD>(2 * t), row_of_column<STORAGE, HD>(2 * t + 1)};
     const int load_row = row_of_column<STORAGE, HD>(g);
@@ -414,11 +474,11 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
     int k_at = 0, lows_at = 0, scale_at[2] = {}, v_at[2] = {};
     if constexpr (L::kCodes) {
         k_at = load_row * L::kRowBytes + swizzled<STORAGE, HD>(load_row, t * 4 * G / 16) * 16 + t * 4 * G % 16;
-        lows_at = 2 * kHalf + load_row * (G * 4) + (2 * t < G ? t * 8 : 0);
+        lows_at = 2 * kKeyBytes + load_row * (G * 4) + (2 * t < G ? t * 8 : 0);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            scale_at[e] = 2 * kHalf + key_row[e] * (G * 4);
-            v_at[e] = kHalf + key_row[e] * L::kRowBytes +
+            scale_at[e] = 2 * kKeyBytes + key_row[e] * (G * 4);
+            v_at[e] = kKeyBytes + key_row[e] * L::kRowBytes +
                       swizzled<STORAGE, HD>(key_row[e], g * 2 * G / 16) * 16 + g * 2 * G % 16;
         }
     }
@@ -428,8 +488,8 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
         cp_wait<L::kStages - 2>();
         __syncwarp();
         const uint32_t ks = ring + stage * L::kStage;
-        const uint32_t vs = ks + kHalf;
-        const uint32_t vss = ks + 2 * kHalf + L::kScaleBytes;
+        const uint32_t vs = ks + kKeyBytes;
+        const uint32_t vss = ks + 2 * kKeyBytes + L::kScaleBytes;
         const int key0 = seen.key(block);
 
         // Scores of keys key0 + 8 nb + key_row[e].
@@ -443,23 +503,27 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
                 load_words<G>(ks + k_at + nb * 8 * L::kRowBytes, w);
                 load_words<G>(ks + scale_at[0] + nb * 8 * (G * 4), sa);  // (step, low) of the two
                 load_words<G>(ks + scale_at[1] + nb * 8 * (G * 4), sb);  // keys this lane scores
-                uint32_t lows;
-                if constexpr (G == 1) {
-                    uint32_t w1[1];
-                    load_words<1>(ks + lows_at + nb * 8 * (G * 4), w1);
-                    lows = w1[0] >> 16;
+                if constexpr (kExact) {
+                    s[0][nb][0] = s[0][nb][1] = 0.0f;
                 } else {
-                    uint32_t w2[2];
-                    load_words<2>(ks + lows_at + nb * 8 * (G * 4), w2);
-                    lows = __byte_perm(w2[0], w2[1], 0x7632);
-                }
-                if (2 * t >= G) lows = 0u;
-                float low[4];
-                product<true>(low, qs, lows, 0u);
+                    uint32_t key_lows;
+                    if constexpr (G == 1) {
+                        uint32_t w1[1];
+                        load_words<1>(ks + lows_at + nb * 8 * (G * 4), w1);
+                        key_lows = w1[0] >> 16;
+                    } else {
+                        uint32_t w2[2];
+                        load_words<2>(ks + lows_at + nb * 8 * (G * 4), w2);
+                        key_lows = __byte_perm(w2[0], w2[1], 0x7632);
+                    }
+                    if (2 * t >= G) key_lows = 0u;
+                    float low[4];
+                    product<false, true>(low, qs, key_lows, 0u);
 #pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    s[r][nb][0] = entry<R, kTerms>(low, r, 0);
-                    s[r][nb][1] = entry<R, kTerms>(low, r, 1);
+                    for (int r = 0; r < R; ++r) {
+                        s[r][nb][0] = entry<R, kTerms>(low, r, 0);
+                        s[r][nb][1] = entry<R, kTerms>(low, r, 1);
+                    }
                 }
 #pragma unroll
                 for (int gr = 0; gr < G; ++gr) {
@@ -471,10 +535,15 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
                         x = __byte_perm(w[gr / 2], w[G / 2 + gr / 2], gr & 1 ? 0x7632 : 0x5410);
                     }
                     float acc[4];
-                    product<true>(acc, qa[2 * gr], x & 0x000f000fu, x & 0x00f000f0u);
-                    x = __umulhi(x, 1u << 24);  // x >> 8
-                    product<false>(acc, qa[2 * gr + 1], x & 0x000f000fu, x & 0x00f000f0u);
+                    product<true, true>(acc, qa[2 * gr], nibble0<kExact>(x), nibble1<kExact>(x));
+                    x >>= 8;
+                    product<true, false>(acc, qa[2 * gr + 1], nibble0<kExact>(x), nibble1<kExact>(x));
                     const float step_a = low_of(sa[gr]), step_b = low_of(sb[gr]);
+                    if constexpr (kExact) {
+                        // The group's middle, low + 8 step, times the sum of the query's channels.
+                        s[0][nb][0] = fmaf(fmaf(8.0f, step_a, high_of(sa[gr])), qsum[gr], s[0][nb][0]);
+                        s[0][nb][1] = fmaf(fmaf(8.0f, step_b, high_of(sb[gr])), qsum[gr], s[0][nb][1]);
+                    }
 #pragma unroll
                     for (int r = 0; r < R; ++r) {
                         s[r][nb][0] = fmaf(step_a, entry<R, kQ>(acc, r, 0), s[r][nb][0]);
@@ -505,7 +574,7 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
                     for (int m = 0; m < 2; ++m) {
                         // All of the query's terms with the key's first, its leading ones with the
                         // others.
-                        product<false>(acc, qa[2 * gr + m], kw[2 * m][0], kw[2 * m + 1][0]);
+                        product<false, false>(acc, qa[2 * gr + m], kw[2 * m][0], kw[2 * m + 1][0]);
 #pragma unroll
                         for (int i = 1; i < kK; ++i) {
                             leading<R, kQ>(acc, qa[2 * gr + m], kw[2 * m][i], kw[2 * m + 1][i]);
@@ -534,7 +603,7 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
                 // A NaN that some query does not see is taken out of the products below; the
                 // queries that see it remember.
                 unsigned bad = 0u;
-                if constexpr (L::kCodes) {
+                if constexpr (L::kCodes && !kExact) {
                     uint32_t w[G];
                     load_words<G>(vss + key_at * (G * 4), w);
 #pragma unroll
@@ -570,7 +639,9 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
             for (int r = 0; r < R; ++r) total[r] *= keep[r];
             // Columns 2 and 3 are row g + 8: of the same query, or of the second.
 #pragma unroll
-            for (int j = 0; j < 4; ++j) scales[j] *= keep[R == 2 ? j / 2 : 0];
+            for (int j = 0; j < 4; ++j) lows[j] *= keep[R == 2 ? j / 2 : 0];
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr) middles[gr] *= keep[0];
 #pragma unroll
             for (int i = 0; i < G * 4; ++i) {
 #pragma unroll
@@ -593,26 +664,34 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
 
         // Weights times values.
         uint32_t pa[R][2][kTerms];
+        if constexpr (!(L::kCodes && kExact)) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            terms_of<kTerms>(p[r][0][0], p[r][0][1], pa[r][0]);
-            terms_of<kTerms>(p[r][1][0], p[r][1][1], pa[r][1]);
+            for (int r = 0; r < R; ++r) {
+                terms_of<kTerms>(p[r][0][0], p[r][0][1], pa[r][0]);
+                terms_of<kTerms>(p[r][1][0], p[r][1][1], pa[r][1]);
+            }
         }
         if constexpr (L::kCodes) {
             uint32_t sv[2][2][G];
             uint32_t wv[2][2][(G + 1) / 2];
-            uint16_t column[2][2];  // entry g of the keys' (step, low) pairs
+            uint16_t column[2][2];  // the keys' lows of group g
 #pragma unroll
             for (int nb = 0; nb < 2; ++nb) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     load_words<G>(ks + scale_at[e] + L::kScaleBytes + nb * 8 * (G * 4), sv[nb][e]);
-                    asm volatile("ld.shared.u16 %0, [%1];"
-                                 : "=h"(column[nb][e])
-                                 : "r"(ks + scale_at[e] + L::kScaleBytes + nb * 8 * (G * 4) +
-                                       (g & (2 * G - 1)) * 2));
-                    if (G < 4 && g >= 2 * G) column[nb][e] = 0;
-                    if (!all && (column[nb][e] & 0x7f80u) == 0x7f80u) column[nb][e] = 0;
+                    if constexpr (!kExact) {
+                        asm volatile("ld.shared.u16 %0, [%1];"
+                                     : "=h"(column[nb][e])
+                                     : "r"(ks + scale_at[e] + L::kScaleBytes + nb * 8 * (G * 4) +
+                                           (g & (G - 1)) * 4 + 2));
+                        if (g >= G) column[nb][e] = 0;
+                        if (!all && (column[nb][e] & 0x7f80u) == 0x7f80u) column[nb][e] = 0;
+                    } else if (!all && s[0][nb][e] == -INFINITY) {
+                        // A key that the query does not see (its low may be a NaN).
+#pragma unroll
+                        for (int gr = 0; gr < G; ++gr) sv[nb][e][gr] = 0u;
+                    }
                     // 16-bit entries [g][0 .. G): nibble j is channel 4 g + j of a group.
                     const uint32_t va = ks + v_at[e] + nb * 8 * L::kRowBytes;
                     if constexpr (G == 1) {
@@ -624,25 +703,54 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
                     }
                 }
             }
-            product<false>(scales, pa, __byte_perm(column[0][0], column[0][1], 0x5410),
-                               __byte_perm(column[1][0], column[1][1], 0x5410));
+            if constexpr (!kExact) {
+                product<false, false>(lows, pa, __byte_perm(column[0][0], column[0][1], 0x5410),
+                                      __byte_perm(column[1][0], column[1][1], 0x5410));
+            }
 #pragma unroll
             for (int gr = 0; gr < G; ++gr) {
-                uint32_t ps[R][2][kTerms], x[2];
+                const float steps[2][2] = {{low_of(sv[0][0][gr]), low_of(sv[0][1][gr])},
+                                           {low_of(sv[1][0][gr]), low_of(sv[1][1][gr])}};
+                const float largest = fmaxf(fmaxf(steps[0][0], steps[0][1]),
+                                            fmaxf(steps[1][0], steps[1][1]));
+                if (__any_sync(kFull, largest * shrink[gr] > 0x1p14f)) {
+                    // A step above the power of two: the next one, for all lanes (each has seen four
+                    // of the keys).
+                    float most = fmaxf(largest, __shfl_xor_sync(kFull, largest, 1));
+                    most = fmaxf(most, __shfl_xor_sync(kFull, most, 2));
+                    const uint32_t above = (__float_as_uint(most) & 0x7f800000u) + 0x00800000u;
+                    const float next = __uint_as_float((268u << 23) - above);  // 2^14 / above
+                    const float by = next / shrink[gr];
+                    shrink[gr] = next;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[4 * gr + j][e] *= by;
+                    }
+                }
+                uint32_t ps[R][2][kHalf], x[2];
 #pragma unroll
                 for (int nb = 0; nb < 2; ++nb) {
-                    const float step0 = low_of(sv[nb][0][gr]), step1 = low_of(sv[nb][1][gr]);
+                    const float step0 = steps[nb][0] * shrink[gr], step1 = steps[nb][1] * shrink[gr];
 #pragma unroll
                     for (int r = 0; r < R; ++r) {
-                        terms_of<kTerms>(p[r][nb][0] * step0, p[r][nb][1] * step1, ps[r][nb]);
+                        half_terms_of<kHalf>(p[r][nb][0] * step0, p[r][nb][1] * step1, ps[r][nb]);
                     }
                     x[nb] = __byte_perm(wv[nb][0][gr / 2], wv[nb][1][gr / 2], gr & 1 ? 0x7632 : 0x5410);
                 }
+                if constexpr (kExact) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    product<false>(o[4 * gr + j], ps, nibbles<!kExact>(x[0], j),
-                                       nibbles<!kExact>(x[1], j));
+                    for (int i = 0; i < 4; ++i) {
+                        middles[gr] = fmaf(p[0][i / 2][i % 2],
+                                           fmaf(8.0f, steps[i / 2][i % 2], high_of(sv[i / 2][i % 2][gr])),
+                                           middles[gr]);
+                    }
                 }
+                const uint32_t y0 = x[0] >> 8, y1 = x[1] >> 8;
+                product<true, false>(o[4 * gr], ps, nibble0<kExact>(x[0]), nibble0<kExact>(x[1]));
+                product<true, false>(o[4 * gr + 1], ps, nibble1<kExact>(x[0]), nibble1<kExact>(x[1]));
+                product<true, false>(o[4 * gr + 2], ps, nibble0<kExact>(y0), nibble0<kExact>(y1));
+                product<true, false>(o[4 * gr + 3], ps, nibble1<kExact>(y0), nibble1<kExact>(y1));
             }
         } else {
 #pragma unroll
@@ -668,7 +776,7 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
                     terms_of<kK>(v[0], v[1], v0);
                     terms_of<kK>(v[2], v[3], v1);
                 }
-                product<false>(o[j], pa, v0[0], v1[0]);
+                product<false, false>(o[j], pa, v0[0], v1[0]);
 #pragma unroll
                 for (int i = 1; i < kK; ++i) {
                     leading<R, kTerms>(o[j], pa, v0[i], v1[i]);
@@ -694,22 +802,29 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
             poison[r] |= __shfl_xor_sync(kFull, poison[r], 2);
         }
         float* mine = merge + (warp * ROWS + g + 8 * r) * (HD + 2);
-        // What the codes of group t stand above: its lows, less the 128 that the codes carry.
-        const float step_sum = entry<R, kTerms>(scales, r, 0), low_sum = entry<R, kTerms>(scales, r, 1);
-        const float below = kExact ? low_sum : fmaf(-128.0f, step_sum, low_sum);
 #pragma unroll
         for (int gr = 0; gr < G; ++gr) {
-            float low = 0.0f;
+            float low = 0.0f, by = 1.0f;
             if constexpr (L::kCodes) {
-                low = __shfl_sync(kFull, below, (lane & ~3) | gr);
-                if ((poison[r] >> gr) & 1u) low = NAN;
+                // The sum of lows of group gr is column gr: entry gr & 1 of lane t = gr / 2.
+                if constexpr (kExact) {
+                    low = middles[gr] + __shfl_xor_sync(kFull, middles[gr], 1);
+                    low += __shfl_xor_sync(kFull, low, 2);
+                } else {
+                    low = __shfl_sync(kFull, entry<R, kTerms>(lows, r, gr & 1), (lane & ~3) | (gr >> 1));
+                    if ((poison[r] >> gr) & 1u) low = NAN;
+                }
+                by = 1.0f / shrink[gr];
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 // Columns 2 t and 2 t + 1: channels 4 n + j of the group (codes) or 8 j + n.
                 const int c0 = L::kCodes ? 32 * gr + 8 * t + j : 32 * gr + 8 * j + 2 * t;
-                mine[c0] = entry<R, kTerms>(o[4 * gr + j], r, 0) + low;
-                mine[c0 + (L::kCodes ? 4 : 1)] = entry<R, kTerms>(o[4 * gr + j], r, 1) + low;
+                constexpr int N = L::kCodes ? kHalf : kTerms;
+                // Nibbles 0 and 2 count 2^-24, 1 and 3 16 times that.
+                const float unit = !L::kCodes || kExact ? 1.0f : (j & 1 ? 0x1p20f : 0x1p24f);
+                mine[c0] = fmaf(entry<R, N>(o[4 * gr + j], r, 0) * unit, by, low);
+                mine[c0 + (L::kCodes ? 4 : 1)] = fmaf(entry<R, N>(o[4 * gr + j], r, 1) * unit, by, low);
             }
         }
         if (t == 0) {
@@ -821,18 +936,25 @@ int rows_of_tile(const Batch& b, const AttnSpec& a) {
     return a.dtype == BST_DTYPE_BF16 && b.tokens * group > 8ll * b.count ? 16 : 8;
 }
 
-// CTAs for about four on every SM, and splits of at most 2048 keys so that a few long sequences
-// among short ones are spread over the SMs too; never less than 128 keys a split. The lengths are
-// on the device, so the bound is what the cache and the window allow; tiles with fewer keys use
-// fewer splits (useful_splits).
+// CTAs that an SM holds, by registers and shared memory.
+int ctas_per_sm(const Cache& c) {
+    const int size = c.head_dim == 128 ? 0 : (c.head_dim == 64 ? 1 : 2);
+    return c.storage == BST_DTYPE_F32 ? 1 << size : (size == 0 ? 2 : (size == 1 ? 4 : 5));
+}
+
+// One full wave of CTAs where the tiles alone are fewer (131 000 keys of eight heads: two waves took
+// 80 us, one @@), and among several sequences splits of at most 4096 keys, so that long ones spread
+// over the SMs beside short ones; never less than 128 keys a split. The lengths are on the device, so
+// the bound is what the cache and the window allow; tiles with fewer keys use fewer splits
+// (useful_splits).
 int split_count(const Cache& c, const Batch& b, const AttnSpec& a) {
     int64_t keys = c.slots;
     if (a.window) keys = std::min<int64_t>(keys, static_cast<int64_t>(a.window) + a.sinks + 2 * kBlock);
     const int64_t units = static_cast<int64_t>(tile_bound(b, a, rows_of_tile(b, a))) * a.kv_heads;
-    const int64_t fill = (148 * 4 + units - 1) / std::max<int64_t>(units, 1);
-    const int64_t even = (keys + 2047) / 2048;
+    const int64_t fill = 148 * ctas_per_sm(c) / std::max<int64_t>(units, 1);
+    const int64_t even = b.count > 1 ? (keys + 4095) / 4096 : 1;
     const int64_t most = std::max<int64_t>(1, keys / 128);
-    return static_cast<int>(std::min<int64_t>({std::max(fill, even), most, kMaxSplits}));
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({std::max(fill, even), most, kMaxSplits})));
 }
 
 }  // namespace
