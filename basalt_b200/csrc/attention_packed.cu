@@ -549,7 +549,9 @@ __device__ __forceinline__ void attend_query(const T* q, const T* k, int64_t k_s
 // values pass through shared memory in tiles, double-buffered with cp.async. float32 operands are
 // split in two tf32 parts, x = h + l with h the upper 10 mantissa bits, and multiplied as
 // h h + h l + l h (2^-21 of a product is left out); bf16 ones are tf32 numbers as they are, their
-// weights rounded to tf32. Splitting happens in registers after the load, so the tiles stay float32.
+// weights rounded to tf32. The tensor cores cut sums where float32 additions round: sums of a whole
+// row came out 3e-6 low, so products are summed 32 channels, or a tile of keys, at a time (the small
+// ones apart) and added up in float32. Splitting happens in registers after the load, so the tiles stay float32.
 // Rows of keys are padded to HD + 8 floats and of values to HD + 4, which keeps the fragments' reads
 // (pairs of channels of eight keys; one channel of four keys two apart) free of bank conflicts.
 // Bound by the tensor cores' mma.sync rate: 6 x 64 x 64 x HD multiply-adds a 64-key tile and warp row.
@@ -557,7 +559,7 @@ __device__ __forceinline__ void attend_query(const T* q, const T* k, int64_t k_s
 template <typename T, int HD>
 struct MmaLayout {
     static constexpr int kRows = 64, kThreads = 128;
-    static constexpr int kKeys = HD == 32 ? 64 : 32;    // three CTAs an SM
+    static constexpr int kKeys = 32;    // three CTAs an SM
     static constexpr int kKPitch = HD + 8, kVPitch = HD + 4;
     static constexpr int kStage = kKeys * (kKPitch + kVPitch);  // floats
     static constexpr int kQPitch = HD + 8;
@@ -571,10 +573,11 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// x = high + low, high with tf32's mantissa; low is rounded by the product itself.
+// x = high + low, both rounded to tf32's mantissa to the nearest (the product itself cuts: with parts
+// that it cuts, every score came out low by the same 5e-7 of itself).
 __device__ __forceinline__ void tf32_parts(float x, uint32_t* high, uint32_t* low) {
-    *high = __float_as_uint(x) & 0xffffe000u;
-    *low = __float_as_uint(x - __uint_as_float(*high));
+    *high = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+    *low = __float_as_uint(x - __uint_as_float(*high)) + 0x1000u;
 }
 
 template <typename T, int HD>
@@ -684,30 +687,45 @@ k_packed_mma(Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride, con
         float s[kBlocks][4];
 #pragma unroll
         for (int n = 0; n < kBlocks; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+        // 32 channels at a time in sums of their own, the small products apart from the large ones.
 #pragma unroll
-        for (int c = 0; c < HD / 8; ++c) {  // channels 8 c + {2 t, 2 t + 1} are k = t and t + 4
-            uint32_t qh[4], ql[4];
-            const float* from = queries + (16 * warp + g) * L::kQPitch + 8 * c + 2 * t;
-            const float2 q0 = *reinterpret_cast<const float2*>(from);
-            const float2 q1 = *reinterpret_cast<const float2*>(from + 8 * L::kQPitch);
-            tf32_parts(q0.x, &qh[0], &ql[0]);
-            tf32_parts(q1.x, &qh[1], &ql[1]);
-            tf32_parts(q0.y, &qh[2], &ql[2]);
-            tf32_parts(q1.y, &qh[3], &ql[3]);
+        for (int c0 = 0; c0 < HD / 8; c0 += 4) {
+            float large[kBlocks][4], small[kBlocks][4];
 #pragma unroll
             for (int n = 0; n < kBlocks; ++n) {
-                if (n < blocks) {
-                    const float2 x = *reinterpret_cast<const float2*>(ks + (8 * n + g) * L::kKPitch +
-                                                                      8 * c + 2 * t);
-                    uint32_t h0, l0, h1, l1;
-                    tf32_parts(x.x, &h0, &l0);
-                    tf32_parts(x.y, &h1, &l1);
-                    mma_tf32(s[n], qh, h0, h1);
-                    if constexpr (kSplit) {
-                        mma_tf32(s[n], qh, l0, l1);
-                        mma_tf32(s[n], ql, h0, h1);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) large[n][e] = small[n][e] = 0.0f;
+            }
+#pragma unroll
+            for (int c = c0; c < c0 + 4; ++c) {  // channels 8 c + {2 t, 2 t + 1} are k = t and t + 4
+                uint32_t qh[4], ql[4];
+                const float* from = queries + (16 * warp + g) * L::kQPitch + 8 * c + 2 * t;
+                const float2 q0 = *reinterpret_cast<const float2*>(from);
+                const float2 q1 = *reinterpret_cast<const float2*>(from + 8 * L::kQPitch);
+                tf32_parts(q0.x, &qh[0], &ql[0]);
+                tf32_parts(q1.x, &qh[1], &ql[1]);
+                tf32_parts(q0.y, &qh[2], &ql[2]);
+                tf32_parts(q1.y, &qh[3], &ql[3]);
+#pragma unroll
+                for (int n = 0; n < kBlocks; ++n) {
+                    if (n < blocks) {
+                        const float2 x = *reinterpret_cast<const float2*>(
+                            ks + (8 * n + g) * L::kKPitch + 8 * c + 2 * t);
+                        uint32_t h0, l0, h1, l1;
+                        tf32_parts(x.x, &h0, &l0);
+                        tf32_parts(x.y, &h1, &l1);
+                        mma_tf32(large[n], qh, h0, h1);
+                        if constexpr (kSplit) {
+                            mma_tf32(small[n], qh, l0, l1);
+                            mma_tf32(small[n], ql, h0, h1);
+                        }
                     }
                 }
+            }
+#pragma unroll
+            for (int n = 0; n < kBlocks; ++n) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[n][e] += kSplit ? large[n][e] + small[n][e] : large[n][e];
             }
         }
         float most[2] = {-INFINITY, -INFINITY};
@@ -727,7 +745,6 @@ k_packed_mma(Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride, con
             }
         }
         float from[2], keep[2];
-        bool grows = false;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             most[r] = fmaxf(most[r], __shfl_xor_sync(kFull, most[r], 1));
@@ -737,40 +754,39 @@ k_packed_mma(Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride, con
             if (up) top[r] = most[r];
             from[r] = top[r] == -INFINITY ? 0.0f : top[r];
             total[r] *= keep[r];
-            grows |= up;
         }
-        if (__any_sync(kFull, grows)) {
+        uint32_t ph[kBlocks][4], pl[kBlocks][4];
 #pragma unroll
-            for (int c = 0; c < HD / 8; ++c) {
+        for (int n = 0; n < kBlocks; ++n) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[c][e] *= keep[e >> 1];
+            for (int e = 0; e < 4; ++e) {
+                const float p = n < blocks ? exp2_fast(s[n][e] - from[e >> 1]) : 0.0f;
+                total[e >> 1] += p;
+                // Column 2 t is k = t, column 2 t + 1 is k = t + 4; rows g and g + 8.
+                const int at = (e >> 1) + 2 * (e & 1);
+                tf32_parts(p, &ph[n][at], &pl[n][at]);
             }
         }
 #pragma unroll
-        for (int n = 0; n < kBlocks; ++n) {
-            if (n < blocks) {
-                uint32_t ph[4], pl[4];
+        for (int c = 0; c < HD / 8; ++c) {
+            float large[4] = {}, small[4] = {};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float p = exp2_fast(s[n][e] - from[e >> 1]);
-                    total[e >> 1] += p;
-                    // Column 2 t is k = t, column 2 t + 1 is k = t + 4; rows g and g + 8.
-                    const int at = (e >> 1) + 2 * (e & 1);
-                    tf32_parts(p, &ph[at], &pl[at]);
-                    if constexpr (!kSplit) ph[at] = __float_as_uint(p) + 0x1000u;  // to the nearest
-                }
-#pragma unroll
-                for (int c = 0; c < HD / 8; ++c) {
+            for (int n = 0; n < kBlocks; ++n) {
+                if (n < blocks) {
                     const float* x = vs + (8 * n + 2 * t) * L::kVPitch + 8 * c + g;
                     uint32_t h0, l0, h1, l1;
                     tf32_parts(x[0], &h0, &l0);
                     tf32_parts(x[L::kVPitch], &h1, &l1);
-                    mma_tf32(o[c], ph, h0, h1);
+                    mma_tf32(large, ph[n], h0, h1);
                     if constexpr (kSplit) {
-                        mma_tf32(o[c], ph, l0, l1);
-                        mma_tf32(o[c], pl, h0, h1);
+                        mma_tf32(small, ph[n], l0, l1);
+                        mma_tf32(small, pl[n], h0, h1);
                     }
                 }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                o[c][e] = fmaf(o[c][e], keep[e >> 1], kSplit ? large[e] + small[e] : large[e]);
             }
         }
     }
