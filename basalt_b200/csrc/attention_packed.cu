@@ -706,20 +706,22 @@ k_packed_mma(Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride, con
                 tf32_parts(q1.x, &qh[1], &ql[1]);
                 tf32_parts(q0.y, &qh[2], &ql[2]);
                 tf32_parts(q1.y, &qh[3], &ql[3]);
+                // Blocks behind `blocks` are multiplied too (their keys are zeros) and masked below.
+                uint32_t h[kBlocks][2], l[kBlocks][2];
 #pragma unroll
                 for (int n = 0; n < kBlocks; ++n) {
-                    if (n < blocks) {
-                        const float2 x = *reinterpret_cast<const float2*>(
-                            ks + (8 * n + g) * L::kKPitch + 8 * c + 2 * t);
-                        uint32_t h0, l0, h1, l1;
-                        tf32_parts(x.x, &h0, &l0);
-                        tf32_parts(x.y, &h1, &l1);
-                        mma_tf32(large[n], qh, h0, h1);
-                        if constexpr (kSplit) {
-                            mma_tf32(small[n], qh, l0, l1);
-                            mma_tf32(small[n], ql, h0, h1);
-                        }
-                    }
+                    const float2 x = *reinterpret_cast<const float2*>(ks + (8 * n + g) * L::kKPitch +
+                                                                      8 * c + 2 * t);
+                    tf32_parts(x.x, &h[n][0], &l[n][0]);
+                    tf32_parts(x.y, &h[n][1], &l[n][1]);
+                }
+#pragma unroll
+                for (int n = 0; n < kBlocks; ++n) mma_tf32(large[n], qh, h[n][0], h[n][1]);
+                if constexpr (kSplit) {
+#pragma unroll
+                    for (int n = 0; n < kBlocks; ++n) mma_tf32(small[n], qh, l[n][0], l[n][1]);
+#pragma unroll
+                    for (int n = 0; n < kBlocks; ++n) mma_tf32(small[n], ql, h[n][0], h[n][1]);
                 }
             }
 #pragma unroll
@@ -767,26 +769,37 @@ k_packed_mma(Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride, con
                 tf32_parts(p, &ph[n][at], &pl[n][at]);
             }
         }
+        // Four columns of channels at a time: independent products follow one another.
 #pragma unroll
-        for (int c = 0; c < HD / 8; ++c) {
-            float large[4] = {}, small[4] = {};
+        for (int c0 = 0; c0 < HD / 8; c0 += 4) {
+            float large[4][4] = {}, small[4][4] = {};
 #pragma unroll
             for (int n = 0; n < kBlocks; ++n) {
                 if (n < blocks) {
-                    const float* x = vs + (8 * n + 2 * t) * L::kVPitch + 8 * c + g;
-                    uint32_t h0, l0, h1, l1;
-                    tf32_parts(x[0], &h0, &l0);
-                    tf32_parts(x[L::kVPitch], &h1, &l1);
-                    mma_tf32(large, ph[n], h0, h1);
+                    uint32_t h[4][2], l[4][2];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const float* x = vs + (8 * n + 2 * t) * L::kVPitch + 8 * (c0 + c) + g;
+                        tf32_parts(x[0], &h[c][0], &l[c][0]);
+                        tf32_parts(x[L::kVPitch], &h[c][1], &l[c][1]);
+                    }
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) mma_tf32(large[c], ph[n], h[c][0], h[c][1]);
                     if constexpr (kSplit) {
-                        mma_tf32(small, ph[n], l0, l1);
-                        mma_tf32(small, pl[n], h0, h1);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) mma_tf32(small[c], ph[n], l[c][0], l[c][1]);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) mma_tf32(small[c], pl[n], h[c][0], h[c][1]);
                     }
                 }
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                o[c][e] = fmaf(o[c][e], keep[e >> 1], kSplit ? large[e] + small[e] : large[e]);
+            for (int c = 0; c < 4; ++c) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    o[c0 + c][e] = fmaf(o[c0 + c][e], keep[e >> 1],
+                                        kSplit ? large[c][e] + small[c][e] : large[c][e]);
+                }
             }
         }
     }
