@@ -115,7 +115,7 @@ __device__ __forceinline__ bool elect_one() {
 }
 
 // bf16 x bf16 -> float32, M = 128; b_mn: B is MN-major.
-__device__ __forceinline__ uint32_t tc_idesc(int n, bool b_mn) {
+__device__ __forceinline__ constexpr uint32_t tc_idesc(int n, bool b_mn) {
     return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn ? 1u << 16 : 0u) |
            (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
 }
@@ -186,7 +186,7 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
     }
     const int rows = min(kTcRows, tile.n * group - tile.r0);
     const int p0 = tile.r0 / group, p1 = (tile.r0 + rows - 1) / group;
-    const KeyTiles<kTcKeys, 32> keys(p0, p1, a.window, a.sinks);
+    const KeyTiles<kTcKeys, kTcKeys> keys(p0, p1, a.window, a.sinks);
     // The second tile of a short CTA has no rows: then all is done for the first alone.
     const int halves = rows > 128 ? 2 : 1;
 
@@ -291,18 +291,20 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
             }
         }
     } else if (warp == 8) {
-        // The whole warp keeps time; one lane issues. All of it is the same in every lane.
-        const uint32_t u_tmem = __shfl_sync(kFull, tmem, 0), u_base = __shfl_sync(kFull, base, 0);
+        // The whole warp keeps time; one lane issues. Tiles are multiplied whole (what lies behind
+        // their keys is masked, or has weights of zero), and all of TMEM starts at address 0, so that
+        // operands are constants but for the slot.
         const int n_tiles = __shfl_sync(kFull, keys.tiles, 0), n_halves = __shfl_sync(kFull, halves, 0);
-        auto slot = [&](int i) { return u_base + 2 * L::kQuery + (i % L::kSlots) * L::kTile; };
-        auto scores = [&](int half, int i, int cols) {  // S = Q K^T
-            const uint32_t d = u_tmem + half * 256 + (i & 1) * 64;
-            const uint32_t qa = desc_k(u_base + half * L::kQuery), ka = desc_k(slot(k_copy(i)));
-            const uint32_t idesc = tc_idesc(cols, false);
+        constexpr uint32_t s_idesc = tc_idesc(kTcKeys, false), o_idesc = tc_idesc(HD, true);
+        const uint32_t q_desc = desc_k(base), kv_at = base + 2 * L::kQuery;
+        auto slot = [&](int i) { return kv_at + (i % L::kSlots) * L::kTile; };
+        auto scores = [&](int half, int i) {  // S = Q K^T
+            const uint32_t d = half * 256 + (i & 1) * 64;
+            const uint32_t qa = q_desc + half * (L::kQuery >> 4), ka = desc_k(slot(k_copy(i)));
 #pragma unroll
             for (int k = 0; k < HD / 16; ++k) {
                 tc_mma_ss(d, qa + (k >> 2) * (16384 >> 4) + (k & 3) * 2,
-                          ka + (k >> 2) * (kTcKeys * 128 >> 4) + (k & 3) * 2, kDescHigh, idesc, k > 0);
+                          ka + (k >> 2) * (kTcKeys * 128 >> 4) + (k & 3) * 2, kDescHigh, s_idesc, k > 0);
             }
             mma_commit(s_full + 2 * half + (i & 1));
         };
@@ -311,35 +313,33 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
             ok = await(k_copy(i), 2, abort);
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const int cols = __shfl_sync(kFull, keys.cols(i), 0);
             if (elect_one()) {
-                for (int h = 0; h < n_halves; ++h) scores(h, i, cols);
+                scores(0, i);
+                if (n_halves > 1) scores(1, i);
                 mma_commit(empty + k_copy(i) % L::kSlots);
             }
             __syncwarp();
         }
-        const uint32_t idesc = tc_idesc(HD, true);
         for (int i = 0; ok && i < n_tiles; ++i) {
             const bool more = i + 2 < n_tiles;
             ok = await(v_copy(i), 3, abort) && (!more || await(k_copy(i + 2), 4, abort));
-            const int steps = __shfl_sync(kFull, keys.cols(i), 0) / 16;
-            const int cols = more ? __shfl_sync(kFull, keys.cols(i + 2), 0) : 0;
             const uint32_t va = desc_mn(slot(v_copy(i)));
-            for (int h = 0; ok && h < n_halves; ++h) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (h >= n_halves || !ok) break;
                 ok = mbar_wait(p_full + 2 * h + (i & 1), (i >> 1) & 1, status, 5, abort);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t d = u_tmem + h * 256 + 128, p = u_tmem + h * 256 + (i & 1) * 64;
                 if (elect_one()) {
+                    const uint32_t p = h * 256 + (i & 1) * 64;
 #pragma unroll
                     for (int k = 0; k < kTcKeys / 16; ++k) {  // O += P V
-                        if (k < steps) {
-                            tc_mma_ts(d, p + 8 * k, va + k * (2048 >> 4), kDescHigh, idesc, i > 0 || k > 0);
-                        }
+                        tc_mma_ts(h * 256 + 128, p + 8 * k, va + k * (2048 >> 4), kDescHigh, o_idesc,
+                                  i > 0 || k > 0);
                     }
                     mma_commit(o_done + h);
                     // Into the buffer that the product above has just read.
-                    if (more) scores(h, i + 2, cols);
+                    if (more) scores(h, i + 2);
                 }
                 __syncwarp();
             }
@@ -394,7 +394,6 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
                 tmem_ld32(buffer + 32, s[1]);
                 tmem_ld_wait();
                 // The columns' visibility as bits: below `last`, and from `low` on or below the sinks.
-                // Columns that were not multiplied are behind `last` for every row.
                 const int last = i < keys.sink_tiles ? min(position, keys.sink_end - 1) : position;
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
