@@ -320,6 +320,7 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
             }
             __syncwarp();
         }
+#pragma unroll 2
         for (int i = 0; ok && i < n_tiles; ++i) {
             const bool more = i + 2 < n_tiles;
             ok = await(v_copy(i), 3, abort) && (!more || await(k_copy(i + 2), 4, abort));

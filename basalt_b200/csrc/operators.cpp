@@ -161,6 +161,13 @@ void limit_window(int keys, AttnSpec* a) {
     if (a->window == 0) a->sinks = 0;
 }
 
+// Query rows are counted in 32 bits.
+int check_rows(const Batch& b, const AttnSpec& a, std::string* why) {
+    if (static_cast<int64_t>(b.tokens) * a.heads <= 0x7fffffff - 65536) return BST_OK;
+    *why = "tokens x heads must stay below 2^31";
+    return BST_SHAPE;
+}
+
 int check_cached(const bst_kv_cache* cache, const bst_sequences* sequences,
                  const bst_attention_spec* spec, Cache* c, Batch* b, AttnSpec* a,
                  std::string* why) {
@@ -172,6 +179,7 @@ int check_cached(const bst_kv_cache* cache, const bst_sequences* sequences,
         *why = "spec and cache disagree on kv_heads or head_dim";
         return BST_SHAPE;
     }
+    if ((st = check_rows(*b, *a, why))) return st;
     limit_window(c->slots, a);
     if (b->starts && c->storage != BST_DTYPE_U4) {
         *why = "a float32 or bf16 cache takes one token per sequence (starts must be null)";
@@ -193,6 +201,7 @@ int check_packed(const bst_sequences* sequences, const bst_attention_spec* spec,
         *why = "packed attention takes no rows and no lengths";
         return BST_INVALID;
     }
+    if ((st = check_rows(*b, *a, why))) return st;
     limit_window(b->tokens, a);
     return BST_OK;
 }
@@ -382,9 +391,9 @@ int32_t bst_sample_tokens(int32_t device, void* stream, const void* logits, int3
     BST_OPERATOR_GUARDED("sample_tokens", {
         std::string why;
         int st = check_dtype(dtype, &why);
-        if (!st && rows < 0) {
+        if (!st && (rows < 0 || rows > (1 << 27))) {
             st = BST_SHAPE;
-            why = "rows must not be negative";
+            why = "rows must be in [0, 2^27]";
         }
         if (!st && (vocabulary < 1 || vocabulary > (1 << 20))) {
             st = BST_SHAPE;

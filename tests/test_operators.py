@@ -88,6 +88,9 @@ def test_attention_arguments_are_checked():
     assert packed(s=batch(starts=256)) == _lib.BST_INVALID         # lengths given
     assert packed(k=None) == _lib.BST_INVALID
     assert packed(k_stride=127) == _lib.BST_SHAPE
+    many = 1 << 29
+    assert packed(s=batch(starts=256, lengths=None, tokens=many)) == _lib.BST_SHAPE
+    assert cached(s=batch(count=many, tokens=many)) == _lib.BST_SHAPE
     size = ctypes.c_int64(0)
     assert _lib.load().bst_attention_cached_workspace(cache(), batch(), spec(),
                                                       None) == _lib.BST_INVALID
@@ -103,7 +106,8 @@ def test_empty_batches_are_no_work():
 
 
 @pytest.mark.parametrize("change,status", [
-    ({"dtype": 5}, _lib.BST_INVALID), ({"rows": -1}, _lib.BST_SHAPE), ({"vocabulary": 0}, _lib.BST_SHAPE),
+    ({"dtype": 5}, _lib.BST_INVALID), ({"rows": -1}, _lib.BST_SHAPE),
+    ({"rows": (1 << 27) + 1}, _lib.BST_SHAPE), ({"vocabulary": 0}, _lib.BST_SHAPE),
     ({"vocabulary": (1 << 20) + 1, "stride": 1 << 21}, _lib.BST_SHAPE), ({"stride": 9}, _lib.BST_SHAPE),
     ({"logits": None}, _lib.BST_INVALID), ({"logits": 258}, _lib.BST_INVALID),
     ({"uniforms": 260}, _lib.BST_INVALID), ({"tokens": None}, _lib.BST_INVALID),
