@@ -15,7 +15,7 @@
 // moves as the maximum of the scores does, by rescaling). fp16 has 11 bits where bf16 has 8: one
 // term is more than bf16 outputs show, and two carry 22 bits for float32. float32 also takes
 // 1024 + c, or 1024 + 16 c, to c - 8 with one fp16 operation: sums of low and of step c would
-// otherwise cancel one another (over 42 000 keys that left 7e-5 of the output where this leaves @@),
+// otherwise cancel one another (over 42 000 keys that left 7e-5 of the output where this leaves 6e-7),
 // and the tensor cores add subnormals with fewer bits.
 // mma.sync m16n8k16 reads its B operand from registers, which is where unpacked codes are;
 // tcgen05 would need them written to shared memory at four times their size first, and a tile
@@ -930,7 +930,7 @@ k_cached_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out,
 }
 
 // Query rows a tile: 16 where bf16 sequences have more than eight to a key head on average. For
-// four tokens of four heads that took a step over 24 caches of up to 16 384 keys from 330 to @@ us.
+// four tokens of four heads that took a step over 24 caches of up to 16 384 keys from 330 to 219 us.
 int rows_of_tile(const Batch& b, const AttnSpec& a) {
     const int64_t group = a.heads / a.kv_heads;
     return a.dtype == BST_DTYPE_BF16 && b.tokens * group > 8ll * b.count ? 16 : 8;
@@ -943,7 +943,7 @@ int ctas_per_sm(const Cache& c) {
 }
 
 // One full wave of CTAs where the tiles alone are fewer (131 000 keys of eight heads: two waves took
-// 80 us, one @@), and among several sequences splits of at most 4096 keys, so that long ones spread
+// 80 us, one 68), and among several sequences splits of at most 4096 keys, so that long ones spread
 // over the SMs beside short ones; never less than 128 keys a split. The lengths are on the device, so
 // the bound is what the cache and the window allow; tiles with fewer keys use fewer splits
 // (useful_splits).
