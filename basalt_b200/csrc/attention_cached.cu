@@ -714,12 +714,14 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
                 const float largest = fmaxf(fmaxf(steps[0][0], steps[0][1]),
                                             fmaxf(steps[1][0], steps[1][1]));
                 if (__any_sync(kFull, largest * shrink[gr] > 0x1p14f)) {
-                    // A step above the power of two: the next one, for all lanes (each has seen four
-                    // of the keys).
+                    // A step above the power of two: the next one, for a row's lanes (each has seen
+                    // four of the keys). A row that sees no larger step, or no key at all, stays.
                     float most = fmaxf(largest, __shfl_xor_sync(kFull, largest, 1));
                     most = fmaxf(most, __shfl_xor_sync(kFull, most, 2));
                     const uint32_t above = (__float_as_uint(most) & 0x7f800000u) + 0x00800000u;
-                    const float next = __uint_as_float((268u << 23) - above);  // 2^14 / above
+                    const float next = most * shrink[gr] > 0x1p14f
+                                           ? __uint_as_float((268u << 23) - above)  // 2^14 / above
+                                           : shrink[gr];
                     const float by = next / shrink[gr];
                     shrink[gr] = next;
 #pragma unroll

@@ -245,6 +245,37 @@ def test_what_is_not_visible_takes_no_part(ops, storage):
     assert (out == 0).all()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (66, 0), (66, 3)])
+def test_later_values_of_another_size_stay_out_of_earlier_rows(ops, dtype, window, sinks):
+    """Steps that grow or shrink from block to block of keys, some of which only a tile's later, or
+    only its earlier, tokens see."""
+    rng = np.random.default_rng(window + sinks)
+    counts, lengths, heads, dim = [24, 24, 5], [70, 134, 33], 2, 64
+    x = rng.standard_normal((3 * 140, heads, dim)).astype(np.float32)
+    sizes = (2.0 ** rng.integers(-6, 7, (3, 20))).astype(np.float32)
+    sizes[0, :9], sizes[0, 9:] = 1, 64                   # the first sequence: from key 63 on
+    values = x * np.repeat(sizes, 7, 1).reshape(-1, 1, 1)
+    cache = ops.KvCache.allocate(3, heads, 140, dim)
+    full, at = ints([140] * 3), ints([0, 140, 280, 420])
+    ops.kv_append(cache, tensor(x), tensor(values), full, starts=at)
+    k, v = (host(t).reshape(3, 140, heads, dim) for t in ops.kv_read(cache, full, starts=at, tokens=420))
+    q = tensor(rng.standard_normal((sum(counts), heads, dim)).astype(np.float32), dtype)
+    starts = np.concatenate([[0], np.cumsum(counts)])
+    got = host(ops.attention_cached(cache, q, ints(lengths), starts=ints(starts), window=window,
+                                    sinks=sinks))
+    # The bounds hold for each query by itself: max|v| over the keys that it sees.
+    qh = host(q)
+    for s, n in enumerate(counts):
+        for i in range(n):
+            position, t = lengths[s] - n + i, starts[s] + i
+            seen = ref.visible(position, lengths[s], window, sinks)
+            want, size = ref.attend(qh[t:t + 1], k[s, :lengths[s]], v[s, :lengths[s]], position, window,
+                                    sinks, 1 / 8)
+            tol = bound(size, dim, lengths[s], np.abs(v[s, :lengths[s]][seen]).max(), want, dtype)
+            assert np.all(np.abs(got[t] - want[0]) <= tol[0]), (s, i)
+
+
 def test_a_long_4_bit_cache(ops):
     """Work split over the keys: one sequence of 40 000 keys, and offsets past 2^31 bytes."""
     torch = torch_()
