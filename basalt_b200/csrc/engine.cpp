@@ -1494,14 +1494,14 @@ int Engine::enqueue_prefill(const StepPlan& p, size_t begin, size_t end) {
                                                                ws.k_new, d, ws.v_new, d, ws.att, d,
                                                                ws.attn_space);
                        }), "prefill attention");
-        } else
-        st = check(launch(bst::kAttnPrefill, attn_bytes, attn_flops, 1, [&] {
-                       return bst::launch_attn_prefill(stream, ws.q, qkv.k_cache, qkv.v_cache,
-                                                       kvbf16, ws.seg_row, ws.seg_start,
-                                                       ws.seg_len, segs, max_len, H, hd, slots,
-                                                       scale, att_planes.planes ? nullptr : ws.att,
-                                                       att_planes);
-                   }), "prefill attention");
+        } else {
+            st = check(launch(bst::kAttnPrefill, attn_bytes, attn_flops, 1, [&] {
+                           return bst::launch_attn_prefill(
+                               stream, ws.q, qkv.k_cache, qkv.v_cache, kvbf16, ws.seg_row,
+                               ws.seg_start, ws.seg_len, segs, max_len, H, hd, slots, scale,
+                               att_planes.planes ? nullptr : ws.att, att_planes);
+                       }), "prefill attention");
+        }
         if (st) return st;
         EpiArgs res;
         res.out = ws.x;
@@ -1782,20 +1782,27 @@ int Engine::decode_after_qkv(int l, int R, const int* rowmap, const int* lengths
         step.count = step.tokens = R;
         step.rows = rowmap;
         step.lengths = lengths;
-        st = check(launch(attn_class, kv_bytes, 4.0 * dp.sum_len * d, 1, [&] {
+        // What the rows see of a 4-bit cache takes 5 bits a value.
+        const double value_bytes = spec.kv_dtype == BST_DTYPE_U4 ? 0.625 : kvb;
+        const double seen = spec.attention_window > 0
+                                ? std::min(static_cast<double>(dp.sum_len),
+                                           R * (static_cast<double>(spec.attention_window) +
+                                                spec.attention_sinks))
+                                : static_cast<double>(dp.sum_len);
+        st = check(launch(attn_class, (seen * 2.0 * value_bytes + R * 8.0) * d, 4.0 * seen * d, 1, [&] {
                        return bst::launch_attention_cached(stream, layer_cache(l), step,
                                                            attention_spec(), ws.q, d, ws.att, d,
                                                            ws.attn_space);
                    }), "decode attention");
-    } else
-    st = check(launch(attn_class, kv_bytes, 4.0 * dp.sum_len * d, 1, [&] {
-                   return bst::launch_attn_decode(stream, ws.q, k_cache, v_cache,
-                                                  kvbf16, rowmap, ws.len, R, H, hd, slots,
-                                                  scale, dp.splits, dp.chunk, ws.part,
-                                                  ws.attn_tickets,
-                                                  att_planes.planes ? nullptr : ws.att,
-                                                  att_planes, qparts);
-               }), "decode attention");
+    } else {
+        st = check(launch(attn_class, kv_bytes, 4.0 * dp.sum_len * d, 1, [&] {
+                       return bst::launch_attn_decode(stream, ws.q, k_cache, v_cache, kvbf16, rowmap,
+                                                      ws.len, R, H, hd, slots, scale, dp.splits,
+                                                      dp.chunk, ws.part, ws.attn_tickets,
+                                                      att_planes.planes ? nullptr : ws.att,
+                                                      att_planes, qparts);
+                   }), "decode attention");
+    }
     if (st) return st;
     const bst::LnArgs ln2{lw.ln2_g, lw.ln2_b, kLayerNormEps};
     bool ffn_in_normalised = false;
@@ -2281,8 +2288,11 @@ int Engine::run(Mode mode, const int32_t* contexts, int32_t rows, int32_t length
             return fail(BST_UNSUPPORTED, "sampling supports vocabularies up to 16384");
         }
     }
-    if (mode == Mode::kFiltered && !filter_uniforms) {
-        return fail(BST_INVALID, "uniforms must not be null");
+    if (mode == Mode::kFiltered) {
+        if (!filter_uniforms) return fail(BST_INVALID, "uniforms must not be null");
+        if (V > (1 << 20)) {
+            return fail(BST_UNSUPPORTED, "filtered sampling supports vocabularies up to 2^20");
+        }
     }
     if (!contexts) return fail(BST_INVALID, "contexts must not be null");
     if (rows < 1) return fail(BST_INVALID, "contexts must not be empty");

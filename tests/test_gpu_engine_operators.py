@@ -235,3 +235,13 @@ def test_refusals(make):
         engine.sampleFiltered(contexts, 3, np.ones((2, 3)))
     with pytest.raises(IllegalArgumentException, match="steps"):
         engine.sampleFiltered(contexts, 0, np.zeros((2, 0)))
+
+
+def test_vocabularies_behind_the_draws_range_are_refused(runtime):
+    from basalt_b200 import BasaltUnsupportedOperationException
+
+    size = 2 ** 20 + 1
+    engine = TextEngine.of(runtime, ModelSpec("char_lm", size, 3, dimension=1, hidden=1), size, 3)
+    with pytest.raises(BasaltUnsupportedOperationException, match="2\\^20"):
+        engine.sampleFiltered(np.zeros((1, 3), np.int32), 1, np.zeros((1, 1)))
+    engine.close()
