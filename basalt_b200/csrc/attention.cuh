@@ -71,7 +71,7 @@ __device__ __forceinline__ bool find_tile(const Batch& b, int group, int tile_ro
         const int s = s0 + lane;
         int from = 0, n = 0;
         if (s < b.count) {
-            from = __ldg(b.starts + s);
+            from = max(0, __ldg(b.starts + s));
             n = max(0, min(__ldg(b.starts + s + 1), b.tokens) - from);
         }
         const int tiles = (n * group + tile_rows - 1) / tile_rows;

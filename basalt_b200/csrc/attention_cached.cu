@@ -882,7 +882,6 @@ k_cached_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out,
     int seq, first, n;
     if (!find_sequence(b, token, &seq, &first, &n)) return;
     // How many splits the query's tile used, as k_cached found it.
-    n = min(n, b.tokens - first);
     const int group = a.heads / a.kv_heads;
     const int row = b.rows ? __ldg(b.rows + seq) : seq;
     const int length = max(0, __ldg(b.lengths + seq));

@@ -31,6 +31,12 @@ int check_batch(const bst_sequences* s, bool lengths_needed, Batch* out, std::st
                std::to_string(s->tokens) + " tokens and " + std::to_string(s->count) + " sequences";
         return BST_SHAPE;
     }
+    for (const void* p : {s->rows, s->starts, s->lengths}) {
+        if (reinterpret_cast<uintptr_t>(p) % 4) {
+            *why = "sequences: rows, starts and lengths must be aligned to 4 bytes";
+            return BST_INVALID;
+        }
+    }
     out->count = s->count;
     out->tokens = s->tokens;
     out->rows = s->rows;
@@ -94,6 +100,10 @@ int check_cache(const bst_kv_cache* c, Cache* out, std::string* why) {
     if (const int st = check_head_dim(c->head_dim, why)) return st;
     if (c->rows < 1 || c->kv_heads < 1 || c->slots < 1 || c->kv_heads > 65535) {
         *why = "cache rows, heads and slots must be positive (and at most 65535 heads)";
+        return BST_SHAPE;
+    }
+    if (c->slots > 0x7fffffff - 65536) {  // slots are counted in 32 bits, in blocks
+        *why = "cache slots must stay below 2^31 - 65536";
         return BST_SHAPE;
     }
     const bool scaled = c->storage == BST_DTYPE_U4;
@@ -416,6 +426,17 @@ int32_t bst_sample_tokens(int32_t device, void* stream, const void* logits, int3
                     reinterpret_cast<uintptr_t>(tokens) % 4)) {
             st = BST_INVALID;
             why = "logits, uniforms and tokens must be aligned to their elements";
+        }
+        if (!st) {
+            for (const void* p : {static_cast<const void*>(sampling->temperatures),
+                                  static_cast<const void*>(sampling->top_ps),
+                                  static_cast<const void*>(sampling->min_ps),
+                                  static_cast<const void*>(sampling->top_ks)}) {
+                if (reinterpret_cast<uintptr_t>(p) % 4) {
+                    st = BST_INVALID;
+                    why = "per-row settings must be aligned to 4 bytes";
+                }
+            }
         }
         if (st) return refuse("sample_tokens", st, why);
         if (rows == 0) return BST_OK;

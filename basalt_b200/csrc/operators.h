@@ -106,7 +106,7 @@ __device__ __forceinline__ bool find_sequence(const Batch& b, int t, int* seq, i
             hi = mid - 1;
         }
     }
-    const int from = __ldg(b.starts + lo), to = __ldg(b.starts + lo + 1);
+    const int from = max(0, __ldg(b.starts + lo)), to = min(__ldg(b.starts + lo + 1), b.tokens);
     *seq = lo;
     *first = from;
     *n = to - from;

@@ -291,7 +291,8 @@ int32_t bst_context_clear_graph(bst_context context);
  * rows is NULL) and the packed tokens [starts[s], starts[s + 1]) of this call (token s alone when
  * starts is NULL, and then tokens == count). lengths[s] counts the row's cached tokens with this
  * call's tokens included: with n tokens, token i of the sequence has position (and cache slot)
- * lengths[s] - n + i. starts must not decrease. The arrays are read on the device: tokens that no
+ * lengths[s] - n + i. starts must not decrease; what of a sequence lies outside [0, tokens) does
+ * not belong to it. The arrays are read on the device: tokens that no
  * sequence owns are left alone (their outputs stay as they were), and tokens whose row or slot lies
  * outside the cache are not stored, see no keys and read as zeros. */
 typedef struct bst_sequences {

@@ -100,6 +100,32 @@ def test_attention_arguments_are_checked():
         assert cached(ws=256, n=size.value - 1) == _lib.BST_SHAPE
 
 
+@pytest.mark.parametrize("name", ["rows", "starts", "lengths"])
+def test_index_arrays_are_aligned(name):
+    s = batch(**{name: 258})
+    assert _lib.load().bst_kv_append(0, None, cache(), s, 256, 128, 256, 128,
+                                     _lib.DTYPE_F32) == _lib.BST_INVALID
+    assert cached(s=s) == _lib.BST_INVALID
+    if name == "starts":
+        assert packed(s=batch(starts=257, lengths=None)) == _lib.BST_INVALID
+
+
+@pytest.mark.parametrize("name", ["temperatures", "top_ps", "min_ps", "top_ks"])
+def test_per_row_settings_are_aligned(name):
+    p = _lib.SamplingStruct()
+    setattr(p, name, 257)
+    assert _lib.load().bst_sample_tokens(0, None, 256, _lib.DTYPE_F32, 2, 10, 10, p, 256,
+                                         256) == _lib.BST_INVALID
+    assert "aligned" in _lib.last_error()
+
+
+def test_slots_are_counted_in_32_bits():
+    for slots in (2 ** 31 - 1, 2 ** 31 - 65536):
+        assert cached(c=cache(slots=slots)) == _lib.BST_SHAPE
+        assert _lib.load().bst_kv_read(0, None, cache(slots=slots), batch(), 256, 128, 256, 128,
+                                       _lib.DTYPE_F32) == _lib.BST_SHAPE
+
+
 def test_empty_batches_are_no_work():
     assert cached(s=batch(count=0, tokens=0, lengths=None), q=None, out=None) == _lib.BST_OK
     assert packed(s=batch(count=0, tokens=0, starts=256, lengths=None), q=None) == _lib.BST_OK
