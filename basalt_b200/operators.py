@@ -3,8 +3,8 @@
 
 Tensors stay on the GPU: every call takes their device pointers, queues its kernels on ``stream``
 (torch's current stream of the tensors' device by default) and returns without waiting. Outputs and
-workspaces come from torch's allocator on that device unless given, so calls can be captured into a
-CUDA graph (call once before the capture, which loads the kernels). ``include/basalt_cuda.h`` has
+workspaces come from torch's allocator, for that stream of that device, unless given, so calls can be
+captured into a CUDA graph (call once before the capture, which loads the kernels). ``include/basalt_cuda.h`` has
 the operators' definitions; a rejected argument raises the exception of its status.
 
 A batch is a list of sequences: ``lengths[s]`` counts the tokens of sequence s with this call's
@@ -86,6 +86,14 @@ def _packed(device, name, t, heads=None, head_dim=None):
     return stride[0] if n > 1 else max(stride[0], h * d)
 
 
+def _empty(shape, dtype, device, stream):
+    """A tensor whose memory is reused in the order of ``stream`` (None: the current one)."""
+    if stream is None:
+        return _module.empty(shape, dtype=dtype, device=device)
+    with _module.cuda.stream(_module.cuda.ExternalStream(stream, device)):
+        return _module.empty(shape, dtype=dtype, device=device)
+
+
 def _stream(device, stream):
     if stream is not None:
         return stream
@@ -161,6 +169,8 @@ def _sequences(device, tokens, lengths, starts, rows):
         at = _index(device, "lengths", lengths)
         count = lengths.shape[0]
     else:
+        if starts is None:
+            raise IllegalArgumentException("starts must be given", _lib.BST_INVALID)
         at, count = None, starts.shape[0] - 1
         if count < 0:
             raise BasaltShapeException("starts must have one entry more than there are sequences",
@@ -197,8 +207,8 @@ def kv_read(cache: KvCache, lengths, starts=None, rows=None, tokens=None, dtype=
             tokens = lengths.shape[0]
         shape = (tokens, cache.kv_heads, cache.head_dim)
         dtype = dtype or _module.float32
-        k = _module.empty(shape, dtype=dtype, device=device)
-        v = _module.empty(shape, dtype=dtype, device=device)
+        k = _empty(shape, dtype, device, stream)
+        v = _empty(shape, dtype, device, stream)
         k_stride = v_stride = cache.kv_heads * cache.head_dim
     else:
         k, v = out
@@ -221,23 +231,25 @@ def _spec(q, kv_heads, window, sinks, scale):
                                     dim ** -0.5 if scale is None and dim else scale or 0.0, 0)
 
 
-def _out(device, q, out):
+def _out(device, q, out, stream):
     if out is None:
-        out = _module.empty(q.shape, dtype=q.dtype, device=device)
+        out = _empty(q.shape, q.dtype, device, stream)
         return out, q.shape[1] * q.shape[2]
     if out.dtype != q.dtype or out.shape != q.shape:
         raise BasaltShapeException("out must be like q", _lib.BST_SHAPE)
     return out, _packed(device, "out", out)
 
 
-def _workspace(device, size, workspace):
+def _workspace(device, size, workspace, stream):
     """(pointer, bytes, tensor) of a workspace of at least ``size`` bytes."""
     if workspace is None:
         if size == 0:
             return None, 0, None
-        workspace = _module.empty(size, dtype=_module.uint8, device=device)
+        workspace = _empty(size, _module.uint8, device, stream)
         return workspace.data_ptr(), size, workspace
     _on(device, "workspace", workspace)
+    if not workspace.is_contiguous():
+        raise IllegalArgumentException("workspace must be contiguous", _lib.BST_INVALID)
     return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
 
 
@@ -248,7 +260,7 @@ def attention_cached(cache: KvCache, q, lengths, starts=None, rows=None, window:
     keys (0: all) and the first ``sinks``. ``scale`` is 1 / sqrt(head_dim) by default."""
     device = cache.device
     q_stride = _packed(device, "q", q, None, cache.head_dim)
-    out, out_stride = _out(device, q, out)
+    out, out_stride = _out(device, q, out, stream)
     s = _sequences(device, q.shape[0], lengths, starts, rows)
     a = _spec(q, cache.kv_heads, window, sinks, scale)
     lib = _lib.load()
@@ -258,7 +270,7 @@ def attention_cached(cache: KvCache, q, lengths, starts=None, rows=None, window:
         size = ctypes.c_int64(0)
         _raise(lib.bst_attention_cached_workspace(cache._ref, s, a, size))
         needed = cache._sizes[key] = size.value
-    pointer, room, workspace = _workspace(device, needed, workspace)
+    pointer, room, workspace = _workspace(device, needed, workspace, stream)
     _raise(lib.bst_attention_cached(device.index, _stream(device, stream), cache._ref, s, a,
                                     q.data_ptr(), q_stride, out.data_ptr(), out_stride, pointer,
                                     room))
@@ -277,13 +289,13 @@ def attention_packed(q, k, v, starts, window: int = 0, sinks: int = 0, scale=Non
     v_stride = _packed(device, "v", v, k.shape[1], q.shape[2])
     if not q.dtype == k.dtype == v.dtype or not q.shape[0] == k.shape[0] == v.shape[0]:
         raise BasaltShapeException("q, k and v must have the same type and tokens", _lib.BST_SHAPE)
-    out, out_stride = _out(device, q, out)
+    out, out_stride = _out(device, q, out, stream)
     s = _sequences(device, q.shape[0], None, starts, None)
     a = _spec(q, k.shape[1], window, sinks, scale)
     lib = _lib.load()
     size = ctypes.c_int64(0)
     _raise(lib.bst_attention_packed_workspace(s, a, size))
-    pointer, room, workspace = _workspace(device, size.value, workspace)
+    pointer, room, workspace = _workspace(device, size.value, workspace, stream)
     _raise(lib.bst_attention_packed(device.index, _stream(device, stream), s, a, q.data_ptr(),
                                     q_stride, k.data_ptr(), k_stride, v.data_ptr(), v_stride,
                                     out.data_ptr(), out_stride, pointer, room))
@@ -319,7 +331,7 @@ def sample_tokens(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0
         raise IllegalArgumentException(f"uniforms must be a contiguous float64 vector of {rows}",
                                        _lib.BST_INVALID)
     if out is None:
-        out = _module.empty(rows, dtype=_module.int32, device=device)
+        out = _empty(rows, _module.int32, device, stream)
     else:
         _index(device, "out", out, rows)
     p = _lib.SamplingStruct()

@@ -536,6 +536,92 @@ def test_captured_steps_and_other_streams(ops):
     assert all(torch.equal(o, one[w]) for w in range(2) for o in both[w])
 
 
+def test_captured_prompts_and_draws(ops):
+    """Packed attention and draws with per-row settings, captured together, on changed inputs."""
+    torch = torch_()
+    rng = np.random.default_rng(8)
+    T, H, KV, d, V = 200, 4, 2, 64, 3000
+    calls = []
+    for dtype in ("f32", "bf16"):
+        q, k, v = (tensor(rng.standard_normal((T, n, d)).astype(np.float32), dtype) for n in (H, KV, KV))
+        starts, u = ints([0, 150, 150, 190]), tensor(rng.random(12))
+        x = tensor(rng.standard_normal((12, V)).astype(np.float32), dtype)
+        warm = tensor(rng.random(12).astype(np.float32) + 0.5)
+        few, most, least = ints(rng.integers(0, 60, 12)), warm - 0.4, warm * 0.01
+        calls.append((q, k, v, starts, u, x, warm, few, most, least))
+
+    def step():
+        return [(ops.attention_packed(q, k, v, starts, window=40, sinks=2)[:190],
+                 ops.sample_tokens(x, u, warm, few, most, least))
+                for q, k, v, starts, u, x, warm, few, most, least in calls]
+
+    step()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=side):
+        held = step()
+    for change in range(3):
+        for q, k, v, starts, u, x, warm, few, most, least in calls:
+            for t in (q, k, v, x):
+                t.copy_(tensor(rng.standard_normal(t.shape).astype(np.float32)))
+            if change == 1:
+                v[rng.integers(0, 190), 0, 3] = float("nan")
+            u.copy_(tensor(rng.random(12)))
+            few.copy_(ints(rng.integers(0, 60, 12)))
+            starts.copy_(ints([0, 20 + change, 100, 190]))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [[t.clone() for t in pair] for pair in held]
+        for pair, (a, b) in zip(got, step()):
+            assert torch.equal(pair[0].nan_to_num(7.0), a.nan_to_num(7.0)) and torch.equal(pair[1], b)
+
+
+def test_memory_belongs_to_the_given_stream(ops):
+    """What a call on a stream of its own allocates may be used again in that stream's order only."""
+    torch = torch_()
+    rng = np.random.default_rng(12)
+    cache, _ = filled_cache(ops, rng, 2, 2, 4000, 64, "u4")
+    q, lengths = tensor(rng.standard_normal((2, 8, 64)).astype(np.float32)), ints([4000, 3999])
+    want = ops.attention_cached(cache, q, lengths)
+    u, x = tensor(rng.random(2)), tensor(rng.standard_normal((2, 50)).astype(np.float32))
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    s = side.cuda_stream
+    outs = [ops.attention_cached(cache, q, lengths, stream=s), ops.sample_tokens(x, u, stream=s),
+            *ops.kv_read(cache, lengths, stream=s),
+            ops.attention_packed(q, q, q, ints([0, 2]), stream=s)]
+    segments = torch.cuda.memory_snapshot()
+    for t in outs:
+        at = t.data_ptr()
+        owner = [g["stream"] for g in segments if g["address"] <= at < g["address"] + g["total_size"]]
+        assert owner == [s]
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want)
+    zero = ops.attention_cached(cache, q, lengths, stream=0)        # the legacy default stream
+    torch.cuda.synchronize()
+    assert torch.equal(zero, want)
+
+
+def test_what_lies_outside_the_tokens_belongs_to_no_sequence(ops):
+    """starts below 0 and behind the last token: the sequences' parts between are what counts."""
+    torch = torch_()
+    rng = np.random.default_rng(13)
+    T, KV, d = 40, 2, 64
+    q, k, v = (tensor(rng.standard_normal((T, n, d)).astype(np.float32)) for n in (4, KV, KV))
+    lengths = ints([9, 60])
+    results = []
+    for starts in ([0, 7, T], [-5, 7, T + 300]):
+        cache = ops.KvCache.allocate(2, KV, 64, d)
+        starts = ints(starts)
+        ops.kv_append(cache, k, v, lengths, starts=starts)
+        results.append([cache.k, cache.v_scale, *ops.kv_read(cache, lengths, starts=starts, tokens=T),
+                        ops.attention_cached(cache, q, lengths, starts=starts),
+                        ops.attention_packed(q, k, v, starts, window=6, sinks=1),
+                        ops.attention_packed(*(x.bfloat16() for x in (q, k, v)), starts)])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
 def test_the_same_call_twice_gives_the_same_bits(ops):
     torch = torch_()
     rng = np.random.default_rng(6)
@@ -546,3 +632,16 @@ def test_the_same_call_twice_gives_the_same_bits(ops):
     x = [tensor(rng.standard_normal((600, 4, 128)).astype(np.float32), "bf16") for _ in range(3)]
     a, b = (ops.attention_packed(*x, ints([0, 600]), window=200, sinks=4) for _ in range(2))
     assert torch.equal(a, b)
+
+
+def test_workspaces_are_checked(ops):
+    torch = torch_()
+    from basalt_b200 import BasaltShapeException, IllegalArgumentException
+
+    x = torch.zeros((40, 2, 64), device="cuda")
+    with pytest.raises(BasaltShapeException, match="workspace"):
+        ops.attention_packed(x, x, x, ints([0, 40]), workspace=torch.empty(1, device="cuda"))
+    with pytest.raises(IllegalArgumentException, match="contiguous"):
+        ops.attention_packed(x, x, x, ints([0, 40]), workspace=torch.empty(1, device="cuda").expand(1 << 20))
+    with pytest.raises(IllegalArgumentException, match="starts"):
+        ops.attention_packed(x, x, x, None)
