@@ -867,6 +867,282 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
     }
 }
 
+// ---- one query a key head ------------------------------------------------------------------------
+// Where a key head has one query the tensor cores' other rows would be empty, so this kernel multiplies
+// on the ordinary units, two operations a value: a nibble masked out of its word is, as a float, the
+// subnormal c 2^(4 i - 149), and the other factor of the fused multiply-add (the query's channel, or
+// weight x step) carries the power of two that is missing. Both are normalised so that neither they
+// nor the products leave float32's range: queries by a power of two of the row, steps by a lane's own
+// largest so far.
+// HD / 8 lanes take a key, a word of eight codes each, and the warp 256 / HD keys a pass. After eight
+// passes the partial sums change places, half as many at every step, so that a lane ends with the
+// whole sums of one key, its own: it loads that key's scales, finishes and masks the score, and hands
+// weight x step back by shuffles. Words go to registers, the values' before the scores and the next
+// keys' behind them.
+// A query sees all keys of two ranges, sinks and window, so nothing inside them is masked; lanes behind
+// the end take the last key with a weight of zero.
+constexpr int kOneWarps = 2;
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kOneWarps * 32, 20 / kOneWarps)
+k_cached_one(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride,
+             T* __restrict__ out, int64_t out_stride, int splits, float* __restrict__ part) {
+    constexpr int G = HD / 32;
+    constexpr int kLanes = HD / 8, kAtOnce = 32 / kLanes, kPasses = 8, kKeys = kAtOnce * kPasses;
+    constexpr int kMine = kLanes < 8 ? 8 / kLanes : 1;  // keys of a lane
+    constexpr int kSums = G == 1 ? 1 : 2;               // groups of a lane's word
+    // Lanes with the same groups: all, or every other one.
+    constexpr int kNext = G == 4 ? 2 : 1;
+    __shared__ float merge[kOneWarps][HD + 2];
+    const int seq = blockIdx.x, head = blockIdx.y, split = blockIdx.z;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int word = lane % kLanes, sub = lane / kLanes;
+    const int row = b.rows ? __ldg(b.rows + seq) : seq;
+    const int position = max(0, __ldg(b.lengths + seq)) - 1;
+    const bool inside = row >= 0 && row < c.rows;
+    const Visible seen(position, inside ? position : -1, c.slots, a.window, a.sinks);
+    const int use = useful_splits(seen.blocks, splits);
+    if (split >= use) return;
+    // Places 0 .. sunk are the sinks before the window, the others the window's keys.
+    const bool sees = inside && position >= 0 && position < c.slots;
+    const int sunk = sees ? min(a.sinks, seen.first) : 0, skipped = seen.first - sunk;
+    const int64_t places = sees ? static_cast<int64_t>(sunk) + seen.end - seen.first : 0;
+    const int x0 = static_cast<int>(places * split / use), x1 = static_cast<int>(places * (split + 1) / use);
+
+    const int64_t at = (static_cast<int64_t>(inside ? row : 0) * c.kv_heads + head) * c.slots;
+    const char* const kb = static_cast<const char*>(c.k) + at * (HD / 2) + word * 4;
+    const char* const vb = static_cast<const char*>(c.v) + at * (HD / 2) + word * 4;
+    const int scale_offset = G == 4 ? (word & 1) * 8 : 0;
+    const char* const ksb = static_cast<const char*>(c.k_scale) + at * (G * 4) + scale_offset;
+    const char* const vsb = static_cast<const char*>(c.v_scale) + at * (G * 4) + scale_offset;
+    const int my_pass = word * 8 / kLanes;  // and the one behind it with two keys a lane
+    auto key_at = [&](int place) {
+        place = min(place, x1 - 1);
+        return static_cast<int64_t>(place + (place >= sunk ? skipped : 0));
+    };
+    // The words of the keys at places x + i kAtOnce + sub, and the scales of the lane's own.
+    auto load = [&](int x, const char* codes, const char* scales, uint32_t (&w)[kPasses],
+                    uint32_t (&sc)[kMine][kSums]) {
+        if (x >= x1) return;
+        if (x + kKeys <= x1 && (x >= sunk || x + kKeys <= sunk)) {
+            const char* const from = codes + key_at(x + sub) * (HD / 2);
+#pragma unroll
+            for (int i = 0; i < kPasses; ++i) {
+                w[i] = __ldg(reinterpret_cast<const uint32_t*>(from + i * kAtOnce * (HD / 2)));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPasses; ++i) {
+                w[i] = __ldg(reinterpret_cast<const uint32_t*>(
+                    codes + key_at(x + i * kAtOnce + sub) * (HD / 2)));
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < kMine; ++m) {
+            const char* const from = scales + key_at(x + (my_pass + m) * kAtOnce + sub) * (G * 4);
+            if constexpr (kSums == 1) {
+                sc[m][0] = __ldg(reinterpret_cast<const uint32_t*>(from));
+            } else {
+                const uint2 both = __ldg(reinterpret_cast<const uint2*>(from));
+                sc[m][0] = both.x;
+                sc[m][1] = both.y;
+            }
+        }
+    };
+    uint32_t kw[kPasses] = {}, ks[kMine][kSums] = {};
+    int x = x0 + warp * kKeys;
+    load(x, kb, ksb, kw, ks);
+
+    // The query's channels of this lane's eight nibbles: of group 0 (HD 32), or nibbles 0-3 of one
+    // group and 4-7 of the next.
+    auto channel = [&](int n) {
+        if constexpr (G == 1) return 8 * word + n;
+        if constexpr (G == 2) return 32 * (n >> 2) + 4 * word + (n & 3);
+        return 32 * (2 * (word & 1) + (n >> 2)) + 4 * (word >> 1) + (n & 3);
+    };
+    float qv[8], qsum[2] = {0.0f, 0.0f}, largest = 0.0f;
+    const T* const src = q + seq * q_stride + head * HD;
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+        qv[n] = to_f(src[channel(n)]);
+        largest = fmaxf(largest, fabsf(qv[n]));
+    }
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(kFull, largest, o));
+    // |q| < 1 then (2 at the upper end); products come out 2^-49 too small.
+    const int e = max(min(static_cast<int>(__float_as_uint(largest) >> 23) - 126, 126), -100);
+    const float to_one = __uint_as_float((127 - e) << 23);
+    const float to_score = a.scale * kLog2e * __uint_as_float((127 + e) << 23);
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+        qv[n] *= to_one;
+        qsum[kSums == 1 ? 0 : n >> 2] += qv[n];
+        qv[n] *= __uint_as_float((127u + 100u - 4u * (n & 3)) << 23);
+    }
+#pragma unroll
+    for (int g = 0; g < kSums; ++g) {
+#pragma unroll
+        for (int o = kLanes / 2; o >= kNext; o >>= 1) qsum[g] += __shfl_xor_sync(kFull, qsum[g], o);
+        qsum[g] *= 0x1p-49f;
+    }
+
+    float acc[8] = {}, lows[kSums] = {}, top = -INFINITY, total = 0.0f;
+    float shrink = 0x1p127f;  // 2^110 over the power of two above the largest step so far, from 2^-17 on
+    auto nibble = [](uint32_t w, int n) {  // of a word's half: c 2^(4 n - 149)
+        return __uint_as_float(w & (15u << (4 * n)));
+    };
+    for (; x < x1; x += kOneWarps * kKeys) {
+        uint32_t vw[kPasses] = {}, vs[kMine][kSums] = {};
+        load(x, vb, vsb, vw, vs);
+        float s[kSums][kPasses];
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+            float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                sum[0] = fmaf(nibble(kw[i], n), qv[n], sum[0]);
+                sum[1] = fmaf(nibble(kw[i] >> 16, n), qv[4 + n], sum[1]);
+            }
+            if constexpr (kSums == 1) {
+                s[0][i] = sum[0] + sum[1];
+            } else {
+                s[0][i] = sum[0];
+                s[1][i] = sum[1];
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < kSums; ++g) {
+#pragma unroll
+            for (int n = kPasses, o = kLanes / 2; o >= kNext; o >>= 1) {
+                n /= 2;
+                const bool upper = lane & o;
+#pragma unroll
+                for (int i = 0; i < n; ++i) {
+                    const float away = upper ? s[g][i] : s[g][i + n];
+                    s[g][i] = (upper ? s[g][i + n] : s[g][i]) + __shfl_xor_sync(kFull, away, o);
+                }
+            }
+        }
+        float score[kMine], most = -INFINITY;
+#pragma unroll
+        for (int m = 0; m < kMine; ++m) {
+            score[m] = 0.0f;
+#pragma unroll
+            for (int g = 0; g < kSums; ++g) {
+                score[m] += fmaf(low_of(ks[m][g]), s[g][m], high_of(ks[m][g]) * qsum[g]);
+            }
+            if constexpr (G == 4) score[m] += __shfl_xor_sync(kFull, score[m], 1);
+            score[m] = score[m] * 0x1p49f * to_score;
+            if (x + (my_pass + m) * kAtOnce + sub >= x1) score[m] = -INFINITY;
+            most = fmaxf(most, score[m]);
+        }
+        load(x + kOneWarps * kKeys, kb, ksb, kw, ks);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(kFull, most, o));
+        if (most > top) {
+            const float keep = top == -INFINITY ? 0.0f : exp2_fast(top - most);
+            top = most;
+            total *= keep;
+#pragma unroll
+            for (int g = 0; g < kSums; ++g) lows[g] *= keep;
+#pragma unroll
+            for (int n = 0; n < 8; ++n) acc[n] *= keep;
+        }
+        const float base = top == -INFINITY ? 0.0f : top;
+        float step = 0.0f;
+#pragma unroll
+        for (int m = 0; m < kMine; ++m) {
+#pragma unroll
+            for (int g = 0; g < kSums; ++g) step = fmaxf(step, low_of(vs[m][g]));
+        }
+        if (__any_sync(kFull, step * shrink > 0x1p110f)) {
+            step = warp_max(step);
+            const uint32_t above = (__float_as_uint(step) & 0x7f800000u) + 0x00800000u;
+            const float next = __uint_as_float(((127u + 110u + 127u) << 23) - above);  // 2^110 / above
+            const float by = next / shrink;
+            shrink = next;
+#pragma unroll
+            for (int n = 0; n < 8; ++n) acc[n] *= by;
+        }
+        float weight[kMine][kSums];  // x step
+#pragma unroll
+        for (int m = 0; m < kMine; ++m) {
+            const float p = exp2_fast(score[m] - base);
+            total += p;
+#pragma unroll
+            for (int g = 0; g < kSums; ++g) {
+                weight[m][g] = p * shrink * low_of(vs[m][g]);
+                lows[g] = fmaf(p, high_of(vs[m][g]), lows[g]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+            const int owner = sub * kLanes + i * kLanes / 8 + (G == 4 ? word & 1 : 0);
+            float w[2];
+            w[0] = w[1] = __shfl_sync(kFull, weight[i % kMine][0], owner);
+            if constexpr (kSums == 2) w[1] = __shfl_sync(kFull, weight[0][kSums - 1], owner);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                acc[n] = fmaf(nibble(vw[i], n), w[0], acc[n]);
+                acc[4 + n] = fmaf(nibble(vw[i] >> 16, n), w[1], acc[4 + n]);
+            }
+        }
+    }
+
+    // The lanes' sums, then the warps'. With four groups two lanes count every weight.
+    total = warp_sum(total) * (G == 4 ? 0.5f : 1.0f);
+#pragma unroll
+    for (int g = 0; g < kSums; ++g) {
+#pragma unroll
+        for (int o = 16; o >= kNext; o >>= 1) lows[g] += __shfl_xor_sync(kFull, lows[g], o);
+    }
+    const float by = 1.0f / shrink;
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+#pragma unroll
+        for (int o = kLanes; o < 32; o <<= 1) acc[n] += __shfl_xor_sync(kFull, acc[n], o);
+    }
+    if (lane < kLanes) {
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            // acc has 2^(4 i - 149) and the normalisation in it.
+            merge[warp][channel(n)] =
+                acc[n] * 0x1p90f * by * __uint_as_float((127u + 59u - 4u * (n & 3)) << 23) +
+                lows[kSums == 1 ? 0 : n >> 2];
+        }
+    }
+    if (lane == 0) {
+        merge[warp][HD] = top;
+        merge[warp][HD + 1] = total;
+    }
+    __syncthreads();
+    for (int ch = threadIdx.x; ch < HD; ch += kOneWarps * 32) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kOneWarps; ++w) m = fmaxf(m, merge[w][HD]);
+        float sum = 0.0f, value = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kOneWarps; ++w) {
+            const float f = merge[w][HD] == -INFINITY ? 0.0f : exp2_fast(merge[w][HD] - m);
+            // A warp that saw no key has nothing to add, and one whose scores are all NaN has that.
+            if (merge[w][HD] != -INFINITY || merge[w][HD + 1] != 0.0f) {
+                sum = fmaf(merge[w][HD + 1], f, sum);
+                value = fmaf(merge[w][ch], f, value);
+            }
+        }
+        if (splits == 1) {
+            put(out + seq * out_stride + head * HD + ch, sum == 0.0f ? 0.0f : value / sum);
+        } else {
+            float* to = part + ((static_cast<int64_t>(seq) * a.heads + head) * splits + split) * (HD + 2);
+            to[ch] = value;
+            if (ch == 0) {
+                to[HD] = m;
+                to[HD + 1] = sum;
+            }
+        }
+    }
+}
+
 // Joins the splits of a query, one CTA each: the splits' factors first, then every warp sums its
 // share of the splits with all loads independent of one another.
 constexpr int kMaxSplits = 512;
@@ -991,7 +1267,12 @@ cudaError_t launch_attention_cached(cudaStream_t s, const Cache& c, const Batch&
                     return cudaGetLastError();
                 };
                 cudaError_t e;
-                if constexpr (sizeof(T) == 2) {
+                if (STORAGE == BST_DTYPE_U4 && a.heads == a.kv_heads && !b.starts) {
+                    k_cached_one<T, HD><<<dim3(b.count, a.heads, splits), kOneWarps * 32, 0, s>>>(
+                        c, b, a, static_cast<const T*>(q), q_stride, static_cast<T*>(out), out_stride,
+                        splits, static_cast<float*>(workspace));
+                    e = cudaGetLastError();
+                } else if constexpr (sizeof(T) == 2) {
                     e = rows == 16 ? run(std::integral_constant<int, 16>())
                                    : run(std::integral_constant<int, 8>());
                 } else {
