@@ -881,10 +881,19 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
 // keys' behind them.
 // A query sees all keys of two ranges, sinks and window, so nothing inside them is masked; lanes behind
 // the end take the last key with a weight of zero.
-constexpr int kOneWarps = 2;
+// Bound by instruction issue: 256 sequences of 257 to 512 keys of eight heads of 64 take 31 us where the
+// kernel above took 45 (64 MB, 2.1 TB/s); 64 sequences of 4000 keys of 16 heads 110 (153); 60 000 keys of
+// 32 heads 51 (82). bf16, which is cheaper above, gains as well: 31 (45), 110 (134), 51 (72). Scaling in
+// the lanes that hold the words, every scale loaded by eight of them, took 36 us for the first.
+constexpr int kOneWarps = 2, kOneCtas = 20 / kOneWarps;  // warps a CTA, CTAs an SM
+
+// Whether a call is for this kernel.
+bool one_query(const Cache& c, const Batch& b, const AttnSpec& a) {
+    return c.storage == BST_DTYPE_U4 && a.heads == a.kv_heads && !b.starts;
+}
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(kOneWarps * 32, 20 / kOneWarps)
+__global__ void __launch_bounds__(kOneWarps * 32, kOneCtas)
 k_cached_one(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride,
              T* __restrict__ out, int64_t out_stride, int splits, float* __restrict__ part) {
     constexpr int G = HD / 32;
@@ -1214,7 +1223,8 @@ int rows_of_tile(const Batch& b, const AttnSpec& a) {
 }
 
 // CTAs that an SM holds, by registers and shared memory.
-int ctas_per_sm(const Cache& c) {
+int ctas_per_sm(const Cache& c, const Batch& b, const AttnSpec& a) {
+    if (one_query(c, b, a)) return kOneCtas;
     const int size = c.head_dim == 128 ? 0 : (c.head_dim == 64 ? 1 : 2);
     return c.storage == BST_DTYPE_F32 ? 1 << size : (size == 0 ? 2 : (size == 1 ? 4 : 5));
 }
@@ -1228,7 +1238,7 @@ int split_count(const Cache& c, const Batch& b, const AttnSpec& a) {
     int64_t keys = c.slots;
     if (a.window) keys = std::min<int64_t>(keys, static_cast<int64_t>(a.window) + a.sinks + 2 * kBlock);
     const int64_t units = static_cast<int64_t>(tile_bound(b, a, rows_of_tile(b, a))) * a.kv_heads;
-    const int64_t fill = 148 * ctas_per_sm(c) / std::max<int64_t>(units, 1);
+    const int64_t fill = 148 * ctas_per_sm(c, b, a) / std::max<int64_t>(units, 1);
     const int64_t even = b.count > 1 ? (keys + 4095) / 4096 : 1;
     const int64_t most = std::max<int64_t>(1, keys / 128);
     return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({std::max(fill, even), most, kMaxSplits})));
@@ -1267,7 +1277,7 @@ cudaError_t launch_attention_cached(cudaStream_t s, const Cache& c, const Batch&
                     return cudaGetLastError();
                 };
                 cudaError_t e;
-                if (STORAGE == BST_DTYPE_U4 && a.heads == a.kv_heads && !b.starts) {
+                if (STORAGE == BST_DTYPE_U4 && one_query(c, b, a)) {
                     k_cached_one<T, HD><<<dim3(b.count, a.heads, splits), kOneWarps * 32, 0, s>>>(
                         c, b, a, static_cast<const T*>(q), q_stride, static_cast<T*>(out), out_stride,
                         splits, static_cast<float*>(workspace));
