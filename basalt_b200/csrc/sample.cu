@@ -41,6 +41,7 @@ namespace cg = cooperative_groups;
 constexpr int kMaxThreads = 512;
 constexpr int kBins = 2048;
 constexpr int kCoarse = 64;                  // bins / kCoarse = 32 bins, a lane each
+constexpr int kCountBins = 256;              // for counts of a list's candidates
 constexpr int kMaxCluster = 8;
 constexpr double kUnit = 4398046511104.0;    // 2^42 units in the largest weight
 constexpr double kCut = -27.725887222397812; // ln 2^-40
@@ -124,6 +125,14 @@ struct Row {
     int begin, count;
     int turn = 0;
 
+    __device__ void sync() {
+        if (ranks == 1) {
+            __syncthreads();
+        } else {
+            cluster.sync();
+        }
+    }
+
     // Sum (or maximum) over all threads of the cluster of two values at once; the CTAs' own
     // results in rank order are in each CTA's exchange slot until the next but one call.
     template <bool MAX>
@@ -145,7 +154,7 @@ struct Row {
                 sh.exchange[turn][1] = y;
             }
         }
-        cluster.sync();
+        sync();
         a = b = 0;
         for (int r = 0; r < ranks; ++r) {
             const u64* e = cluster.map_shared_rank(&sh.exchange[turn][0], r);
@@ -161,9 +170,9 @@ struct Row {
 
 // Where a running sum from the largest logit down reaches a target.
 struct Threshold {
-    uint32_t key;  // the smallest key kept; 0: everything
-    u64 above;     // the sum over larger keys
-    u64 total;     // the sum over this key's tokens, where it is known
+    uint32_t key;   // the smallest key kept; 0: everything
+    u64 above;      // the sum over larger keys
+    u64 target;
 };
 
 // Clears the histogram.
@@ -183,7 +192,7 @@ __device__ void find_bin(Row<T>& row, u64 above, u64 target) {
         const u64 v = warp_sum_u(bin(&sh, i * 32 + (threadIdx.x & 31)));
         if ((threadIdx.x & 31) == 0) sh.coarse[i] = v;
     }
-    row.cluster.sync();
+    row.sync();
     if (threadIdx.x < 32) {
         const int lane = threadIdx.x;
         u64 c0 = 0, c1 = 0;
@@ -226,7 +235,7 @@ __device__ void find_bin(Row<T>& row, u64 above, u64 target) {
             sh.result[2] = fine;
         }
     }
-    row.cluster.sync();  // every CTA has read the others' bins
+    row.sync();  // every CTA has read the others' bins
 }
 
 // Bins by the distance from the largest logit, over [least, top].
@@ -245,17 +254,18 @@ struct Distance {
     __device__ int bin(uint32_t key) const { return bin(float_of(key)); }
 };
 
-// The key at which the sum of weight(key), over the tokens with key >= least, reaches target (which
-// must be between 1 and their whole sum). extra is a sum that belongs to the key extra_key (tokens
-// that weight() leaves out there).
-template <typename T, typename W>
+// The key at which the sum of weight(key), over the tokens with key >= least, reaches target, which
+// must be at least 1; with SHARE it is target_of(whole sum), where 1 or less ends the search at the
+// largest key. extra is a sum that belongs to the key extra_key (tokens that weight() leaves out there).
+template <bool SHARE, typename T, typename W, typename U>
 __device__ Threshold find_threshold(Row<T>& row, uint32_t top, uint32_t least, u64 target,
-                                    uint32_t extra_key, u64 extra, W&& weight) {
+                                    uint32_t extra_key, u64 extra, W&& weight, U&& target_of) {
     Shared& sh = row.sh;
     const Distance distance(top, least);
     bool by_distance = distance.usable;
     uint32_t lo = least, hi = top;
     u64 above = 0;
+    bool first = SHARE;
     while (true) {
         int shift = 0;
         while (((hi - lo) >> shift) >= kBins) ++shift;
@@ -264,21 +274,29 @@ __device__ Threshold find_threshold(Row<T>& row, uint32_t top, uint32_t least, u
             return by_distance ? distance.bin(key) : static_cast<int>((hi - key) >> shift);
         };
         clear_bins(sh);
+        u64 sum = 0;
         for (int i = threadIdx.x; i < row.count; i += threads()) {
             const uint32_t key = key_of(row.at(i));
             if (key < lo || key > hi) continue;
             const u64 w = weight(key);
+            sum += w;
             if (w) add_to(sh, bin_of(key), w);
         }
         if (extra && row.rank == 0 && threadIdx.x == 0 && extra_key >= lo && extra_key <= hi) {
             add_to(sh, bin_of(extra_key), extra);
         }
+        if (first) {
+            u64 unused = 0;
+            row.template reduce<false>(sum, unused);
+            target = target_of(sum + extra);
+            if (target <= 1) return Threshold{top, 0, target};
+            first = false;
+        }
         find_bin(row, above, target);
         const int bin = static_cast<int>(sh.result[0]);
         above = sh.result[1];
-        const u64 total = sh.result[2];
         if (!by_distance && shift == 0) {
-            return Threshold{hi - static_cast<uint32_t>(bin), above, total};
+            return Threshold{hi - static_cast<uint32_t>(bin), above, target};
         }
         if (!by_distance) {
             const uint32_t new_hi = hi - (static_cast<uint32_t>(bin) << shift);
@@ -290,7 +308,7 @@ __device__ Threshold find_threshold(Row<T>& row, uint32_t top, uint32_t least, u
         // The bin's tokens, collected by CTA 0 (their keys; weights follow from those).
         __syncthreads();
         if (threadIdx.x == 0) sh.listed = 0;
-        row.cluster.sync();
+        row.sync();
         Shared* const home = row.cluster.map_shared_rank(&sh, 0);
         u64 high = 0, low = 0;  // the keys' range; low as its complement, so that both are maxima
         for (int i = threadIdx.x; i < row.count; i += threads()) {
@@ -307,7 +325,7 @@ __device__ Threshold find_threshold(Row<T>& row, uint32_t top, uint32_t least, u
         lo = ~static_cast<uint32_t>(low);
         by_distance = false;
         if (n > kList) {
-            row.cluster.sync();  // the list's place is cleared next
+            row.sync();  // the list's place is cleared next
             continue;
         }
         if (row.rank == 0) {
@@ -352,11 +370,11 @@ __device__ Threshold find_threshold(Row<T>& row, uint32_t top, uint32_t least, u
                 }
             }
         }
-        row.cluster.sync();
+        row.sync();
         const uint32_t edge = static_cast<uint32_t>(home->result[0]);
         const u64 larger = home->result[1];
-        row.cluster.sync();  // read by all before it is written again
-        return Threshold{edge, larger, 0};
+        row.sync();  // read by all before it is written again
+        return Threshold{edge, larger, target};
     }
 }
 
@@ -449,6 +467,79 @@ __device__ void finish_list(Shared& sh, int n, int top_k, float top_p, bool floo
     }
 }
 
+// The same from a list of at most kRanked: every token finds its rank by comparing, and its running
+// sum, in the order of the indices, by adding (tens of cycles a token where the steps of a sort and of
+// two walks wait for one another).
+constexpr int kRanked = 512;
+template <typename W, typename F, typename U>
+__device__ void finish_short_list(Shared& sh, int n, int top_k, float top_p, bool floored, W&& weight,
+                                  F&& above_floor, U&& target_of, int* token) {
+    const u64* const list = list_of(&sh);
+    u64* const sorted = list_of(&sh) + kRanked;
+    u64* const weights = sorted + kRanked;
+    for (int i = threadIdx.x; i < n; i += threads()) {
+        const u64 mine = list[i];
+        int rank = 0;
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) rank += list[j] > mine;
+        sorted[rank] = mine;
+        weights[rank] = weight(static_cast<uint32_t>(mine >> 32));
+    }
+    int m = min(n, top_k);
+    __syncthreads();
+    const int lane = threadIdx.x & 31;
+    // A lane's share of the first m, and the sum up to its end.
+    auto scan = [&](int each) {
+        u64 sum = 0;
+        for (int i = lane * each; i < min(m, lane * each + each); ++i) sum += weights[i];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const u64 v = __shfl_up_sync(kFull, sum, o);
+            if (lane >= o) sum += v;
+        }
+        return sum;
+    };
+    if (top_p < 1.0f) {
+        if (threadIdx.x < 32) {
+            const int each = (m + 31) / 32;
+            const u64 upto = scan(each), sum = __shfl_sync(kFull, upto, 31);
+            const double want = static_cast<double>(top_p) * static_cast<double>(sum);
+            const u64 target = want > 0.0 ? min(sum, static_cast<u64>(ceil(want))) : 0;
+            // The first token at which the running sum reaches the target.
+            const int who = __ffs(__ballot_sync(kFull, upto >= target)) - 1;
+            if (lane == who) {
+                int i = min(m, lane * each + each) - 1;
+                for (u64 run = upto - weights[i]; i > lane * each && run >= target; run -= weights[i]) --i;
+                sh.result[0] = target <= 1 ? 1 : i + 1;
+            }
+        }
+        __syncthreads();
+        m = static_cast<int>(sh.result[0]);
+    }
+    if (floored) {
+        int kept = 0;
+        for (int i0 = 0; i0 < m; i0 += threads()) {
+            const int i = i0 + static_cast<int>(threadIdx.x);
+            kept += __syncthreads_count(i < m && above_floor(static_cast<uint32_t>(sorted[i] >> 32)));
+        }
+        m = kept;
+    }
+    if (threadIdx.x < 32) {
+        const u64 whole = scan((m + 31) / 32);
+        if (lane == 31) sh.result[1] = target_of(whole);
+    }
+    __syncthreads();
+    const u64 target = sh.result[1];
+    for (int i = threadIdx.x; i < m; i += threads()) {
+        // The low words are the indices' complements.
+        const uint32_t mine = static_cast<uint32_t>(sorted[i]);
+        u64 before = 0;
+#pragma unroll 4
+        for (int j = 0; j < m; ++j) before += static_cast<uint32_t>(sorted[j]) > mine ? weights[j] : 0;
+        if (before <= target && target < before + weights[i]) *token = static_cast<int>(~mine);
+    }
+}
+
 struct Args {
     const void* logits;
     int V, per;            // per: a CTA's slice
@@ -511,7 +602,7 @@ __global__ void __launch_bounds__(kMaxThreads) k_sample_tokens(Args a) {
         if (rank == 0 && threadIdx.x == 0) {
             a.tokens[r] = largest == -INFINITY ? -1 : a.V - static_cast<int>(rest);
         }
-        cluster.sync();  // the exchange slots are read by others until here
+        row.sync();  // the exchange slots are read by others until here
         return;
     }
 
@@ -566,49 +657,87 @@ __global__ void __launch_bounds__(kMaxThreads) k_sample_tokens(Args a) {
         return min(static_cast<u64>(u * static_cast<double>(whole)), whole - 1);
     };
 
-    // A top_k whose candidates fit a list: collected, sorted and finished by CTA 0.
+    // A top_k whose candidates fit a list: collected and finished by CTA 0. The k-th largest of the
+    // threads' own largest logits bounds the k-th largest of all from below, closely as long as k is
+    // well below the threads' number, so those alone are counted in bins; with fewer threads than k
+    // all logits are.
     const Distance distance(top, least);
     if (top_k > 0 && top_k <= kList / 2 && distance.usable) {
-        clear_bins(sh);
         const float least_f = float_of(least);
-        u64 n = 0;
-        for (int i = threadIdx.x; i < row.count; i += threads()) {
-            const float x = row.at(i);
-            if (x >= least_f) {
-                ++n;
-                atomicAdd(&sh.low[distance.bin(x)], 1u);
-            }
-        }
-        unused = 0;
-        row.template reduce<false>(n, unused);
-        int last = kBins - 1;
-        u64 candidates = n;
-        if (n > static_cast<u64>(top_k)) {
-            find_bin(row, 0, static_cast<u64>(top_k));
-            last = static_cast<int>(sh.result[0]);
-            candidates = sh.result[1] + sh.result[2];
-            __syncthreads();
-        }
-        if (candidates <= kList) {
-            if (threadIdx.x == 0) sh.listed = 0;
-            cluster.sync();
-            Shared* const home = cluster.map_shared_rank(&sh, 0);
+        for (int i = threadIdx.x; i < kCountBins; i += threads()) sh.low[i] = 0u;
+        if (threadIdx.x == 0) sh.listed = 0;
+        __syncthreads();
+        auto count_bin = [&](float x) { return distance.bin(x) / (kBins / kCountBins); };
+        if (top_k <= ranks * threads()) {
+            if (most >= least_f) atomicAdd(&sh.low[count_bin(most)], 1u);
+        } else {
             for (int i = threadIdx.x; i < row.count; i += threads()) {
                 const float x = row.at(i);
-                if (x >= least_f && distance.bin(x) <= last) {
-                    const unsigned at = atomicAdd(&home->listed, 1u);
+                if (x >= least_f) atomicAdd(&sh.low[count_bin(x)], 1u);
+            }
+        }
+        row.sync();
+        if (threadIdx.x < 32) {
+            // A lane sums eight bins; the first bin at which the running sum reaches top_k.
+            constexpr int kEach = kCountBins / 32;
+            static_assert(kEach == 8, "two 16-byte loads a lane");
+            uint32_t bins[kEach] = {};
+            for (int q = 0; q < ranks; ++q) {
+                const uint4* from = reinterpret_cast<const uint4*>(cluster.map_shared_rank(sh.low, q)) +
+                                    2 * threadIdx.x;
+                const uint4 x = from[0], y = from[1];
+                bins[0] += x.x; bins[1] += x.y; bins[2] += x.z; bins[3] += x.w;
+                bins[4] += y.x; bins[5] += y.y; bins[6] += y.z; bins[7] += y.w;
+            }
+            uint32_t upto = 0;
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) upto += bins[i];
+            const uint32_t own = upto;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t v = __shfl_up_sync(kFull, upto, o);
+                if (static_cast<int>(threadIdx.x) >= o) upto += v;
+            }
+            const unsigned hit = __ballot_sync(kFull, upto >= static_cast<uint32_t>(top_k));
+            const int who = hit ? __ffs(hit) - 1 : 31;
+            if (static_cast<int>(threadIdx.x) == who) {
+                int last = 0;  // bins of these before which the sum stays below top_k
+                uint32_t run = upto - own;
+#pragma unroll
+                for (int i = 0; i < kEach - 1; ++i) {
+                    run += bins[i];
+                    if (run < static_cast<uint32_t>(top_k)) last = i + 1;
+                }
+                sh.result[0] = who * kEach + last;
+            }
+        }
+        row.sync();  // every CTA has read the others' bins, whose place the list takes
+        const int last = static_cast<int>(sh.result[0]);
+        Shared* const home = cluster.map_shared_rank(&sh, 0);
+        for (int i = threadIdx.x; i < row.count; i += threads()) {
+            const float x = row.at(i);
+            if (x >= least_f && count_bin(x) <= last) {
+                const unsigned at = atomicAdd(&home->listed, 1u);
+                if (at < kList) {
                     list_of(home)[at] = (static_cast<u64>(key_of(x)) << 32) |
                                         static_cast<uint32_t>(~(begin + i));
                 }
             }
-            cluster.sync();  // the last access to other CTAs' memory
-            if (rank == 0) {
-                finish_list(sh, static_cast<int>(candidates), top_k, top_p, floored, weight,
-                            above_floor, target_of, a.tokens + r);
+        }
+        row.sync();
+        const unsigned listed = home->listed;
+        row.sync();  // the last access to other CTAs' memory, where the list is finished
+        if (listed <= kList) {
+            if (rank != 0) return;
+            if (listed <= kRanked) {
+                finish_short_list(sh, static_cast<int>(listed), top_k, top_p, floored, weight,
+                                  above_floor, target_of, a.tokens + r);
+            } else {
+                finish_list(sh, static_cast<int>(listed), top_k, top_p, floored, weight, above_floor,
+                            target_of, a.tokens + r);
             }
             return;
         }
-        cluster.sync();
     }
 
     // Kept: keys above `edge` and the first `ties` tokens, by index, with exactly that key.
@@ -620,36 +749,30 @@ __global__ void __launch_bounds__(kMaxThreads) k_sample_tokens(Args a) {
         unused = 0;
         row.template reduce<false>(n, unused);
         if (n > static_cast<u64>(top_k)) {
-            const Threshold t = find_threshold(row, top, least, static_cast<u64>(top_k), 0u, 0ull,
-                                               [](uint32_t) -> u64 { return 1; });
+            const Threshold t = find_threshold<false>(row, top, least, static_cast<u64>(top_k), 0u, 0ull,
+                                                      [](uint32_t) -> u64 { return 1; },
+                                                      [](u64) -> u64 { return 0; });
             edge = t.key;
             ties = static_cast<u64>(top_k) - t.above;
         }
     }
     if (top_p < 1.0f) {
-        u64 sum = 0;
-        unused = 0;
         const uint32_t from = max(least, edge + (edge ? 1u : 0u));
-        for (int i = threadIdx.x; i < row.count; i += threads()) {
-            const uint32_t key = key_of(row.at(i));
-            if (key >= from) sum += weight(key);
-        }
-        row.template reduce<false>(sum, unused);
         const u64 tied = edge ? ties * weight(edge) : 0;
-        sum += tied;
-        const double want = static_cast<double>(top_p) * static_cast<double>(sum);
-        // The fewest tokens whose sum is at least want: the sum has to reach ceil(want), at least 1.
-        const u64 target = want > 0.0 ? min(sum, static_cast<u64>(ceil(want))) : 0;
-        if (target <= 1) {
+        const Threshold t = find_threshold<true>(
+            row, top, edge ? edge : least, 0, edge, tied,
+            [&](uint32_t key) -> u64 { return key >= from ? weight(key) : 0; },
+            [&](u64 sum) -> u64 {
+                // The fewest tokens whose sum is at least want: the sum has to reach ceil(want).
+                const double want = static_cast<double>(top_p) * static_cast<double>(sum);
+                return want > 0.0 ? min(sum, static_cast<u64>(ceil(want))) : 0;
+            });
+        if (t.target <= 1) {
             edge = top;
             ties = 1;
         } else {
-            const Threshold t = find_threshold(row, top, edge ? edge : least, target, edge, tied,
-                                               [&](uint32_t key) -> u64 {
-                                                   return key >= from ? weight(key) : 0;
-                                               });
             const u64 w = weight(t.key);
-            u64 need = (target - t.above + w - 1) / w;
+            u64 need = (t.target - t.above + w - 1) / w;
             if (t.key == edge) need = min(need, ties);
             edge = t.key;
             ties = need;
@@ -727,7 +850,7 @@ __global__ void __launch_bounds__(kMaxThreads) k_sample_tokens(Args a) {
             before_ties += n;
         }
     }
-    cluster.sync();  // the last access to other CTAs' memory
+    row.sync();  // the last access to other CTAs' memory
     if (!mine) return;
     // Twice: the sums of the warps' parts pick one, and its elements become the next parts.
     int from = 0, to = row.count;

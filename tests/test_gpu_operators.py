@@ -415,6 +415,22 @@ def test_draws_with_ties(ops):
     check_draws(ops, flat * 0, rng.random(16), top_k=7)
 
 
+@pytest.mark.parametrize("V", [3000, 8191, 20000, 131072])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_draws_from_many_candidates(ops, V, dtype):
+    """top_k around what the lists and the CTAs' threads hold, and ties that overflow them."""
+    rng = np.random.default_rng(V + 1)
+    rows = 10
+    top_k = [255, 257, 400, 512, 513, 700, 1000, 1024, 1025, 2500]
+    x = rng.standard_normal((rows, V)) * 2
+    check_draws(ops, x, rng.random(rows), dtype, top_k=top_k)
+    check_draws(ops, x, rng.random(rows), dtype, top_k=top_k, top_p=0.9, min_p=0.003)
+    check_draws(ops, np.sort(x, 1)[:, ::-1], rng.random(rows), dtype, top_k=top_k, top_p=0.99)
+    few = np.round(x)                                          # thousands of tokens a value
+    check_draws(ops, few, rng.random(rows), dtype, top_k=top_k, top_p=0.97)
+    check_draws(ops, few, rng.random(rows), dtype, top_k=20, top_p=0.5, min_p=0.2)
+
+
 def test_draws_at_the_edges(ops):
     inf, nan = np.inf, np.nan
     x = np.full((8, 70), -inf)
