@@ -644,15 +644,17 @@ k_packed_mma(Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride, con
     };
     fetch(0);
     const float to_log2 = a.scale * kLog2e;
-    for (int x = threadIdx.x; x < L::kRows * HD; x += L::kThreads) {
-        const int r = x / HD, c = x % HD, row = tile.r0 + r;
-        float value = 0.0f;
-        if (r < rows) {
-            const int token = row / group;
-            value = to_f(q[(tile.first + static_cast<int64_t>(token)) * q_stride +
-                           (kvh * group + row - token * group) * HD + c]);
+    // Queries, a warp a row, many loads at once (rows behind the last are copies that become zeros).
+#pragma unroll 8
+    for (int r = warp; r < L::kRows; r += L::kThreads / 32) {
+        const int row = tile.r0 + min(r, rows - 1), token = row / group;
+        const T* const from = q + (tile.first + static_cast<int64_t>(token)) * q_stride +
+                              (kvh * group + row - token * group) * HD + lane;
+#pragma unroll
+        for (int c = 0; c < HD / 32; ++c) {
+            const float value = to_f(from[32 * c]);
+            queries[r * L::kQPitch + 32 * c + lane] = r < rows ? value : 0.0f;
         }
-        queries[r * L::kQPitch + c] = value;
     }
     int position[2], low[2];
 #pragma unroll
