@@ -175,10 +175,12 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
     constexpr int kBlocks = HD / 64;     // 128-byte columns of a tile
     extern __shared__ unsigned char raw[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int group = a.heads / a.kv_heads, kvh = blockIdx.y;
-    // The last tiles first: without a window they see the most keys.
-    const int index = gridDim.x - 1 - blockIdx.x;
-    int* const flag = flags + kvh * gridDim.x + index;
+    const int group = a.heads / a.kv_heads, tiles = gridDim.x / a.kv_heads;
+    // The last tiles of all heads first: a sequence's first ones see the fewest keys and fill the end
+    // (4096 tokens of eight heads, no window: 534 -> 474 us in float32, 279 -> 274 for 8192 in bf16).
+    const int place_of = blockIdx.x / a.kv_heads, kvh = blockIdx.x - place_of * a.kv_heads;
+    const int index = tiles - 1 - place_of;
+    int* const flag = flags + kvh * tiles + index;
     Tile tile;
     if (!find_tile(b, group, kTcRows, index, &tile)) {
         if (threadIdx.x == 0) *flag = 0;
@@ -590,9 +592,10 @@ k_packed_mma(Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride, con
     extern __shared__ __align__(16) float shared[];
     __shared__ int redo;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int group = a.heads / a.kv_heads, kvh = blockIdx.y;
-    const int index = gridDim.x - 1 - blockIdx.x;
-    int* const flag = flags + kvh * gridDim.x + index;
+    const int group = a.heads / a.kv_heads, tiles = gridDim.x / a.kv_heads;
+    const int place_of = blockIdx.x / a.kv_heads, kvh = blockIdx.x - place_of * a.kv_heads;
+    const int index = tiles - 1 - place_of;  // as above
+    int* const flag = flags + kvh * tiles + index;
     Tile tile;
     if (!find_tile(b, group, L::kRows, index, &tile)) {
         if (threadIdx.x == 0) *flag = 0;
@@ -898,7 +901,7 @@ cudaError_t launch_attention_packed(cudaStream_t s, const Batch& b, const AttnSp
                                                  TcLayout<HD>::kSmem);
                     }
                     if (e) return e;
-                    k_packed_tc<HD><<<dim3(tiles, a.kv_heads), kTcThreads, TcLayout<HD>::kSmem, s>>>(
+                    k_packed_tc<HD><<<tiles * a.kv_heads, kTcThreads, TcLayout<HD>::kSmem, s>>>(
                         k_map, v_map, b, a, q, q_stride, out, out_stride, flags);
                 }
             }
@@ -911,7 +914,7 @@ cudaError_t launch_attention_packed(cudaStream_t s, const Batch& b, const AttnSp
                 e = cudaFuncSetAttribute(k_packed_mma<T, HD>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
                 if (e) return e;
-                k_packed_mma<T, HD><<<dim3(tiles, a.kv_heads), L::kThreads, L::kSmem, s>>>(
+                k_packed_mma<T, HD><<<tiles * a.kv_heads, L::kThreads, L::kSmem, s>>>(
                     b, a, q, q_stride, k, k_stride, v, v_stride, out, out_stride, vector, flags);
             }
             if ((e = cudaGetLastError())) return e;
