@@ -707,16 +707,23 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
                 product<false, false>(lows, pa, __byte_perm(column[0][0], column[0][1], 0x5410),
                                       __byte_perm(column[1][0], column[1][1], 0x5410));
             }
+            // One test for all groups, so that their products below stand side by side. Steps are the low
+            // halves, and order as whole numbers do.
+            float largest[G];
+            bool above_any = false;
 #pragma unroll
             for (int gr = 0; gr < G; ++gr) {
-                const float steps[2][2] = {{low_of(sv[0][0][gr]), low_of(sv[0][1][gr])},
-                                           {low_of(sv[1][0][gr]), low_of(sv[1][1][gr])}};
-                const float largest = fmaxf(fmaxf(steps[0][0], steps[0][1]),
-                                            fmaxf(steps[1][0], steps[1][1]));
-                if (__any_sync(kFull, largest * shrink[gr] > 0x1p14f)) {
-                    // A step above the power of two: the next one, for a row's lanes (each has seen
-                    // four of the keys). A row that sees no larger step, or no key at all, stays.
-                    float most = fmaxf(largest, __shfl_xor_sync(kFull, largest, 1));
+                const uint32_t most = __vimax3_u16x2(__vmaxu2(sv[0][0][gr], sv[0][1][gr]),
+                                                     sv[1][0][gr], sv[1][1][gr]);
+                largest[gr] = low_of(most);
+                above_any |= largest[gr] * shrink[gr] > 0x1p14f;
+            }
+            if (__any_sync(kFull, above_any)) {
+                // A step above its group's power of two: the next one, for a row's lanes (each has seen
+                // four of the keys). A row that sees no larger step, or no key at all, stays.
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr) {
+                    float most = fmaxf(largest[gr], __shfl_xor_sync(kFull, largest[gr], 1));
                     most = fmaxf(most, __shfl_xor_sync(kFull, most, 2));
                     const uint32_t above = (__float_as_uint(most) & 0x7f800000u) + 0x00800000u;
                     const float next = most * shrink[gr] > 0x1p14f
@@ -730,6 +737,11 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
                         for (int e = 0; e < 4; ++e) o[4 * gr + j][e] *= by;
                     }
                 }
+            }
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr) {
+                const float steps[2][2] = {{low_of(sv[0][0][gr]), low_of(sv[0][1][gr])},
+                                           {low_of(sv[1][0][gr]), low_of(sv[1][1][gr])}};
                 uint32_t ps[R][2][kHalf], x[2];
 #pragma unroll
                 for (int nb = 0; nb < 2; ++nb) {
