@@ -1,4 +1,5 @@
-// Internal interface of the serving operators (kv_cache.cu, attention.cu, sample.cu): device views
+// Internal interface of the serving operators (kv_cache.cu, attention_cached.cu,
+// attention_packed.cu, sample.cu): device views
 // of the ABI structs and the launchers shared with the engine. Launchers queue on the given stream
 // of the current device and return the launch's error.
 #pragma once

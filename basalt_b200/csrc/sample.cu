@@ -20,7 +20,9 @@
 // A row is worked on by a cluster of CTAs, each with a slice of the row in its shared memory; sums,
 // histograms and lists meet through distributed shared memory. The row is read once; what bounds the
 // kernel are its passes over the slices in shared memory, the double operations, and for few rows the
-// latency of the steps between them.
+// latency of the steps between them: 32 rows of 4096 with top_k 40 take 10 us (16 with all logits counted
+// and the list sorted), 2048 unfiltered rows of 8192 take 61, 64 rows of 131 072 with settings of their
+// own 67, the time of those whose top_p needs the histogram of weights.
 
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -37,7 +39,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 // Threads a CTA: half as many where a CTA has a whole row, so that more rows share an SM and cover one
-// another's steps (2048 rows of 8192: 101 -> 78 us; 64 rows of 131 072 are slower so).
+// another's steps (2048 rows of 8192 at that step: 101 -> 78 us; 64 rows of 131 072 are slower so).
 constexpr int kMaxThreads = 512;
 constexpr int kBins = 2048;
 constexpr int kCoarse = 64;                  // bins / kCoarse = 32 bins, a lane each

@@ -308,8 +308,9 @@ typedef struct bst_sequences {
  * [rows][kv_heads][slots][head_dim / 32][2] bf16: (step, low) of every 32 channels. A code c stands
  * for low + c * step. low is the 32 channels' minimum rounded down to bf16, step is
  * (maximum - low) / 15 rounded up to bf16, and codes are (x - low) / step rounded to nearest even;
- * 32 channels that hold a NaN, an infinity or a value below bf16's lowest read back as NaN. The codes of a token's head are [8][head_dim / 32][4] nibbles, low nibble first: channel
- * 32 g + 4 h + j is nibble j of the 16 bits at [h][g]. */
+ * 32 channels that hold a NaN, an infinity or a value below bf16's lowest read back as NaN. The codes
+ * of a token's head are [8][head_dim / 32][4] nibbles, low nibble first: channel 32 g + 4 h + j is
+ * nibble j of the 16 bits at [h][g]. */
 typedef struct bst_kv_cache {
     int32_t storage; /* BST_DTYPE_F32, BST_DTYPE_BF16 or BST_DTYPE_U4 */
     int32_t rows, kv_heads, slots, head_dim;

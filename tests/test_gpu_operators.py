@@ -276,6 +276,56 @@ def test_later_values_of_another_size_stay_out_of_earlier_rows(ops, dtype, windo
             assert np.all(np.abs(got[t] - want[0]) <= tol[0]), (s, i)
 
 
+@pytest.mark.parametrize("heads,dim,lengths,window,sinks", [
+    (3, 64, [700, 5, 0, 130], 64, 9), (2, 128, [5000], 0, 0), (2, 128, [9000, 40], 3000, 50),
+    (5, 32, [3333, 64, 63], 1000, 7), (1, 64, [33], 31, 1), (2, 32, [20000], 0, 0)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("size", [1.0, 2.0 ** 40, 2.0 ** -60])
+def test_one_query_a_key_head_over_4_bits(ops, dtype, heads, dim, lengths, window, sinks, size):
+    """Every key head with one query, values of different sizes from block to block, and queries and
+    values far from one."""
+    rng = np.random.default_rng(dim + sum(lengths))
+    S, slots = len(lengths), max(lengths) + 5
+    k = rng.standard_normal((S * slots, heads, dim)).astype(np.float32)
+    v = rng.standard_normal((S * slots, heads, dim)).astype(np.float32)
+    v *= (2.0 ** rng.integers(-8, 9, (S * slots, 1, 1)) * size).astype(np.float32)
+    cache = ops.KvCache.allocate(S, heads, slots, dim)
+    starts, full = ints(np.arange(S + 1) * slots), ints([slots] * S)
+    ops.kv_append(cache, tensor(k), tensor(v), full, starts=starts)
+    k, v = (host(t).reshape(S, slots, heads, dim)
+            for t in ops.kv_read(cache, full, starts=starts, tokens=S * slots))
+    q = tensor((rng.standard_normal((S, heads, dim)) / size).astype(np.float32), dtype)
+    scale = size / math.sqrt(dim)
+    got = host(ops.attention_cached(cache, q, ints(lengths), window=window, sinks=sinks, scale=scale))
+    check_cached(q, got, k, v, np.arange(S), lengths, [1] * S, window, sinks, dtype, scale)
+
+
+def test_one_query_a_key_head_and_values_that_are_not_finite(ops):
+    """Unseen ones take no part; a seen one reaches the 32 channels that it shares a scale with."""
+    torch = torch_()
+    rng = np.random.default_rng(14)
+    for dim in (32, 64, 128):
+        x = rng.standard_normal((2 * 300, 2, dim)).astype(np.float32)
+        bad = x.reshape(2, 300, 2, dim).copy()
+        bad[:, 250:], bad[:, 3:150] = np.nan, -np.inf
+        starts, full, lengths = ints([0, 300, 600]), ints([300] * 2), ints([250, 249])
+        q = tensor(rng.standard_normal((2, 2, dim)).astype(np.float32))
+        outs = []
+        for values in (x, bad.reshape(x.shape)):
+            cache = ops.KvCache.allocate(2, 2, 300, dim)
+            ops.kv_append(cache, tensor(values), tensor(values), full, starts=starts)
+            outs.append(ops.attention_cached(cache, q, lengths, window=99, sinks=3))
+        assert torch.equal(outs[0], outs[1]) and torch.isfinite(outs[0]).all()
+        values = x.copy()
+        values[200, 1, 5] = np.nan
+        cache = ops.KvCache.allocate(2, 2, 300, dim)
+        ops.kv_append(cache, tensor(x), tensor(values), full, starts=starts)
+        out = ops.attention_cached(cache, q, lengths)
+        assert torch.isnan(out[0, 1, :32]).all()
+        assert torch.isfinite(out[0, 1, 32:]).all() and torch.isfinite(out[0, 0]).all()
+        assert torch.isfinite(out[1]).all()
+
+
 def test_a_long_4_bit_cache(ops):
     """Work split over the keys: one sequence of 40 000 keys, and offsets past 2^31 bytes."""
     torch = torch_()
