@@ -21,14 +21,15 @@
 // histograms and lists meet through distributed shared memory. The row is read once; what bounds the
 // kernel are its passes over the slices in shared memory, the double operations, and for few rows the
 // latency of the steps between them: 32 rows of 4096 with top_k 40 take 10 us (16 with all logits counted
-// and the list sorted), 2048 unfiltered rows of 8192 take 61, 64 rows of 131 072 with settings of their
-// own 67, the time of those whose top_p needs the histogram of weights.
+// and the list sorted), 2048 unfiltered rows of 8192 take 53, 64 rows of 131 072 with settings of their
+// own 64, the time of those whose top_p needs the histogram of weights.
 
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
 #include <algorithm>
 #include <cfloat>
+#include <cstddef>
 
 #include "device.cuh"
 #include "operators.h"
@@ -38,17 +39,17 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-// Threads a CTA: half as many where a CTA has a whole row, so that more rows share an SM and cover one
-// another's steps (2048 rows of 8192 at that step: 101 -> 78 us; 64 rows of 131 072 are slower so).
-constexpr int kMaxThreads = 512;
+// Threads a CTA: few, so that more CTAs share an SM and cover one another's steps (512 took 101 us
+// instead of 78 for 2048 rows of 8192 at that step, and the same for 64 rows of 131 072).
+constexpr int kThreads = 256;
 constexpr int kBins = 2048;
 constexpr int kCoarse = 64;                  // bins / kCoarse = 32 bins, a lane each
 constexpr int kCountBins = 256;              // for counts of a list's candidates
 constexpr int kMaxCluster = 8;
-constexpr double kUnit = 4398046511104.0;    // 2^42 units in the largest weight
 constexpr double kCut = -27.725887222397812; // ln 2^-40
 using u64 = unsigned long long;
 
+// Not the constant, with which loops are unrolled into spills (53 -> 57 us for 2048 rows of 8192).
 __device__ __forceinline__ int threads() { return static_cast<int>(blockDim.x); }
 __device__ __forceinline__ int warps() { return static_cast<int>(blockDim.x >> 5); }
 
@@ -66,15 +67,17 @@ __device__ __forceinline__ float float_of(uint32_t key) {
 constexpr int kList = 2048;   // tokens that a list holds
 
 struct Shared {
-    uint32_t low[kBins], high[kBins];  // a histogram's 64-bit sums; both halves are a list otherwise
     u64 coarse[kCoarse];
     double powers[32];                 // 2^(k / 32)
     unsigned listed;                   // tokens that asked for a place in the list
     u64 exchange[2][2];     // this CTA's value of a reduction over the cluster, two pairs in turn
-    u64 warp_a[kMaxThreads / 32], warp_b[kMaxThreads / 32];
+    u64 warp_a[kThreads / 32], warp_b[kThreads / 32];
     u64 result[4];
-    u64 padding;  // the slice behind it is 16-byte aligned
+    // Rows without filters end here.
+    alignas(16) uint32_t low[kBins];  // a histogram's 64-bit sums; both halves are a list otherwise
+    uint32_t high[kBins];
 };
+static_assert(sizeof(Shared) % 16 == 0 && offsetof(Shared, low) % 16 == 0, "slices are 16-byte aligned");
 static_assert(kList * 8 == kBins * 8, "a list lies in the histogram's place");
 
 // A histogram's 64-bit sum grows by v: two native 32-bit additions, the carry by hand.
@@ -554,11 +557,14 @@ struct Args {
     int* tokens;
 };
 
-template <typename T>
-__global__ void __launch_bounds__(kMaxThreads) k_sample_tokens(Args a) {
+// FILTERS false: no row has any, which leaves the histogram's memory to more CTAs an SM and half of the
+// code out (2048 rows of 8192: 61.6 -> 53.3 us).
+template <typename T, bool FILTERS>
+__global__ void __launch_bounds__(kThreads, FILTERS ? 3 : 6)
+k_sample_tokens(Args a) {
     extern __shared__ __align__(16) unsigned char smem[];
     Shared& sh = *reinterpret_cast<Shared*>(smem);
-    T* staged = reinterpret_cast<T*>(smem + sizeof(Shared));
+    T* staged = reinterpret_cast<T*>(smem + (FILTERS ? sizeof(Shared) : offsetof(Shared, low)));
     cg::cluster_group cluster = cg::this_cluster();
     const int ranks = static_cast<int>(cluster.num_blocks());
     const int rank = static_cast<int>(cluster.block_rank());
@@ -568,9 +574,9 @@ __global__ void __launch_bounds__(kMaxThreads) k_sample_tokens(Args a) {
     Row<T> row{sh, cluster, ranks, rank, a.staged ? staged : global, begin, end - begin};
 
     const float temperature = a.p.temperatures ? a.p.temperatures[r] : a.p.temperature;
-    const float top_p = a.p.top_ps ? a.p.top_ps[r] : a.p.top_p;
-    const float min_p = a.p.min_ps ? a.p.min_ps[r] : a.p.min_p;
-    const int top_k = a.p.top_ks ? a.p.top_ks[r] : a.p.top_k;
+    const float top_p = !FILTERS ? 1.0f : a.p.top_ps ? a.p.top_ps[r] : a.p.top_p;
+    const float min_p = !FILTERS ? 0.0f : a.p.min_ps ? a.p.min_ps[r] : a.p.min_p;
+    const int top_k = !FILTERS ? 0 : a.p.top_ks ? a.p.top_ks[r] : a.p.top_k;
 
     if (threadIdx.x < 32) sh.powers[threadIdx.x] = exp2(threadIdx.x / 32.0);
     // The largest logit (fmaxf passes over NaN).
@@ -664,7 +670,7 @@ __global__ void __launch_bounds__(kMaxThreads) k_sample_tokens(Args a) {
     // well below the threads' number, so those alone are counted in bins; with fewer threads than k
     // all logits are.
     const Distance distance(top, least);
-    if (top_k > 0 && top_k <= kList / 2 && distance.usable) {
+    if constexpr (FILTERS) if (top_k > 0 && top_k <= kList / 2 && distance.usable) {
         const float least_f = float_of(least);
         for (int i = threadIdx.x; i < kCountBins; i += threads()) sh.low[i] = 0u;
         if (threadIdx.x == 0) sh.listed = 0;
@@ -745,7 +751,7 @@ __global__ void __launch_bounds__(kMaxThreads) k_sample_tokens(Args a) {
     // Kept: keys above `edge` and the first `ties` tokens, by index, with exactly that key.
     uint32_t edge = 0;
     u64 ties = 0;
-    if (top_k > 0 && top_k < a.V) {
+    if constexpr (FILTERS) if (top_k > 0 && top_k < a.V) {
         u64 n = 0;
         for (int i = threadIdx.x; i < row.count; i += threads()) n += key_of(row.at(i)) >= least;
         unused = 0;
@@ -758,7 +764,7 @@ __global__ void __launch_bounds__(kMaxThreads) k_sample_tokens(Args a) {
             ties = static_cast<u64>(top_k) - t.above;
         }
     }
-    if (top_p < 1.0f) {
+    if constexpr (FILTERS) if (top_p < 1.0f) {
         const uint32_t from = max(least, edge + (edge ? 1u : 0u));
         const u64 tied = edge ? ties * weight(edge) : 0;
         const Threshold t = find_threshold<true>(
@@ -780,7 +786,7 @@ __global__ void __launch_bounds__(kMaxThreads) k_sample_tokens(Args a) {
             ties = need;
         }
     }
-    if (floored) {
+    if constexpr (FILTERS) if (floored) {
         // The smallest key with a weight of at least min_p; all of its tokens are kept.
         if (threadIdx.x < 32) {
             uint32_t low = top;
@@ -901,7 +907,7 @@ __global__ void __launch_bounds__(kMaxThreads) k_sample_tokens(Args a) {
     }
 }
 
-template <typename T>
+template <typename T, bool FILTERS>
 cudaError_t launch_typed(cudaStream_t s, Args a, int rows) {
     // A slice of at most 16 Ki logits a CTA keeps the passes over it short; beyond eight CTAs (the
     // portable cluster) slices grow, and past the shared memory they are read through L2.
@@ -909,14 +915,15 @@ cudaError_t launch_typed(cudaStream_t s, Args a, int rows) {
     while (cluster < kMaxCluster && (a.V + cluster - 1) / cluster > (1 << 14)) cluster *= 2;
     a.per = ((a.V + cluster - 1) / cluster + 7) / 8 * 8;  // 16-byte chunks do not straddle slices
     const size_t slice = static_cast<size_t>(a.per) * sizeof(T);
-    a.staged = sizeof(Shared) + slice <= 200 * 1024;
-    const size_t smem = sizeof(Shared) + (a.staged ? slice : 0);
-    cudaError_t e = cudaFuncSetAttribute(k_sample_tokens<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         200 * 1024);
+    const size_t fixed = FILTERS ? sizeof(Shared) : offsetof(Shared, low);
+    a.staged = fixed + slice <= 200 * 1024;
+    const size_t smem = fixed + (a.staged ? slice : 0);
+    const auto kernel = k_sample_tokens<T, FILTERS>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
     if (e) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(rows) * cluster);
-    cfg.blockDim = dim3(cluster == 1 ? kMaxThreads / 2 : kMaxThreads);
+    cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
@@ -926,7 +933,7 @@ cudaError_t launch_typed(cudaStream_t s, Args a, int rows) {
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k_sample_tokens<T>, a);
+    return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
 }  // namespace
@@ -944,8 +951,13 @@ cudaError_t launch_sample_tokens(cudaStream_t s, const void* logits, int dtype, 
     a.uniform_stride = uniform_stride;
     a.step = step;
     a.tokens = tokens;
-    return dtype == BST_DTYPE_BF16 ? launch_typed<__nv_bfloat16>(s, a, rows)
-                                   : launch_typed<float>(s, a, rows);
+    const Sampling& p = a.p;
+    const bool filters = p.top_ks || p.top_ps || p.min_ps || p.top_k > 0 || p.top_p < 1.0f || p.min_p > 0.0f;
+    if (dtype == BST_DTYPE_BF16) {
+        return filters ? launch_typed<__nv_bfloat16, true>(s, a, rows)
+                       : launch_typed<__nv_bfloat16, false>(s, a, rows);
+    }
+    return filters ? launch_typed<float, true>(s, a, rows) : launch_typed<float, false>(s, a, rows);
 }
 
 }  // namespace bst
