@@ -642,6 +642,31 @@ def test_captured_prompts_and_draws(ops):
             assert torch.equal(pair[0].nan_to_num(7.0), a.nan_to_num(7.0)) and torch.equal(pair[1], b)
 
 
+def test_prompts_and_draws_on_two_streams_at_once(ops):
+    torch = torch_()
+    rng = np.random.default_rng(15)
+    T, H, KV, d = 1500, 8, 2, 128
+    starts = ints([0, 700, T])
+    u, x = tensor(rng.random(300)), tensor(rng.standard_normal((300, 20000)).astype(np.float32))
+    sets = [[tensor(rng.standard_normal((T, n, d)).astype(np.float32), dtype) for n in (H, KV, KV)]
+            for dtype in ("bf16", "bf16", "f32")]
+
+    def step(i):
+        return (ops.attention_packed(*sets[i], starts, window=(0, 300, 100)[i], sinks=2),
+                ops.sample_tokens(x, u, top_k=(0, 50, 900)[i], top_p=(0.9, 1.0, 0.8)[i]))
+
+    want = [step(i) for i in range(3)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = [[] for _ in range(3)]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step(i))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for i in range(3) for g in got[i] for a, b in zip(g, want[i]))
+
+
 def test_memory_belongs_to_the_given_stream(ops):
     """What a call on a stream of its own allocates may be used again in that stream's order only."""
     torch = torch_()
