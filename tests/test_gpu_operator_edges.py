@@ -1,0 +1,85 @@
+"""The serving operators on the GPU at the edges of their arguments, against plain 64-bit formulas.
+
+Tolerances are those of test_gpu_operators.py's bound(): a score of d products is off by at most
+(d + 8) 2^-23 sum|q k| scale, a weight by twice that and 2^-21, a sum of n weights by (n + 16) 2^-23,
+each in units of the largest value that the query sees; bf16 adds 2^-8 of that and of the output.
+"""
+import math
+
+import numpy as np
+import pytest
+
+import operator_reference as ref
+from test_gpu_operators import bound, host, ints, ops, tensor, torch_  # noqa: F401 (ops: a fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+def attend(q, k, v, first=0, window=0, sinks=0, scale=None):
+    """One sequence by the formula alone, NaN and infinities as 64-bit arithmetic has them; and the
+    bound's sizes: per query and head the largest sum |q k| scale, per output the largest finite
+    |v| that the query sees."""
+    n, H, d = q.shape
+    scale = 1 / math.sqrt(d) if scale is None else scale
+    out, size, most = np.zeros((n, H, d)), np.zeros((n, H)), np.zeros((n, H, d))
+    with np.errstate(all="ignore"):
+        for i in range(n):
+            if first + i < 0:
+                continue
+            seen = ref.visible(first + i, k.shape[0], window, sinks)
+            for h in range(H):
+                kk, vv = k[seen, h * k.shape[1] // H], v[seen, h * k.shape[1] // H]
+                s = kk @ q[i, h] * scale
+                p = np.exp(s - s.max())
+                out[i, h] = p @ vv / p.sum()
+                sizes = np.abs(kk) @ np.abs(q[i, h]) * abs(scale)
+                size[i, h] = sizes[np.isfinite(sizes)].max(initial=0.0)
+                most[i, h] = np.where(np.isfinite(vv), np.abs(vv), 0).max(0)
+    return out, size, most
+
+
+def check(got, want, size, most, d, n, dtype):
+    """NaN and infinities where the formula has them, elsewhere numbers within the bound."""
+    tol = bound(size, d, n, most, np.where(np.isfinite(want), want, 0), dtype)
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    whole = np.isinf(want)
+    assert np.array_equal(got[whole], want[whole])
+    ok = np.isfinite(want)
+    assert np.all(np.abs(got[ok] - want[ok]) <= tol[ok]), np.abs(got[ok] - want[ok]).max()
+
+
+def prompt(rng, T, heads, kv_heads, dim, dtype):
+    return [tensor(rng.standard_normal((T, h, dim)).astype(np.float32), dtype)
+            for h in (heads, kv_heads, kv_heads)]
+
+
+# ---- packed prompts ----------------------------------------------------------------------------
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("which", [0, 1, 2], ids="qkv")
+@pytest.mark.parametrize("dtype,bits", [("f32", 0x7fffffff), ("f32", -1), ("f32", 0x7f800001),
+                                        ("f32", 0x7fc00000), ("bf16", 0x7fff), ("bf16", -1)])
+def test_any_nan_of_a_prompt_reaches_the_queries_that_see_it(ops, dtype, bits, which, dim):
+    """Whatever its bits, in tiles of keys that all of a tile's queries see and in others."""
+    torch = torch_()
+    x = prompt(np.random.default_rng(dim + which), 200, 2, 2, dim, dtype)
+    x[which].view(torch.int32 if dtype == "f32" else torch.int16)[20, 1, 3] = bits
+    got = host(ops.attention_packed(*x, ints([0, 200])))
+    want, size, most = attend(*[host(t) for t in x])
+    assert np.isnan(want).any() and np.isfinite(want[:, 0]).all()
+    check(got, want, size, most, dim, 200, dtype)
+
+
+def test_a_nan_group_of_a_4_bit_cache_stays_one_in_a_prompt(ops):
+    """Values read back from the cache go into a prompt's attention, as an engine's do."""
+    rng = np.random.default_rng(21)
+    q, k, v = prompt(rng, 150, 2, 2, 64, "f32")
+    k[30, 0, 40], v[20, 1, 5] = float("nan"), float("inf")
+    cache, starts = ops.KvCache.allocate(1, 2, 150, 64), ints([0, 150])
+    ops.kv_append(cache, k, v, ints([150]), starts=starts)
+    k, v = ops.kv_read(cache, ints([150]), starts=starts, tokens=150)
+    want, size, most = attend(host(q), host(k), host(v))
+    assert np.isnan(want[30:, 0]).all() and np.isnan(want[20:, 1, :32]).all()
+    check(host(ops.attention_packed(q, k, v, starts)), want, size, most, 64, 150, "f32")
+    # and the cached form of the last query sees the same
+    got = host(ops.attention_cached(cache, q[149:], ints([150])))
+    check(got, want[149:], size[149:], most[149:], 64, 150, "f32")
