@@ -5,7 +5,8 @@
 //   s_ij = scale q_i . k_j over the keys j that query i sees; zeros when it sees none.
 //
 // A running maximum and sum per query let every kernel read each key and value once; a key that a
-// query does not see takes no part at all, whatever it holds (NaN and infinities included).
+// query does not see takes no part at all, whatever it holds (NaN and infinities included), and those
+// that it sees count as in float32 arithmetic.
 
 #include <cuda_bf16.h>
 
@@ -554,7 +555,7 @@ __device__ __forceinline__ void attend_query(const T* q, const T* k, int64_t k_s
 // values pass through shared memory in tiles, double-buffered with cp.async. float32 operands are
 // split in two tf32 parts, x = h + l with h the upper 10 mantissa bits, and multiplied as
 // h h + h l + l h (2^-21 of a product is left out); bf16 ones are tf32 numbers as they are, their
-// weights rounded to tf32. The tensor cores cut sums where float32 additions round: sums of a whole
+// weights rounded to tf32. A CTA whose outputs are not all finite has them computed again. The tensor cores cut sums where float32 additions round: sums of a whole
 // row came out 3e-6 low, so products are summed 32 channels, or a tile of keys, at a time (the small
 // ones apart) and added up in float32. Splitting happens in registers after the load, so the tiles stay float32.
 // Rows of keys are padded to HD + 8 floats and of values to HD + 4, which keeps the fragments' reads
@@ -827,11 +828,17 @@ k_packed_mma(Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride, con
         if (row < rows) {
             const int token = position[r], head = kvh * group + tile.r0 + row - token * group;
             T* to = out + (tile.first + static_cast<int64_t>(token)) * out_stride + head * HD + 2 * t;
+            float most = fabsf(total[r]);
 #pragma unroll
             for (int c = 0; c < HD / 8; ++c) {
-                put(to + 8 * c, o[c][2 * r] * by);
-                put(to + 8 * c + 1, o[c][2 * r + 1] * by);
+                const float x = o[c][2 * r] * by, y = o[c][2 * r + 1] * by;
+                put(to + 8 * c, x);
+                put(to + 8 * c + 1, y);
+                most = max_nan(most, max_nan(fabsf(x), fabsf(y)));
             }
+            // The parts of an infinity, and of a float that rounds to one, leave NaN where the formula
+            // may have a weight of zero, an infinity or a number.
+            if (!(most <= FLT_MAX)) redo = 1;
         }
     }
     __syncthreads();

@@ -53,18 +53,6 @@ __device__ __forceinline__ float group_step(float low, float high) {
     return bf16_up_positive(__double2float_ru(d));
 }
 
-// min and max that hand on a NaN.
-__device__ __forceinline__ float min_nan(float a, float b) {
-    float r;
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
-
 // The codes rint((x - low) / step), of the double quotient, of four values in 16 bits. A float
 // quotient q is within 15 * 4 * 2^-24 < 4e-6 of it (the reciprocal is good to 2^-23), so only a q within
 // 1e-5 of a tie needs the double (and one that is no number, for steps below 2^-126). Adding 1.5 * 2^23 rounds q to nearest

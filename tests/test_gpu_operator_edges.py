@@ -83,3 +83,40 @@ def test_a_nan_group_of_a_4_bit_cache_stays_one_in_a_prompt(ops):
     # and the cached form of the last query sees the same
     got = host(ops.attention_cached(cache, q[149:], ints([150])))
     check(got, want[149:], size[149:], most[149:], 64, 150, "f32")
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (90, 3)])
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("which,value", [(1, math.inf), (1, -math.inf), (2, math.inf), (2, -math.inf),
+                                         (1, -3.4025e38), (2, 3.4028e38)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_visible_infinities_count_as_the_formula_has_them(ops, dtype, which, value, dim, window, sinks):
+    """A key of -inf weighs nothing, one of +inf leaves NaN, an infinite value an infinity: in tiles
+    that all queries see as in others. The last two values are floats that the parts of tf32, and
+    bf16, round to infinity."""
+    rng = np.random.default_rng(dim)
+    x = prompt(rng, 200, 2, 2, dim, dtype)
+    x[0][:, :, 3] = x[0][:, :, 3].abs() * 0.1 + 0.5       # the sign of the score
+    x[which][20, 1, 3] = value
+    got = host(ops.attention_packed(*x, ints([0, 200]), window=window, sinks=sinks))
+    xh = [host(t) for t in x]
+    want, size, most = attend(*xh, 0, window, sinks)
+    if which == 1:   # the largest score decides the bound, not the one that weighs nothing
+        size = attend(xh[0], np.where(np.abs(xh[1]) > 1e38, 0, xh[1]), xh[2], 0, window, sinks)[1]
+    check(got, want, size, most, dim, 200, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("heads,kv_heads,scale", [(2, 2, None), (6, 2, -0.2), (5, 1, 0.5)])
+def test_rows_that_are_computed_again_are_as_good(ops, dtype, dim, heads, kv_heads, scale):
+    """A value that is not finite has its neighbours' rows computed by another kernel: to the bounds
+    that all rows have."""
+    rng = np.random.default_rng(dim + heads)
+    q, k, v = prompt(rng, 230, heads, kv_heads, dim, dtype)
+    k[150, kv_heads - 1], v[150, kv_heads - 1] = math.nan, math.inf
+    starts = [0, 30, 230]
+    got = host(ops.attention_packed(q, k, v, ints(starts), window=50, sinks=2, scale=scale))
+    for a, b in zip(starts, starts[1:]):
+        want, size, most = attend(*[host(t)[a:b] for t in (q, k, v)], 0, 50, 2, scale)
+        check(got[a:b], want, size, most, dim, 200, dtype)
