@@ -366,7 +366,7 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
         // Rows behind the last query see nothing.
         const int position = at < rows ? my_token : -1;
         const int low = a.window ? position - a.window + 1 : 0;  // the window's first key
-        const float slack = 8.0f / scale;                        // scale 0: infinite, never moved
+        const float slack = 8.0f / scale;                        // infinite for the smallest scales: never moved
         float top = -INFINITY, from = 0.0f, total = 0.0f;
         // A wait that runs out ends no loop here: the tile's threads meet at a barrier behind it, and
         // what they write then is computed again.
@@ -872,13 +872,14 @@ k_packed_again(Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride,
     }
 }
 
-// Whether TMA and 16-byte accesses can address these bf16 tensors.
-bool tc_takes(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
-              int64_t v_stride, const void* out, int64_t out_stride) {
+// Whether TMA and 16-byte accesses can address these bf16 tensors, and the scale is not zero: the kernel
+// multiplies by it behind the mask, whose -inf it would turn into NaN.
+bool tc_takes(float scale, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+              const void* v, int64_t v_stride, const void* out, int64_t out_stride) {
     auto aligned = [](const void* p, int64_t stride) {
         return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 8 == 0;
     };
-    return aligned(q, q_stride) && aligned(k, k_stride) && aligned(v, v_stride) &&
+    return scale != 0.0f && aligned(q, q_stride) && aligned(k, k_stride) && aligned(v, v_stride) &&
            aligned(out, out_stride);
 }
 
@@ -905,7 +906,7 @@ cudaError_t launch_attention_packed(cudaStream_t s, const Batch& b, const AttnSp
             int tile_rows = 0, tiles = 0;
             cudaError_t e = cudaSuccess;
             if constexpr (sizeof(T) == 2 && HD >= 64) {
-                if (tc_takes(q, q_stride, k, k_stride, v, v_stride, out, out_stride)) {
+                if (tc_takes(a.scale, q, q_stride, k, k_stride, v, v_stride, out, out_stride)) {
                     tile_rows = kTcRows;
                     tiles = tile_bound(b, a, tile_rows);
                     CUtensorMap k_map, v_map;

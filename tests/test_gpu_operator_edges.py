@@ -120,3 +120,34 @@ def test_rows_that_are_computed_again_are_as_good(ops, dtype, dim, heads, kv_hea
     for a, b in zip(starts, starts[1:]):
         want, size, most = attend(*[host(t)[a:b] for t in (q, k, v)], 0, 50, 2, scale)
         check(got[a:b], want, size, most, dim, 200, dtype)
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (37, 4)])
+@pytest.mark.parametrize("scale", [0.0, -0.0, -0.2, 3.0, 1e-40])
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_prompts_at_any_scale(ops, dtype, dim, scale, window, sinks):
+    """Zero gives the mean of the visible values, a negative one turns the order around. Aligned
+    tensors, so that bf16 takes the tensor-core kernel, and heads that share keys."""
+    rng = np.random.default_rng(dim + window)
+    q, k, v = prompt(rng, 500, 6, 2, dim, dtype)
+    starts = [0, 99, 99, 500]
+    got = host(ops.attention_packed(q, k, v, ints(starts), window=window, sinks=sinks, scale=scale))
+    for a, b in zip(starts, starts[1:]):
+        want, size, most = attend(*[host(t)[a:b] for t in (q, k, v)], 0, window, sinks, scale)
+        check(got[a:b], want, size, most, dim, 500, dtype)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 2.0])
+@pytest.mark.parametrize("group", [1, 3, 20])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("storage", ["u4", "f32", "bf16"])
+def test_cached_attention_at_any_scale(ops, storage, dtype, group, scale):
+    rng = np.random.default_rng(group)
+    k, v = (tensor(rng.standard_normal((60, 2, 64)).astype(np.float32)) for _ in range(2))
+    cache, starts = ops.KvCache.allocate(1, 2, 64, 64, storage), ints([0, 60])
+    ops.kv_append(cache, k, v, ints([60]), starts=starts)
+    k, v = (host(t) for t in ops.kv_read(cache, ints([60]), starts=starts, tokens=60))
+    q = tensor(rng.standard_normal((1, 2 * group, 64)).astype(np.float32), dtype)
+    want, size, most = attend(host(q), k, v, 59, 0, 0, scale)
+    check(host(ops.attention_cached(cache, q, ints([60]), scale=scale)), want, size, most, 64, 60, dtype)
