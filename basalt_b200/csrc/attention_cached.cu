@@ -1260,16 +1260,26 @@ int ctas_per_sm(const Cache& c, const Batch& b, const AttnSpec& a) {
 }
 
 // One full wave of CTAs where the tiles alone are fewer (131 000 keys of eight heads: two waves took
-// 80 us, one 68), and among several sequences splits of at most 4096 keys, so that long ones spread
-// over the SMs beside short ones; never less than 128 keys a split. The lengths are on the device, so
-// the bound is what the cache and the window allow; tiles with fewer keys use fewer splits
-// (useful_splits).
+// 80 us, one 68 at that step), and among several sequences splits of at most 4096 keys, so that long ones
+// spread over the SMs beside short ones; never less than 128 keys a split. The lengths are on the device,
+// so the bound is what the cache and the window allow; tiles with fewer keys use fewer splits
+// (useful_splits). Splits of 4096 keys end where a sequence's own tiles and their splits fill the card,
+// and where their workspace would pass kSplitBytes: two prompts' chunks of 4096 tokens over 131 072 slots
+// (32 heads of 128 over 8) took 4.4 GB, of which no SM had any use, and now take none.
+constexpr int64_t kSplitBytes = 128 << 20;  // about what L2 holds
 int split_count(const Cache& c, const Batch& b, const AttnSpec& a) {
     int64_t keys = c.slots;
     if (a.window) keys = std::min<int64_t>(keys, static_cast<int64_t>(a.window) + a.sinks + 2 * kBlock);
     const int64_t units = static_cast<int64_t>(tile_bound(b, a, rows_of_tile(b, a))) * a.kv_heads;
-    const int64_t fill = 148 * ctas_per_sm(c, b, a) / std::max<int64_t>(units, 1);
-    const int64_t even = b.count > 1 ? (keys + 4095) / 4096 : 1;
+    const int64_t card = 148 * ctas_per_sm(c, b, a);
+    const int64_t fill = card / std::max<int64_t>(units, 1);
+    int64_t even = 1;
+    if (b.count > 1) {
+        const int64_t own = std::max<int64_t>(1, units / b.count);
+        const int64_t split = static_cast<int64_t>(b.tokens) * a.heads * (a.head_dim + 2) * sizeof(float);
+        even = std::min<int64_t>({(keys + 4095) / 4096, (card + own - 1) / own,
+                                  std::max<int64_t>(1, kSplitBytes / std::max<int64_t>(split, 1))});
+    }
     const int64_t most = std::max<int64_t>(1, keys / 128);
     return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({std::max(fill, even), most, kMaxSplits})));
 }

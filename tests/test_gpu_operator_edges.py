@@ -151,3 +151,34 @@ def test_cached_attention_at_any_scale(ops, storage, dtype, group, scale):
     q = tensor(rng.standard_normal((1, 2 * group, 64)).astype(np.float32), dtype)
     want, size, most = attend(host(q), k, v, 59, 0, 0, scale)
     check(host(ops.attention_cached(cache, q, ints([60]), scale=scale)), want, size, most, 64, 60, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("counts,lengths,window", [([300, 301], [5000, 700], 0),
+                                                   ([1, 2, 150], [9000, 40, 8000], 0),
+                                                   ([300, 301], [5000, 700], 1000)])
+def test_chunks_of_prompts_over_a_long_cache(ops, dtype, counts, lengths, window):
+    torch = torch_()
+    rng = np.random.default_rng(sum(counts))
+    S, slots, heads, kv_heads, dim = len(counts), 20000, 8, 2, 64
+    cache = ops.KvCache.allocate(S, kv_heads, slots, dim)
+    stored = np.concatenate([[0], np.cumsum(lengths)])
+    x = [tensor(rng.standard_normal((stored[-1], kv_heads, dim)).astype(np.float32)) for _ in range(2)]
+    ops.kv_append(cache, *x, ints(lengths), starts=ints(stored))
+    k, v = (t.double() for t in ops.kv_read(cache, ints(lengths), starts=ints(stored),
+                                            tokens=int(stored[-1])))
+    q = tensor(rng.standard_normal((sum(counts), heads, dim)).astype(np.float32), dtype)
+    starts = np.concatenate([[0], np.cumsum(counts)])
+    got = ops.attention_cached(cache, q, ints(lengths), starts=ints(starts), window=window).double()
+    for s, n in enumerate(counts):
+        a, L = starts[s], lengths[s]
+        kk, vv = (t[stored[s]:stored[s] + L].repeat_interleave(heads // kv_heads, 1) for t in (k, v))
+        qq = q[a:a + n].double()
+        score = torch.einsum("nhd,khd->nhk", qq, kk) / math.sqrt(dim)
+        size = torch.einsum("nhd,khd->nhk", qq.abs(), kk.abs()).amax(-1) / math.sqrt(dim)
+        at, key = torch.arange(L - n, L, device="cuda")[:, None], torch.arange(L, device="cuda")
+        seen = (key <= at) & ((at - key < window) | (window == 0))
+        p = torch.softmax(score.masked_fill(~seen[:, None], -math.inf), -1)
+        want = torch.einsum("nhk,khd->nhd", p, vv)
+        tol = bound(host(size), dim, L, host(vv).__abs__().max(), host(want), dtype)
+        assert np.all(np.abs(host(got[a:a + n]) - host(want)) <= tol)
