@@ -80,6 +80,29 @@ int check_tensor(const char* name, const void* p, int64_t stride, int64_t heads,
     return BST_OK;
 }
 
+// A packed tensor's place in memory: `tokens` runs of `run` bytes, `stride` bytes apart.
+struct Span {
+    uint64_t at, stride, run;
+    int64_t tokens;
+    uint64_t end() const { return at + (tokens - 1) * stride + run; }
+};
+
+// Whether two of them share a byte. Runs at the same stride may lie between one another (slices of
+// one tensor); at different ones no byte between the first and the last may be shared.
+bool overlap(const Span& x, const Span& y) {
+    if (x.end() <= y.at || y.end() <= x.at) return false;
+    if (x.stride != y.stride || x.tokens == 1) return true;
+    const uint64_t ahead = y.at >= x.at ? (y.at - x.at) % x.stride
+                                        : (x.stride - (x.at - y.at) % x.stride) % x.stride;
+    return ahead < x.run || x.stride - ahead < y.run;
+}
+
+Span span_of(const void* p, int64_t stride, int64_t heads, const AttnSpec& a, int tokens) {
+    const uint64_t size = size_of(a.dtype);
+    return Span{reinterpret_cast<uint64_t>(p), static_cast<uint64_t>(stride) * size,
+                static_cast<uint64_t>(heads) * a.head_dim * size, tokens};
+}
+
 }  // namespace
 
 int check_cache(const bst_kv_cache* c, Cache* out, std::string* why) {
@@ -339,6 +362,13 @@ int32_t bst_attention_cached(int32_t device, void* stream, const bst_kv_cache* c
         if (b.tokens == 0 || b.count == 0) return BST_OK;
         st = check_tensor("q", q, q_stride, a.heads, a.head_dim, a.dtype, &why);
         if (!st) st = check_tensor("out", out, out_stride, a.heads, a.head_dim, a.dtype, &why);
+        // Every CTA has read its queries when it writes their outputs: those may take their place.
+        if (!st && !(out == q && out_stride == q_stride) &&
+            overlap(span_of(q, q_stride, a.heads, a, b.tokens),
+                    span_of(out, out_stride, a.heads, a, b.tokens))) {
+            st = BST_INVALID;
+            why = "out overlaps q (it may only be q itself)";
+        }
         if (!st) {
             st = check_workspace(attention_cached_workspace(c, b, a), workspace, workspace_bytes,
                                  &why);
@@ -383,6 +413,16 @@ int32_t bst_attention_packed(int32_t device, void* stream, const bst_sequences* 
         if (!st) st = check_tensor("k", k, k_stride, a.kv_heads, a.head_dim, a.dtype, &why);
         if (!st) st = check_tensor("v", v, v_stride, a.kv_heads, a.head_dim, a.dtype, &why);
         if (!st) st = check_tensor("out", out, out_stride, a.heads, a.head_dim, a.dtype, &why);
+        // Keys and values are read by many CTAs, and queries again where rows are computed again.
+        if (!st) {
+            const Span to = span_of(out, out_stride, a.heads, a, b.tokens);
+            if (overlap(to, span_of(q, q_stride, a.heads, a, b.tokens)) ||
+                overlap(to, span_of(k, k_stride, a.kv_heads, a, b.tokens)) ||
+                overlap(to, span_of(v, v_stride, a.kv_heads, a, b.tokens))) {
+                st = BST_INVALID;
+                why = "out must not overlap q, k or v";
+            }
+        }
         if (!st) {
             st = check_workspace(attention_packed_workspace(b, a), workspace, workspace_bytes, &why);
         }

@@ -264,7 +264,8 @@ def attention_cached(cache: KvCache, q, lengths, starts=None, rows=None, window:
                      sinks: int = 0, scale=None, out=None, workspace=None, stream=None):
     """Attention of q ([tokens, heads, head_dim]) over the sequences' rows of ``cache``, whose
     current tokens were appended before. ``window`` and ``sinks``: a query sees the last ``window``
-    keys (0: all) and the first ``sinks``. ``scale`` is 1 / sqrt(head_dim) by default."""
+    keys (0: all) and the first ``sinks``. ``scale`` is 1 / sqrt(head_dim) by default. ``out`` may be
+    ``q`` itself."""
     device = cache.device
     q_stride = _packed(device, "q", q, None, cache.head_dim)
     out, out_stride = _out(device, q, out, stream)
@@ -287,7 +288,7 @@ def attention_cached(cache: KvCache, q, lengths, starts=None, rows=None, window:
 def attention_packed(q, k, v, starts, window: int = 0, sinks: int = 0, scale=None, out=None,
                      workspace=None, stream=None):
     """Causal attention of packed sequences over their own keys and values: q [tokens, heads,
-    head_dim], k and v [tokens, kv_heads, head_dim], all of one type."""
+    head_dim], k and v [tokens, kv_heads, head_dim], all of one type. ``out`` must not overlap them."""
     _torch()
     device = q.device
     _on(device, "q", q)

@@ -342,10 +342,10 @@ typedef struct bst_attention_spec {
 
 /* out[t] = attention of the batch's queries over their rows of the cache, this call's own tokens
  * included (append them first). q and out: [tokens][heads][head_dim], tokens q_stride and
- * out_stride elements apart. A cache of float32 or bf16 takes one token per sequence (starts
- * NULL); a 4-bit cache takes any number. workspace: at least the bytes that
- * bst_attention_cached_workspace gives for the same arguments (16-byte aligned, may be NULL when
- * that is 0), not shared with calls that run at the same time. */
+ * out_stride elements apart; out may be q itself, and overlaps it in no other way. A cache of
+ * float32 or bf16 takes one token per sequence (starts NULL); a 4-bit cache takes any number.
+ * workspace: at least the bytes that bst_attention_cached_workspace gives for the same arguments
+ * (16-byte aligned, may be NULL when that is 0), not shared with calls that run at the same time. */
 int32_t bst_attention_cached_workspace(const bst_kv_cache* cache, const bst_sequences* sequences,
                                        const bst_attention_spec* spec, int64_t* bytes);
 int32_t bst_attention_cached(int32_t device, void* stream, const bst_kv_cache* cache,
@@ -355,7 +355,8 @@ int32_t bst_attention_cached(int32_t device, void* stream, const bst_kv_cache* c
 
 /* Causal attention of packed sequences over their own keys and values (prompts that need no cache
  * yet): sequences->starts is required, rows and lengths must be NULL, positions count from 0.
- * q and out [tokens][heads][head_dim], k and v [tokens][kv_heads][head_dim]. */
+ * q and out [tokens][heads][head_dim], k and v [tokens][kv_heads][head_dim]. out shares no byte with
+ * q, k or v (at the same distance between tokens it may lie between theirs). */
 int32_t bst_attention_packed_workspace(const bst_sequences* sequences,
                                        const bst_attention_spec* spec, int64_t* bytes);
 int32_t bst_attention_packed(int32_t device, void* stream, const bst_sequences* sequences,

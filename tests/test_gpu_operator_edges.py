@@ -182,3 +182,41 @@ def test_chunks_of_prompts_over_a_long_cache(ops, dtype, counts, lengths, window
         want = torch.einsum("nhk,khd->nhd", p, vv)
         tol = bound(host(size), dim, L, host(vv).__abs__().max(), host(want), dtype)
         assert np.all(np.abs(host(got[a:a + n]) - host(want)) <= tol)
+
+
+@pytest.mark.parametrize("storage,heads,kv_heads,tokens", [("u4", 2, 2, 1), ("u4", 8, 2, 1), ("u4", 8, 2, 5),
+                                                           ("bf16", 8, 2, 1), ("f32", 8, 2, 1)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_cached_outputs_may_take_the_queries_place(ops, dtype, storage, heads, kv_heads, tokens):
+    torch = torch_()
+    rng = np.random.default_rng(heads)
+    k, v = (tensor(rng.standard_normal((3 * 900, kv_heads, 64)).astype(np.float32)) for _ in range(2))
+    cache = ops.KvCache.allocate(3, kv_heads, 900, 64, storage)
+    ops.kv_append(cache, k, v, ints([900] * 3), starts=ints([0, 900, 1800, 2700]))
+    q = tensor(rng.standard_normal((3 * tokens, heads, 64)).astype(np.float32), dtype)
+    lengths, starts = ints([900, 17, 300]), ints(np.arange(4) * tokens) if tokens > 1 else None
+    want = ops.attention_cached(cache, q, lengths, starts=starts)
+    assert ops.attention_cached(cache, q, lengths, starts=starts, out=q) is q
+    assert torch.equal(q, want)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_packed_outputs_stay_out_of_what_is_read(ops, dtype):
+    """Rows may be computed twice, from queries that have to be there still."""
+    from basalt_b200 import IllegalArgumentException
+
+    torch = torch_()
+    rng = np.random.default_rng(4)
+    wide = tensor(rng.standard_normal((200, 8, 64)).astype(np.float32), dtype)
+    q, k, v, out = (wide[:, a:b] for a, b in ((0, 2), (2, 4), (4, 6), (6, 8)))
+    v[100, 1, 3] = math.inf
+    starts = ints([0, 200])
+    want = ops.attention_packed(q, k, v, starts, window=50)
+    assert torch.isfinite(want[:100]).all() and not torch.isfinite(want[100:150, 1, 3]).any()
+    for bad in (q, k, v, wide[:, 1:3]):
+        before = wide.clone()
+        with pytest.raises(IllegalArgumentException, match="overlap"):
+            ops.attention_packed(q, k, v, starts, window=50, out=bad)
+        assert torch.equal(wide.nan_to_num(), before.nan_to_num())
+    ops.attention_packed(q, k, v, starts, window=50, out=out)
+    assert torch.equal(out, want)

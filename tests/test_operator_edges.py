@@ -33,3 +33,33 @@ def test_few_tokens_over_long_caches_are_split():
     assert workspace(24, 96, 16384, 32, 8, 128) == 4 * 96 * row
     assert workspace(256, 256, 131072, 32, 8, 128, starts=False) >= 16 * 256 * row
     assert workspace(1, 1, 131072, 32, 8, 128, starts=False) == 148 * 2 // 8 * row
+
+
+def test_outputs_do_not_overlap_what_is_read():
+    """Tokens of 4 heads of 64 float32 (1024 bytes), keys and values of 2 heads (512 bytes)."""
+    lib, at = _lib.load(), 1 << 20
+
+    def packed(out, out_stride=256, q=at, q_stride=256, k=at + (1 << 16), v=at + (2 << 16), stride=128,
+               tokens=2):
+        # far pointers pass the check and stop at the workspace, which is missing
+        return lib.bst_attention_packed(0, None, batch(tokens=tokens, starts=256, lengths=None), spec(), q,
+                                        q_stride, k, stride, v, stride, out, out_stride, None, 0)
+
+    def cached(out, out_stride=256, q_stride=256):
+        return lib.bst_attention_cached(0, None, cache(rows=2, slots=1 << 20), batch(), spec(), at,
+                                        q_stride, out, out_stride, None, 0)
+
+    assert packed(at + (3 << 16)) == _lib.BST_SHAPE
+    assert packed(at + 2048) == _lib.BST_SHAPE                         # right behind q
+    for out in (at, at + 4, at + 2044, at - 2044, at + (1 << 16), at + (1 << 16) + 1020, at + (2 << 16)):
+        assert packed(out) == _lib.BST_INVALID
+        assert "overlap" in _lib.last_error()
+    # slices of one tensor: q at 0, keys at 256, values at 384, outputs at 512 of 768 elements
+    slices = dict(q_stride=768, k=at + 1024, v=at + 1536, stride=768, out_stride=768)
+    assert packed(at + 2048, **slices) == _lib.BST_SHAPE
+    for out in (at + 2044, at + 2052, at, at + 1536, at - 1020):
+        assert packed(out, **slices) == _lib.BST_INVALID
+    assert packed(at + 2048, **{**slices, "out_stride": 769}) == _lib.BST_INVALID
+    assert packed(at + 2048, tokens=1, **{**slices, "out_stride": 769}) == _lib.BST_SHAPE
+    assert cached(at) == cached(at + 2048) == _lib.BST_SHAPE           # q itself; behind it
+    assert cached(at + 4) == cached(at, 260) == cached(at + 1024) == _lib.BST_INVALID
