@@ -7,6 +7,7 @@ another implementation.
 from __future__ import annotations
 
 import ctypes
+import operator
 from pathlib import Path
 
 PACKAGE = Path(__file__).resolve().parent
@@ -71,6 +72,12 @@ class SamplingStruct(ctypes.Structure):
                 ("min_p", ctypes.c_float), ("top_k", ctypes.c_int32),
                 ("temperatures", ctypes.c_void_p), ("top_ps", ctypes.c_void_p),
                 ("min_ps", ctypes.c_void_p), ("top_ks", ctypes.c_void_p)]
+
+
+def int32(value) -> int:
+    """The nearest 32-bit whole number, for counts of which those beyond mean no more than it (ctypes
+    would drop their upper bits)."""
+    return max(-2 ** 31, min(2 ** 31 - 1, operator.index(value)))
 
 
 TOKEN_SINK = ctypes.CFUNCTYPE(ctypes.c_int32, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32,

@@ -231,7 +231,8 @@ def kv_read(cache: KvCache, lengths, starts=None, rows=None, tokens=None, dtype=
 
 def _spec(q, kv_heads, window, sinks, scale):
     _, heads, dim = q.shape
-    return _lib.AttentionSpecStruct(heads, kv_heads, dim, _dtype("q", q), window, sinks,
+    return _lib.AttentionSpecStruct(heads, kv_heads, dim, _dtype("q", q),
+                                    _lib.int32(window), _lib.int32(sinks),
                                     dim ** -0.5 if scale is None and dim else scale or 0.0, 0)
 
 
@@ -313,7 +314,7 @@ def attention_packed(q, k, v, starts, window: int = 0, sinks: int = 0, scale=Non
 def _setting(device, rows, name, value, dtype):
     """(scalar, pointer) of a sampling setting given as a number or as one value per row."""
     if not hasattr(value, "data_ptr"):
-        return (int(value) if dtype == "torch.int32" else float(value)), None
+        return (_lib.int32(int(value)) if dtype == "torch.int32" else float(value)), None
     _on(device, name, value)
     if str(value.dtype) != dtype or tuple(value.shape) != (rows,) or not value.is_contiguous():
         raise IllegalArgumentException(f"{name} must be a number or a contiguous {dtype} vector "

@@ -123,8 +123,8 @@ class ModelSpec:
         s.weight_dtype = DTYPES[self.weight_dtype]
         s.kv_dtype = DTYPES[self.kv_dtype]
         s.max_rows = self.max_rows
-        s.attention_window = self.attention_window
-        s.attention_sinks = self.attention_sinks
+        s.attention_window = _lib.int32(self.attention_window)
+        s.attention_sinks = _lib.int32(self.attention_sinks)
         return s
 
 
@@ -346,7 +346,7 @@ class TextEngine:
                                            f"{list(u.shape)}", _lib.BST_INVALID)
         if not np.all((u >= 0) & (u < 1)):
             raise IllegalArgumentException("uniforms must lie in [0, 1)", _lib.BST_INVALID)
-        return arr, u, _lib.SamplingStruct(temperature, topP, minP, topK)
+        return arr, u, _lib.SamplingStruct(temperature, topP, minP, _lib.int32(topK))
 
     def seed(self, seed: int):
         self._call(self._lib.bst_seed(self._h, int(seed)))

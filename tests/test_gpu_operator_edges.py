@@ -220,3 +220,19 @@ def test_packed_outputs_stay_out_of_what_is_read(ops, dtype):
         assert torch.equal(wide.nan_to_num(), before.nan_to_num())
     ops.attention_packed(q, k, v, starts, window=50, out=out)
     assert torch.equal(out, want)
+
+
+def test_counts_beyond_32_bits_keep_their_meaning(ops):
+    torch = torch_()
+    rng = np.random.default_rng(9)
+    q, k, v = prompt(rng, 40, 2, 2, 64, "f32")
+    starts = ints([0, 40])
+    whole = ops.attention_packed(q, k, v, starts)
+    assert torch.equal(ops.attention_packed(q, k, v, starts, window=2 ** 32 + 5), whole)
+    cache = ops.KvCache.allocate(1, 2, 40, 64)
+    ops.kv_append(cache, k, v, ints([40]), starts=starts)
+    whole = ops.attention_cached(cache, q[39:], ints([40]))
+    assert torch.equal(ops.attention_cached(cache, q[39:], ints([40]), window=2 ** 32 + 5), whole)
+    logits = tensor(rng.standard_normal((50, 300)).astype(np.float32))
+    u = tensor(rng.random(50))
+    assert torch.equal(ops.sample_tokens(logits, u, top_k=2 ** 32 + 1), ops.sample_tokens(logits, u))

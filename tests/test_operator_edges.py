@@ -63,3 +63,20 @@ def test_outputs_do_not_overlap_what_is_read():
     assert packed(at + 2048, tokens=1, **{**slices, "out_stride": 769}) == _lib.BST_SHAPE
     assert cached(at) == cached(at + 2048) == _lib.BST_SHAPE           # q itself; behind it
     assert cached(at + 4) == cached(at, 260) == cached(at + 1024) == _lib.BST_INVALID
+
+
+@pytest.mark.parametrize("given,want", [(2 ** 32 + 5, 2 ** 31 - 1), (2 ** 31, 2 ** 31 - 1), (7, 7), (0, 0),
+                                        (-2 ** 32 + 5, -2 ** 31), (-1, -1)])
+def test_counts_beyond_32_bits_keep_their_meaning(given, want):
+    """A window or a top_k wider than anything, not what its lower 32 bits say."""
+    import torch
+
+    from basalt_b200 import ModelSpec, operators
+
+    operators._torch()
+    a = operators._spec(torch.zeros((1, 2, 64)), 1, given, given, None)
+    assert (a.window, a.sinks) == (want, want)
+    assert operators._setting(torch.device("cpu"), 1, "top_k", given, "torch.int32") == (want, None)
+    s = ModelSpec("padded_decoder", 10, 8, 64, 1, 2, 32, attention_window=given,
+                  attention_sinks=given).struct()
+    assert (s.attention_window, s.attention_sinks) == (want, want)
