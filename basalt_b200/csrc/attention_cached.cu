@@ -11,7 +11,7 @@
 // A nibble becomes an fp16 number without a conversion: its bits in the lowest mantissa bits, c or
 // 16 c, are the subnormals c 2^-24 and 16 c 2^-24. The other operand carries the 2^15 or 2^11 that
 // bring them near one: queries, normalised by a power of two per row so that nothing overflows, and
-// weights p step, normalised by the power of two above the largest step of the group so far (which
+// weights p step, normalised by a power of two above the largest of the group so far (which
 // moves as the maximum of the scores does, by rescaling). fp16 has 11 bits where bf16 has 8: one
 // term is more than bf16 outputs show, and two carry 22 bits for float32. float32 also takes
 // 1024 + c, or 1024 + 16 c, to c - 8 with one fp16 operation: sums of low and of step c would
@@ -33,9 +33,11 @@
 // and output in the workspace and a second kernel joins them.
 //
 // What that reaches: a bf16 cache is read at 0.92 of the copy rate (64 sequences of 2052 keys, 8 heads
-// of 128: 82 us). With codes instruction issue is the limit: 131 000 keys of 8 heads of 128 with 32
-// query heads take 63 us (2.6 TB/s), 24 sequences of 900 to 16 384 keys with 4 tokens each 175 us
-// (1.6 TB/s, for four times the products). One query a key head has a kernel of its own below.
+// of 128: 82 us). With codes a warp's own chain of unpacking, scaling and multiplying is the limit, at
+// the two warps a scheduler that registers leave (half of the issue slots are empty): 131 000 keys of 8
+// heads of 128 with 32 query heads take 64 us (2.6 TB/s), 24 sequences of 900 to 16 384 keys with 4
+// tokens each 183 us (1.5 TB/s, for four times the products; 174 with one normalisation of weight x step
+// for all queries of a lane, by the steps alone, which lost what a few large values hid). One query a key head has a kernel of its own below.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -53,6 +55,7 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kBlock = 16;   // keys a warp takes at a time
+constexpr float kLeastSteps = 0x1p114f;  // the normalisation of steps below 2^-100
 
 template <int STORAGE, int HD>
 struct Layout {
@@ -457,8 +460,11 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
     }
 
     // Output columns, and with codes the sums over keys of weight x low (column n: of group n) and the
-    // steps' normalisation: 2^14 over the power of two above a group's largest step so far.
-    float o[G * 4][4], lows[4] = {}, middles[G] = {}, top[R], total[R], shrink[G];
+    // normalisation of weight x step, a power of two for each query and group: 2^14 over the one above
+    // the largest step so far, or above 64 times the largest weight x step where that is less (steps of
+    // keys that a query does not see, or gives next to no weight, would leave the others no bits). It
+    // moves up again by what the maximum of the scores has grown since, in steps of 2^6 or more.
+    float o[G * 4][4], lows[4] = {}, middles[G] = {}, top[R], total[R], shrink[R][G], grown[R] = {};
     unsigned poison[R];  // groups in which a key that the query sees holds a NaN
 #pragma unroll
     for (int i = 0; i < G * 4; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
@@ -469,7 +475,10 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
         poison[r] = 0u;
     }
 #pragma unroll
-    for (int gr = 0; gr < G; ++gr) shrink[gr] = 0x1p114f;  // steps below 2^-100
+    for (int gr = 0; gr < G; ++gr) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) shrink[r][gr] = kLeastSteps;
+    }
     // The key rows of this lane's score columns 2 t and 2 t + 1, and of the key that it loads.
     const int key_row[2] = {row_of_column<STORAGE, HD>(2 * t), row_of_column<STORAGE, HD>(2 * t + 1)};
     const int load_row = row_of_column<STORAGE, HD>(g);
@@ -636,6 +645,7 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
             block_top = fmaxf(block_top, __shfl_xor_sync(kFull, block_top, 2));
             const bool up = block_top > top[r];
             keep[r] = up ? (top[r] == -INFINITY ? 0.0f : exp2_fast(top[r] - block_top)) : 1.0f;
+            if constexpr (L::kCodes) grown[r] += up && top[r] != -INFINITY ? block_top - top[r] : 0.0f;
             top[r] = up ? block_top : top[r];
             grows |= up;
         }
@@ -651,6 +661,32 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
             for (int i = 0; i < G * 4; ++i) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) o[i][j] *= keep[R == 2 ? j / 2 : 0];
+            }
+            if constexpr (L::kCodes) {
+                bool far = false;
+#pragma unroll
+                for (int r = 0; r < R; ++r) far |= grown[r] >= 6.0f;
+                if (__any_sync(kFull, far)) {
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        if (grown[r] < 6.0f) continue;
+                        const uint32_t by_most = min(static_cast<int>(grown[r]), 126);
+                        grown[r] = 0.0f;
+#pragma unroll
+                        for (int gr = 0; gr < G; ++gr) {
+                            const uint32_t room = (__float_as_uint(kLeastSteps) - __float_as_uint(shrink[r][gr])) >> 23;
+                            const float by = __uint_as_float((127u + min(by_most, room)) << 23);
+                            shrink[r][gr] *= by;
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    if (R == 1 || e / 2 == r) o[4 * gr + j][e] *= by;
+                                }
+                            }
+                        }
+                    }
+                }
             }
         }
         float p[R][2][2];
@@ -721,25 +757,39 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
                 const uint32_t most = __vimax3_u16x2(__vmaxu2(sv[0][0][gr], sv[0][1][gr]),
                                                      sv[1][0][gr], sv[1][1][gr]);
                 largest[gr] = low_of(most);
-                above_any |= largest[gr] * shrink[gr] > 0x1p14f;
+#pragma unroll
+                for (int r = 0; r < R; ++r) above_any |= largest[gr] * shrink[r][gr] > 0x1p14f;
             }
             if (__any_sync(kFull, above_any)) {
                 // A step above its group's power of two: the next one, for a row's lanes (each has seen
-                // four of the keys). A row that sees no larger step, or no key at all, stays.
+                // four of the keys), if the row gives it any weight.
 #pragma unroll
                 for (int gr = 0; gr < G; ++gr) {
-                    float most = fmaxf(largest[gr], __shfl_xor_sync(kFull, largest[gr], 1));
-                    most = fmaxf(most, __shfl_xor_sync(kFull, most, 2));
-                    const uint32_t above = (__float_as_uint(most) & 0x7f800000u) + 0x00800000u;
-                    const float next = most * shrink[gr] > 0x1p14f
-                                           ? __uint_as_float((268u << 23) - above)  // 2^14 / above
-                                           : shrink[gr];
-                    const float by = next / shrink[gr];
-                    shrink[gr] = next;
+                    float step = fmaxf(largest[gr], __shfl_xor_sync(kFull, largest[gr], 1));
+                    step = fmaxf(step, __shfl_xor_sync(kFull, step, 2));
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
+                    for (int r = 0; r < R; ++r) {
+                        float most = 0.0f;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) o[4 * gr + j][e] *= by;
+                        for (int i = 0; i < 4; ++i) {
+                            most = fmaxf(most, p[r][i / 2][i % 2] * low_of(sv[i / 2][i % 2][gr]));
+                        }
+                        most = fmaxf(most, __shfl_xor_sync(kFull, most, 1));
+                        most = fmaxf(most, __shfl_xor_sync(kFull, most, 2));
+                        most = fminf(64.0f * most, step);
+                        const uint32_t above = (__float_as_uint(most) & 0x7f800000u) + 0x00800000u;
+                        const float next = most * shrink[r][gr] > 0x1p14f
+                                               ? __uint_as_float((268u << 23) - above)  // 2^14 / above
+                                               : shrink[r][gr];
+                        const float by = next / shrink[r][gr];
+                        shrink[r][gr] = next;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                if (R == 1 || e / 2 == r) o[4 * gr + j][e] *= by;
+                            }
+                        }
                     }
                 }
             }
@@ -750,10 +800,11 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
                 uint32_t ps[R][2][kHalf], x[2];
 #pragma unroll
                 for (int nb = 0; nb < 2; ++nb) {
-                    const float step0 = steps[nb][0] * shrink[gr], step1 = steps[nb][1] * shrink[gr];
+                    // The weight first: zero times a step that is far above the normalisation is zero.
 #pragma unroll
                     for (int r = 0; r < R; ++r) {
-                        half_terms_of<kHalf>(p[r][nb][0] * step0, p[r][nb][1] * step1, ps[r][nb]);
+                        half_terms_of<kHalf>(p[r][nb][0] * shrink[r][gr] * steps[nb][0],
+                                             p[r][nb][1] * shrink[r][gr] * steps[nb][1], ps[r][nb]);
                     }
                     x[nb] = __byte_perm(wv[nb][0][gr / 2], wv[nb][1][gr / 2], gr & 1 ? 0x7632 : 0x5410);
                 }
@@ -833,7 +884,7 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
                     low = __shfl_sync(kFull, entry<R, kTerms>(lows, r, gr & 1), (lane & ~3) | (gr >> 1));
                     if ((poison[r] >> gr) & 1u) low = NAN;
                 }
-                by = 1.0f / shrink[gr];
+                by = 1.0f / shrink[r][gr];
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {

@@ -236,3 +236,49 @@ def test_counts_beyond_32_bits_keep_their_meaning(ops):
     logits = tensor(rng.standard_normal((50, 300)).astype(np.float32))
     u = tensor(rng.random(50))
     assert torch.equal(ops.sample_tokens(logits, u, top_k=2 ** 32 + 1), ops.sample_tokens(logits, u))
+
+
+@pytest.mark.parametrize("where", ["hidden", "light", "early"])
+@pytest.mark.parametrize("ratio", [2.0 ** 10, 2.0 ** 20, 2.0 ** 40, 2.0 ** 60])
+@pytest.mark.parametrize("heads,kv_heads,tokens", [(2, 2, 4), (6, 2, 1), (8, 2, 4), (16, 2, 3), (2, 2, 1),
+                                                   (24, 2, 1)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_large_values_without_weight_leave_the_others_theirs(ops, dtype, heads, kv_heads, tokens, ratio,
+                                                             where):
+    """Values far above the others at a key that only the last token sees, at one whose score is far
+    below the others', or in a first block of keys of which that holds. The bound counts every value
+    by its weight: v below is the sum of weight |v|, to which the products of weight and step add
+    n 2^-24 of it (they are held to 2^-39 of a power of two that is at most 2^13 times the largest of
+    them, and multiply codes of up to 15)."""
+    rng = np.random.default_rng(heads + tokens)
+    L, dim = 150, 64
+    k = rng.standard_normal((L, kv_heads, dim)).astype(np.float32)
+    v = rng.standard_normal((L, kv_heads, dim)).astype(np.float32)
+    q = rng.standard_normal((tokens, heads, dim)).astype(np.float32)
+    keys = {"hidden": [L - 1], "light": [0, 50, 120], "early": list(range(16))}[where]
+    v[keys] *= np.float32(ratio)
+    if where != "hidden":
+        q[..., 0], k[:, :, 0] = 12.0, 0.0
+        k[keys, :, 0] = -45.0 * math.log2(ratio) / 40       # weights of about 2^-1.3 / ratio^2.4
+    cache, starts = ops.KvCache.allocate(1, kv_heads, L + 10, dim), ints([0, L])
+    ops.kv_append(cache, tensor(k), tensor(v), ints([L]), starts=starts)
+    k, v = (host(t) for t in ops.kv_read(cache, ints([L]), starts=starts, tokens=L))
+    q = tensor(q, dtype)
+    got = host(ops.attention_cached(cache, q, ints([L]),
+                                    starts=ints([0, tokens]) if tokens > 1 else None))
+    qh = host(q)
+    want, size, _ = attend(qh, k, v, L - tokens)
+    for i in range(tokens):
+        n = L - tokens + i + 1
+        for h in range(heads):
+            kk, vv = (x[:n, h * kv_heads // heads] for x in (k, v))
+            s = kk @ qh[i, h] / 8
+            p = np.exp(s - s.max())
+            weighed = (p / p.sum()) @ np.abs(vv).max(1)
+            if where == "hidden" and i < tokens - 1:
+                assert weighed < 4
+            # the scores that matter decide their error
+            most = (np.abs(kk) @ np.abs(qh[i, h]) / 8)[p > 1e-3].max()
+            tol = bound(np.array([most]), dim, n, weighed, want[i, h], dtype) + n * 2.0 ** -24 * weighed
+            assert np.all(np.abs(got[i, h] - want[i, h]) <= tol), (i, h, np.abs(got[i, h] - want[i, h]).max(),
+                                                                   tol.min())
