@@ -21,6 +21,7 @@ from . import _lib
 from .text_engine import (BasaltShapeException, BasaltUnsupportedOperationException,
                           IllegalArgumentException, _raise)
 
+_KEPT = 256   # workspace sizes that a cache keeps: batches come in ever new counts
 _CODES = {}   # torch dtype -> BST_DTYPE_*, filled with the module below
 _module = None
 _raw_stream = None   # device index -> its current cudaStream_t
@@ -278,6 +279,8 @@ def attention_cached(cache: KvCache, q, lengths, starts=None, rows=None, window:
     if needed is None:
         size = ctypes.c_int64(0)
         _raise(lib.bst_attention_cached_workspace(cache._ref, s, a, size))
+        if len(cache._sizes) >= _KEPT:
+            cache._sizes.clear()
         needed = cache._sizes[key] = size.value
     pointer, room, workspace = _workspace(device, needed, workspace, stream)
     _raise(lib.bst_attention_cached(device.index, _stream(device, stream), cache._ref, s, a,

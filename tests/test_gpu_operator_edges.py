@@ -282,3 +282,12 @@ def test_large_values_without_weight_leave_the_others_theirs(ops, dtype, heads, 
             tol = bound(np.array([most]), dim, n, weighed, want[i, h], dtype) + n * 2.0 ** -24 * weighed
             assert np.all(np.abs(got[i, h] - want[i, h]) <= tol), (i, h, np.abs(got[i, h] - want[i, h]).max(),
                                                                    tol.min())
+
+
+def test_a_cache_keeps_few_sizes(ops):
+    torch = torch_()
+    cache = ops.KvCache.allocate(1, 1, 2000, 32)
+    q = torch.zeros((1, 1, 32), device="cuda")
+    for window in range(1, 1001):
+        ops.attention_cached(cache, q, ints([0]), window=window)
+    assert len(cache._sizes) <= 256
