@@ -1,8 +1,9 @@
 """The serving operators of libbasalt_cuda.so on torch tensors: a cache of keys and values held in
 4 bits, bf16 or float32, attention over it, attention over packed prompts, and drawing tokens.
 
-Tensors stay on the GPU: every call takes their device pointers, queues its kernels on ``stream``
-(torch's current stream of the tensors' device by default) and returns without waiting. Outputs and
+Tensors stay on the GPU: every call takes their device pointers, queues its kernels on ``stream`` (a
+torch.cuda.Stream or a cudaStream_t as a number; torch's current stream of the tensors' device by
+default) and returns without waiting. Outputs and
 workspaces come from torch's allocator, for that stream of that device, unless given, so calls can be
 captured into a CUDA graph (call once before the capture, which loads the kernels). ``include/basalt_cuda.h`` has
 the operators' definitions; a rejected argument raises the exception of its status.
@@ -99,6 +100,16 @@ def _empty(shape, dtype, device, stream):
         return _module.empty(shape, dtype=dtype, device=device)
 
 
+def _given(device, stream):
+    """The pointer of a given stream (a torch.cuda.Stream of the device, or the pointer itself); None
+    for none."""
+    pointer = getattr(stream, "cuda_stream", stream)
+    if pointer is not stream and stream.device != device:
+        raise IllegalArgumentException(f"stream is on {stream.device}, expected {device}",
+                                       _lib.BST_INVALID)
+    return pointer
+
+
 def _stream(device, stream):
     if stream is not None:
         return stream
@@ -188,6 +199,7 @@ def kv_append(cache: KvCache, k, v, lengths, starts=None, rows=None, stream=None
     """Stores the batch's keys and values ([tokens, kv_heads, head_dim], float32 or bfloat16) in
     their slots of ``cache``."""
     device = cache.device
+    stream = _given(device, stream)
     k_stride = _packed(device, "k", k, cache.kv_heads, cache.head_dim)
     v_stride = _packed(device, "v", v, cache.kv_heads, cache.head_dim)
     if k.dtype != v.dtype or k.shape[0] != v.shape[0]:
@@ -204,6 +216,7 @@ def kv_read(cache: KvCache, lengths, starts=None, rows=None, tokens=None, dtype=
     is the packed count (the number of sequences without ``starts``), ``out`` a pair of tensors to
     fill; otherwise new ones of ``dtype`` (float32)."""
     device = cache.device
+    stream = _given(device, stream)
     if out is None:
         if tokens is None:
             if starts is not None:
@@ -269,6 +282,7 @@ def attention_cached(cache: KvCache, q, lengths, starts=None, rows=None, window:
     keys (0: all) and the first ``sinks``. ``scale`` is 1 / sqrt(head_dim) by default. ``out`` may be
     ``q`` itself."""
     device = cache.device
+    stream = _given(device, stream)
     q_stride = _packed(device, "q", q, None, cache.head_dim)
     out, out_stride = _out(device, q, out, stream)
     s = _sequences(device, q.shape[0], lengths, starts, rows)
@@ -295,6 +309,7 @@ def attention_packed(q, k, v, starts, window: int = 0, sinks: int = 0, scale=Non
     head_dim], k and v [tokens, kv_heads, head_dim], all of one type. ``out`` must not overlap them."""
     _torch()
     device = q.device
+    stream = _given(device, stream)
     _on(device, "q", q)
     q_stride = _packed(device, "q", q)
     k_stride = _packed(device, "k", k, None, q.shape[2])
@@ -332,6 +347,7 @@ def sample_tokens(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0
     int32, on the device). Rows with nothing to draw give -1."""
     _torch()
     device = logits.device
+    stream = _given(device, stream)
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise BasaltShapeException("logits must be [rows, vocabulary] with contiguous rows",
                                    _lib.BST_SHAPE)

@@ -291,3 +291,35 @@ def test_a_cache_keeps_few_sizes(ops):
     for window in range(1, 1001):
         ops.attention_cached(cache, q, ints([0]), window=window)
     assert len(cache._sizes) <= 256
+
+
+@pytest.mark.parametrize("form", ["object", "pointer"])
+def test_streams_are_given_as_objects_or_pointers(ops, form):
+    """Every call on a stream that waits for nothing of the current one but what it needs."""
+    from basalt_b200 import IllegalArgumentException
+
+    torch = torch_()
+    rng = np.random.default_rng(6)
+    x = prompt(rng, 70, 2, 2, 64, "f32")
+    starts, n, one = ints([0, 70]), ints([70]), x[0][69:]
+    logits, u = tensor(rng.standard_normal((5, 100)).astype(np.float32)), tensor(rng.random(5))
+
+    def calls(**on):
+        cache = ops.KvCache.allocate(1, 2, 70, 64)
+        torch.cuda.synchronize()
+        ops.kv_append(cache, x[1], x[2], n, starts=starts, **on)
+        return (*ops.kv_read(cache, n, starts=starts, tokens=70, **on),
+                ops.attention_cached(cache, one, n, **on), ops.attention_packed(*x, starts, **on),
+                ops.sample_tokens(logits, u, **on))
+
+    stream = torch.cuda.Stream()
+    want = calls()
+    got = calls(stream=stream if form == "object" else stream.cuda_stream)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+    class Elsewhere:
+        device, cuda_stream = torch.device("cuda", 7), stream.cuda_stream
+
+    with pytest.raises(IllegalArgumentException, match="stream is on cuda:7"):
+        calls(stream=Elsewhere())
