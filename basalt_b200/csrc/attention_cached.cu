@@ -289,6 +289,41 @@ __device__ __forceinline__ float entry(const float (&c)[4], int r, int e) {
     return c[e] + c[2 + e];
 }
 
+// The sums of one query over the keys of blocks [b0, b1) of an unquantised cache, plainly, by one warp:
+// [HD outputs, maximum, sum] as k_cached leaves them.
+template <typename T, typename S, int HD>
+__device__ __noinline__ void attend_plainly(const S* k, const S* v, const T* q, float scale,
+                                            const Visible& seen, int b0, int b1, float* to) {
+    constexpr int C = HD / 32;
+    const int lane = threadIdx.x & 31;
+    float x[C], value[C] = {}, top = -INFINITY, total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < C; ++i) x[i] = to_f(q[lane + 32 * i]);
+    for (int block = b0; block < b1; ++block) {
+        const int key0 = seen.key(block);
+        for (int key = key0; key < key0 + kBlock; ++key) {
+            if (!seen.holds(key)) continue;
+            const int64_t at = static_cast<int64_t>(key) * HD + lane;
+            float dot = 0.0f;
+#pragma unroll
+            for (int i = 0; i < C; ++i) dot = fmaf(x[i], to_f(k[at + 32 * i]), dot);
+            const float s = warp_sum(dot) * scale, most = fmaxf(top, s);
+            const float keep = top == -INFINITY ? 0.0f : exp2f(top - most);
+            const float p = s == -INFINITY ? 0.0f : exp2f(s - most);  // a NaN stays one
+            total = fmaf(total, keep, p);
+#pragma unroll
+            for (int i = 0; i < C; ++i) value[i] = fmaf(p, to_f(v[at + 32 * i]), value[i] * keep);
+            top = most;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < C; ++i) to[lane + 32 * i] = value[i];
+    if (lane == 0) {
+        to[HD] = top;
+        to[HD + 1] = total;
+    }
+}
+
 // ROWS queries a tile: 8, or 16 for bf16 batches that have more than eight to a key head, so that
 // unpacking the codes, which bounds the kernel, is shared by twice as many.
 template <typename T, int STORAGE, int HD, int ROWS>
@@ -863,6 +898,7 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
 
     // The warps' results: [warp][row][HD outputs, maximum, sum].
     float* merge = reinterpret_cast<float*>(smem);
+    float largest_result = 0.0f;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         total[r] += __shfl_xor_sync(kFull, total[r], 1);
@@ -893,16 +929,38 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
                 constexpr int N = L::kCodes ? kHalf : kTerms;
                 // Nibbles 0 and 2 count 2^-24, 1 and 3 16 times that.
                 const float unit = !L::kCodes || kExact ? 1.0f : (j & 1 ? 0x1p20f : 0x1p24f);
-                mine[c0] = fmaf(entry<R, N>(o[4 * gr + j], r, 0) * unit, by, low);
-                mine[c0 + (L::kCodes ? 4 : 1)] = fmaf(entry<R, N>(o[4 * gr + j], r, 1) * unit, by, low);
+                const float y0 = fmaf(entry<R, N>(o[4 * gr + j], r, 0) * unit, by, low);
+                const float y1 = fmaf(entry<R, N>(o[4 * gr + j], r, 1) * unit, by, low);
+                mine[c0] = y0;
+                mine[c0 + (L::kCodes ? 4 : 1)] = y1;
+                largest_result = max_nan(largest_result, max_nan(fabsf(y0), fabsf(y1)));
             }
         }
         if (t == 0) {
             mine[HD] = top[r];
             mine[HD + 1] = total[r];
         }
+        largest_result = max_nan(largest_result, total[r]);
     }
-    __syncthreads();
+    if constexpr (L::kCodes) {
+        __syncthreads();
+    } else if (__syncthreads_or(!(largest_result <= FLT_MAX))) {
+        // The terms of an infinity, and of a float that bf16 rounds to one, leave NaN where the formula
+        // may have a weight of zero, an infinity or a number: the CTA's sums again, a warp a row.
+        using S = typename std::conditional<STORAGE == BST_DTYPE_F32, float, __nv_bfloat16>::type;
+        for (int r = warp; r < rows; r += kWarps) {
+            // A sequence has one token here.
+            const T* src = q + tile.first * q_stride + (kvh * group + tile.r0 + r) * HD;
+            attend_plainly<T, S, HD>(reinterpret_cast<const S*>(kb), reinterpret_cast<const S*>(vb), src,
+                                     a.scale * kLog2e, seen, b0, b1, merge + r * (HD + 2));
+            for (int w = 1; w < kWarps && lane == 0; ++w) {
+                float* none = merge + (w * ROWS + r) * (HD + 2);
+                none[HD] = -INFINITY;
+                none[HD + 1] = 0.0f;
+            }
+        }
+        __syncthreads();
+    }
     for (int i = threadIdx.x; i < rows * HD; i += kThreads) {
         const int r = i / HD, ch = i % HD;
         float m = -INFINITY;

@@ -323,3 +323,40 @@ def test_streams_are_given_as_objects_or_pointers(ops, form):
 
     with pytest.raises(IllegalArgumentException, match="stream is on cuda:7"):
         calls(stream=Elsewhere())
+
+
+@pytest.mark.parametrize("which,value", [(0, math.inf), (0, -math.inf), (1, math.inf), (1, -math.inf),
+                                         (0, -3.4025e38), (1, 3.4028e38), (0, math.nan), (1, math.nan)])
+@pytest.mark.parametrize("group,dim,window", [(1, 64, 0), (3, 32, 0), (20, 128, 60)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("storage", ["f32", "bf16"])
+def test_infinities_of_a_cache_count_as_the_formula_has_them(ops, storage, dtype, group, dim, window,
+                                                             which, value):
+    """Seen by the first two sequences (one of them split over its keys), not by the others. The finite
+    ones are floats that bf16 terms round to infinity."""
+    rng = np.random.default_rng(dim + which)
+    S, slots, kv_heads = 4, 3000, 2
+    lengths = [3000, 1500, 1400, 0]
+    x = rng.standard_normal((2, S, slots, kv_heads, dim)).astype(np.float32)
+    place = 1480 if window else 1400
+    if window:
+        lengths[0] = 1500
+    x[which, :, place, 1, 3] = value
+    cache, starts = ops.KvCache.allocate(S, kv_heads, slots, dim, storage), ints(np.arange(S + 1) * slots)
+    ops.kv_append(cache, *(tensor(t.reshape(-1, kv_heads, dim)) for t in x), ints([slots] * S), starts=starts)
+    q = rng.standard_normal((S, kv_heads * group, dim)).astype(np.float32)
+    q[..., 3] = 0.5 + 0.1 * np.abs(q[..., 3])
+    q = tensor(q, dtype)
+    got = host(ops.attention_cached(cache, q, ints(lengths), window=window, sinks=2))
+    kv = [host(t).reshape(S, slots, kv_heads, dim) for t in (cache.k.transpose(1, 2), cache.v.transpose(1, 2))]
+    for s, n in enumerate(lengths):
+        if n == 0:
+            assert (got[s] == 0).all()
+            continue
+        k, v = (t[s, :n] for t in kv)
+        qs = host(q)[s:s + 1]
+        want, size, most = attend(qs, k, v, n - 1, window, 2)
+        size = attend(qs, np.where(np.abs(k) < 1e38, k, 0), v, n - 1, window, 2)[1]
+        check(got[s:s + 1], want, size, most, dim, n, dtype)
+        if s == 2:
+            assert np.isfinite(got[s]).all()
