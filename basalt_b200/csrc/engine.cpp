@@ -705,11 +705,12 @@ class Engine {
                bool presplit = false, bool presplit_xs = false);
     // x += X W^T + bias (a residual projection) followed by the LayerNorm `next` of the new x.
     // On the tensor-core path with a K split, one fused fix-up kernel does both and leaves the
-    // normalised rows as operand planes in ws.xs_* (*normalised = true); otherwise it runs the
-    // plain residual projection and the caller applies `next` itself.
+    // normalised rows as operand planes in ws.xs_* (*normalised = true); otherwise, or where the
+    // projection that follows (`to`, to_n columns) takes no planes, it runs the plain residual
+    // projection and the caller applies `next` itself.
     int residual_ln(const float* x, int ldx, const Matrix& m, const float* bias, int M, int N,
-                    int K, bool presplit, const bst::LnArgs& next, const char* what,
-                    bool* normalised);
+                    int K, bool presplit, const bst::LnArgs& next, const Matrix& to, int to_n,
+                    const char* what, bool* normalised);
     // Whether linear() takes the tensor-core path for this shape, and the operand planes a
     // producer should write for it (into ws.ys_*; none when the GEMV path consumes fp32).
     bool linear_on_tc(const Matrix& m, int M, int N, int K) const;
@@ -1253,8 +1254,8 @@ bst::PlaneOut Engine::planes_for(const Matrix& m, int M, int N, int K) const {
 }
 
 int Engine::residual_ln(const float* x, int ldx, const Matrix& m, const float* bias, int M, int N,
-                        int K, bool presplit, const bst::LnArgs& next, const char* what,
-                        bool* normalised) {
+                        int K, bool presplit, const bst::LnArgs& next, const Matrix& to, int to_n,
+                        const char* what, bool* normalised) {
     *normalised = false;
     EpiArgs res;
     res.out = ws.x;
@@ -1262,7 +1263,7 @@ int Engine::residual_ln(const float* x, int ldx, const Matrix& m, const float* b
     const int splits = linear_on_tc(m, M, N, K)
                            ? bst::tc_plan(M, N, K, wbf16, bst::tc_part_bytes_max(), nullptr)
                            : 1;
-    if (splits <= 1 || N > 1024 || N != d) {
+    if (splits <= 1 || N > 1024 || N != d || !linear_on_tc(to, M, to_n, N)) {
         return linear(x, ldx, m, bias, M, N, K, Epi::kResidual, res, what, nullptr, presplit);
     }
     const double plane = static_cast<double>(bst::tc_split_bytes(M, K, wbf16));
@@ -1806,7 +1807,7 @@ int Engine::decode_after_qkv(int l, int R, const int* rowmap, const int* lengths
     if (st) return st;
     const bst::LnArgs ln2{lw.ln2_g, lw.ln2_b, kLayerNormEps};
     bool ffn_in_normalised = false;
-    st = residual_ln(ws.att, d, lw.wo, lw.bo, R, d, d, att_planes.planes != 0, ln2,
+    st = residual_ln(ws.att, d, lw.wo, lw.bo, R, d, d, att_planes.planes != 0, ln2, lw.w1, F,
                      "output projection", &ffn_in_normalised);
     if (st) return st;
     EpiArgs act;
@@ -1821,7 +1822,8 @@ int Engine::decode_after_qkv(int l, int R, const int* rowmap, const int* lengths
     const bst::LnArgs next = l + 1 < L ? bst::LnArgs{layers[l + 1].ln1_g, layers[l + 1].ln1_b,
                                                      kLayerNormEps}
                                        : bst::LnArgs{lnf_g, lnf_b, kLayerNormEps};
-    return residual_ln(ws.ffn, F, lw.w2, lw.b2, R, d, F, act.split.planes != 0, next, "ffn2",
+    return residual_ln(ws.ffn, F, lw.w2, lw.b2, R, d, F, act.split.planes != 0, next,
+                       l + 1 < L ? layers[l + 1].wqkv : head_w, l + 1 < L ? 3 * d : V, "ffn2",
                        x_normalised);
 }
 
