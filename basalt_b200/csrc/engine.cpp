@@ -1607,6 +1607,7 @@ int Engine::enqueue_decode(int R, const int* rowmap, const std::vector<int>& len
             w.x += static_cast<size_t>(r0) * d;
             w.q += static_cast<size_t>(r0) * d;
             w.att += static_cast<size_t>(r0) * d;
+            w.h += static_cast<size_t>(r0) * d;
             w.ffn += static_cast<size_t>(r0) * F;
             w.slot += r0;
             w.attn_tickets += static_cast<size_t>(r0) * H;

@@ -27,3 +27,12 @@ def test_split_projections_feed_ones_without_operand_planes(runtime, tmp_path, v
                                                             rows, kw):
     check(runtime, tmp_path / "w.bin", ModelSpec("padded_decoder", vocabulary, 40, dim, 2, heads, hidden,
                                                  **kw), rows, 6, 8)
+
+
+@pytest.mark.parametrize("vocabulary,dim,heads,hidden", [(5, 128, 2, 64), (15, 96, 3, 48), (5, 64, 1, 24),
+                                                         (97, 64, 2, 8), (9, 256, 4, 8)])
+@pytest.mark.parametrize("rows", [18, 33, 200])
+def test_rows_in_lanes_keep_their_own_normalised_inputs(runtime, tmp_path, vocabulary, dim, heads, hidden,
+                                                        rows):
+    check(runtime, tmp_path / "w.bin", ModelSpec("padded_decoder", vocabulary, 40, dim, 2, heads, hidden),
+          rows, 6, 8)
