@@ -360,3 +360,28 @@ def test_infinities_of_a_cache_count_as_the_formula_has_them(ops, storage, dtype
         check(got[s:s + 1], want, size, most, dim, n, dtype)
         if s == 2:
             assert np.isfinite(got[s]).all()
+
+
+@pytest.mark.parametrize("group,kv_heads,counts", [(5, 1, [40, 3, 1, 290]), (12, 2, [65, 130]),
+                                                   (300, 1, [5, 1, 3]), (70, 2, [9, 4])])
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_many_heads_to_a_key_head(ops, dtype, dim, group, kv_heads, counts):
+    """Groups that are no powers of two, and tokens whose heads span several tiles of rows: in prompts,
+    and as several new tokens over a 4-bit cache."""
+    rng = np.random.default_rng(group + dim)
+    starts = np.concatenate([[0], np.cumsum(counts)])
+    q, k, v = prompt(rng, starts[-1], group * kv_heads, kv_heads, dim, dtype)
+    got = host(ops.attention_packed(q, k, v, ints(starts), window=29, sinks=2, scale=0.2))
+    for a, b in zip(starts, starts[1:]):
+        want, size, most = attend(*[host(t)[a:b] for t in (q, k, v)], 0, 29, 2, 0.2)
+        check(got[a:b], want, size, np.full_like(most, most.max()), dim, b - a, dtype)
+    S, slots = len(counts), 400
+    cache = ops.KvCache.allocate(S, kv_heads, slots, dim)
+    ops.kv_append(cache, k, v, ints(counts), starts=ints(starts))
+    k, v = (host(t) for t in ops.kv_read(cache, ints(counts), starts=ints(starts), tokens=int(starts[-1])))
+    got = host(ops.attention_cached(cache, q, ints(counts), starts=ints(starts), window=29, sinks=2,
+                                    scale=0.2))
+    for a, b in zip(starts, starts[1:]):
+        want, size, most = attend(host(q)[a:b], k[a:b], v[a:b], 0, 29, 2, 0.2)
+        check(got[a:b], want, size, np.full_like(most, most.max()), dim, b - a, dtype)
