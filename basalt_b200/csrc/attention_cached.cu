@@ -32,12 +32,14 @@
 // fragments' key columns 2 t and 2 t + 1 of either half of the 16. Splits leave their maximum, sum
 // and output in the workspace and a second kernel joins them.
 //
-// What that reaches: a bf16 cache is read at 0.92 of the copy rate (64 sequences of 2052 keys, 8 heads
-// of 128: 82 us). With codes a warp's own chain of unpacking, scaling and multiplying is the limit, at
+// What that reaches: a bf16 cache is read at 0.90 of the copy rate (64 sequences of 2052 keys, 8 heads
+// of 128: 84 us), a float32 one, whose entries are split in three terms by every warp, at half of it (the
+// same in float32: 283 us). With codes a warp's own chain of unpacking, scaling and multiplying is the limit, at
 // the two warps a scheduler that registers leave (half of the issue slots are empty): 131 000 keys of 8
 // heads of 128 with 32 query heads take 64 us (2.6 TB/s), 24 sequences of 900 to 16 384 keys with 4
 // tokens each 183 us (1.5 TB/s, for four times the products; 174 with one normalisation of weight x step
-// for all queries of a lane, by the steps alone, which lost what a few large values hid). One query a key head has a kernel of its own below.
+// for all queries of a lane, by the steps alone, which lost what a few large values hid). One query a
+// key head has a kernel of its own below.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -1009,8 +1011,9 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
 // keys' behind them.
 // A query sees all keys of two ranges, sinks and window, so nothing inside them is masked; lanes behind
 // the end take the last key with a weight of zero.
-// Bound by instruction issue: 256 sequences of 257 to 512 keys of eight heads of 64 take 31 us where the
-// kernel above took 45 (64 MB, 2.1 TB/s); 64 sequences of 4000 keys of 16 heads 110 (153); 60 000 keys of
+// 256 sequences of 257 to 512 keys of eight heads of 64 take 32 us where the kernel above took 45 (64 MB,
+// 2.0 TB/s), in 1.4 waves of CTAs of unequal length, five warp instructions a value at 53-55 % of the issue
+// slots; 64 sequences of 4000 keys of 16 heads 110 (153); 60 000 keys of
 // 32 heads 51 (82). bf16, which is cheaper above, gains as well: 31 (45), 110 (134), 51 (72). Scaling in
 // the lanes that hold the words, every scale loaded by eight of them, took 36 us for the first.
 constexpr int kOneWarps = 2, kOneCtas = 20 / kOneWarps;  // warps a CTA, CTAs an SM

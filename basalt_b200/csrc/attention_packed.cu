@@ -63,7 +63,7 @@ struct KeyTiles {
 // What bounds it: per 128 keys the exponentials (32 768 at 16 a cycle, 2048 cycles) beside the
 // products (4 x 128 x 128 x 128 multiply-adds, 2048 cycles at the nominal rate; the scores' half
 // takes half as long again, because 64 columns a product read Q from shared memory twice as often).
-// 8192 tokens of 16 heads over 4 of 128, window 1024: 113 us, 0.35 of the measured bf16 rate, in four
+// 8192 tokens of 16 heads over 4 of 128, window 1024: 115 us, 0.34 of the measured bf16 rate, in four
 // waves of 18 tiles a CTA, a third of whose time is its beginning and end. (CTAs of 128 rows, two an SM
 // with half of TMEM each, took 121: the rings then hold half as many tiles.)
 //
@@ -555,13 +555,13 @@ __device__ __forceinline__ void attend_query(const T* q, const T* k, int64_t k_s
 // values pass through shared memory in tiles, double-buffered with cp.async. float32 operands are
 // split in two tf32 parts, x = h + l with h the upper 10 mantissa bits, and multiplied as
 // h h + h l + l h (2^-21 of a product is left out); bf16 ones are tf32 numbers as they are, their
-// weights rounded to tf32. A CTA whose outputs are not all finite has them computed again. The tensor cores cut sums where float32 additions round: sums of a whole
-// row came out 3e-6 low, so products are summed 32 channels, or a tile of keys, at a time (the small
-// ones apart) and added up in float32. Splitting happens in registers after the load, so the tiles stay float32.
+// weights rounded to tf32. A CTA whose outputs are not all finite has them computed again. The tensor
+// cores cut sums where float32 additions round: sums of a whole row came out 3e-6 low, so products are
+// summed 32 channels, or a tile of keys, at a time (the small ones apart) and added up in float32. Splitting happens in registers after the load, so the tiles stay float32.
 // Rows of keys are padded to HD + 8 floats and of values to HD + 4, which keeps the fragments' reads
 // (pairs of channels of eight keys; one channel of four keys two apart) free of bank conflicts.
 // Bound by the latency between a warp's own instructions at 12 warps an SM (24 float32 sequences of up to
-// 700 tokens, 8 heads of 64, window 256: 138 us, tensor cores 43 % busy, issue 53 %). Keys and values
+// 700 tokens, 8 heads of 64, window 256: 140 us, tensor cores 42 % busy, issue 53 %). Keys and values
 // split once a tile in shared memory instead of by every warp are 15 % fewer instructions and no faster.
 
 template <typename T, int HD>

@@ -15,7 +15,9 @@
 // 65 536 tokens of 8 heads of 64 float32 channels (310 MB either way, 47 us at the copy rate): reading
 // takes 58 us, bound by the stores; storing 75 us, bound by instruction issue (30 a value at first, 20
 // with codes rounded and packed as floats and each lane carrying one group's extremes to the end),
-// with a lane's next values on their way while it works on the last.
+// with a lane's next values on their way while it works on the last. bf16 values take 123 us: they lie
+// on the middle between two codes far more often (0.27 % against 0.002 % of normal ones within 1e-5 of
+// it), so that every fourth warp meets the double quotient.
 
 #include <cuda_bf16.h>
 

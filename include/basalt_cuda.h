@@ -332,7 +332,12 @@ int32_t bst_kv_read(int32_t device, void* stream, const bst_kv_cache* cache,
 /* heads must be a multiple of kv_heads: query head h reads key head h * kv_heads / heads. A query
  * at position i sees key j when j <= i and (window == 0, or i - j < window, or j < sinks): the
  * last `window` tokens and the first `sinks`. A query that sees nothing gives zeros. dtype is the
- * type of q and out (and of packed k and v); scores, weights and sums are float32. */
+ * type of q and out (and of packed k and v). Scores, their maximum, the sums of weights and the
+ * outputs' sums are float32, and so are the weights that are summed. In the products with values,
+ * weights keep 21 bits or more in float32 calls; in bf16 calls 16 over a float32 or bf16 cache, 11
+ * over a 4-bit one (as weight times step), and 8 in prompts (11 with 32 channels, or where the
+ * tensors are not aligned to 16 bytes). NaN and infinities that a query sees count as in float32
+ * arithmetic, others not at all. */
 typedef struct bst_attention_spec {
     int32_t heads, kv_heads, head_dim, dtype;
     int32_t window, sinks;
@@ -356,7 +361,9 @@ int32_t bst_attention_cached(int32_t device, void* stream, const bst_kv_cache* c
 /* Causal attention of packed sequences over their own keys and values (prompts that need no cache
  * yet): sequences->starts is required, rows and lengths must be NULL, positions count from 0.
  * q and out [tokens][heads][head_dim], k and v [tokens][kv_heads][head_dim]. out shares no byte with
- * q, k or v (at the same distance between tokens it may lie between theirs). */
+ * q, k or v (at the same distance between tokens it may lie between theirs). Should a wait inside
+ * the bf16 kernel run out (2 s), its rows are computed again by another kernel: the call is slow,
+ * its outputs are right. */
 int32_t bst_attention_packed_workspace(const bst_sequences* sequences,
                                        const bst_attention_spec* spec, int64_t* bytes);
 int32_t bst_attention_packed(int32_t device, void* stream, const bst_sequences* sequences,
