@@ -95,6 +95,65 @@ __device__ __forceinline__ bool find_tile(const Batch& b, int group, int tile_ro
     return false;
 }
 
+// One query's attention over keys key_of(0) .. key_of(n - 1) (negative: none) by one warp, plainly: what
+// rows with values that are not finite are added up by. 32 keys at a time: the lanes hold channels, and
+// their partial sums change places, half as many at every step, so that lane i ends with the score of
+// key i. Leaves the maximum of the scores (to base 2), the sum of weights, and channels lane + 32 i.
+template <int C, typename T, typename S, typename K>
+__device__ __forceinline__ void attend_row(const T* q, const S* k, int64_t k_stride, const S* v,
+                                           int64_t v_stride, float scale, int64_t n, K&& key_of,
+                                           float (&value)[C], float* top_, float* total_) {
+    const int lane = threadIdx.x & 31;
+    float x[C], top = -INFINITY, total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+        x[i] = to_f(q[lane + 32 * i]);
+        value[i] = 0.0f;
+    }
+    for (int64_t at = 0; at < n; at += 32) {
+        const int64_t mine = at + lane < n ? key_of(at + lane) : -1;
+        const unsigned seen = __ballot_sync(kFull, mine >= 0);
+        // Keys that are not there are read as key 0, and left out below.
+        const int64_t from = max(mine, static_cast<int64_t>(0));
+        float s[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            const S* row = k + __shfl_sync(kFull, from, j) * k_stride + lane;
+            s[j] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < C; ++i) s[j] = fmaf(x[i], to_f(row[32 * i]), s[j]);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const bool upper = lane & o;
+#pragma unroll
+            for (int j = 0; j < o; ++j) {
+                const float away = upper ? s[j] : s[j + o];
+                s[j] = (upper ? s[j + o] : s[j]) + __shfl_xor_sync(kFull, away, o);
+            }
+        }
+        const float score = mine >= 0 ? s[0] * scale : -INFINITY;
+        const float most = fmaxf(top, warp_max(score));
+        const float keep = top == -INFINITY ? 0.0f : exp2f(top - most);
+        const float p = score == -INFINITY ? 0.0f : exp2f(score - most);  // a NaN stays one
+        total = fmaf(total, keep, warp_sum(p));
+        top = most;
+        if (isnan(total)) break;  // and so is every channel
+#pragma unroll
+        for (int i = 0; i < C; ++i) value[i] *= keep;
+#pragma unroll 8
+        for (int j = 0; j < 32; ++j) {
+            const float weight = __shfl_sync(kFull, p, j);
+            const S* row = v + __shfl_sync(kFull, from, j) * v_stride + lane;
+            if (!((seen >> j) & 1u)) continue;
+#pragma unroll
+            for (int i = 0; i < C; ++i) value[i] = fmaf(weight, to_f(row[32 * i]), value[i]);
+        }
+    }
+    *top_ = top;
+    *total_ = total;
+}
+
 // Tiles of `rows` query rows: exact without starts, at most one partial tile a sequence with them.
 inline int tile_bound(const Batch& b, const AttnSpec& a, int64_t rows) {
     const int64_t group = a.heads / a.kv_heads;

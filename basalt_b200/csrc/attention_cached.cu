@@ -298,32 +298,49 @@ __device__ __noinline__ void attend_plainly(const S* k, const S* v, const T* q, 
                                             const Visible& seen, int b0, int b1, float* to) {
     constexpr int C = HD / 32;
     const int lane = threadIdx.x & 31;
-    float x[C], value[C] = {}, top = -INFINITY, total = 0.0f;
-#pragma unroll
-    for (int i = 0; i < C; ++i) x[i] = to_f(q[lane + 32 * i]);
-    for (int block = b0; block < b1; ++block) {
-        const int key0 = seen.key(block);
-        for (int key = key0; key < key0 + kBlock; ++key) {
-            if (!seen.holds(key)) continue;
-            const int64_t at = static_cast<int64_t>(key) * HD + lane;
-            float dot = 0.0f;
-#pragma unroll
-            for (int i = 0; i < C; ++i) dot = fmaf(x[i], to_f(k[at + 32 * i]), dot);
-            const float s = warp_sum(dot) * scale, most = fmaxf(top, s);
-            const float keep = top == -INFINITY ? 0.0f : exp2f(top - most);
-            const float p = s == -INFINITY ? 0.0f : exp2f(s - most);  // a NaN stays one
-            total = fmaf(total, keep, p);
-#pragma unroll
-            for (int i = 0; i < C; ++i) value[i] = fmaf(p, to_f(v[at + 32 * i]), value[i] * keep);
-            top = most;
-        }
-    }
+    float value[C], top, total;
+    attend_row<C>(q, k, HD, v, HD, scale, static_cast<int64_t>(b1 - b0) * kBlock,
+                  [&](int64_t at) {
+                      const int key = seen.key(b0 + static_cast<int>(at / kBlock)) + static_cast<int>(at % kBlock);
+                      return static_cast<int64_t>(seen.holds(key) ? key : -1);
+                  },
+                  value, &top, &total);
 #pragma unroll
     for (int i = 0; i < C; ++i) to[lane + 32 * i] = value[i];
     if (lane == 0) {
         to[HD] = top;
         to[HD + 1] = total;
     }
+}
+
+// Whether the keys and values of blocks [b0, b1), or `rows` queries of one token, hold an infinity or a
+// float that bf16 rounds to one. This thread's share of the CTA's.
+template <typename T, int STORAGE, int HD>
+__device__ __noinline__ bool meets_infinity(const char* k, const char* v, const Visible& seen, int b0, int b1,
+                                            const T* q, int rows) {
+    auto rounds = [](uint32_t u) { return (u & 0x7fffffffu) - 0x7f7f8000u <= 0x8000u; };
+    auto bad = [&](uint32_t u) {
+        return STORAGE == BST_DTYPE_F32 ? rounds(u) : ((u & 0x7fffu) == 0x7f80u) | ((u & 0x7fff0000u) == 0x7f800000u);
+    };
+    using L = Layout<STORAGE, HD>;
+    constexpr int kChunks = L::kRowBytes / 16;
+    bool found = false;
+    for (int block = b0; block < b1; ++block) {
+        const int key0 = seen.key(block);
+#pragma unroll 4
+        for (int x = threadIdx.x; x < kBlock * kChunks; x += kThreads) {
+            const int key = key0 + x / kChunks;
+            uint4 u = {}, w = {};
+            if (seen.holds(key)) {
+                const int64_t at = static_cast<int64_t>(key) * kChunks + x % kChunks;
+                u = reinterpret_cast<const uint4*>(k)[at];
+                w = reinterpret_cast<const uint4*>(v)[at];
+            }
+            found |= bad(u.x) | bad(u.y) | bad(u.z) | bad(u.w) | bad(w.x) | bad(w.y) | bad(w.z) | bad(w.w);
+        }
+    }
+    for (int x = threadIdx.x; x < rows * HD; x += kThreads) found |= rounds(__float_as_uint(to_f(q[x])));
+    return found;
 }
 
 // ROWS queries a tile: 8, or 16 for bf16 batches that have more than eight to a key head, so that
@@ -946,9 +963,12 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
     }
     if constexpr (L::kCodes) {
         __syncthreads();
-    } else if (__syncthreads_or(!(largest_result <= FLT_MAX))) {
+    } else if (__syncthreads_or(!(largest_result <= FLT_MAX)) &&
+               __syncthreads_or(meets_infinity<T, STORAGE, HD>(
+                   kb, vb, seen, b0, b1, q + tile.first * q_stride + (kvh * group + tile.r0) * HD, rows))) {
         // The terms of an infinity, and of a float that bf16 rounds to one, leave NaN where the formula
-        // may have a weight of zero, an infinity or a number: the CTA's sums again, a warp a row.
+        // may have a weight of zero, an infinity or a number (a NaN leaves what it should): the CTA's sums
+        // again, a warp a row.
         using S = typename std::conditional<STORAGE == BST_DTYPE_F32, float, __nv_bfloat16>::type;
         for (int r = warp; r < rows; r += kWarps) {
             // A sequence has one token here.

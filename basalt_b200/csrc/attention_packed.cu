@@ -516,48 +516,16 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
     }
 }
 
-// One query by one warp: lanes over the channels, one key at a time.
-template <typename T, int HD>
-__device__ __forceinline__ void attend_query(const T* q, const T* k, int64_t k_stride, const T* v,
-                                             int64_t v_stride, T* out, int64_t position, int window,
-                                             int sinks, float scale, int lane) {
-    constexpr int C = HD / 32;
-    float qv[C], acc[C], m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < C; ++i) {
-        qv[i] = to_f(q[lane + 32 * i]);
-        acc[i] = 0.0f;
-    }
-    const int64_t first = window ? max(static_cast<int64_t>(0), position - window + 1) : 0;
-    const int64_t sunk = min(static_cast<int64_t>(sinks), first);  // keys below this come first
-    for (int64_t at = 0; at < sunk + position + 1 - first; ++at) {
-        const int64_t j = at < sunk ? at : first + (at - sunk);
-        float dot = 0.0f;
-#pragma unroll
-        for (int i = 0; i < C; ++i) dot = fmaf(qv[i], to_f(k[j * k_stride + lane + 32 * i]), dot);
-        const float s = warp_sum(dot) * scale;
-        const float top = fmaxf(m, s);
-        const float keep = m == -INFINITY ? 0.0f : expf(m - top);
-        const float p = s == -INFINITY ? 0.0f : expf(s - top);  // NaN scores stay NaN
-        l = l * keep + p;
-#pragma unroll
-        for (int i = 0; i < C; ++i) {
-            acc[i] = fmaf(p, to_f(v[j * v_stride + lane + 32 * i]), acc[i] * keep);
-        }
-        m = top;
-    }
-#pragma unroll
-    for (int i = 0; i < C; ++i) put(out + lane + 32 * i, l == 0.0f ? 0.0f : acc[i] / l);
-}
-
 // ---- float32, and bf16 that the kernel above does not take --------------------------------------
 // The same scheme on mma.sync m16n8k8 (tf32): a CTA takes 64 query rows, a warp 16 of them, keys and
 // values pass through shared memory in tiles, double-buffered with cp.async. float32 operands are
 // split in two tf32 parts, x = h + l with h the upper 10 mantissa bits, and multiplied as
 // h h + h l + l h (2^-21 of a product is left out); bf16 ones are tf32 numbers as they are, their
-// weights rounded to tf32. A CTA whose outputs are not all finite has them computed again. The tensor
+// weights rounded to tf32. A CTA that meets infinities and whose outputs are not all finite has them
+// computed again (4096 causal tokens of 8 heads of 64, an infinity in the first value: 0.55 -> 9 ms). The tensor
 // cores cut sums where float32 additions round: sums of a whole row came out 3e-6 low, so products are
-// summed 32 channels, or a tile of keys, at a time (the small ones apart) and added up in float32. Splitting happens in registers after the load, so the tiles stay float32.
+// summed 32 channels, or a tile of keys, at a time (the small ones apart) and added up in float32.
+// Splitting happens in registers after the load, so the tiles stay float32.
 // Rows of keys are padded to HD + 8 floats and of values to HD + 4, which keeps the fragments' reads
 // (pairs of channels of eight keys; one channel of four keys two apart) free of bank conflicts.
 // Bound by the latency between a warp's own instructions at 12 warps an SM (24 float32 sequences of up to
@@ -819,6 +787,7 @@ k_packed_mma(Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride, con
             }
         }
     }
+    bool whole = true;  // all outputs are finite
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
         total[r] += __shfl_xor_sync(kFull, total[r], 1);
@@ -836,9 +805,31 @@ k_packed_mma(Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride, con
                 put(to + 8 * c + 1, y);
                 most = max_nan(most, max_nan(fabsf(x), fabsf(y)));
             }
-            // The parts of an infinity, and of a float that rounds to one, leave NaN where the formula
-            // may have a weight of zero, an infinity or a number.
-            if (!(most <= FLT_MAX)) redo = 1;
+            whole &= most <= FLT_MAX;
+        }
+    }
+    // The parts of an infinity, and of a float that rounds to one, leave NaN where the formula may have a
+    // weight of zero, an infinity or a number. A NaN leaves what it should: rows that are not finite are
+    // computed again only if the CTA has met one of the former.
+    if constexpr (kSplit) {
+        if (__syncthreads_or(!whole)) {
+            auto splits = [](float x) {
+                const uint32_t u = __float_as_uint(x) & 0x7fffffffu;
+                return u - 0x7f7ff000u <= 0x1000u;
+            };
+            bool found = false;
+            for (int i = 0; i < keys.tiles; ++i) {
+                const int key0 = keys.key(i), stop = min(keys.stop(i), key0 + L::kKeys);
+#pragma unroll 4
+                for (int x = threadIdx.x; x < (stop - key0) * HD; x += L::kThreads) {
+                    const int64_t key = key0 + x / HD;
+                    found |= splits(to_f(kb[key * k_stride + x % HD])) | splits(to_f(vb[key * v_stride + x % HD]));
+                }
+            }
+            for (int x = threadIdx.x; x < rows * HD; x += L::kThreads) {
+                found |= splits(queries[x / HD * L::kQPitch + x % HD]);
+            }
+            if (found) redo = 1;
         }
     }
     __syncthreads();
@@ -847,11 +838,13 @@ k_packed_mma(Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride, con
 
 // The rows of CTAs that raised their flag, computed plainly.
 template <typename T, int HD>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 2)
 k_packed_again(Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride,
                const T* __restrict__ k, int64_t k_stride, const T* __restrict__ v, int64_t v_stride,
                T* __restrict__ out, int64_t out_stride, const int* __restrict__ flags, int tiles,
                int tile_rows) {
+    constexpr int C = HD / 32;
+    const int lane = threadIdx.x & 31;
     pdl_wait();
     for (int i = blockIdx.x; i < tiles * a.kv_heads; i += gridDim.x) {
         if (flags[i] == 0) continue;
@@ -861,13 +854,19 @@ k_packed_again(Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride,
         const int rows = min(tile_rows, tile.n * group - tile.r0);
         for (int r = threadIdx.x >> 5; r < rows; r += 8) {
             const int row = tile.r0 + r;
-            const int64_t token = row / group, head = kvh * group + row % group;
-            attend_query<T, HD>(
-                q + (tile.first + token) * q_stride + head * HD,
-                k + tile.first * k_stride + kvh * HD, k_stride,
-                v + tile.first * v_stride + kvh * HD, v_stride,
-                out + (tile.first + token) * out_stride + head * HD, token, a.window, a.sinks,
-                a.scale, threadIdx.x & 31);
+            const int64_t position = row / group, head = kvh * group + row % group;
+            const int64_t first = a.window ? max(static_cast<int64_t>(0), position - a.window + 1) : 0;
+            const int64_t sunk = min(static_cast<int64_t>(a.sinks), first);  // keys below this come first
+            float value[C], top, total;
+            attend_row<C>(q + (tile.first + position) * q_stride + head * HD,
+                          k + tile.first * k_stride + kvh * HD, k_stride,
+                          v + tile.first * v_stride + kvh * HD, v_stride, a.scale * kLog2e,
+                          sunk + position + 1 - first,
+                          [&](int64_t at) { return at < sunk ? at : first + (at - sunk); }, value, &top,
+                          &total);
+            T* to = out + (tile.first + position) * out_stride + head * HD + lane;
+#pragma unroll
+            for (int c = 0; c < C; ++c) put(to + 32 * c, total == 0.0f ? 0.0f : value[c] / total);
         }
     }
 }
@@ -936,7 +935,7 @@ cudaError_t launch_attention_packed(cudaStream_t s, const Batch& b, const AttnSp
                     b, a, q, q_stride, k, k_stride, v, v_stride, out, out_stride, vector, flags);
             }
             if ((e = cudaGetLastError())) return e;
-            return launch_pdl(k_packed_again<T, HD>, dim3(std::min(148, tiles * a.kv_heads)), dim3(256),
+            return launch_pdl(k_packed_again<T, HD>, dim3(std::min(2 * 148, tiles * a.kv_heads)), dim3(256),
                               0, s, b, a, q, q_stride, k, k_stride, v, v_stride, out, out_stride,
                               static_cast<const int*>(flags), tiles, tile_rows);
         });
