@@ -684,6 +684,10 @@ class Engine {
     // The serving operators' views of layer l's cache and of this model's attention.
     bst::Cache layer_cache(int l) const;
     bst::AttnSpec attention_spec() const;
+    // What a cached value takes, with its share of the scales in 4 bits.
+    double value_bytes() const {
+        return spec.kv_dtype == BST_DTYPE_U4 ? 0.625 : (kvbf16 ? 2.0 : 4.0);
+    }
     // Stores the keys and values in ws.k_new and ws.v_new ([tokens][d]) in layer l's cache.
     int append_step(int l, const bst::Batch& batch);
     void free_workspace();
@@ -1176,7 +1180,7 @@ bst::AttnSpec Engine::attention_spec() const {
 }
 
 int Engine::append_step(int l, const bst::Batch& batch) {
-    const double bytes = 2.0 * batch.tokens * d * (4.0 + 4.0);
+    const double bytes = 2.0 * batch.tokens * d * (4.0 + value_bytes());
     const cudaError_t err = launch(bst::kMisc, bytes, 0, 1, [&] {
         return bst::launch_kv_append(stream, layer_cache(l), batch, ws.k_new, d, ws.v_new, d,
                                      BST_DTYPE_F32);
@@ -1481,7 +1485,7 @@ int Engine::enqueue_prefill(const StepPlan& p, size_t begin, size_t end) {
             att_planes = bst::PlaneOut{};
             // The prompt sees the values that later steps will read.
             if (spec.kv_dtype != BST_DTYPE_F32) {
-                err = launch(bst::kMisc, 2.0 * T * d * 8.0, 0, 1, [&] {
+                err = launch(bst::kMisc, 2.0 * T * d * (4.0 + value_bytes()), 0, 1, [&] {
                     return bst::launch_kv_read(stream, layer_cache(l), prompts, ws.k_new, d, ws.v_new,
                                                d, BST_DTYPE_F32);
                 });
@@ -1784,14 +1788,14 @@ int Engine::decode_after_qkv(int l, int R, const int* rowmap, const int* lengths
         step.count = step.tokens = R;
         step.rows = rowmap;
         step.lengths = lengths;
-        // What the rows see of a 4-bit cache takes 5 bits a value.
-        const double value_bytes = spec.kv_dtype == BST_DTYPE_U4 ? 0.625 : kvb;
         const double seen = spec.attention_window > 0
                                 ? std::min(static_cast<double>(dp.sum_len),
                                            R * (static_cast<double>(spec.attention_window) +
                                                 spec.attention_sinks))
                                 : static_cast<double>(dp.sum_len);
-        st = check(launch(attn_class, (seen * 2.0 * value_bytes + R * 8.0) * d, 4.0 * seen * d, 1, [&] {
+        // With splits a second kernel joins them.
+        const int kernels = bst::attention_cached_workspace(layer_cache(l), step, attention_spec()) ? 2 : 1;
+        st = check(launch(attn_class, (seen * 2.0 * value_bytes() + R * 8.0) * d, 4.0 * seen * d, kernels, [&] {
                        return bst::launch_attention_cached(stream, layer_cache(l), step,
                                                            attention_spec(), ws.q, d, ws.att, d,
                                                            ws.attn_space);
