@@ -331,13 +331,14 @@ int32_t bst_kv_read(int32_t device, void* stream, const bst_kv_cache* cache,
 
 /* heads must be a multiple of kv_heads: query head h reads key head h * kv_heads / heads. A query
  * at position i sees key j when j <= i and (window == 0, or i - j < window, or j < sinks): the
- * last `window` tokens and the first `sinks`. A query that sees nothing gives zeros. dtype is the
- * type of q and out (and of packed k and v). Scores, their maximum, the sums of weights and the
- * outputs' sums are float32, and so are the weights that are summed. In the products with values,
- * weights keep 21 bits or more in float32 calls; in bf16 calls 16 over a float32 or bf16 cache, 11
- * over a 4-bit one (as weight times step), and 8 in prompts (11 with 32 channels, or where the
- * tensors are not aligned to 16 bytes). NaN and infinities that a query sees count as in float32
- * arithmetic, others not at all. */
+ * last `window` tokens and the first `sinks`. A query that sees nothing, or whose scores are all
+ * -infinity, gives zeros. dtype is the type of q and out (and of packed k and v). Scores, their
+ * maximum, the sums of weights and the outputs' sums are float32, and so are the weights that are
+ * summed. In the products with values, weights keep 21 bits or more in float32 calls; in bf16 calls
+ * 16 over a float32 or bf16 cache, 11 over a 4-bit one (as weight times step), and 8 in prompts (11
+ * with 32 channels, or where the tensors are not aligned to 16 bytes). NaN and infinities that a
+ * query sees count as in float32 arithmetic (but a query that holds an infinity gives NaN over a
+ * 4-bit cache), others not at all. */
 typedef struct bst_attention_spec {
     int32_t heads, kv_heads, head_dim, dtype;
     int32_t window, sinks;
