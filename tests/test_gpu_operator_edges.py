@@ -385,3 +385,16 @@ def test_many_heads_to_a_key_head(ops, dtype, dim, group, kv_heads, counts):
     for a, b in zip(starts, starts[1:]):
         want, size, most = attend(host(q)[a:b], k[a:b], v[a:b], 0, 29, 2, 0.2)
         check(got[a:b], want, size, np.full_like(most, most.max()), dim, b - a, dtype)
+
+
+@pytest.mark.parametrize("which,value,again", [(0, math.nan, 0), (1, math.nan, 0), (2, math.nan, 1), (1, -math.inf, 4),
+                                               (2, math.inf, 4)])
+def test_only_infinities_have_rows_computed_again(ops, which, value, again):
+    """The workspace holds a flag for each of the four CTAs of 64 rows: a NaN leaves what it should, but
+    for a value in a tile that some of a CTA's rows do not see."""
+    torch = torch_()
+    x = prompt(np.random.default_rng(8), 200, 1, 1, 64, "f32")
+    x[which][0, 0, 3] = value
+    size = torch.full((4,), 7, dtype=torch.int32, device="cuda")
+    ops.attention_packed(*x, ints([0, 200]), workspace=size)
+    assert size.tolist().count(1) == again and size.tolist().count(0) == 4 - again
