@@ -179,6 +179,23 @@ SIGNATURES = {
                                               _P(SequencesStruct), _P(AttentionSpecStruct),
                                               ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
                                               ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64]),
+    "bst_attention_shared_workspace": (ctypes.c_int32, [
+        _P(KvCacheStruct), _P(SequencesStruct), _P(AttentionSpecStruct), _P(KvCacheStruct), ctypes.c_int32,
+        ctypes.c_int32, _i64p]),
+    "bst_attention_shared": (ctypes.c_int32, [
+        ctypes.c_int32, ctypes.c_void_p, _P(KvCacheStruct), _P(SequencesStruct), _P(AttentionSpecStruct),
+        _P(KvCacheStruct), ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
+        ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64]),
+    "bst_attention_weights_workspace": (ctypes.c_int32, [_P(KvCacheStruct), _P(SequencesStruct),
+                                                         _P(AttentionSpecStruct), _i64p]),
+    "bst_attention_weights": (ctypes.c_int32, [
+        ctypes.c_int32, ctypes.c_void_p, _P(KvCacheStruct), _P(SequencesStruct), _P(AttentionSpecStruct),
+        ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_float,
+        ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64]),
+    "bst_kv_evict": (ctypes.c_int32, [
+        ctypes.c_int32, ctypes.c_void_p, _P(KvCacheStruct), _P(SequencesStruct), ctypes.c_void_p,
+        ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, _P(KvCacheStruct), ctypes.c_void_p, ctypes.c_void_p,
+        ctypes.c_void_p, ctypes.c_void_p]),
     "bst_attention_packed_workspace": (ctypes.c_int32, [_P(SequencesStruct),
                                                         _P(AttentionSpecStruct), _i64p]),
     "bst_attention_packed": (ctypes.c_int32, [ctypes.c_int32, ctypes.c_void_p,

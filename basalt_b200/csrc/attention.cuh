@@ -98,11 +98,16 @@ __device__ __forceinline__ bool find_tile(const Batch& b, int group, int tile_ro
 // One query's attention over keys key_of(0) .. key_of(n - 1) (negative: none) by one warp, plainly: what
 // rows with values that are not finite are added up by. 32 keys at a time: the lanes hold channels, and
 // their partial sums change places, half as many at every step, so that lane i ends with the score of
-// key i. Leaves the maximum of the scores (to base 2), the sum of weights, and channels lane + 32 i.
-template <int C, typename T, typename S, typename K>
+// key i. Leaves the maximum of the scores (to base 2), the sum of weights, and channels lane + 32 i; each
+// key's score goes to write_score, up to the first NaN (behind it every weight is one).
+struct NoScores {
+    __device__ void operator()(int64_t, float) const {}
+};
+template <int C, typename T, typename S, typename K, typename W = NoScores>
 __device__ __forceinline__ void attend_row(const T* q, const S* k, int64_t k_stride, const S* v,
                                            int64_t v_stride, float scale, int64_t n, K&& key_of,
-                                           float (&value)[C], float* top_, float* total_) {
+                                           float (&value)[C], float* top_, float* total_,
+                                           W&& write_score = W()) {
     const int lane = threadIdx.x & 31;
     float x[C], top = -INFINITY, total = 0.0f;
 #pragma unroll
@@ -133,6 +138,7 @@ __device__ __forceinline__ void attend_row(const T* q, const S* k, int64_t k_str
             }
         }
         const float score = mine >= 0 ? s[0] * scale : -INFINITY;
+        if (mine >= 0) write_score(mine, score);
         const float most = fmaxf(top, warp_max(score));
         const float keep = top == -INFINITY ? 0.0f : exp2f(top - most);
         const float p = score == -INFINITY ? 0.0f : exp2f(score - most);  // a NaN stays one

@@ -1,0 +1,92 @@
+// Attention for a batch that shares a long prefix: every query sees the keys of one common row of a cache
+// besides those of its own sequence's row.
+//
+//   out_i = sum_x exp(s_ix - m_i) v_x / sum_x exp(s_ix - m_i),  x over the prefix and the own keys
+//
+// Sums over disjoint sets of keys join exactly (each set leaves its maximum, its sum of weights and its
+// weighted values), so the prefix is a pass of its own: its queries are those of the whole batch, a tile of
+// them reads it once, where attention over a copy in every row would read it once a sequence. The own keys
+// are the pass of attention_cached, and one kernel joins both passes' splits.
+
+#include "attention_cached.cuh"
+
+namespace bst {
+namespace {
+
+struct Plan {
+    CachedPlan own;
+    int rows, tiles, splits;  // of the prefix: query rows a tile, tiles, splits (0: no prefix)
+};
+
+Plan plan_shared(const Cache& c, const Batch& b, const AttnSpec& a, const Prefix& p) {
+    Plan plan{plan_cached(c, b, a), 8, 0, 0};
+    const int64_t queries = static_cast<int64_t>(b.tokens) * (a.heads / a.kv_heads);
+    if (a.dtype == BST_DTYPE_BF16 && queries > 8) plan.rows = 16;
+    plan.tiles = static_cast<int>((queries + plan.rows - 1) / plan.rows);
+    if (p.length > 0) {
+        const int64_t units = static_cast<int64_t>(plan.tiles) * a.kv_heads;
+        const int64_t fill = 148 * ctas_per_sm(p.cache) / units;
+        plan.splits = static_cast<int>(std::max<int64_t>(
+            1, std::min<int64_t>({fill, p.length / 128, static_cast<int64_t>(kMaxSplits)})));
+    }
+    return plan;
+}
+
+size_t part_bytes(const Batch& b, const AttnSpec& a, int splits) {
+    return static_cast<size_t>(b.tokens) * a.heads * splits * (a.head_dim + 2) * sizeof(float);
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kThreads)
+k_shared_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out, int64_t out_stride,
+              int own_splits, const float* __restrict__ own, int prefix_splits,
+              const float* __restrict__ prefix) {
+    const int token = blockIdx.x, head = blockIdx.y;
+    int seq, first, n;
+    if (!find_sequence(b, token, &seq, &first, &n)) return;
+    const int use = used_splits(c, b, a, tile_rows, own_splits, seq, token - first, n, head);
+    pdl_wait();
+    const int64_t query = static_cast<int64_t>(token) * a.heads + head;
+    const float* const mine = own + query * own_splits * (HD + 2);
+    const float* const common = prefix + query * prefix_splits * (HD + 2);
+    join_splits<2 * kMaxSplits, T, HD>(
+        use + prefix_splits,
+        [&](int s) { return s < use ? mine + s * (HD + 2) : common + (s - use) * (HD + 2); },
+        out + token * out_stride + head * HD);
+}
+
+}  // namespace
+
+size_t attention_shared_workspace(const Cache& c, const Batch& b, const AttnSpec& a, const Prefix& p) {
+    const Plan plan = plan_shared(c, b, a, p);
+    return part_bytes(b, a, plan.own.splits + plan.splits);
+}
+
+cudaError_t launch_attention_shared(cudaStream_t s, const Cache& c, const Batch& b, const AttnSpec& a,
+                                    const Prefix& p, const void* q, int64_t q_stride, void* out,
+                                    int64_t out_stride, void* workspace) {
+    if (b.tokens < 1 || b.count < 1) return cudaSuccess;
+    const Plan plan = plan_shared(c, b, a, p);
+    float* const own = static_cast<float*>(workspace);
+    float* const prefix = own + part_bytes(b, a, plan.own.splits) / sizeof(float);
+    if (plan.splits > 0) {
+        Extra extra;
+        extra.row = p.row;
+        extra.length = p.length;
+        const cudaError_t e = run_cached<kPrefix>(s, p.cache, b, a, q, q_stride, nullptr, 0, plan.tiles,
+                                                  plan.rows, plan.splits, prefix, extra);
+        if (e) return e;
+    }
+    if (const cudaError_t e = launch_cached_parts(s, c, b, a, plan.own, q, q_stride, own)) return e;
+    return by_dtype(a.dtype, [&](auto type) {
+        using T = decltype(type);
+        return by_head_dim(a.head_dim, [&](auto hd) {
+            constexpr int HD = decltype(hd)::value;
+            return launch_pdl(k_shared_join<T, HD>, dim3(b.tokens, a.heads), dim3(kThreads), 0, s, c, b, a,
+                              plan.own.rows, static_cast<T*>(out), out_stride, plan.own.splits,
+                              static_cast<const float*>(own), plan.splits, static_cast<const float*>(prefix));
+        });
+    });
+}
+
+}  // namespace bst

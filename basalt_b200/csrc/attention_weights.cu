@@ -1,0 +1,170 @@
+// Attention over a cache that also adds up the weight each key receives:
+//
+//   mass'_j = decay mass_j + sum over the sequence's queries i and the key head's query heads of p_ij,
+//   p_ij = exp(s_ij - max s_i) / sum exp(s_ij - max s_i)
+//
+// A weight is known only when all of a query's scores are, so the pass over the cache keeps every score
+// (4 bytes a query and key, where reading the keys again takes 80 to 512 a key) and a second kernel joins
+// the splits and turns scores into weights. Its CTAs own keys: each adds the weights of all queries to a key
+// in the order of the queries, so that results do not depend on how CTAs are scheduled.
+
+#include "attention_cached.cuh"
+
+namespace bst {
+namespace {
+
+constexpr int kMassKeys = 8 * kThreads;   // keys of a CTA: eight a thread
+constexpr int kMassRows = 64;             // query rows whose maxima and sums are held at a time
+
+// Whether the batch's sequence `seq` is the first that names its row, and the next one that names the same.
+// (A row that is named twice gets the weights of both.)
+__device__ __forceinline__ bool first_of_row(const Batch& b, int seq, int row) {
+    if (!b.rows) return true;
+    bool before = false;
+    for (int s = threadIdx.x; s < seq; s += kThreads) before |= __ldg(b.rows + s) == row;
+    return !__syncthreads_or(before);
+}
+__device__ __forceinline__ int next_of_row(const Batch& b, int seq, int row) {
+    if (!b.rows) return b.count;
+    __shared__ int next;
+    __syncthreads();
+    if (threadIdx.x == 0) next = b.count;
+    __syncthreads();
+    for (int s0 = seq + 1; s0 < b.count; s0 += kThreads) {
+        const int s = s0 + threadIdx.x;
+        const bool hit = s < b.count && __ldg(b.rows + s) == row;
+        if (hit) atomicMin(&next, s);
+        if (__syncthreads_or(hit)) break;
+    }
+    return next;
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kThreads)
+k_weights_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out, int64_t out_stride,
+               int splits, const float* __restrict__ part, const float* __restrict__ scores, int64_t pitch,
+               const float* previous, float decay, float* mass) {
+    const int64_t queries = static_cast<int64_t>(b.tokens) * a.heads;
+    if (blockIdx.x < queries) {
+        const int token = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
+        int seq, first, n;
+        if (!find_sequence(b, token, &seq, &first, &n)) return;
+        const int use = used_splits(c, b, a, tile_rows, splits, seq, token - first, n, head);
+        pdl_wait();
+        const float* from = part + (static_cast<int64_t>(token) * a.heads + head) * splits * (HD + 2);
+        join_splits<kMaxSplits, T, HD>(use, [&](int s) { return from + s * (HD + 2); },
+                                       out + token * out_stride + head * HD);
+        return;
+    }
+    __shared__ float tops[kMassRows], inverse[kMassRows];
+    const int chunks = (c.slots + kMassKeys - 1) / kMassKeys;
+    const int64_t place = blockIdx.x - queries;
+    const int kvh = static_cast<int>(place % a.kv_heads);
+    const int64_t rest = place / a.kv_heads;
+    const int key0 = static_cast<int>(rest % chunks) * kMassKeys;
+    int seq = static_cast<int>(rest / chunks);
+    const int row = b.rows ? __ldg(b.rows + seq) : seq;
+    if (row < 0 || row >= c.rows || !first_of_row(b, seq, row)) return;
+    const int group = a.heads / a.kv_heads, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int N = kMassKeys / kThreads;
+    float sum[N] = {};
+    int end = 0;
+    pdl_wait();
+    for (; seq < b.count; seq = next_of_row(b, seq, row)) {
+        const int length = min(max(0, __ldg(b.lengths + seq)), c.slots);
+        end = max(end, length);
+        if (length <= key0) continue;
+        int first = seq, n = 1;
+        if (b.starts) {
+            first = max(0, __ldg(b.starts + seq));
+            n = max(0, min(__ldg(b.starts + seq + 1), b.tokens) - first);
+        }
+        const int position = max(0, __ldg(b.lengths + seq)) - n;  // of its first token
+        for (int64_t r0 = 0; r0 < static_cast<int64_t>(n) * group; r0 += kMassRows) {
+            const int rows = static_cast<int>(min(static_cast<int64_t>(kMassRows), static_cast<int64_t>(n) * group - r0));
+            __syncthreads();
+            for (int r = warp; r < rows; r += kWarps) {
+                const int at = static_cast<int>((r0 + r) / group), head = kvh * group + static_cast<int>((r0 + r) % group);
+                const int use = used_splits(c, b, a, tile_rows, splits, seq, at, n, head);
+                const float* from = part + (static_cast<int64_t>(first + at) * a.heads + head) * splits * (HD + 2) + HD;
+                float m = -INFINITY, total = 0.0f;
+                for (int s = lane; s < use; s += 32) m = fmaxf(m, from[s * (HD + 2)]);
+                m = warp_max(m);
+                for (int s = lane; s < use; s += 32) {
+                    const float top = from[s * (HD + 2)], t = from[s * (HD + 2) + 1];
+                    total = fmaf(t, top == -INFINITY ? (t == 0.0f ? 0.0f : t) : exp2_fast(top - m), total);
+                }
+                total = warp_sum(total);
+                if (lane == 0) {
+                    tops[r] = m == -INFINITY ? 0.0f : m;
+                    inverse[r] = total == 0.0f ? 0.0f : 1.0f / total;
+                }
+            }
+            __syncthreads();
+            for (int r = 0; r < rows; ++r) {
+                const int at = static_cast<int>((r0 + r) / group), head = kvh * group + static_cast<int>((r0 + r) % group);
+                const int p = min(position + at, c.slots - 1);
+                const float* from = scores + (static_cast<int64_t>(first + at) * a.heads + head) * pitch;
+                if (position + at >= c.slots) continue;  // a token outside the cache sees nothing
+                const float top = tops[r], by = inverse[r];
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int key = key0 + threadIdx.x + i * kThreads;
+                    const bool seen = key <= p && (a.window == 0 || p - key < a.window || key < a.sinks);
+                    if (seen) sum[i] = fmaf(exp2_fast(from[key] - top), by, sum[i]);
+                }
+            }
+        }
+    }
+    const int64_t base = (static_cast<int64_t>(row) * c.kv_heads + kvh) * c.slots;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int key = key0 + threadIdx.x + i * kThreads;
+        if (key >= end) continue;
+        // Without decay the old mass is not read: it may be anything.
+        mass[base + key] = decay == 0.0f ? sum[i] : fmaf(decay, previous[base + key], sum[i]);
+    }
+}
+
+int64_t pitch_of(const Cache& c) { return (static_cast<int64_t>(c.slots) + kBlock - 1) / kBlock * kBlock; }
+
+size_t score_bytes(const Cache& c, const Batch& b, const AttnSpec& a) {
+    return static_cast<size_t>(b.tokens) * a.heads * pitch_of(c) * sizeof(float);
+}
+
+}  // namespace
+
+size_t attention_weights_workspace(const Cache& c, const Batch& b, const AttnSpec& a) {
+    const size_t query = static_cast<size_t>(split_count(c, b, a)) * (a.head_dim + 2) * sizeof(float);
+    return score_bytes(c, b, a) + static_cast<size_t>(b.tokens) * a.heads * query;
+}
+
+cudaError_t launch_attention_weights(cudaStream_t s, const Cache& c, const Batch& b, const AttnSpec& a,
+                                     const void* q, int64_t q_stride, void* out, int64_t out_stride,
+                                     const float* previous, float decay, float* mass, void* workspace) {
+    if (b.count < 1) return cudaSuccess;
+    const int splits = split_count(c, b, a), rows = rows_of_tile(b, a);
+    Extra extra;
+    extra.scores = static_cast<float*>(workspace);
+    extra.pitch = pitch_of(c);
+    float* const part = extra.scores + score_bytes(c, b, a) / sizeof(float);
+    if (b.tokens > 0) {
+        const cudaError_t e = run_cached<kScores>(s, c, b, a, q, q_stride, nullptr, 0, tile_bound(b, a, rows),
+                                                  rows, splits, part, extra);
+        if (e) return e;
+    }
+    const int64_t blocks = static_cast<int64_t>(b.tokens) * a.heads +
+                           static_cast<int64_t>(b.count) * a.kv_heads * ((c.slots + kMassKeys - 1) / kMassKeys);
+    return by_dtype(a.dtype, [&](auto type) {
+        using T = decltype(type);
+        return by_head_dim(a.head_dim, [&](auto hd) {
+            constexpr int HD = decltype(hd)::value;
+            return launch_pdl(k_weights_join<T, HD>, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, s, c,
+                              b, a, rows, static_cast<T*>(out), out_stride, splits,
+                              static_cast<const float*>(part), static_cast<const float*>(extra.scores),
+                              extra.pitch, previous, decay, mass);
+        });
+    });
+}
+
+}  // namespace bst

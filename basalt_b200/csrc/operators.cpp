@@ -239,6 +239,155 @@ int check_packed(const bst_sequences* sequences, const bst_attention_spec* spec,
     return BST_OK;
 }
 
+int check_shared(const bst_kv_cache* cache, const bst_sequences* sequences, const bst_attention_spec* spec,
+                 const bst_kv_cache* prefix, int32_t row, int32_t length, Cache* c, Batch* b, AttnSpec* a,
+                 Prefix* p, std::string* why) {
+    int st = check_cached(cache, sequences, spec, c, b, a, why);
+    if (st) return st;
+    if (spec->window != 0 || spec->sinks != 0) {
+        *why = "attention behind a prefix takes no window and no sinks";
+        return BST_UNSUPPORTED;
+    }
+    if ((st = check_cache(prefix, &p->cache, why))) {
+        *why = "prefix: " + *why;
+        return st;
+    }
+    if (p->cache.kv_heads != c->kv_heads || p->cache.head_dim != c->head_dim) {
+        *why = "prefix and cache disagree on kv_heads or head_dim";
+        return BST_SHAPE;
+    }
+    if (row < 0 || row >= p->cache.rows || length < 0 || length > p->cache.slots) {
+        *why = "the prefix is " + std::to_string(length) + " keys of row " + std::to_string(row) +
+               ", its cache has " + std::to_string(p->cache.rows) + " rows of " +
+               std::to_string(p->cache.slots);
+        return BST_SHAPE;
+    }
+    p->row = row;
+    p->length = length;
+    return BST_OK;
+}
+
+// A call's CTAs are counted in 31 bits.
+int check_blocks(int64_t blocks, std::string* why) {
+    if (blocks <= 0x7fffffff) return BST_OK;
+    *why = "too many sequences, heads and slots for one call";
+    return BST_SHAPE;
+}
+
+// Bytes of a whole array, and whether two such share one.
+struct Range {
+    uint64_t at, bytes;
+};
+bool overlap(const Range& x, const Range& y) {
+    return x.bytes && y.bytes && x.at < y.at + y.bytes && y.at < x.at + x.bytes;
+}
+Range range_of(const void* p, uint64_t bytes) { return Range{reinterpret_cast<uint64_t>(p), bytes}; }
+Range mass_range(const void* mass, const Cache& c) {
+    return range_of(mass, 4ull * c.rows * c.kv_heads * c.slots);
+}
+Range span_range(const Span& x) { return Range{x.at, x.end() - x.at}; }
+// A cache's four buffers.
+struct Buffers {
+    Range each[4];
+    explicit Buffers(const Cache& c) {
+        const uint64_t values = static_cast<uint64_t>(c.rows) * c.kv_heads * c.slots * c.head_dim;
+        const bool u4 = c.storage == BST_DTYPE_U4;
+        const uint64_t bytes = u4 ? values / 2 : values * size_of(c.storage), scale = u4 ? values / 8 : 0;
+        each[0] = range_of(c.k, bytes);
+        each[1] = range_of(c.v, bytes);
+        each[2] = range_of(c.k_scale, scale);
+        each[3] = range_of(c.v_scale, scale);
+    }
+    bool meets(const Range& x) const {
+        return overlap(each[0], x) || overlap(each[1], x) || overlap(each[2], x) || overlap(each[3], x);
+    }
+    bool meets(const Buffers& x) const {
+        return meets(x.each[0]) || meets(x.each[1]) || meets(x.each[2]) || meets(x.each[3]);
+    }
+};
+
+int check_eviction(const bst_kv_cache* cache, const bst_sequences* sequences, const float* mass, int32_t keep,
+                   int32_t recent, int32_t sinks, const bst_kv_cache* to, const int32_t* to_rows, float* to_mass,
+                   int32_t* lengths, int32_t* kept, Cache* c, Batch* b, Eviction* e, std::string* why) {
+    int st = check_cache(cache, c, why);
+    if (!st) st = check_batch(sequences, true, b, why);
+    if (st) return st;
+    if (b->starts) {
+        *why = "an eviction takes no tokens (starts must be null)";
+        return BST_INVALID;
+    }
+    if (keep < 1 || recent < 0 || sinks < 0 || static_cast<int64_t>(recent) + sinks > keep) {
+        *why = "keep must be positive, recent and sinks not negative and together at most keep, got " +
+               std::to_string(keep) + ", " + std::to_string(recent) + " and " + std::to_string(sinks);
+        return BST_SHAPE;
+    }
+    if (to) {
+        if ((st = check_cache(to, &e->to, why))) {
+            *why = "to: " + *why;
+            return st;
+        }
+        if (e->to.storage != c->storage || e->to.kv_heads != c->kv_heads || e->to.head_dim != c->head_dim) {
+            *why = "to must have the cache's storage, kv_heads and head_dim";
+            return BST_SHAPE;
+        }
+    } else {
+        if (to_rows) {
+            *why = "in place keys stay in their rows (to_rows must be null)";
+            return BST_INVALID;
+        }
+        e->to = *c;
+    }
+    if (keep > e->to.slots) {
+        *why = "keep is " + std::to_string(keep) + ", the cache that is written has " +
+               std::to_string(e->to.slots) + " slots";
+        return BST_SHAPE;
+    }
+    if ((st = check_blocks(static_cast<int64_t>(b->count) * c->kv_heads * ((keep + 63) / 64), why))) return st;
+    if (b->count > 0) {
+        if (!mass || !to_mass || !lengths || !kept) {
+            *why = "masses, new lengths and kept slots must not be null";
+            return BST_INVALID;
+        }
+        for (const void* p : {static_cast<const void*>(mass), static_cast<const void*>(to_mass),
+                              static_cast<const void*>(lengths), static_cast<const void*>(kept),
+                              static_cast<const void*>(to_rows)}) {
+            if (reinterpret_cast<uintptr_t>(p) % 4) {
+                *why = "masses, rows, lengths and kept slots must be aligned to 4 bytes";
+                return BST_INVALID;
+            }
+        }
+        const Buffers read(*c), written(e->to);
+        const Range masses = mass_range(mass, *c), to_masses = mass_range(to_mass, e->to);
+        const Range slots = range_of(kept, 4ull * b->count * c->kv_heads * keep);
+        const Range counts = range_of(lengths, 4ull * b->count);
+        const Range indices[3] = {range_of(b->lengths, 4ull * b->count),
+                                  range_of(b->rows, b->rows ? 4ull * b->count : 0),
+                                  range_of(to_rows, to_rows ? 4ull * b->count : 0)};
+        bool bad = to && read.meets(written);
+        bad |= !(!to && to_mass == mass) && overlap(masses, to_masses);
+        bad |= overlap(slots, counts);
+        for (const Range& x : {to_masses, slots, counts}) {
+            bad |= read.meets(x) || written.meets(x);
+            for (const Range& y : indices) bad |= overlap(x, y);
+        }
+        bad |= overlap(slots, masses) || overlap(slots, to_masses) || overlap(counts, masses) ||
+               overlap(counts, to_masses);
+        if (bad) {
+            *why = "what is written must not overlap anything else (masses may stay in place when keys do)";
+            return BST_INVALID;
+        }
+    }
+    e->keep = keep;
+    e->recent = recent;
+    e->sinks = sinks;
+    e->mass = mass;
+    e->to_rows = to ? to_rows : b->rows;
+    e->to_mass = to_mass;
+    e->lengths = lengths;
+    e->kept = kept;
+    return BST_OK;
+}
+
 int check_workspace(size_t needed, const void* workspace, int64_t bytes, std::string* why) {
     if (needed == 0) return BST_OK;
     if (!workspace || bytes < 0 || static_cast<size_t>(bytes) < needed) {
@@ -378,6 +527,154 @@ int32_t bst_attention_cached(int32_t device, void* stream, const bst_kv_cache* c
             return launch_attention_cached(static_cast<cudaStream_t>(stream), c, b, a, q, q_stride,
                                            out, out_stride, workspace);
         });
+    })
+}
+
+int32_t bst_attention_shared_workspace(const bst_kv_cache* cache, const bst_sequences* sequences,
+                                       const bst_attention_spec* spec, const bst_kv_cache* prefix,
+                                       int32_t prefix_row, int32_t prefix_length, int64_t* bytes) {
+    using namespace bst;
+    BST_OPERATOR_GUARDED("attention_shared", {
+        Cache c;
+        Batch b;
+        AttnSpec a;
+        Prefix p;
+        std::string why;
+        const int st =
+            check_shared(cache, sequences, spec, prefix, prefix_row, prefix_length, &c, &b, &a, &p, &why);
+        if (st) return refuse("attention_shared", st, why);
+        if (!bytes) return refuse("attention_shared", BST_INVALID, "bytes must not be null");
+        *bytes = static_cast<int64_t>(attention_shared_workspace(c, b, a, p));
+        return BST_OK;
+    })
+}
+
+int32_t bst_attention_shared(int32_t device, void* stream, const bst_kv_cache* cache,
+                             const bst_sequences* sequences, const bst_attention_spec* spec,
+                             const bst_kv_cache* prefix, int32_t prefix_row, int32_t prefix_length,
+                             const void* q, int64_t q_stride, void* out, int64_t out_stride,
+                             void* workspace, int64_t workspace_bytes) {
+    using namespace bst;
+    BST_OPERATOR_GUARDED("attention_shared", {
+        Cache c;
+        Batch b;
+        AttnSpec a;
+        Prefix p;
+        std::string why;
+        int st = check_shared(cache, sequences, spec, prefix, prefix_row, prefix_length, &c, &b, &a, &p, &why);
+        if (st) return refuse("attention_shared", st, why);
+        if (b.tokens == 0 || b.count == 0) return BST_OK;
+        st = check_tensor("q", q, q_stride, a.heads, a.head_dim, a.dtype, &why);
+        if (!st) st = check_tensor("out", out, out_stride, a.heads, a.head_dim, a.dtype, &why);
+        // Outputs are written by the kernel that joins, behind all that read queries.
+        if (!st && !(out == q && out_stride == q_stride) &&
+            overlap(span_of(q, q_stride, a.heads, a, b.tokens),
+                    span_of(out, out_stride, a.heads, a, b.tokens))) {
+            st = BST_INVALID;
+            why = "out overlaps q (it may only be q itself)";
+        }
+        if (!st) {
+            st = check_workspace(attention_shared_workspace(c, b, a, p), workspace, workspace_bytes, &why);
+        }
+        if (st) return refuse("attention_shared", st, why);
+        return queue(device, "attention_shared", [&] {
+            return launch_attention_shared(static_cast<cudaStream_t>(stream), c, b, a, p, q, q_stride, out,
+                                           out_stride, workspace);
+        });
+    })
+}
+
+int32_t bst_attention_weights_workspace(const bst_kv_cache* cache, const bst_sequences* sequences,
+                                        const bst_attention_spec* spec, int64_t* bytes) {
+    using namespace bst;
+    BST_OPERATOR_GUARDED("attention_weights", {
+        Cache c;
+        Batch b;
+        AttnSpec a;
+        std::string why;
+        const int st = check_cached(cache, sequences, spec, &c, &b, &a, &why);
+        if (st) return refuse("attention_weights", st, why);
+        if (!bytes) return refuse("attention_weights", BST_INVALID, "bytes must not be null");
+        *bytes = static_cast<int64_t>(attention_weights_workspace(c, b, a));
+        return BST_OK;
+    })
+}
+
+int32_t bst_attention_weights(int32_t device, void* stream, const bst_kv_cache* cache,
+                              const bst_sequences* sequences, const bst_attention_spec* spec, const void* q,
+                              int64_t q_stride, void* out, int64_t out_stride, const float* previous,
+                              float decay, float* mass, void* workspace, int64_t workspace_bytes) {
+    using namespace bst;
+    BST_OPERATOR_GUARDED("attention_weights", {
+        Cache c;
+        Batch b;
+        AttnSpec a;
+        std::string why;
+        int st = check_cached(cache, sequences, spec, &c, &b, &a, &why);
+        if (!st && !(std::isfinite(decay) && decay >= 0.0f)) {
+            st = BST_INVALID;
+            why = "decay must be finite and not negative";
+        }
+        if (st) return refuse("attention_weights", st, why);
+        if (b.count == 0) return BST_OK;
+        if (b.tokens > 0) {
+            st = check_tensor("q", q, q_stride, a.heads, a.head_dim, a.dtype, &why);
+            if (!st) st = check_tensor("out", out, out_stride, a.heads, a.head_dim, a.dtype, &why);
+        }
+        if (!st && (!mass || (!previous && decay != 0.0f))) {
+            st = BST_INVALID;
+            why = "mass must not be null, nor previous unless decay is 0";
+        }
+        if (!st && (reinterpret_cast<uintptr_t>(mass) % 4 || reinterpret_cast<uintptr_t>(previous) % 4)) {
+            st = BST_INVALID;
+            why = "masses must be aligned to 4 bytes";
+        }
+        if (!st) {
+            const Range to = mass_range(mass, c);
+            const Range from = decay == 0.0f ? Range{0, 0} : mass_range(previous, c);
+            bool bad = Buffers(c).meets(to) || (previous != mass && overlap(to, from));
+            if (b.tokens > 0) {
+                const Span query = span_of(q, q_stride, a.heads, a, b.tokens);
+                const Span result = span_of(out, out_stride, a.heads, a, b.tokens);
+                bad |= overlap(to, span_range(query)) || overlap(to, span_range(result)) ||
+                       overlap(from, span_range(result)) ||
+                       (!(out == q && out_stride == q_stride) && overlap(query, result));
+            }
+            if (bad) {
+                st = BST_INVALID;
+                why = "mass and out must not overlap what is read (mass may be previous, out may be q)";
+            }
+        }
+        if (!st) {
+            const int64_t chunks = (static_cast<int64_t>(c.slots) + 1023) / 1024;
+            st = check_blocks(static_cast<int64_t>(b.tokens) * a.heads + chunks * a.kv_heads * b.count, &why);
+        }
+        if (!st) {
+            st = check_workspace(attention_weights_workspace(c, b, a), workspace, workspace_bytes, &why);
+        }
+        if (st) return refuse("attention_weights", st, why);
+        return queue(device, "attention_weights", [&] {
+            return launch_attention_weights(static_cast<cudaStream_t>(stream), c, b, a, q, q_stride, out,
+                                            out_stride, previous, decay, mass, workspace);
+        });
+    })
+}
+
+int32_t bst_kv_evict(int32_t device, void* stream, const bst_kv_cache* cache, const bst_sequences* sequences,
+                     const float* mass, int32_t keep, int32_t recent, int32_t sinks, const bst_kv_cache* to,
+                     const int32_t* to_rows, float* to_mass, int32_t* lengths, int32_t* kept) {
+    using namespace bst;
+    BST_OPERATOR_GUARDED("kv_evict", {
+        Cache c;
+        Batch b;
+        Eviction e;
+        std::string why;
+        const int st = check_eviction(cache, sequences, mass, keep, recent, sinks, to, to_rows, to_mass, lengths,
+                                      kept, &c, &b, &e, &why);
+        if (st) return refuse("kv_evict", st, why);
+        if (b.count == 0) return BST_OK;
+        return queue(device, "kv_evict",
+                     [&] { return launch_kv_evict(static_cast<cudaStream_t>(stream), c, b, e); });
     })
 }
 

@@ -1,5 +1,5 @@
-// Internal interface of the serving operators (kv_cache.cu, attention_cached.cu,
-// attention_packed.cu, sample.cu): device views
+// Internal interface of the serving operators (kv_cache.cu, kv_evict.cu, attention_cached.cu,
+// attention_packed.cu, attention_shared.cu, attention_weights.cu, sample.cu): device views
 // of the ABI structs and the launchers shared with the engine. Launchers queue on the given stream
 // of the current device and return the launch's error.
 #pragma once
@@ -41,6 +41,41 @@ size_t attention_cached_workspace(const Cache& c, const Batch& b, const AttnSpec
 cudaError_t launch_attention_cached(cudaStream_t s, const Cache& c, const Batch& b,
                                     const AttnSpec& a, const void* q, int64_t q_stride, void* out,
                                     int64_t out_stride, void* workspace);
+// The splits of a cached call and its query rows a tile; the pass that leaves every split's sums in `part`,
+// [tokens][heads][splits][head_dim outputs, maximum (base 2), sum of weights].
+struct CachedPlan {
+    int splits, rows;
+};
+CachedPlan plan_cached(const Cache& c, const Batch& b, const AttnSpec& a);
+cudaError_t launch_cached_parts(cudaStream_t s, const Cache& c, const Batch& b, const AttnSpec& a,
+                                const CachedPlan& plan, const void* q, int64_t q_stride, float* part);
+
+// Keys that a batch shares: the first `length` of a row of a cache.
+struct Prefix {
+    Cache cache;
+    int row = 0, length = 0;
+};
+size_t attention_shared_workspace(const Cache& c, const Batch& b, const AttnSpec& a, const Prefix& p);
+cudaError_t launch_attention_shared(cudaStream_t s, const Cache& c, const Batch& b, const AttnSpec& a,
+                                    const Prefix& p, const void* q, int64_t q_stride, void* out,
+                                    int64_t out_stride, void* workspace);
+
+size_t attention_weights_workspace(const Cache& c, const Batch& b, const AttnSpec& a);
+cudaError_t launch_attention_weights(cudaStream_t s, const Cache& c, const Batch& b, const AttnSpec& a,
+                                     const void* q, int64_t q_stride, void* out, int64_t out_stride,
+                                     const float* previous, float decay, float* mass, void* workspace);
+
+// What an eviction keeps, and where it goes.
+struct Eviction {
+    int keep = 0, recent = 0, sinks = 0;
+    const float* mass = nullptr;   // [rows][kv_heads][slots] of the cache
+    Cache to;                      // the cache itself: keys move in place
+    const int* to_rows = nullptr;
+    float* to_mass = nullptr;      // of `to`
+    int *lengths = nullptr, *kept = nullptr;
+};
+cudaError_t launch_kv_evict(cudaStream_t s, const Cache& c, const Batch& b, const Eviction& e);
+
 size_t attention_packed_workspace(const Batch& b, const AttnSpec& a);
 cudaError_t launch_attention_packed(cudaStream_t s, const Batch& b, const AttnSpec& a,
                                     const void* q, int64_t q_stride, const void* k,
@@ -88,6 +123,12 @@ int check_batch(const bst_sequences* s, bool lengths_needed, Batch* out, std::st
 int check_cache(const bst_kv_cache* c, Cache* out, std::string* why);
 
 #ifdef __CUDACC__
+// The packed tokens that sequences own, [*first, *first + *n); false when there are none.
+__device__ __forceinline__ bool owned_tokens(const Batch& b, int* first, int* n) {
+    *first = b.starts ? max(0, __ldg(b.starts)) : 0;
+    *n = (b.starts ? min(__ldg(b.starts + b.count), b.tokens) : b.tokens) - *first;
+    return *n > 0;
+}
 // The sequence that owns packed token t and the token's place in it; false when none does.
 __device__ __forceinline__ bool find_sequence(const Batch& b, int t, int* seq, int* first, int* n) {
     if (!b.starts) {

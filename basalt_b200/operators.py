@@ -1,5 +1,6 @@
 """The serving operators of libbasalt_cuda.so on torch tensors: a cache of keys and values held in
-4 bits, bf16 or float32, attention over it, attention over packed prompts, and drawing tokens.
+4 bits, bf16 or float32, attention over it, alone or behind a prefix that the batch shares, the weight
+that its keys gather and eviction by it, attention over packed prompts, and drawing tokens.
 
 Tensors stay on the GPU: every call takes their device pointers, queues its kernels on ``stream`` (a
 torch.cuda.Stream or a cudaStream_t as a number; torch's current stream of the tensors' device by
@@ -157,6 +158,13 @@ class KvCache:
         s.v_scale = v_scale.data_ptr() if u4 else None
         self._struct = s
         self._ref = ctypes.byref(s)
+        self._shape = (self.storage, self.slots)   # what workspaces over it depend on
+
+    def _keep(self, key, size):
+        if len(self._sizes) >= _KEPT:
+            self._sizes.clear()
+        self._sizes[key] = size
+        return size
 
     @staticmethod
     def allocate(rows: int, kv_heads: int, slots: int, head_dim: int, storage: str = "u4",
@@ -293,14 +301,115 @@ def attention_cached(cache: KvCache, q, lengths, starts=None, rows=None, window:
     if needed is None:
         size = ctypes.c_int64(0)
         _raise(lib.bst_attention_cached_workspace(cache._ref, s, a, size))
-        if len(cache._sizes) >= _KEPT:
-            cache._sizes.clear()
-        needed = cache._sizes[key] = size.value
+        needed = cache._keep(key, size.value)
     pointer, room, workspace = _workspace(device, needed, workspace, stream)
     _raise(lib.bst_attention_cached(device.index, _stream(device, stream), cache._ref, s, a,
                                     q.data_ptr(), q_stride, out.data_ptr(), out_stride, pointer,
                                     room))
     return out
+
+
+def attention_shared(cache: KvCache, q, lengths, prefix: KvCache, prefix_length: int, prefix_row: int = 0,
+                     starts=None, rows=None, scale=None, out=None, workspace=None, stream=None):
+    """Attention of q ([tokens, heads, head_dim]) over the first ``prefix_length`` keys of row ``prefix_row``
+    of ``prefix``, which all sequences share, and the sequences' own rows of ``cache`` behind them (as
+    ``attention_cached`` without a window). The prefix is read once for the whole batch; ``prefix`` may be
+    ``cache`` itself, or hold its keys in another storage. ``out`` may be ``q`` itself."""
+    device = cache.device
+    stream = _given(device, stream)
+    if prefix.device != device:
+        _on(device, "prefix", prefix.k)
+    q_stride = _packed(device, "q", q, None, cache.head_dim)
+    out, out_stride = _out(device, q, out, stream)
+    s = _sequences(device, q.shape[0], lengths, starts, rows)
+    a = _spec(q, cache.kv_heads, 0, 0, scale)
+    prefix_row, prefix_length = _lib.int32(prefix_row), _lib.int32(prefix_length)
+    lib = _lib.load()
+    key = (s.count, s.tokens, starts is None, a.heads, a.dtype, prefix._shape, prefix_length)
+    needed = cache._sizes.get(key)
+    if needed is None:
+        size = ctypes.c_int64(0)
+        _raise(lib.bst_attention_shared_workspace(cache._ref, s, a, prefix._ref, prefix_row, prefix_length,
+                                                  size))
+        needed = cache._keep(key, size.value)
+    pointer, room, workspace = _workspace(device, needed, workspace, stream)
+    _raise(lib.bst_attention_shared(device.index, _stream(device, stream), cache._ref, s, a, prefix._ref,
+                                    prefix_row, prefix_length, q.data_ptr(), q_stride, out.data_ptr(),
+                                    out_stride, pointer, room))
+    return out
+
+
+def _mass(device, name, t, cache):
+    """Checks masses [rows, kv_heads, slots] of a cache."""
+    _on(device, name, t)
+    if t.dtype is not _module.float32 or not t.is_contiguous():
+        raise IllegalArgumentException(f"{name} must be contiguous float32", _lib.BST_INVALID)
+    if t.shape != (cache.rows, cache.kv_heads, cache.slots):
+        raise BasaltShapeException(f"{name} is {tuple(t.shape)}, expected "
+                                   f"{(cache.rows, cache.kv_heads, cache.slots)}", _lib.BST_SHAPE)
+    return t.data_ptr()
+
+
+def attention_weights(cache: KvCache, q, lengths, mass, previous=None, decay: float = 1.0, starts=None,
+                      rows=None, window: int = 0, sinks: int = 0, scale=None, out=None, workspace=None,
+                      stream=None):
+    """``attention_cached``, which also adds up the weight each key gets: for the slots j < length of the
+    sequences' rows ``mass[row, h, j] = decay * previous[row, h, j] +`` the weights that the call's tokens
+    and the query heads of key head h give key j. ``mass`` and ``previous`` (``mass`` itself by default) are
+    float32 [rows, kv_heads, slots]; with ``decay`` 0 what was there is not read. Returns the outputs."""
+    device = cache.device
+    stream = _given(device, stream)
+    to = _mass(device, "mass", mass, cache)
+    before = to if previous is None else _mass(device, "previous", previous, cache)
+    q_stride = _packed(device, "q", q, None, cache.head_dim)
+    out, out_stride = _out(device, q, out, stream)
+    s = _sequences(device, q.shape[0], lengths, starts, rows)
+    a = _spec(q, cache.kv_heads, window, sinks, scale)
+    lib = _lib.load()
+    key = (s.count, s.tokens, starts is None, a.heads, a.dtype, a.window, a.sinks, "weights")
+    needed = cache._sizes.get(key)
+    if needed is None:
+        size = ctypes.c_int64(0)
+        _raise(lib.bst_attention_weights_workspace(cache._ref, s, a, size))
+        needed = cache._keep(key, size.value)
+    pointer, room, workspace = _workspace(device, needed, workspace, stream)
+    _raise(lib.bst_attention_weights(device.index, _stream(device, stream), cache._ref, s, a, q.data_ptr(),
+                                     q_stride, out.data_ptr(), out_stride, before, decay, to, pointer, room))
+    return out
+
+
+def kv_evict(cache: KvCache, mass, lengths, keep: int, recent: int = 0, sinks: int = 0, rows=None,
+             to: KvCache | None = None, to_mass=None, to_rows=None, kept=None, stream=None):
+    """Shrinks the sequences to ``keep`` keys in each key head: the first ``sinks``, the last ``recent`` and
+    of the others those of the largest ``mass`` ([rows, kv_heads, slots] float32, as ``attention_weights``
+    leaves it). They move in order to the first slots, in place, or to rows ``to_rows`` (s when omitted) of
+    the cache ``to`` with their masses in ``to_mass``; masses behind them become zero. Returns the new
+    lengths (int32) and the kept slots [count, kv_heads, keep] (int32, -1 behind the last; ``kept`` if
+    given)."""
+    device = cache.device
+    stream = _given(device, stream)
+    keep = _lib.int32(keep)
+    target = cache if to is None else to
+    if target.device != device:
+        _on(device, "to", target.k)
+    at = _mass(device, "mass", mass, cache)
+    if to is not None and to_mass is None:
+        raise IllegalArgumentException("to_mass must be given beside to", _lib.BST_INVALID)
+    to_at = at if to_mass is None else _mass(device, "to_mass", to_mass, target)
+    s = _sequences(device, lengths.shape[0], lengths, None, rows)
+    new = _empty((s.count,), _module.int32, device, stream)
+    shape = (s.count, cache.kv_heads, max(keep, 0))
+    if kept is None:
+        kept = _empty(shape, _module.int32, device, stream)
+    else:
+        _on(device, "kept", kept)
+        if kept.dtype is not _module.int32 or not kept.is_contiguous() or tuple(kept.shape) != shape:
+            raise BasaltShapeException(f"kept must be contiguous int32 {shape}", _lib.BST_SHAPE)
+    _raise(_lib.load().bst_kv_evict(device.index, _stream(device, stream), cache._ref, s, at, keep,
+                                    _lib.int32(recent), _lib.int32(sinks), None if to is None else to._ref,
+                                    _index(device, "to_rows", to_rows, s.count), to_at, new.data_ptr(),
+                                    kept.data_ptr()))
+    return new, kept
 
 
 def attention_packed(q, k, v, starts, window: int = 0, sinks: int = 0, scale=None, out=None,

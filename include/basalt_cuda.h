@@ -359,6 +359,55 @@ int32_t bst_attention_cached(int32_t device, void* stream, const bst_kv_cache* c
                              const void* q, int64_t q_stride, void* out, int64_t out_stride,
                              void* workspace, int64_t workspace_bytes);
 
+/* Attention of a batch whose sequences all begin with the same tokens: a query sees every one of the
+ * first prefix_length keys of row prefix_row of `prefix` and, of its sequence's own row of `cache`, what
+ * it sees in bst_attention_cached without a window (spec->window and sinks must be 0; own slots and
+ * lengths count from behind the prefix, and a sequence may have no own key). The prefix is read once for
+ * the batch, not once a sequence. `prefix` may be `cache` itself, and may hold another storage; heads and
+ * head_dim are the same. 0 <= prefix_length <= its slots. Types, the own rows' one token without a 4-bit
+ * cache, out and workspace are as in bst_attention_cached; over a 4-bit prefix any q counts as there. */
+int32_t bst_attention_shared_workspace(const bst_kv_cache* cache, const bst_sequences* sequences,
+                                       const bst_attention_spec* spec, const bst_kv_cache* prefix,
+                                       int32_t prefix_row, int32_t prefix_length, int64_t* bytes);
+int32_t bst_attention_shared(int32_t device, void* stream, const bst_kv_cache* cache,
+                             const bst_sequences* sequences, const bst_attention_spec* spec,
+                             const bst_kv_cache* prefix, int32_t prefix_row, int32_t prefix_length,
+                             const void* q, int64_t q_stride, void* out, int64_t out_stride,
+                             void* workspace, int64_t workspace_bytes);
+
+/* bst_attention_cached, and what weight every key gets: for each sequence, key head h and slot
+ * j < lengths[s],
+ *   mass[row][h][j] = decay * previous[row][h][j] + the sum of the weights (softmax of the scores) that
+ *                     key j has for the call's tokens of the sequence and the query heads of key head h.
+ * A key that no query sees gets 0, and one with a NaN among its scores NaN. mass and previous are float32
+ * [rows][kv_heads][slots], weights float32 whatever the types. Other slots and rows of mass stay as they
+ * were. previous may be mass itself (a running sum with decay 1) and shares nothing with it otherwise
+ * (drafted tokens that may be rejected); with decay 0 it is not read and may be NULL. Should two
+ * sequences name the same row, its keys get the weights of both. The workspace holds a float for every
+ * query head and slot. */
+int32_t bst_attention_weights_workspace(const bst_kv_cache* cache, const bst_sequences* sequences,
+                                        const bst_attention_spec* spec, int64_t* bytes);
+int32_t bst_attention_weights(int32_t device, void* stream, const bst_kv_cache* cache,
+                              const bst_sequences* sequences, const bst_attention_spec* spec, const void* q,
+                              int64_t q_stride, void* out, int64_t out_stride, const float* previous,
+                              float decay, float* mass, void* workspace, int64_t workspace_bytes);
+
+/* Eviction: of a sequence with more than `keep` keys each key head keeps `keep`: the first `sinks`, the
+ * last `recent`, and of the others those of the largest mass (float32 [rows][kv_heads][slots]; ties: the
+ * lowest slot; NaN counts below all). They move in order to slots 0 .. keep - 1, and their masses with
+ * them; shorter sequences keep all. With `to` NULL this happens in place (to_rows must be NULL, to_mass
+ * may be mass); otherwise keys and values go to row to_rows[s] (s when NULL) of `to`, a cache of the same
+ * storage, kv_heads and head_dim with keep slots or more that shares no memory with `cache`, which stays
+ * as it was. Of to_mass ([rows][kv_heads][slots] of `to`) the slots behind the kept ones become 0, so
+ * that tokens which are appended start from there; keys and values there stay as they were.
+ * lengths_out[s] becomes the number of keys kept (min(lengths[s], keep)) and kept [count][kv_heads][keep]
+ * the slots they had, in order, -1 behind the last. A sequence whose rows lie outside the caches, or
+ * whose row to write an earlier sequence names too, keeps none: length 0, kept -1. 1 <= keep,
+ * sinks + recent <= keep; sequences->starts must be NULL. */
+int32_t bst_kv_evict(int32_t device, void* stream, const bst_kv_cache* cache, const bst_sequences* sequences,
+                     const float* mass, int32_t keep, int32_t recent, int32_t sinks, const bst_kv_cache* to,
+                     const int32_t* to_rows, float* to_mass, int32_t* lengths_out, int32_t* kept);
+
 /* Causal attention of packed sequences over their own keys and values (prompts that need no cache
  * yet): sequences->starts is required, rows and lengths must be NULL, positions count from 0.
  * q and out [tokens][heads][head_dim], k and v [tokens][kv_heads][head_dim]. out shares no byte with

@@ -1,0 +1,513 @@
+"""Attention behind a shared prefix, attention that adds up weights, and eviction, against plain 64-bit
+implementations.
+
+Tolerances. Outputs as for attention over a cache: a score of d products is off by at most
+(d + 8) 2^-23 sum|q k| scale, a weight by twice that of itself and the exponential's 2^-21, a sum over n
+weights adds n 2^-24 on either side of the quotient, and an output is off by at most max|v| times their sum;
+bf16 outputs add their weights' 2^-8 of max|v|, what bf16 values of 4-bit codes add on the tensor cores
+(2^-8 of max|v| again, and 2^-11 of a score for keys in fp16), and their own 2^-8. A mass is a sum of
+weights (float32 for every type): it is off by the weights' relative error times their sum, and by 2^-23 of
+the old mass, which is multiplied and added.
+"""
+import numpy as np
+import pytest
+
+import operator_reference as ref
+from test_gpu_operators import bound, host, ints, tensor, torch_
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops(runtime):
+    from basalt_b200 import operators
+
+    return operators
+
+
+def filled(ops, rng, rows, kv_heads, slots, dim, storage):
+    """A cache whose every slot is stored, and the values [rows, slots, kv_heads, dim] it stands for."""
+    cache = ops.KvCache.allocate(rows, kv_heads, slots, dim, storage)
+    starts, lengths = ints(np.arange(rows + 1) * slots), ints([slots] * rows)
+    x = rng.standard_normal((2, rows * slots, kv_heads, dim)).astype(np.float32)
+    x[0] += 2.0 * rng.standard_normal((1, kv_heads, dim)) * (rng.random((1, kv_heads, dim)) < 0.1)
+    ops.kv_append(cache, tensor(x[0]), tensor(x[1]), lengths, starts=starts)
+    k, v = ops.kv_read(cache, lengths, starts=starts, tokens=rows * slots)
+    return cache, *(host(t).reshape(rows, slots, kv_heads, dim) for t in (k, v))
+
+
+def spoil(cache, row, slot):
+    """NaN in every value of a row's slots from `slot` on."""
+    for t in (cache.k, cache.v) if cache.k_scale is None else (cache.k_scale, cache.v_scale):
+        t[row, :, slot:] = float("nan")
+
+
+def queries(rng, tokens, heads, dim, dtype):
+    """Queries as a slice of a wider tensor, and what they are in 64 bits."""
+    wide = tensor(rng.standard_normal((tokens, heads * dim + 64)).astype(np.float32), dtype)
+    q = wide[:, 32:32 + heads * dim].unflatten(-1, (heads, dim))
+    return q, host(q)
+
+
+def softmax(score):
+    p = np.exp(score - score.max())
+    return p / p.sum()
+
+
+# ---- a shared prefix -----------------------------------------------------------------------------
+def shared_reference(q, keys, values, own_k, own_v, first, scale):
+    """q [n, H, d] of one sequence, its own keys [m, KV, d] from position `first`; out and sizes."""
+    n, H, d = q.shape
+    out, size = np.zeros((n, H, d)), np.zeros((n, H))
+    for i in range(n):
+        m = min(max(first + i + 1, 0), own_k.shape[0]) if first + i < own_k.shape[0] else 0
+        for h in range(H):
+            at = h * keys.shape[1] // H
+            k = np.concatenate([keys[:, at], own_k[:m, at]])
+            v = np.concatenate([values[:, at], own_v[:m, at]])
+            if len(k):
+                out[i, h] = softmax(k @ q[i, h] * scale) @ v
+                size[i, h] = (np.abs(k) @ np.abs(q[i, h])).max() * abs(scale)
+    return out, size
+
+
+def shared_bound(size, d, n, vmax, out, dtype, prefix_storage):
+    tol = bound(size, d, n, vmax, out, dtype)
+    if dtype == "bf16" and prefix_storage == "u4":
+        tol = tol + vmax * (2.0 ** -8 + 2.2 * 2.0 ** -11 * size[..., None])
+    return tol
+
+
+def check_shared(ops, rng, storage, prefix_storage, dtype, dim, heads, kv_heads, prefix, lengths, counts=None,
+                 slots=None, scale=None, ahead=0):
+    slots = slots or max(lengths) + 5
+    count = len(lengths)
+    own, own_k, own_v = filled(ops, rng, count + 1, kv_heads, slots, dim, storage)
+    common, keys, values = filled(ops, rng, 3, kv_heads, prefix + 9, dim, prefix_storage)
+    spoil(common, 1, prefix)
+    rows = rng.permutation(count + 1)[:count]
+    for s, n in enumerate(lengths):
+        spoil(own, rows[s], max(n, 0))
+    starts = None if counts is None else ahead + np.concatenate([[0], np.cumsum(counts)])
+    counts = counts or [1] * count
+    tokens = count if starts is None else int(starts[-1]) + 2
+    q, q64 = queries(rng, tokens, heads, dim, dtype)
+    out = torch_().full((tokens, heads, dim), 7.5, dtype=q.dtype, device="cuda")
+    got = ops.attention_shared(own, q, ints(lengths), common, prefix, prefix_row=1, rows=ints(rows),
+                               starts=None if starts is None else ints(starts), scale=scale, out=out)
+    assert got is out
+    got = host(got)
+    vmax = max(np.abs(values[1]).max(), np.abs(own_v).max())
+    for s, n in enumerate(lengths):
+        at = s if starts is None else int(starts[s])
+        mine = q64[at:at + counts[s]]
+        want, size = shared_reference(mine, keys[1, :prefix], values[1, :prefix], own_k[rows[s], :max(n, 0)],
+                                      own_v[rows[s], :max(n, 0)], n - counts[s],
+                                      dim ** -0.5 if scale is None else scale)
+        tol = shared_bound(size, dim, prefix + max(n, 0), vmax, want, dtype, prefix_storage)
+        assert np.all(np.abs(got[at:at + counts[s]] - want) <= tol), (s, np.abs(got[at:at + counts[s]] - want).max())
+    if starts is not None:
+        assert np.all(got[:ahead] == 7.5) and np.all(got[int(starts[-1]):] == 7.5)
+
+
+@pytest.mark.parametrize("prefix", [0, 1, 15, 64, 200, 1000])
+@pytest.mark.parametrize("storage,prefix_storage,dtype", [
+    ("u4", "u4", "f32"), ("f32", "f32", "f32"), ("bf16", "bf16", "bf16"), ("u4", "u4", "bf16"),
+    ("bf16", "u4", "bf16"), ("u4", "f32", "bf16"), ("f32", "bf16", "f32")])
+def test_shared_prefix(ops, storage, prefix_storage, dtype, prefix):
+    rng = np.random.default_rng(prefix + len(storage))
+    check_shared(ops, rng, storage, prefix_storage, dtype, 64, 4, 2, prefix, [3, 1, 0, 40, 17])
+
+
+@pytest.mark.parametrize("dim,heads,kv_heads,count", [(32, 3, 3, 7), (32, 8, 1, 40), (64, 12, 3, 33), (128, 8, 8, 70),
+                                                      (128, 16, 2, 50), (64, 5, 5, 1), (128, 24, 4, 150)])
+@pytest.mark.parametrize("storage,dtype", [("u4", "bf16"), ("bf16", "bf16"), ("u4", "f32"), ("f32", "f32")])
+def test_shared_prefix_of_many_queries(ops, dim, heads, kv_heads, count, storage, dtype):
+    rng = np.random.default_rng(dim + count)
+    check_shared(ops, rng, storage, storage, dtype, dim, heads, kv_heads, 333, list(rng.integers(0, 30, count)))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("prefix_storage", ["u4", "bf16", "f32"])
+def test_shared_prefix_with_several_tokens(ops, dtype, prefix_storage):
+    rng = np.random.default_rng(3)
+    check_shared(ops, rng, "u4", prefix_storage, dtype, 64, 6, 2, 130, [9, 5, 0, 33, 2], counts=[4, 0, 3, 33, 7],
+                 ahead=3)   # a sequence without tokens, one whose tokens have no keys, one longer than its row
+    check_shared(ops, rng, "u4", prefix_storage, dtype, 128, 8, 2, 700, [300, 41], counts=[90, 41])
+
+
+@pytest.mark.parametrize("prefix_storage", ["u4", "bf16", "f32"])
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1e-30, 3.0])
+def test_shared_prefix_scales(ops, prefix_storage, scale):
+    rng = np.random.default_rng(4)
+    for dtype in ("bf16", "f32"):
+        check_shared(ops, rng, "u4", prefix_storage, dtype, 64, 8, 2, 150, list(rng.integers(0, 9, 40)), scale=scale)
+
+
+def test_a_prefix_in_the_same_cache_and_out_over_q(ops):
+    torch = torch_()
+    rng = np.random.default_rng(5)
+    cache, k, v = filled(ops, rng, 4, 2, 90, 64, "bf16")
+    q, q64 = queries(rng, 3, 4, 64, "bf16")
+    q = q.contiguous()
+    lengths, rows = [5, 1, 30], [1, 3, 0]
+    got = ops.attention_shared(cache, q, ints(lengths), cache, 77, prefix_row=2, rows=ints(rows), out=q)
+    assert got is q
+    for s in range(3):
+        want, size = shared_reference(q64[s:s + 1], k[2, :77], v[2, :77], k[rows[s], :lengths[s]],
+                                      v[rows[s], :lengths[s]], lengths[s] - 1, 0.125)
+        assert np.all(np.abs(host(got)[s] - want[0]) <= bound(size, 64, 110, np.abs(v).max(), want, "bf16")[0])
+    # rows outside the cache have no keys of their own
+    q, q64 = queries(rng, 2, 4, 64, "f32")
+    got = host(ops.attention_shared(cache, q, ints([5, 5]), cache, 9, rows=ints([-1, 4])))
+    for s in range(2):
+        want, size = shared_reference(q64[s:s + 1], k[0, :9], v[0, :9], k[0, :0], v[0, :0], -1, 0.125)
+        assert np.all(np.abs(got[s] - want[0]) <= bound(size, 64, 9, np.abs(v).max(), want, "f32")[0])
+    # no keys at all: zeros
+    got = ops.attention_shared(cache, q, ints([0, 0]), cache, 0)
+    assert torch.equal(got, torch.zeros_like(got))
+
+
+@pytest.mark.parametrize("storage,dtype", [("bf16", "bf16"), ("f32", "f32"), ("f32", "bf16"), ("bf16", "f32")])
+@pytest.mark.parametrize("heads,count", [(2, 3), (8, 40)])
+def test_values_of_a_prefix_that_are_not_finite(ops, storage, dtype, heads, count):
+    """They count as in the formula: a NaN makes every output NaN, a key whose score is -infinity takes no
+    part, an infinite value makes its channel infinite."""
+    torch = torch_()
+    rng = np.random.default_rng(6)
+    dim, prefix = 64, 200
+    own, _, _ = filled(ops, rng, count, 2, 8, dim, storage)
+    common, keys, values = filled(ops, rng, 1, 2, prefix, dim, storage)
+    common.k[0, 0, 70] = 0.0
+    common.k[0, 0, 70, 0] = -float("inf")      # score -inf where q[0] > 0
+    common.v[0, 1, 199, 5] = float("inf")
+    q = torch.rand((count, heads, dim), device="cuda").to(getattr(torch, {"f32": "float32", "bf16": "bfloat16"}[dtype])) + 0.1
+    got = host(ops.attention_shared(own, q, ints([8] * count), common, prefix))
+    assert np.isfinite(got[:, :heads // 2]).all()
+    late = got[:, heads // 2:]
+    assert np.all(late[..., 5] == np.inf) and np.isfinite(np.delete(late, 5, -1)).all()
+    common.k[0, 1, 3, 9] = float("nan")
+    got = host(ops.attention_shared(own, q, ints([8] * count), common, prefix))
+    assert np.isfinite(got[:, :heads // 2]).all() and np.isnan(got[:, heads // 2:]).all()
+
+
+# ---- weights ---------------------------------------------------------------------------------------
+def check_weights(ops, rng, storage, dtype, dim, heads, kv_heads, lengths, counts=None, window=0, sinks=0,
+                  decay=1.0, slots=None, rows=None, in_place=True, scale=None):
+    count, slots = len(lengths), slots or max(lengths) + 3
+    cache, k, v = filled(ops, rng, count + 2, kv_heads, slots, dim, storage)
+    rows = list(rng.permutation(count + 2)[:count]) if rows is None else rows
+    starts = None if counts is None else 1 + np.concatenate([[0], np.cumsum(counts)])
+    counts = counts or [1] * count
+    tokens = count if starts is None else int(starts[-1]) + 2
+    q, q64 = queries(rng, tokens, heads, dim, dtype)
+    before = (rng.random((count + 2, kv_heads, slots)) ** 4 * 5).astype(np.float32)
+    mass = tensor(before)
+    previous = None
+    if not in_place:
+        previous, mass = mass, torch_().full_like(mass, -3.0)
+        if decay == 0:
+            previous.fill_(float("nan"))
+    kept = host(mass)
+    out = ops.attention_weights(cache, q, ints(lengths), mass, previous=previous, decay=decay, rows=ints(rows),
+                                starts=None if starts is None else ints(starts), window=window, sinks=sinks,
+                                scale=scale)
+    plain = ops.attention_cached(cache, q, ints(lengths), rows=ints(rows), window=window, sinks=sinks,
+                                 starts=None if starts is None else ints(starts), scale=scale)
+    got, out, plain = host(mass), host(out), host(plain)
+    scale = dim ** -0.5 if scale is None else scale
+    added, tol, end = np.zeros_like(before, np.float64), np.zeros_like(before, np.float64), {}
+    for s, n in enumerate(lengths):
+        first, row = (s if starts is None else int(starts[s])), rows[s]
+        inside = 0 <= row < count + 2
+        kk, vv = (x[row] if inside else x[0, :0] for x in (k, v))
+        want, size = ref.attend(q64[first:first + counts[s]], kk[:max(0, min(n, slots))], vv[:max(0, min(n, slots))],
+                                n - counts[s], window, sinks, scale)
+        for i in range(counts[s]):
+            if n - counts[s] + i >= slots:     # a token outside the cache sees nothing
+                want[i], size[i] = 0, 0
+        t = bound(size, dim, n, np.abs(v).max(), want, dtype)
+        assert np.all(np.abs(out[first:first + counts[s]] - want) <= t), s
+        assert np.all(np.abs(plain[first:first + counts[s]] - want) <= t), s
+        if not inside:
+            continue
+        end[row] = max(end.get(row, 0), min(max(n, 0), slots))
+        for i in range(counts[s]):
+            position = n - counts[s] + i
+            if position < 0 or position >= slots:
+                continue
+            seen = ref.visible(position, slots, window, sinks)
+            for h in range(heads):
+                at = h * kv_heads // heads
+                p = np.zeros(slots)
+                p[seen] = softmax(k[row, seen, at] @ q64[first + i, h] * scale)
+                added[row, at] += p
+                tol[row, at] += p * (2.2 * (dim + 8) * 2.0 ** -23 * size[i, h] + 2.0 ** -20 + (n + 16) * 2.0 ** -23)
+    want = kept.copy()
+    for row, n in end.items():
+        old = before[row, :, :n] * float(np.float32(decay)) if decay else 0.0
+        want[row, :, :n] = old + added[row, :, :n]
+        tol[row, :, :n] += 2.0 ** -22 * want[row, :, :n]
+    assert np.all(np.abs(got - want) <= tol), np.nanmax(np.abs(got - want) - tol)
+
+
+@pytest.mark.parametrize("storage,dtype", [("u4", "f32"), ("u4", "bf16"), ("bf16", "bf16"), ("f32", "f32"),
+                                           ("bf16", "f32"), ("f32", "bf16")])
+@pytest.mark.parametrize("dim,heads,kv_heads", [(32, 2, 2), (64, 8, 2), (128, 4, 4), (64, 12, 1), (128, 24, 2)])
+def test_weights(ops, storage, dtype, dim, heads, kv_heads):
+    rng = np.random.default_rng(dim + heads)
+    check_weights(ops, rng, storage, dtype, dim, heads, kv_heads, [1, 40, 0, 17, 300])
+    check_weights(ops, rng, storage, dtype, dim, heads, kv_heads, [33, 150], window=20, sinks=3, decay=0.5)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads", [(3, 3), (8, 2), (6, 1)])
+def test_weights_of_several_tokens(ops, dtype, heads, kv_heads):
+    rng = np.random.default_rng(heads)
+    for dim in (32, 64, 128):
+        check_weights(ops, rng, "u4", dtype, dim, heads, kv_heads, [20, 5, 0, 41, 2], counts=[4, 0, 2, 41, 7],
+                      decay=0.0, in_place=False)
+        check_weights(ops, rng, "u4", dtype, dim, heads, kv_heads, [60, 90, 33], counts=[8, 17, 1], window=13,
+                      sinks=5, decay=0.9)
+
+
+def test_weights_of_long_rows_are_split(ops):
+    rng = np.random.default_rng(8)
+    check_weights(ops, rng, "u4", "bf16", 128, 8, 2, [9001], decay=0.25, in_place=False)
+    check_weights(ops, rng, "u4", "f32", 64, 2, 2, [5000, 2047, 1])
+    check_weights(ops, rng, "bf16", "bf16", 64, 8, 1, [4097, 1025], window=2000, sinks=17)
+    check_weights(ops, rng, "f32", "f32", 32, 1, 1, [3000])
+
+
+def test_weights_with_rows_named_twice_outside_and_too_long(ops):
+    rng = np.random.default_rng(9)
+    for storage in ("u4", "bf16"):
+        check_weights(ops, rng, storage, "f32", 64, 4, 2, [30, 12, 25, 30, 7], rows=[2, 0, 2, 7, -1])
+        check_weights(ops, rng, storage, "f32", 64, 4, 2, [40, 39, 41], slots=40)
+        check_weights(ops, rng, storage, "bf16", 64, 4, 2, [30, 12], scale=-0.3)
+        check_weights(ops, rng, storage, "bf16", 64, 4, 2, [30, 12], scale=0.0)
+
+
+def test_weights_beside_infinities_and_nan(ops):
+    """A key of score -infinity weighs nothing; a NaN key makes the weights of the queries that see it NaN;
+    what lies behind the length, or outside the window, is not looked at."""
+    torch = torch_()
+    rng = np.random.default_rng(10)
+    for storage, dtype in (("bf16", "bf16"), ("f32", "f32"), ("f32", "bf16"), ("bf16", "f32")):
+        cache, _, _ = filled(ops, rng, 3, 2, 64, 64, storage)
+        cache.k[0, 0, 9] = 0.0
+        cache.k[0, 0, 9, 0] = -float("inf")
+        cache.k[1, 1, 20, 3] = float("nan")
+        spoil(cache, 0, 50)
+        spoil(cache, 2, 10)
+        q = torch.rand((3, 4, 64), device="cuda").to(getattr(torch, {"f32": "float32", "bf16": "bfloat16"}[dtype])) + 0.1
+        mass = torch.full((3, 2, 64), 2.0, device="cuda")
+        ops.attention_weights(cache, q, ints([50, 40, 10]), mass, decay=0.0)
+        got = host(mass)
+        assert got[0, 0, 9] == 0 and np.isfinite(got[0]).all()
+        assert np.allclose(got[0, :, :50].sum(-1), 2.0, atol=1e-4) and np.all(got[0, :, 50:] == 2)
+        assert np.isfinite(got[1, 0]).all() and np.isnan(got[1, 1, :40]).all() and np.all(got[1, :, 40:] == 2)
+        assert np.allclose(got[2, :, :10].sum(-1), 2.0, atol=1e-4) and np.all(got[2, :, 10:] == 2)
+        ops.attention_weights(cache, q, ints([50, 40, 10]), mass, decay=0.0, window=15)
+        got = host(mass)
+        assert np.isfinite(got).all() and np.all(got[1, 1, :25] == 0)
+        assert np.allclose(got[1, :, 25:40].sum(-1), 2.0, atol=1e-4)
+
+
+# ---- eviction --------------------------------------------------------------------------------------
+def kept_places(mass, length, keep, recent, sinks):
+    if length <= keep:
+        return list(range(max(length, 0)))
+    m = np.where(np.isnan(mass), -np.inf, mass)
+    middle = range(sinks, length - recent)
+    rank = [(np.isnan(mass[j]), -m[j], j) for j in middle]
+    best = [j for _, _, j in sorted(rank)[:keep - sinks - recent]]
+    return sorted([*range(sinks), *best, *range(length - recent, length)])
+
+
+def raw(cache):
+    return [t.clone() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale) if t is not None]
+
+
+def check_evict(ops, rng, storage, dim, kv_heads, slots, lengths, keep, recent=0, sinks=0, rows=None, to=None,
+                to_rows=None, mass=None):
+    torch = torch_()
+    count, n_rows = len(lengths), len(lengths) + 1
+    cache, _, _ = filled(ops, rng, n_rows, kv_heads, slots, dim, storage)
+    before = raw(cache)
+    m = (rng.random((n_rows, kv_heads, slots)) ** 3).astype(np.float32) if mass is None else mass(n_rows, kv_heads, slots)
+    masses = tensor(m)
+    use = list(range(count)) if rows is None else rows
+    given = None if rows is None else ints(rows)
+    target = None
+    if to is not None:
+        target = ops.KvCache.allocate(n_rows, kv_heads, to, dim, storage)
+        old = raw(target)
+        to_mass = torch.full((n_rows, kv_heads, to), 9.0, device="cuda")
+        new, kept = ops.kv_evict(cache, masses, ints(lengths), keep, recent, sinks, rows=given, to=target,
+                                 to_mass=to_mass, to_rows=None if to_rows is None else ints(to_rows))
+        dest = list(range(count)) if to_rows is None else to_rows
+        assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(raw(cache), before))
+        assert torch.equal(masses.view(torch.int32), tensor(m).view(torch.int32))
+    else:
+        old = [t.clone() for t in before]
+        new, kept = ops.kv_evict(cache, masses, ints(lengths), keep, recent, sinks, rows=given)
+        target, to_mass, dest = cache, masses, use
+        to = slots
+    want_kept = np.full((count, kv_heads, keep), -1)
+    want_new = np.zeros(count, int)
+    want_mass = np.full((n_rows, kv_heads, to), 9.0, np.float32) if target is not cache else m.copy()
+    want = [t.clone() for t in old]
+    for s, length in enumerate(lengths):
+        there = 0 <= dest[s] < n_rows and dest[s] not in dest[:s]
+        length = min(max(length, 0), slots) if there and 0 <= use[s] < n_rows else 0
+        want_new[s] = min(length, keep)
+        if not there:
+            continue
+        for h in range(kv_heads):
+            places = kept_places(m[use[s], h], length, keep, recent, sinks) if length else []
+            want_kept[s, h, :len(places)] = places
+            want_mass[dest[s], h, :len(places)] = m[use[s], h, places] if places else []
+            want_mass[dest[s], h, len(places):] = 0
+            for x, y in zip(want, before):
+                if places:
+                    x[dest[s], h, :len(places)] = y[use[s], h, torch.tensor(places, device="cuda")]
+    assert np.array_equal(new.cpu().numpy(), want_new)
+    assert np.array_equal(kept.cpu().numpy(), want_kept)
+    assert np.array_equal(to_mass.cpu().numpy(), want_mass, equal_nan=True)
+    for x, y in zip(raw(target), want):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
+@pytest.mark.parametrize("storage", ["u4", "bf16", "f32"])
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("to", [None, 57])
+def test_evict(ops, storage, dim, to):
+    rng = np.random.default_rng(dim)
+    check_evict(ops, rng, storage, dim, 3, 200, [200, 51, 50, 49, 0, 1, 130], 50, 8, 4, to=to)
+    check_evict(ops, rng, storage, dim, 1, 90, [80, 90, 33], 33, 0, 0, rows=[2, 0, 3], to=to)
+    check_evict(ops, rng, storage, dim, 2, 90, [80, 90, 33], 20, 16, 4, to=to)       # nothing by mass
+    check_evict(ops, rng, storage, dim, 2, 40, [40, 7], 1, 0, 1, to=to)
+    check_evict(ops, rng, storage, dim, 2, 40, [40, 7], 1, 0, 0, to=to)
+
+
+@pytest.mark.parametrize("to", [None, 5000])
+@pytest.mark.parametrize("slots,keep", [(4096, 4095), (4097, 1), (9000, 4500), (20000, 3001)])
+def test_evict_long_rows(ops, to, slots, keep):
+    rng = np.random.default_rng(slots)
+    check_evict(ops, rng, "u4", 32, 2, slots, [slots, slots - 1], keep, min(keep // 3, 900), min(keep // 2, 3), to=to)
+    check_evict(ops, rng, "bf16", 64, 1, slots, [slots], keep, 0, 0, to=to)
+
+
+@pytest.mark.parametrize("to", [None, 300])
+def test_evict_ties_signs_and_nan(ops, to):
+    rng = np.random.default_rng(11)
+
+    def few(*shape):
+        return rng.choice(np.float32([0.0, -0.0, 1.0, 0.5, -2.0]), shape)
+
+    def odd(*shape):
+        m = rng.standard_normal(shape).astype(np.float32)
+        m[rng.random(shape) < 0.3] = np.nan
+        m[rng.random(shape) < 0.1] = np.inf
+        m[rng.random(shape) < 0.1] = -np.inf
+        m[rng.random(shape) < 0.1] = 1e-42
+        return m
+
+    def close(*shape):   # masses that differ in their last bits
+        return (np.float32(1.0) + rng.integers(0, 4, shape).astype(np.float32) * np.float32(2.0 ** -23))
+
+    for mass in (few, odd, close, lambda *shape: np.ones(shape, np.float32), lambda *shape: np.full(shape, np.nan, np.float32)):
+        check_evict(ops, rng, "u4", 32, 2, 5000, [5000, 4999, 299], 300, 20, 4, to=to, mass=mass)
+
+
+def test_evict_rows_named_twice_and_outside(ops):
+    rng = np.random.default_rng(12)
+    check_evict(ops, rng, "bf16", 64, 2, 60, [60, 50, 40, 30], 20, 4, 2, rows=[1, 1, -1, 5])
+    check_evict(ops, rng, "bf16", 64, 2, 60, [60, 50, 40, 30], 20, 4, 2, rows=[1, 1, 0, 0], to=33, to_rows=[2, 3, 2, 0])
+    check_evict(ops, rng, "u4", 64, 2, 60, [60, 50, 40, 99], 20, 4, 2, rows=[1, 7, 0, 3], to=33, to_rows=[9, 3, -1, 0])
+
+
+# ---- together --------------------------------------------------------------------------------------
+@pytest.mark.parametrize("storage,dtype", [("u4", "bf16"), ("u4", "f32"), ("bf16", "bf16"), ("f32", "f32")])
+def test_a_server_with_a_budget(ops, storage, dtype):
+    """Prompts whose last queries vote are evicted into a small cache; decode steps behind a shared prefix
+    append, attend, gather weight, and evict in place. Every step against 64 bits on what the cache holds."""
+    torch = torch_()
+    rng = np.random.default_rng(13)
+    heads, kv_heads, dim, budget, slack = 4, 2, 64, 48, 6
+    lengths = [150, 90, 31]
+    prompts, _, _ = filled(ops, rng, 3, kv_heads, 150, dim, storage)
+    system, sys_k, sys_v = filled(ops, rng, 1, kv_heads, 80, dim, storage)
+    votes = torch.zeros((3, kv_heads, 150), device="cuda")
+    q, _ = queries(rng, 3, heads, dim, dtype)
+    ops.attention_weights(prompts, q, ints(lengths), votes, decay=0.0)
+    cache = ops.KvCache.allocate(3, kv_heads, budget + slack, dim, storage)
+    mass = torch.full((3, kv_heads, budget + slack), float("nan"), device="cuda")
+    at, kept = ops.kv_evict(prompts, votes, ints(lengths), budget, 8, 4, to=cache, to_mass=mass)
+    assert at.tolist() == [48, 48, 31]
+    for step in range(2 * slack):
+        at = at + 1
+        new = torch.from_numpy(rng.standard_normal((2, 3, kv_heads, dim)).astype(np.float32)).cuda().to(q.dtype)
+        ops.kv_append(cache, new[0], new[1], at)
+        q, q64 = queries(rng, 3, heads, dim, dtype)
+        n = at.tolist()
+        k, v = (host(t).reshape(3, -1, kv_heads, dim) for t in ops.kv_read(
+            cache, ints([budget + slack] * 3), starts=ints(np.arange(4) * (budget + slack)), tokens=3 * (budget + slack)))
+        old = host(mass)
+        own = host(ops.attention_weights(cache, q, at, mass))
+        out = host(ops.attention_shared(cache, q, at, system, 80))
+        gained = host(mass) - old
+        for s in range(3):
+            want, size = ref.attend(q64[s:s + 1], k[s, :n[s]], v[s, :n[s]], n[s] - 1, 0, 0, 0.125)
+            assert np.all(np.abs(own[s] - want[0]) <= bound(size, dim, n[s], np.abs(v).max(), want, dtype)[0])
+            want, size = shared_reference(q64[s:s + 1], sys_k[0], sys_v[0], k[s, :n[s]], v[s, :n[s]], n[s] - 1, 0.125)
+            vmax = max(np.abs(v).max(), np.abs(sys_v).max())
+            assert np.all(np.abs(out[s] - want[0]) <= shared_bound(size, dim, 80 + n[s], vmax, want, dtype, storage)[0])
+            assert np.allclose(gained[s, :, :n[s]].sum(-1), heads // kv_heads, atol=1e-3)
+            assert np.all(old[s, :, n[s] - 1] == 0) and np.all(host(mass)[s, :, n[s]:] == 0)
+        if max(n) == budget + slack:
+            at, kept = ops.kv_evict(cache, mass, at, budget, 8, 4)
+            assert at.tolist() == [min(x, budget) for x in n]
+
+
+def test_captured_and_on_other_streams(ops):
+    """A decode step captured once and replayed with new inputs equals the calls; calls on a side stream too."""
+    torch = torch_()
+    rng = np.random.default_rng(14)
+    cache, _, _ = filled(ops, rng, 8, 2, 2000, 64, "u4")
+    system, _, _ = filled(ops, rng, 1, 2, 500, 64, "bf16")
+    to = ops.KvCache.allocate(8, 2, 300, 64, "u4")
+    q = torch.randn((8, 8, 64), device="cuda").bfloat16()
+    lengths = ints(rng.integers(500, 2000, 8))
+    mass, to_mass = torch.rand((8, 2, 2000), device="cuda"), torch.zeros((8, 2, 300), device="cuda")
+
+    def step(stream=None):
+        new = torch.zeros_like(mass) if stream is None else None
+        if new is None:
+            with torch.cuda.stream(stream):
+                new = torch.zeros_like(mass)
+        a = ops.attention_shared(cache, q, lengths, system, 500, stream=stream)
+        b = ops.attention_weights(cache, q, lengths, new, previous=mass, decay=0.5, stream=stream)
+        n, kept = ops.kv_evict(cache, new, lengths, 250, 20, 4, to=to, to_mass=to_mass, stream=stream)
+        return a, b, new, n, kept, to_mass.clone() if stream is None else to_mass
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        held = step()
+    for seed in range(3):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        q.copy_(torch.randn(q.shape, generator=g, device="cuda"))
+        lengths.copy_(torch.randint(200, 2000, (8,), generator=g, device="cuda", dtype=torch.int32))
+        graph.replay()
+        want = [t.clone() for t in held]
+        again = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(want, again))
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        third = step(side)
+        side.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(want, third))
