@@ -21,10 +21,10 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-I", str(INCLUDE),
           "-I", str(CSRC)]
 SOURCES = ["kernels.cu", "gemm_tc.cu", "decode_fused.cu", "ops.cu", "ops_static.cu", "tensors.cu",
-           "kv_cache.cu", "kv_evict.cu", "attention_cached.cu", "attention_packed.cu", "attention_shared.cu",
+           "kv_cache.cu", "kv_evict.cu", "attention_cached.cu", "attention_packed.cu", "attention_prefix.cu", "attention_shared.cu",
            "attention_weights.cu", "sample.cu", "operators.cpp", "engine.cpp"]
 HEADERS = ["kernels.h", "java_random.h", "epilogue.cuh", "device.cuh", "select.cuh",
-           "operators.h", "attention.cuh", "attention_cached.cuh",
+           "operators.h", "attention.cuh", "attention_cached.cuh", "attention_tc.cuh",
            "sm100.cuh"]
 
 

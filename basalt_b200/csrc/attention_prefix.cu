@@ -1,0 +1,632 @@
+// Attention of a whole batch's queries over one prefix, on tcgen05: the sums of attention_shared's first pass.
+//
+//   S = Q K^T,  P = exp2(S f - m),  O = P V  over a share of the prefix's keys; m the running maximum
+//
+// A CTA takes 256 query rows of one key head (tokens x heads of its group: every row sees every key, so nothing
+// but the end of the prefix is masked) and a share of the keys, in tiles of 64: two M = 128 tiles of queries,
+// whose scores, weights and outputs live in TMEM and take turns, as in attention over packed prompts. It leaves
+// outputs, maximum and sum of weights of every row in float32; the shares are joined with the sequences' own
+// keys' sums. Weights are bf16 (8 bits) in the product with values, whose rounding is of the size of bf16
+// outputs' own; maxima and sums are float32.
+//
+// A 4-bit prefix is unpacked on its way into shared memory by four warps in the copy's place, so that every key
+// is unpacked once for 256 rows: keys become fp16 (11 bits; a tile is brought near one by a power of two, and so
+// is every query row, which the scores' factor f takes back), because an error of a score grows with it; values
+// become bf16 as weights are, by one fused multiply-add a value pair, rounded once.
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <cfloat>
+
+#include "attention_tc.cuh"
+#include "operators.h"
+
+namespace bst {
+namespace {
+
+constexpr int kRows = 256;
+// Warps 0-3 and 4-7: a tile's rows, a thread each; 8: products; 9 on: copies, or four warps that unpack.
+constexpr int kSoft = 256, kUnpack = 128;
+template <bool CODES>
+constexpr int kThreadsOf = kSoft + 32 + (CODES ? kUnpack : 32);
+
+template <int HD>
+struct PrefixLayout {
+    static constexpr int kQuery = 128 * HD * 2;       // a tile of query rows
+    static constexpr int kTile = kTcKeys * HD * 2;    // a tile of keys or values
+    static constexpr int kSlots = 8;
+    static constexpr int kBars = 2 * kQuery + kSlots * kTile;
+    static constexpr int kEnd = kBars + 256 + (kRows + 16) * 4;
+    // More than half of an SM's shared memory: one CTA an SM, which owns all of TMEM.
+    static constexpr int kBytes = kEnd > 120 * 1024 ? kEnd : 120 * 1024;
+    static constexpr int kSmem = kBytes + 1024;       // the base is aligned to 1024 bytes
+    static_assert(kSlots * kTile >= kRows * HD * 4, "outputs are staged in the ring");
+};
+
+// The channels of one head of one key of a 4-bit cache, for rows that are added up plainly.
+__device__ __forceinline__ float code_value(const unsigned char* codes, const __nv_bfloat16* scales, int groups,
+                                            int channel) {
+    const int g = channel >> 5, h = (channel >> 2) & 7, j = channel & 3;
+    const int byte = codes[(h * groups + g) * 2 + (j >> 1)];
+    return fmaf(static_cast<float>(j & 1 ? byte >> 4 : byte & 15), __bfloat162float(scales[2 * g]),
+                __bfloat162float(scales[2 * g + 1]));
+}
+
+__device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t sub_f16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+__device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+
+// 2^e for e in [-126, 127], and the e for which |x| < 2^e, within [-100, 126] (0 for zero).
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
+__device__ __forceinline__ int exponent_above(uint32_t bits) {
+    return bits == 0u ? 0 : max(min(static_cast<int>(bits >> 23) - 126, 126), -100);
+}
+
+// One word of codes (nibble j of the low half: channel j of one group; of the high half: of the next) and its
+// successor (the next four channels) as 16 bytes for each of the two groups.
+template <bool KEYS>
+__device__ __forceinline__ void unpack(uint32_t a, uint32_t b, uint32_t step, uint32_t low, uint4* first,
+                                       uint4* second) {
+    // 1024 + c in fp16, 128 + c in bf16: both exact, as is c.
+    constexpr uint32_t base = KEYS ? 0x64006400u : 0x43004300u;
+    uint32_t x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const uint32_t w = ((j < 4 ? a : b) >> (4 * (j & 3)) & 0x000f000fu) | base;
+        x[j] = KEYS ? fma_f16x2(sub_f16x2(w, base), step, low) : fma_bf16x2(sub_bf16x2(w, base), step, low);
+    }
+    *first = make_uint4(__byte_perm(x[0], x[1], 0x5410), __byte_perm(x[2], x[3], 0x5410),
+                        __byte_perm(x[4], x[5], 0x5410), __byte_perm(x[6], x[7], 0x5410));
+    *second = make_uint4(__byte_perm(x[0], x[1], 0x7632), __byte_perm(x[2], x[3], 0x7632),
+                         __byte_perm(x[4], x[5], 0x7632), __byte_perm(x[6], x[7], 0x7632));
+}
+
+template <int HD, bool CODES>
+__global__ void __launch_bounds__(kThreadsOf<CODES>, 1)
+k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, Prefix prefix,
+            Batch b, AttnSpec a, const __nv_bfloat16* __restrict__ q, int64_t q_stride, int tiles, int splits,
+            float* __restrict__ part) {
+    using L = PrefixLayout<HD>;
+    constexpr int kBlocks = HD / 64;     // 128-byte columns of a tile
+    extern __shared__ unsigned char raw[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int group = a.heads / a.kv_heads;
+    // The tiles of a share of a head's keys stand next to one another, so that they read it together.
+    const int kvh = blockIdx.x / tiles % a.kv_heads, split = blockIdx.x / tiles / a.kv_heads;
+    int first, n;
+    if (!owned_tokens(b, &first, &n)) return;
+    const int64_t r0 = static_cast<int64_t>(blockIdx.x % tiles) * kRows;
+    if (r0 >= static_cast<int64_t>(n) * group) return;
+    const int rows = static_cast<int>(min(static_cast<int64_t>(kRows), static_cast<int64_t>(n) * group - r0));
+    const int all = (prefix.length + kTcKeys - 1) / kTcKeys;
+    const int t0 = static_cast<int>(static_cast<int64_t>(all) * split / splits);
+    const int key_tiles = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / splits) - t0;  // at least one
+    const int halves = rows > 128 ? 2 : 1;
+
+    const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+    unsigned char* const smem = raw + (base - smem_u32(raw));
+    uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
+    uint64_t* const full = bars;                 // [kSlots] a tile has arrived
+    uint64_t* const empty = full + L::kSlots;    // [kSlots] its readers are done
+    uint64_t* const s_full = empty + L::kSlots;  // [half][buffer] scores are done
+    uint64_t* const p_full = s_full + 4;         // [half][buffer] weights are written
+    uint64_t* const o_done = p_full + 4;         // [half] a product into O is done
+    // [half] the last one is. (Its phase of o_done can be over, and the parity of the one before it be that of
+    // the next, when a warp that was held up comes to wait for that.)
+    uint64_t* const o_last = o_done + 2;
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(o_last + 2);
+    int* const status = reinterpret_cast<int*>(tmem_slot + 1);  // [0] error code, [1] abort
+    float* const row_factor = reinterpret_cast<float*>(smem + L::kBars + 256);  // what a row was divided by
+    float* const tile_factor = row_factor + kRows;                              // and a tile of keys, [8]
+    uint32_t* const warp_most = reinterpret_cast<uint32_t*>(tile_factor + 8);   // [2][4]
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < L::kSlots; ++i) {
+            mbar_init(full + i, CODES ? kUnpack : 1);
+            mbar_init(empty + i, 1);
+        }
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(s_full + i, 1);
+            mbar_init(p_full + i, kSoft / 2);
+        }
+        for (int i = 0; i < 4; ++i) mbar_init(o_done + i, 1);
+        status[0] = status[1] = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         smem_u32(tmem_slot)),
+                     "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    // Token and head of the CTA's query row `at`: the quotient of two small numbers, in float.
+    const int token0 = static_cast<int>(r0 / group), r_first = static_cast<int>(r0 - static_cast<int64_t>(token0) * group);
+    const float by_group = 1.0f / static_cast<float>(group);
+    auto place = [&](int at, int64_t* token, int* head) {
+        const int x = static_cast<int>((static_cast<float>(r_first + at) + 0.5f) * by_group);
+        *token = static_cast<int64_t>(first) + token0 + x;
+        *head = kvh * group + r_first + at - x * group;
+    };
+    __syncthreads();  // the barriers are there: copies may start
+    // The tiles in the order in which they are used: K0 K1 V0 K2 V1 K3 ... V(n-1).
+    const int copies = 2 * key_tiles;
+    auto k_copy = [&](int i) { return i == 0 ? 0 : 2 * i - 1; };
+    auto v_copy = [&](int i) { return i == key_tiles - 1 ? 2 * i + 1 : 2 * i + 2; };
+    auto copy_of_keys = [&](int i) { return i == 0 || ((i & 1) && i != copies - 1); };
+    auto copy_tile = [&](int i) {
+        return i == 0 ? 0 : (copy_of_keys(i) ? (i + 1) / 2 : (i == copies - 1 ? key_tiles - 1 : i / 2 - 1));
+    };
+    auto copy = [&](int i) {
+        const int slot = i % L::kSlots;
+        mbar_expect_tx(full + slot, L::kTile);
+        for (int x = 0; x < kBlocks; ++x) {
+            tma_load_3d(copy_of_keys(i) ? &k_map : &v_map, full + slot,
+                        smem + 2 * L::kQuery + slot * L::kTile + x * (kTcKeys * 128), 64 * x,
+                        (t0 + copy_tile(i)) * kTcKeys, kvh);
+        }
+    };
+    volatile int* const abort = status + 1;
+    auto await = [&](int i, int code) {
+        return mbar_wait(full + i % L::kSlots, (i / L::kSlots) & 1, status, code, abort);
+    };
+    if (!CODES && threadIdx.x == 9 * 32) {
+        for (int i = 0; i < min(copies, L::kSlots); ++i) copy(i);
+    }
+    // Queries, 16-byte chunks into the swizzle, all loads of a thread at once. A negative scale moves
+    // into them.
+    if (threadIdx.x < kSoft) {
+        const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+        constexpr int kLoads = kRows * (HD / 8) / kSoft;
+        uint4 x[kLoads];
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int at = (threadIdx.x + i * kSoft) / (HD / 8), c = threadIdx.x % (HD / 8);
+            int64_t token;
+            int head;
+            place(at, &token, &head);
+            x[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (at < rows) x[i] = *reinterpret_cast<const uint4*>(q + token * q_stride + head * HD + 8 * c);
+        }
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int at = (threadIdx.x + i * kSoft) / (HD / 8), c = threadIdx.x % (HD / 8), r = at & 127;
+            uint32_t w[4] = {x[i].x ^ flip, x[i].y ^ flip, x[i].z ^ flip, x[i].w ^ flip};
+            if constexpr (CODES) {
+                // The row to fp16 below 2^8, by the exponent of its largest.
+                uint32_t most = 0u;
+#pragma unroll
+                for (int y = 0; y < 4; ++y) most = max(most, max((w[y] << 16) & 0x7fff0000u, w[y] & 0x7fff0000u));
+#pragma unroll
+                for (int o = HD / 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(kFull, most, o));
+                const int e = exponent_above(most);
+                const float by = power_of_two(-e);
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    w[y] = half2_of(__uint_as_float(w[y] << 16) * by * 256.0f,
+                                    __uint_as_float(w[y] & 0xffff0000u) * by * 256.0f);
+                }
+                // A query that is not finite makes every score NaN.
+                if (c == 0) row_factor[at] = most >= 0x7f800000u ? NAN : power_of_two(e) * 0x1p-8f;
+            }
+            *reinterpret_cast<uint4*>(smem + (at >> 7) * L::kQuery + r * 128 + (c >> 3) * 16384 +
+                                      (((c & 7) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *tmem_slot;
+    if (warp >= 9) {
+        if constexpr (!CODES) {
+            if (lane == 0) {
+                for (int i = L::kSlots; i < copies; ++i) {
+                    if (!mbar_wait(empty + i % L::kSlots, ((i / L::kSlots) - 1) & 1, status, 1, abort)) break;
+                    copy(i);
+                }
+            }
+        } else {
+            // A key a thread, or half of one with 128 channels: chunks of 16 code bytes.
+            constexpr int G = HD / 32, kChunks = HD / 32 / (kUnpack / kTcKeys);
+            const int tid = threadIdx.x - 9 * 32, key = tid & (kTcKeys - 1), part_of = tid / kTcKeys;
+            const int64_t at = (static_cast<int64_t>(prefix.row) * a.kv_heads + kvh) * prefix.cache.slots;
+            struct Held {
+                uint4 codes[kChunks];
+                uint32_t scale[G];
+            };
+            auto load = [&](int i, Held& h) {
+                const int my_key = (t0 + copy_tile(i)) * kTcKeys + key;
+                const bool keys = copy_of_keys(i);
+                if (i < copies && my_key < prefix.length) {
+                    const char* codes = static_cast<const char*>(keys ? prefix.cache.k : prefix.cache.v) +
+                                        (at + my_key) * (HD / 2) + part_of * kChunks * 16;
+                    const char* scale = static_cast<const char*>(keys ? prefix.cache.k_scale : prefix.cache.v_scale) +
+                                        (at + my_key) * (G * 4);
+#pragma unroll
+                    for (int x = 0; x < kChunks; ++x) h.codes[x] = __ldg(reinterpret_cast<const uint4*>(codes) + x);
+                    if constexpr (G == 4) {
+                        const uint4 s = __ldg(reinterpret_cast<const uint4*>(scale));
+                        h.scale[0] = s.x; h.scale[1] = s.y; h.scale[2] = s.z; h.scale[3] = s.w;
+                    } else {
+                        const uint2 s = __ldg(reinterpret_cast<const uint2*>(scale));
+                        h.scale[0] = s.x; h.scale[1] = s.y;
+                    }
+                } else {  // behind the prefix: zeros
+#pragma unroll
+                    for (int x = 0; x < kChunks; ++x) h.codes[x] = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+                    for (int g = 0; g < G; ++g) h.scale[g] = 0u;
+                }
+            };
+            auto store = [&](int i, const Held& h, bool keys, float by) {
+                unsigned char* const to = smem + 2 * L::kQuery + (i % L::kSlots) * L::kTile + key * 128;
+#pragma unroll
+                for (int g = 0; g < G; g += 2) {
+                    uint32_t step = __byte_perm(h.scale[g], h.scale[g + 1], 0x5410);
+                    uint32_t low = __byte_perm(h.scale[g], h.scale[g + 1], 0x7632);
+                    if (keys) {
+                        step = half2_of(__uint_as_float(step << 16) * by, __uint_as_float(step & 0xffff0000u) * by);
+                        low = half2_of(__uint_as_float(low << 16) * by, __uint_as_float(low & 0xffff0000u) * by);
+                    }
+#pragma unroll
+                    for (int x = 0; x < kChunks * 4 / G; ++x) {  // eight channels of both groups
+                        // Words of a chunk: [two halves of eight channels][pairs of groups], or, with two
+                        // groups, [four halves].
+                        const uint32_t w[4] = {h.codes[G == 4 ? x : 0].x, h.codes[G == 4 ? x : 0].y,
+                                               h.codes[G == 4 ? x : 0].z, h.codes[G == 4 ? x : 0].w};
+                        const uint32_t a0 = G == 4 ? w[g / 2] : w[2 * x], a1 = G == 4 ? w[2 + g / 2] : w[2 * x + 1];
+                        const int eighth = part_of * (kChunks * 4 / G) + x;  // which eight of a group's 32
+                        uint4 one, two;
+                        if (keys) {
+                            unpack<true>(a0, a1, step, low, &one, &two);
+                        } else {
+                            unpack<false>(a0, a1, step, low, &one, &two);
+                        }
+                        unsigned char* const block = to + (g >> 1) * (kTcKeys * 128);
+                        *reinterpret_cast<uint4*>(block + ((eighth ^ (key & 7)) << 4)) = one;
+                        *reinterpret_cast<uint4*>(block + (((4 + eighth) ^ (key & 7)) << 4)) = two;
+                    }
+                }
+            };
+            Held now, next;
+            load(0, now);
+            bool ok = true;
+            for (int i = 0; i < copies; ++i) {
+                load(i + 1, next);
+                const bool keys = copy_of_keys(i);
+                float by = 1.0f;
+                if (keys) {
+                    // The tile's largest key is at most max |low| + 15 step (not of a NaN).
+                    const int tile = copy_tile(i);
+                    uint32_t most = 0u;
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {
+                        const float top = fmaf(15.0f, __uint_as_float(now.scale[g] << 16),
+                                               fabsf(__uint_as_float(now.scale[g] & 0xffff0000u)));
+                        most = max(most, top <= FLT_MAX ? __float_as_uint(top) : (isnan(top) ? 0u : 0x7f000000u));
+                    }
+                    most = __reduce_max_sync(kFull, most);
+                    if (lane == 0) warp_most[(tile & 1) * 4 + (warp - 9)] = most;
+                    asm volatile("bar.sync 3, %0;" ::"n"(kUnpack) : "memory");
+                    const uint32_t* const all_most = warp_most + (tile & 1) * 4;
+                    const int e = exponent_above(max(max(all_most[0], all_most[1]), max(all_most[2], all_most[3])));
+                    by = power_of_two(-e);
+                    if (tid == 0) tile_factor[tile & 7] = power_of_two(e);
+                }
+                if (ok && i >= L::kSlots) {
+                    ok = mbar_wait(empty + i % L::kSlots, ((i / L::kSlots) - 1) & 1, status, 1, abort);
+                }
+                if (ok) {  // a wait that ran out ends no loop: the warps meet at the barrier above
+                    store(i, now, keys, by);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    mbar_arrive(full + i % L::kSlots);
+                }
+                now = next;
+            }
+        }
+    } else if (warp == 8) {
+        // The whole warp keeps time; one lane issues. Tiles are multiplied whole (what lies behind
+        // their keys is masked), and all of TMEM starts at address 0, so that operands are constants but for
+        // the slot.
+        const int n_tiles = __shfl_sync(kFull, key_tiles, 0), n_halves = __shfl_sync(kFull, halves, 0);
+        constexpr uint32_t s_idesc = tc_idesc(kTcKeys, false, CODES), o_idesc = tc_idesc(HD, true);
+        const uint32_t q_desc = desc_k(base), kv_at = base + 2 * L::kQuery;
+        auto slot = [&](int i) { return kv_at + (i % L::kSlots) * L::kTile; };
+        auto scores = [&](int half, int i) {  // S = Q K^T
+            const uint32_t d = half * 256 + (i & 1) * 64;
+            const uint32_t qa = q_desc + half * (L::kQuery >> 4), ka = desc_k(slot(k_copy(i)));
+#pragma unroll
+            for (int k = 0; k < HD / 16; ++k) {
+                tc_mma_ss(d, qa + (k >> 2) * (16384 >> 4) + (k & 3) * 2,
+                          ka + (k >> 2) * (kTcKeys * 128 >> 4) + (k & 3) * 2, kDescHigh, s_idesc, k > 0);
+            }
+            mma_commit(s_full + 2 * half + (i & 1));
+        };
+        bool ok = true;
+        for (int i = 0; ok && i < min(2, n_tiles); ++i) {
+            ok = await(k_copy(i), 2);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (elect_one()) {
+                scores(0, i);
+                if (n_halves > 1) scores(1, i);
+                mma_commit(empty + k_copy(i) % L::kSlots);
+            }
+            __syncwarp();
+        }
+#pragma unroll 2
+        for (int i = 0; ok && i < n_tiles; ++i) {
+            const bool more = i + 2 < n_tiles;
+            ok = await(v_copy(i), 3) && (!more || await(k_copy(i + 2), 4));
+            const uint32_t va = desc_mn(slot(v_copy(i)));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (h >= n_halves || !ok) break;
+                ok = mbar_wait(p_full + 2 * h + (i & 1), (i >> 1) & 1, status, 5, abort);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (elect_one()) {
+                    const uint32_t p = h * 256 + (i & 1) * 64;
+#pragma unroll
+                    for (int k = 0; k < kTcKeys / 16; ++k) {  // O += P V
+                        tc_mma_ts(h * 256 + 128, p + 8 * k, va + k * (2048 >> 4), kDescHigh, o_idesc,
+                                  i > 0 || k > 0);
+                    }
+                    mma_commit(i + 1 < n_tiles ? o_done + h : o_last + h);
+                    // Into the buffer that the product above has just read.
+                    if (more) scores(h, i + 2);
+                }
+                __syncwarp();
+            }
+            if (ok && elect_one()) {
+                mma_commit(empty + v_copy(i) % L::kSlots);
+                if (more) mma_commit(empty + k_copy(i + 2) % L::kSlots);
+            }
+            __syncwarp();
+        }
+    } else {
+        const int half = warp >> 2, in_tile = threadIdx.x & 127, at = 128 * half + in_tile;
+        const uint32_t s_at = tmem + half * 256 + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
+        const uint32_t o_at = s_at + 128;
+        // A score's factor to base 2. It stays above zero: the mask's -infinity is multiplied by it.
+        const float scale = fabsf(a.scale) * kLog2e * (CODES ? row_factor[at] : 1.0f);
+        float top = -INFINITY, total = 0.0f;
+        // A wait that runs out ends no loop here: the tile's threads meet at a barrier behind it, and
+        // what they write then is computed again.
+        bool ok = true;
+        for (int i = 0; half < halves && i < key_tiles; ++i) {
+            const uint32_t buffer = s_at + (i & 1) * 64;
+            uint32_t s[2][32];
+            ok = ok && mbar_wait(s_full + 2 * half + (i & 1), (i >> 1) & 1, status, 7, abort);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            tmem_ld32(buffer, s[0]);
+            tmem_ld32(buffer + 32, s[1]);
+            float by = CODES ? scale * tile_factor[i & 7] : scale;
+            by = by < FLT_MIN ? FLT_MIN : by;
+            tmem_ld_wait();
+            const int left = prefix.length - (t0 + i) * kTcKeys;  // keys of the tile, or more
+            if (left < kTcKeys) {
+#pragma unroll
+                for (int x = 0; x < 64; ++x) {
+                    if (x >= left) s[x >> 5][x & 31] = 0xff800000u;
+                }
+            }
+            float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int x = 0; x < 64; ++x) m[x & 3] = fmaxf(m[x & 3], __uint_as_float(s[x >> 5][x & 31]));
+            const float most = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * by;
+            // The maximum that weights are taken against moves only when a row's grows by more than 2^8.
+            const bool move = most > top + 8.0f || (top == -INFINITY && most > top);
+            if (__any_sync(kFull, move)) {
+                const float keep = move ? (top == -INFINITY ? 0.0f : exp2_fast(top - most)) : 1.0f;
+                if (move) top = most;
+                total *= keep;
+                if (i > 0) {
+                    ok = ok && mbar_wait(o_done + half, (i - 1) & 1, status, 8, abort);
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                    for (int c = 0; c < HD / 32; ++c) {
+                        uint32_t o[32];
+                        tmem_ld32(o_at + 32 * c, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * keep);
+                        tmem_st16(o_at + 32 * c, o);
+                        tmem_st16(o_at + 32 * c + 16, o + 16);
+                    }
+                }
+            }
+            const float from = top == -INFINITY ? 0.0f : top;
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                uint32_t p[16];
+#pragma unroll
+                for (int x = 0; x < 16; ++x) {
+                    const float e0 = exp2_fast(fmaf(__uint_as_float(s[c][2 * x]), by, -from));
+                    const float e1 = exp2_fast(fmaf(__uint_as_float(s[c][2 * x + 1]), by, -from));
+                    sum[(2 * x) & 3] += e0;
+                    sum[(2 * x + 1) & 3] += e1;
+                    p[x] = pack2(e0, e1);
+                }
+                tmem_st16(buffer + 16 * c, p);
+            }
+            total += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tmem_st_wait();
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            mbar_arrive(p_full + 2 * half + (i & 1));
+        }
+        if (half < halves) {
+            // Products are done in order.
+            ok = ok && mbar_wait(o_last + half, 0, status, 9, abort);
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        // Both halves' products are done, so the ring may hold the rows, which are then written whole.
+        asm volatile("bar.sync 1, %0;" ::"n"(kSoft) : "memory");
+        unsigned char* const rows_at = smem + 2 * L::kQuery;
+        if (half < halves) {
+#pragma unroll
+            for (int c = 0; c < HD / 32; ++c) {
+                uint32_t o[32];
+                tmem_ld32(o_at + 32 * c, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int x = 0; x < 8; ++x) {
+                    *reinterpret_cast<uint4*>(rows_at + at * (HD * 4) + (((8 * c + x) ^ (in_tile & 7)) << 4)) =
+                        make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+                }
+            }
+            if (at < rows) {
+                int64_t token;
+                int head;
+                place(at, &token, &head);
+                float* const to = part + ((token * a.heads + head) * splits + split) * (HD + 2) + HD;
+                *reinterpret_cast<float2*>(to) = make_float2(top, total);
+            }
+        }
+        __syncwarp();
+        // A warp writes the rows that its own threads staged.
+        for (int r = 0; half < halves && r < 32; ++r) {
+            const int row = 32 * warp + r;
+            if (row >= rows) break;
+            int64_t token;
+            int head;
+            place(row, &token, &head);
+            float* const to = part + ((token * a.heads + head) * splits + split) * (HD + 2);
+#pragma unroll
+            for (int x = 0; x < HD / 64; ++x) {
+                const int c = 2 * lane + 64 * x;  // channels c and c + 1
+                *reinterpret_cast<float2*>(to + c) = *reinterpret_cast<const float2*>(
+                    rows_at + row * (HD * 4) + (((c >> 2) ^ (row & 7)) << 4) + (c & 3) * 4);
+            }
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    const bool again = status[0] != 0;
+    if (again && threadIdx.x == 0) {
+        // A wait ran out: let the copies that were issued land before the memory goes away.
+        const uint64_t start = global_ns();
+        while (global_ns() - start < 2000000ull) {
+        }
+    }
+    __syncthreads();
+    if (warp == 8) {
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    }
+    if (!again) return;
+    // Its rows once more, plainly, a warp a row and a key at a time: slow, but right.
+    constexpr int C = HD / 32;
+    const int64_t keys_at = (static_cast<int64_t>(prefix.row) * a.kv_heads + kvh) * prefix.cache.slots;
+    for (int r = warp; r < rows; r += kThreadsOf<CODES> / 32) {
+        int64_t token;
+        int head;
+        place(r, &token, &head);
+        float value[C] = {}, x[C], top = -INFINITY, total = 0.0f;
+#pragma unroll
+        for (int i = 0; i < C; ++i) x[i] = __bfloat162float(q[token * q_stride + head * HD + lane + 32 * i]);
+        const int end = min(prefix.length, (t0 + key_tiles) * kTcKeys);
+        for (int key = t0 * kTcKeys; key < end; ++key) {
+            auto read = [&](const void* values, const void* scales, int channel) {
+                if constexpr (CODES) {
+                    return code_value(static_cast<const unsigned char*>(values) + (keys_at + key) * (HD / 2),
+                                      static_cast<const __nv_bfloat16*>(scales) + (keys_at + key) * (HD / 16), C, channel);
+                } else {
+                    return __bfloat162float(static_cast<const __nv_bfloat16*>(values)[(keys_at + key) * HD + channel]);
+                }
+            };
+            float s = 0.0f;
+#pragma unroll
+            for (int i = 0; i < C; ++i) s = fmaf(x[i], read(prefix.cache.k, prefix.cache.k_scale, lane + 32 * i), s);
+            s = warp_sum(s) * a.scale * kLog2e;
+            const float up = fmaxf(top, s), keep = top == -INFINITY ? 0.0f : exp2f(top - up);
+            const float p = s == -INFINITY ? 0.0f : exp2f(s - up);
+            top = up;
+            total = fmaf(total, keep, p);
+#pragma unroll
+            for (int i = 0; i < C; ++i) {
+                value[i] *= keep;
+                if (p != 0.0f || isnan(p)) value[i] = fmaf(p, read(prefix.cache.v, prefix.cache.v_scale, lane + 32 * i), value[i]);
+            }
+        }
+        float* const to = part + ((token * a.heads + head) * splits + split) * (HD + 2);
+#pragma unroll
+        for (int i = 0; i < C; ++i) to[lane + 32 * i] = value[i];
+        if (lane == 0) {
+            to[HD] = top;
+            to[HD + 1] = total;
+        }
+    }
+}
+
+template <int HD, bool CODES>
+cudaError_t run(cudaStream_t s, const Prefix& p, const Batch& b, const AttnSpec& a, const __nv_bfloat16* q,
+                int64_t q_stride, int tiles, int splits, float* part) {
+    using L = PrefixLayout<HD>;
+    CUtensorMap k_map{}, v_map{};
+    if constexpr (!CODES) {
+        const int64_t head = static_cast<int64_t>(p.cache.slots) * HD * 2, row = head * a.kv_heads * p.row;
+        // Keys behind the prefix lie outside the maps and read as zeros, whatever their slots hold.
+        cudaError_t e = make_head_map(&k_map, static_cast<const char*>(p.cache.k) + row, a.kv_heads, p.length, HD,
+                                      head, kTcKeys);
+        if (!e) {
+            e = make_head_map(&v_map, static_cast<const char*>(p.cache.v) + row, a.kv_heads, p.length, HD, head,
+                              kTcKeys);
+        }
+        if (e) return e;
+    }
+    const cudaError_t e =
+        cudaFuncSetAttribute(k_prefix_tc<HD, CODES>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
+    if (e) return e;
+    k_prefix_tc<HD, CODES><<<tiles * a.kv_heads * splits, kThreadsOf<CODES>, L::kSmem, s>>>(
+        k_map, v_map, p, b, a, q, q_stride, tiles, splits, part);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+int prefix_tc_tiles(const Batch& b, const AttnSpec& a) {
+    const int64_t queries = static_cast<int64_t>(b.tokens) * (a.heads / a.kv_heads);
+    return static_cast<int>((queries + kRows - 1) / kRows);
+}
+
+bool prefix_tc_takes(const Prefix& p, const AttnSpec& a) {
+    return a.dtype == BST_DTYPE_BF16 && a.head_dim >= 64 && p.cache.storage != BST_DTYPE_F32 && a.scale != 0.0f;
+}
+
+cudaError_t launch_prefix_tc(cudaStream_t s, const Prefix& p, const Batch& b, const AttnSpec& a, const void* q_,
+                             int64_t q_stride, int tiles, int splits, float* part) {
+    const __nv_bfloat16* const q = static_cast<const __nv_bfloat16*>(q_);
+    const bool codes = p.cache.storage == BST_DTYPE_U4;
+    if (a.head_dim == 128) {
+        return codes ? run<128, true>(s, p, b, a, q, q_stride, tiles, splits, part)
+                     : run<128, false>(s, p, b, a, q, q_stride, tiles, splits, part);
+    }
+    return codes ? run<64, true>(s, p, b, a, q, q_stride, tiles, splits, part)
+                 : run<64, false>(s, p, b, a, q, q_stride, tiles, splits, part);
+}
+
+}  // namespace bst

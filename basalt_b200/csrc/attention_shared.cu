@@ -14,22 +14,43 @@ namespace bst {
 namespace {
 
 struct Plan {
-    CachedPlan own;
-    int rows, tiles, splits;  // of the prefix: query rows a tile, tiles, splits (0: no prefix)
+    int rows, tiles, splits;  // query rows a tile, tiles, splits of the keys
 };
 
-Plan plan_shared(const Cache& c, const Batch& b, const AttnSpec& a, const Prefix& p) {
-    Plan plan{plan_cached(c, b, a), 8, 0, 0};
+// On mma.sync, 8 or 16 query rows a tile.
+Plan plan_small(const Batch& b, const AttnSpec& a, const Prefix& p) {
+    Plan plan{8, 0, 1};
     const int64_t queries = static_cast<int64_t>(b.tokens) * (a.heads / a.kv_heads);
     if (a.dtype == BST_DTYPE_BF16 && queries > 8) plan.rows = 16;
     plan.tiles = static_cast<int>((queries + plan.rows - 1) / plan.rows);
-    if (p.length > 0) {
-        const int64_t units = static_cast<int64_t>(plan.tiles) * a.kv_heads;
-        const int64_t fill = 148 * ctas_per_sm(p.cache) / units;
-        plan.splits = static_cast<int>(std::max<int64_t>(
-            1, std::min<int64_t>({fill, p.length / 128, static_cast<int64_t>(kMaxSplits)})));
+    const int64_t units = static_cast<int64_t>(plan.tiles) * a.kv_heads;
+    const int64_t fill = 148 * ctas_per_sm(p.cache) / units;
+    plan.splits = static_cast<int>(
+        std::max<int64_t>(1, std::min<int64_t>({fill, p.length / 128, static_cast<int64_t>(kMaxSplits)})));
+    return plan;
+}
+
+// On tcgen05, 256 rows a tile and a CTA an SM: the split with the least waves x (tiles of 64 keys a CTA and
+// what a CTA costs besides, in such tiles).
+constexpr int kCost = 6, kMostShares = 64;
+Plan plan_large(const Batch& b, const AttnSpec& a, const Prefix& p) {
+    Plan plan{256, prefix_tc_tiles(b, a), 1};
+    const int64_t units = static_cast<int64_t>(plan.tiles) * a.kv_heads, keys = (p.length + 63) / 64;
+    int64_t best = 0;
+    for (int splits = 1; splits <= std::min<int64_t>(kMostShares, keys); ++splits) {
+        const int64_t time = (units * splits + 147) / 148 * ((keys + splits - 1) / splits + kCost);
+        if (splits == 1 || time < best) {
+            best = time;
+            plan.splits = splits;
+        }
     }
     return plan;
+}
+
+// Rows of a key head from which on the tensor cores' tiles of 128 pay.
+constexpr int kLargeRows = 48;
+bool large(const Batch& b, const AttnSpec& a, const Prefix& p) {
+    return prefix_tc_takes(p, a) && static_cast<int64_t>(b.tokens) * (a.heads / a.kv_heads) >= kLargeRows;
 }
 
 size_t part_bytes(const Batch& b, const AttnSpec& a, int splits) {
@@ -58,33 +79,45 @@ k_shared_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out, 
 }  // namespace
 
 size_t attention_shared_workspace(const Cache& c, const Batch& b, const AttnSpec& a, const Prefix& p) {
-    const Plan plan = plan_shared(c, b, a, p);
-    return part_bytes(b, a, plan.own.splits + plan.splits);
+    if (b.tokens < 1) return 0;
+    int splits = p.length > 0 ? plan_small(b, a, p).splits : 0;
+    if (p.length > 0 && large(b, a, p)) splits = std::max(splits, plan_large(b, a, p).splits);
+    return part_bytes(b, a, plan_cached(c, b, a).splits + splits);
 }
 
 cudaError_t launch_attention_shared(cudaStream_t s, const Cache& c, const Batch& b, const AttnSpec& a,
                                     const Prefix& p, const void* q, int64_t q_stride, void* out,
                                     int64_t out_stride, void* workspace) {
     if (b.tokens < 1 || b.count < 1) return cudaSuccess;
-    const Plan plan = plan_shared(c, b, a, p);
+    const CachedPlan plan = plan_cached(c, b, a);
     float* const own = static_cast<float*>(workspace);
-    float* const prefix = own + part_bytes(b, a, plan.own.splits) / sizeof(float);
-    if (plan.splits > 0) {
-        Extra extra;
-        extra.row = p.row;
-        extra.length = p.length;
-        const cudaError_t e = run_cached<kPrefix>(s, p.cache, b, a, q, q_stride, nullptr, 0, plan.tiles,
-                                                  plan.rows, plan.splits, prefix, extra);
+    float* const prefix = own + part_bytes(b, a, plan.splits) / sizeof(float);
+    int splits = 0;
+    if (p.length > 0) {
+        cudaError_t e;
+        if (large(b, a, p) && reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_stride % 8 == 0) {
+            const Plan of = plan_large(b, a, p);
+            splits = of.splits;
+            e = launch_prefix_tc(s, p, b, a, q, q_stride, of.tiles, splits, prefix);
+        } else {
+            const Plan of = plan_small(b, a, p);
+            splits = of.splits;
+            Extra extra;
+            extra.row = p.row;
+            extra.length = p.length;
+            e = run_cached<kPrefix>(s, p.cache, b, a, q, q_stride, nullptr, 0, of.tiles, of.rows, splits, prefix,
+                                    extra);
+        }
         if (e) return e;
     }
-    if (const cudaError_t e = launch_cached_parts(s, c, b, a, plan.own, q, q_stride, own)) return e;
+    if (const cudaError_t e = launch_cached_parts(s, c, b, a, plan, q, q_stride, own)) return e;
     return by_dtype(a.dtype, [&](auto type) {
         using T = decltype(type);
         return by_head_dim(a.head_dim, [&](auto hd) {
             constexpr int HD = decltype(hd)::value;
             return launch_pdl(k_shared_join<T, HD>, dim3(b.tokens, a.heads), dim3(kThreads), 0, s, c, b, a,
-                              plan.own.rows, static_cast<T*>(out), out_stride, plan.own.splits,
-                              static_cast<const float*>(own), plan.splits, static_cast<const float*>(prefix));
+                              plan.rows, static_cast<T*>(out), out_stride, plan.splits,
+                              static_cast<const float*>(own), splits, static_cast<const float*>(prefix));
         });
     });
 }

@@ -1238,4 +1238,18 @@ cudaError_t make_tile_map(CUtensorMap* map, const void* ptr, int rows, int K, in
     return e ? e : make_pitched_map(map, ptr, rows, K, pitch, bf16, box_rows);
 }
 
+cudaError_t make_head_map(CUtensorMap* map, const void* ptr, int heads, int rows, int K, int64_t pitch,
+                          int box_rows) {
+    if (const cudaError_t e = encoder()) return e;
+    cuuint64_t dims[3] = {static_cast<cuuint64_t>(K), static_cast<cuuint64_t>(rows),
+                          static_cast<cuuint64_t>(heads)};
+    cuuint64_t strides[2] = {static_cast<cuuint64_t>(K) * 2, static_cast<cuuint64_t>(pitch)};
+    cuuint32_t box[3] = {kRowBytes / 2, static_cast<cuuint32_t>(box_rows), 1};
+    cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(ptr), dims, strides,
+                                box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 }  // namespace bst

@@ -60,6 +60,13 @@ cudaError_t launch_attention_shared(cudaStream_t s, const Cache& c, const Batch&
                                     const Prefix& p, const void* q, int64_t q_stride, void* out,
                                     int64_t out_stride, void* workspace);
 
+// The prefix's pass on tcgen05: whether it takes the types (q aligned to 16 bytes, like its tokens' distance),
+// its tiles of query rows, and the pass, which leaves the sums of every split as launch_cached_parts does.
+bool prefix_tc_takes(const Prefix& p, const AttnSpec& a);
+int prefix_tc_tiles(const Batch& b, const AttnSpec& a);
+cudaError_t launch_prefix_tc(cudaStream_t s, const Prefix& p, const Batch& b, const AttnSpec& a, const void* q,
+                             int64_t q_stride, int tiles, int splits, float* part);
+
 size_t attention_weights_workspace(const Cache& c, const Batch& b, const AttnSpec& a);
 cudaError_t launch_attention_weights(cudaStream_t s, const Cache& c, const Batch& b, const AttnSpec& a,
                                      const void* q, int64_t q_stride, void* out, int64_t out_stride,

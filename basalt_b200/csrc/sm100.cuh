@@ -85,6 +85,15 @@ __device__ __forceinline__ void tma_load_2d(const CUtensorMap* map, uint64_t* ba
         : "memory");
 }
 
+__device__ __forceinline__ void tma_load_3d(const CUtensorMap* map, uint64_t* bar, void* dst,
+                                            int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+
 // Shared-memory matrix descriptor for a K-major tile of 128-byte rows with the 128-byte swizzle:
 // 8-row groups 1024 bytes apart (SBO), leading offset unused (1), descriptor version 1.
 __device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {
@@ -137,6 +146,9 @@ __device__ __forceinline__ void tmem_ld(uint32_t taddr, float* v) {
 // box_rows rows in the 128-byte swizzle; what lies outside reads as zeros. ptr and pitch are
 // multiples of 16 bytes.
 cudaError_t make_tile_map(CUtensorMap* map, const void* ptr, int rows, int K, int64_t pitch, bool bf16,
+                          int box_rows);
+// The same of [heads, rows, K] bf16, heads `pitch` bytes apart and rows contiguous, one head a box.
+cudaError_t make_head_map(CUtensorMap* map, const void* ptr, int heads, int rows, int K, int64_t pitch,
                           int box_rows);
 
 }  // namespace bst

@@ -144,6 +144,43 @@ def test_shared_prefix_scales(ops, prefix_storage, scale):
         check_shared(ops, rng, "u4", prefix_storage, dtype, 64, 8, 2, 150, list(rng.integers(0, 9, 40)), scale=scale)
 
 
+@pytest.mark.parametrize("storage,dtype", [("u4", "bf16"), ("bf16", "bf16"), ("u4", "f32"), ("f32", "f32")])
+@pytest.mark.parametrize("dim,heads,kv_heads,count,prefix", [
+    (64, 8, 2, 70, 5001), (128, 32, 8, 150, 4159), (128, 4, 4, 300, 9000), (64, 16, 1, 37, 40003), (128, 40, 8, 24, 2048)])
+def test_long_prefixes(ops, storage, dtype, dim, heads, kv_heads, count, prefix):
+    """Many tiles of keys a CTA, against 64 bits on the GPU."""
+    torch = torch_()
+    rng = np.random.default_rng(prefix)
+    g = torch.Generator(device="cuda").manual_seed(prefix)
+    common = ops.KvCache.allocate(1, kv_heads, prefix + 3, dim, storage)
+    x = torch.randn((2, prefix, kv_heads, dim), generator=g, device="cuda")
+    x[0] += 3 * torch.randn((1, kv_heads, dim), generator=g, device="cuda").clamp(min=1)
+    x[0, prefix // 2] *= 4                       # a key that moves many a maximum
+    x[1, prefix // 3:] *= 30                     # values that grow on the way
+    ops.kv_append(common, x[0], x[1], ints([prefix]), starts=ints([0, prefix]))
+    k, v = (t.double().transpose(0, 1) for t in ops.kv_read(common, ints([prefix]), starts=ints([0, prefix]), tokens=prefix))
+    spoil(common, 0, prefix)
+    own, own_k, own_v = filled(ops, rng, count, kv_heads, 4, dim, storage)
+    q = torch.randn((count, heads, dim), generator=g, device="cuda").to(getattr(torch, {"f32": "float32", "bf16": "bfloat16"}[dtype]))
+    lengths = rng.integers(0, 5, count)
+    got = host(ops.attention_shared(own, q, ints(lengths), common, prefix))
+    own_k, own_v = (torch.from_numpy(t).cuda() for t in (own_k, own_v))      # [count, slots, kv_heads, dim]
+    group, scale = heads // kv_heads, dim ** -0.5
+    hidden = torch.arange(4, device="cuda") >= ints(lengths)[:, None]
+    for h in range(kv_heads):
+        qh = q[:, h * group:(h + 1) * group].double()                        # [count, group, dim]
+        score = torch.cat([qh @ k[h].T, torch.einsum("sgd,sjd->sgj", qh, own_k[:, :, h])
+                           .masked_fill(hidden[:, None], -np.inf)], -1) * scale
+        p = torch.softmax(score, -1)
+        want = p[..., :prefix] @ v[h] + torch.einsum("sgj,sjd->sgd", p[..., prefix:], own_v[:, :, h])
+        size = (qh.abs() @ k[h].abs().T).amax(-1).cpu().numpy() * scale
+        spread = float(max(v[h].abs().max(), own_v.abs().max()))
+        want = want.cpu().numpy()
+        tol = shared_bound(size, dim, prefix + 4, spread, want, dtype, storage)
+        off = np.abs(got[:, h * group:(h + 1) * group] - want)
+        assert np.all(off <= tol), (off / tol).max()
+
+
 def test_a_prefix_in_the_same_cache_and_out_over_q(ops):
     torch = torch_()
     rng = np.random.default_rng(5)
