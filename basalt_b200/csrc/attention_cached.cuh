@@ -1387,15 +1387,45 @@ k_cached_one(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_st
 constexpr int kMaxSplits = 512;
 
 // How many splits the tile of a query used, as k_cached found it: token `at` of its sequence's n.
-__device__ __forceinline__ int used_splits(const Cache& c, const Batch& b, const AttnSpec& a, int tile_rows,
-                                           int splits, int seq, int at, int n, int head) {
+__device__ __forceinline__ int used_splits(const Cache& c, const AttnSpec& a, int tile_rows, int splits, int row,
+                                           int length, int at, int n, int head) {
     const int group = a.heads / a.kv_heads;
-    const int row = b.rows ? __ldg(b.rows + seq) : seq;
-    const int length = max(0, __ldg(b.lengths + seq));
     const int r0 = (at * group + head % group) / tile_rows * tile_rows;
     const int rows = min(tile_rows, n * group - r0);
     const int p_last = row >= 0 && row < c.rows ? length - n + (r0 + rows - 1) / group : -1;
     return useful_splits(Visible(length - n + r0 / group, p_last, c.slots, a.window, a.sinks).blocks, splits);
+}
+
+__device__ __forceinline__ int used_splits(const Cache& c, const Batch& b, const AttnSpec& a, int tile_rows,
+                                           int splits, int seq, int at, int n, int head) {
+    const int row = b.rows ? __ldg(b.rows + seq) : seq;
+    return used_splits(c, a, tile_rows, splits, row, max(0, __ldg(b.lengths + seq)), at, n, head);
+}
+
+// The same as below by one warp, for at most 32 splits: a lane a split, then a lane HD / 32 channels.
+template <typename T, int HD, typename At>
+__device__ __forceinline__ void join_by_warp(int use, At&& at, T* to) {
+    constexpr int C = HD / 32;
+    const int lane = threadIdx.x & 31;
+    float top = -INFINITY, total = 0.0f;
+    if (lane < use) {
+        top = at(lane)[HD];
+        total = at(lane)[HD + 1];
+    }
+    const float m = warp_max(top);
+    // A split that saw nothing has nothing to add; one whose scores are NaN has.
+    const float f = top == -INFINITY ? (total == 0.0f ? 0.0f : total) : exp2_fast(top - m);
+    const float sum = warp_sum(total * f);
+    float value[C] = {};
+#pragma unroll 8
+    for (int s = 0; s < use; ++s) {
+        const float* const x = at(s) + lane;
+        const float by = __shfl_sync(kFull, f, s);
+#pragma unroll
+        for (int i = 0; i < C; ++i) value[i] = fmaf(x[32 * i], by, value[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < C; ++i) put(to + lane + 32 * i, sum == 0.0f ? 0.0f : value[i] / sum);
 }
 
 // The CTA's query from the sums at(0) .. at(use - 1), [HD outputs, maximum, sum] each. N: the most of them.

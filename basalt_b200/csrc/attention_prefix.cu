@@ -6,13 +6,17 @@
 // but the end of the prefix is masked) and a share of the keys, in tiles of 64: two M = 128 tiles of queries,
 // whose scores, weights and outputs live in TMEM and take turns, as in attention over packed prompts. It leaves
 // outputs, maximum and sum of weights of every row in float32; the shares are joined with the sequences' own
-// keys' sums. Weights are bf16 (8 bits) in the product with values, whose rounding is of the size of bf16
-// outputs' own; maxima and sums are float32.
+// keys' sums. Weights are bf16 (8 bits) in the product with bf16 values (a product's operands are of one type),
+// whose rounding is of the size of bf16 outputs' own; maxima and sums are float32.
 //
 // A 4-bit prefix is unpacked on its way into shared memory by four warps in the copy's place, so that every key
-// is unpacked once for 256 rows: keys become fp16 (11 bits; a tile is brought near one by a power of two, and so
-// is every query row, which the scores' factor f takes back), because an error of a score grows with it; values
-// become bf16 as weights are, by one fused multiply-add a value pair, rounded once.
+// is unpacked once for 256 rows. Keys, values, queries and weights become fp16, 11 bits, by one fused
+// multiply-add for two values, rounded once (bf16 ones took the error from 1.0 to 1.6 of the outputs' own
+// rounding). Powers of two keep them in fp16's range: one for each query row and each tile of keys, which the
+// scores' factor f takes back; and one for values, that of the largest so far with four bits to spare, by which
+// O is rescaled when a tile passes it (values 2^-25 of the largest so far begin to lose bits).
+// Codes and scales pass through a ring of their own in shared memory, three tiles ahead: with loads one tile
+// ahead the memory's latency was the bound (24 x 4 drafts of 32 heads behind 16 384 keys: 73 us).
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -38,10 +42,15 @@ struct PrefixLayout {
     static constexpr int kTile = kTcKeys * HD * 2;    // a tile of keys or values
     static constexpr int kSlots = 8;
     static constexpr int kBars = 2 * kQuery + kSlots * kTile;
-    static constexpr int kEnd = kBars + 256 + (kRows + 16) * 4;
+    static constexpr int kFactors = kBars + 256;      // of rows, tiles of keys, tiles of values, warps
+    static constexpr int kRaw = kFactors + (kRows + 24) * 4;
+    // Codes and scales as the unpacking threads copy them: [stage][16-byte pieces][thread].
+    static constexpr int kStages = 4, kPieces = HD / 64 + 1;
+    static constexpr int end(bool codes) { return kRaw + (codes ? kStages * kPieces * kUnpack * 16 : 0); }
     // More than half of an SM's shared memory: one CTA an SM, which owns all of TMEM.
-    static constexpr int kBytes = kEnd > 120 * 1024 ? kEnd : 120 * 1024;
-    static constexpr int kSmem = kBytes + 1024;       // the base is aligned to 1024 bytes
+    static constexpr int smem(bool codes) {           // the base is aligned to 1024 bytes
+        return (end(codes) > 120 * 1024 ? end(codes) : 120 * 1024) + 1024;
+    }
     static_assert(kSlots * kTile >= kRows * HD * 4, "outputs are staged in the ring");
 };
 
@@ -68,35 +77,21 @@ __device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c
     asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
     return r;
 }
-__device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
-__device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
-    uint32_t r;
-    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
-    return r;
-}
-
-// 2^e for e in [-126, 127], and the e for which |x| < 2^e, within [-100, 126] (0 for zero).
+// 2^e for e in [-126, 127], and the e for which |x| < 2^e, within [-100, 126].
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
 __device__ __forceinline__ int exponent_above(uint32_t bits) {
-    return bits == 0u ? 0 : max(min(static_cast<int>(bits >> 23) - 126, 126), -100);
+    return max(min(static_cast<int>(bits >> 23) - 126, 126), -100);
 }
 
 // One word of codes (nibble j of the low half: channel j of one group; of the high half: of the next) and its
-// successor (the next four channels) as 16 bytes for each of the two groups.
-template <bool KEYS>
+// successor (the next four channels) as 16 bytes of fp16 for each of the two groups.
 __device__ __forceinline__ void unpack(uint32_t a, uint32_t b, uint32_t step, uint32_t low, uint4* first,
                                        uint4* second) {
-    // 1024 + c in fp16, 128 + c in bf16: both exact, as is c.
-    constexpr uint32_t base = KEYS ? 0x64006400u : 0x43004300u;
     uint32_t x[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const uint32_t w = ((j < 4 ? a : b) >> (4 * (j & 3)) & 0x000f000fu) | base;
-        x[j] = KEYS ? fma_f16x2(sub_f16x2(w, base), step, low) : fma_bf16x2(sub_bf16x2(w, base), step, low);
+    for (int j = 0; j < 8; ++j) {  // 1024 + c is exact, as is c
+        const uint32_t w = ((j < 4 ? a : b) >> (4 * (j & 3)) & 0x000f000fu) | 0x64006400u;
+        x[j] = fma_f16x2(sub_f16x2(w, 0x64006400u), step, low);
     }
     *first = make_uint4(__byte_perm(x[0], x[1], 0x5410), __byte_perm(x[2], x[3], 0x5410),
                         __byte_perm(x[4], x[5], 0x5410), __byte_perm(x[6], x[7], 0x5410));
@@ -139,9 +134,10 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
     uint64_t* const o_last = o_done + 2;
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(o_last + 2);
     int* const status = reinterpret_cast<int*>(tmem_slot + 1);  // [0] error code, [1] abort
-    float* const row_factor = reinterpret_cast<float*>(smem + L::kBars + 256);  // what a row was divided by
-    float* const tile_factor = row_factor + kRows;                              // and a tile of keys, [8]
-    uint32_t* const warp_most = reinterpret_cast<uint32_t*>(tile_factor + 8);   // [2][4]
+    float* const row_factor = reinterpret_cast<float*>(smem + L::kFactors);   // what a row was divided by,
+    float* const key_factor = row_factor + kRows;                             // a tile of keys, [8],
+    float* const value_factor = key_factor + 8;                               // and of values and weights, [8]
+    uint32_t* const warp_most = reinterpret_cast<uint32_t*>(value_factor + 8);  // [2][4]
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < L::kSlots; ++i) {
@@ -249,102 +245,104 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
                 }
             }
         } else {
-            // A key a thread, or half of one with 128 channels: chunks of 16 code bytes.
-            constexpr int G = HD / 32, kChunks = HD / 32 / (kUnpack / kTcKeys);
+            // Two threads a key: a chunk of 16 code bytes each, or two with 128 channels.
+            constexpr int G = HD / 32, kChunks = HD / 64;
             const int tid = threadIdx.x - 9 * 32, key = tid & (kTcKeys - 1), part_of = tid / kTcKeys;
             const int64_t at = (static_cast<int64_t>(prefix.row) * a.kv_heads + kvh) * prefix.cache.slots;
-            struct Held {
+            const uint32_t mine = base + L::kRaw + tid * 16;
+            auto piece = [&](int i, int x) {
+                return mine + ((i % L::kStages) * L::kPieces + x) * (kUnpack * 16);
+            };
+            auto load = [&](int i) {
+                if (i < copies) {
+                    const int my_key = (t0 + copy_tile(i)) * kTcKeys + key;
+                    const bool keys = copy_of_keys(i), there = my_key < prefix.length;  // behind it: zeros
+                    const int64_t from = at + (there ? my_key : 0);
+                    const char* codes = static_cast<const char*>(keys ? prefix.cache.k : prefix.cache.v) +
+                                        from * (HD / 2) + part_of * kChunks * 16;
+                    const char* scale = static_cast<const char*>(keys ? prefix.cache.k_scale : prefix.cache.v_scale) +
+                                        from * (G * 4);
+#pragma unroll
+                    for (int x = 0; x < kChunks; ++x) cp_async<16>(piece(i, x), codes + 16 * x, there ? 16 : 0);
+                    cp_async<G * 4>(piece(i, kChunks), scale, there ? G * 4 : 0);
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+#pragma unroll
+            for (int i = 0; i < L::kStages - 1; ++i) load(i);
+            int values_below = -1000;  // values are below 2^this; what they are divided by goes with it
+            bool ok = true;
+            for (int i = 0; i < copies; ++i) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 2) : "memory");
                 uint4 codes[kChunks];
                 uint32_t scale[G];
-            };
-            auto load = [&](int i, Held& h) {
-                const int my_key = (t0 + copy_tile(i)) * kTcKeys + key;
-                const bool keys = copy_of_keys(i);
-                if (i < copies && my_key < prefix.length) {
-                    const char* codes = static_cast<const char*>(keys ? prefix.cache.k : prefix.cache.v) +
-                                        (at + my_key) * (HD / 2) + part_of * kChunks * 16;
-                    const char* scale = static_cast<const char*>(keys ? prefix.cache.k_scale : prefix.cache.v_scale) +
-                                        (at + my_key) * (G * 4);
 #pragma unroll
-                    for (int x = 0; x < kChunks; ++x) h.codes[x] = __ldg(reinterpret_cast<const uint4*>(codes) + x);
-                    if constexpr (G == 4) {
-                        const uint4 s = __ldg(reinterpret_cast<const uint4*>(scale));
-                        h.scale[0] = s.x; h.scale[1] = s.y; h.scale[2] = s.z; h.scale[3] = s.w;
-                    } else {
-                        const uint2 s = __ldg(reinterpret_cast<const uint2*>(scale));
-                        h.scale[0] = s.x; h.scale[1] = s.y;
-                    }
-                } else {  // behind the prefix: zeros
-#pragma unroll
-                    for (int x = 0; x < kChunks; ++x) h.codes[x] = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-                    for (int g = 0; g < G; ++g) h.scale[g] = 0u;
+                for (int x = 0; x < kChunks; ++x) {
+                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(codes[x].x), "=r"(codes[x].y), "=r"(codes[x].z), "=r"(codes[x].w)
+                                 : "r"(piece(i, x)));
                 }
-            };
-            auto store = [&](int i, const Held& h, bool keys, float by) {
+                if constexpr (G == 4) {
+                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(scale[0]), "=r"(scale[1]), "=r"(scale[2]), "=r"(scale[3])
+                                 : "r"(piece(i, kChunks)));
+                } else {
+                    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
+                                 : "=r"(scale[0]), "=r"(scale[1]) : "r"(piece(i, kChunks)));
+                }
+                load(i + L::kStages - 1);  // into the stage before this one, which this thread alone has read
+                // The tile's largest is at most max |low| + 15 step (not of a NaN).
+                const int tile = copy_tile(i);
+                uint32_t most = 0u;
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    const float top = fmaf(15.0f, __uint_as_float(scale[g] << 16),
+                                           fabsf(__uint_as_float(scale[g] & 0xffff0000u)));
+                    most = max(most, top <= FLT_MAX ? __float_as_uint(top) : (isnan(top) ? 0u : 0x7f000000u));
+                }
+                most = __reduce_max_sync(kFull, most);
+                if (lane == 0) warp_most[(i & 1) * 4 + (warp - 9)] = most;
+                asm volatile("bar.sync 3, %0;" ::"n"(kUnpack) : "memory");
+                const uint32_t* const all_most = warp_most + (i & 1) * 4;
+                const int e = exponent_above(max(max(all_most[0], all_most[1]), max(all_most[2], all_most[3])));
+                float by;
+                if (copy_of_keys(i)) {
+                    by = power_of_two(-e);
+                    if (tid == 0) key_factor[tile & 7] = power_of_two(e);
+                } else {
+                    if (e > values_below) values_below = e + 4;
+                    by = power_of_two(15 - values_below);
+                    // Weights are 2^7 too large.
+                    if (tid == 0) value_factor[tile & 7] = power_of_two(values_below - 22);
+                }
+                if (ok && i >= L::kSlots) {
+                    ok = mbar_wait(empty + i % L::kSlots, ((i / L::kSlots) - 1) & 1, status, 1, abort);
+                }
+                if (!ok) continue;  // a wait that ran out ends no loop: the warps meet at the barrier above
                 unsigned char* const to = smem + 2 * L::kQuery + (i % L::kSlots) * L::kTile + key * 128;
 #pragma unroll
                 for (int g = 0; g < G; g += 2) {
-                    uint32_t step = __byte_perm(h.scale[g], h.scale[g + 1], 0x5410);
-                    uint32_t low = __byte_perm(h.scale[g], h.scale[g + 1], 0x7632);
-                    if (keys) {
-                        step = half2_of(__uint_as_float(step << 16) * by, __uint_as_float(step & 0xffff0000u) * by);
-                        low = half2_of(__uint_as_float(low << 16) * by, __uint_as_float(low & 0xffff0000u) * by);
-                    }
+                    const uint32_t step = half2_of(__uint_as_float(scale[g] << 16) * by,
+                                                   __uint_as_float(scale[g + 1] << 16) * by);
+                    const uint32_t low = half2_of(__uint_as_float(scale[g] & 0xffff0000u) * by,
+                                                  __uint_as_float(scale[g + 1] & 0xffff0000u) * by);
 #pragma unroll
-                    for (int x = 0; x < kChunks * 4 / G; ++x) {  // eight channels of both groups
-                        // Words of a chunk: [two halves of eight channels][pairs of groups], or, with two
-                        // groups, [four halves].
-                        const uint32_t w[4] = {h.codes[G == 4 ? x : 0].x, h.codes[G == 4 ? x : 0].y,
-                                               h.codes[G == 4 ? x : 0].z, h.codes[G == 4 ? x : 0].w};
-                        const uint32_t a0 = G == 4 ? w[g / 2] : w[2 * x], a1 = G == 4 ? w[2 + g / 2] : w[2 * x + 1];
-                        const int eighth = part_of * (kChunks * 4 / G) + x;  // which eight of a group's 32
+                    for (int x = 0; x < 2; ++x) {  // eight channels of both groups
+                        // Words of a chunk: [halves of eight channels][pairs of groups], or, with two groups,
+                        // four halves.
+                        const uint4 c = codes[G == 4 ? x : 0];
+                        const uint32_t w0 = G == 4 ? (g ? c.y : c.x) : (x ? c.z : c.x);
+                        const uint32_t w1 = G == 4 ? (g ? c.w : c.z) : (x ? c.w : c.y);
+                        const int eighth = part_of * 2 + x;  // which eight of a group's 32
                         uint4 one, two;
-                        if (keys) {
-                            unpack<true>(a0, a1, step, low, &one, &two);
-                        } else {
-                            unpack<false>(a0, a1, step, low, &one, &two);
-                        }
+                        unpack(w0, w1, step, low, &one, &two);
                         unsigned char* const block = to + (g >> 1) * (kTcKeys * 128);
                         *reinterpret_cast<uint4*>(block + ((eighth ^ (key & 7)) << 4)) = one;
                         *reinterpret_cast<uint4*>(block + (((4 + eighth) ^ (key & 7)) << 4)) = two;
                     }
                 }
-            };
-            Held now, next;
-            load(0, now);
-            bool ok = true;
-            for (int i = 0; i < copies; ++i) {
-                load(i + 1, next);
-                const bool keys = copy_of_keys(i);
-                float by = 1.0f;
-                if (keys) {
-                    // The tile's largest key is at most max |low| + 15 step (not of a NaN).
-                    const int tile = copy_tile(i);
-                    uint32_t most = 0u;
-#pragma unroll
-                    for (int g = 0; g < G; ++g) {
-                        const float top = fmaf(15.0f, __uint_as_float(now.scale[g] << 16),
-                                               fabsf(__uint_as_float(now.scale[g] & 0xffff0000u)));
-                        most = max(most, top <= FLT_MAX ? __float_as_uint(top) : (isnan(top) ? 0u : 0x7f000000u));
-                    }
-                    most = __reduce_max_sync(kFull, most);
-                    if (lane == 0) warp_most[(tile & 1) * 4 + (warp - 9)] = most;
-                    asm volatile("bar.sync 3, %0;" ::"n"(kUnpack) : "memory");
-                    const uint32_t* const all_most = warp_most + (tile & 1) * 4;
-                    const int e = exponent_above(max(max(all_most[0], all_most[1]), max(all_most[2], all_most[3])));
-                    by = power_of_two(-e);
-                    if (tid == 0) tile_factor[tile & 7] = power_of_two(e);
-                }
-                if (ok && i >= L::kSlots) {
-                    ok = mbar_wait(empty + i % L::kSlots, ((i / L::kSlots) - 1) & 1, status, 1, abort);
-                }
-                if (ok) {  // a wait that ran out ends no loop: the warps meet at the barrier above
-                    store(i, now, keys, by);
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    mbar_arrive(full + i % L::kSlots);
-                }
-                now = next;
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                mbar_arrive(full + i % L::kSlots);
             }
         }
     } else if (warp == 8) {
@@ -352,7 +350,7 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
         // their keys is masked), and all of TMEM starts at address 0, so that operands are constants but for
         // the slot.
         const int n_tiles = __shfl_sync(kFull, key_tiles, 0), n_halves = __shfl_sync(kFull, halves, 0);
-        constexpr uint32_t s_idesc = tc_idesc(kTcKeys, false, CODES), o_idesc = tc_idesc(HD, true);
+        constexpr uint32_t s_idesc = tc_idesc(kTcKeys, false, CODES), o_idesc = tc_idesc(HD, true, CODES);
         const uint32_t q_desc = desc_k(base), kv_at = base + 2 * L::kQuery;
         auto slot = [&](int i) { return kv_at + (i % L::kSlots) * L::kTile; };
         auto scores = [&](int half, int i) {  // S = Q K^T
@@ -413,7 +411,7 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
         const uint32_t o_at = s_at + 128;
         // A score's factor to base 2. It stays above zero: the mask's -infinity is multiplied by it.
         const float scale = fabsf(a.scale) * kLog2e * (CODES ? row_factor[at] : 1.0f);
-        float top = -INFINITY, total = 0.0f;
+        float top = -INFINITY, total = 0.0f, values_by = 1.0f;
         // A wait that runs out ends no loop here: the tile's threads meet at a barrier behind it, and
         // what they write then is computed again.
         bool ok = true;
@@ -424,7 +422,7 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             tmem_ld32(buffer, s[0]);
             tmem_ld32(buffer + 32, s[1]);
-            float by = CODES ? scale * tile_factor[i & 7] : scale;
+            float by = CODES ? scale * key_factor[i & 7] : scale;
             by = by < FLT_MIN ? FLT_MIN : by;
             tmem_ld_wait();
             const int left = prefix.length - (t0 + i) * kTcKeys;  // keys of the tile, or more
@@ -440,10 +438,20 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
             const float most = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * by;
             // The maximum that weights are taken against moves only when a row's grows by more than 2^8.
             const bool move = most > top + 8.0f || (top == -INFINITY && most > top);
-            if (__any_sync(kFull, move)) {
-                const float keep = move ? (top == -INFINITY ? 0.0f : exp2_fast(top - most)) : 1.0f;
+            float rescale = 1.0f;
+            if constexpr (CODES) {
+                // Values of this tile that are divided by more than those before: what was summed has to be, too.
+                // (The tile is there until these weights have been multiplied with it.)
+                ok = ok && await(v_copy(i), 6);
+                const float now = value_factor[i & 7];
+                rescale = values_by / now;
+                values_by = now;
+            }
+            if (__any_sync(kFull, move) || (CODES && i > 0 && rescale != 1.0f)) {
+                float keep = move ? (top == -INFINITY ? 0.0f : exp2_fast(top - most)) : 1.0f;
                 if (move) top = most;
                 total *= keep;
+                keep *= rescale;
                 if (i > 0) {
                     ok = ok && mbar_wait(o_done + half, (i - 1) & 1, status, 8, abort);
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -470,7 +478,7 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
                     const float e1 = exp2_fast(fmaf(__uint_as_float(s[c][2 * x + 1]), by, -from));
                     sum[(2 * x) & 3] += e0;
                     sum[(2 * x + 1) & 3] += e1;
-                    p[x] = pack2(e0, e1);
+                    p[x] = CODES ? half2_of(e0 * 128.0f, e1 * 128.0f) : pack2(e0, e1);
                 }
                 tmem_st16(buffer + 16 * c, p);
             }
@@ -493,6 +501,10 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
                 uint32_t o[32];
                 tmem_ld32(o_at + 32 * c, o);
                 tmem_ld_wait();
+                if constexpr (CODES) {
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * values_by);
+                }
 #pragma unroll
                 for (int x = 0; x < 8; ++x) {
                     *reinterpret_cast<uint4*>(rows_at + at * (HD * 4) + (((8 * c + x) ^ (in_tile & 7)) << 4)) =
@@ -599,9 +611,9 @@ cudaError_t run(cudaStream_t s, const Prefix& p, const Batch& b, const AttnSpec&
         if (e) return e;
     }
     const cudaError_t e =
-        cudaFuncSetAttribute(k_prefix_tc<HD, CODES>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
+        cudaFuncSetAttribute(k_prefix_tc<HD, CODES>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::smem(CODES));
     if (e) return e;
-    k_prefix_tc<HD, CODES><<<tiles * a.kv_heads * splits, kThreadsOf<CODES>, L::kSmem, s>>>(
+    k_prefix_tc<HD, CODES><<<tiles * a.kv_heads * splits, kThreadsOf<CODES>, L::smem(CODES), s>>>(
         k_map, v_map, p, b, a, q, q_stride, tiles, splits, part);
     return cudaGetLastError();
 }

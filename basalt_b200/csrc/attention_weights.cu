@@ -39,84 +39,108 @@ __device__ __forceinline__ int next_of_row(const Batch& b, int seq, int row) {
     return next;
 }
 
-template <typename T, int HD>
+template <typename T, int HD, bool WARP>
 __global__ void __launch_bounds__(kThreads)
 k_weights_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out, int64_t out_stride,
                int splits, const float* __restrict__ part, const float* __restrict__ scores, int64_t pitch,
-               const float* previous, float decay, float* mass) {
-    const int64_t queries = static_cast<int64_t>(b.tokens) * a.heads;
-    if (blockIdx.x < queries) {
-        const int token = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
+               const float* previous, float decay, float* mass, int joins) {
+    if (blockIdx.x < joins) {
+        const int64_t query = WARP ? static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5) : blockIdx.x;
+        const int token = static_cast<int>(query / a.heads), head = static_cast<int>(query - static_cast<int64_t>(token) * a.heads);
         int seq, first, n;
-        if (!find_sequence(b, token, &seq, &first, &n)) return;
+        if (token >= b.tokens || !find_sequence(b, token, &seq, &first, &n)) return;
         const int use = used_splits(c, b, a, tile_rows, splits, seq, token - first, n, head);
         pdl_wait();
-        const float* from = part + (static_cast<int64_t>(token) * a.heads + head) * splits * (HD + 2);
-        join_splits<kMaxSplits, T, HD>(use, [&](int s) { return from + s * (HD + 2); },
-                                       out + token * out_stride + head * HD);
+        const float* const from = part + query * splits * (HD + 2);
+        auto at = [&](int s) { return from + s * (HD + 2); };
+        T* const to = out + token * out_stride + head * HD;
+        if constexpr (WARP) {
+            join_by_warp<T, HD>(use, at, to);
+        } else {
+            join_splits<kMaxSplits, T, HD>(use, at, to);
+        }
         return;
     }
     __shared__ float tops[kMassRows], inverse[kMassRows];
     const int chunks = (c.slots + kMassKeys - 1) / kMassKeys;
-    const int64_t place = blockIdx.x - queries;
+    const int64_t place = blockIdx.x - joins;
     const int kvh = static_cast<int>(place % a.kv_heads);
     const int64_t rest = place / a.kv_heads;
     const int key0 = static_cast<int>(rest % chunks) * kMassKeys;
     int seq = static_cast<int>(rest / chunks);
     const int row = b.rows ? __ldg(b.rows + seq) : seq;
     if (row < 0 || row >= c.rows || !first_of_row(b, seq, row)) return;
-    const int group = a.heads / a.kv_heads, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int group = a.heads / a.kv_heads, lane = threadIdx.x & 31;
     constexpr int N = kMassKeys / kThreads;
     float sum[N] = {};
     int end = 0;
-    pdl_wait();
+    bool waited = false;
     for (; seq < b.count; seq = next_of_row(b, seq, row)) {
-        const int length = min(max(0, __ldg(b.lengths + seq)), c.slots);
-        end = max(end, length);
-        if (length <= key0) continue;
+        const int length = max(0, __ldg(b.lengths + seq));
+        end = max(end, min(length, c.slots));
+        if (min(length, c.slots) <= key0) continue;
         int first = seq, n = 1;
         if (b.starts) {
             first = max(0, __ldg(b.starts + seq));
             n = max(0, min(__ldg(b.starts + seq + 1), b.tokens) - first);
         }
-        const int position = max(0, __ldg(b.lengths + seq)) - n;  // of its first token
-        for (int64_t r0 = 0; r0 < static_cast<int64_t>(n) * group; r0 += kMassRows) {
-            const int rows = static_cast<int>(min(static_cast<int64_t>(kMassRows), static_cast<int64_t>(n) * group - r0));
+        if (!waited) pdl_wait();
+        waited = true;
+        const int64_t all = static_cast<int64_t>(n) * group;
+        for (int64_t r0 = 0; r0 < all; r0 += kMassRows) {
+            const int rows = static_cast<int>(min(static_cast<int64_t>(kMassRows), all - r0));
+            // Maxima and sums of the rows: as many lanes a row as there are to spare.
+            int lanes = 32;
+            while (lanes > 1 && rows * lanes > kThreads) lanes >>= 1;
             __syncthreads();
-            for (int r = warp; r < rows; r += kWarps) {
-                const int at = static_cast<int>((r0 + r) / group), head = kvh * group + static_cast<int>((r0 + r) % group);
-                const int use = used_splits(c, b, a, tile_rows, splits, seq, at, n, head);
-                const float* from = part + (static_cast<int64_t>(first + at) * a.heads + head) * splits * (HD + 2) + HD;
+            const int of_warp = 32 / lanes;  // a warp takes that many rows at a time
+            for (int r = threadIdx.x / lanes; r < (rows + of_warp - 1) / of_warp * of_warp; r += kThreads / lanes) {
                 float m = -INFINITY, total = 0.0f;
-                for (int s = lane; s < use; s += 32) m = fmaxf(m, from[s * (HD + 2)]);
-                m = warp_max(m);
-                for (int s = lane; s < use; s += 32) {
-                    const float top = from[s * (HD + 2)], t = from[s * (HD + 2) + 1];
-                    total = fmaf(t, top == -INFINITY ? (t == 0.0f ? 0.0f : t) : exp2_fast(top - m), total);
+                if (r < rows) {
+                    const int at = static_cast<int>((r0 + r) / group), head = kvh * group + static_cast<int>((r0 + r) % group);
+                    const int use = used_splits(c, a, tile_rows, splits, row, length, at, n, head);
+                    const float* from = part + (static_cast<int64_t>(first + at) * a.heads + head) * splits * (HD + 2) + HD;
+#pragma unroll 4
+                    for (int s = lane % lanes; s < use; s += lanes) {
+                        const float2 x = *reinterpret_cast<const float2*>(from + s * (HD + 2));
+                        const float most = fmaxf(m, x.x);
+                        // A split that saw nothing has nothing to add; one whose scores are NaN has.
+                        total = fmaf(total, m == -INFINITY ? (total == 0.0f ? 0.0f : 1.0f) : exp2_fast(m - most),
+                                     x.y * (x.x == -INFINITY ? (x.y == 0.0f ? 0.0f : 1.0f) : exp2_fast(x.x - most)));
+                        m = most;
+                    }
                 }
-                total = warp_sum(total);
-                if (lane == 0) {
+                for (int o = lanes / 2; o > 0; o >>= 1) {
+                    const float other = __shfl_xor_sync(kFull, m, o), others = __shfl_xor_sync(kFull, total, o);
+                    const float most = fmaxf(m, other);
+                    total = total * (m == -INFINITY ? (total == 0.0f ? 0.0f : 1.0f) : exp2_fast(m - most)) +
+                            others * (other == -INFINITY ? (others == 0.0f ? 0.0f : 1.0f) : exp2_fast(other - most));
+                    m = most;
+                }
+                if (r < rows && lane % lanes == 0) {
                     tops[r] = m == -INFINITY ? 0.0f : m;
                     inverse[r] = total == 0.0f ? 0.0f : 1.0f / total;
                 }
             }
             __syncthreads();
+#pragma unroll 4
             for (int r = 0; r < rows; ++r) {
-                const int at = static_cast<int>((r0 + r) / group), head = kvh * group + static_cast<int>((r0 + r) % group);
-                const int p = min(position + at, c.slots - 1);
+                const int at = static_cast<int>(r0 + r) / group, head = kvh * group + static_cast<int>(r0 + r) % group;
+                const int p = length - n + at;
                 const float* from = scores + (static_cast<int64_t>(first + at) * a.heads + head) * pitch;
-                if (position + at >= c.slots) continue;  // a token outside the cache sees nothing
                 const float top = tops[r], by = inverse[r];
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const int key = key0 + threadIdx.x + i * kThreads;
-                    const bool seen = key <= p && (a.window == 0 || p - key < a.window || key < a.sinks);
-                    if (seen) sum[i] = fmaf(exp2_fast(from[key] - top), by, sum[i]);
+                    // A token outside the cache sees nothing.
+                    const bool seen = key <= p && p < c.slots && (a.window == 0 || p - key < a.window || key < a.sinks);
+                    if (seen) sum[i] = fmaf(exp2_fast(__ldcs(from + key) - top), by, sum[i]);
                 }
             }
         }
     }
     const int64_t base = (static_cast<int64_t>(row) * c.kv_heads + kvh) * c.slots;
+    if (!waited) pdl_wait();  // the stream's earlier writers of masses
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const int key = key0 + threadIdx.x + i * kThreads;
@@ -153,16 +177,19 @@ cudaError_t launch_attention_weights(cudaStream_t s, const Cache& c, const Batch
                                                   rows, splits, part, extra);
         if (e) return e;
     }
-    const int64_t blocks = static_cast<int64_t>(b.tokens) * a.heads +
-                           static_cast<int64_t>(b.count) * a.kv_heads * ((c.slots + kMassKeys - 1) / kMassKeys);
+    const int64_t queries = static_cast<int64_t>(b.tokens) * a.heads;
+    const bool warp = splits <= 32;
+    const int64_t joins = warp ? (queries + kWarps - 1) / kWarps : queries;
+    const int64_t blocks = joins + static_cast<int64_t>(b.count) * a.kv_heads * ((c.slots + kMassKeys - 1) / kMassKeys);
     return by_dtype(a.dtype, [&](auto type) {
         using T = decltype(type);
         return by_head_dim(a.head_dim, [&](auto hd) {
             constexpr int HD = decltype(hd)::value;
-            return launch_pdl(k_weights_join<T, HD>, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, s, c,
-                              b, a, rows, static_cast<T*>(out), out_stride, splits,
-                              static_cast<const float*>(part), static_cast<const float*>(extra.scores),
-                              extra.pitch, previous, decay, mass);
+            return launch_pdl(warp ? k_weights_join<T, HD, true> : k_weights_join<T, HD, false>,
+                              dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, s, c, b, a, rows,
+                              static_cast<T*>(out), out_stride, splits, static_cast<const float*>(part),
+                              static_cast<const float*>(extra.scores), extra.pitch, previous, decay, mass,
+                              static_cast<int>(joins));
         });
     });
 }

@@ -342,7 +342,7 @@ int check_eviction(const bst_kv_cache* cache, const bst_sequences* sequences, co
                std::to_string(e->to.slots) + " slots";
         return BST_SHAPE;
     }
-    if ((st = check_blocks(static_cast<int64_t>(b->count) * c->kv_heads * ((keep + 63) / 64), why))) return st;
+    if ((st = check_blocks(static_cast<int64_t>(b->count) * c->kv_heads * (8 + keep / 64), why))) return st;
     if (b->count > 0) {
         if (!mass || !to_mass || !lengths || !kept) {
             *why = "masses, new lengths and kept slots must not be null";
