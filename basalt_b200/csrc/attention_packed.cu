@@ -132,7 +132,10 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
     uint64_t* const s_full = empty + L::kSlots;  // [tile][buffer] scores are done
     uint64_t* const p_full = s_full + 4;         // [tile][buffer] weights are written
     uint64_t* const o_done = p_full + 4;         // [tile] a product into O is done
-    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(o_done + 2);
+    // [tile] the last one is. (Its phase of o_done can be over, and the parity of the one before it be that of
+    // the next, when a warp that was held up comes to wait for that.)
+    uint64_t* const o_last = o_done + 2;
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(o_last + 2);
     int* const status = reinterpret_cast<int*>(tmem_slot + 1);  // [0] error code, [1] abort, [2] redo
 
     if (threadIdx.x == 0) {
@@ -144,8 +147,7 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
             mbar_init(s_full + i, 1);
             mbar_init(p_full + i, kTcSoft / 2);
         }
-        mbar_init(o_done, 1);
-        mbar_init(o_done + 1, 1);
+        for (int i = 0; i < 4; ++i) mbar_init(o_done + i, 1);
         status[0] = status[1] = status[2] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -272,7 +274,7 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
                         tc_mma_ts(h * 256 + 128, p + 8 * k, va + k * (2048 >> 4), kDescHigh, o_idesc,
                                   i > 0 || k > 0);
                     }
-                    mma_commit(o_done + h);
+                    mma_commit(i + 1 < n_tiles ? o_done + h : o_last + h);
                     // Into the buffer that the product above has just read.
                     if (more) scores(h, i + 2);
                 }
@@ -389,9 +391,8 @@ k_packed_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
             key0 = i + 1 == keys.sink_tiles ? keys.first : key0 + kTcKeys;
         }
         if (half < halves) {
-            // The last two products into O (those before were done when the last scores were).
-            if (keys.tiles > 1) ok = ok && mbar_wait(o_done + half, keys.tiles & 1, status, 9, abort);
-            ok = ok && mbar_wait(o_done + half, (keys.tiles - 1) & 1, status, 10, abort);
+            // Products are done in order.
+            ok = ok && mbar_wait(o_last + half, 0, status, 9, abort);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const float by = total == 0.0f ? 0.0f : 1.0f / total;
             // Through the queries' place in shared memory, so that rows are written whole.
