@@ -31,14 +31,4 @@ cudaError_t launch_attention_cached(cudaStream_t s, const Cache& c, const Batch&
     });
 }
 
-CachedPlan plan_cached(const Cache& c, const Batch& b, const AttnSpec& a) {
-    return CachedPlan{split_count(c, b, a), rows_of_tile(b, a)};
-}
-
-cudaError_t launch_cached_parts(cudaStream_t s, const Cache& c, const Batch& b, const AttnSpec& a,
-                                const CachedPlan& plan, const void* q, int64_t q_stride, float* part) {
-    return run_cached<kOwn>(s, c, b, a, q, q_stride, nullptr, 0, tile_bound(b, a, plan.rows), plan.rows,
-                            plan.splits, part, Extra());
-}
-
 }  // namespace bst

@@ -354,11 +354,13 @@ enum Pass {
     kOwn,     // attention of the sequences over their own rows
     kScores,  // the same, and every score (base 2, -infinity where hidden) goes to Extra::scores
     kPrefix,  // attention of all tokens over the first Extra::length keys of row Extra::row
+    kBeside,  // kOwn that leaves sums and runs beside a pass before it, for whose end one more CTA waits
 };
 struct Extra {
     float* scores = nullptr;  // [tokens][heads][pitch]
     int64_t pitch = 0;        // slots, rounded up to a block
     int row = 0, length = 0;
+    bool early = false;       // kBeside: may start before the pass before it ends
 };
 
 // ROWS queries a tile: 8, or 16 for bf16 batches that have more than eight to a key head, so that
@@ -390,6 +392,14 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     Tile tile;
     int row, length;
+    if constexpr (PASS == kPrefix) pdl_trigger();
+    if constexpr (PASS == kBeside) {
+        // The pass before this one need not be over; the kernel behind both waits for this one alone.
+        if (blockIdx.x == gridDim.x - 1) {
+            if (blockIdx.y + blockIdx.z == 0) pdl_wait();
+            return;
+        }
+    }
     if constexpr (PASS == kPrefix) {
         // All tokens that sequences own are one sequence of queries, each of which sees every key.
         if (!owned_tokens(b, &tile.first, &tile.n)) return;
@@ -1115,6 +1125,12 @@ k_cached_one(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_st
     // Lanes with the same groups: all, or every other one.
     constexpr int kNext = G == 4 ? 2 : 1;
     __shared__ float merge[kOneWarps][HD + 2];
+    if constexpr (PASS == kBeside) {
+        if (blockIdx.x == gridDim.x - 1) {
+            if (blockIdx.y + blockIdx.z == 0) pdl_wait();
+            return;
+        }
+    }
     const int seq = blockIdx.x, head = blockIdx.y, split = blockIdx.z;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int word = lane % kLanes, sub = lane / kLanes;
@@ -1382,6 +1398,181 @@ k_cached_one(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_st
     }
 }
 
+// One query a key head over a float32 or bf16 cache, on the ordinary units too: two multiply-adds a value are
+// far below what memory takes, while on the tensor cores seven of eight rows would be empty and float32 entries
+// have to be split in three (32 sequences of 33 to 512 keys of eight float32 heads of 64: 18 us there). Lanes
+// hold 16 bytes of a key, the warp kAtOnce keys a pass; the scores of eight passes change places as above.
+// Sums are plain float32, so NaN and infinities come out as in the formula; what lies behind the end is not read.
+constexpr int kPlainWarps = 4;
+
+// Whether a pass is for this kernel.
+inline bool plain_query(const Cache& c, const Batch& b, const AttnSpec& a) {
+    return c.storage != BST_DTYPE_U4 && a.heads == a.kv_heads && !b.starts;
+}
+
+template <typename S>
+__device__ __forceinline__ void entries_of(const uint4& u, float (&x)[16 / sizeof(S)]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(S) == 4) {
+            x[i] = __uint_as_float(w[i]);
+        } else {
+            x[2 * i] = low_of(w[i]);
+            x[2 * i + 1] = high_of(w[i]);
+        }
+    }
+}
+
+template <typename T, typename S, int HD, int PASS>
+__global__ void __launch_bounds__(kPlainWarps * 32, 4)
+k_cached_plain(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride, int splits,
+               float* __restrict__ part, Extra extra) {
+    constexpr int kVec = 16 / sizeof(S), kLanes = HD / kVec, kAtOnce = 32 / kLanes, kPasses = 8;
+    constexpr int kKeys = kAtOnce * kPasses, kMine = kLanes < 8 ? 8 / kLanes : 1, kCopies = kLanes > 8 ? kLanes / 8 : 1;
+    __shared__ float merge[kPlainWarps][HD + 2];
+    if constexpr (PASS == kBeside) {
+        if (blockIdx.x == gridDim.x - 1) {
+            if (blockIdx.y + blockIdx.z == 0) pdl_wait();
+            return;
+        }
+    }
+    const int seq = blockIdx.x, head = blockIdx.y, split = blockIdx.z;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, word = lane % kLanes, sub = lane / kLanes;
+    const int row = b.rows ? __ldg(b.rows + seq) : seq;
+    const int position = max(0, __ldg(b.lengths + seq)) - 1;
+    const bool inside = row >= 0 && row < c.rows;
+    const Visible seen(position, inside ? position : -1, c.slots, a.window, a.sinks);
+    const int use = useful_splits(seen.blocks, splits);
+    if (split >= use) return;
+    // Places 0 .. sunk are the sinks before the window, the others the window's keys.
+    const bool sees = inside && position >= 0 && position < c.slots;
+    const int sunk = sees ? min(a.sinks, seen.first) : 0, skipped = seen.first - sunk;
+    const int64_t places = sees ? static_cast<int64_t>(sunk) + seen.end - seen.first : 0;
+    const int x0 = static_cast<int>(places * split / use), x1 = static_cast<int>(places * (split + 1) / use);
+    const int64_t at = ((static_cast<int64_t>(inside ? row : 0) * c.kv_heads + head) * c.slots * HD) + word * kVec;
+    const S* const kb = static_cast<const S*>(c.k) + at;
+    const S* const vb = static_cast<const S*>(c.v) + at;
+    auto key_at = [&](int place) { return static_cast<int64_t>(place + (place >= sunk ? skipped : 0)); };
+    // The entries of the keys at places x + i kAtOnce + sub; zeros behind the end.
+    auto load = [&](int x, const S* from, uint4 (&w)[kPasses]) {
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+            const int place = x + i * kAtOnce + sub;
+            w[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (place < x1) w[i] = __ldcs(reinterpret_cast<const uint4*>(from + key_at(place) * HD));
+        }
+    };
+    uint4 kw[kPasses];
+    int x = x0 + warp * kKeys;
+    load(x, kb, kw);
+    float qv[kVec];
+    const T* const src = q + seq * q_stride + head * HD + word * kVec;
+#pragma unroll
+    for (int n = 0; n < kVec; ++n) qv[n] = to_f(src[n]);
+    const float to_score = a.scale * kLog2e;
+    const int my_pass = word * 8 / kLanes;  // and the one behind it with two keys a lane
+    float* const keep_scores = extra.scores + (static_cast<int64_t>(seq) * a.heads + head) * extra.pitch;
+
+    float acc[kVec] = {}, top = -INFINITY, total = 0.0f;
+    for (; x < x1; x += kPlainWarps * kKeys) {
+        uint4 vw[kPasses];
+        load(x, vb, vw);
+        float s[kPasses];
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+            float k[kVec];
+            entries_of<S>(kw[i], k);
+            s[i] = 0.0f;
+#pragma unroll
+            for (int n = 0; n < kVec; ++n) s[i] = fmaf(k[n], qv[n], s[i]);
+        }
+        load(x + kPlainWarps * kKeys, kb, kw);
+#pragma unroll
+        for (int n = kPasses / 2, o = kLanes / 2; o > 0; o >>= 1, n = n > 1 ? n / 2 : (n == 1 ? 0 : 0)) {
+            if (n > 0) {
+                const bool upper = lane & o;
+#pragma unroll
+                for (int i = 0; i < n; ++i) {
+                    const float away = upper ? s[i] : s[i + n];
+                    s[i] = (upper ? s[i + n] : s[i]) + __shfl_xor_sync(kFull, away, o);
+                }
+            } else {
+                s[0] += __shfl_xor_sync(kFull, s[0], o);
+            }
+        }
+        float score[kMine], most = -INFINITY;
+#pragma unroll
+        for (int m = 0; m < kMine; ++m) {
+            const int place = x + (my_pass + m) * kAtOnce + sub;
+            score[m] = s[m] * to_score;
+            if (place >= x1) {
+                score[m] = -INFINITY;
+            } else if constexpr (PASS == kScores) {
+                if (word % kCopies == 0) keep_scores[key_at(place)] = score[m];
+            }
+            most = fmaxf(most, score[m]);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(kFull, most, o));
+        if (most > top) {
+            const float keep = top == -INFINITY ? 0.0f : exp2_fast(top - most);
+            top = most;
+            total *= keep;
+#pragma unroll
+            for (int n = 0; n < kVec; ++n) acc[n] *= keep;
+        }
+        const float base = top == -INFINITY ? 0.0f : top;
+        float p[kMine];
+#pragma unroll
+        for (int m = 0; m < kMine; ++m) {
+            p[m] = exp2_fast(score[m] - base);
+            total += p[m];
+        }
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+            const float weight = __shfl_sync(kFull, p[i % kMine], sub * kLanes + i * kLanes / 8);
+            float v[kVec];
+            entries_of<S>(vw[i], v);
+#pragma unroll
+            for (int n = 0; n < kVec; ++n) acc[n] = fmaf(weight, v[n], acc[n]);
+        }
+    }
+    // The lanes' sums, then the warps'. Where lanes share a key each counts its weight.
+    total = warp_sum(total) * (1.0f / kCopies);
+#pragma unroll
+    for (int n = 0; n < kVec; ++n) {
+#pragma unroll
+        for (int o = kLanes; o < 32; o <<= 1) acc[n] += __shfl_xor_sync(kFull, acc[n], o);
+        if (lane < kLanes) merge[warp][word * kVec + n] = acc[n];
+    }
+    if (lane == 0) {
+        merge[warp][HD] = top;
+        merge[warp][HD + 1] = total;
+    }
+    __syncthreads();
+    for (int ch = threadIdx.x; ch < HD; ch += kPlainWarps * 32) {
+        float m = -INFINITY, sum = 0.0f, value = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kPlainWarps; ++w) m = fmaxf(m, merge[w][HD]);
+#pragma unroll
+        for (int w = 0; w < kPlainWarps; ++w) {
+            const float f = merge[w][HD] == -INFINITY ? 0.0f : exp2_fast(merge[w][HD] - m);
+            // A warp that saw no key has nothing to add, and one whose scores are all NaN has that.
+            if (merge[w][HD] != -INFINITY || merge[w][HD + 1] != 0.0f) {
+                sum = fmaf(merge[w][HD + 1], f, sum);
+                value = fmaf(merge[w][ch], f, value);
+            }
+        }
+        float* const to = part + ((static_cast<int64_t>(seq) * a.heads + head) * splits + split) * (HD + 2);
+        to[ch] = value;
+        if (ch == 0) {
+            to[HD] = m;
+            to[HD + 1] = sum;
+        }
+    }
+}
+
 // Joins the splits of a query, one CTA each: the splits' factors first, then every warp sums its
 // share of the splits with all loads independent of one another.
 constexpr int kMaxSplits = 512;
@@ -1506,11 +1697,11 @@ inline int ctas_per_sm(const Cache& c) {
 // and where their workspace would pass kSplitBytes: two prompts' chunks of 4096 tokens over 131 072 slots
 // (32 heads of 128 over 8) took 4.4 GB, of which no SM had any use, and now take none.
 constexpr int64_t kSplitBytes = 128 << 20;  // about what L2 holds
-inline int split_count(const Cache& c, const Batch& b, const AttnSpec& a) {
+inline int split_count(const Cache& c, const Batch& b, const AttnSpec& a, int per_sm = 0) {
     int64_t keys = c.slots;
     if (a.window) keys = std::min<int64_t>(keys, static_cast<int64_t>(a.window) + a.sinks + 2 * kBlock);
     const int64_t units = static_cast<int64_t>(tile_bound(b, a, rows_of_tile(b, a))) * a.kv_heads;
-    const int64_t card = 148 * (one_query(c, b, a) ? kOneCtas : ctas_per_sm(c));
+    const int64_t card = 148 * (per_sm ? per_sm : one_query(c, b, a) ? kOneCtas : ctas_per_sm(c));
     const int64_t fill = card / std::max<int64_t>(units, 1);
     int64_t even = 1;
     if (b.count > 1) {
@@ -1523,14 +1714,25 @@ inline int split_count(const Cache& c, const Batch& b, const AttnSpec& a) {
     return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({std::max(fill, even), most, kMaxSplits})));
 }
 
-// Queues k_cached (or k_cached_one) for one pass: `tiles` tiles of `rows` query rows, each key head, and
-// `splits` of the keys.
+// Queues the kernel of one pass: `tiles` tiles of `rows` query rows, each key head, and `splits` of the keys.
 template <int PASS>
 cudaError_t run_cached(cudaStream_t s, const Cache& c, const Batch& b, const AttnSpec& a, const void* q,
                        int64_t q_stride, void* out, int64_t out_stride, int tiles, int rows, int splits,
                        float* part, const Extra& extra) {
     return by_dtype(a.dtype, [&](auto type) {
         using T = decltype(type);
+        const T* const from = static_cast<const T*>(q);
+        T* const to = static_cast<T*>(out);
+        constexpr int kMore = PASS == kBeside ? 1 : 0;  // the CTA that waits
+        auto launch = [&](auto kernel, dim3 grid, int threads, int smem, auto... args) {
+            if (smem > 48 << 10) {
+                const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+                if (e) return e;
+            }
+            if (PASS == kBeside && extra.early) return launch_pdl(kernel, grid, dim3(threads), smem, s, args...);
+            kernel<<<grid, threads, smem, s>>>(args...);
+            return cudaGetLastError();
+        };
         return by_head_dim(a.head_dim, [&](auto hd) {
             constexpr int HD = decltype(hd)::value;
             return by_storage(c.storage, [&](auto st) {
@@ -1538,22 +1740,22 @@ cudaError_t run_cached(cudaStream_t s, const Cache& c, const Batch& b, const Att
                 using L = Layout<STORAGE, HD>;
                 auto run = [&](auto tile_rows) {
                     constexpr int ROWS = decltype(tile_rows)::value;
-                    const auto kernel = k_cached<T, STORAGE, HD, ROWS, PASS>;
-                    const cudaError_t err = cudaFuncSetAttribute(
-                        kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::smem(ROWS));
-                    if (err) return err;
-                    kernel<<<dim3(tiles, a.kv_heads, splits), kThreads, L::smem(ROWS), s>>>(
-                        c, b, a, static_cast<const T*>(q), q_stride, static_cast<T*>(out), out_stride,
-                        splits, part, extra);
-                    return cudaGetLastError();
+                    return launch(k_cached<T, STORAGE, HD, ROWS, PASS>, dim3(tiles + kMore, a.kv_heads, splits),
+                                  kThreads, L::smem(ROWS), c, b, a, from, q_stride, to, out_stride, splits, part,
+                                  extra);
                 };
                 if constexpr (STORAGE == BST_DTYPE_U4 && PASS != kPrefix) {
                     if (one_query(c, b, a)) {
-                        k_cached_one<T, HD, PASS>
-                            <<<dim3(b.count, a.heads, splits), kOneWarps * 32, 0, s>>>(
-                                c, b, a, static_cast<const T*>(q), q_stride, static_cast<T*>(out),
-                                out_stride, splits, part, extra);
-                        return cudaGetLastError();
+                        return launch(k_cached_one<T, HD, PASS>, dim3(b.count + kMore, a.heads, splits),
+                                      kOneWarps * 32, 0, c, b, a, from, q_stride, to, out_stride, splits, part,
+                                      extra);
+                    }
+                }
+                if constexpr (STORAGE != BST_DTYPE_U4 && (PASS == kScores || PASS == kBeside)) {
+                    using S = typename std::conditional<STORAGE == BST_DTYPE_F32, float, __nv_bfloat16>::type;
+                    if (plain_query(c, b, a)) {
+                        return launch(k_cached_plain<T, S, HD, PASS>, dim3(b.count + kMore, a.heads, splits),
+                                      kPlainWarps * 32, 0, c, b, a, from, q_stride, splits, part, extra);
                     }
                 }
                 if constexpr (sizeof(T) == 2) {

@@ -112,6 +112,7 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
     // The tiles of a share of a head's keys stand next to one another, so that they read it together.
     const int kvh = blockIdx.x / tiles % a.kv_heads, split = blockIdx.x / tiles / a.kv_heads;
     int first, n;
+    pdl_trigger();  // the own keys' pass may fill what this one leaves free
     if (!owned_tokens(b, &first, &n)) return;
     const int64_t r0 = static_cast<int64_t>(blockIdx.x % tiles) * kRows;
     if (r0 >= static_cast<int64_t>(n) * group) return;

@@ -6,7 +6,8 @@
 // Sums over disjoint sets of keys join exactly (each set leaves its maximum, its sum of weights and its
 // weighted values), so the prefix is a pass of its own: its queries are those of the whole batch, a tile of
 // them reads it once, where attention over a copy in every row would read it once a sequence. The own keys
-// are the pass of attention_cached, and one kernel joins both passes' splits.
+// are the pass of attention_cached, which runs beside the first as far as that leaves room, and one kernel
+// joins both passes' splits.
 
 #include "attention_cached.cuh"
 
@@ -53,6 +54,16 @@ bool large(const Batch& b, const AttnSpec& a, const Prefix& p) {
     return prefix_tc_takes(p, a) && static_cast<int64_t>(b.tokens) * (a.heads / a.kv_heads) >= kLargeRows;
 }
 
+// Splits of the own keys. They are joined anyway, so that rows of uneven lengths may be split where they fill
+// the card once but not evenly: four waves (64 rows of 20 to 1000 keys: 33 us in 1.7 waves without splits).
+int own_splits(const Cache& c, const Batch& b, const AttnSpec& a) {
+    const int per_sm = plain_query(c, b, a) ? 4 : one_query(c, b, a) ? kOneCtas : ctas_per_sm(c);
+    const int64_t units = static_cast<int64_t>(tile_bound(b, a, rows_of_tile(b, a))) * a.kv_heads;
+    const int64_t waves = 4 * 148 * per_sm / std::max<int64_t>(1, units);
+    const int64_t most = std::min<int64_t>(c.slots / 128, 16);
+    return std::max(split_count(c, b, a, per_sm), static_cast<int>(std::min(waves, most)));
+}
+
 size_t part_bytes(const Batch& b, const AttnSpec& a, int splits) {
     return static_cast<size_t>(b.tokens) * a.heads * splits * (a.head_dim + 2) * sizeof(float);
 }
@@ -64,14 +75,17 @@ __global__ void __launch_bounds__(kThreads)
 k_shared_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out, int64_t out_stride,
               int own_splits, const float* __restrict__ own, int prefix_splits,
               const float* __restrict__ prefix) {
-    const int64_t query = WARP ? static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5) : blockIdx.x;
-    const int token = static_cast<int>(query / a.heads), head = static_cast<int>(query - static_cast<int64_t>(token) * a.heads);
+    const uint32_t query = WARP ? blockIdx.x * kWarps + (threadIdx.x >> 5) : blockIdx.x;
+    const int token = query / static_cast<uint32_t>(a.heads), head = query - static_cast<uint32_t>(token) * a.heads;
     int seq, first, n;
-    if (token >= b.tokens || !find_sequence(b, token, &seq, &first, &n)) return;
+    if (token >= b.tokens || !find_sequence(b, token, &seq, &first, &n)) {
+        pdl_wait();  // every CTA does: this kernel's end is that of all three
+        return;
+    }
     const int use = used_splits(c, b, a, tile_rows, own_splits, seq, token - first, n, head);
     pdl_wait();
-    const float* const mine = own + query * own_splits * (HD + 2);
-    const float* const common = prefix + query * prefix_splits * (HD + 2);
+    const float* const mine = own + static_cast<int64_t>(query) * own_splits * (HD + 2);
+    const float* const common = prefix + static_cast<int64_t>(query) * prefix_splits * (HD + 2);
     auto at = [&](int s) { return s < use ? mine + s * (HD + 2) : common + (s - use) * (HD + 2); };
     T* const to = out + token * out_stride + head * HD;
     if constexpr (WARP) {
@@ -87,16 +101,16 @@ size_t attention_shared_workspace(const Cache& c, const Batch& b, const AttnSpec
     if (b.tokens < 1) return 0;
     int splits = p.length > 0 ? plan_small(b, a, p).splits : 0;
     if (p.length > 0 && large(b, a, p)) splits = std::max(splits, plan_large(b, a, p).splits);
-    return part_bytes(b, a, plan_cached(c, b, a).splits + splits);
+    return part_bytes(b, a, own_splits(c, b, a) + splits);
 }
 
 cudaError_t launch_attention_shared(cudaStream_t s, const Cache& c, const Batch& b, const AttnSpec& a,
                                     const Prefix& p, const void* q, int64_t q_stride, void* out,
                                     int64_t out_stride, void* workspace) {
     if (b.tokens < 1 || b.count < 1) return cudaSuccess;
-    const CachedPlan plan = plan_cached(c, b, a);
+    const int own_count = own_splits(c, b, a), rows = rows_of_tile(b, a);
     float* const own = static_cast<float*>(workspace);
-    float* const prefix = own + part_bytes(b, a, plan.splits) / sizeof(float);
+    float* const prefix = own + part_bytes(b, a, own_count) / sizeof(float);
     int splits = 0;
     if (p.length > 0) {
         cudaError_t e;
@@ -115,16 +129,20 @@ cudaError_t launch_attention_shared(cudaStream_t s, const Cache& c, const Batch&
         }
         if (e) return e;
     }
-    if (const cudaError_t e = launch_cached_parts(s, c, b, a, plan, q, q_stride, own)) return e;
+    Extra beside;
+    beside.early = splits > 0;
+    const cudaError_t e = run_cached<kBeside>(s, c, b, a, q, q_stride, nullptr, 0, tile_bound(b, a, rows), rows,
+                                              own_count, own, beside);
+    if (e) return e;
     return by_dtype(a.dtype, [&](auto type) {
         using T = decltype(type);
         return by_head_dim(a.head_dim, [&](auto hd) {
             constexpr int HD = decltype(hd)::value;
             const int64_t queries = static_cast<int64_t>(b.tokens) * a.heads;
-            const bool warp = plan.splits + splits <= 32;
+            const bool warp = own_count + splits <= 32;
             return launch_pdl(warp ? k_shared_join<T, HD, true> : k_shared_join<T, HD, false>,
                               dim3(static_cast<unsigned>(warp ? (queries + kWarps - 1) / kWarps : queries)),
-                              dim3(kThreads), 0, s, c, b, a, plan.rows, static_cast<T*>(out), out_stride, plan.splits,
+                              dim3(kThreads), 0, s, c, b, a, rows, static_cast<T*>(out), out_stride, own_count,
                               static_cast<const float*>(own), splits, static_cast<const float*>(prefix));
         });
     });

@@ -39,19 +39,28 @@ __device__ __forceinline__ int next_of_row(const Batch& b, int seq, int row) {
     return next;
 }
 
+// A split's maximum and sum into those of the splits before. One that saw nothing has nothing to add; one whose
+// scores are NaN has.
+__device__ __forceinline__ void add_split(float* m, float* total, float top, float sum) {
+    const float most = fmaxf(*m, top);
+    auto scaled = [&](float x, float at) { return at == -INFINITY ? (x == 0.0f ? 0.0f : x) : x * exp2_fast(at - most); };
+    *total = scaled(*total, *m) + scaled(sum, top);
+    *m = most;
+}
+
 template <typename T, int HD, bool WARP>
 __global__ void __launch_bounds__(kThreads)
 k_weights_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out, int64_t out_stride,
                int splits, const float* __restrict__ part, const float* __restrict__ scores, int64_t pitch,
                const float* previous, float decay, float* mass, int joins) {
     if (blockIdx.x < joins) {
-        const int64_t query = WARP ? static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5) : blockIdx.x;
-        const int token = static_cast<int>(query / a.heads), head = static_cast<int>(query - static_cast<int64_t>(token) * a.heads);
+        const uint32_t query = WARP ? blockIdx.x * kWarps + (threadIdx.x >> 5) : blockIdx.x;
+        const int token = query / static_cast<uint32_t>(a.heads), head = query - static_cast<uint32_t>(token) * a.heads;
         int seq, first, n;
         if (token >= b.tokens || !find_sequence(b, token, &seq, &first, &n)) return;
         const int use = used_splits(c, b, a, tile_rows, splits, seq, token - first, n, head);
         pdl_wait();
-        const float* const from = part + query * splits * (HD + 2);
+        const float* const from = part + static_cast<int64_t>(query) * splits * (HD + 2);
         auto at = [&](int s) { return from + s * (HD + 2); };
         T* const to = out + token * out_stride + head * HD;
         if constexpr (WARP) {
@@ -62,16 +71,20 @@ k_weights_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out,
         return;
     }
     __shared__ float tops[kMassRows], inverse[kMassRows];
-    const int chunks = (c.slots + kMassKeys - 1) / kMassKeys;
-    const int64_t place = blockIdx.x - joins;
-    const int kvh = static_cast<int>(place % a.kv_heads);
-    const int64_t rest = place / a.kv_heads;
-    const int key0 = static_cast<int>(rest % chunks) * kMassKeys;
-    int seq = static_cast<int>(rest / chunks);
+    // In 32 bits: the quotients of 64 took a third of all instructions.
+    const uint32_t chunks = (c.slots + kMassKeys - 1) / kMassKeys, place = blockIdx.x - joins;
+    const uint32_t of_head = place / chunks;
+    const int key0 = static_cast<int>(place - of_head * chunks) * kMassKeys;
+    int seq = of_head / static_cast<uint32_t>(a.kv_heads);
+    const int kvh = of_head - static_cast<uint32_t>(seq) * a.kv_heads;
     const int row = b.rows ? __ldg(b.rows + seq) : seq;
     if (row < 0 || row >= c.rows || !first_of_row(b, seq, row)) return;
     const int group = a.heads / a.kv_heads, lane = threadIdx.x & 31;
-    constexpr int N = kMassKeys / kThreads;
+    constexpr int N = kMassKeys / kThreads, kBatch = 2;  // rows whose scores are under way together
+    const int my_key = key0 + threadIdx.x;
+    int offset[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) offset[i] = min(my_key + i * kThreads, static_cast<int>(pitch) - 1);
     float sum[N] = {};
     int end = 0;
     bool waited = false;
@@ -86,36 +99,46 @@ k_weights_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out,
         }
         if (!waited) pdl_wait();
         waited = true;
-        const int64_t all = static_cast<int64_t>(n) * group;
-        for (int64_t r0 = 0; r0 < all; r0 += kMassRows) {
-            const int rows = static_cast<int>(min(static_cast<int64_t>(kMassRows), all - r0));
+        const int all = n * group;
+        // Scores of kBatch rows from r on; what lies beside the rows or what they see is read, not used.
+        int load_at = 0, load_head = 0;
+        auto load = [&](float (&x)[kBatch][N]) {
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                const float* from = scores + (static_cast<int64_t>(first + load_at) * a.heads + kvh * group + load_head) * pitch;
+#pragma unroll
+                for (int i = 0; i < N; ++i) x[k][i] = load_at < n ? __ldcs(from + offset[i]) : 0.0f;
+                if (++load_head == group) {
+                    load_head = 0;
+                    ++load_at;
+                }
+            }
+        };
+        float x[kBatch][N];
+        load(x);
+        int at = 0, head_of = 0;
+        for (int r0 = 0; r0 < all; r0 += kMassRows) {
+            const int rows = min(kMassRows, all - r0);
             // Maxima and sums of the rows: as many lanes a row as there are to spare.
             int lanes = 32;
             while (lanes > 1 && rows * lanes > kThreads) lanes >>= 1;
-            __syncthreads();
             const int of_warp = 32 / lanes;  // a warp takes that many rows at a time
+            __syncthreads();
             for (int r = threadIdx.x / lanes; r < (rows + of_warp - 1) / of_warp * of_warp; r += kThreads / lanes) {
                 float m = -INFINITY, total = 0.0f;
                 if (r < rows) {
-                    const int at = static_cast<int>((r0 + r) / group), head = kvh * group + static_cast<int>((r0 + r) % group);
-                    const int use = used_splits(c, a, tile_rows, splits, row, length, at, n, head);
-                    const float* from = part + (static_cast<int64_t>(first + at) * a.heads + head) * splits * (HD + 2) + HD;
+                    const int token = (r0 + r) / group, head = kvh * group + (r0 + r) - token * group;
+                    const int use = used_splits(c, a, tile_rows, splits, row, length, token, n, head);
+                    const float* from = part + (static_cast<int64_t>(first + token) * a.heads + head) * splits * (HD + 2) + HD;
 #pragma unroll 4
                     for (int s = lane % lanes; s < use; s += lanes) {
-                        const float2 x = *reinterpret_cast<const float2*>(from + s * (HD + 2));
-                        const float most = fmaxf(m, x.x);
-                        // A split that saw nothing has nothing to add; one whose scores are NaN has.
-                        total = fmaf(total, m == -INFINITY ? (total == 0.0f ? 0.0f : 1.0f) : exp2_fast(m - most),
-                                     x.y * (x.x == -INFINITY ? (x.y == 0.0f ? 0.0f : 1.0f) : exp2_fast(x.x - most)));
-                        m = most;
+                        const float2 y = *reinterpret_cast<const float2*>(from + s * (HD + 2));
+                        add_split(&m, &total, y.x, y.y);
                     }
                 }
                 for (int o = lanes / 2; o > 0; o >>= 1) {
                     const float other = __shfl_xor_sync(kFull, m, o), others = __shfl_xor_sync(kFull, total, o);
-                    const float most = fmaxf(m, other);
-                    total = total * (m == -INFINITY ? (total == 0.0f ? 0.0f : 1.0f) : exp2_fast(m - most)) +
-                            others * (other == -INFINITY ? (others == 0.0f ? 0.0f : 1.0f) : exp2_fast(other - most));
-                    m = most;
+                    add_split(&m, &total, other, others);
                 }
                 if (r < rows && lane % lanes == 0) {
                     tops[r] = m == -INFINITY ? 0.0f : m;
@@ -123,18 +146,37 @@ k_weights_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out,
                 }
             }
             __syncthreads();
-#pragma unroll 4
-            for (int r = 0; r < rows; ++r) {
-                const int at = static_cast<int>(r0 + r) / group, head = kvh * group + static_cast<int>(r0 + r) % group;
-                const int p = length - n + at;
-                const float* from = scores + (static_cast<int64_t>(first + at) * a.heads + head) * pitch;
-                const float top = tops[r], by = inverse[r];
+            for (int r = 0; r < rows; r += kBatch) {  // 64 rows are whole batches
+                float next[kBatch][N];
+                load(next);
 #pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const int key = key0 + threadIdx.x + i * kThreads;
-                    // A token outside the cache sees nothing.
-                    const bool seen = key <= p && p < c.slots && (a.window == 0 || p - key < a.window || key < a.sinks);
-                    if (seen) sum[i] = fmaf(exp2_fast(__ldcs(from + key) - top), by, sum[i]);
+                for (int k = 0; k < kBatch; ++k) {
+                    if (r + k < rows) {
+                        // A token outside the cache sees nothing.
+                        const int p = length - n + at;
+                        const float top = tops[r + k], by = inverse[r + k];
+                        if (a.window == 0 && key0 + kMassKeys - 1 <= p && p < c.slots) {
+#pragma unroll
+                            for (int i = 0; i < N; ++i) sum[i] = fmaf(exp2_fast(x[k][i] - top), by, sum[i]);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < N; ++i) {
+                                const int key = my_key + i * kThreads;
+                                const bool seen = key <= p && p < c.slots && (a.window == 0 || p - key < a.window || key < a.sinks);
+                                const float more = fmaf(exp2_fast(x[k][i] - top), by, sum[i]);
+                                sum[i] = seen ? more : sum[i];
+                            }
+                        }
+                    }
+                    if (++head_of == group) {
+                        head_of = 0;
+                        ++at;
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) x[k][i] = next[k][i];
                 }
             }
         }
@@ -150,6 +192,10 @@ k_weights_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out,
     }
 }
 
+int weights_splits(const Cache& c, const Batch& b, const AttnSpec& a) {
+    return split_count(c, b, a, plain_query(c, b, a) ? 4 : 0);
+}
+
 int64_t pitch_of(const Cache& c) { return (static_cast<int64_t>(c.slots) + kBlock - 1) / kBlock * kBlock; }
 
 size_t score_bytes(const Cache& c, const Batch& b, const AttnSpec& a) {
@@ -159,7 +205,7 @@ size_t score_bytes(const Cache& c, const Batch& b, const AttnSpec& a) {
 }  // namespace
 
 size_t attention_weights_workspace(const Cache& c, const Batch& b, const AttnSpec& a) {
-    const size_t query = static_cast<size_t>(split_count(c, b, a)) * (a.head_dim + 2) * sizeof(float);
+    const size_t query = static_cast<size_t>(weights_splits(c, b, a)) * (a.head_dim + 2) * sizeof(float);
     return score_bytes(c, b, a) + static_cast<size_t>(b.tokens) * a.heads * query;
 }
 
@@ -167,7 +213,7 @@ cudaError_t launch_attention_weights(cudaStream_t s, const Cache& c, const Batch
                                      const void* q, int64_t q_stride, void* out, int64_t out_stride,
                                      const float* previous, float decay, float* mass, void* workspace) {
     if (b.count < 1) return cudaSuccess;
-    const int splits = split_count(c, b, a), rows = rows_of_tile(b, a);
+    const int splits = weights_splits(c, b, a), rows = rows_of_tile(b, a);
     Extra extra;
     extra.scores = static_cast<float*>(workspace);
     extra.pitch = pitch_of(c);

@@ -281,8 +281,10 @@ template <int CTAS>
 cudaError_t choose(cudaStream_t s, const Cache& c, const Batch& b, const Eviction& e) {
     const int run = ((c.slots + CTAS * kChoose - 1) / (CTAS * kChoose)) | 1;
     const int held = static_cast<int64_t>(run) * kChoose <= kHeld ? run * kChoose : 0;
-    cudaError_t err = cudaFuncSetAttribute(k_evict_choose<CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeld * 4);
-    if (err) return err;
+    if (held > 4096) {  // beside 24 KB of counts, more than a kernel has by itself
+        const cudaError_t err = cudaFuncSetAttribute(k_evict_choose<CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, held * 4);
+        if (err) return err;
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(c.kv_heads) * b.count * CTAS));
     cfg.blockDim = dim3(kChoose);

@@ -646,7 +646,7 @@ int32_t bst_attention_weights(int32_t device, void* stream, const bst_kv_cache* 
             }
         }
         if (!st) {
-            const int64_t chunks = (static_cast<int64_t>(c.slots) + 1023) / 1024;
+            const int64_t chunks = (static_cast<int64_t>(c.slots) + 511) / 512;
             st = check_blocks(static_cast<int64_t>(b.tokens) * a.heads + chunks * a.kv_heads * b.count, &why);
         }
         if (!st) {

@@ -41,15 +41,6 @@ size_t attention_cached_workspace(const Cache& c, const Batch& b, const AttnSpec
 cudaError_t launch_attention_cached(cudaStream_t s, const Cache& c, const Batch& b,
                                     const AttnSpec& a, const void* q, int64_t q_stride, void* out,
                                     int64_t out_stride, void* workspace);
-// The splits of a cached call and its query rows a tile; the pass that leaves every split's sums in `part`,
-// [tokens][heads][splits][head_dim outputs, maximum (base 2), sum of weights].
-struct CachedPlan {
-    int splits, rows;
-};
-CachedPlan plan_cached(const Cache& c, const Batch& b, const AttnSpec& a);
-cudaError_t launch_cached_parts(cudaStream_t s, const Cache& c, const Batch& b, const AttnSpec& a,
-                                const CachedPlan& plan, const void* q, int64_t q_stride, float* part);
-
 // Keys that a batch shares: the first `length` of a row of a cache.
 struct Prefix {
     Cache cache;
@@ -61,7 +52,8 @@ cudaError_t launch_attention_shared(cudaStream_t s, const Cache& c, const Batch&
                                     int64_t out_stride, void* workspace);
 
 // The prefix's pass on tcgen05: whether it takes the types (q aligned to 16 bytes, like its tokens' distance),
-// its tiles of query rows, and the pass, which leaves the sums of every split as launch_cached_parts does.
+// its tiles of query rows, and the pass, which leaves the sums of every split in `part`,
+// [tokens][heads][splits][head_dim outputs, maximum (base 2), sum of weights].
 bool prefix_tc_takes(const Prefix& p, const AttnSpec& a);
 int prefix_tc_tiles(const Batch& b, const AttnSpec& a);
 cudaError_t launch_prefix_tc(cudaStream_t s, const Prefix& p, const Batch& b, const AttnSpec& a, const void* q,

@@ -129,7 +129,7 @@ class KvCache:
         _torch()
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.device = k.device
-        self._sizes = {}  # workspace bytes by what they depend on
+        self._sizes = {}  # workspace bytes, and the call's spec, by what they depend on
         u4 = str(k.dtype) == "torch.uint8"
         if u4 != (k_scale is not None) or u4 != (v_scale is not None):
             raise IllegalArgumentException("a 4-bit cache, and only that, has scales",
@@ -159,12 +159,13 @@ class KvCache:
         self._struct = s
         self._ref = ctypes.byref(s)
         self._shape = (self.storage, self.slots)   # what workspaces over it depend on
+        self._places = k.shape[:3]
 
-    def _keep(self, key, size):
+    def _keep(self, key, plan):
         if len(self._sizes) >= _KEPT:
             self._sizes.clear()
-        self._sizes[key] = size
-        return size
+        self._sizes[key] = plan
+        return plan
 
     @staticmethod
     def allocate(rows: int, kv_heads: int, slots: int, head_dim: int, storage: str = "u4",
@@ -322,16 +323,17 @@ def attention_shared(cache: KvCache, q, lengths, prefix: KvCache, prefix_length:
     q_stride = _packed(device, "q", q, None, cache.head_dim)
     out, out_stride = _out(device, q, out, stream)
     s = _sequences(device, q.shape[0], lengths, starts, rows)
-    a = _spec(q, cache.kv_heads, 0, 0, scale)
     prefix_row, prefix_length = _lib.int32(prefix_row), _lib.int32(prefix_length)
     lib = _lib.load()
-    key = (s.count, s.tokens, starts is None, a.heads, a.dtype, prefix._shape, prefix_length)
-    needed = cache._sizes.get(key)
-    if needed is None:
+    key = (s.count, s.tokens, starts is None, q.shape[1], q.dtype, scale, prefix._shape, prefix_length)
+    plan = cache._sizes.get(key)
+    if plan is None:
+        a = _spec(q, cache.kv_heads, 0, 0, scale)
         size = ctypes.c_int64(0)
         _raise(lib.bst_attention_shared_workspace(cache._ref, s, a, prefix._ref, prefix_row, prefix_length,
                                                   size))
-        needed = cache._keep(key, size.value)
+        plan = cache._keep(key, (size.value, a))
+    needed, a = plan
     pointer, room, workspace = _workspace(device, needed, workspace, stream)
     _raise(lib.bst_attention_shared(device.index, _stream(device, stream), cache._ref, s, a, prefix._ref,
                                     prefix_row, prefix_length, q.data_ptr(), q_stride, out.data_ptr(),
@@ -340,13 +342,14 @@ def attention_shared(cache: KvCache, q, lengths, prefix: KvCache, prefix_length:
 
 
 def _mass(device, name, t, cache):
-    """Checks masses [rows, kv_heads, slots] of a cache."""
-    _on(device, name, t)
+    """Checks masses [rows, kv_heads, slots] of a cache; their pointer."""
+    if t.device != device:
+        _on(device, name, t)
     if t.dtype is not _module.float32 or not t.is_contiguous():
         raise IllegalArgumentException(f"{name} must be contiguous float32", _lib.BST_INVALID)
-    if t.shape != (cache.rows, cache.kv_heads, cache.slots):
-        raise BasaltShapeException(f"{name} is {tuple(t.shape)}, expected "
-                                   f"{(cache.rows, cache.kv_heads, cache.slots)}", _lib.BST_SHAPE)
+    if t.shape != cache._places:
+        raise BasaltShapeException(f"{name} is {tuple(t.shape)}, expected {tuple(cache._places)}",
+                                   _lib.BST_SHAPE)
     return t.data_ptr()
 
 
@@ -364,14 +367,15 @@ def attention_weights(cache: KvCache, q, lengths, mass, previous=None, decay: fl
     q_stride = _packed(device, "q", q, None, cache.head_dim)
     out, out_stride = _out(device, q, out, stream)
     s = _sequences(device, q.shape[0], lengths, starts, rows)
-    a = _spec(q, cache.kv_heads, window, sinks, scale)
     lib = _lib.load()
-    key = (s.count, s.tokens, starts is None, a.heads, a.dtype, a.window, a.sinks, "weights")
-    needed = cache._sizes.get(key)
-    if needed is None:
+    key = (s.count, s.tokens, starts is None, q.shape[1], q.dtype, scale, window, sinks, "weights")
+    plan = cache._sizes.get(key)
+    if plan is None:
+        a = _spec(q, cache.kv_heads, window, sinks, scale)
         size = ctypes.c_int64(0)
         _raise(lib.bst_attention_weights_workspace(cache._ref, s, a, size))
-        needed = cache._keep(key, size.value)
+        plan = cache._keep(key, (size.value, a))
+    needed, a = plan
     pointer, room, workspace = _workspace(device, needed, workspace, stream)
     _raise(lib.bst_attention_weights(device.index, _stream(device, stream), cache._ref, s, a, q.data_ptr(),
                                      q_stride, out.data_ptr(), out_stride, before, decay, to, pointer, room))
