@@ -36,22 +36,20 @@ constexpr int kSoft = 256, kUnpack = 128;
 template <bool CODES>
 constexpr int kThreadsOf = kSoft + 32 + (CODES ? kUnpack : 32);
 
-template <int HD>
+template <int HD, bool CODES>
 struct PrefixLayout {
     static constexpr int kQuery = 128 * HD * 2;       // a tile of query rows
     static constexpr int kTile = kTcKeys * HD * 2;    // a tile of keys or values
-    static constexpr int kSlots = 8;
+    static constexpr int kSlots = CODES ? 6 : 8;
     static constexpr int kBars = 2 * kQuery + kSlots * kTile;
-    static constexpr int kFactors = kBars + 256;      // of rows, tiles of keys, tiles of values, warps
-    static constexpr int kRaw = kFactors + (kRows + 24) * 4;
-    // Codes and scales as the unpacking threads copy them: [stage][16-byte pieces][thread].
-    static constexpr int kStages = 4, kPieces = HD / 64 + 1;
-    static constexpr int end(bool codes) { return kRaw + (codes ? kStages * kPieces * kUnpack * 16 : 0); }
+    static constexpr int kFactors = kBars + 256;      // of rows, tiles of keys, tiles of values
+    static constexpr int kRaw = kFactors + (kRows + 16) * 4;
+    // Codes and scales as the unpacking lanes copy them: [warp][stage][16-byte pieces][lane].
+    static constexpr int kStages = 2, kPieces = HD / 16 + 4;
+    static constexpr int kEnd = kRaw + (CODES ? kUnpack * kStages * kPieces * 16 : 0);
     // More than half of an SM's shared memory: one CTA an SM, which owns all of TMEM.
-    static constexpr int smem(bool codes) {           // the base is aligned to 1024 bytes
-        return (end(codes) > 120 * 1024 ? end(codes) : 120 * 1024) + 1024;
-    }
-    static_assert(kSlots * kTile >= kRows * HD * 4, "outputs are staged in the ring");
+    static constexpr int kSmem = (kEnd > 120 * 1024 ? kEnd : 120 * 1024) + 1024;  // the base is aligned to 1024 bytes
+    static_assert(kBars >= kRows * HD * 4, "outputs are staged where queries and the ring are");
 };
 
 // The channels of one head of one key of a 4-bit cache, for rows that are added up plainly.
@@ -61,6 +59,31 @@ __device__ __forceinline__ float code_value(const unsigned char* codes, const __
     const int byte = codes[(h * groups + g) * 2 + (j >> 1)];
     return fmaf(static_cast<float>(j & 1 ? byte >> 4 : byte & 15), __bfloat162float(scales[2 * g]),
                 __bfloat162float(scales[2 * g + 1]));
+}
+
+// Two floats a register pair, and operations on both at once.
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void of_pair(uint64_t x, float* a, float* b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(*a), "=f"(*b) : "l"(x));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
 
 __device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
@@ -104,7 +127,7 @@ __global__ void __launch_bounds__(kThreadsOf<CODES>, 1)
 k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, Prefix prefix,
             Batch b, AttnSpec a, const __nv_bfloat16* __restrict__ q, int64_t q_stride, int tiles, int splits,
             float* __restrict__ part) {
-    using L = PrefixLayout<HD>;
+    using L = PrefixLayout<HD, CODES>;
     constexpr int kBlocks = HD / 64;     // 128-byte columns of a tile
     extern __shared__ unsigned char raw[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -138,11 +161,10 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
     float* const row_factor = reinterpret_cast<float*>(smem + L::kFactors);   // what a row was divided by,
     float* const key_factor = row_factor + kRows;                             // a tile of keys, [8],
     float* const value_factor = key_factor + 8;                               // and of values and weights, [8]
-    uint32_t* const warp_most = reinterpret_cast<uint32_t*>(value_factor + 8);  // [2][4]
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < L::kSlots; ++i) {
-            mbar_init(full + i, CODES ? kUnpack : 1);
+            mbar_init(full + i, CODES ? 32 : 1);
             mbar_init(empty + i, 1);
         }
         for (int i = 0; i < 4; ++i) {
@@ -246,105 +268,118 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
                 }
             }
         } else {
-            // Two threads a key: a chunk of 16 code bytes each, or two with 128 channels.
-            constexpr int G = HD / 32, kChunks = HD / 64;
-            const int tid = threadIdx.x - 9 * 32, key = tid & (kTcKeys - 1), part_of = tid / kTcKeys;
+            // Two warps take the keys' even and odd tiles, two the values'; a lane has two keys of a tile.
+            constexpr int G = HD / 32, kChunks = HD / 32;  // chunks of 16 code bytes of a key
+            const int u = warp - 9;
+            const bool keys = u < 2;
+            const char* const codes_at = static_cast<const char*>(keys ? prefix.cache.k : prefix.cache.v);
+            const char* const scales_at = static_cast<const char*>(keys ? prefix.cache.k_scale : prefix.cache.v_scale);
             const int64_t at = (static_cast<int64_t>(prefix.row) * a.kv_heads + kvh) * prefix.cache.slots;
-            const uint32_t mine = base + L::kRaw + tid * 16;
-            auto piece = [&](int i, int x) {
-                return mine + ((i % L::kStages) * L::kPieces + x) * (kUnpack * 16);
+            auto piece = [&](int stage, int x) {
+                return base + L::kRaw + (((u * L::kStages + stage) * L::kPieces + x) * 32 + lane) * 16;
             };
-            auto load = [&](int i) {
-                if (i < copies) {
-                    const int my_key = (t0 + copy_tile(i)) * kTcKeys + key;
-                    const bool keys = copy_of_keys(i), there = my_key < prefix.length;  // behind it: zeros
-                    const int64_t from = at + (there ? my_key : 0);
-                    const char* codes = static_cast<const char*>(keys ? prefix.cache.k : prefix.cache.v) +
-                                        from * (HD / 2) + part_of * kChunks * 16;
-                    const char* scale = static_cast<const char*>(keys ? prefix.cache.k_scale : prefix.cache.v_scale) +
-                                        from * (G * 4);
+            auto load = [&](int tile, int stage) {
+                if (tile < key_tiles) {
 #pragma unroll
-                    for (int x = 0; x < kChunks; ++x) cp_async<16>(piece(i, x), codes + 16 * x, there ? 16 : 0);
-                    cp_async<G * 4>(piece(i, kChunks), scale, there ? G * 4 : 0);
+                    for (int half = 0; half < 2; ++half) {
+                        const int key = (t0 + tile) * kTcKeys + 32 * half + lane;
+                        const bool there = key < prefix.length;  // zeros behind it
+                        const int64_t from = at + (there ? key : 0);
+#pragma unroll
+                        for (int x = 0; x < kChunks; ++x) {
+                            cp_async<16>(piece(stage, half * kChunks + x), codes_at + from * (HD / 2) + 16 * x, there ? 16 : 0);
+                        }
+                        cp_async<G * 4>(piece(stage, 2 * kChunks + half), scales_at + from * (G * 4), there ? G * 4 : 0);
+                        // The scales of the tile before, which the other warp unpacks.
+                        if (!keys && tile > 0) {
+                            cp_async<G * 4>(piece(stage, 2 * kChunks + 2 + half), scales_at + (at + key - kTcKeys) * (G * 4), G * 4);
+                        }
+                    }
                 }
                 asm volatile("cp.async.commit_group;" ::: "memory");
             };
-#pragma unroll
-            for (int i = 0; i < L::kStages - 1; ++i) load(i);
-            int values_below = -1000;  // values are below 2^this; what they are divided by goes with it
-            bool ok = true;
-            for (int i = 0; i < copies; ++i) {
-                asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 2) : "memory");
-                uint4 codes[kChunks];
-                uint32_t scale[G];
-#pragma unroll
-                for (int x = 0; x < kChunks; ++x) {
-                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                                 : "=r"(codes[x].x), "=r"(codes[x].y), "=r"(codes[x].z), "=r"(codes[x].w)
-                                 : "r"(piece(i, x)));
-                }
+            auto scale_words = [&](int stage, int x, uint32_t (&w)[G]) {
                 if constexpr (G == 4) {
                     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                                 : "=r"(scale[0]), "=r"(scale[1]), "=r"(scale[2]), "=r"(scale[3])
-                                 : "r"(piece(i, kChunks)));
+                                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(piece(stage, x)));
                 } else {
-                    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
-                                 : "=r"(scale[0]), "=r"(scale[1]) : "r"(piece(i, kChunks)));
+                    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(piece(stage, x)));
                 }
-                load(i + L::kStages - 1);  // into the stage before this one, which this thread alone has read
-                // The tile's largest is at most max |low| + 15 step (not of a NaN).
-                const int tile = copy_tile(i);
+            };
+            // The exponent above a tile's largest, which is at most max |low| + 15 step (not of a NaN).
+            auto exponent_of = [&](int stage, int x) {
                 uint32_t most = 0u;
 #pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    const float top = fmaf(15.0f, __uint_as_float(scale[g] << 16),
-                                           fabsf(__uint_as_float(scale[g] & 0xffff0000u)));
-                    most = max(most, top <= FLT_MAX ? __float_as_uint(top) : (isnan(top) ? 0u : 0x7f000000u));
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t w[G];
+                    scale_words(stage, x + half, w);
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {
+                        const float top = fmaf(15.0f, __uint_as_float(w[g] << 16), fabsf(__uint_as_float(w[g] & 0xffff0000u)));
+                        most = max(most, top <= FLT_MAX ? __float_as_uint(top) : (isnan(top) ? 0u : 0x7f000000u));
+                    }
                 }
-                most = __reduce_max_sync(kFull, most);
-                if (lane == 0) warp_most[(i & 1) * 4 + (warp - 9)] = most;
-                asm volatile("bar.sync 3, %0;" ::"n"(kUnpack) : "memory");
-                const uint32_t* const all_most = warp_most + (i & 1) * 4;
-                const int e = exponent_above(max(max(all_most[0], all_most[1]), max(all_most[2], all_most[3])));
-                float by;
-                if (copy_of_keys(i)) {
-                    by = power_of_two(-e);
-                    if (tid == 0) key_factor[tile & 7] = power_of_two(e);
-                } else {
+                return exponent_above(__reduce_max_sync(kFull, most));
+            };
+            int values_below = -1000;  // values are below 2^this; what they are divided by goes with it
+            load(u & 1, 0);
+            for (int tile = u & 1, stage = 0; tile < key_tiles; tile += 2, stage ^= 1) {
+                load(tile + 2, stage ^ 1);
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+                __syncwarp();
+                const int i = keys ? k_copy(tile) : v_copy(tile);
+                if (!keys && tile > 0) {
+                    const int e = exponent_of(stage, 2 * kChunks + 2);
                     if (e > values_below) values_below = e + 4;
-                    by = power_of_two(15 - values_below);
-                    // Weights are 2^7 too large.
-                    if (tid == 0) value_factor[tile & 7] = power_of_two(values_below - 22);
                 }
-                if (ok && i >= L::kSlots) {
-                    ok = mbar_wait(empty + i % L::kSlots, ((i / L::kSlots) - 1) & 1, status, 1, abort);
+                const int e = exponent_of(stage, 2 * kChunks);
+                if (!keys && e > values_below) values_below = e + 4;
+                const float by = power_of_two(keys ? -e : 15 - values_below);
+                if (i >= L::kSlots && !mbar_wait(empty + i % L::kSlots, ((i / L::kSlots) - 1) & 1, status, 1, abort)) break;
+                if (lane == 0) {
+                    if (keys) {
+                        key_factor[tile & 7] = power_of_two(e);
+                    } else {
+                        value_factor[tile & 7] = power_of_two(values_below - 22);  // weights are 2^7 too large
+                    }
                 }
-                if (!ok) continue;  // a wait that ran out ends no loop: the warps meet at the barrier above
-                unsigned char* const to = smem + 2 * L::kQuery + (i % L::kSlots) * L::kTile + key * 128;
+#pragma unroll 1
+                for (int half = 0; half < 2; ++half) {
+                    const int key = 32 * half + lane;
+                    unsigned char* const to = smem + 2 * L::kQuery + (i % L::kSlots) * L::kTile + key * 128;
+                    uint32_t scale[G], step[G / 2], low[G / 2];
+                    scale_words(stage, 2 * kChunks + half, scale);
 #pragma unroll
-                for (int g = 0; g < G; g += 2) {
-                    const uint32_t step = half2_of(__uint_as_float(scale[g] << 16) * by,
-                                                   __uint_as_float(scale[g + 1] << 16) * by);
-                    const uint32_t low = half2_of(__uint_as_float(scale[g] & 0xffff0000u) * by,
-                                                  __uint_as_float(scale[g + 1] & 0xffff0000u) * by);
+                    for (int g = 0; g < G; g += 2) {
+                        step[g / 2] = half2_of(__uint_as_float(scale[g] << 16) * by, __uint_as_float(scale[g + 1] << 16) * by);
+                        low[g / 2] = half2_of(__uint_as_float(scale[g] & 0xffff0000u) * by,
+                                              __uint_as_float(scale[g + 1] & 0xffff0000u) * by);
+                    }
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {  // eight channels of both groups
-                        // Words of a chunk: [halves of eight channels][pairs of groups], or, with two groups,
-                        // four halves.
-                        const uint4 c = codes[G == 4 ? x : 0];
-                        const uint32_t w0 = G == 4 ? (g ? c.y : c.x) : (x ? c.z : c.x);
-                        const uint32_t w1 = G == 4 ? (g ? c.w : c.z) : (x ? c.w : c.y);
-                        const int eighth = part_of * 2 + x;  // which eight of a group's 32
-                        uint4 one, two;
-                        unpack(w0, w1, step, low, &one, &two);
-                        unsigned char* const block = to + (g >> 1) * (kTcKeys * 128);
-                        *reinterpret_cast<uint4*>(block + ((eighth ^ (key & 7)) << 4)) = one;
-                        *reinterpret_cast<uint4*>(block + (((4 + eighth) ^ (key & 7)) << 4)) = two;
+                    for (int x = 0; x < kChunks; ++x) {
+                        // Words of a chunk: two halves of eight channels by pairs of groups (128 channels), or four
+                        // halves.
+                        uint32_t w[4];
+                        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                                     : "r"(piece(stage, half * kChunks + x)));
+#pragma unroll
+                        for (int y = 0; y < 2; ++y) {
+                            const int g = G == 4 ? y : 0;               // pair of groups
+                            const int eighth = G == 4 ? x : 2 * x + y;  // which eight of a group's 32 channels
+                            uint4 one, two;
+                            unpack(w[G == 4 ? y : 2 * y], w[G == 4 ? 2 + y : 2 * y + 1], step[g], low[g], &one, &two);
+                            unsigned char* const block = to + g * (kTcKeys * 128);
+                            *reinterpret_cast<uint4*>(block + ((eighth ^ (key & 7)) << 4)) = one;
+                            *reinterpret_cast<uint4*>(block + (((4 + eighth) ^ (key & 7)) << 4)) = two;
+                        }
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 mbar_arrive(full + i % L::kSlots);
+                __syncwarp();  // the stage has been read before it is loaded again
             }
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
         }
     } else if (warp == 8) {
         // The whole warp keeps time; one lane issues. Tiles are multiplied whole (what lies behind
@@ -435,55 +470,62 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
             }
             float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int x = 0; x < 64; ++x) m[x & 3] = fmaxf(m[x & 3], __uint_as_float(s[x >> 5][x & 31]));
-            const float most = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * by;
+            for (int x = 0; x < 64; x += 2) {
+                m[(x >> 1) & 3] = max3(m[(x >> 1) & 3], __uint_as_float(s[x >> 5][x & 31]), __uint_as_float(s[x >> 5][(x & 31) + 1]));
+            }
+            const float most = fmaxf(max3(m[0], m[1], m[2]), m[3]) * by;
             // The maximum that weights are taken against moves only when a row's grows by more than 2^8.
             const bool move = most > top + 8.0f || (top == -INFINITY && most > top);
-            float rescale = 1.0f;
-            if constexpr (CODES) {
-                // Values of this tile that are divided by more than those before: what was summed has to be, too.
-                // (The tile is there until these weights have been multiplied with it.)
-                ok = ok && await(v_copy(i), 6);
-                const float now = value_factor[i & 7];
-                rescale = values_by / now;
-                values_by = now;
-            }
-            if (__any_sync(kFull, move) || (CODES && i > 0 && rescale != 1.0f)) {
-                float keep = move ? (top == -INFINITY ? 0.0f : exp2_fast(top - most)) : 1.0f;
+            auto rescale = [&](float keep) {
+                ok = ok && mbar_wait(o_done + half, (i - 1) & 1, status, 8, abort);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                for (int c = 0; c < HD / 32; ++c) {
+                    uint32_t o[32];
+                    tmem_ld32(o_at + 32 * c, o);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * keep);
+                    tmem_st16(o_at + 32 * c, o);
+                    tmem_st16(o_at + 32 * c + 16, o + 16);
+                }
+            };
+            if (__any_sync(kFull, move)) {
+                const float keep = move ? (top == -INFINITY ? 0.0f : exp2_fast(top - most)) : 1.0f;
                 if (move) top = most;
                 total *= keep;
-                keep *= rescale;
-                if (i > 0) {
-                    ok = ok && mbar_wait(o_done + half, (i - 1) & 1, status, 8, abort);
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll
-                    for (int c = 0; c < HD / 32; ++c) {
-                        uint32_t o[32];
-                        tmem_ld32(o_at + 32 * c, o);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * keep);
-                        tmem_st16(o_at + 32 * c, o);
-                        tmem_st16(o_at + 32 * c + 16, o + 16);
-                    }
-                }
+                if (i > 0) rescale(keep);
             }
-            const float from = top == -INFINITY ? 0.0f : top;
-            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            // Weights for fp16 are 2^7 too large, and so is their sum.
+            const float from = (CODES ? 7.0f : 0.0f) - (top == -INFINITY ? 0.0f : top);
+            const uint64_t by2 = pair_of(by, by), from2 = pair_of(from, from);
+            uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 uint32_t p[16];
 #pragma unroll
                 for (int x = 0; x < 16; ++x) {
-                    const float e0 = exp2_fast(fmaf(__uint_as_float(s[c][2 * x]), by, -from));
-                    const float e1 = exp2_fast(fmaf(__uint_as_float(s[c][2 * x + 1]), by, -from));
-                    sum[(2 * x) & 3] += e0;
-                    sum[(2 * x + 1) & 3] += e1;
-                    p[x] = CODES ? half2_of(e0 * 128.0f, e1 * 128.0f) : pack2(e0, e1);
+                    const uint64_t y = fma2(pair_of(__uint_as_float(s[c][2 * x]), __uint_as_float(s[c][2 * x + 1])), by2, from2);
+                    float e0, e1;
+                    of_pair(y, &e0, &e1);
+                    e0 = exp2_fast(e0);
+                    e1 = exp2_fast(e1);
+                    sum[x & 1] = add2(sum[x & 1], pair_of(e0, e1));
+                    p[x] = CODES ? half2_of(e0, e1) : pack2(e0, e1);
                 }
                 tmem_st16(buffer + 16 * c, p);
             }
-            total += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            float sum0, sum1;
+            of_pair(add2(sum[0], sum[1]), &sum0, &sum1);
+            total += sum0 + sum1;
+            if constexpr (CODES) {
+                // Values of this tile that are divided by more than those before: what was summed has to be, too.
+                // (The tile is there until these weights have been multiplied with it.)
+                ok = ok && await(v_copy(i), 6);
+                const float now = value_factor[i & 7];
+                if (i > 0 && now != values_by) rescale(values_by / now);
+                values_by = now;
+            }
             tmem_st_wait();
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             mbar_arrive(p_full + 2 * half + (i & 1));
@@ -493,9 +535,9 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
             ok = ok && mbar_wait(o_last + half, 0, status, 9, abort);
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        // Both halves' products are done, so the ring may hold the rows, which are then written whole.
+        // Both halves' products are done, so queries and ring may give way to the rows, which are then written whole.
         asm volatile("bar.sync 1, %0;" ::"n"(kSoft) : "memory");
-        unsigned char* const rows_at = smem + 2 * L::kQuery;
+        unsigned char* const rows_at = smem;
         if (half < halves) {
 #pragma unroll
             for (int c = 0; c < HD / 32; ++c) {
@@ -517,7 +559,7 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
                 int head;
                 place(at, &token, &head);
                 float* const to = part + ((token * a.heads + head) * splits + split) * (HD + 2) + HD;
-                *reinterpret_cast<float2*>(to) = make_float2(top, total);
+                *reinterpret_cast<float2*>(to) = make_float2(top, CODES ? total * 0x1p-7f : total);
             }
         }
         __syncwarp();
@@ -598,7 +640,7 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
 template <int HD, bool CODES>
 cudaError_t run(cudaStream_t s, const Prefix& p, const Batch& b, const AttnSpec& a, const __nv_bfloat16* q,
                 int64_t q_stride, int tiles, int splits, float* part) {
-    using L = PrefixLayout<HD>;
+    using L = PrefixLayout<HD, CODES>;
     CUtensorMap k_map{}, v_map{};
     if constexpr (!CODES) {
         const int64_t head = static_cast<int64_t>(p.cache.slots) * HD * 2, row = head * a.kv_heads * p.row;
@@ -612,9 +654,9 @@ cudaError_t run(cudaStream_t s, const Prefix& p, const Batch& b, const AttnSpec&
         if (e) return e;
     }
     const cudaError_t e =
-        cudaFuncSetAttribute(k_prefix_tc<HD, CODES>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::smem(CODES));
+        cudaFuncSetAttribute(k_prefix_tc<HD, CODES>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
     if (e) return e;
-    k_prefix_tc<HD, CODES><<<tiles * a.kv_heads * splits, kThreadsOf<CODES>, L::smem(CODES), s>>>(
+    k_prefix_tc<HD, CODES><<<tiles * a.kv_heads * splits, kThreadsOf<CODES>, L::kSmem, s>>>(
         k_map, v_map, p, b, a, q, q_stride, tiles, splits, part);
     return cudaGetLastError();
 }

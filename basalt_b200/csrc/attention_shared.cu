@@ -68,14 +68,14 @@ size_t part_bytes(const Batch& b, const AttnSpec& a, int splits) {
     return static_cast<size_t>(b.tokens) * a.heads * splits * (a.head_dim + 2) * sizeof(float);
 }
 
-// A CTA a query; or, for at most 32 splits in all, a warp (8192 queries of 10 splits of 128 channels: 20 us
-// with a CTA each).
+// A CTA a query; or, for at most 32 splits in all, a warp for 32 channels of one.
 template <typename T, int HD, bool WARP>
 __global__ void __launch_bounds__(kThreads)
 k_shared_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out, int64_t out_stride,
               int own_splits, const float* __restrict__ own, int prefix_splits,
               const float* __restrict__ prefix) {
-    const uint32_t query = WARP ? blockIdx.x * kWarps + (threadIdx.x >> 5) : blockIdx.x;
+    const uint32_t unit = WARP ? blockIdx.x * kWarps + (threadIdx.x >> 5) : blockIdx.x;
+    const uint32_t query = WARP ? unit / (HD / 32) : unit;
     const int token = query / static_cast<uint32_t>(a.heads), head = query - static_cast<uint32_t>(token) * a.heads;
     int seq, first, n;
     if (token >= b.tokens || !find_sequence(b, token, &seq, &first, &n)) {
@@ -89,7 +89,7 @@ k_shared_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out, 
     auto at = [&](int s) { return s < use ? mine + s * (HD + 2) : common + (s - use) * (HD + 2); };
     T* const to = out + token * out_stride + head * HD;
     if constexpr (WARP) {
-        join_by_warp<T, HD>(use + prefix_splits, at, to);
+        join_by_warp<T, HD>(use + prefix_splits, at, to, unit % (HD / 32));
     } else {
         join_splits<2 * kMaxSplits, T, HD>(use + prefix_splits, at, to);
     }
@@ -141,7 +141,7 @@ cudaError_t launch_attention_shared(cudaStream_t s, const Cache& c, const Batch&
             const int64_t queries = static_cast<int64_t>(b.tokens) * a.heads;
             const bool warp = own_count + splits <= 32;
             return launch_pdl(warp ? k_shared_join<T, HD, true> : k_shared_join<T, HD, false>,
-                              dim3(static_cast<unsigned>(warp ? (queries + kWarps - 1) / kWarps : queries)),
+                              dim3(static_cast<unsigned>(warp ? (queries * (HD / 32) + kWarps - 1) / kWarps : queries)),
                               dim3(kThreads), 0, s, c, b, a, rows, static_cast<T*>(out), out_stride, own_count,
                               static_cast<const float*>(own), splits, static_cast<const float*>(prefix));
         });

@@ -13,7 +13,7 @@
 namespace bst {
 namespace {
 
-constexpr int kMassKeys = 8 * kThreads;   // keys of a CTA: eight a thread
+constexpr int kMassKeys = 4 * kThreads;   // keys of a CTA at a time: four next to one another a thread
 constexpr int kMassRows = 64;             // query rows whose maxima and sums are held at a time
 
 // Whether the batch's sequence `seq` is the first that names its row, and the next one that names the same.
@@ -52,9 +52,10 @@ template <typename T, int HD, bool WARP>
 __global__ void __launch_bounds__(kThreads)
 k_weights_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out, int64_t out_stride,
                int splits, const float* __restrict__ part, const float* __restrict__ scores, int64_t pitch,
-               const float* previous, float decay, float* mass, int joins) {
+               const float* previous, float decay, float* mass, int joins, int per) {
     if (blockIdx.x < joins) {
-        const uint32_t query = WARP ? blockIdx.x * kWarps + (threadIdx.x >> 5) : blockIdx.x;
+        const uint32_t unit = WARP ? blockIdx.x * kWarps + (threadIdx.x >> 5) : blockIdx.x;
+        const uint32_t query = WARP ? unit / (HD / 32) : unit;
         const int token = query / static_cast<uint32_t>(a.heads), head = query - static_cast<uint32_t>(token) * a.heads;
         int seq, first, n;
         if (token >= b.tokens || !find_sequence(b, token, &seq, &first, &n)) return;
@@ -64,131 +65,135 @@ k_weights_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out,
         auto at = [&](int s) { return from + s * (HD + 2); };
         T* const to = out + token * out_stride + head * HD;
         if constexpr (WARP) {
-            join_by_warp<T, HD>(use, at, to);
+            join_by_warp<T, HD>(use, at, to, unit % (HD / 32));
         } else {
             join_splits<kMaxSplits, T, HD>(use, at, to);
         }
         return;
     }
     __shared__ float tops[kMassRows], inverse[kMassRows];
-    // In 32 bits: the quotients of 64 took a third of all instructions.
-    const uint32_t chunks = (c.slots + kMassKeys - 1) / kMassKeys, place = blockIdx.x - joins;
-    const uint32_t of_head = place / chunks;
-    const int key0 = static_cast<int>(place - of_head * chunks) * kMassKeys;
-    int seq = of_head / static_cast<uint32_t>(a.kv_heads);
-    const int kvh = of_head - static_cast<uint32_t>(seq) * a.kv_heads;
-    const int row = b.rows ? __ldg(b.rows + seq) : seq;
-    if (row < 0 || row >= c.rows || !first_of_row(b, seq, row)) return;
+    // In 32 bits: the quotients of 64 took a third of all instructions. A CTA has `per` chunks of keys.
+    const uint32_t shares = (c.slots + per * kMassKeys - 1) / (per * kMassKeys), place = blockIdx.x - joins;
+    const uint32_t of_head = place / shares;
+    const int begin = static_cast<int>(place - of_head * shares) * per * kMassKeys;
+    const int first_seq = of_head / static_cast<uint32_t>(a.kv_heads);
+    const int kvh = of_head - static_cast<uint32_t>(first_seq) * a.kv_heads;
+    const int row = b.rows ? __ldg(b.rows + first_seq) : first_seq;
+    if (row < 0 || row >= c.rows || !first_of_row(b, first_seq, row)) return;
     const int group = a.heads / a.kv_heads, lane = threadIdx.x & 31;
-    constexpr int N = kMassKeys / kThreads, kBatch = 2;  // rows whose scores are under way together
-    const int my_key = key0 + threadIdx.x;
-    int offset[N];
+    constexpr int N = 4, kBatch = 4;  // rows whose scores are under way together
+    static_assert(N * kThreads == kMassKeys, "four keys a thread");
+    const int64_t base = (static_cast<int64_t>(row) * c.kv_heads + kvh) * c.slots;
+    int known = -1;  // the sequence whose maxima and sums are held, all of them
+    pdl_wait();
+    for (int chunk = 0; chunk < per; ++chunk) {
+        const int key0 = begin + chunk * kMassKeys;
+        if (key0 >= c.slots) break;
+        const int my_key = key0 + N * threadIdx.x, offset = min(my_key, static_cast<int>(pitch) - N);
+        float sum[N] = {}, old[N] = {};
+        if (decay != 0.0f) {  // without decay the old mass is not read: it may be anything
 #pragma unroll
-    for (int i = 0; i < N; ++i) offset[i] = min(my_key + i * kThreads, static_cast<int>(pitch) - 1);
-    float sum[N] = {};
-    int end = 0;
-    bool waited = false;
-    for (; seq < b.count; seq = next_of_row(b, seq, row)) {
-        const int length = max(0, __ldg(b.lengths + seq));
-        end = max(end, min(length, c.slots));
-        if (min(length, c.slots) <= key0) continue;
-        int first = seq, n = 1;
-        if (b.starts) {
-            first = max(0, __ldg(b.starts + seq));
-            n = max(0, min(__ldg(b.starts + seq + 1), b.tokens) - first);
+            for (int i = 0; i < N; ++i) old[i] = my_key + i < c.slots ? previous[base + my_key + i] : 0.0f;
         }
-        if (!waited) pdl_wait();
-        waited = true;
-        const int all = n * group;
-        // Scores of kBatch rows from r on; what lies beside the rows or what they see is read, not used.
-        int load_at = 0, load_head = 0;
-        auto load = [&](float (&x)[kBatch][N]) {
-#pragma unroll
-            for (int k = 0; k < kBatch; ++k) {
-                const float* from = scores + (static_cast<int64_t>(first + load_at) * a.heads + kvh * group + load_head) * pitch;
-#pragma unroll
-                for (int i = 0; i < N; ++i) x[k][i] = load_at < n ? __ldcs(from + offset[i]) : 0.0f;
-                if (++load_head == group) {
-                    load_head = 0;
-                    ++load_at;
-                }
+        int end = 0;
+        for (int seq = first_seq; seq < b.count; seq = next_of_row(b, seq, row)) {
+            const int length = max(0, __ldg(b.lengths + seq));
+            end = max(end, min(length, c.slots));
+            if (min(length, c.slots) <= key0) continue;
+            int first = seq, n = 1;
+            if (b.starts) {
+                first = max(0, __ldg(b.starts + seq));
+                n = max(0, min(__ldg(b.starts + seq + 1), b.tokens) - first);
             }
-        };
-        float x[kBatch][N];
-        load(x);
-        int at = 0, head_of = 0;
-        for (int r0 = 0; r0 < all; r0 += kMassRows) {
-            const int rows = min(kMassRows, all - r0);
-            // Maxima and sums of the rows: as many lanes a row as there are to spare.
-            int lanes = 32;
-            while (lanes > 1 && rows * lanes > kThreads) lanes >>= 1;
-            const int of_warp = 32 / lanes;  // a warp takes that many rows at a time
-            __syncthreads();
-            for (int r = threadIdx.x / lanes; r < (rows + of_warp - 1) / of_warp * of_warp; r += kThreads / lanes) {
-                float m = -INFINITY, total = 0.0f;
-                if (r < rows) {
-                    const int token = (r0 + r) / group, head = kvh * group + (r0 + r) - token * group;
-                    const int use = used_splits(c, a, tile_rows, splits, row, length, token, n, head);
-                    const float* from = part + (static_cast<int64_t>(first + token) * a.heads + head) * splits * (HD + 2) + HD;
-#pragma unroll 4
-                    for (int s = lane % lanes; s < use; s += lanes) {
-                        const float2 y = *reinterpret_cast<const float2*>(from + s * (HD + 2));
-                        add_split(&m, &total, y.x, y.y);
-                    }
-                }
-                for (int o = lanes / 2; o > 0; o >>= 1) {
-                    const float other = __shfl_xor_sync(kFull, m, o), others = __shfl_xor_sync(kFull, total, o);
-                    add_split(&m, &total, other, others);
-                }
-                if (r < rows && lane % lanes == 0) {
-                    tops[r] = m == -INFINITY ? 0.0f : m;
-                    inverse[r] = total == 0.0f ? 0.0f : 1.0f / total;
-                }
-            }
-            __syncthreads();
-            for (int r = 0; r < rows; r += kBatch) {  // 64 rows are whole batches
-                float next[kBatch][N];
-                load(next);
+            const int all = n * group;
+            // Scores of kBatch rows from r on; what lies beside the rows or what they see is read, not used.
+            int load_at = 0, load_head = 0;
+            const float* const rows_at = scores + (static_cast<int64_t>(first) * a.heads + kvh * group) * pitch + offset;
+            auto load = [&](float4 (&x)[kBatch]) {
 #pragma unroll
                 for (int k = 0; k < kBatch; ++k) {
-                    if (r + k < rows) {
-                        // A token outside the cache sees nothing.
-                        const int p = length - n + at;
-                        const float top = tops[r + k], by = inverse[r + k];
-                        if (a.window == 0 && key0 + kMassKeys - 1 <= p && p < c.slots) {
-#pragma unroll
-                            for (int i = 0; i < N; ++i) sum[i] = fmaf(exp2_fast(x[k][i] - top), by, sum[i]);
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < N; ++i) {
-                                const int key = my_key + i * kThreads;
-                                const bool seen = key <= p && p < c.slots && (a.window == 0 || p - key < a.window || key < a.sinks);
-                                const float more = fmaf(exp2_fast(x[k][i] - top), by, sum[i]);
-                                sum[i] = seen ? more : sum[i];
+                    x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (load_at < n) {
+                        x[k] = __ldcs(reinterpret_cast<const float4*>(rows_at + (static_cast<int64_t>(load_at) * a.heads + load_head) * pitch));
+                    }
+                    if (++load_head == group) {
+                        load_head = 0;
+                        ++load_at;
+                    }
+                }
+            };
+            float4 x[kBatch];
+            load(x);
+            int at = 0, head_of = 0;
+            for (int r0 = 0; r0 < all; r0 += kMassRows) {
+                const int rows = min(kMassRows, all - r0);
+                if (known != seq) {
+                    // Maxima and sums of the rows: as many lanes a row as there are to spare.
+                    int lanes = 32;
+                    while (lanes > 1 && rows * lanes > kThreads) lanes >>= 1;
+                    const int of_warp = 32 / lanes;  // a warp takes that many rows at a time
+                    __syncthreads();
+                    for (int r = threadIdx.x / lanes; r < (rows + of_warp - 1) / of_warp * of_warp; r += kThreads / lanes) {
+                        float m = -INFINITY, total = 0.0f;
+                        if (r < rows) {
+                            const int token = (r0 + r) / group, head = kvh * group + (r0 + r) - token * group;
+                            const int use = used_splits(c, a, tile_rows, splits, row, length, token, n, head);
+                            const float* from = part + (static_cast<int64_t>(first + token) * a.heads + head) * splits * (HD + 2) + HD;
+#pragma unroll 4
+                            for (int s = lane % lanes; s < use; s += lanes) {
+                                const float2 y = *reinterpret_cast<const float2*>(from + s * (HD + 2));
+                                add_split(&m, &total, y.x, y.y);
                             }
                         }
+                        for (int o = lanes / 2; o > 0; o >>= 1) {
+                            const float other = __shfl_xor_sync(kFull, m, o), others = __shfl_xor_sync(kFull, total, o);
+                            add_split(&m, &total, other, others);
+                        }
+                        if (r < rows && lane % lanes == 0) {
+                            tops[r] = m == -INFINITY ? 0.0f : m;
+                            inverse[r] = total == 0.0f ? 0.0f : 1.0f / total;
+                        }
                     }
-                    if (++head_of == group) {
-                        head_of = 0;
-                        ++at;
-                    }
+                    __syncthreads();
+                    known = all <= kMassRows ? seq : -1;
                 }
+                for (int r = 0; r < rows; r += kBatch) {  // kMassRows are whole batches
+                    float4 next[kBatch];
+                    load(next);
 #pragma unroll
-                for (int k = 0; k < kBatch; ++k) {
+                    for (int k = 0; k < kBatch; ++k) {
+                        if (r + k < rows) {
+                            // A token outside the cache sees nothing.
+                            const int p = length - n + at;
+                            const float top = tops[r + k], by = inverse[r + k];
+                            const float s[N] = {x[k].x, x[k].y, x[k].z, x[k].w};
+                            if (a.window == 0 && key0 + kMassKeys - 1 <= p && p < c.slots) {
 #pragma unroll
-                    for (int i = 0; i < N; ++i) x[k][i] = next[k][i];
+                                for (int i = 0; i < N; ++i) sum[i] = fmaf(exp2_fast(s[i] - top), by, sum[i]);
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < N; ++i) {
+                                    const int key = my_key + i;
+                                    const bool seen = key <= p && p < c.slots && (a.window == 0 || p - key < a.window || key < a.sinks);
+                                    const float more = fmaf(exp2_fast(s[i] - top), by, sum[i]);
+                                    sum[i] = seen ? more : sum[i];
+                                }
+                            }
+                        }
+                        if (++head_of == group) {
+                            head_of = 0;
+                            ++at;
+                        }
+                        x[k] = next[k];
+                    }
                 }
             }
         }
-    }
-    const int64_t base = (static_cast<int64_t>(row) * c.kv_heads + kvh) * c.slots;
-    if (!waited) pdl_wait();  // the stream's earlier writers of masses
+        if (end <= key0) break;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int key = key0 + threadIdx.x + i * kThreads;
-        if (key >= end) continue;
-        // Without decay the old mass is not read: it may be anything.
-        mass[base + key] = decay == 0.0f ? sum[i] : fmaf(decay, previous[base + key], sum[i]);
+        for (int i = 0; i < N; ++i) {
+            if (my_key + i < end) mass[base + my_key + i] = decay == 0.0f ? sum[i] : fmaf(decay, old[i], sum[i]);
+        }
     }
 }
 
@@ -225,8 +230,11 @@ cudaError_t launch_attention_weights(cudaStream_t s, const Cache& c, const Batch
     }
     const int64_t queries = static_cast<int64_t>(b.tokens) * a.heads;
     const bool warp = splits <= 32;
-    const int64_t joins = warp ? (queries + kWarps - 1) / kWarps : queries;
-    const int64_t blocks = joins + static_cast<int64_t>(b.count) * a.kv_heads * ((c.slots + kMassKeys - 1) / kMassKeys);
+    const int64_t joins = warp ? (queries * (a.head_dim / 32) + kWarps - 1) / kWarps : queries;
+    // Six CTAs an SM, each of whole chunks (one chunk a CTA: 35 instead of 20 us for 64 rows of up to 8192 keys).
+    const int64_t heads = static_cast<int64_t>(b.count) * a.kv_heads, chunks = (c.slots + kMassKeys - 1) / kMassKeys;
+    const int64_t per = std::min(chunks, (heads * chunks + 148 * 6 - 1) / (148 * 6));
+    const int64_t blocks = joins + heads * ((c.slots + per * kMassKeys - 1) / (per * kMassKeys));
     return by_dtype(a.dtype, [&](auto type) {
         using T = decltype(type);
         return by_head_dim(a.head_dim, [&](auto hd) {
@@ -235,7 +243,7 @@ cudaError_t launch_attention_weights(cudaStream_t s, const Cache& c, const Batch
                               dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, s, c, b, a, rows,
                               static_cast<T*>(out), out_stride, splits, static_cast<const float*>(part),
                               static_cast<const float*>(extra.scores), extra.pitch, previous, decay, mass,
-                              static_cast<int>(joins));
+                              static_cast<int>(joins), static_cast<int>(per));
         });
     });
 }

@@ -110,16 +110,20 @@ k_evict_choose(Cache c, Batch b, Eviction e, int held) {
     const int lo = min(rank * run * kChoose, length), hi = lo + min(run * kChoose, length - lo);
     const float* mass = e.mass + (static_cast<int64_t>(route.from) * c.kv_heads + head) * c.slots + lo;
     for (int i = threadIdx.x; i < 3 * kBins; i += kChoose) bins[0][i] = 0u;
-    if (run * kChoose <= held) {
-#pragma unroll 8
-        for (int i = threadIdx.x; i < hi - lo; i += kChoose) masses[i] = mass[i];
-        mass = masses;
-    }
     __syncthreads();
     // The keys that compete: [first, last), `need` of them stay.
     const int first = e.sinks, last = length - e.recent;
     uint32_t need = e.keep - e.sinks - e.recent;
     uint32_t border = 0xffffffffu;  // ordered masses above it stay, and `need` of those equal to it
+    // The upper bits are counted on the way into shared memory, or from where masses lie.
+    const bool fits = run * kChoose <= held;
+#pragma unroll 8
+    for (int i = threadIdx.x; i < hi - lo; i += kChoose) {
+        const float m = mass[i];
+        if (fits) masses[i] = m;
+        if (lo + i >= first && lo + i < last) atomicAdd(bins[0] + (ordered(m) >> 21), 1u);
+    }
+    if (fits) mass = masses;
     if (need > 0) {
         uint32_t known = 0, mask = 0;
 #pragma unroll
@@ -127,7 +131,7 @@ k_evict_choose(Cache c, Batch b, Eviction e, int held) {
             constexpr int kShift[3] = {21, 10, 0};
             const int shift = pass == 0 ? kShift[0] : (pass == 1 ? kShift[1] : kShift[2]);
             const uint32_t digit = pass == 2 ? 1023u : 2047u;
-            const int end = min(hi, last) - lo;
+            const int end = pass == 0 ? 0 : min(hi, last) - lo;
 #pragma unroll 4
             for (int i = max(lo, first) - lo + threadIdx.x; i < end; i += kChoose) {
                 const uint32_t u = ordered(mass[i]);
@@ -161,6 +165,7 @@ k_evict_choose(Cache c, Batch b, Eviction e, int held) {
         }
         border = known;
     }
+    __syncthreads();
     // This thread's keys above the border (or kept anyway) and at it, then where its places begin.
     const int mine = threadIdx.x * run, n = min(run, hi - lo - mine);
     uint32_t above = 0, equal = 0;
