@@ -53,6 +53,14 @@ struct Tile {
     int r0;              // the tile's first query row: row r is token r / group, head r % group
 };
 
+// Tensor-core tiles over a sequence's own row: query rows a tile; the keys that a tile whose last token stands at
+// `position` sees, [0, end); and of `splits` the ones that are worth it, 512 keys or more each.
+constexpr int kTcTileRows = 256;
+__device__ __forceinline__ int tc_end(int position, int row, const Cache& c) {
+    return row >= 0 && row < c.rows ? max(0, min(position + 1, c.slots)) : 0;
+}
+__device__ __forceinline__ int tc_useful(int end, int splits) { return max(1, min(splits, end / 512)); }
+
 // Tile number `index` of a batch whose sequences have n group rows each, tile_rows to a tile. Without
 // starts every sequence has the same number of tiles; with them the tiles before each sequence are
 // summed, 32 sequences at a time.

@@ -1583,6 +1583,7 @@ __device__ __forceinline__ int used_splits(const Cache& c, const AttnSpec& a, in
     const int group = a.heads / a.kv_heads;
     const int r0 = (at * group + head % group) / tile_rows * tile_rows;
     const int rows = min(tile_rows, n * group - r0);
+    if (tile_rows == kTcTileRows) return tc_useful(tc_end(length - n + (r0 + rows - 1) / group, row, c), splits);
     const int p_last = row >= 0 && row < c.rows ? length - n + (r0 + rows - 1) / group : -1;
     return useful_splits(Visible(length - n + r0 / group, p_last, c.slots, a.window, a.sinks).blocks, splits);
 }

@@ -10,13 +10,18 @@
 // whose rounding is of the size of bf16 outputs' own; maxima and sums are float32.
 //
 // A 4-bit prefix is unpacked on its way into shared memory by four warps in the copy's place, so that every key
-// is unpacked once for 256 rows. Keys, values, queries and weights become fp16, 11 bits, by one fused
-// multiply-add for two values, rounded once (bf16 ones took the error from 1.0 to 1.6 of the outputs' own
-// rounding). Powers of two keep them in fp16's range: one for each query row and each tile of keys, which the
-// scores' factor f takes back; and one for values, that of the largest so far with four bits to spare, by which
-// O is rescaled when a tile passes it (values 2^-25 of the largest so far begin to lose bits).
-// Codes and scales pass through a ring of their own in shared memory, three tiles ahead: with loads one tile
-// ahead the memory's latency was the bound (24 x 4 drafts of 32 heads behind 16 384 keys: 73 us).
+// is unpacked once for 256 rows. Scores are good to float32: a key's channel is (c - 8) step + middle, of which
+// the first, a code of 4 bits times a step of 8, is an fp16 number as it is; the middles, low + 8 step, are one more
+// step of the product, sixteen deep: of every group the query's sum and the middle, both in two fp16 terms, whose
+// smallest product is left out. Values and weights become fp16, 11 bits, values by one fused multiply-add for two
+// of them, rounded once (with bf16 ones the error was 1.6 times the outputs' own rounding instead of 1.0). Powers
+// of two keep all of it in fp16's range: one for each query row and each tile of keys, which the scores' factor f
+// takes back; and one for values, that of the largest so far with four bits to spare, by which O is rescaled when a
+// tile passes it (values 2^-25 of the largest so far begin to lose bits).
+// Each of the four warps unpacks whole tiles by itself, so that they wait for one another nowhere.
+//
+// The same kernel takes several tokens of each sequence over its own 4-bit row (OWN): then rows see the keys up to
+// their position, and every score may be kept.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -30,7 +35,7 @@
 namespace bst {
 namespace {
 
-constexpr int kRows = 256;
+constexpr int kRows = kTcTileRows;
 // Warps 0-3 and 4-7: a tile's rows, a thread each; 8: products; 9 on: copies, or four warps that unpack.
 constexpr int kSoft = 256, kUnpack = 128;
 template <bool CODES>
@@ -42,13 +47,16 @@ struct PrefixLayout {
     static constexpr int kTile = kTcKeys * HD * 2;    // a tile of keys or values
     static constexpr int kSlots = CODES ? 6 : 8;
     static constexpr int kBars = 2 * kQuery + kSlots * kTile;
-    static constexpr int kFactors = kBars + 256;      // of rows, tiles of keys, tiles of values
-    static constexpr int kRaw = kFactors + (kRows + 16) * 4;
+    static constexpr int kFactors = kBars + 256;      // of rows, tiles of keys, tiles of values (8 each, of 96)
+    // Middles: the queries' sums, [half][128 rows], and four tiles of keys, 32 bytes a row in the 32-byte swizzle.
+    static constexpr int kSums = kFactors + (kRows + 64) * 4, kMiddles = kSums + (CODES ? 2 * 128 * 32 : 0);
+    static constexpr int kRaw = kMiddles + (CODES ? 4 * kTcKeys * 32 : 0);
     // Codes and scales as the unpacking lanes copy them: [warp][stage][16-byte pieces][lane].
     static constexpr int kStages = 2, kPieces = HD / 16 + 4;
     static constexpr int kEnd = kRaw + (CODES ? kUnpack * kStages * kPieces * 16 : 0);
     // More than half of an SM's shared memory: one CTA an SM, which owns all of TMEM.
     static constexpr int kSmem = (kEnd > 120 * 1024 ? kEnd : 120 * 1024) + 1024;  // the base is aligned to 1024 bytes
+    static_assert(kSums % 256 == 0, "swizzled tiles start at whole atoms");
     static_assert(kBars >= kRows * HD * 4, "outputs are staged where queries and the ring are");
 };
 
@@ -106,15 +114,23 @@ __device__ __forceinline__ int exponent_above(uint32_t bits) {
     return max(min(static_cast<int>(bits >> 23) - 126, 126), -100);
 }
 
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
 // One word of codes (nibble j of the low half: channel j of one group; of the high half: of the next) and its
-// successor (the next four channels) as 16 bytes of fp16 for each of the two groups.
+// successor (the next four channels) as 16 bytes of fp16 for each of the two groups: c step + low, or, of keys,
+// (c - 8) step.
+template <bool KEYS>
 __device__ __forceinline__ void unpack(uint32_t a, uint32_t b, uint32_t step, uint32_t low, uint4* first,
                                        uint4* second) {
     uint32_t x[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {  // 1024 + c is exact, as is c
+    for (int j = 0; j < 8; ++j) {  // 1024 + c is exact, as are c and c - 8
         const uint32_t w = ((j < 4 ? a : b) >> (4 * (j & 3)) & 0x000f000fu) | 0x64006400u;
-        x[j] = fma_f16x2(sub_f16x2(w, 0x64006400u), step, low);
+        x[j] = KEYS ? mul_f16x2(sub_f16x2(w, 0x64086408u), step) : fma_f16x2(sub_f16x2(w, 0x64006400u), step, low);
     }
     *first = make_uint4(__byte_perm(x[0], x[1], 0x5410), __byte_perm(x[2], x[3], 0x5410),
                         __byte_perm(x[4], x[5], 0x5410), __byte_perm(x[6], x[7], 0x5410));
@@ -122,11 +138,21 @@ __device__ __forceinline__ void unpack(uint32_t a, uint32_t b, uint32_t step, ui
                          __byte_perm(x[4], x[5], 0x7632), __byte_perm(x[6], x[7], 0x7632));
 }
 
-template <int HD, bool CODES>
+// Tiles of 32-byte rows in the 32-byte swizzle: atoms of eight rows, 256 bytes apart.
+constexpr uint32_t kDesc32High = (256u >> 4) | (1u << 14) | (6u << 29);
+__device__ __forceinline__ int middle_at(int row, int chunk) { return row * 32 + ((chunk ^ ((row >> 2) & 1)) << 4); }
+// x in two fp16 terms, the first in the low half.
+__device__ __forceinline__ uint32_t two_halves(float x) {
+    const __half high = __float2half_rn(x);
+    return half2_of(__half2float(high), x - __half2float(high));
+}
+
+template <int HD, bool CODES, bool OWN>
 __global__ void __launch_bounds__(kThreadsOf<CODES>, 1)
 k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, Prefix prefix,
             Batch b, AttnSpec a, const __nv_bfloat16* __restrict__ q, int64_t q_stride, int tiles, int splits,
-            float* __restrict__ part) {
+            float* __restrict__ part, float* __restrict__ scores, int64_t pitch) {
+    static_assert(CODES || !OWN, "own rows are in 4 bits");
     using L = PrefixLayout<HD, CODES>;
     constexpr int kBlocks = HD / 64;     // 128-byte columns of a tile
     extern __shared__ unsigned char raw[];
@@ -134,15 +160,32 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
     const int group = a.heads / a.kv_heads;
     // The tiles of a share of a head's keys stand next to one another, so that they read it together.
     const int kvh = blockIdx.x / tiles % a.kv_heads, split = blockIdx.x / tiles / a.kv_heads;
-    int first, n;
-    pdl_trigger();  // the own keys' pass may fill what this one leaves free
-    if (!owned_tokens(b, &first, &n)) return;
-    const int64_t r0 = static_cast<int64_t>(blockIdx.x % tiles) * kRows;
-    if (r0 >= static_cast<int64_t>(n) * group) return;
+    int first, n, end;             // the tokens, and the keys that some row sees: those below `end`
+    int64_t r0;
+    int cache_row = prefix.row, position0 = 0;  // of OWN: the first token's position
+    if constexpr (OWN) {
+        Tile tile;
+        if (!find_tile(b, group, kRows, blockIdx.x % tiles, &tile)) return;
+        first = tile.first;
+        n = tile.n;
+        r0 = tile.r0;
+        cache_row = b.rows ? __ldg(b.rows + tile.seq) : tile.seq;
+        position0 = max(0, __ldg(b.lengths + tile.seq)) - n;
+        end = 0;
+    } else {
+        pdl_trigger();  // the own keys' pass may fill what this one leaves free
+        if (!owned_tokens(b, &first, &n)) return;
+        r0 = static_cast<int64_t>(blockIdx.x % tiles) * kRows;
+        if (r0 >= static_cast<int64_t>(n) * group) return;
+        end = prefix.length;
+    }
     const int rows = static_cast<int>(min(static_cast<int64_t>(kRows), static_cast<int64_t>(n) * group - r0));
-    const int all = (prefix.length + kTcKeys - 1) / kTcKeys;
-    const int t0 = static_cast<int>(static_cast<int64_t>(all) * split / splits);
-    const int key_tiles = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / splits) - t0;  // at least one
+    if constexpr (OWN) end = tc_end(position0 + static_cast<int>((r0 + rows - 1) / group), cache_row, prefix.cache);
+    const int all = (end + kTcKeys - 1) / kTcKeys, use = OWN ? tc_useful(end, splits) : splits;
+    if (split >= use) return;
+    const int t0 = static_cast<int>(static_cast<int64_t>(all) * split / use);
+    const int key_tiles = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / use) - t0;
+    const int sees_all = OWN ? position0 + static_cast<int>(r0 / group) : end - 1;  // keys up to it: every row
     const int halves = rows > 128 ? 2 : 1;
 
     const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
@@ -157,7 +200,7 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
     // the next, when a warp that was held up comes to wait for that.)
     uint64_t* const o_last = o_done + 2;
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(o_last + 2);
-    int* const status = reinterpret_cast<int*>(tmem_slot + 1);  // [0] error code, [1] abort
+    int* const status = reinterpret_cast<int*>(tmem_slot + 1);  // [0] error code, [1] abort, [2] redo
     float* const row_factor = reinterpret_cast<float*>(smem + L::kFactors);   // what a row was divided by,
     float* const key_factor = row_factor + kRows;                             // a tile of keys, [8],
     float* const value_factor = key_factor + 8;                               // and of values and weights, [8]
@@ -172,14 +215,8 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
             mbar_init(p_full + i, kSoft / 2);
         }
         for (int i = 0; i < 4; ++i) mbar_init(o_done + i, 1);
-        status[0] = status[1] = 0;
+        status[0] = status[1] = status[2] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    if (warp == 8) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                         smem_u32(tmem_slot)),
-                     "r"(512));
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     // Token and head of the CTA's query row `at`: the quotient of two small numbers, in float.
     const int token0 = static_cast<int>(r0 / group), r_first = static_cast<int>(r0 - static_cast<int64_t>(token0) * group);
@@ -189,6 +226,22 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
         *token = static_cast<int64_t>(first) + token0 + x;
         *head = kvh * group + r_first + at - x * group;
     };
+    if (OWN && key_tiles == 0) {  // nobody sees a key
+        for (int x = threadIdx.x; x < rows * (HD + 2); x += kThreadsOf<CODES>) {
+            int64_t token;
+            int head;
+            place(x / (HD + 2), &token, &head);
+            const int ch = x % (HD + 2);
+            part[((token * a.heads + head) * splits + split) * (HD + 2) + ch] = ch == HD ? -INFINITY : 0.0f;
+        }
+        return;
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         smem_u32(tmem_slot)),
+                     "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
     __syncthreads();  // the barriers are there: copies may start
     // The tiles in the order in which they are used: K0 K1 V0 K2 V1 K3 ... V(n-1).
     const int copies = 2 * key_tiles;
@@ -249,6 +302,28 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
                 }
                 // A query that is not finite makes every score NaN.
                 if (c == 0) row_factor[at] = most >= 0x7f800000u ? NAN : power_of_two(e) * 0x1p-8f;
+                // The sums of its groups: high terms, low ones, high ones again, zeros (four groups' places each).
+                float sum = 0.0f;
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    const __half2 h = *reinterpret_cast<const __half2*>(&w[y]);
+                    sum += __low2float(h) + __high2float(h);
+                }
+                sum += __shfl_xor_sync(kFull, sum, 1);
+                sum += __shfl_xor_sync(kFull, sum, 2);
+                if ((c & 3) == 0) {
+                    constexpr int kSpare = 4 / (HD / 32);  // places a group fills, the others with zeros
+                    const uint32_t terms = two_halves(sum);
+                    unsigned char* const to = smem + L::kSums + (at >> 7) * (128 * 32);
+#pragma unroll
+                    for (int y = 0; y < kSpare; ++y) {
+                        const int g = (c >> 2) + y * (HD / 32);
+                        *reinterpret_cast<uint16_t*>(to + middle_at(r, 0) + 2 * g) = y == 0 ? terms & 0xffffu : 0u;
+                        *reinterpret_cast<uint16_t*>(to + middle_at(r, 0) + 8 + 2 * g) = y == 0 ? terms >> 16 : 0u;
+                        *reinterpret_cast<uint16_t*>(to + middle_at(r, 1) + 2 * g) = y == 0 ? terms & 0xffffu : 0u;
+                        *reinterpret_cast<uint16_t*>(to + middle_at(r, 1) + 8 + 2 * g) = 0u;
+                    }
+                }
             }
             *reinterpret_cast<uint4*>(smem + (at >> 7) * L::kQuery + r * 128 + (c >> 3) * 16384 +
                                       (((c & 7) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -274,7 +349,7 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
             const bool keys = u < 2;
             const char* const codes_at = static_cast<const char*>(keys ? prefix.cache.k : prefix.cache.v);
             const char* const scales_at = static_cast<const char*>(keys ? prefix.cache.k_scale : prefix.cache.v_scale);
-            const int64_t at = (static_cast<int64_t>(prefix.row) * a.kv_heads + kvh) * prefix.cache.slots;
+            const int64_t at = (static_cast<int64_t>(cache_row) * a.kv_heads + kvh) * prefix.cache.slots;
             auto piece = [&](int stage, int x) {
                 return base + L::kRaw + (((u * L::kStages + stage) * L::kPieces + x) * 32 + lane) * 16;
             };
@@ -283,7 +358,7 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         const int key = (t0 + tile) * kTcKeys + 32 * half + lane;
-                        const bool there = key < prefix.length;  // zeros behind it
+                        const bool there = key < end;  // zeros behind it
                         const int64_t from = at + (there ? key : 0);
 #pragma unroll
                         for (int x = 0; x < kChunks; ++x) {
@@ -349,30 +424,63 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
                     unsigned char* const to = smem + 2 * L::kQuery + (i % L::kSlots) * L::kTile + key * 128;
                     uint32_t scale[G], step[G / 2], low[G / 2];
                     scale_words(stage, 2 * kChunks + half, scale);
+                    if (OWN && !keys && (t0 + tile) * kTcKeys + key > sees_all) {
+                        // Zero times a NaN is one: rows that do not see it must not get it, the others have to.
+                        bool bad = false;
+#pragma unroll
+                        for (int g = 0; g < G; ++g) bad |= (scale[g] & 0x7f80u) == 0x7f80u || (scale[g] & 0x7f800000u) == 0x7f800000u;
+                        if (bad) {
+                            status[2] = 1;
+#pragma unroll
+                            for (int g = 0; g < G; ++g) scale[g] = 0u;
+                        }
+                    }
 #pragma unroll
                     for (int g = 0; g < G; g += 2) {
                         step[g / 2] = half2_of(__uint_as_float(scale[g] << 16) * by, __uint_as_float(scale[g + 1] << 16) * by);
                         low[g / 2] = half2_of(__uint_as_float(scale[g] & 0xffff0000u) * by,
                                               __uint_as_float(scale[g + 1] & 0xffff0000u) * by);
                     }
+                    if (keys) {
+                        // Middles beside the queries' sums: high terms twice, low ones, zeros.
+                        uint32_t terms[4] = {};
 #pragma unroll
-                    for (int x = 0; x < kChunks; ++x) {
-                        // Words of a chunk: two halves of eight channels by pairs of groups (128 channels), or four
-                        // halves.
-                        uint32_t w[4];
-                        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                                     : "r"(piece(stage, half * kChunks + x)));
-#pragma unroll
-                        for (int y = 0; y < 2; ++y) {
-                            const int g = G == 4 ? y : 0;               // pair of groups
-                            const int eighth = G == 4 ? x : 2 * x + y;  // which eight of a group's 32 channels
-                            uint4 one, two;
-                            unpack(w[G == 4 ? y : 2 * y], w[G == 4 ? 2 + y : 2 * y + 1], step[g], low[g], &one, &two);
-                            unsigned char* const block = to + g * (kTcKeys * 128);
-                            *reinterpret_cast<uint4*>(block + ((eighth ^ (key & 7)) << 4)) = one;
-                            *reinterpret_cast<uint4*>(block + (((4 + eighth) ^ (key & 7)) << 4)) = two;
+                        for (int g = 0; g < G; ++g) {
+                            terms[g] = two_halves(fmaf(8.0f, __uint_as_float(scale[g] << 16), __uint_as_float(scale[g] & 0xffff0000u)) * by);
                         }
+                        unsigned char* const middle = smem + L::kMiddles + (tile & 3) * (kTcKeys * 32);
+                        const uint32_t h0 = __byte_perm(terms[0], terms[1], 0x5410), h1 = __byte_perm(terms[2], terms[3], 0x5410);
+                        *reinterpret_cast<uint4*>(middle + middle_at(key, 0)) = make_uint4(h0, h1, h0, h1);
+                        *reinterpret_cast<uint4*>(middle + middle_at(key, 1)) =
+                            make_uint4(__byte_perm(terms[0], terms[1], 0x7632), __byte_perm(terms[2], terms[3], 0x7632), 0u, 0u);
+                    }
+                    // A loop that is not unrolled: all warps together run at the rate at which instructions arrive.
+                    auto unpack_all = [&](auto of_keys) {
+                        constexpr bool KEYS = decltype(of_keys)::value;
+#pragma unroll 1
+                        for (int x = 0; x < kChunks; ++x) {
+                            // Words of a chunk: two halves of eight channels by pairs of groups (128 channels), or
+                            // four halves.
+                            uint32_t w[4];
+                            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                                         : "r"(piece(stage, half * kChunks + x)));
+#pragma unroll
+                            for (int y = 0; y < 2; ++y) {
+                                const int g = G == 4 ? y : 0;               // pair of groups
+                                const int eighth = G == 4 ? x : 2 * x + y;  // which eight of a group's 32 channels
+                                uint4 one, two;
+                                unpack<KEYS>(w[G == 4 ? y : 2 * y], w[G == 4 ? 2 + y : 2 * y + 1], step[g], low[g], &one, &two);
+                                unsigned char* const block = to + g * (kTcKeys * 128);
+                                *reinterpret_cast<uint4*>(block + ((eighth ^ (key & 7)) << 4)) = one;
+                                *reinterpret_cast<uint4*>(block + (((4 + eighth) ^ (key & 7)) << 4)) = two;
+                            }
+                        }
+                    };
+                    if (keys) {
+                        unpack_all(std::true_type());
+                    } else {
+                        unpack_all(std::false_type());
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -396,6 +504,10 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
             for (int k = 0; k < HD / 16; ++k) {
                 tc_mma_ss(d, qa + (k >> 2) * (16384 >> 4) + (k & 3) * 2,
                           ka + (k >> 2) * (kTcKeys * 128 >> 4) + (k & 3) * 2, kDescHigh, s_idesc, k > 0);
+            }
+            if constexpr (CODES) {  // the middles
+                tc_mma_ss(d, desc_k(base + L::kSums + half * (128 * 32)), desc_k(base + L::kMiddles + (i & 3) * (kTcKeys * 32)),
+                          kDesc32High, s_idesc, true);
             }
             mma_commit(s_full + 2 * half + (i & 1));
         };
@@ -448,6 +560,17 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
         // A score's factor to base 2. It stays above zero: the mask's -infinity is multiplied by it.
         const float scale = fabsf(a.scale) * kLog2e * (CODES ? row_factor[at] : 1.0f);
         float top = -INFINITY, total = 0.0f, values_by = 1.0f;
+        // Keys that the row sees, and where its scores go.
+        int sees = end;
+        float* kept = nullptr;
+        if constexpr (OWN) {
+            int64_t token;
+            int head;
+            place(at, &token, &head);
+            const int position = position0 + static_cast<int>(token - first);
+            sees = at < rows && position < prefix.cache.slots ? position + 1 : 0;
+            if (at < rows) kept = scores + (token * a.heads + head) * pitch;
+        }
         // A wait that runs out ends no loop here: the tile's threads meet at a barrier behind it, and
         // what they write then is computed again.
         bool ok = true;
@@ -461,11 +584,23 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
             float by = CODES ? scale * key_factor[i & 7] : scale;
             by = by < FLT_MIN ? FLT_MIN : by;
             tmem_ld_wait();
-            const int left = prefix.length - (t0 + i) * kTcKeys;  // keys of the tile, or more
+            const int left = sees - (t0 + i) * kTcKeys;  // keys of the tile, or more
             if (left < kTcKeys) {
 #pragma unroll
                 for (int x = 0; x < 64; ++x) {
                     if (x >= left) s[x >> 5][x & 31] = 0xff800000u;
+                }
+            }
+            if constexpr (OWN) {
+                float* const to = kept + (t0 + i) * kTcKeys;
+                const int64_t room = pitch - static_cast<int64_t>(t0 + i) * kTcKeys;  // whole blocks of 16
+#pragma unroll
+                for (int x = 0; x < 64; x += 4) {
+                    if (kept && x < room) {
+                        const uint32_t* const y = &s[x >> 5][x & 31];
+                        *reinterpret_cast<float4*>(to + x) = make_float4(__uint_as_float(y[0]) * by, __uint_as_float(y[1]) * by,
+                                                                         __uint_as_float(y[2]) * by, __uint_as_float(y[3]) * by);
+                    }
                 }
             }
             float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -581,8 +716,8 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    const bool again = status[0] != 0;
-    if (again && threadIdx.x == 0) {
+    const bool again = status[0] != 0 || status[2] != 0;
+    if (status[0] != 0 && threadIdx.x == 0) {
         // A wait ran out: let the copies that were issued land before the memory goes away.
         const uint64_t start = global_ns();
         while (global_ns() - start < 2000000ull) {
@@ -595,7 +730,7 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
     if (!again) return;
     // Its rows once more, plainly, a warp a row and a key at a time: slow, but right.
     constexpr int C = HD / 32;
-    const int64_t keys_at = (static_cast<int64_t>(prefix.row) * a.kv_heads + kvh) * prefix.cache.slots;
+    const int64_t keys_at = (static_cast<int64_t>(cache_row) * a.kv_heads + kvh) * prefix.cache.slots;
     for (int r = warp; r < rows; r += kThreadsOf<CODES> / 32) {
         int64_t token;
         int head;
@@ -603,8 +738,12 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
         float value[C] = {}, x[C], top = -INFINITY, total = 0.0f;
 #pragma unroll
         for (int i = 0; i < C; ++i) x[i] = __bfloat162float(q[token * q_stride + head * HD + lane + 32 * i]);
-        const int end = min(prefix.length, (t0 + key_tiles) * kTcKeys);
-        for (int key = t0 * kTcKeys; key < end; ++key) {
+        int stop = min(end, (t0 + key_tiles) * kTcKeys);
+        if constexpr (OWN) {
+            const int position = position0 + static_cast<int>(token - first);
+            stop = position < prefix.cache.slots ? min(stop, position + 1) : 0;
+        }
+        for (int key = t0 * kTcKeys; key < stop; ++key) {
             auto read = [&](const void* values, const void* scales, int channel) {
                 if constexpr (CODES) {
                     return code_value(static_cast<const unsigned char*>(values) + (keys_at + key) * (HD / 2),
@@ -617,6 +756,7 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
 #pragma unroll
             for (int i = 0; i < C; ++i) s = fmaf(x[i], read(prefix.cache.k, prefix.cache.k_scale, lane + 32 * i), s);
             s = warp_sum(s) * a.scale * kLog2e;
+            if (OWN && lane == 0) scores[(token * a.heads + head) * pitch + key] = s;
             const float up = fmaxf(top, s), keep = top == -INFINITY ? 0.0f : exp2f(top - up);
             const float p = s == -INFINITY ? 0.0f : exp2f(s - up);
             top = up;
@@ -637,9 +777,9 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
     }
 }
 
-template <int HD, bool CODES>
+template <int HD, bool CODES, bool OWN>
 cudaError_t run(cudaStream_t s, const Prefix& p, const Batch& b, const AttnSpec& a, const __nv_bfloat16* q,
-                int64_t q_stride, int tiles, int splits, float* part) {
+                int64_t q_stride, int tiles, int splits, float* part, float* scores, int64_t pitch) {
     using L = PrefixLayout<HD, CODES>;
     CUtensorMap k_map{}, v_map{};
     if constexpr (!CODES) {
@@ -653,11 +793,11 @@ cudaError_t run(cudaStream_t s, const Prefix& p, const Batch& b, const AttnSpec&
         }
         if (e) return e;
     }
-    const cudaError_t e =
-        cudaFuncSetAttribute(k_prefix_tc<HD, CODES>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
+    const auto kernel = k_prefix_tc<HD, CODES, OWN>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
     if (e) return e;
-    k_prefix_tc<HD, CODES><<<tiles * a.kv_heads * splits, kThreadsOf<CODES>, L::kSmem, s>>>(
-        k_map, v_map, p, b, a, q, q_stride, tiles, splits, part);
+    kernel<<<tiles * a.kv_heads * splits, kThreadsOf<CODES>, L::kSmem, s>>>(k_map, v_map, p, b, a, q, q_stride, tiles,
+                                                                          splits, part, scores, pitch);
     return cudaGetLastError();
 }
 
@@ -676,12 +816,27 @@ cudaError_t launch_prefix_tc(cudaStream_t s, const Prefix& p, const Batch& b, co
                              int64_t q_stride, int tiles, int splits, float* part) {
     const __nv_bfloat16* const q = static_cast<const __nv_bfloat16*>(q_);
     const bool codes = p.cache.storage == BST_DTYPE_U4;
-    if (a.head_dim == 128) {
-        return codes ? run<128, true>(s, p, b, a, q, q_stride, tiles, splits, part)
-                     : run<128, false>(s, p, b, a, q, q_stride, tiles, splits, part);
-    }
-    return codes ? run<64, true>(s, p, b, a, q, q_stride, tiles, splits, part)
-                 : run<64, false>(s, p, b, a, q, q_stride, tiles, splits, part);
+    auto go = [&](auto hd) {
+        constexpr int HD = decltype(hd)::value;
+        return codes ? run<HD, true, false>(s, p, b, a, q, q_stride, tiles, splits, part, nullptr, 0)
+                     : run<HD, false, false>(s, p, b, a, q, q_stride, tiles, splits, part, nullptr, 0);
+    };
+    return a.head_dim == 128 ? go(std::integral_constant<int, 128>()) : go(std::integral_constant<int, 64>());
+}
+
+bool own_tc_takes(const Cache& c, const Batch& b, const AttnSpec& a) {
+    return c.storage == BST_DTYPE_U4 && a.dtype == BST_DTYPE_BF16 && a.head_dim >= 64 && a.scale != 0.0f &&
+           a.window == 0 && b.starts;
+}
+
+cudaError_t launch_own_tc(cudaStream_t s, const Cache& c, const Batch& b, const AttnSpec& a, const void* q_,
+                          int64_t q_stride, int splits, float* part, float* scores, int64_t pitch) {
+    const __nv_bfloat16* const q = static_cast<const __nv_bfloat16*>(q_);
+    Prefix p;
+    p.cache = c;
+    const int tiles = tile_bound(b, a, kRows);
+    return a.head_dim == 128 ? run<128, true, true>(s, p, b, a, q, q_stride, tiles, splits, part, scores, pitch)
+                             : run<64, true, true>(s, p, b, a, q, q_stride, tiles, splits, part, scores, pitch);
 }
 
 }  // namespace bst

@@ -54,14 +54,10 @@ bool large(const Batch& b, const AttnSpec& a, const Prefix& p) {
     return prefix_tc_takes(p, a) && static_cast<int64_t>(b.tokens) * (a.heads / a.kv_heads) >= kLargeRows;
 }
 
-// Splits of the own keys. They are joined anyway, so that rows of uneven lengths may be split where they fill
-// the card once but not evenly: four waves (64 rows of 20 to 1000 keys: 33 us in 1.7 waves without splits).
+// Splits of the own keys: no more than fill the card (spreading 64 rows of 20 to 1000 keys over four waves took
+// 64 us where this takes 62, 24 x 4 drafts 93 instead of 88).
 int own_splits(const Cache& c, const Batch& b, const AttnSpec& a) {
-    const int per_sm = plain_query(c, b, a) ? 4 : one_query(c, b, a) ? kOneCtas : ctas_per_sm(c);
-    const int64_t units = static_cast<int64_t>(tile_bound(b, a, rows_of_tile(b, a))) * a.kv_heads;
-    const int64_t waves = 4 * 148 * per_sm / std::max<int64_t>(1, units);
-    const int64_t most = std::min<int64_t>(c.slots / 128, 16);
-    return std::max(split_count(c, b, a, per_sm), static_cast<int>(std::min(waves, most)));
+    return split_count(c, b, a, plain_query(c, b, a) ? 4 : 0);
 }
 
 size_t part_bytes(const Batch& b, const AttnSpec& a, int splits) {

@@ -197,7 +197,19 @@ k_weights_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out,
     }
 }
 
-int weights_splits(const Cache& c, const Batch& b, const AttnSpec& a) {
+// Several tokens of each sequence on tcgen05, from kLargeRows query rows a sequence and key head on.
+constexpr int kLargeRows = 24;
+bool large(const Cache& c, const Batch& b, const AttnSpec& a) {
+    return own_tc_takes(c, b, a) && static_cast<int64_t>(b.tokens) * (a.heads / a.kv_heads) >= static_cast<int64_t>(b.count) * kLargeRows;
+}
+
+// Four waves of CTAs there, since lengths differ and are not known here.
+int large_splits(const Cache& c, const Batch& b, const AttnSpec& a) {
+    const int64_t units = static_cast<int64_t>(tile_bound(b, a, kTcTileRows)) * a.kv_heads;
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({4 * 148 / std::max<int64_t>(1, units), c.slots / 512, 32})));
+}
+
+int small_splits(const Cache& c, const Batch& b, const AttnSpec& a) {
     return split_count(c, b, a, plain_query(c, b, a) ? 4 : 0);
 }
 
@@ -210,7 +222,8 @@ size_t score_bytes(const Cache& c, const Batch& b, const AttnSpec& a) {
 }  // namespace
 
 size_t attention_weights_workspace(const Cache& c, const Batch& b, const AttnSpec& a) {
-    const size_t query = static_cast<size_t>(weights_splits(c, b, a)) * (a.head_dim + 2) * sizeof(float);
+    const int splits = std::max(small_splits(c, b, a), large(c, b, a) ? large_splits(c, b, a) : 0);
+    const size_t query = static_cast<size_t>(splits) * (a.head_dim + 2) * sizeof(float);
     return score_bytes(c, b, a) + static_cast<size_t>(b.tokens) * a.heads * query;
 }
 
@@ -218,14 +231,16 @@ cudaError_t launch_attention_weights(cudaStream_t s, const Cache& c, const Batch
                                      const void* q, int64_t q_stride, void* out, int64_t out_stride,
                                      const float* previous, float decay, float* mass, void* workspace) {
     if (b.count < 1) return cudaSuccess;
-    const int splits = weights_splits(c, b, a), rows = rows_of_tile(b, a);
+    const bool tc = b.tokens > 0 && large(c, b, a) && reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_stride % 8 == 0;
+    const int splits = tc ? large_splits(c, b, a) : small_splits(c, b, a), rows = tc ? kTcTileRows : rows_of_tile(b, a);
     Extra extra;
     extra.scores = static_cast<float*>(workspace);
     extra.pitch = pitch_of(c);
     float* const part = extra.scores + score_bytes(c, b, a) / sizeof(float);
     if (b.tokens > 0) {
-        const cudaError_t e = run_cached<kScores>(s, c, b, a, q, q_stride, nullptr, 0, tile_bound(b, a, rows),
-                                                  rows, splits, part, extra);
+        const cudaError_t e = tc ? launch_own_tc(s, c, b, a, q, q_stride, splits, part, extra.scores, extra.pitch)
+                                 : run_cached<kScores>(s, c, b, a, q, q_stride, nullptr, 0, tile_bound(b, a, rows),
+                                                       rows, splits, part, extra);
         if (e) return e;
     }
     const int64_t queries = static_cast<int64_t>(b.tokens) * a.heads;

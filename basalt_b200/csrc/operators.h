@@ -59,6 +59,12 @@ int prefix_tc_tiles(const Batch& b, const AttnSpec& a);
 cudaError_t launch_prefix_tc(cudaStream_t s, const Prefix& p, const Batch& b, const AttnSpec& a, const void* q,
                              int64_t q_stride, int tiles, int splits, float* part);
 
+// The same kernel for several tokens of each sequence over its own 4-bit row without a window, which keeps every
+// score (scores[token][head][pitch], base 2). Tiles of kTcTileRows query rows, splits as tc_useful has them.
+bool own_tc_takes(const Cache& c, const Batch& b, const AttnSpec& a);
+cudaError_t launch_own_tc(cudaStream_t s, const Cache& c, const Batch& b, const AttnSpec& a, const void* q,
+                          int64_t q_stride, int splits, float* part, float* scores, int64_t pitch);
+
 size_t attention_weights_workspace(const Cache& c, const Batch& b, const AttnSpec& a);
 cudaError_t launch_attention_weights(cudaStream_t s, const Cache& c, const Batch& b, const AttnSpec& a,
                                      const void* q, int64_t q_stride, void* out, int64_t out_stride,

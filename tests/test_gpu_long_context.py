@@ -308,6 +308,41 @@ def test_weights_of_several_tokens(ops, dtype, heads, kv_heads):
                       sinks=5, decay=0.9)
 
 
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 8, 2), (128, 16, 2), (64, 3, 1), (128, 8, 1)])
+def test_weights_of_many_tokens(ops, dim, heads, kv_heads):
+    """Query rows by the dozen: votes of prompts' last tokens, and tokens beside sequences of few or none."""
+    rng = np.random.default_rng(dim + heads)
+    check_weights(ops, rng, "u4", "bf16", dim, heads, kv_heads, [1500, 700, 64, 40], counts=[16, 16, 16, 40], decay=0.5)
+    check_weights(ops, rng, "u4", "bf16", dim, heads, kv_heads, [130, 90, 5, 0, 260], counts=[130, 3, 9, 0, 100],
+                  decay=0.0, in_place=False)
+    check_weights(ops, rng, "u4", "bf16", dim, heads, kv_heads, [300, 301, 200], counts=[40, 50, 40], slots=280)
+    check_weights(ops, rng, "u4", "bf16", dim, heads, kv_heads, [90, 200], counts=[60, 60], scale=-0.25, rows=[3, 3])
+    check_weights(ops, rng, "u4", "bf16", dim, heads, kv_heads, [90, 200], counts=[60, 60], rows=[-1, 4])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_weights_of_tokens_that_see_nan_or_not(ops, dtype, dim):
+    """A value that is NaN reaches the tokens that see its key, a key that is NaN their weights too."""
+    torch = torch_()
+    rng = np.random.default_rng(15)
+    cache, _, _ = filled(ops, rng, 2, 2, 200, dim, "u4")
+    cache.v_scale[0, 0, 150, 1, 0] = float("nan")       # tokens from position 150 on, channels 32 to 63
+    cache.k_scale[0, 1, 160, 0, 1] = float("nan")       # tokens from position 160 on
+    q, _ = queries(rng, 60, 16, dim, dtype)
+    mass = torch.zeros((2, 2, 200), device="cuda")
+    out = host(ops.attention_weights(cache, q, ints([190, 120]), mass, starts=ints([0, 50, 60]), decay=0.0))
+    got = host(mass)
+    position = np.arange(140, 190)
+    first, second = out[:50, :8], out[:50, 8:]
+    assert np.isnan(first[position >= 150][..., 32:64]).all() and np.isfinite(np.delete(first, range(32, 64), -1)).all()
+    assert np.isfinite(first[position < 150]).all()
+    assert np.isnan(second[position >= 160]).all() and np.isfinite(second[position < 160]).all()
+    assert np.isfinite(out[50:]).all() and np.isfinite(got[0, 0]).all() and np.isfinite(got[1]).all()
+    assert np.isnan(got[0, 1, :190]).all()
+    assert np.allclose(got[0, 0, :190].sum(), 50 * 8, rtol=1e-4)
+
+
 def test_weights_of_long_rows_are_split(ops):
     rng = np.random.default_rng(8)
     check_weights(ops, rng, "u4", "bf16", 128, 8, 2, [9001], decay=0.25, in_place=False)
