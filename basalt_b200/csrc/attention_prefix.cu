@@ -120,22 +120,22 @@ __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
     return r;
 }
 
-// One word of codes (nibble j of the low half: channel j of one group; of the high half: of the next) and its
-// successor (the next four channels) as 16 bytes of fp16 for each of the two groups: c step + low, or, of keys,
-// (c - 8) step.
+// One word of codes (nibble j of the low half: channel j of one group; of the high half: of the next) as 16 bytes of
+// fp16, c step + low, or, of keys, (c - 8) step. The two groups' channels stay next to one another, so tiles hold
+// channels in an order of their own: 16-byte place 4 y + x of a pair of groups has channels 8 x + 4 y .. + 3 of both,
+// in turn. Queries are laid out alike, and outputs are put in order when they are written.
 template <bool KEYS>
-__device__ __forceinline__ void unpack(uint32_t a, uint32_t b, uint32_t step, uint32_t low, uint4* first,
-                                       uint4* second) {
-    uint32_t x[8];
+__device__ __forceinline__ uint4 unpack(uint32_t w, uint32_t step, uint32_t low) {
+    constexpr uint32_t base = 0x64006400u;      // 1024; in an odd place a code counts 16 times
+    constexpr uint32_t sixteenth = 0x2c002c00u, zero0 = KEYS ? 0x64086408u : base, zero1 = KEYS ? 0xd480d480u : 0xd400d400u;
+    const uint32_t z = w >> 8;
+    uint32_t x[4] = {(w & 0x000f000fu) | base, (w & 0x00f000f0u) | base, (z & 0x000f000fu) | base, (z & 0x00f000f0u) | base};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {  // 1024 + c is exact, as are c and c - 8
-        const uint32_t w = ((j < 4 ? a : b) >> (4 * (j & 3)) & 0x000f000fu) | 0x64006400u;
-        x[j] = KEYS ? mul_f16x2(sub_f16x2(w, 0x64086408u), step) : fma_f16x2(sub_f16x2(w, 0x64006400u), step, low);
+    for (int j = 0; j < 4; ++j) {  // c or c - 8, exactly
+        x[j] = j & 1 ? fma_f16x2(x[j], sixteenth, zero1) : sub_f16x2(x[j], zero0);
+        x[j] = KEYS ? mul_f16x2(x[j], step) : fma_f16x2(x[j], step, low);
     }
-    *first = make_uint4(__byte_perm(x[0], x[1], 0x5410), __byte_perm(x[2], x[3], 0x5410),
-                        __byte_perm(x[4], x[5], 0x5410), __byte_perm(x[6], x[7], 0x5410));
-    *second = make_uint4(__byte_perm(x[0], x[1], 0x7632), __byte_perm(x[2], x[3], 0x7632),
-                         __byte_perm(x[4], x[5], 0x7632), __byte_perm(x[6], x[7], 0x7632));
+    return make_uint4(x[0], x[1], x[2], x[3]);
 }
 
 // Tiles of 32-byte rows in the 32-byte swizzle: atoms of eight rows, 256 bytes apart.
@@ -324,6 +324,16 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
                         *reinterpret_cast<uint16_t*>(to + middle_at(r, 1) + 8 + 2 * g) = 0u;
                     }
                 }
+                // Places of keys: this thread's four channels and those of its neighbour's group, in turn.
+                const bool odd = c & 4;
+                const uint32_t other0 = __shfl_xor_sync(kFull, odd ? w[0] : w[2], 4);
+                const uint32_t other1 = __shfl_xor_sync(kFull, odd ? w[1] : w[3], 4);
+                const uint32_t a0 = odd ? other0 : w[0], a1 = odd ? other1 : w[1];
+                const uint32_t b0 = odd ? w[2] : other0, b1 = odd ? w[3] : other1;
+                w[0] = __byte_perm(a0, b0, 0x5410);
+                w[1] = __byte_perm(a0, b0, 0x7632);
+                w[2] = __byte_perm(a1, b1, 0x5410);
+                w[3] = __byte_perm(a1, b1, 0x7632);
             }
             *reinterpret_cast<uint4*>(smem + (at >> 7) * L::kQuery + r * 128 + (c >> 3) * 16384 +
                                       (((c & 7) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -469,11 +479,11 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
                             for (int y = 0; y < 2; ++y) {
                                 const int g = G == 4 ? y : 0;               // pair of groups
                                 const int eighth = G == 4 ? x : 2 * x + y;  // which eight of a group's 32 channels
-                                uint4 one, two;
-                                unpack<KEYS>(w[G == 4 ? y : 2 * y], w[G == 4 ? 2 + y : 2 * y + 1], step[g], low[g], &one, &two);
                                 unsigned char* const block = to + g * (kTcKeys * 128);
-                                *reinterpret_cast<uint4*>(block + ((eighth ^ (key & 7)) << 4)) = one;
-                                *reinterpret_cast<uint4*>(block + (((4 + eighth) ^ (key & 7)) << 4)) = two;
+                                *reinterpret_cast<uint4*>(block + ((eighth ^ (key & 7)) << 4)) =
+                                    unpack<KEYS>(w[G == 4 ? y : 2 * y], step[g], low[g]);
+                                *reinterpret_cast<uint4*>(block + (((4 + eighth) ^ (key & 7)) << 4)) =
+                                    unpack<KEYS>(w[G == 4 ? 2 + y : 2 * y + 1], step[g], low[g]);
                             }
                         }
                     };
@@ -555,6 +565,7 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
         }
     } else {
         const int half = warp >> 2, in_tile = threadIdx.x & 127, at = 128 * half + in_tile;
+        constexpr int kUnroll = CODES ? 1 : 2;
         const uint32_t s_at = tmem + half * 256 + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
         const uint32_t o_at = s_at + 128;
         // A score's factor to base 2. It stays above zero: the mask's -infinity is multiplied by it.
@@ -576,37 +587,42 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
         bool ok = true;
         for (int i = 0; half < halves && i < key_tiles; ++i) {
             const uint32_t buffer = s_at + (i & 1) * 64;
-            uint32_t s[2][32];
             ok = ok && mbar_wait(s_full + 2 * half + (i & 1), (i >> 1) & 1, status, 7, abort);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            tmem_ld32(buffer, s[0]);
-            tmem_ld32(buffer + 32, s[1]);
             float by = CODES ? scale * key_factor[i & 7] : scale;
             by = by < FLT_MIN ? FLT_MIN : by;
-            tmem_ld_wait();
             const int left = sees - (t0 + i) * kTcKeys;  // keys of the tile, or more
-            if (left < kTcKeys) {
+            // Scores are read twice, 32 at a time: 64 held, the registers that thirteen warps leave were spilled.
+            auto columns = [&](int c, uint32_t (&s)[32]) {
+                tmem_ld32(buffer + 32 * c, s);
+                tmem_ld_wait();
+                if (left < 32 * c + 32) {
 #pragma unroll
-                for (int x = 0; x < 64; ++x) {
-                    if (x >= left) s[x >> 5][x & 31] = 0xff800000u;
-                }
-            }
-            if constexpr (OWN) {
-                float* const to = kept + (t0 + i) * kTcKeys;
-                const int64_t room = pitch - static_cast<int64_t>(t0 + i) * kTcKeys;  // whole blocks of 16
-#pragma unroll
-                for (int x = 0; x < 64; x += 4) {
-                    if (kept && x < room) {
-                        const uint32_t* const y = &s[x >> 5][x & 31];
-                        *reinterpret_cast<float4*>(to + x) = make_float4(__uint_as_float(y[0]) * by, __uint_as_float(y[1]) * by,
-                                                                         __uint_as_float(y[2]) * by, __uint_as_float(y[3]) * by);
+                    for (int x = 0; x < 32; ++x) {
+                        if (32 * c + x >= left) s[x] = 0xff800000u;
                     }
                 }
-            }
+            };
             float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll kUnroll
+            for (int c = 0; c < 2; ++c) {
+                uint32_t s[32];
+                columns(c, s);
+                if constexpr (OWN) {
+                    float* const to = kept + (t0 + i) * kTcKeys + 32 * c;
+                    const int64_t room = pitch - static_cast<int64_t>(t0 + i) * kTcKeys - 32 * c;  // whole blocks of 16
 #pragma unroll
-            for (int x = 0; x < 64; x += 2) {
-                m[(x >> 1) & 3] = max3(m[(x >> 1) & 3], __uint_as_float(s[x >> 5][x & 31]), __uint_as_float(s[x >> 5][(x & 31) + 1]));
+                    for (int x = 0; x < 32; x += 4) {
+                        if (kept && x < room) {
+                            *reinterpret_cast<float4*>(to + x) = make_float4(__uint_as_float(s[x]) * by, __uint_as_float(s[x + 1]) * by,
+                                                                             __uint_as_float(s[x + 2]) * by, __uint_as_float(s[x + 3]) * by);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int x = 0; x < 32; x += 2) {
+                    m[(x >> 1) & 3] = max3(m[(x >> 1) & 3], __uint_as_float(s[x]), __uint_as_float(s[x + 1]));
+                }
             }
             const float most = fmaxf(max3(m[0], m[1], m[2]), m[3]) * by;
             // The maximum that weights are taken against moves only when a row's grows by more than 2^8.
@@ -635,12 +651,13 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
             const float from = (CODES ? 7.0f : 0.0f) - (top == -INFINITY ? 0.0f : top);
             const uint64_t by2 = pair_of(by, by), from2 = pair_of(from, from);
             uint64_t sum[2] = {0ull, 0ull};
-#pragma unroll
+#pragma unroll kUnroll
             for (int c = 0; c < 2; ++c) {
-                uint32_t p[16];
+                uint32_t s[32], p[16];
+                columns(c, s);
 #pragma unroll
                 for (int x = 0; x < 16; ++x) {
-                    const uint64_t y = fma2(pair_of(__uint_as_float(s[c][2 * x]), __uint_as_float(s[c][2 * x + 1])), by2, from2);
+                    const uint64_t y = fma2(pair_of(__uint_as_float(s[2 * x]), __uint_as_float(s[2 * x + 1])), by2, from2);
                     float e0, e1;
                     of_pair(y, &e0, &e1);
                     e0 = exp2_fast(e0);
@@ -685,8 +702,16 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
                 }
 #pragma unroll
                 for (int x = 0; x < 8; ++x) {
-                    *reinterpret_cast<uint4*>(rows_at + at * (HD * 4) + (((8 * c + x) ^ (in_tile & 7)) << 4)) =
-                        make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+                    // Columns 32 c + 8 (x / 2) .. + 7, the even ones or the odd ones: four channels of a group.
+                    const uint32_t* const y = o + 8 * (x >> 1);
+                    int chunk = 8 * c + x;
+                    uint4 z = make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+                    if constexpr (CODES) {
+                        // Place 4 c' + x / 2 of pair c / 2: channels 64 (c / 2) + 32 (x & 1) + 8 (x / 2) + 4 c'.
+                        chunk = 16 * (c >> 1) + 8 * (x & 1) + 2 * (x >> 1) + (c & 1);
+                        z = x & 1 ? make_uint4(y[1], y[3], y[5], y[7]) : make_uint4(y[0], y[2], y[4], y[6]);
+                    }
+                    *reinterpret_cast<uint4*>(rows_at + at * (HD * 4) + ((chunk ^ (in_tile & 7)) << 4)) = z;
                 }
             }
             if (at < rows) {
