@@ -319,11 +319,23 @@ __device__ __noinline__ void attend_plainly(const S* k, const S* v, const T* q, 
     }
 }
 
-// Whether the keys and values of blocks [b0, b1), or `rows` queries (row r at query(r)), hold an infinity
-// or a float that bf16 rounds to one. This thread's share of the CTA's.
-template <typename T, int STORAGE, int HD, typename Q>
+// Where a tile's queries are: row r is token (r0 + r) / group of its sequence.
+template <typename T, int HD>
+struct Queries {
+    const T* q;
+    int64_t stride;
+    int first, r0, group, kvh;
+    bool one;  // a single token, of which the tile has some of the heads
+    __device__ int64_t token(int r) const { return first + static_cast<int64_t>(one ? 0 : (r0 + r) / group); }
+    __device__ int head(int r) const { return kvh * group + r0 + r - static_cast<int>(token(r) - first) * group; }
+    __device__ const T* operator()(int r) const { return q + token(r) * stride + head(r) * HD; }
+};
+
+// Whether the keys and values of blocks [b0, b1), or the first `rows` of the queries, hold an infinity or a
+// float that bf16 rounds to one. This thread's share of the CTA's.
+template <typename T, int STORAGE, int HD>
 __device__ __noinline__ bool meets_infinity(const char* k, const char* v, const Visible& seen, int b0, int b1,
-                                            Q&& query, int rows) {
+                                            Queries<T, HD> query, int rows) {
     auto rounds = [](uint32_t u) { return (u & 0x7fffffffu) - 0x7f7f8000u <= 0x8000u; };
     auto bad = [&](uint32_t u) {
         return STORAGE == BST_DTYPE_F32 ? rounds(u) : ((u & 0x7fffu) == 0x7f80u) | ((u & 0x7fff0000u) == 0x7f800000u);
@@ -374,6 +386,10 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
     constexpr int G = L::kGroups;
     constexpr int R = ROWS / 8;                  // query rows of a lane: g, and g + 8
     constexpr bool kExact = sizeof(T) == 4;      // float32: 24-bit operands
+    // float32 sums over float32 and bf16 entries in float32 additions but for the products of a group of channels or
+    // of a block of keys: the tensor cores cut where those round, and over 20 000 keys that came to 1.2e-5 of the
+    // outputs (plain float32: 2.5e-6).
+    constexpr bool kRounded = kExact && !L::kCodes && PASS != kOwn;
     // Scores good to float32 (with codes): scores that are kept become float32 weights, whatever T is.
     constexpr bool kFine = kExact || PASS == kScores;
     constexpr int kTerms = kExact ? 3 : 2;       // of the weights and query sums, in bf16
@@ -673,9 +689,16 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
                     }
                 }
             } else {
-                float acc[4] = {};
+                float acc[4] = {}, whole[4] = {};
 #pragma unroll
                 for (int gr = 0; gr < G; ++gr) {
+                    if constexpr (kRounded) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            whole[i] += acc[i];
+                            acc[i] = 0.0f;
+                        }
+                    }
                     uint32_t kw[4][kK];  // channels 8 t .. 8 t + 7 of the group, in pairs
                     if constexpr (STORAGE == BST_DTYPE_BF16) {
                         uint32_t w[4];
@@ -702,6 +725,10 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
                             leading<R, kQ>(acc, qa[2 * gr + m], kw[2 * m][i], kw[2 * m + 1][i]);
                         }
                     }
+                }
+                if constexpr (kRounded) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[i] += whole[i];
                 }
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
@@ -964,10 +991,17 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
                     terms_of<kK>(v[0], v[1], v0);
                     terms_of<kK>(v[2], v[3], v1);
                 }
-                product<false, false>(o[j], pa, v0[0], v1[0]);
+                if constexpr (kRounded) {
+                    float block_sum[4] = {};
+                    product<false, false>(block_sum, pa, v0[0], v1[0]);
 #pragma unroll
-                for (int i = 1; i < kK; ++i) {
-                    leading<R, kTerms>(o[j], pa, v0[i], v1[i]);
+                    for (int i = 1; i < kK; ++i) leading<R, kTerms>(block_sum, pa, v0[i], v1[i]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[j][i] += block_sum[i];
+                } else {
+                    product<false, false>(o[j], pa, v0[0], v1[0]);
+#pragma unroll
+                    for (int i = 1; i < kK; ++i) leading<R, kTerms>(o[j], pa, v0[i], v1[i]);
                 }
             }
         }
@@ -1025,27 +1059,21 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
         }
         largest_result = max_nan(largest_result, total[r]);
     }
-    // Query row r of the tile: its token, head and place.
-    auto token_of = [&](int r) {
-        return tile.first + static_cast<int64_t>(tile.n == 1 ? 0 : (tile.r0 + r) / group);
-    };
-    auto head_of = [&](int r) {
-        return kvh * group + tile.r0 + r - static_cast<int>(token_of(r) - tile.first) * group;
-    };
-    auto query_at = [&](int r) { return q + token_of(r) * q_stride + head_of(r) * HD; };
     if constexpr (L::kCodes) {
         __syncthreads();
     } else if (__syncthreads_or(!(largest_result <= FLT_MAX)) &&
-               __syncthreads_or(meets_infinity<T, STORAGE, HD>(kb, vb, seen, b0, b1, query_at, rows))) {
+               __syncthreads_or(meets_infinity<T, STORAGE, HD>(
+                   kb, vb, seen, b0, b1, Queries<T, HD>{q, q_stride, tile.first, tile.r0, group, kvh, tile.n == 1}, rows))) {
         // The terms of an infinity, and of a float that bf16 rounds to one, leave NaN where the formula
         // may have a weight of zero, an infinity or a number (a NaN leaves what it should): the CTA's sums
         // again, a warp a row.
         using S = typename std::conditional<STORAGE == BST_DTYPE_F32, float, __nv_bfloat16>::type;
         for (int r = warp; r < rows; r += kWarps) {
             // The tile's queries see the same keys: of one token here, or all of a prefix.
+            const Queries<T, HD> query{q, q_stride, tile.first, tile.r0, group, kvh, tile.n == 1};
             float* const scores =
-                PASS == kScores ? extra.scores + (token_of(r) * a.heads + head_of(r)) * extra.pitch : nullptr;
-            attend_plainly<T, S, HD>(reinterpret_cast<const S*>(kb), reinterpret_cast<const S*>(vb), query_at(r),
+                PASS == kScores ? extra.scores + (query.token(r) * a.heads + query.head(r)) * extra.pitch : nullptr;
+            attend_plainly<T, S, HD>(reinterpret_cast<const S*>(kb), reinterpret_cast<const S*>(vb), query(r),
                                      a.scale * kLog2e, seen, b0, b1, merge + r * (HD + 2), scores);
             for (int w = 1; w < kWarps && lane == 0; ++w) {
                 float* none = merge + (w * ROWS + r) * (HD + 2);
@@ -1071,9 +1099,10 @@ k_cached(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride
                 value = fmaf(from[ch], f, value);
             }
         }
-        const int64_t token = token_of(r);
-        const int head = head_of(r);
-        if (!part) {
+        const int query = tile.r0 + r, my_token = tile.n == 1 ? 0 : query / group;
+        const int64_t token = tile.first + my_token;
+        const int head = kvh * group + query - my_token * group;
+        if (PASS == kOwn ? splits == 1 : !part) {
             put(out + token * out_stride + head * HD + ch, sum == 0.0f ? 0.0f : value / sum);
         } else {
             float* to = part + ((token * a.heads + head) * splits + split) * (HD + 2);

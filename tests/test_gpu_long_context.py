@@ -181,6 +181,29 @@ def test_long_prefixes(ops, storage, dtype, dim, heads, kv_heads, count, prefix)
         assert np.all(off <= tol), (off / tol).max()
 
 
+@pytest.mark.parametrize("storage", ["f32", "bf16", "u4"])
+def test_float32_sums_over_a_long_prefix(ops, storage):
+    """n = 20 000 keys in float32. A running sum is rounded once for 16 keys, 2^-24 of itself; such errors add up as
+    random ones do over the n / 16 roundings of all splits together, to sqrt(1250) 2^-24 = 2.1e-6. Scores of up to
+    16 are off by 2^-22 of themselves, which every key's weight carries on its own: 16 ln 2 2^-22 / 2 = 1.3e-6. Sums
+    that are cut instead of rounded were 1.2e-5 off."""
+    torch = torch_()
+    g = torch.Generator(device="cuda").manual_seed(1)
+    n, kv_heads, dim, heads = 20000, 3, 128, 9
+    common = ops.KvCache.allocate(1, kv_heads, n, dim, storage)
+    x = torch.randn((2, n, kv_heads, dim), generator=g, device="cuda")
+    x[0] += 2 * torch.randn((1, kv_heads, dim), generator=g, device="cuda") * (torch.rand((1, kv_heads, dim), generator=g, device="cuda") < 0.1)
+    ops.kv_append(common, x[0], x[1], ints([n]), starts=ints([0, n]))
+    k, v = (t.double() for t in ops.kv_read(common, ints([n]), starts=ints([0, n]), tokens=n))
+    own = ops.KvCache.allocate(14, kv_heads, 4, dim, "u4")
+    q = torch.randn((14, heads, dim), generator=g, device="cuda")
+    got = ops.attention_shared(own, q, ints([0] * 14), common, n).double()
+    qh = q.double().unflatten(1, (kv_heads, -1))
+    want = torch.einsum("shgj,jhd->shgd", torch.softmax(torch.einsum("shgd,jhd->shgj", qh, k) * dim ** -0.5, -1), v)
+    off = (got - want.flatten(1, 2)).norm() / want.norm()
+    assert off <= 2.1e-6 + 1.3e-6, off
+
+
 def test_a_prefix_in_the_same_cache_and_out_over_q(ops):
     torch = torch_()
     rng = np.random.default_rng(5)
