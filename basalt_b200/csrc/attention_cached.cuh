@@ -1427,17 +1427,27 @@ k_cached_one(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_st
     }
 }
 
-// One query a key head over a float32 or bf16 cache, on the ordinary units too: two multiply-adds a value are
-// far below what memory takes, while on the tensor cores seven of eight rows would be empty and float32 entries
-// have to be split in three (32 sequences of 33 to 512 keys of eight float32 heads of 64: 18 us there). Lanes
-// hold 16 bytes of a key, the warp kAtOnce keys a pass; the scores of eight passes change places as above.
+// One to four queries a key head over a float32 or bf16 cache, on the ordinary units too: two multiply-adds a value
+// and query are below what memory takes, while on the tensor cores four to seven of eight rows would be empty and
+// float32 entries have to be split in three. Lanes hold 16 bytes of a key, the warp kAtOnce keys a pass; the scores of
+// eight passes change places as above.
 // Sums are plain float32, so NaN and infinities come out as in the formula; what lies behind the end is not read.
+// 64 sequences of 500 to 4000 keys of eight heads, here and there (us, with weights), for one query a key head:
+// float32 of 128 channels 197 and 471, of 64 105 and 146; bf16 of 128 113 and 123, of 32 40 and 52. For two: 222
+// and 475, 118 and 150; 131 and 125, 48 and 55. For four: 311 and 484, 166 and 155; 229 and 132, 80 and 57.
 constexpr int kPlainWarps = 4;
 
 // Whether a pass is for this kernel.
 inline bool plain_query(const Cache& c, const Batch& b, const AttnSpec& a) {
-    return c.storage != BST_DTYPE_U4 && a.heads == a.kv_heads && !b.starts;
+    if (c.storage == BST_DTYPE_U4 || b.starts) return false;
+    const int group = a.heads / a.kv_heads;
+    const bool wide = a.head_dim == 128;
+    if (group == 2) return !(wide && c.storage == BST_DTYPE_BF16 && a.dtype == BST_DTYPE_BF16);
+    return group == 1 || (group <= 4 && wide && c.storage == BST_DTYPE_F32 && a.dtype == BST_DTYPE_F32);
 }
+// Its CTAs an SM.
+constexpr int plain_ctas(int group) { return group == 1 ? 4 : 3; }
+inline int plain_per_sm(const AttnSpec& a) { return plain_ctas(a.heads / a.kv_heads); }
 
 template <typename S>
 __device__ __forceinline__ void entries_of(const uint4& u, float (&x)[16 / sizeof(S)]) {
@@ -1453,20 +1463,21 @@ __device__ __forceinline__ void entries_of(const uint4& u, float (&x)[16 / sizeo
     }
 }
 
-template <typename T, typename S, int HD, int PASS>
-__global__ void __launch_bounds__(kPlainWarps * 32, 4)
+// GROUP: the queries, or the next number of them that is built.
+template <typename T, typename S, int HD, int GROUP, int PASS>
+__global__ void __launch_bounds__(kPlainWarps * 32, plain_ctas(GROUP))
 k_cached_plain(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_stride, int splits,
                float* __restrict__ part, Extra extra) {
     constexpr int kVec = 16 / sizeof(S), kLanes = HD / kVec, kAtOnce = 32 / kLanes, kPasses = 8;
     constexpr int kKeys = kAtOnce * kPasses, kMine = kLanes < 8 ? 8 / kLanes : 1, kCopies = kLanes > 8 ? kLanes / 8 : 1;
-    __shared__ float merge[kPlainWarps][HD + 2];
+    __shared__ float merge[kPlainWarps][GROUP][HD + 2];
     if constexpr (PASS == kBeside) {
         if (blockIdx.x == gridDim.x - 1) {
             if (blockIdx.y + blockIdx.z == 0) pdl_wait();
             return;
         }
     }
-    const int seq = blockIdx.x, head = blockIdx.y, split = blockIdx.z;
+    const int seq = blockIdx.x, kvh = blockIdx.y, split = blockIdx.z, group = GROUP == 1 ? 1 : a.heads / a.kv_heads;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, word = lane % kLanes, sub = lane / kLanes;
     const int row = b.rows ? __ldg(b.rows + seq) : seq;
     const int position = max(0, __ldg(b.lengths + seq)) - 1;
@@ -1479,7 +1490,7 @@ k_cached_plain(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_
     const int sunk = sees ? min(a.sinks, seen.first) : 0, skipped = seen.first - sunk;
     const int64_t places = sees ? static_cast<int64_t>(sunk) + seen.end - seen.first : 0;
     const int x0 = static_cast<int>(places * split / use), x1 = static_cast<int>(places * (split + 1) / use);
-    const int64_t at = ((static_cast<int64_t>(inside ? row : 0) * c.kv_heads + head) * c.slots * HD) + word * kVec;
+    const int64_t at = ((static_cast<int64_t>(inside ? row : 0) * c.kv_heads + kvh) * c.slots * HD) + word * kVec;
     const S* const kb = static_cast<const S*>(c.k) + at;
     const S* const vb = static_cast<const S*>(c.v) + at;
     auto key_at = [&](int place) { return static_cast<int64_t>(place + (place >= sunk ? skipped : 0)); };
@@ -1495,105 +1506,125 @@ k_cached_plain(Cache c, Batch b, AttnSpec a, const T* __restrict__ q, int64_t q_
     uint4 kw[kPasses];
     int x = x0 + warp * kKeys;
     load(x, kb, kw);
-    float qv[kVec];
-    const T* const src = q + seq * q_stride + head * HD + word * kVec;
+    const int64_t head0 = static_cast<int64_t>(kvh) * group;
+    float qv[GROUP][kVec];
 #pragma unroll
-    for (int n = 0; n < kVec; ++n) qv[n] = to_f(src[n]);
+    for (int h = 0; h < GROUP; ++h) {
+        const T* const src = q + seq * q_stride + (head0 + h) * HD + word * kVec;
+#pragma unroll
+        for (int n = 0; n < kVec; ++n) qv[h][n] = h < group ? to_f(src[n]) : 0.0f;
+    }
     const float to_score = a.scale * kLog2e;
     const int my_pass = word * 8 / kLanes;  // and the one behind it with two keys a lane
-    float* const keep_scores = extra.scores + (static_cast<int64_t>(seq) * a.heads + head) * extra.pitch;
+    float* const keep_scores = extra.scores + (static_cast<int64_t>(seq) * a.heads + head0) * extra.pitch;
 
-    float acc[kVec] = {}, top = -INFINITY, total = 0.0f;
+    float acc[GROUP][kVec] = {}, top[GROUP], total[GROUP] = {};
+#pragma unroll
+    for (int h = 0; h < GROUP; ++h) top[h] = -INFINITY;
     for (; x < x1; x += kPlainWarps * kKeys) {
         uint4 vw[kPasses];
         load(x, vb, vw);
-        float s[kPasses];
+        float s[GROUP][kPasses];
 #pragma unroll
         for (int i = 0; i < kPasses; ++i) {
             float k[kVec];
             entries_of<S>(kw[i], k);
-            s[i] = 0.0f;
 #pragma unroll
-            for (int n = 0; n < kVec; ++n) s[i] = fmaf(k[n], qv[n], s[i]);
+            for (int h = 0; h < GROUP; ++h) {
+                s[h][i] = 0.0f;
+#pragma unroll
+                for (int n = 0; n < kVec; ++n) s[h][i] = fmaf(k[n], qv[h][n], s[h][i]);
+            }
         }
         load(x + kPlainWarps * kKeys, kb, kw);
+        float p[GROUP][kMine];
 #pragma unroll
-        for (int n = kPasses / 2, o = kLanes / 2; o > 0; o >>= 1, n = n > 1 ? n / 2 : (n == 1 ? 0 : 0)) {
-            if (n > 0) {
-                const bool upper = lane & o;
+        for (int h = 0; h < GROUP; ++h) {
 #pragma unroll
-                for (int i = 0; i < n; ++i) {
-                    const float away = upper ? s[i] : s[i + n];
-                    s[i] = (upper ? s[i + n] : s[i]) + __shfl_xor_sync(kFull, away, o);
+            for (int n = kPasses / 2, o = kLanes / 2; o > 0; o >>= 1, n /= 2) {
+                if (n > 0) {
+                    const bool upper = lane & o;
+#pragma unroll
+                    for (int i = 0; i < n; ++i) {
+                        const float away = upper ? s[h][i] : s[h][i + n];
+                        s[h][i] = (upper ? s[h][i + n] : s[h][i]) + __shfl_xor_sync(kFull, away, o);
+                    }
+                } else {
+                    s[h][0] += __shfl_xor_sync(kFull, s[h][0], o);
                 }
-            } else {
-                s[0] += __shfl_xor_sync(kFull, s[0], o);
             }
-        }
-        float score[kMine], most = -INFINITY;
+            float most = -INFINITY;
 #pragma unroll
-        for (int m = 0; m < kMine; ++m) {
-            const int place = x + (my_pass + m) * kAtOnce + sub;
-            score[m] = s[m] * to_score;
-            if (place >= x1) {
-                score[m] = -INFINITY;
-            } else if constexpr (PASS == kScores) {
-                if (word % kCopies == 0) keep_scores[key_at(place)] = score[m];
+            for (int m = 0; m < kMine; ++m) {
+                const int place = x + (my_pass + m) * kAtOnce + sub;
+                s[h][m] *= to_score;
+                if (place >= x1) {
+                    s[h][m] = -INFINITY;
+                } else if constexpr (PASS == kScores) {
+                    if (word % kCopies == 0 && h < group) keep_scores[h * extra.pitch + key_at(place)] = s[h][m];
+                }
+                most = fmaxf(most, s[h][m]);
             }
-            most = fmaxf(most, score[m]);
-        }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(kFull, most, o));
-        if (most > top) {
-            const float keep = top == -INFINITY ? 0.0f : exp2_fast(top - most);
-            top = most;
-            total *= keep;
+            for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(kFull, most, o));
+            if (most > top[h]) {
+                const float keep = top[h] == -INFINITY ? 0.0f : exp2_fast(top[h] - most);
+                top[h] = most;
+                total[h] *= keep;
 #pragma unroll
-            for (int n = 0; n < kVec; ++n) acc[n] *= keep;
-        }
-        const float base = top == -INFINITY ? 0.0f : top;
-        float p[kMine];
+                for (int n = 0; n < kVec; ++n) acc[h][n] *= keep;
+            }
+            const float base = top[h] == -INFINITY ? 0.0f : top[h];
 #pragma unroll
-        for (int m = 0; m < kMine; ++m) {
-            p[m] = exp2_fast(score[m] - base);
-            total += p[m];
+            for (int m = 0; m < kMine; ++m) {
+                p[h][m] = exp2_fast(s[h][m] - base);
+                total[h] += p[h][m];
+            }
         }
 #pragma unroll
         for (int i = 0; i < kPasses; ++i) {
-            const float weight = __shfl_sync(kFull, p[i % kMine], sub * kLanes + i * kLanes / 8);
             float v[kVec];
             entries_of<S>(vw[i], v);
 #pragma unroll
-            for (int n = 0; n < kVec; ++n) acc[n] = fmaf(weight, v[n], acc[n]);
+            for (int h = 0; h < GROUP; ++h) {
+                const float weight = __shfl_sync(kFull, p[h][i % kMine], sub * kLanes + i * kLanes / 8);
+#pragma unroll
+                for (int n = 0; n < kVec; ++n) acc[h][n] = fmaf(weight, v[n], acc[h][n]);
+            }
         }
     }
     // The lanes' sums, then the warps'. Where lanes share a key each counts its weight.
-    total = warp_sum(total) * (1.0f / kCopies);
 #pragma unroll
-    for (int n = 0; n < kVec; ++n) {
+    for (int h = 0; h < GROUP; ++h) {
+        const float sum = warp_sum(total[h]) * (1.0f / kCopies);
 #pragma unroll
-        for (int o = kLanes; o < 32; o <<= 1) acc[n] += __shfl_xor_sync(kFull, acc[n], o);
-        if (lane < kLanes) merge[warp][word * kVec + n] = acc[n];
-    }
-    if (lane == 0) {
-        merge[warp][HD] = top;
-        merge[warp][HD + 1] = total;
+        for (int n = 0; n < kVec; ++n) {
+#pragma unroll
+            for (int o = kLanes; o < 32; o <<= 1) acc[h][n] += __shfl_xor_sync(kFull, acc[h][n], o);
+            if (lane < kLanes) merge[warp][h][word * kVec + n] = acc[h][n];
+        }
+        if (lane == 0) {
+            merge[warp][h][HD] = top[h];
+            merge[warp][h][HD + 1] = sum;
+        }
     }
     __syncthreads();
-    for (int ch = threadIdx.x; ch < HD; ch += kPlainWarps * 32) {
+    for (int i = threadIdx.x; i < group * HD; i += kPlainWarps * 32) {
+        const int h = i / HD, ch = i % HD;
         float m = -INFINITY, sum = 0.0f, value = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kPlainWarps; ++w) m = fmaxf(m, merge[w][HD]);
+        for (int w = 0; w < kPlainWarps; ++w) m = fmaxf(m, merge[w][h][HD]);
 #pragma unroll
         for (int w = 0; w < kPlainWarps; ++w) {
-            const float f = merge[w][HD] == -INFINITY ? 0.0f : exp2_fast(merge[w][HD] - m);
+            const float* const from = merge[w][h];
+            const float f = from[HD] == -INFINITY ? 0.0f : exp2_fast(from[HD] - m);
             // A warp that saw no key has nothing to add, and one whose scores are all NaN has that.
-            if (merge[w][HD] != -INFINITY || merge[w][HD + 1] != 0.0f) {
-                sum = fmaf(merge[w][HD + 1], f, sum);
-                value = fmaf(merge[w][ch], f, value);
+            if (from[HD] != -INFINITY || from[HD + 1] != 0.0f) {
+                sum = fmaf(from[HD + 1], f, sum);
+                value = fmaf(from[ch], f, value);
             }
         }
-        float* const to = part + ((static_cast<int64_t>(seq) * a.heads + head) * splits + split) * (HD + 2);
+        float* const to = part + ((static_cast<int64_t>(seq) * a.heads + head0 + h) * splits + split) * (HD + 2);
         to[ch] = value;
         if (ch == 0) {
             to[HD] = m;
@@ -1787,9 +1818,20 @@ cudaError_t run_cached(cudaStream_t s, const Cache& c, const Batch& b, const Att
                 }
                 if constexpr (STORAGE != BST_DTYPE_U4 && (PASS == kScores || PASS == kBeside)) {
                     using S = typename std::conditional<STORAGE == BST_DTYPE_F32, float, __nv_bfloat16>::type;
+                    auto plain = [&](auto n) {
+                        return launch(k_cached_plain<T, S, HD, decltype(n)::value, PASS>,
+                                      dim3(b.count + kMore, a.kv_heads, splits), kPlainWarps * 32, 0, c, b, a, from,
+                                      q_stride, splits, part, extra);
+                    };
                     if (plain_query(c, b, a)) {
-                        return launch(k_cached_plain<T, S, HD, PASS>, dim3(b.count + kMore, a.heads, splits),
-                                      kPlainWarps * 32, 0, c, b, a, from, q_stride, splits, part, extra);
+                        const int group = a.heads / a.kv_heads;
+                        if (group == 1) return plain(std::integral_constant<int, 1>());
+                        if constexpr (sizeof(T) == 4 && sizeof(S) == 4 && HD == 128) {
+                            if (group > 2) return plain(std::integral_constant<int, 4>());
+                        }
+                        if constexpr (sizeof(T) == 4 || sizeof(S) == 4 || HD < 128) {
+                            return plain(std::integral_constant<int, 2>());
+                        }
                     }
                 }
                 if constexpr (sizeof(T) == 2) {

@@ -57,7 +57,7 @@ bool large(const Batch& b, const AttnSpec& a, const Prefix& p) {
 // Splits of the own keys: no more than fill the card (spreading 64 rows of 20 to 1000 keys over four waves took
 // 64 us where this takes 62, 24 x 4 drafts 93 instead of 88).
 int own_splits(const Cache& c, const Batch& b, const AttnSpec& a) {
-    return split_count(c, b, a, plain_query(c, b, a) ? 4 : 0);
+    return split_count(c, b, a, plain_query(c, b, a) ? plain_per_sm(a) : 0);
 }
 
 size_t part_bytes(const Batch& b, const AttnSpec& a, int splits) {

@@ -210,7 +210,7 @@ int large_splits(const Cache& c, const Batch& b, const AttnSpec& a) {
 }
 
 int small_splits(const Cache& c, const Batch& b, const AttnSpec& a) {
-    return split_count(c, b, a, plain_query(c, b, a) ? 4 : 0);
+    return split_count(c, b, a, plain_query(c, b, a) ? plain_per_sm(a) : 0);
 }
 
 int64_t pitch_of(const Cache& c) { return (static_cast<int64_t>(c.slots) + kBlock - 1) / kBlock * kBlock; }

@@ -320,6 +320,18 @@ def test_weights(ops, storage, dtype, dim, heads, kv_heads):
     check_weights(ops, rng, storage, dtype, dim, heads, kv_heads, [33, 150], window=20, sinks=3, decay=0.5)
 
 
+@pytest.mark.parametrize("storage", ["bf16", "f32"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [32, 64, 128])
+def test_weights_of_small_groups(ops, storage, dtype, dim):
+    """One to four queries a key head, which float32 and bf16 caches take in kernels of their own."""
+    rng = np.random.default_rng(dim)
+    for heads in (2, 4, 6, 8):
+        check_weights(ops, rng, storage, dtype, dim, heads, 2, [200, 1, 0, 77], window=0 if heads < 6 else 50, sinks=7,
+                      decay=0.3)
+        check_shared(ops, rng, storage, storage, dtype, dim, heads, 2, 40, [190, 0, 1, 33])
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("heads,kv_heads", [(3, 3), (8, 2), (6, 1)])
 def test_weights_of_several_tokens(ops, dtype, heads, kv_heads):
