@@ -48,10 +48,15 @@ Plan plan_large(const Batch& b, const AttnSpec& a, const Prefix& p) {
     return plan;
 }
 
-// Rows of a key head from which on the tensor cores' tiles of 128 pay.
-constexpr int kLargeRows = 48;
+// Rows of a key head from which on tcgen05's tiles of 128 pay, however few of them are filled. Whole calls, eight key
+// heads of 128, tcgen05 and mma.sync (us): bf16 behind 500 keys 10.1 and 10.9 with 8 rows, 10.5 and 13.4 with 12; behind
+// 4000 14.6 and 18.1, 14.8 and 21.0; behind 30 000 32.7 and 36.3, 33.4 and 39.7. 4 bits, which take longer to unpack
+// for tcgen05, behind 500 keys 16.3 and 17.0 with 16 rows, 17.4 and 17.2 with 32, 18.5 and 18.7 with 64; behind 30 000
+// 46.5 and 37.6, 47.8 and 49.7, 52.8 and 76.1. (Of 64 channels behind 30 000 keys bf16 gains from 48 rows on: 32 and 39.)
+constexpr int kLargeRows = 12, kLargeCodeRows = 32;
 bool large(const Batch& b, const AttnSpec& a, const Prefix& p) {
-    return prefix_tc_takes(p, a) && static_cast<int64_t>(b.tokens) * (a.heads / a.kv_heads) >= kLargeRows;
+    const int64_t rows = static_cast<int64_t>(b.tokens) * (a.heads / a.kv_heads);
+    return prefix_tc_takes(p, a) && rows >= (p.cache.storage == BST_DTYPE_U4 ? kLargeCodeRows : kLargeRows);
 }
 
 // Splits of the own keys: no more than fill the card (spreading 64 rows of 20 to 1000 keys over four waves took

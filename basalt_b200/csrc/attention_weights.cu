@@ -197,10 +197,15 @@ k_weights_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out,
     }
 }
 
-// Several tokens of each sequence on tcgen05, from kLargeRows query rows a sequence and key head on.
-constexpr int kLargeRows = 24;
+// Several tokens of each sequence on tcgen05, from kLargeRows query rows a sequence and key head and kLargeSlots on.
+// Whole calls of eight sequences, eight key heads of 128, tcgen05 and mma.sync (us): rows of 200 to 600 keys 52 and 50
+// with 64 query rows, 80 and 93 with 128; of 700 to 2000 keys 76 and 72 with 48, 81 and 80 with 64, 112 and 145 with
+// 128; of 1700 to 5000 keys 101 and 80 with 32, 121 and 144 with 64, 167 and 256 with 128. Four key heads of 64: of 200
+// to 600 keys 60 and 49 with 128, of 700 to 2000 47 and 44 with 64, 67 and 68 with 128, of 1700 to 5000 90 and 107.
+constexpr int kLargeRows = 64, kLargeSlots = 2048;
 bool large(const Cache& c, const Batch& b, const AttnSpec& a) {
-    return own_tc_takes(c, b, a) && static_cast<int64_t>(b.tokens) * (a.heads / a.kv_heads) >= static_cast<int64_t>(b.count) * kLargeRows;
+    return own_tc_takes(c, b, a) && c.slots >= kLargeSlots &&
+           static_cast<int64_t>(b.tokens) * (a.heads / a.kv_heads) >= static_cast<int64_t>(b.count) * kLargeRows;
 }
 
 // Four waves of CTAs there, since lengths differ and are not known here.

@@ -190,6 +190,8 @@ class KvCache:
 
 def _sequences(device, tokens, lengths, starts, rows):
     """The batch's struct; the tensors it points to belong to the caller."""
+    if starts is None and rows is None and lengths is not None:
+        return _lib.SequencesStruct(lengths.shape[0], tokens, None, None, _index(device, "lengths", lengths))
     if lengths is not None:
         at = _index(device, "lengths", lengths)
         count = lengths.shape[0]
@@ -317,7 +319,8 @@ def attention_shared(cache: KvCache, q, lengths, prefix: KvCache, prefix_length:
     ``attention_cached`` without a window). The prefix is read once for the whole batch; ``prefix`` may be
     ``cache`` itself, or hold its keys in another storage. ``out`` may be ``q`` itself."""
     device = cache.device
-    stream = _given(device, stream)
+    if stream is not None:
+        stream = _given(device, stream)
     if prefix.device != device:
         _on(device, "prefix", prefix.k)
     q_stride = _packed(device, "q", q, None, cache.head_dim)
@@ -325,7 +328,7 @@ def attention_shared(cache: KvCache, q, lengths, prefix: KvCache, prefix_length:
     s = _sequences(device, q.shape[0], lengths, starts, rows)
     prefix_row, prefix_length = _lib.int32(prefix_row), _lib.int32(prefix_length)
     lib = _lib.load()
-    key = (s.count, s.tokens, starts is None, q.shape[1], q.dtype, scale, prefix._shape, prefix_length)
+    key = (lengths.shape[0], q.shape[0], starts is None, q.shape[1], q.dtype, scale, prefix._shape, prefix_length)
     plan = cache._sizes.get(key)
     if plan is None:
         a = _spec(q, cache.kv_heads, 0, 0, scale)
@@ -335,9 +338,11 @@ def attention_shared(cache: KvCache, q, lengths, prefix: KvCache, prefix_length:
         plan = cache._keep(key, (size.value, a))
     needed, a = plan
     pointer, room, workspace = _workspace(device, needed, workspace, stream)
-    _raise(lib.bst_attention_shared(device.index, _stream(device, stream), cache._ref, s, a, prefix._ref,
-                                    prefix_row, prefix_length, q.data_ptr(), q_stride, out.data_ptr(),
-                                    out_stride, pointer, room))
+    status = lib.bst_attention_shared(device.index, _raw_stream(device.index) if stream is None else stream,
+                                      cache._ref, s, a, prefix._ref, prefix_row, prefix_length, q.data_ptr(),
+                                      q_stride, out.data_ptr(), out_stride, pointer, room)
+    if status:
+        _raise(status)
     return out
 
 
@@ -361,14 +366,15 @@ def attention_weights(cache: KvCache, q, lengths, mass, previous=None, decay: fl
     and the query heads of key head h give key j. ``mass`` and ``previous`` (``mass`` itself by default) are
     float32 [rows, kv_heads, slots]; with ``decay`` 0 what was there is not read. Returns the outputs."""
     device = cache.device
-    stream = _given(device, stream)
+    if stream is not None:
+        stream = _given(device, stream)
     to = _mass(device, "mass", mass, cache)
     before = to if previous is None else _mass(device, "previous", previous, cache)
     q_stride = _packed(device, "q", q, None, cache.head_dim)
     out, out_stride = _out(device, q, out, stream)
     s = _sequences(device, q.shape[0], lengths, starts, rows)
     lib = _lib.load()
-    key = (s.count, s.tokens, starts is None, q.shape[1], q.dtype, scale, window, sinks, "weights")
+    key = (lengths.shape[0], q.shape[0], starts is None, q.shape[1], q.dtype, scale, window, sinks, "weights")
     plan = cache._sizes.get(key)
     if plan is None:
         a = _spec(q, cache.kv_heads, window, sinks, scale)
@@ -377,8 +383,11 @@ def attention_weights(cache: KvCache, q, lengths, mass, previous=None, decay: fl
         plan = cache._keep(key, (size.value, a))
     needed, a = plan
     pointer, room, workspace = _workspace(device, needed, workspace, stream)
-    _raise(lib.bst_attention_weights(device.index, _stream(device, stream), cache._ref, s, a, q.data_ptr(),
-                                     q_stride, out.data_ptr(), out_stride, before, decay, to, pointer, room))
+    status = lib.bst_attention_weights(device.index, _raw_stream(device.index) if stream is None else stream,
+                                       cache._ref, s, a, q.data_ptr(), q_stride, out.data_ptr(), out_stride, before,
+                                       decay, to, pointer, room)
+    if status:
+        _raise(status)
     return out
 
 
@@ -391,7 +400,8 @@ def kv_evict(cache: KvCache, mass, lengths, keep: int, recent: int = 0, sinks: i
     lengths (int32) and the kept slots [count, kv_heads, keep] (int32, -1 behind the last; ``kept`` if
     given)."""
     device = cache.device
-    stream = _given(device, stream)
+    if stream is not None:
+        stream = _given(device, stream)
     keep = _lib.int32(keep)
     target = cache if to is None else to
     if target.device != device:
@@ -401,8 +411,11 @@ def kv_evict(cache: KvCache, mass, lengths, keep: int, recent: int = 0, sinks: i
         raise IllegalArgumentException("to_mass must be given beside to", _lib.BST_INVALID)
     to_at = at if to_mass is None else _mass(device, "to_mass", to_mass, target)
     s = _sequences(device, lengths.shape[0], lengths, None, rows)
-    new = _empty((s.count,), _module.int32, device, stream)
-    shape = (s.count, cache.kv_heads, max(keep, 0))
+    if not 1 <= keep <= target.slots:  # before memory is taken for it
+        raise BasaltShapeException(f"keep is {keep}, the cache that is written has {target.slots} slots",
+                                   _lib.BST_SHAPE)
+    shape = (lengths.shape[0], cache.kv_heads, keep)
+    new = _empty(shape[:1], _module.int32, device, stream)
     if kept is None:
         kept = _empty(shape, _module.int32, device, stream)
     else:

@@ -347,25 +347,30 @@ def test_weights_of_several_tokens(ops, dtype, heads, kv_heads):
 def test_weights_of_many_tokens(ops, dim, heads, kv_heads):
     """Query rows by the dozen: votes of prompts' last tokens, and tokens beside sequences of few or none."""
     rng = np.random.default_rng(dim + heads)
-    check_weights(ops, rng, "u4", "bf16", dim, heads, kv_heads, [1500, 700, 64, 40], counts=[16, 16, 16, 40], decay=0.5)
-    check_weights(ops, rng, "u4", "bf16", dim, heads, kv_heads, [130, 90, 5, 0, 260], counts=[130, 3, 9, 0, 100],
-                  decay=0.0, in_place=False)
+    for slots in (None, 2100):   # with many slots on the tensor cores' large tiles, if there are rows enough
+        check_weights(ops, rng, "u4", "bf16", dim, heads, kv_heads, [1500, 700, 64, 40], counts=[16, 16, 16, 40],
+                      decay=0.5, slots=slots)
+        check_weights(ops, rng, "u4", "bf16", dim, heads, kv_heads, [130, 90, 5, 0, 260], counts=[130, 3, 9, 0, 100],
+                      decay=0.0, in_place=False, slots=slots)
+        check_weights(ops, rng, "u4", "bf16", dim, heads, kv_heads, [90, 200], counts=[60, 60], scale=-0.25, rows=[3, 3],
+                      slots=slots)
+        check_weights(ops, rng, "u4", "bf16", dim, heads, kv_heads, [90, 200], counts=[60, 60], rows=[-1, 4], slots=slots)
     check_weights(ops, rng, "u4", "bf16", dim, heads, kv_heads, [300, 301, 200], counts=[40, 50, 40], slots=280)
-    check_weights(ops, rng, "u4", "bf16", dim, heads, kv_heads, [90, 200], counts=[60, 60], scale=-0.25, rows=[3, 3])
-    check_weights(ops, rng, "u4", "bf16", dim, heads, kv_heads, [90, 200], counts=[60, 60], rows=[-1, 4])
+    check_weights(ops, rng, "u4", "bf16", dim, heads, kv_heads, [2070, 2099], counts=[64, 70], slots=2060)
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("dim", [64, 128])
-def test_weights_of_tokens_that_see_nan_or_not(ops, dtype, dim):
+@pytest.mark.parametrize("slots", [200, 2048])
+def test_weights_of_tokens_that_see_nan_or_not(ops, dtype, dim, slots):
     """A value that is NaN reaches the tokens that see its key, a key that is NaN their weights too."""
     torch = torch_()
     rng = np.random.default_rng(15)
-    cache, _, _ = filled(ops, rng, 2, 2, 200, dim, "u4")
+    cache, _, _ = filled(ops, rng, 2, 2, slots, dim, "u4")
     cache.v_scale[0, 0, 150, 1, 0] = float("nan")       # tokens from position 150 on, channels 32 to 63
     cache.k_scale[0, 1, 160, 0, 1] = float("nan")       # tokens from position 160 on
     q, _ = queries(rng, 60, 16, dim, dtype)
-    mass = torch.zeros((2, 2, 200), device="cuda")
+    mass = torch.zeros((2, 2, slots), device="cuda")
     out = host(ops.attention_weights(cache, q, ints([190, 120]), mass, starts=ints([0, 50, 60]), decay=0.0))
     got = host(mass)
     position = np.arange(140, 190)
