@@ -58,7 +58,10 @@ k_weights_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out,
         const uint32_t query = WARP ? unit / (HD / 32) : unit;
         const int token = query / static_cast<uint32_t>(a.heads), head = query - static_cast<uint32_t>(token) * a.heads;
         int seq, first, n;
-        if (token >= b.tokens || !find_sequence(b, token, &seq, &first, &n)) return;
+        if (token >= b.tokens || !find_sequence(b, token, &seq, &first, &n)) {
+            pdl_wait();  // every CTA does: this kernel's end is that of the pass before it
+            return;
+        }
         const int use = used_splits(c, b, a, tile_rows, splits, seq, token - first, n, head);
         pdl_wait();
         const float* const from = part + static_cast<int64_t>(query) * splits * (HD + 2);
@@ -79,13 +82,14 @@ k_weights_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out,
     const int first_seq = of_head / static_cast<uint32_t>(a.kv_heads);
     const int kvh = of_head - static_cast<uint32_t>(first_seq) * a.kv_heads;
     const int row = b.rows ? __ldg(b.rows + first_seq) : first_seq;
-    if (row < 0 || row >= c.rows || !first_of_row(b, first_seq, row)) return;
+    const bool first_one = first_of_row(b, first_seq, row);
+    pdl_wait();
+    if (row < 0 || row >= c.rows || !first_one) return;
     const int group = a.heads / a.kv_heads, lane = threadIdx.x & 31;
     constexpr int N = 4, kBatch = 4;  // rows whose scores are under way together
     static_assert(N * kThreads == kMassKeys, "four keys a thread");
     const int64_t base = (static_cast<int64_t>(row) * c.kv_heads + kvh) * c.slots;
     int known = -1;  // the sequence whose maxima and sums are held, all of them
-    pdl_wait();
     for (int chunk = 0; chunk < per; ++chunk) {
         const int key0 = begin + chunk * kMassKeys;
         if (key0 >= c.slots) break;

@@ -437,8 +437,12 @@ def kept_places(mass, length, keep, recent, sinks):
     return sorted([*range(sinks), *best, *range(length - recent, length)])
 
 
+def raw_parts(cache):
+    return [t for t in (cache.k, cache.v, cache.k_scale, cache.v_scale) if t is not None]
+
+
 def raw(cache):
-    return [t.clone() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale) if t is not None]
+    return [t.clone() for t in raw_parts(cache)]
 
 
 def check_evict(ops, rng, storage, dim, kv_heads, slots, lengths, keep, recent=0, sinks=0, rows=None, to=None,
@@ -538,6 +542,85 @@ def test_evict_rows_named_twice_and_outside(ops):
     check_evict(ops, rng, "bf16", 64, 2, 60, [60, 50, 40, 30], 20, 4, 2, rows=[1, 1, -1, 5])
     check_evict(ops, rng, "bf16", 64, 2, 60, [60, 50, 40, 30], 20, 4, 2, rows=[1, 1, 0, 0], to=33, to_rows=[2, 3, 2, 0])
     check_evict(ops, rng, "u4", 64, 2, 60, [60, 50, 40, 99], 20, 4, 2, rows=[1, 7, 0, 3], to=33, to_rows=[9, 3, -1, 0])
+
+
+# ---- places --------------------------------------------------------------------------------------
+@pytest.mark.parametrize("storage", ["u4", "bf16"])
+def test_queries_at_odd_places(ops, storage):
+    """bf16 queries that 16-byte accesses cannot read give what aligned ones give, within the two kernels' errors."""
+    torch = torch_()
+    rng = np.random.default_rng(16)
+    common, _, v = filled(ops, rng, 1, 2, 700, 64, storage)
+    cache, _, _ = filled(ops, rng, 50, 2, 9, 64, "u4")
+    g = torch.Generator(device="cuda").manual_seed(3)
+    wide = torch.randn((50, 8 * 64 + 3), generator=g, device="cuda").bfloat16()
+    lengths = ints(rng.integers(0, 10, 50))
+    for at in (0, 1, 2):
+        odd = wide[:, at:at + 512].unflatten(-1, (8, 64))
+        straight = odd.contiguous()
+        a = host(ops.attention_shared(cache, odd, lengths, common, 700))
+        b = host(ops.attention_shared(cache, straight, lengths, common, 700))
+        assert np.abs(a - b).max() <= 4 * 2.0 ** -8 * np.abs(v).max()
+    long, _, lv = filled(ops, rng, 2, 2, 2100, 64, "u4")
+    wide = torch.randn((40, 8 * 64 + 3), generator=g, device="cuda").bfloat16()
+    masses = [torch.zeros((2, 2, 2100), device="cuda") for _ in range(2)]
+    for q, mass in zip((wide[:, 1:513].unflatten(-1, (8, 64)), wide[:, 1:513].unflatten(-1, (8, 64)).contiguous()), masses):
+        ops.attention_weights(long, q, ints([2100, 1500]), mass, starts=ints([0, 20, 40]), decay=0.0)
+    assert torch.allclose(*masses, rtol=1e-4, atol=1e-7)
+
+
+def test_rows_without_tokens_fade(ops):
+    torch = torch_()
+    cache = ops.KvCache.allocate(3, 2, 50, 64)
+    for decay in (0.0, 0.25):
+        mass = torch.ones((3, 2, 50), device="cuda")
+        q = torch.zeros((0, 4, 64), device="cuda")
+        out = ops.attention_weights(cache, q, ints([30, 50]), mass, starts=ints([0, 0, 0]), rows=ints([2, 0]), decay=decay)
+        assert out.shape == (0, 4, 64)
+        got = host(mass)
+        assert (got[1] == 1).all() and (got[0] == decay).all() and (got[2, :, :30] == decay).all() and (got[2, :, 30:] == 1).all()
+    # no sequence at all
+    ops.attention_weights(cache, q, ints([]), mass, starts=ints([0]))
+    ops.attention_shared(cache, q, ints([]), cache, 7, starts=ints([0]))
+    n, kept = ops.kv_evict(cache, mass, ints([]), 5)
+    assert n.shape == (0,) and kept.shape == (0, 2, 5)
+    with pytest.raises(Exception, match="keep"):
+        ops.kv_evict(cache, mass, ints([3]), 51)
+    with pytest.raises(Exception, match="keep"):
+        ops.kv_evict(cache, mass, ints([3]), 2 ** 33)
+
+
+@pytest.mark.parametrize("storage,dtype", [("bf16", "bf16"), ("u4", "bf16"), ("f32", "f32")])
+def test_rows_far_into_a_cache(ops, storage, dtype):
+    """Entries behind the 2^32nd: the last row of a cache is what the same row of a small cache is."""
+    torch = torch_()
+    rng = np.random.default_rng(17)
+    slots, kv_heads, dim, heads = 65000, 4, 128, 16
+    rows = {"f32": 140, "bf16": 140, "u4": 280}[storage]     # 4.7 to 9.3 thousand million entries
+    far = ops.KvCache.allocate(rows, kv_heads, slots, dim, storage)
+    near = ops.KvCache.allocate(2, kv_heads, slots, dim, storage)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    for t in (near.k, near.v):
+        t.copy_(torch.randint(0, 256, t.shape, generator=g, device="cuda") if storage == "u4" else torch.randn(t.shape, generator=g, device="cuda"))
+    if storage == "u4":
+        for t in (near.k_scale, near.v_scale):
+            t.copy_(torch.rand(t.shape, generator=g, device="cuda") - torch.tensor([0.0, 4.0], device="cuda"))
+    for x, y in zip(raw_parts(far), raw_parts(near)):
+        x[rows - 1].copy_(y[1])
+    q = torch.randn((20, heads, dim), generator=g, device="cuda").to(getattr(torch, {"f32": "float32", "bf16": "bfloat16"}[dtype]))
+    lengths, some = ints([64999]), q[:1]
+    masses = [torch.rand((r, kv_heads, slots), generator=g, device="cuda") for r in (2, rows)]
+    masses[1][rows - 1].copy_(masses[0][1])
+    results = []
+    for cache, row, mass in ((near, 1, masses[0]), (far, rows - 1, masses[1])):
+        a = ops.attention_weights(cache, some, lengths, mass, rows=ints([row]), decay=0.5)
+        own = ops.KvCache.allocate(20, kv_heads, 8, dim, "u4")
+        b = ops.attention_shared(own, q, ints([0] * 20), cache, 64999, prefix_row=row)
+        c = ops.attention_shared(cache, some, lengths, near, 100, rows=ints([row]))
+        n, kept = ops.kv_evict(cache, mass, lengths, 3000, 100, 4, rows=ints([row]))
+        results.append([a, b, c, mass[row].clone(), n, kept] + [t[row, :, :3000].clone() for t in raw_parts(cache)])
+    for x, y in zip(*results):
+        assert torch.equal(x.view(torch.uint8) if x.is_floating_point() else x, y.view(torch.uint8) if y.is_floating_point() else y)
 
 
 # ---- together --------------------------------------------------------------------------------------
