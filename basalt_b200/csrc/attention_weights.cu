@@ -48,6 +48,41 @@ __device__ __forceinline__ void add_split(float* m, float* total, float top, flo
     *m = most;
 }
 
+// Maxima and sums of query rows r0 .. r0 + rows - 1 of a sequence and key head, by the CTA: as many lanes a row as
+// there are to spare.
+template <int HD>
+__device__ __forceinline__ void row_sums(const Cache& c, const AttnSpec& a, int tile_rows, int splits,
+                                         const float* part, int row, int length, int first, int n, int kvh, int r0,
+                                         int rows, float* tops, float* inverse) {
+    const int group = a.heads / a.kv_heads, lane = threadIdx.x & 31;
+    int lanes = 32;
+    while (lanes > 1 && rows * lanes > kThreads) lanes >>= 1;
+    const int of_warp = 32 / lanes;  // a warp takes that many rows at a time
+    __syncthreads();
+    for (int r = threadIdx.x / lanes; r < (rows + of_warp - 1) / of_warp * of_warp; r += kThreads / lanes) {
+        float m = -INFINITY, total = 0.0f;
+        if (r < rows) {
+            const int token = (r0 + r) / group, head = kvh * group + (r0 + r) - token * group;
+            const int use = used_splits(c, a, tile_rows, splits, row, length, token, n, head);
+            const float* from = part + (static_cast<int64_t>(first + token) * a.heads + head) * splits * (HD + 2) + HD;
+#pragma unroll 4
+            for (int s = lane % lanes; s < use; s += lanes) {
+                const float2 y = *reinterpret_cast<const float2*>(from + s * (HD + 2));
+                add_split(&m, &total, y.x, y.y);
+            }
+        }
+        for (int o = lanes / 2; o > 0; o >>= 1) {
+            const float other = __shfl_xor_sync(kFull, m, o), others = __shfl_xor_sync(kFull, total, o);
+            add_split(&m, &total, other, others);
+        }
+        if (r < rows && lane % lanes == 0) {
+            tops[r] = m == -INFINITY ? 0.0f : m;
+            inverse[r] = total == 0.0f ? 0.0f : 1.0f / total;
+        }
+    }
+    __syncthreads();
+}
+
 template <typename T, int HD, bool WARP>
 __global__ void __launch_bounds__(kThreads)
 k_weights_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out, int64_t out_stride,
@@ -85,10 +120,66 @@ k_weights_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out,
     const bool first_one = first_of_row(b, first_seq, row);
     pdl_wait();
     if (row < 0 || row >= c.rows || !first_one) return;
-    const int group = a.heads / a.kv_heads, lane = threadIdx.x & 31;
+    const int group = a.heads / a.kv_heads;
     constexpr int N = 4, kBatch = 4;  // rows whose scores are under way together
     static_assert(N * kThreads == kMassKeys, "four keys a thread");
     const int64_t base = (static_cast<int64_t>(row) * c.kv_heads + kvh) * c.slots;
+    // The usual case, one sequence a row with a token for a few heads: what its rows need is in registers, and a
+    // chunk's scores and masses are loaded while the chunk before it is added up (64 rows of up to 8192 keys: 35 us
+    // by the general loop below).
+    const int only = b.rows ? next_of_row(b, first_seq, row) : b.count;
+    if (only == b.count && !b.starts && group <= kBatch) {
+        const int length = max(0, __ldg(b.lengths + first_seq)), stop = min(min(length, c.slots), begin + per * kMassKeys);
+        if (stop <= begin) return;
+        row_sums<HD>(c, a, tile_rows, splits, part, row, length, first_seq, 1, kvh, 0, group, tops, inverse);
+        float top[kBatch], by[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            top[k] = tops[min(k, group - 1)];
+            by[k] = inverse[min(k, group - 1)];
+        }
+        const float* const from = scores + (static_cast<int64_t>(first_seq) * a.heads + kvh * group) * pitch;
+        const int position = length - 1;
+        auto load = [&](int key, float4 (&x)[kBatch], float (&old)[N]) {
+            if (key >= stop) return;
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                if (k < group) x[k] = __ldcs(reinterpret_cast<const float4*>(from + k * pitch + key));
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) old[i] = decay != 0.0f && key + i < stop ? previous[base + key + i] : 0.0f;
+        };
+        float4 x[kBatch] = {}, next[kBatch] = {};
+        float old[N] = {}, next_old[N] = {};
+        int key = begin + N * static_cast<int>(threadIdx.x);
+        load(key, x, old);
+        for (; key < stop; key += kMassKeys) {
+            load(key + kMassKeys, next, next_old);
+            float sum[N] = {};
+            // A token outside the cache sees nothing.
+            if (position < c.slots) {
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k) {
+                    if (k >= group) continue;
+                    const float s[N] = {x[k].x, x[k].y, x[k].z, x[k].w};
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        const float more = fmaf(exp2_fast(s[i] - top[k]), by[k], sum[i]);
+                        const bool seen = a.window == 0 || position - (key + i) < a.window || key + i < a.sinks;
+                        sum[i] = seen ? more : sum[i];
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                if (key + i < stop) mass[base + key + i] = decay == 0.0f ? sum[i] : fmaf(decay, old[i], sum[i]);
+                old[i] = next_old[i];
+            }
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) x[k] = next[k];
+        }
+        return;
+    }
     int known = -1;  // the sequence whose maxima and sums are held, all of them
     for (int chunk = 0; chunk < per; ++chunk) {
         const int key0 = begin + chunk * kMassKeys;
@@ -132,33 +223,7 @@ k_weights_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out,
             for (int r0 = 0; r0 < all; r0 += kMassRows) {
                 const int rows = min(kMassRows, all - r0);
                 if (known != seq) {
-                    // Maxima and sums of the rows: as many lanes a row as there are to spare.
-                    int lanes = 32;
-                    while (lanes > 1 && rows * lanes > kThreads) lanes >>= 1;
-                    const int of_warp = 32 / lanes;  // a warp takes that many rows at a time
-                    __syncthreads();
-                    for (int r = threadIdx.x / lanes; r < (rows + of_warp - 1) / of_warp * of_warp; r += kThreads / lanes) {
-                        float m = -INFINITY, total = 0.0f;
-                        if (r < rows) {
-                            const int token = (r0 + r) / group, head = kvh * group + (r0 + r) - token * group;
-                            const int use = used_splits(c, a, tile_rows, splits, row, length, token, n, head);
-                            const float* from = part + (static_cast<int64_t>(first + token) * a.heads + head) * splits * (HD + 2) + HD;
-#pragma unroll 4
-                            for (int s = lane % lanes; s < use; s += lanes) {
-                                const float2 y = *reinterpret_cast<const float2*>(from + s * (HD + 2));
-                                add_split(&m, &total, y.x, y.y);
-                            }
-                        }
-                        for (int o = lanes / 2; o > 0; o >>= 1) {
-                            const float other = __shfl_xor_sync(kFull, m, o), others = __shfl_xor_sync(kFull, total, o);
-                            add_split(&m, &total, other, others);
-                        }
-                        if (r < rows && lane % lanes == 0) {
-                            tops[r] = m == -INFINITY ? 0.0f : m;
-                            inverse[r] = total == 0.0f ? 0.0f : 1.0f / total;
-                        }
-                    }
-                    __syncthreads();
+                    row_sums<HD>(c, a, tile_rows, splits, part, row, length, first, n, kvh, r0, rows, tops, inverse);
                     known = all <= kMassRows ? seq : -1;
                 }
                 for (int r = 0; r < rows; r += kBatch) {  // kMassRows are whole batches
