@@ -16,8 +16,9 @@
 // smallest product is left out. Values and weights become fp16, 11 bits, values by one fused multiply-add for two
 // of them, rounded once (with bf16 ones the error was 1.6 times the outputs' own rounding instead of 1.0). Powers
 // of two keep all of it in fp16's range: one for each query row and each tile of keys, which the scores' factor f
-// takes back; and one for values, that of the largest so far with four bits to spare, by which O is rescaled when a
-// tile passes it (values 2^-25 of the largest so far begin to lose bits).
+// takes back; and one for the values of each group of 32 channels, that of the largest so far with two bits to spare,
+// by which O is rescaled when a tile passes it. Where that leaves an entry too few bits (keys 2^-12 of the tile's
+// largest, values 2^-20 of the group's so far: no trained model's) the CTA's rows are added up again, plainly.
 // Each of the four warps unpacks whole tiles by itself, so that they wait for one another nowhere.
 //
 // The same kernel takes several tokens of each sequence over its own 4-bit row (OWN): then rows see the keys up to
@@ -47,7 +48,7 @@ struct PrefixLayout {
     static constexpr int kTile = kTcKeys * HD * 2;    // a tile of keys or values
     static constexpr int kSlots = CODES ? 6 : 8;
     static constexpr int kBars = 2 * kQuery + kSlots * kTile;
-    static constexpr int kFactors = kBars + 256;      // of rows, tiles of keys, tiles of values (8 each, of 96)
+    static constexpr int kFactors = kBars + 256;      // of rows, eight tiles of keys, eight tiles of values by groups
     // Middles: the queries' sums, [half][128 rows], and four tiles of keys, 32 bytes a row in the 32-byte swizzle.
     static constexpr int kSums = kFactors + (kRows + 64) * 4, kMiddles = kSums + (CODES ? 2 * 128 * 32 : 0);
     static constexpr int kRaw = kMiddles + (CODES ? 4 * kTcKeys * 32 : 0);
@@ -203,7 +204,7 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
     int* const status = reinterpret_cast<int*>(tmem_slot + 1);  // [0] error code, [1] abort, [2] redo
     float* const row_factor = reinterpret_cast<float*>(smem + L::kFactors);   // what a row was divided by,
     float* const key_factor = row_factor + kRows;                             // a tile of keys, [8],
-    float* const value_factor = key_factor + 8;                               // and of values and weights, [8]
+    float* const value_factor = key_factor + 8;                               // and of values and weights, [8][groups]
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < L::kSlots; ++i) {
@@ -391,41 +392,61 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
                     asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(piece(stage, x)));
                 }
             };
-            // The exponent above a tile's largest, which is at most max |low| + 15 step (not of a NaN).
-            auto exponent_of = [&](int stage, int x) {
-                uint32_t most = 0u;
+            // What a group's entries are at most: |low| + 15 step.
+            auto top_of = [](uint32_t w) {
+                return fmaf(15.0f, __uint_as_float(w << 16), fabsf(__uint_as_float(w & 0xffff0000u)));
+            };
+            // The exponents above the groups' largest entries in a tile (not of a NaN).
+            auto exponents_of = [&](int stage, int x, int (&e)[G]) {
+                uint32_t most[G] = {};
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     uint32_t w[G];
                     scale_words(stage, x + half, w);
 #pragma unroll
                     for (int g = 0; g < G; ++g) {
-                        const float top = fmaf(15.0f, __uint_as_float(w[g] << 16), fabsf(__uint_as_float(w[g] & 0xffff0000u)));
-                        most = max(most, top <= FLT_MAX ? __float_as_uint(top) : (isnan(top) ? 0u : 0x7f000000u));
+                        const float top = top_of(w[g]);
+                        most[g] = max(most[g], top <= FLT_MAX ? __float_as_uint(top) : (isnan(top) ? 0u : 0x7f000000u));
                     }
                 }
-                return exponent_above(__reduce_max_sync(kFull, most));
+#pragma unroll
+                for (int g = 0; g < G; ++g) e[g] = exponent_above(__reduce_max_sync(kFull, most[g]));
             };
-            int values_below = -1000;  // values are below 2^this; what they are divided by goes with it
+            int below[G];  // values of the groups are below 2^this; what they are divided by goes with it
+#pragma unroll
+            for (int g = 0; g < G; ++g) below[g] = -1000;
             load(u & 1, 0);
             for (int tile = u & 1, stage = 0; tile < key_tiles; tile += 2, stage ^= 1) {
                 load(tile + 2, stage ^ 1);
                 asm volatile("cp.async.wait_group 1;" ::: "memory");
                 __syncwarp();
                 const int i = keys ? k_copy(tile) : v_copy(tile);
+                float by[G];
+                int e[G];
                 if (!keys && tile > 0) {
-                    const int e = exponent_of(stage, 2 * kChunks + 2);
-                    if (e > values_below) values_below = e + 4;
+                    exponents_of(stage, 2 * kChunks + 2, e);
+#pragma unroll
+                    for (int g = 0; g < G; ++g) below[g] = e[g] > below[g] ? e[g] + 2 : below[g];
                 }
-                const int e = exponent_of(stage, 2 * kChunks);
-                if (!keys && e > values_below) values_below = e + 4;
-                const float by = power_of_two(keys ? -e : 15 - values_below);
+                exponents_of(stage, 2 * kChunks, e);
+                if (keys) {
+#pragma unroll
+                    for (int g = 1; g < G; ++g) e[0] = max(e[0], e[g]);
+                }
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    if (!keys) below[g] = e[g] > below[g] ? e[g] + 2 : below[g];
+                    by[g] = power_of_two(keys ? 8 - e[0] : 15 - below[g]);
+                }
                 if (i >= L::kSlots && !mbar_wait(empty + i % L::kSlots, ((i / L::kSlots) - 1) & 1, status, 1, abort)) break;
                 if (lane == 0) {
                     if (keys) {
-                        key_factor[tile & 7] = power_of_two(e);
+                        key_factor[tile & 7] = power_of_two(e[0] - 8);
                     } else {
-                        value_factor[tile & 7] = power_of_two(values_below - 22);  // weights are 2^7 too large
+#pragma unroll
+                        for (int g = 0; g < G; ++g) {
+                            value_factor[(tile & 7) * 4 + g] = power_of_two(below[g] - 22);  // weights are 2^7 too large
+                        }
                     }
                 }
 #pragma unroll 1
@@ -434,6 +455,17 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
                     unsigned char* const to = smem + 2 * L::kQuery + (i % L::kSlots) * L::kTile + key * 128;
                     uint32_t scale[G], step[G / 2], low[G / 2];
                     scale_words(stage, 2 * kChunks + half, scale);
+                    // A key 2^-12 of the tile's largest, or values 2^-20 of the largest so far in their group, would
+                    // have too few bits: the rows are added up plainly.
+                    float key_top = 0.0f;
+                    bool small = false;
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {
+                        const float top = top_of(scale[g]);
+                        key_top = fmaxf(key_top, top);
+                        small |= !keys && top > 0.0f && top * by[g] < 0x1p-7f;
+                    }
+                    if (small || (keys && key_top > 0.0f && key_top * by[0] < 0x1p-4f)) status[2] = 1;
                     if (OWN && !keys && (t0 + tile) * kTcKeys + key > sees_all) {
                         // Zero times a NaN is one: rows that do not see it must not get it, the others have to.
                         bool bad = false;
@@ -447,16 +479,16 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
                     }
 #pragma unroll
                     for (int g = 0; g < G; g += 2) {
-                        step[g / 2] = half2_of(__uint_as_float(scale[g] << 16) * by, __uint_as_float(scale[g + 1] << 16) * by);
-                        low[g / 2] = half2_of(__uint_as_float(scale[g] & 0xffff0000u) * by,
-                                              __uint_as_float(scale[g + 1] & 0xffff0000u) * by);
+                        step[g / 2] = half2_of(__uint_as_float(scale[g] << 16) * by[g], __uint_as_float(scale[g + 1] << 16) * by[g + 1]);
+                        low[g / 2] = half2_of(__uint_as_float(scale[g] & 0xffff0000u) * by[g],
+                                              __uint_as_float(scale[g + 1] & 0xffff0000u) * by[g + 1]);
                     }
                     if (keys) {
                         // Middles beside the queries' sums: high terms twice, low ones, zeros.
                         uint32_t terms[4] = {};
 #pragma unroll
                         for (int g = 0; g < G; ++g) {
-                            terms[g] = two_halves(fmaf(8.0f, __uint_as_float(scale[g] << 16), __uint_as_float(scale[g] & 0xffff0000u)) * by);
+                            terms[g] = two_halves(fmaf(8.0f, __uint_as_float(scale[g] << 16), __uint_as_float(scale[g] & 0xffff0000u)) * by[0]);
                         }
                         unsigned char* const middle = smem + L::kMiddles + (tile & 3) * (kTcKeys * 32);
                         const uint32_t h0 = __byte_perm(terms[0], terms[1], 0x5410), h1 = __byte_perm(terms[2], terms[3], 0x5410);
@@ -570,7 +602,10 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
         const uint32_t o_at = s_at + 128;
         // A score's factor to base 2. It stays above zero: the mask's -infinity is multiplied by it.
         const float scale = fabsf(a.scale) * kLog2e * (CODES ? row_factor[at] : 1.0f);
-        float top = -INFINITY, total = 0.0f, values_by = 1.0f;
+        constexpr int G = HD / 32;
+        float top = -INFINITY, total = 0.0f, values_by[G];
+#pragma unroll
+        for (int g = 0; g < G; ++g) values_by[g] = 1.0f;
         // Keys that the row sees, and where its scores go.
         int sees = end;
         float* kept = nullptr;
@@ -627,7 +662,7 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
             const float most = fmaxf(max3(m[0], m[1], m[2]), m[3]) * by;
             // The maximum that weights are taken against moves only when a row's grows by more than 2^8.
             const bool move = most > top + 8.0f || (top == -INFINITY && most > top);
-            auto rescale = [&](float keep) {
+            auto rescale = [&](const float (&keep)[G]) {
                 ok = ok && mbar_wait(o_done + half, (i - 1) & 1, status, 8, abort);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
@@ -636,15 +671,20 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
                     tmem_ld32(o_at + 32 * c, o);
                     tmem_ld_wait();
 #pragma unroll
-                    for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * keep);
+                    for (int x = 0; x < 32; ++x) {  // columns of two groups in turn
+                        o[x] = __float_as_uint(__uint_as_float(o[x]) * keep[c / 2 * 2 + (x & 1)]);
+                    }
                     tmem_st16(o_at + 32 * c, o);
                     tmem_st16(o_at + 32 * c + 16, o + 16);
                 }
             };
             if (__any_sync(kFull, move)) {
-                const float keep = move ? (top == -INFINITY ? 0.0f : exp2_fast(top - most)) : 1.0f;
+                float keep[G];
+                keep[0] = move ? (top == -INFINITY ? 0.0f : exp2_fast(top - most)) : 1.0f;
+#pragma unroll
+                for (int g = 1; g < G; ++g) keep[g] = keep[0];
                 if (move) top = most;
-                total *= keep;
+                total *= keep[0];
                 if (i > 0) rescale(keep);
             }
             // Weights for fp16 are 2^7 too large, and so is their sum.
@@ -674,9 +714,16 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
                 // Values of this tile that are divided by more than those before: what was summed has to be, too.
                 // (The tile is there until these weights have been multiplied with it.)
                 ok = ok && await(v_copy(i), 6);
-                const float now = value_factor[i & 7];
-                if (i > 0 && now != values_by) rescale(values_by / now);
-                values_by = now;
+                float keep[G];
+                bool changed = false;
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    const float now = value_factor[(i & 7) * 4 + g];
+                    keep[g] = values_by[g] / now;
+                    changed |= now != values_by[g];
+                    values_by[g] = now;
+                }
+                if (i > 0 && changed) rescale(keep);
             }
             tmem_st_wait();
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -698,7 +745,7 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
                 tmem_ld_wait();
                 if constexpr (CODES) {
 #pragma unroll
-                    for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * values_by);
+                    for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * values_by[c / 2 * 2 + (x & 1)]);
                 }
 #pragma unroll
                 for (int x = 0; x < 8; ++x) {
@@ -753,7 +800,7 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
     if (!again) return;
-    // Its rows once more, plainly, a warp a row and a key at a time: slow, but right.
+    // Its rows once more, plainly, a warp a row and a key at a time: slow, but right whatever the entries are.
     constexpr int C = HD / 32;
     const int64_t keys_at = (static_cast<int64_t>(cache_row) * a.kv_heads + kvh) * prefix.cache.slots;
     for (int r = warp; r < rows; r += kThreadsOf<CODES> / 32) {

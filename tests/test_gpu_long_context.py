@@ -544,6 +544,77 @@ def test_evict_rows_named_twice_and_outside(ops):
     check_evict(ops, rng, "u4", 64, 2, 60, [60, 50, 40, 99], 20, 4, 2, rows=[1, 7, 0, 3], to=33, to_rows=[9, 3, -1, 0])
 
 
+# ---- large entries ---------------------------------------------------------------------------------
+@pytest.mark.parametrize("ratio", [2.0 ** 10, 2.0 ** 19, 2.0 ** 24, 2.0 ** 40, 2.0 ** 60])
+@pytest.mark.parametrize("where", ["hidden", "light", "early"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_large_values_without_weight_leave_the_others_theirs(ops, dim, where, ratio):
+    """Values far above the others at a key that only the last tokens see, at keys whose scores are far below the
+    others', or in a first block of keys of which that holds, in front of many queries over 4 bits. Values count by
+    their weight: `weighed` is the largest sum of weight |v| of a channel of the query's."""
+    rng = np.random.default_rng(int(np.log2(ratio)) + dim)
+    L, kv_heads, heads, tokens = 2100 if where == "hidden" else 700, 2, 16, 20
+    k = rng.standard_normal((L, kv_heads, dim)).astype(np.float32)
+    v = rng.standard_normal((L, kv_heads, dim)).astype(np.float32)
+    q = rng.standard_normal((tokens, heads, dim)).astype(np.float32)
+    keys = {"hidden": [L - 1], "light": [0, 50, 320], "early": list(range(64))}[where]
+    v[keys] *= np.float32(ratio)
+    if where != "hidden":
+        q[..., 0], k[:, :, 0] = 12.0, 0.0
+        k[keys, :, 0] = -45.0 * np.log2(ratio) / 40 * (dim / 64) ** 0.5   # weights of about 2^-1.3 / ratio^2.4
+    cache, starts = ops.KvCache.allocate(1, kv_heads, L + 10, dim), ints([0, L])
+    ops.kv_append(cache, tensor(k), tensor(v), ints([L]), starts=starts)
+    k, v = (host(t) for t in ops.kv_read(cache, ints([L]), starts=starts, tokens=L))
+    q = tensor(q, "bf16")
+    qh = host(q)
+    if where == "hidden":
+        mass = torch_().zeros((1, kv_heads, L + 10), device="cuda")
+        got = host(ops.attention_weights(cache, q, ints([L]), mass, starts=ints([0, tokens]), decay=0.0))
+        added = np.zeros((kv_heads, L))
+    else:
+        own = ops.KvCache.allocate(tokens, kv_heads, 4, dim)
+        got = host(ops.attention_shared(own, q, ints([0] * tokens), cache, L))
+    for i in range(tokens):
+        n = L - tokens + i + 1 if where == "hidden" else L
+        for h in range(heads):
+            kk, vv = (x[:n, h * kv_heads // heads] for x in (k, v))
+            p = softmax(kk @ qh[i, h] * dim ** -0.5)
+            weighed = (p @ np.abs(vv)).max()
+            size = np.array([(np.abs(kk) @ np.abs(qh[i, h]) * dim ** -0.5)[p > 1e-3 * p.max()].max()])
+            want = p @ vv
+            tol = shared_bound(size, dim, n, weighed, want, "bf16", "u4")
+            assert np.all(np.abs(got[i, h] - want) <= tol), (i, h, (np.abs(got[i, h] - want) / tol).max())
+            if where == "hidden":
+                added[h * kv_heads // heads, :n] += p
+    if where == "hidden":
+        assert np.abs(host(mass)[0, :, :L] - added).max() <= 1e-4 * added.max()
+
+
+@pytest.mark.parametrize("ratio", [2.0 ** -30, 2.0 ** -16, 2.0 ** -8, 2.0 ** 8, 2.0 ** 30])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_keys_of_very_different_sizes(ops, dim, ratio):
+    """Keys far above or below the others of their tile, of scores that do not matter or do."""
+    torch = torch_()
+    rng = np.random.default_rng(dim)
+    n, kv_heads, heads, count = 500, 2, 16, 20
+    x = rng.standard_normal((2, n, kv_heads, dim)).astype(np.float32)
+    x[0, ::37] *= np.float32(ratio)
+    x[0, ::37] = -np.abs(x[0, ::37])                       # and far below the others' scores where they are large
+    common = ops.KvCache.allocate(1, kv_heads, n, dim)
+    ops.kv_append(common, tensor(x[0]), tensor(x[1]), ints([n]), starts=ints([0, n]))
+    k, v = (host(t) for t in ops.kv_read(common, ints([n]), starts=ints([0, n]), tokens=n))
+    own = ops.KvCache.allocate(count, kv_heads, 4, dim)
+    q = torch.from_numpy(np.abs(rng.standard_normal((count, heads, dim))).astype(np.float32)).cuda().bfloat16()
+    got, qh = host(ops.attention_shared(own, q, ints([0] * count), common, n)), host(q)
+    for i in range(count):
+        for h in range(heads):
+            kk, vv = k[:, h * kv_heads // heads], v[:, h * kv_heads // heads]
+            p = softmax(kk @ qh[i, h] * dim ** -0.5)
+            size = np.array([(np.abs(kk) @ np.abs(qh[i, h]) * dim ** -0.5)[p > 1e-3 * p.max()].max()])
+            tol = shared_bound(size, dim, n, np.abs(vv).max(), p @ vv, "bf16", "u4")
+            assert np.all(np.abs(got[i, h] - p @ vv) <= tol), (i, h, (np.abs(got[i, h] - p @ vv) / tol).max())
+
+
 # ---- places --------------------------------------------------------------------------------------
 @pytest.mark.parametrize("storage", ["u4", "bf16"])
 def test_queries_at_odd_places(ops, storage):
