@@ -44,7 +44,10 @@ __device__ __forceinline__ Route route_of(const Cache& c, const Batch& b, const 
 }
 
 // ---- which keys stay ---------------------------------------------------------------------------
-constexpr int kChoose = 512;           // threads of a choosing CTA
+// Threads of a choosing CTA, more where a head has long rows and a cluster: 131 000 keys evicted down to 16 384 take
+// 52 us with 512 and 49 with 1024, 32 prompts of up to 8192 keys, a CTA a head, 68 and 70.
+template <int CTAS>
+constexpr int kChooseThreads = CTAS > 1 ? 1024 : 512;
 constexpr int kBins = 2048;
 constexpr int kSegment = 8192;         // slots from which on a head has more CTAs than one
 constexpr int kHeld = 40960;           // masses that a CTA's shared memory holds
@@ -57,8 +60,9 @@ __device__ __forceinline__ uint32_t ordered(float x) {
 }
 
 // The sum of `x` over the CTA's earlier threads.
+template <int THREADS>
 __device__ __forceinline__ uint32_t sum_before(uint32_t x, uint32_t* sums, uint32_t* all) {
-    constexpr int kWarps = kChoose / 32;
+    constexpr int kWarps = THREADS / 32;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint32_t run = x;
 #pragma unroll
@@ -82,8 +86,9 @@ __device__ __forceinline__ uint32_t sum_before(uint32_t x, uint32_t* sums, uint3
 
 // CTAS: of a cluster, which has one head.
 template <int CTAS>
-__global__ void __launch_bounds__(kChoose)
+__global__ void __launch_bounds__(kChooseThreads<CTAS>)
 k_evict_choose(Cache c, Batch b, Eviction e, int held) {
+    constexpr int kChoose = kChooseThreads<CTAS>;
     __shared__ __align__(16) uint32_t bins[3][kBins];
     __shared__ uint32_t sums[kChoose / 32], found[2], counts[2];
     extern __shared__ float masses[];
@@ -138,10 +143,10 @@ k_evict_choose(Cache c, Batch b, Eviction e, int held) {
                 if ((u & mask) == known) atomicAdd(bins[pass] + ((u >> shift) & digit), 1u);
             }
             meet();
-            // Counts of the cluster, from the highest bin down: thread i has bins 2047 - 4 i to 2044 - 4 i.
+            // Counts of the cluster, from the highest bin down: thread i has bins 2047 - 4 i to 2044 - 4 i, if any.
             uint4 x = {};
 #pragma unroll
-            for (int r = 0; r < CTAS; ++r) {
+            for (int r = 0; r < CTAS && threadIdx.x < kBins / 4; ++r) {
                 const uint32_t* of = bins[pass];
                 if constexpr (CTAS > 1) of = cg::this_cluster().map_shared_rank(bins[pass], (rank + r) % CTAS);
                 const uint4 y = reinterpret_cast<const uint4*>(of)[kBins / 4 - 1 - threadIdx.x];
@@ -149,7 +154,7 @@ k_evict_choose(Cache c, Batch b, Eviction e, int held) {
             }
             const uint32_t each[4] = {x.w, x.z, x.y, x.x};
             uint32_t total;
-            uint32_t before = sum_before(x.x + x.y + x.z + x.w, sums, &total);
+            uint32_t before = sum_before<kChoose>(x.x + x.y + x.z + x.w, sums, &total);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if (before < need && before + each[i] >= need) {
@@ -177,9 +182,9 @@ k_evict_choose(Cache c, Batch b, Eviction e, int held) {
         equal += !free && u == border;
     }
     uint32_t total;
-    uint32_t above_before = sum_before(above, sums, &total);
+    uint32_t above_before = sum_before<kChoose>(above, sums, &total);
     if (threadIdx.x == 0) counts[0] = total;
-    uint32_t ties = sum_before(equal, sums, &total);
+    uint32_t ties = sum_before<kChoose>(equal, sums, &total);
     if (threadIdx.x == 0) counts[1] = total;
     meet();
     if constexpr (CTAS > 1) {
@@ -284,6 +289,7 @@ k_evict_move(Cache c, Batch b, Eviction e, int row_units, int scale_units, int r
 
 template <int CTAS>
 cudaError_t choose(cudaStream_t s, const Cache& c, const Batch& b, const Eviction& e) {
+    constexpr int kChoose = kChooseThreads<CTAS>;
     const int run = ((c.slots + CTAS * kChoose - 1) / (CTAS * kChoose)) | 1;
     const int held = static_cast<int64_t>(run) * kChoose <= kHeld ? run * kChoose : 0;
     if (held > 4096) {  // beside 24 KB of counts, more than a kernel has by itself
