@@ -88,8 +88,11 @@ __global__ void __launch_bounds__(kThreads)
 k_weights_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out, int64_t out_stride,
                int splits, const float* __restrict__ part, const float* __restrict__ scores, int64_t pitch,
                const float* previous, float decay, float* mass, int joins, int per) {
-    if (blockIdx.x < joins) {
-        const uint32_t unit = WARP ? blockIdx.x * kWarps + (threadIdx.x >> 5) : blockIdx.x;
+    // The last CTAs join: short ones, which fill up what the others leave (first, they took a batch from 210 to 214 us).
+    const uint32_t weights = gridDim.x - joins;
+    if (blockIdx.x >= weights) {
+        const uint32_t block = blockIdx.x - weights;
+        const uint32_t unit = WARP ? block * kWarps + (threadIdx.x >> 5) : block;
         const uint32_t query = WARP ? unit / (HD / 32) : unit;
         const int token = query / static_cast<uint32_t>(a.heads), head = query - static_cast<uint32_t>(token) * a.heads;
         int seq, first, n;
@@ -111,7 +114,7 @@ k_weights_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out,
     }
     __shared__ float tops[kMassRows], inverse[kMassRows];
     // In 32 bits: the quotients of 64 took a third of all instructions. A CTA has `per` chunks of keys.
-    const uint32_t shares = (c.slots + per * kMassKeys - 1) / (per * kMassKeys), place = blockIdx.x - joins;
+    const uint32_t shares = (c.slots + per * kMassKeys - 1) / (per * kMassKeys), place = blockIdx.x;
     const uint32_t of_head = place / shares;
     const int begin = static_cast<int>(place - of_head * shares) * per * kMassKeys;
     const int first_seq = of_head / static_cast<uint32_t>(a.kv_heads);
@@ -322,7 +325,12 @@ cudaError_t launch_attention_weights(cudaStream_t s, const Cache& c, const Batch
     const int64_t joins = warp ? (queries * (a.head_dim / 32) + kWarps - 1) / kWarps : queries;
     // Six CTAs an SM, each of whole chunks (one chunk a CTA: 35 instead of 20 us for 64 rows of up to 8192 keys).
     const int64_t heads = static_cast<int64_t>(b.count) * a.kv_heads, chunks = (c.slots + kMassKeys - 1) / kMassKeys;
-    const int64_t per = std::min(chunks, (heads * chunks + 148 * 6 - 1) / (148 * 6));
+    // From 16 query rows a sequence on two chunks at most: eight sequences' 8 tokens of four heads over 16 384 keys take
+    // 183 us, with three 191, with one 185; four rows of 64 sequences, without this, 343 with nineteen and 352 with two.
+    int64_t per = std::min(chunks, (heads * chunks + 148 * 6 - 1) / (148 * 6));
+    if (static_cast<int64_t>(b.tokens) * (a.heads / a.kv_heads) >= 16 * static_cast<int64_t>(b.count)) {
+        per = std::min<int64_t>(per, 2);
+    }
     const int64_t blocks = joins + heads * ((c.slots + per * kMassKeys - 1) / (per * kMassKeys));
     return by_dtype(a.dtype, [&](auto type) {
         using T = decltype(type);
