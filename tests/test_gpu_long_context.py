@@ -391,6 +391,18 @@ def test_weights_of_long_rows_are_split(ops):
     check_weights(ops, rng, "f32", "f32", 32, 1, 1, [3000])
 
 
+@pytest.mark.parametrize("heads,counts", [(8, None), (40, None), (8, [3] * 30), (8, [17] * 28 + [0, 40])])
+def test_weights_of_many_long_rows(ops, heads, counts):
+    """So many keys in all that a CTA adds up several chunks of them: some whole, some ragged, some behind the end."""
+    rng = np.random.default_rng(heads)
+    lengths = [4600, 1, 511, 512, 513, 0, 1024, 1025, 1536, 1537, 2600, 4097] + [40] * 17 + [2048]
+    if counts is not None:
+        lengths = [max(n, k) for n, k in zip(lengths, counts)]
+    check_weights(ops, rng, "u4", "f32", 32, heads, 8, lengths, counts=counts, decay=0.5, slots=4600)
+    check_weights(ops, rng, "u4", "f32", 32, heads, 8, lengths, counts=counts, decay=0.0, in_place=False, window=700,
+                  sinks=5, slots=4600)
+
+
 def test_weights_with_rows_named_twice_outside_and_too_long(ops):
     rng = np.random.default_rng(9)
     for storage in ("u4", "bf16"):
