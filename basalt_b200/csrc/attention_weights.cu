@@ -84,7 +84,7 @@ __device__ __forceinline__ void row_sums(const Cache& c, const AttnSpec& a, int 
 }
 
 // Joins splits, and turns scores into weights: 64 sequences of 500 to 8192 keys with 32 query heads take 15 us (36 MB
-// of scores, 18 of masses: 3.5 TB/s), eight of 1000 to 16 384 with 16 tokens each 37 (127 MB). Bound by how many scores
+// of scores, 18 of masses: 3.5 TB/s), eight of 1000 to 16 384 with 16 tokens each 31 (127 MB). Bound by how many scores
 // are under way: a thread's four rows of four keys, and the four after them.
 template <typename T, int HD, bool WARP>
 __global__ void __launch_bounds__(kThreads)
@@ -115,7 +115,7 @@ k_weights_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out,
         }
         return;
     }
-    __shared__ float tops[kMassRows], inverse[kMassRows];
+    __shared__ __align__(16) float tops[kMassRows], inverse[kMassRows];
     // In 32 bits: the quotients of 64 took a third of all instructions. A CTA has `per` chunks of keys.
     const uint32_t shares = (c.slots + per * kMassKeys - 1) / (per * kMassKeys), place = blockIdx.x;
     const uint32_t of_head = place / shares;
@@ -186,6 +186,7 @@ k_weights_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out,
         }
         return;
     }
+    const int64_t to_next = static_cast<int64_t>(a.heads - group) * pitch;  // behind a token's heads to the next's
     int known = -1;  // the sequence whose maxima and sums are held, all of them
     for (int chunk = 0; chunk < per; ++chunk) {
         const int key0 = begin + chunk * kMassKeys;
@@ -208,24 +209,24 @@ k_weights_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out,
             }
             const int all = n * group;
             // Scores of kBatch rows from r on; what lies beside the rows or what they see is read, not used.
-            int load_at = 0, load_head = 0;
-            const float* const rows_at = scores + (static_cast<int64_t>(first) * a.heads + kvh * group) * pitch + offset;
+            int load_left = all, load_head = 0;
+            const float* row_at = scores + (static_cast<int64_t>(first) * a.heads + kvh * group) * pitch + offset;
             auto load = [&](float4 (&x)[kBatch]) {
 #pragma unroll
                 for (int k = 0; k < kBatch; ++k) {
                     x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    if (load_at < n) {
-                        x[k] = __ldcs(reinterpret_cast<const float4*>(rows_at + (static_cast<int64_t>(load_at) * a.heads + load_head) * pitch));
-                    }
+                    if (load_left-- > 0) x[k] = __ldcs(reinterpret_cast<const float4*>(row_at));
+                    row_at += pitch;
                     if (++load_head == group) {
                         load_head = 0;
-                        ++load_at;
+                        row_at += to_next;
                     }
                 }
             };
+            // Whether all tokens see all of the chunk (one outside the cache sees nothing).
+            const bool whole = a.window == 0 && key0 + kMassKeys - 1 <= length - n && length <= c.slots;
             float4 x[kBatch];
             load(x);
-            int at = 0, head_of = 0;
             for (int r0 = 0; r0 < all; r0 += kMassRows) {
                 const int rows = min(kMassRows, all - r0);
                 if (known != seq) {
@@ -235,6 +236,22 @@ k_weights_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out,
                 for (int r = 0; r < rows; r += kBatch) {  // kMassRows are whole batches
                     float4 next[kBatch];
                     load(next);
+                    if (whole && r + kBatch <= rows) {
+                        const float4 top4 = *reinterpret_cast<const float4*>(tops + r);
+                        const float4 by4 = *reinterpret_cast<const float4*>(inverse + r);
+                        const float top[kBatch] = {top4.x, top4.y, top4.z, top4.w};
+                        const float by[kBatch] = {by4.x, by4.y, by4.z, by4.w};
+#pragma unroll
+                        for (int k = 0; k < kBatch; ++k) {
+                            const float s[N] = {x[k].x, x[k].y, x[k].z, x[k].w};
+#pragma unroll
+                            for (int i = 0; i < N; ++i) sum[i] = fmaf(exp2_fast(s[i] - top[k]), by[k], sum[i]);
+                            x[k] = next[k];
+                        }
+                        continue;
+                    }
+                    // The first of the rows' tokens and heads.
+                    int at = (r0 + r) / group, head_of = r0 + r - at * group;
 #pragma unroll
                     for (int k = 0; k < kBatch; ++k) {
                         if (r + k < rows) {
@@ -242,17 +259,13 @@ k_weights_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out,
                             const int p = length - n + at;
                             const float top = tops[r + k], by = inverse[r + k];
                             const float s[N] = {x[k].x, x[k].y, x[k].z, x[k].w};
-                            if (a.window == 0 && key0 + kMassKeys - 1 <= p && p < c.slots) {
 #pragma unroll
-                                for (int i = 0; i < N; ++i) sum[i] = fmaf(exp2_fast(s[i] - top), by, sum[i]);
-                            } else {
-#pragma unroll
-                                for (int i = 0; i < N; ++i) {
-                                    const int key = my_key + i;
-                                    const bool seen = key <= p && p < c.slots && (a.window == 0 || p - key < a.window || key < a.sinks);
-                                    const float more = fmaf(exp2_fast(s[i] - top), by, sum[i]);
-                                    sum[i] = seen ? more : sum[i];
-                                }
+                            for (int i = 0; i < N; ++i) {
+                                const int key = my_key + i;
+                                const bool seen =
+                                    key <= p && p < c.slots && (a.window == 0 || p - key < a.window || key < a.sinks);
+                                const float more = fmaf(exp2_fast(s[i] - top), by, sum[i]);
+                                sum[i] = seen ? more : sum[i];
                             }
                         }
                         if (++head_of == group) {
@@ -328,8 +341,8 @@ cudaError_t launch_attention_weights(cudaStream_t s, const Cache& c, const Batch
     const int64_t joins = warp ? (queries * (a.head_dim / 32) + kWarps - 1) / kWarps : queries;
     // Six CTAs an SM, each of whole chunks (one chunk a CTA: 35 instead of 20 us for 64 rows of up to 8192 keys).
     const int64_t heads = static_cast<int64_t>(b.count) * a.kv_heads, chunks = (c.slots + kMassKeys - 1) / kMassKeys;
-    // From 16 query rows a sequence on two chunks at most: eight sequences' 8 tokens of four heads over 16 384 keys take
-    // 183 us, with three 191, with one 185; four rows of 64 sequences, without this, 343 with nineteen and 352 with two.
+    // From 16 query rows a sequence on two chunks at most: eight sequences' 16 tokens of four heads over 16 384 keys take
+    // 231 us, with three 240, with one 237; four rows of 64 sequences, without this, 343 with nineteen, 352 with two.
     int64_t per = std::min(chunks, (heads * chunks + 148 * 6 - 1) / (148 * 6));
     if (static_cast<int64_t>(b.tokens) * (a.heads / a.kv_heads) >= 16 * static_cast<int64_t>(b.count)) {
         per = std::min<int64_t>(per, 2);
