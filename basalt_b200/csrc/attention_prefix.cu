@@ -682,6 +682,7 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
                     tmem_st16(o_at + 32 * c, o);
                     tmem_st16(o_at + 32 * c + 16, o + 16);
                 }
+                tmem_st_wait();  // a tile may rescale twice: the second time reads what the first has written
             };
             if (__any_sync(kFull, move)) {
                 float keep[G];

@@ -1,0 +1,66 @@
+"""Long-context operators where their pieces meet: masses in a place of their own, two host threads, tokens that
+see nothing, arguments that are tensors, tiles that move two scales at once, and errors by the outputs' norm."""
+import threading
+
+import numpy as np
+import pytest
+
+from test_gpu_long_context import filled, kept_places, raw, softmax
+from test_gpu_operators import host, ints, tensor, torch_
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops(runtime):
+    from basalt_b200 import operators
+
+    return operators
+
+
+def norm_error(got, want):
+    return np.linalg.norm(got - want) / np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("own", [False, True])
+def test_maxima_and_values_that_grow_in_the_same_tile(ops, dim, own):
+    """4-bit keys whose scores grow by about 2^12 from each tile of 64 to the next, and values by 2^3 at the same
+    keys: what was summed before is scaled for both (a factor that is lost leaves 2^-3 of the output and more). In
+    every third tile only one of them grows. Outputs are rounded to bf16: 2^-8 of each entry at most, and so of a
+    row's norm. Weights and values in fp16 add 2^-11 each, scores of up to 320 (base 2) that are good to 2^-20 another
+    3e-4; all are well within a second 2^-8."""
+    torch = torch_()
+    rng = np.random.default_rng(dim)
+    kv_heads, heads, tiles, tokens = 2, 16, 40, 20
+    n = 64 * tiles
+    k, v = rng.standard_normal((2, n, kv_heads, dim)).astype(np.float32) * np.float32([[[[0.1]]], [[[1.0]]]])
+    tile = np.arange(n) // 64
+    scores, values = np.cumsum(np.arange(tiles) % 3 != 1), np.cumsum(np.arange(tiles) % 3 != 2)
+    k[..., 0] = 8.0 * scores[tile, None] * (dim / 64) ** 0.5
+    v *= (2.0 ** (3.0 * values[tile]))[:, None, None].astype(np.float32)
+    cache, starts = ops.KvCache.allocate(1, kv_heads, n, dim), ints([0, n])
+    ops.kv_append(cache, tensor(k), tensor(v), ints([n]), starts=starts)
+    k, v = (host(t) for t in ops.kv_read(cache, ints([n]), starts=starts, tokens=n))
+    q = rng.standard_normal((tokens, heads, dim)).astype(np.float32)
+    q[..., 0] = 8.0
+    q = tensor(q, "bf16")
+    qh = host(q)
+    # Rows end in every part of the keys: the later ones see all the growth, the first ones little of it.
+    ends = [n - tokens] if own else [n, 64 * 9, 64 * 20 + 5, 64, 130]
+    for end in ends:
+        if own:
+            mass = torch.zeros((1, kv_heads, n), device="cuda")
+            got = host(ops.attention_weights(cache, q, ints([n]), mass, starts=ints([0, tokens])))
+            assert np.allclose(host(mass).sum(-1), tokens * heads // kv_heads, rtol=1e-4)
+        else:
+            empty = ops.KvCache.allocate(tokens, kv_heads, 4, dim)
+            got = host(ops.attention_shared(empty, q, ints([0] * tokens), cache, end))
+        for i in range(tokens):
+            stop = end + i + 1 if own else end
+            for h in range(heads):
+                at = h * kv_heads // heads
+                want = softmax(k[:stop, at] @ qh[i, h] * dim ** -0.5) @ v[:stop, at]
+                assert norm_error(got[i, h], want) <= 2 * 2.0 ** -8, (end, i, h)
+
+
