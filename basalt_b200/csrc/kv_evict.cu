@@ -284,7 +284,9 @@ k_evict_move(Cache c, Batch b, Eviction e, int row_units, int scale_units, int r
                                       i1, scale_units, 0, scale_units);
     }
     if (of_values || !first) return;
-    move_rows<float, IN_PLACE>(e.mass + from, e.to_mass + to, places, i0, i1, 0, 0, 0);
+    // In place too masses may go to another array, and then those of the keys that stay as well.
+    const int m0 = IN_PLACE && e.to_mass != e.mass ? 0 : i0;
+    move_rows<float, IN_PLACE>(e.mass + from, e.to_mass + to, places, m0, i1, 0, 0, 0);
     const int step = IN_PLACE ? kMove : shares * kMove;
     for (int i = kept + (IN_PLACE ? 0 : share * kMove) + threadIdx.x; i < e.to.slots; i += step) e.to_mass[to + i] = 0.0f;
 }

@@ -396,8 +396,8 @@ def kv_evict(cache: KvCache, mass, lengths, keep: int, recent: int = 0, sinks: i
     """Shrinks the sequences to ``keep`` keys in each key head: the first ``sinks``, the last ``recent`` and
     of the others those of the largest ``mass`` ([rows, kv_heads, slots] float32, as ``attention_weights``
     leaves it). They move in order to the first slots, in place, or to rows ``to_rows`` (s when omitted) of
-    the cache ``to`` with their masses in ``to_mass``; masses behind them become zero. Returns the new
-    lengths (int32) and the kept slots [count, kv_heads, keep] (int32, -1 behind the last; ``kept`` if
+    the cache ``to``. Their masses go to ``to_mass`` (in place ``mass`` itself by default); those behind them
+    become zero. Returns the new lengths (int32) and the kept slots [count, kv_heads, keep] (int32, -1 behind the last; ``kept`` if
     given)."""
     device = cache.device
     if stream is not None:

@@ -395,11 +395,12 @@ int32_t bst_attention_weights(int32_t device, void* stream, const bst_kv_cache* 
 /* Eviction: of a sequence with more than `keep` keys each key head keeps `keep`: the first `sinks`, the
  * last `recent`, and of the others those of the largest mass (float32 [rows][kv_heads][slots]; ties: the
  * lowest slot; NaN counts below all). They move in order to slots 0 .. keep - 1, and their masses with
- * them; shorter sequences keep all. With `to` NULL this happens in place (to_rows must be NULL, to_mass
- * may be mass); otherwise keys and values go to row to_rows[s] (s when NULL) of `to`, a cache of the same
- * storage, kv_heads and head_dim with keep slots or more that shares no memory with `cache`, which stays
- * as it was. Of to_mass ([rows][kv_heads][slots] of `to`) the slots behind the kept ones become 0, so
- * that tokens which are appended start from there; keys and values there stay as they were.
+ * them; shorter sequences keep all. With `to` NULL this happens in place (to_rows must be NULL; to_mass
+ * is mass, or shares nothing with it and gets the masses of all keys that are kept); otherwise keys and
+ * values go to row to_rows[s] (s when NULL) of `to`, a cache of the same storage, kv_heads and head_dim
+ * with keep slots or more that shares no memory with `cache`, which stays as it was. Of to_mass
+ * ([rows][kv_heads][slots] of `to`) the slots behind the kept ones become 0, so that tokens which are
+ * appended start from there; keys and values there stay as they were.
  * lengths_out[s] becomes the number of keys kept (min(lengths[s], keep)) and kept [count][kv_heads][keep]
  * the slots they had, in order, -1 behind the last. A sequence whose rows lie outside the caches, or
  * whose row to write an earlier sequence names too, keeps none: length 0, kept -1. 1 <= keep,

@@ -64,3 +64,31 @@ def test_maxima_and_values_that_grow_in_the_same_tile(ops, dim, own):
                 assert norm_error(got[i, h], want) <= 2 * 2.0 ** -8, (end, i, h)
 
 
+@pytest.mark.parametrize("storage,dim", [("u4", 32), ("u4", 128), ("bf16", 64), ("f32", 128)])
+@pytest.mark.parametrize("slots,keep,recent,sinks", [(90, 40, 7, 5), (90, 40, 0, 0), (9000, 4500, 900, 3)])
+def test_evicting_in_place_with_masses_elsewhere(ops, storage, dim, slots, keep, recent, sinks):
+    """The masses of every kept key arrive, of those too that stay in their slots; `mass` is left as it was."""
+    torch = torch_()
+    rng = np.random.default_rng(slots + keep)
+    lengths, rows = [slots, keep + 1, keep, keep - 1, 1, 0], [3, 0, 6, 2, 5, 1]
+    cache, _, _ = filled(ops, rng, 7, 2, slots, dim, storage)
+    before = raw(cache)
+    m = (rng.random((7, 2, slots)) ** 3).astype(np.float32)
+    m[3, 1] = np.sort(m[3, 1])[::-1]      # the first keys stay where they are
+    mass, to_mass = tensor(m), torch.full((7, 2, slots), 9.0, device="cuda")
+    new, kept = ops.kv_evict(cache, mass, ints(lengths), keep, recent, sinks, rows=ints(rows), to_mass=to_mass)
+    assert new.tolist() == [min(n, keep) for n in lengths]
+    assert np.array_equal(mass.cpu().numpy(), m)
+    want, kept = np.full_like(m, 9.0), kept.cpu().numpy()
+    for s, (row, n) in enumerate(zip(rows, lengths)):
+        want[row] = 0.0
+        for h in range(2):
+            places = kept_places(m[row, h], n, keep, recent, sinks)
+            assert kept[s, h, :len(places)].tolist() == places
+            want[row, h, :len(places)] = m[row, h, places]
+            for x, y in zip(raw(cache), before):
+                moved = y[row, h][torch.tensor(places, device="cuda", dtype=torch.long)]
+                assert torch.equal(x[row, h, :len(places)].view(torch.uint8), moved.view(torch.uint8))
+    assert np.array_equal(to_mass.cpu().numpy(), want)
+
+
