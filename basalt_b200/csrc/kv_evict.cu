@@ -297,7 +297,9 @@ cudaError_t choose(cudaStream_t s, const Cache& c, const Batch& b, const Evictio
     const int run = ((c.slots + CTAS * kChoose - 1) / (CTAS * kChoose)) | 1;
     const int held = static_cast<int64_t>(run) * kChoose <= kHeld ? run * kChoose : 0;
     if (held > 4096) {  // beside 24 KB of counts, more than a kernel has by itself
-        const cudaError_t err = cudaFuncSetAttribute(k_evict_choose<CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, held * 4);
+        // The limit is the kernel's, not the call's, so it is the same for all: one thread's call could lower it between
+        // another's and its launch.
+        const cudaError_t err = cudaFuncSetAttribute(k_evict_choose<CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeld * 4);
         if (err) return err;
     }
     cudaLaunchConfig_t cfg = {};

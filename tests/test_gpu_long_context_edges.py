@@ -92,3 +92,36 @@ def test_evicting_in_place_with_masses_elsewhere(ops, storage, dim, slots, keep,
     assert np.array_equal(to_mass.cpu().numpy(), want)
 
 
+@pytest.mark.parametrize("slots", [(8192, 5000), (30000, 20000)])
+def test_evictions_of_two_threads(ops, slots):
+    """Two host threads, each with a stream and a cache of its own, whose rows need different room in shared memory."""
+    torch = torch_()
+    failed = []
+
+    def serve(n, results):
+        try:
+            g = torch.Generator(device="cuda").manual_seed(n)
+            stream = torch.cuda.Stream()
+            cache = ops.KvCache.allocate(1, 1, n, 32)
+            to, to_mass = ops.KvCache.allocate(1, 1, 64, 32), torch.zeros((1, 1, 64), device="cuda")
+            mass = torch.rand((1, 1, n), generator=g, device="cuda")
+            lengths, kept = ints([n]), torch.empty((1, 1, 64), dtype=torch.int32, device="cuda")
+            torch.cuda.synchronize()
+            for _ in range(4000):
+                ops.kv_evict(cache, mass, lengths, 64, 8, 4, to=to, to_mass=to_mass, kept=kept, stream=stream)
+            stream.synchronize()
+            results[n] = kept[0, 0].tolist()
+            assert results[n] == kept_places(mass[0, 0].cpu().numpy(), n, 64, 8, 4)
+        except Exception as e:  # noqa: BLE001 - the thread's failure is the test's
+            failed.append(e)
+
+    results = {}
+    threads = [threading.Thread(target=serve, args=(n, results)) for n in slots]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    assert len(results) == 2
+
+
