@@ -606,7 +606,7 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
         const uint32_t s_at = tmem + half * 256 + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
         const uint32_t o_at = s_at + 128;
         // A score's factor to base 2. It stays above zero: the mask's -infinity is multiplied by it.
-        const float scale = fabsf(a.scale) * kLog2e * (CODES ? row_factor[at] : 1.0f);
+        float scale = fabsf(a.scale) * kLog2e * (CODES ? row_factor[at] : 1.0f);
         constexpr int G = HD / 32;
         float top = -INFINITY, total = 0.0f, values_by[G];
 #pragma unroll
@@ -620,6 +620,7 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
             place(at, &token, &head);
             const int position = position0 + static_cast<int>(token - first);
             sees = at < rows && position < prefix.cache.slots ? position + 1 : 0;
+            if (sees <= 0) scale = 0.0f;  // nothing of a query that sees nothing counts, its NaN neither
             if (at < rows) kept = scores + (token * a.heads + head) * pitch;
         }
         // A wait that runs out ends no loop here: the tile's threads meet at a barrier behind it, and

@@ -125,3 +125,25 @@ def test_evictions_of_two_threads(ops, slots):
     assert len(results) == 2
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("slots", [300, 2100])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_tokens_that_see_nothing_give_zeros_whatever_they_hold(ops, dim, slots, bad):
+    """Tokens before the row's first key and behind its last slot, in tiles of which other tokens see keys."""
+    torch = torch_()
+    rng = np.random.default_rng(dim)
+    cache, _, _ = filled(ops, rng, 3, 2, slots, dim, "u4")
+    lengths, n = [3, slots + 20, 100], 40
+    q = torch.randn((3 * n, 8, dim), device="cuda").bfloat16()
+    blind = np.zeros(3 * n, bool)
+    blind[:n - 3] = blind[2 * n - 20:2 * n] = True
+    q[torch.from_numpy(np.flatnonzero(blind)[::2]).cuda()] = bad
+    mass = torch.zeros((3, 2, slots), device="cuda")
+    out = host(ops.attention_weights(cache, q, ints(lengths), mass, starts=ints(np.arange(4) * n)))
+    assert np.all(out[blind] == 0)
+    assert np.isfinite(out).all() and np.all(np.abs(out[~blind]).max((1, 2)) > 0)
+    # Every token that sees keys gives each key head four times a weight of one in all.
+    got = host(mass)
+    assert np.allclose(got.sum(-1), np.array([[3], [20], [40]]) * 4, rtol=1e-4)
+
+
