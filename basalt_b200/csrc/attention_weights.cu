@@ -352,11 +352,18 @@ cudaError_t launch_attention_weights(cudaStream_t s, const Cache& c, const Batch
         using T = decltype(type);
         return by_head_dim(a.head_dim, [&](auto hd) {
             constexpr int HD = decltype(hd)::value;
-            return launch_pdl(warp ? k_weights_join<T, HD, true> : k_weights_join<T, HD, false>,
-                              dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, s, c, b, a, rows,
-                              static_cast<T*>(out), out_stride, splits, static_cast<const float*>(part),
-                              static_cast<const float*>(extra.scores), extra.pitch, previous, decay, mass,
-                              static_cast<int>(joins), static_cast<int>(per));
+            const auto kernel = warp ? k_weights_join<T, HD, true> : k_weights_join<T, HD, false>;
+            const dim3 grid(static_cast<unsigned>(blocks));
+            auto launch = [&](auto... args) {
+                if (b.tokens > 0) return launch_pdl(kernel, grid, dim3(kThreads), 0, s, args...);
+                // Without a pass before it the kernel stands behind the caller's own, which may write `rows`, read here
+                // before the wait.
+                kernel<<<grid, kThreads, 0, s>>>(args...);
+                return cudaGetLastError();
+            };
+            return launch(c, b, a, rows, static_cast<T*>(out), out_stride, splits, static_cast<const float*>(part),
+                          static_cast<const float*>(extra.scores), extra.pitch, previous, decay, mass,
+                          static_cast<int>(joins), static_cast<int>(per));
         });
     });
 }

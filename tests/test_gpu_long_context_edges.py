@@ -147,3 +147,25 @@ def test_tokens_that_see_nothing_give_zeros_whatever_they_hold(ops, dim, slots, 
     assert np.allclose(got.sum(-1), np.array([[3], [20], [40]]) * 4, rtol=1e-4)
 
 
+def test_rows_without_tokens_fade_where_a_kernel_before_says(ops):
+    """`rows` and `lengths` are written on the stream right before the call."""
+    torch = torch_()
+    cache = ops.KvCache.allocate(64, 2, 700, 64)
+    q, starts = torch.zeros((0, 4, 64), device="cuda"), torch.zeros(33, dtype=torch.int32, device="cuda")
+    rows, lengths = (torch.empty(32, dtype=torch.int32, device="cuda") for _ in range(2))
+    g = torch.Generator(device="cuda").manual_seed(1)
+    mass = torch.rand((64, 2, 700), generator=g, device="cuda")
+    for _ in range(50):
+        want, order = mass.clone(), torch.randperm(64, generator=g, device="cuda")[:32]
+        n = torch.randint(0, 701, (32,), generator=g, device="cuda")
+        faded = torch.arange(700, device="cuda") < n[:, None, None]
+        want[order] = torch.where(faded, want[order] * 0.5, want[order])
+        rows.zero_()
+        lengths.zero_()
+        torch.cuda._sleep(20000)
+        rows.copy_(order)
+        lengths.copy_(n)
+        ops.attention_weights(cache, q, lengths, mass, decay=0.5, starts=starts, rows=rows)
+        assert torch.equal(mass, want)
+
+
