@@ -117,9 +117,10 @@ k_weights_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out,
     }
     __shared__ __align__(16) float tops[kMassRows], inverse[kMassRows];
     // In 32 bits: the quotients of 64 took a third of all instructions. A CTA has `per` chunks of keys.
-    const uint32_t shares = (c.slots + per * kMassKeys - 1) / (per * kMassKeys), place = blockIdx.x;
+    const int span = per * kMassKeys;
+    const uint32_t shares = 1 + (c.slots - 1) / span, place = blockIdx.x;  // slots and a span may pass 2^31
     const uint32_t of_head = place / shares;
-    const int begin = static_cast<int>(place - of_head * shares) * per * kMassKeys;
+    const int begin = static_cast<int>(place - of_head * shares) * span;
     const int first_seq = of_head / static_cast<uint32_t>(a.kv_heads);
     const int kvh = of_head - static_cast<uint32_t>(first_seq) * a.kv_heads;
     const int row = b.rows ? __ldg(b.rows + first_seq) : first_seq;
@@ -135,7 +136,7 @@ k_weights_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out,
     // by the general loop below).
     const int only = b.rows ? next_of_row(b, first_seq, row) : b.count;
     if (only == b.count && !b.starts && group <= kBatch) {
-        const int length = max(0, __ldg(b.lengths + first_seq)), stop = min(min(length, c.slots), begin + per * kMassKeys);
+        const int length = max(0, __ldg(b.lengths + first_seq)), stop = min(min(length, c.slots), begin + min(span, c.slots - begin));
         if (stop <= begin) return;
         row_sums<HD>(c, a, tile_rows, splits, part, row, length, first_seq, 1, kvh, 0, group, tops, inverse);
         float top[kBatch], by[kBatch];

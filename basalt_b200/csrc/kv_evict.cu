@@ -264,7 +264,7 @@ k_evict_move(Cache c, Batch b, Eviction e, int row_units, int scale_units, int r
     if (IN_PLACE) {
         // Keys before the first one that went stay where they are.
         for (int hi = kept; i0 < hi;) {
-            const int mid = (i0 + hi) >> 1;
+            const int mid = i0 + ((hi - i0) >> 1);
             if (places[mid] == mid) {
                 i0 = mid + 1;
             } else {
@@ -287,8 +287,10 @@ k_evict_move(Cache c, Batch b, Eviction e, int row_units, int scale_units, int r
     // In place too masses may go to another array, and then those of the keys that stay as well.
     const int m0 = IN_PLACE && e.to_mass != e.mass ? 0 : i0;
     move_rows<float, IN_PLACE>(e.mass + from, e.to_mass + to, places, m0, i1, 0, 0, 0);
-    const int step = IN_PLACE ? kMove : shares * kMove;
-    for (int i = kept + (IN_PLACE ? 0 : share * kMove) + threadIdx.x; i < e.to.slots; i += step) e.to_mass[to + i] = 0.0f;
+    const int64_t step = IN_PLACE ? kMove : static_cast<int64_t>(shares) * kMove;
+    for (int64_t i = kept + (IN_PLACE ? 0 : static_cast<int64_t>(share) * kMove) + threadIdx.x; i < e.to.slots; i += step) {
+        e.to_mass[to + i] = 0.0f;
+    }
 }
 
 template <int CTAS>

@@ -169,3 +169,45 @@ def test_rows_without_tokens_fade_where_a_kernel_before_says(ops):
         assert torch.equal(mass, want)
 
 
+def test_a_row_of_nearly_2_31_slots(ops):
+    """Places and strides near the end of 32 bits: eviction into such a row and within it, weights of all its keys."""
+    torch = torch_()
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 125 << 30:
+        pytest.skip("needs 125 GB of free memory")
+    n = 2 ** 31 - 65537
+    row = ops.KvCache.allocate(1, 1, n, 32)
+    mass = torch.full((1, 1, n), 9.0, device="cuda")
+
+    def others(low, high, but=0):   # all masses but the last `but` lie in [low, high]
+        rest = mass[0, 0, :n - but]
+        return low <= float(rest.min()) and float(rest.max()) <= high
+
+    # 1000 keys move into it: masses behind them become zero up to the last.
+    few = ops.KvCache.allocate(1, 1, 1000, 32)
+    new, kept = ops.kv_evict(few, torch.ones((1, 1, 1000), device="cuda"), ints([1000]), 600000, to=row, to_mass=mass)
+    assert new.tolist() == [1000] and (mass[0, 0, :1000] == 1).all()
+    mass[0, 0, :1000] = 0.0
+    assert others(0.0, 0.0)
+    del kept
+    # All keys but the last are alike; that one weighs about as much as the others together.
+    row.k_scale[0, 0, n - 1, 0, 1] = 3.796875
+    row.v_scale[0, 0, n - 1, 0, 1] = 1.0
+    q, e = torch.ones((1, 1, 32), device="cuda"), float(np.exp(32 * 3.796875 * 32 ** -0.5))
+    for starts in (None, ints([0, 1])):
+        mass.fill_(9.0)
+        out = host(ops.attention_weights(row, q, ints([n]), mass, decay=0.0, starts=starts))
+        last, rest = e / (e + n - 1), 1.0 / (e + n - 1)
+        assert np.allclose(out, last, rtol=1e-4, atol=0)
+        assert abs(float(mass[0, 0, n - 1]) / last - 1) < 1e-4 and others(rest * (1 - 1e-4), rest * (1 + 1e-4), 1)
+    # In place, ties: the last five go.
+    mass.fill_(0.5)
+    new, kept = ops.kv_evict(row, mass, ints([n]), n - 5)
+    assert new.tolist() == [n - 5] and (mass[0, 0, n - 5:] == 0).all() and others(0.5, 0.5, 5)
+    for at in range(0, n - 5, 1 << 27):
+        some = kept[0, 0, at:at + (1 << 27)]
+        assert torch.equal(some, torch.arange(at, at + some.shape[0], dtype=torch.int32, device="cuda"))
+    del row, mass, kept
+    torch.cuda.empty_cache()
+
+
