@@ -191,7 +191,8 @@ class KvCache:
 def _sequences(device, tokens, lengths, starts, rows):
     """The batch's struct; the tensors it points to belong to the caller."""
     if starts is None and rows is None and lengths is not None:
-        return _lib.SequencesStruct(lengths.shape[0], tokens, None, None, _index(device, "lengths", lengths))
+        at = _index(device, "lengths", lengths)
+        return _lib.SequencesStruct(lengths.shape[0], tokens, None, None, at)
     if lengths is not None:
         at = _index(device, "lengths", lengths)
         count = lengths.shape[0]
@@ -328,7 +329,7 @@ def attention_shared(cache: KvCache, q, lengths, prefix: KvCache, prefix_length:
     s = _sequences(device, q.shape[0], lengths, starts, rows)
     prefix_row, prefix_length = _lib.int32(prefix_row), _lib.int32(prefix_length)
     lib = _lib.load()
-    key = (lengths.shape[0], q.shape[0], starts is None, q.shape[1], q.dtype, scale, prefix._shape, prefix_length)
+    key = (s.count, s.tokens, starts is None, q.shape[1], q.dtype, scale, prefix._shape, prefix_length)
     plan = cache._sizes.get(key)
     if plan is None:
         a = _spec(q, cache.kv_heads, 0, 0, scale)
@@ -374,7 +375,7 @@ def attention_weights(cache: KvCache, q, lengths, mass, previous=None, decay: fl
     out, out_stride = _out(device, q, out, stream)
     s = _sequences(device, q.shape[0], lengths, starts, rows)
     lib = _lib.load()
-    key = (lengths.shape[0], q.shape[0], starts is None, q.shape[1], q.dtype, scale, window, sinks, "weights")
+    key = (s.count, s.tokens, starts is None, q.shape[1], q.dtype, scale, window, sinks, "weights")
     plan = cache._sizes.get(key)
     if plan is None:
         a = _spec(q, cache.kv_heads, window, sinks, scale)
@@ -410,6 +411,8 @@ def kv_evict(cache: KvCache, mass, lengths, keep: int, recent: int = 0, sinks: i
     if to is not None and to_mass is None:
         raise IllegalArgumentException("to_mass must be given beside to", _lib.BST_INVALID)
     to_at = at if to_mass is None else _mass(device, "to_mass", to_mass, target)
+    if _index(device, "lengths", lengths) is None:
+        raise IllegalArgumentException("lengths must be given", _lib.BST_INVALID)
     s = _sequences(device, lengths.shape[0], lengths, None, rows)
     if not 1 <= keep <= target.slots:  # before memory is taken for it
         raise BasaltShapeException(f"keep is {keep}, the cache that is written has {target.slots} slots",

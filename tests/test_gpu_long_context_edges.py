@@ -211,3 +211,19 @@ def test_a_row_of_nearly_2_31_slots(ops):
     torch.cuda.empty_cache()
 
 
+def test_lengths_must_be_a_vector(ops):
+    from basalt_b200.text_engine import IllegalArgumentException
+
+    torch = torch_()
+    cache = ops.KvCache.allocate(1, 2, 20, 64)
+    q, mass = torch.zeros((1, 4, 64), device="cuda"), torch.zeros((1, 2, 20), device="cuda")
+    one = torch.tensor(5, dtype=torch.int32, device="cuda")
+    for call in (lambda: ops.attention_cached(cache, q, one), lambda: ops.attention_shared(cache, q, one, cache, 3),
+                 lambda: ops.attention_weights(cache, q, one, mass), lambda: ops.kv_evict(cache, mass, one, 3),
+                 lambda: ops.kv_append(cache, q[:, :2], q[:, :2], one), lambda: ops.kv_read(cache, one, tokens=1)):
+        with pytest.raises(IllegalArgumentException, match="lengths"):
+            call()
+    for call in (lambda: ops.attention_cached(cache, q, None), lambda: ops.attention_shared(cache, q, None, cache, 3),
+                 lambda: ops.attention_weights(cache, q, None, mass), lambda: ops.kv_evict(cache, mass, None, 3)):
+        with pytest.raises(IllegalArgumentException):
+            call()
