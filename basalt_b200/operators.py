@@ -300,7 +300,7 @@ def attention_cached(cache: KvCache, q, lengths, starts=None, rows=None, window:
     s = _sequences(device, q.shape[0], lengths, starts, rows)
     a = _spec(q, cache.kv_heads, window, sinks, scale)
     lib = _lib.load()
-    key = (s.count, s.tokens, starts is None, a.heads, a.dtype, window, sinks)
+    key = (s.count, s.tokens, starts is None, a.heads, a.dtype, a.window, a.sinks)
     needed = cache._sizes.get(key)
     if needed is None:
         size = ctypes.c_int64(0)
@@ -328,6 +328,8 @@ def attention_shared(cache: KvCache, q, lengths, prefix: KvCache, prefix_length:
     out, out_stride = _out(device, q, out, stream)
     s = _sequences(device, q.shape[0], lengths, starts, rows)
     prefix_row, prefix_length = _lib.int32(prefix_row), _lib.int32(prefix_length)
+    if scale is not None:
+        scale = float(scale)  # plans are kept by numbers, not by tensors that hold them now
     lib = _lib.load()
     key = (s.count, s.tokens, starts is None, q.shape[1], q.dtype, scale, prefix._shape, prefix_length)
     plan = cache._sizes.get(key)
@@ -374,6 +376,10 @@ def attention_weights(cache: KvCache, q, lengths, mass, previous=None, decay: fl
     q_stride = _packed(device, "q", q, None, cache.head_dim)
     out, out_stride = _out(device, q, out, stream)
     s = _sequences(device, q.shape[0], lengths, starts, rows)
+    if type(window) is not int or type(sinks) is not int:
+        window, sinks = _lib.int32(window), _lib.int32(sinks)
+    if scale is not None:
+        scale = float(scale)  # plans are kept by numbers, not by tensors that hold them now
     lib = _lib.load()
     key = (s.count, s.tokens, starts is None, q.shape[1], q.dtype, scale, window, sinks, "weights")
     plan = cache._sizes.get(key)

@@ -211,6 +211,29 @@ def test_a_row_of_nearly_2_31_slots(ops):
     torch.cuda.empty_cache()
 
 
+def test_arguments_that_are_tensors_count_as_they_are_now(ops):
+    """A scale, window or number of sinks in a tensor that is filled anew between calls."""
+    torch = torch_()
+    rng = np.random.default_rng(2)
+    cache, _, _ = filled(ops, rng, 2, 2, 3000, 64, "bf16")
+    common, _, _ = filled(ops, rng, 1, 2, 60, 64, "bf16")
+    q = torch.randn((2, 4, 64), device="cuda").bfloat16()
+    lengths, scale, window, sinks = ints([3000, 2999]), torch.tensor(0.25), torch.tensor(3), torch.tensor(2)
+
+    def calls(scale, window, sinks):
+        mass = torch.zeros((2, 2, 3000), device="cuda")
+        weighed = ops.attention_weights(cache, q, lengths, mass, scale=scale, window=window, sinks=sinks)
+        return (ops.attention_shared(cache, q, lengths, common, 60, scale=scale), weighed, mass,
+                ops.attention_cached(cache, q, lengths, scale=scale, window=window, sinks=sinks))
+
+    for s, w, n in ((0.25, 3, 2), (0.0625, 3000, 0), (1.0, 700, 41)):
+        scale.fill_(s)
+        window.fill_(w)
+        sinks.fill_(n)
+        for x, y in zip(calls(scale, window, sinks), calls(s, w, n)):
+            assert torch.equal(x, y)
+
+
 def test_lengths_must_be_a_vector(ops):
     from basalt_b200.text_engine import IllegalArgumentException
 
