@@ -250,3 +250,76 @@ def test_lengths_must_be_a_vector(ops):
                  lambda: ops.attention_weights(cache, q, None, mass), lambda: ops.kv_evict(cache, mass, None, 3)):
         with pytest.raises(IllegalArgumentException):
             call()
+
+
+# ---- errors by the outputs' norm ---------------------------------------------------------------------
+# Rounding x to bf16 moves it by up to 2^-8 of the power of two below it, uniformly: 2^-8 / sqrt 3 of x in the root mean
+# square, or less. Weights in 8 bits do the same to each term of a sum of values without a common part, and so to the
+# sum's norm. 11 bits (weights times values or steps, and values of 4-bit codes) are 2^-11 / sqrt 3 each. Independent
+# errors add up by squares. A single row of 64 entries and more stays within twice its share.
+ROUNDED, FP16 = 2.0 ** -8 / 3 ** 0.5, 2.0 ** -11 / 3 ** 0.5
+BITS = {8: (2 * ROUNDED ** 2) ** 0.5, 11: (ROUNDED ** 2 + 2 * FP16 ** 2) ** 0.5, 16: ROUNDED * (1 + 2.0 ** -8)}
+
+
+def check_norms(got, want, limit):
+    """All rows together, and each of them."""
+    off, size = np.linalg.norm(got - want, axis=-1), np.linalg.norm(want, axis=-1)
+    assert np.linalg.norm(off) <= limit * np.linalg.norm(size), np.linalg.norm(off) / np.linalg.norm(size)
+    assert np.all(off <= 2 * limit * size), (off / size).max()
+
+
+@pytest.mark.parametrize("dim,prefix", [(64, 5001), (128, 9000), (128, 40003)])
+@pytest.mark.parametrize("storage,rows,bits", [
+    ("bf16", 4, 16), ("bf16", 8, 16), ("bf16", 200, 8), ("bf16", 700, 8),   # on tcgen05 weights are bf16
+    ("u4", 4, 11), ("u4", 24, 11), ("u4", 200, 11), ("u4", 700, 11)])
+def test_bf16_outputs_behind_a_prefix_by_their_norm(ops, storage, rows, bits, dim, prefix):
+    """`rows` queries of each of two key heads behind one long prefix."""
+    torch = torch_()
+    g = torch.Generator(device="cuda").manual_seed(prefix + rows)
+    heads = 8 if rows >= 8 else 4
+    count = 2 * rows // heads
+    common = ops.KvCache.allocate(1, 2, prefix, dim, storage)
+    x = torch.randn((2, prefix, 2, dim), generator=g, device="cuda")
+    x[0] += 2 * torch.randn((1, 2, dim), generator=g, device="cuda") * (torch.rand((1, 2, dim), generator=g, device="cuda") < 0.1)
+    starts = ints([0, prefix])
+    ops.kv_append(common, x[0], x[1], ints([prefix]), starts=starts)
+    k, v = (t.double() for t in ops.kv_read(common, ints([prefix]), starts=starts, tokens=prefix))
+    own = ops.KvCache.allocate(count, 2, 4, dim, storage)
+    q = torch.randn((count, heads, dim), generator=g, device="cuda").bfloat16()
+    got = host(ops.attention_shared(own, q, ints([0] * count), common, prefix))
+    score = torch.einsum("shgd,jhd->shgj", q.double().unflatten(1, (2, -1)), k) * dim ** -0.5
+    want = torch.einsum("shgj,jhd->shgd", torch.softmax(score, -1), v).flatten(1, 2)
+    check_norms(got, host(want), BITS[bits])
+
+
+@pytest.mark.parametrize("storage,dim,heads,tokens,bits", [
+    ("u4", 128, 8, 1, 11), ("u4", 64, 8, 1, 11), ("u4", 128, 2, 1, 16), ("u4", 128, 8, 16, 11), ("u4", 64, 16, 40, 11),
+    ("bf16", 128, 8, 1, 16), ("bf16", 64, 2, 1, 16)])
+def test_bf16_outputs_and_masses_of_weights_by_their_norm(ops, storage, dim, heads, tokens, bits):
+    """The last tokens of long rows, of two key heads. Masses are float32: a score is good to 2^-20 of the sum of its
+    products' sizes, and the exponential and the sums to 2^-20 of a weight."""
+    torch = torch_()
+    g = torch.Generator(device="cuda").manual_seed(dim + heads + tokens)
+    n, rows = 6007, 3
+    cache = ops.KvCache.allocate(rows, 2, n, dim, storage)
+    x = torch.randn((2, rows * n, 2, dim), generator=g, device="cuda")
+    starts, lengths = ints(np.arange(rows + 1) * n), ints([n] * rows)
+    if storage == "u4":
+        ops.kv_append(cache, x[0], x[1], lengths, starts=starts)
+        k, v = (t.double().unflatten(0, (rows, n)) for t in ops.kv_read(cache, lengths, starts=starts, tokens=rows * n))
+    else:
+        for t, y in zip((cache.k, cache.v), x):
+            t.copy_(y.unflatten(0, (rows, n)).transpose(1, 2))
+        k, v = (t.double().transpose(1, 2) for t in (cache.k, cache.v))
+    q = torch.randn((rows * tokens, heads, dim), generator=g, device="cuda").bfloat16()
+    mass = torch.zeros((rows, 2, n), device="cuda")
+    got = host(ops.attention_weights(cache, q, lengths, mass, decay=0.0,
+                                     starts=None if tokens == 1 else ints(np.arange(rows + 1) * tokens)))
+    qh = q.double().unflatten(0, (rows, tokens)).unflatten(2, (2, -1))      # [rows, tokens, 2, group, dim]
+    score = torch.einsum("stgad,sjgd->stgaj", qh, k) * dim ** -0.5
+    size = float(torch.einsum("stgad,sjgd->stgaj", qh.abs(), k.abs()).max()) * dim ** -0.5
+    hidden = torch.arange(n, device="cuda") > torch.arange(n - tokens, n, device="cuda")[:, None]
+    p = torch.softmax(score.masked_fill(hidden[:, None, None], -np.inf), -1)
+    want = torch.einsum("stgaj,sjgd->stgad", p, v).flatten(0, 1).flatten(1, 2)
+    check_norms(got, host(want), BITS[bits])
+    check_norms(host(mass), host(p.sum((1, 3))), 2.0 ** -20 * (size + 1))
