@@ -5,7 +5,7 @@
 //
 // Two kernels. The first finds a head's border, the mass that the last kept key has, by counting 11, 11 and
 // 10 bits of the masses' ordered bits at a time, then writes the kept slots in order. A head is one CTA, or,
-// where it has more than kSegment slots, a cluster of up to eight that add up their counts through one
+// where rows are long and heads few, a cluster of up to eight that add up their counts through one
 // another's shared memory. Bound by the latency of its few steps: masses are read once, into shared memory. 32
 // sequences of 900 to 8192 keys of eight heads take 18 us, one of 131 000 23 (its 64 CTAs have 64 of the SMs).
 // The second moves keys, values and masses: bound by memory, every kept byte is read and written once. 32 x 1024
@@ -51,7 +51,6 @@ __device__ __forceinline__ Route route_of(const Cache& c, const Batch& b, const 
 template <int CTAS>
 constexpr int kChooseThreads = CTAS > 1 ? 1024 : 512;
 constexpr int kBins = 2048;
-constexpr int kSegment = 8192;         // slots from which on a head has more CTAs than one
 constexpr int kHeld = 40960;           // masses that a CTA's shared memory holds
 
 // Masses in the order of whole numbers: NaN below all, -0 as 0.
@@ -318,6 +317,18 @@ cudaError_t choose(cudaStream_t s, const Cache& c, const Batch& b, const Evictio
     return cudaLaunchKernelEx(&cfg, k_evict_choose<CTAS>, c, b, e, held);
 }
 
+// CTAs a head, so that long rows get several and many heads leave one another the card (a cluster of eight with 1024
+// threads each has an SM a CTA, and twelve such clusters fit). Calls of 1, 64 and 256 heads with one, two, four and eight
+// CTAs each (us): 8192 slots 16 15 16 18, 16 16 23 75, 27 44 74 253; 16 384 slots 23 18 19 21, 26 21 29 83, 47 62 96 286;
+// 40 000 slots 40 25 22 22, 50 35 45 100, 137 126 156 368; 131 072 slots 207 77 35 29, 270 126 107 164, 691 453 443 610.
+int ctas_of(int64_t heads, int slots) {
+    if (slots > 40960 && heads <= 12) return 8;
+    if (slots > 16384 && heads <= 32) return 4;
+    if (slots > 98304) return 4;
+    // Fewer heads than a wave, or masses that one CTA could hardly keep in shared memory.
+    return (slots > 8192 && heads <= 64) || slots > 32768 ? 2 : 1;
+}
+
 int log2_of(int x) {
     int n = 0;
     while (x >>= 1) ++n;
@@ -328,10 +339,11 @@ int log2_of(int x) {
 
 cudaError_t launch_kv_evict(cudaStream_t s, const Cache& c, const Batch& b, const Eviction& e) {
     if (b.count < 1) return cudaSuccess;
-    const cudaError_t err = c.slots <= kSegment       ? choose<1>(s, c, b, e)
-                            : c.slots <= 2 * kSegment ? choose<2>(s, c, b, e)
-                            : c.slots <= 4 * kSegment ? choose<4>(s, c, b, e)
-                                                      : choose<8>(s, c, b, e);
+    const int ctas = ctas_of(static_cast<int64_t>(c.kv_heads) * b.count, c.slots);
+    const cudaError_t err = ctas == 1   ? choose<1>(s, c, b, e)
+                            : ctas == 2 ? choose<2>(s, c, b, e)
+                            : ctas == 4 ? choose<4>(s, c, b, e)
+                                        : choose<8>(s, c, b, e);
     if (err) return err;
     const bool u4 = c.storage == BST_DTYPE_U4, in_place = e.to.k == c.k;
     const int row_bytes = u4 ? c.head_dim / 2 : c.head_dim * (c.storage == BST_DTYPE_BF16 ? 2 : 4);

@@ -252,6 +252,28 @@ def test_lengths_must_be_a_vector(ops):
             call()
 
 
+@pytest.mark.parametrize("slots", [8192, 8193, 16385, 32769, 40961, 98305])
+@pytest.mark.parametrize("kv_heads,count", [(1, 1), (13, 1), (3, 11), (5, 13)])
+def test_evictions_of_few_and_many_heads(ops, slots, kv_heads, count):
+    """The clusters of few heads with long rows, and the CTAs that many heads leave one another, around every border."""
+    torch = torch_()
+    g = torch.Generator(device="cuda").manual_seed(slots + kv_heads)
+    keep, recent, sinks = 700, 50, 3
+    cache = ops.KvCache.allocate(count, kv_heads, slots, 32)
+    to, to_mass = ops.KvCache.allocate(count, kv_heads, keep, 32), torch.empty((count, kv_heads, keep), device="cuda")
+    mass = torch.rand((count, kv_heads, slots), generator=g, device="cuda")
+    mass[:, :, ::3] = 0.75     # ties, some of which stay
+    lengths = torch.randint(slots // 2, slots + 1, (count,), generator=g, device="cuda", dtype=torch.int32)
+    lengths[0] = slots
+    new, kept = ops.kv_evict(cache, mass, lengths, keep, recent, sinks, to=to, to_mass=to_mass)
+    n = lengths.long()[:, None, None]
+    j = torch.arange(slots, device="cuda")
+    worth = mass.masked_fill((j < sinks) | (j >= n - recent), float("inf")).masked_fill(j >= n, -float("inf"))
+    want = torch.sort(worth, dim=-1, descending=True, stable=True).indices[..., :keep].sort(-1).values
+    assert (new == keep).all() and torch.equal(kept.long(), want)
+    assert torch.equal(to_mass, mass.gather(2, want))
+
+
 # ---- errors by the outputs' norm ---------------------------------------------------------------------
 # Rounding x to bf16 moves it by up to 2^-8 of the power of two below it, uniformly: 2^-8 / sqrt 3 of x in the root mean
 # square, or less. Weights in 8 bits do the same to each term of a sum of values without a common part, and so to the
