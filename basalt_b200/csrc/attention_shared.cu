@@ -48,15 +48,28 @@ Plan plan_large(const Batch& b, const AttnSpec& a, const Prefix& p) {
     return plan;
 }
 
-// Rows of a key head from which on tcgen05's tiles of 128 pay, however few of them are filled. Whole calls, eight key
-// heads of 128, tcgen05 and mma.sync (us): bf16 behind 500 keys 10.1 and 10.9 with 8 rows, 10.5 and 13.4 with 12; behind
-// 4000 14.6 and 18.1, 14.8 and 21.0; behind 30 000 32.7 and 36.3, 33.4 and 39.7. 4 bits, which take longer to unpack
-// for tcgen05, behind 500 keys 16.3 and 17.0 with 16 rows, 17.4 and 17.2 with 32, 18.5 and 18.7 with 64; behind 30 000
-// 46.5 and 37.6, 47.8 and 49.7, 52.8 and 76.1. (Of 64 channels behind 30 000 keys bf16 gains from 48 rows on: 32 and 39.)
-constexpr int kLargeRows = 12, kLargeCodeRows = 32;
+// Rows of a key head from which on tcgen05's tiles of 128 pay, however few of them are filled. Whole calls with own keys
+// of 10 to 120, eight key heads, tcgen05 and mma.sync (us).
+// bf16 of 128 channels: behind 500 keys 9.8 and 10.6 with 8 rows, 10.2 and 13.1 with 12; behind 4000 14.5 and 17.5, 14.9
+// and 20.6; behind 30 000 33.9 and 34.4, 33.9 and 38.5. Of 64 channels: behind 4000 keys 13.7 and 18.6 with 12 rows, behind
+// 16 000 21.2 and 21.2; but where every SM has more than 1000 keys, one CTA's chain of tiles takes longer than four small
+// CTAs beside one another: behind 30 000 29.6 and 24.0 with 12, 31.3 and 29.1 with 32, 33.1 and 38.9 with 48 (six key heads 28.5 and 30.0 with
+// 40; two heads behind 120 000, whose small CTAs leave too many splits to join, 32.1 and 35.2 with 12).
+// 4 bits, which take longer to unpack for tcgen05: of 128 channels behind 500 keys 17.9 and 16.9 with 32 rows, 18.6 and 18.4
+// with 64, 18.9 and 20.8 with 96; behind 1500 20.5 and 20.1, 20.5 and 21.1 with 40; behind 16 000 40.3 and 38.6, 40.7 and
+// 45.0 with 48; behind 30 000 (four heads) 40.0 and 38.2, 40.0 and 42.5. Of 64 behind 1000 16.2 and 12.2, 17.7 and 14.1 with
+// 64, 21.0 and 15.4 with 96; behind 30 000 42.7 and 35.5, 42.7 and 49.0 with 48.
+constexpr int kLargeRows = 12, kLargeRowsLong = 40, kLongKeys = 148 * 1024;
+constexpr int kLargeCodeRows = 40, kLargeCodeRowsShort = 96, kShortKeys = 1280;
 bool large(const Batch& b, const AttnSpec& a, const Prefix& p) {
     const int64_t rows = static_cast<int64_t>(b.tokens) * (a.heads / a.kv_heads);
-    return prefix_tc_takes(p, a) && rows >= (p.cache.storage == BST_DTYPE_U4 ? kLargeCodeRows : kLargeRows);
+    int least = kLargeRows;
+    if (p.cache.storage == BST_DTYPE_U4) {
+        least = p.length < kShortKeys ? kLargeCodeRowsShort : kLargeCodeRows;
+    } else if (a.head_dim == 64 && a.kv_heads >= 4 && static_cast<int64_t>(p.length) * a.kv_heads >= kLongKeys) {
+        least = kLargeRowsLong;
+    }
+    return prefix_tc_takes(p, a) && rows >= least;
 }
 
 // Splits of the own keys: no more than fill the card (spreading 64 rows of 20 to 1000 keys over four waves took
