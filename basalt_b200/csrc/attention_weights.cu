@@ -286,15 +286,19 @@ k_weights_join(Cache c, Batch b, AttnSpec a, int tile_rows, T* __restrict__ out,
     }
 }
 
-// Several tokens of each sequence on tcgen05, from kLargeRows query rows a sequence and key head and kLargeSlots on.
-// Whole calls of eight sequences, eight key heads of 128, tcgen05 and mma.sync (us): rows of 200 to 600 keys 52 and 50
-// with 64 query rows, 80 and 93 with 128; of 700 to 2000 keys 76 and 72 with 48, 81 and 80 with 64, 112 and 145 with
-// 128; of 1700 to 5000 keys 101 and 80 with 32, 121 and 144 with 64, 167 and 256 with 128. Four key heads of 64: of 200
-// to 600 keys 60 and 49 with 128, of 700 to 2000 47 and 44 with 64, 67 and 68 with 128, of 1700 to 5000 90 and 107.
-constexpr int kLargeRows = 64, kLargeSlots = 2048;
+// Several tokens of each sequence on tcgen05, from kLargeRows query rows a sequence and key head and kLargeSlots on (what
+// the lengths are is not known here). Whole calls of eight sequences, eight key heads, tcgen05 and mma.sync (us). Of 128
+// channels: rows of 700 to 2000 keys 72.6 and 66.5 with 48 query rows, 74.9 and 71.3 with 64, 85.7 and 113 with 96; of 1700 to
+// 5000 keys 99 and 76 with 32, 116 and 136 with 64; of 200 to 600 47.9 and 44.6 with 64, 58 and 72 with 96. Of 64 channels,
+// whose products leave the unpacking less behind: of 700 to 2000 keys 62.5 and 59.7 with 64, 71.9 and 74.6 with 96; of 1700 to
+// 5000 96.5 and 92.0 with 64, 114 and 133 with 96; of 5000 to 16 000 227 and 176 with 48, 208 and 221 with 64. (Four key heads
+// of 64: of 700 to 2000 keys 45.4 and 42.2 with 64, 54.0 and 53.8 with 96; of 5000 to 16 000 131 and 134 with 64.)
+constexpr int kLargeRows = 64, kLargeSlots = 2048, kLargeRowsOf64 = 96, kLargeSlotsOf64 = 8192;
 bool large(const Cache& c, const Batch& b, const AttnSpec& a) {
-    return own_tc_takes(c, b, a) && c.slots >= kLargeSlots &&
-           static_cast<int64_t>(b.tokens) * (a.heads / a.kv_heads) >= static_cast<int64_t>(b.count) * kLargeRows;
+    if (!own_tc_takes(c, b, a) || c.slots < kLargeSlots) return false;
+    const int64_t rows = static_cast<int64_t>(b.tokens) * (a.heads / a.kv_heads);
+    const int least = a.head_dim == 64 && c.slots < kLargeSlotsOf64 ? kLargeRowsOf64 : kLargeRows;
+    return rows >= static_cast<int64_t>(b.count) * least;
 }
 
 // Four waves of CTAs there, since lengths differ and are not known here.
