@@ -17,9 +17,10 @@
 // of them, rounded once (with bf16 ones the error was 1.6 times the outputs' own rounding instead of 1.0). Powers
 // of two keep all of it in fp16's range: one for each query row and each tile of keys, which the scores' factor f
 // takes back; and one for the values of each group of 32 channels, that of the largest so far with two bits to spare,
-// by which O is rescaled when a tile passes it. Where that leaves an entry too few bits (keys 2^-12 of the tile's
-// largest, values 2^-20 of the group's so far: no trained model's) the CTA's rows are added up again, plainly.
-// Each of the four warps unpacks whole tiles by itself, so that they wait for one another nowhere.
+// by which O is rescaled when a tile passes it. Entries far below those keep fewer bits: keys 2^-12 of the tile's largest
+// are off by up to 2^-30 of that, values 2^-20 of the group's so far by 2^-38 of that. Where that could move a score by 2^-12
+// or an output by 2^-11 of itself (sizes that no trained model has) the CTA's rows are added up again, plainly, which
+// takes 200 times as long: 21 ms for 96 tokens of 32 heads behind 16 384 keys. Each of the four warps unpacks whole tiles by itself, so that they wait for one another nowhere.
 //
 // The same kernel takes several tokens of each sequence over its own 4-bit row (OWN): then rows see the keys up to
 // their position, and every score may be kept.
@@ -206,7 +207,7 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
     // the next, when a warp that was held up comes to wait for that.)
     uint64_t* const o_last = o_done + 2;
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(o_last + 2);
-    int* const status = reinterpret_cast<int*>(tmem_slot + 1);  // [0] error code, [1] abort, [2] redo
+    int* const status = reinterpret_cast<int*>(tmem_slot + 1);  // [0] error code, [1] abort, [2] redo, [3] small values
     float* const row_factor = reinterpret_cast<float*>(smem + L::kFactors);   // what a row was divided by,
     float* const key_factor = row_factor + kRows;                             // a tile of keys, [8],
     float* const value_factor = key_factor + 8;                               // and of values and weights, [8][groups]
@@ -221,7 +222,7 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
             mbar_init(p_full + i, kSoft / 2);
         }
         for (int i = 0; i < 4; ++i) mbar_init(o_done + i, 1);
-        status[0] = status[1] = status[2] = 0;
+        status[0] = status[1] = status[2] = status[3] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     // Token and head of the CTA's query row `at`: the quotient of two small numbers, in float.
@@ -454,23 +455,21 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
                         }
                     }
                 }
+                bool small = false;  // whether an entry of the lane's keys has fewer bits
 #pragma unroll 1
                 for (int half = 0; half < 2; ++half) {
                     const int key = 32 * half + lane;
                     unsigned char* const to = smem + 2 * L::kQuery + (i % L::kSlots) * L::kTile + key * 128;
                     uint32_t scale[G], step[G / 2], low[G / 2];
                     scale_words(stage, 2 * kChunks + half, scale);
-                    // A key 2^-12 of the tile's largest, or values 2^-20 of the largest so far in their group, would
-                    // have too few bits: the rows are added up plainly.
                     float key_top = 0.0f;
-                    bool small = false;
 #pragma unroll
                     for (int g = 0; g < G; ++g) {
                         const float top = top_of(scale[g]);
                         key_top = fmaxf(key_top, top);
                         small |= !keys && top > 0.0f && top * by[g] < 0x1p-7f;
                     }
-                    if (small || (keys && key_top > 0.0f && key_top * by[0] < 0x1p-4f)) status[2] = 1;
+                    small |= keys && key_top > 0.0f && key_top * by[0] < 0x1p-4f;
                     if (OWN && !keys && (t0 + tile) * kTcKeys + key > sees_all) {
                         // Zero times a NaN is one: rows that do not see it must not get it, the others have to.
                         bool bad = false;
@@ -528,6 +527,14 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
                         unpack_all(std::true_type());
                     } else {
                         unpack_all(std::false_type());
+                    }
+                }
+                // The softmax's threads know what that means for their rows.
+                if (__any_sync(kFull, small) && lane == 0) {
+                    if (keys) {
+                        key_factor[tile & 7] = -key_factor[tile & 7];
+                    } else {
+                        status[3] = 1;
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -631,6 +638,13 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
             ok = ok && mbar_wait(s_full + 2 * half + (i & 1), (i >> 1) & 1, status, 7, abort);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             float by = CODES ? scale * key_factor[i & 7] : scale;
+            if constexpr (CODES) {
+                // Negative: some of the tile's keys have channels that are off by 2^-22, beside queries below 2^8.
+                if (by < 0.0f) {
+                    by = -by;
+                    if (by * (HD * 0x1p-14f) > 0x1p-12f) status[2] = 1;
+                }
+            }
             by = by < FLT_MIN ? FLT_MIN : by;
             const int left = sees - (t0 + i) * kTcKeys;  // keys of the tile, or more
             // Scores are read twice, 32 at a time: 64 held, the registers that thirteen warps leave were spilled.
@@ -745,12 +759,19 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
         asm volatile("bar.sync 1, %0;" ::"n"(kSoft) : "memory");
         unsigned char* const rows_at = smem;
         if (half < halves) {
+            float largest[G] = {};  // of the groups' outputs
 #pragma unroll
             for (int c = 0; c < HD / 32; ++c) {
                 uint32_t o[32];
                 tmem_ld32(o_at + 32 * c, o);
                 tmem_ld_wait();
                 if constexpr (CODES) {
+                    if (status[3] != 0) {
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) {
+                            largest[c / 2 * 2 + (x & 1)] = fmaxf(largest[c / 2 * 2 + (x & 1)], fabsf(__uint_as_float(o[x])));
+                        }
+                    }
 #pragma unroll
                     for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * values_by[c / 2 * 2 + (x & 1)]);
                 }
@@ -766,6 +787,13 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
                         z = x & 1 ? make_uint4(y[1], y[3], y[5], y[7]) : make_uint4(y[0], y[2], y[4], y[6]);
                     }
                     *reinterpret_cast<uint4*>(rows_at + at * (HD * 4) + ((chunk ^ (in_tile & 7)) << 4)) = z;
+                }
+            }
+            if (CODES && status[3] != 0) {
+                // Values as they were multiplied are off by up to 2^-25, and the sum of weights times that is the output's.
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    if (at < rows && largest[g] < total * 0x1p-14f) status[2] = 1;
                 }
             }
             if (at < rows) {

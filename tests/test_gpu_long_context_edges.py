@@ -345,3 +345,65 @@ def test_bf16_outputs_and_masses_of_weights_by_their_norm(ops, storage, dim, hea
     want = torch.einsum("stgaj,sjgd->stgad", p, v).flatten(0, 1).flatten(1, 2)
     check_norms(got, host(want), BITS[bits])
     check_norms(host(mass), host(p.sum((1, 3))), 2.0 ** -20 * (size + 1))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("own", [False, True])
+@pytest.mark.parametrize("small,large", [(-16, 0), (-30, 0), (-60, 0), (-6, 4), (-6, 9), (-12, 20)])
+def test_small_entries_beside_large_ones(ops, dim, own, small, large):
+    """4-bit keys and values of which some are 2^small of the usual size, and some keys 2^large with scores that leave
+    them no weight, in every tile of 64. A score may be off by 2^-12 (base 2) by what the large keys' fp16 leaves the
+    small ones, which moves a weight by 2^-12 ln 2; outputs otherwise as above."""
+    torch = torch_()
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    n, kv_heads, heads, tokens = 2600, 2, 16, 24
+    x = torch.randn((2, n, kv_heads, dim), generator=g, device="cuda")
+    x[:, 5::32] *= 2.0 ** small
+    x[1, 6::64] *= 2.0 ** small
+    if large:
+        x[0, 9::64] = -2.0 ** large * x[0, 9::64].abs()
+    cache, starts = ops.KvCache.allocate(1, kv_heads, n, dim), ints([0, n])
+    ops.kv_append(cache, x[0], x[1], ints([n]), starts=starts)
+    k, v = (t.double() for t in ops.kv_read(cache, ints([n]), starts=starts, tokens=n))
+    q = torch.randn((tokens, heads, dim), generator=g, device="cuda")
+    q = (q.abs() if large else q).bfloat16()
+    if own:
+        mass = torch.zeros((1, kv_heads, n), device="cuda")
+        got = host(ops.attention_weights(cache, q, ints([n]), mass, starts=ints([0, tokens]), decay=0.0))
+    else:
+        empty = ops.KvCache.allocate(tokens, kv_heads, 4, dim)
+        got = host(ops.attention_shared(empty, q, ints([0] * tokens), cache, n))
+    score = torch.einsum("sgad,jgd->sgaj", q.double().unflatten(1, (2, -1)), k) * dim ** -0.5
+    if own:
+        hidden = torch.arange(n, device="cuda") > torch.arange(n - tokens, n, device="cuda")[:, None]
+        score.masked_fill_(hidden[:, None, None], -np.inf)
+    p = torch.softmax(score, -1)
+    moved = 2.0 ** -12 * np.log(2)
+    check_norms(got, host(torch.einsum("sgaj,jgd->sgad", p, v).flatten(1, 2)), BITS[11] + moved)
+    if own:
+        check_norms(host(mass)[0], host(p.sum((0, 2))), moved)
+
+
+def test_a_small_entry_does_not_slow_a_call(ops):
+    """One token a tile with a key and a value 2^-30 of the others' leaves the time of a call as it is, within a factor of
+    three (rows that are added up plainly take a hundred times as long)."""
+    torch = torch_()
+    cache, own = ops.KvCache.allocate(1, 8, 8192, 128), ops.KvCache.allocate(96, 8, 4, 128)
+    x = torch.randn((2, 8192, 8, 128), device="cuda")
+    q, lengths = torch.randn((96, 32, 128), device="cuda").bfloat16(), ints([0] * 96)
+    mass = torch.zeros((1, 8, 8192), device="cuda")
+    times = []
+    for factor in (1.0, 2.0 ** -30):
+        x[:, ::64] *= factor
+        ops.kv_append(cache, x[0], x[1], ints([8192]), starts=ints([0, 8192]))
+        for call in (lambda: ops.attention_shared(own, q, lengths, cache, 8192),
+                     lambda: ops.attention_weights(cache, q, ints([8192]), mass, starts=ints([0, 96]), decay=0.0)):
+            call()
+            e = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+            e[0].record()
+            for _ in range(20):
+                call()
+            e[1].record()
+            torch.cuda.synchronize()
+            times.append(e[0].elapsed_time(e[1]))
+    assert times[2] <= 3 * times[0] and times[3] <= 3 * times[1], times
