@@ -680,7 +680,8 @@ k_prefix_tc(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ C
                 }
             }
             const float most = fmaxf(max3(m[0], m[1], m[2]), m[3]) * by;
-            // The maximum that weights are taken against moves only when a row's grows by more than 2^8.
+            // The maximum that weights are taken against moves only when a row's grows by more than 2^8 (a published
+            // step of attention kernels for this architecture).
             const bool move = most > top + 8.0f || (top == -INFINITY && most > top);
             auto rescale = [&](const float (&keep)[G]) {
                 ok = ok && mbar_wait(o_done + half, (i - 1) & 1, status, 8, abort);

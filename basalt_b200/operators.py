@@ -318,7 +318,8 @@ def attention_shared(cache: KvCache, q, lengths, prefix: KvCache, prefix_length:
     """Attention of q ([tokens, heads, head_dim]) over the first ``prefix_length`` keys of row ``prefix_row``
     of ``prefix``, which all sequences share, and the sequences' own rows of ``cache`` behind them (as
     ``attention_cached`` without a window). The prefix is read once for the whole batch; ``prefix`` may be
-    ``cache`` itself, or hold its keys in another storage. ``out`` may be ``q`` itself."""
+    ``cache`` itself, or hold its keys in another storage. ``out`` may be ``q`` itself. bf16 calls with a dozen or
+    more query rows a key head multiply weights in 8 bits with a bf16 prefix's values, as prompts do."""
     device = cache.device
     if stream is not None:
         stream = _given(device, stream)
@@ -367,7 +368,8 @@ def attention_weights(cache: KvCache, q, lengths, mass, previous=None, decay: fl
     """``attention_cached``, which also adds up the weight each key gets: for the slots j < length of the
     sequences' rows ``mass[row, h, j] = decay * previous[row, h, j] +`` the weights that the call's tokens
     and the query heads of key head h give key j. ``mass`` and ``previous`` (``mass`` itself by default) are
-    float32 [rows, kv_heads, slots]; with ``decay`` 0 what was there is not read. Returns the outputs."""
+    float32 [rows, kv_heads, slots]; with ``decay`` 0 what was there is not read. Returns the outputs. The
+    workspace holds a float for every token, query head and slot."""
     device = cache.device
     if stream is not None:
         stream = _given(device, stream)

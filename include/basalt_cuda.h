@@ -363,9 +363,14 @@ int32_t bst_attention_cached(int32_t device, void* stream, const bst_kv_cache* c
  * first prefix_length keys of row prefix_row of `prefix` and, of its sequence's own row of `cache`, what
  * it sees in bst_attention_cached without a window (spec->window and sinks must be 0; own slots and
  * lengths count from behind the prefix, and a sequence may have no own key). The prefix is read once for
- * the batch, not once a sequence. `prefix` may be `cache` itself, and may hold another storage; heads and
- * head_dim are the same. 0 <= prefix_length <= its slots. Types, the own rows' one token without a 4-bit
- * cache, out and workspace are as in bst_attention_cached; over a 4-bit prefix any q counts as there. */
+ * the batch, not once a sequence. `prefix` may be `cache` itself, and may hold another storage; heads
+ * and head_dim are the same. 0 <= prefix_length <= its slots. Types, the own rows' one token without a
+ * 4-bit cache, out and workspace are as in bst_attention_cached; over a 4-bit prefix any q counts as
+ * there. So are the bits of weights, with one exception: of 64 or 128 channels, a batch with a dozen or
+ * more query rows (tokens x heads) to a key head multiplies them in 8 bits with the values of a bf16
+ * prefix, as prompts do (outputs are then off by 2.3e-3 of their norm; the rounding of bf16 outputs
+ * alone is 1.7e-3), and from some forty rows on in 11 bits with those of a 4-bit one, rounded to 11 bits
+ * too. */
 int32_t bst_attention_shared_workspace(const bst_kv_cache* cache, const bst_sequences* sequences,
                                        const bst_attention_spec* spec, const bst_kv_cache* prefix,
                                        int32_t prefix_row, int32_t prefix_length, int64_t* bytes);
@@ -379,12 +384,15 @@ int32_t bst_attention_shared(int32_t device, void* stream, const bst_kv_cache* c
  * j < lengths[s],
  *   mass[row][h][j] = decay * previous[row][h][j] + the sum of the weights (softmax of the scores) that
  *                     key j has for the call's tokens of the sequence and the query heads of key head h.
- * A key that no query sees gets 0, and one with a NaN among its scores NaN. mass and previous are float32
- * [rows][kv_heads][slots], weights float32 whatever the types. Other slots and rows of mass stay as they
- * were. previous may be mass itself (a running sum with decay 1) and shares nothing with it otherwise
- * (drafted tokens that may be rejected); with decay 0 it is not read and may be NULL. Should two
- * sequences name the same row, its keys get the weights of both. The workspace holds a float for every
- * query head and slot. */
+ * A key that no query sees gets 0, and one with a NaN among its scores NaN. mass and previous are
+ * float32 [rows][kv_heads][slots], weights that are added up float32 whatever the types (for the
+ * outputs they have the bits that they have in bst_attention_cached; many tokens of bf16 over 4 bits
+ * hold them, and values, in 11). Other slots and rows of mass stay as they were. previous may be mass
+ * itself (a running sum with decay 1) and shares nothing with it otherwise (drafted tokens that may be
+ * rejected); with decay 0 it is not read and may be NULL. Should two sequences name the same row, its
+ * keys get the weights of both. The workspace holds a float for every token, query head and slot: a
+ * prompt votes with its last tokens, not with all of them. Weights are those of the softmax over the
+ * row's own keys; behind a shared prefix, too. */
 int32_t bst_attention_weights_workspace(const bst_kv_cache* cache, const bst_sequences* sequences,
                                         const bst_attention_spec* spec, int64_t* bytes);
 int32_t bst_attention_weights(int32_t device, void* stream, const bst_kv_cache* cache,
